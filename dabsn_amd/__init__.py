@@ -10,6 +10,8 @@ token by token against a bank that grows in place.
 
 from . import kernels
 from .core import DABSNCore
+from .distill import chunked_linear_distillation, distillation_from_logits
+from .embedding import scaled_embedding
 from .events import (
     EventCode,
     StrictFallbackError,
@@ -21,6 +23,7 @@ from .loss import chunked_cross_entropy_from_logits, chunked_linear_cross_entrop
 from .memory import DABSNMemory, LayerMemory, forward_with_memory, ingest
 from .model import DABSNBlock, DABSNSequenceLM
 from .read import DABSNRead
+from .scoring import TokenLogprobs, chunked_linear_token_logprobs, token_logprobs
 
 __all__ = [
     "DABSNBlock",
@@ -31,12 +34,18 @@ __all__ = [
     "EventCode",
     "StrictFallbackError",
     "LayerMemory",
+    "TokenLogprobs",
     "chunked_cross_entropy_from_logits",
     "chunked_linear_cross_entropy",
+    "chunked_linear_distillation",
+    "chunked_linear_token_logprobs",
     "add_event_listener",
+    "distillation_from_logits",
     "forward_with_memory",
     "ingest",
     "kernels",
     "remove_event_listener",
+    "scaled_embedding",
     "strict_events",
+    "token_logprobs",
 ]

@@ -13,7 +13,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_build" / "libdabsn_hip.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 _lock = threading.Lock()
 _lib = None
@@ -167,6 +167,26 @@ _SIGNATURES = {
         [i64, i64, vp, i64, vp, i64, vp, vp, vp, i64, i64, vp, vp, vp], i32),
     "dabsn_hip_ce_bias": ([i64, i64, vp, i32, vp, vp], i32),
     "dabsn_hip_ce_join": ([i64, vp, vp, vp], i32),
+    "dabsn_hip_token_logprobs": (
+        [i32, i64, i64, vp, i64, vp, vp, i64, ctypes.c_float, i64] + [vp] * 7, i32),
+    "dabsn_hip_token_logprobs_bwd": (
+        [i32, i64, i64, vp, i64, vp, vp, i64, ctypes.c_float, i64] + [vp] * 7 + [i64, i64, vp],
+        i32),
+    "dabsn_hip_distill_rows": ([i64, i64, i64, i32, vp, vp, i64, vp, vp], i32),
+    "dabsn_hip_distill_mean": ([i64, vp, ctypes.c_float, vp, vp, vp], i32),
+    "dabsn_hip_distill": (
+        [i32, i64, i64, vp, i64, vp, i64, i32, vp, vp, i64, ctypes.c_float, vp, vp, vp, vp, vp, vp,
+         i64, i64, vp, vp], i32),
+    "dabsn_hip_distill_bwd": (
+        [i32, i64, i64, vp, i64, i64, vp, ctypes.c_float, vp, vp, vp, vp, vp, vp], i32),
+    "dabsn_hip_column_sums_partials": ([i64, i64], sz),
+    "dabsn_hip_column_sums": ([i64, i64, i64, vp, i32, vp, vp, vp], i32),
+    "dabsn_hip_scaled": ([i32, i64, vp, vp, vp, vp], i32),
+    "dabsn_hip_embedding_fwd": (
+        [i32, i64, i64, i64, vp, vp, i64, ctypes.c_float, vp, vp, vp], i32),
+    "dabsn_hip_embedding_workspace_bytes": ([i64, i64, i64], sz),
+    "dabsn_hip_embedding_bwd": (
+        [i32, i64, i64, i64, vp, i64, vp, ctypes.c_float, vp, vp, sz, vp], i32),
     "dabsn_hip_read3_decode": (
         [i32, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, PTR4,
          vp, vp, sz, vp],

@@ -1,0 +1,502 @@
+// Scaled token embedding and the gradient of its table.
+//
+// Forward: out[i] = scale * weight[id_i], a copy of rows bound by memory.
+// Backward: dweight[v] = scale * (the sum of the rows grad[i] with id_i = v, in token order),
+// fp32 sums, one rounding; a row of zeros where no token is v. The order is fixed, so the same
+// inputs give the same bits: no float atomics. The tokens are sorted by word (stable, so each
+// word's tokens stay in order), the sorted list is cut into pieces of equal length whatever the
+// words' frequencies, a wave sums a piece's rows word by word, and words that cross pieces are
+// joined from partial sums, piece after piece.
+#include <algorithm>
+
+#include "../../include/dabsn_hip.h"
+#include "capi.hpp"
+#include "common.hpp"
+
+namespace dabsn {
+namespace embed {
+
+constexpr uint32_t kErrToken = 1u;
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+// Eight neighbouring values at any element alignment as floats.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4_any*>(p);
+  const u32x4 b = *reinterpret_cast<const u32x4_any*>(p + 4);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t x = a[k], y = b[k];  // a cast of the element itself reads element 0
+    v[k] = __builtin_bit_cast(float, x);
+    v[4 + k] = __builtin_bit_cast(float, y);
+  }
+}
+__device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4_any*>(p);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[2 * k] = __builtin_bit_cast(float, a[k] << 16);
+    v[2 * k + 1] = __builtin_bit_cast(float, a[k] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  u32x4 a, b;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    a[k] = __builtin_bit_cast(uint32_t, v[k]);
+    b[k] = __builtin_bit_cast(uint32_t, v[4 + k]);
+  }
+  *reinterpret_cast<u32x4_any*>(p) = a;
+  *reinterpret_cast<u32x4_any*>(p + 4) = b;
+}
+__device__ __forceinline__ void store8(bf16* p, const float (&v)[8]) {
+  u32x4 a;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    a[k] = static_cast<uint32_t>(f2bf(v[2 * k])) | static_cast<uint32_t>(f2bf(v[2 * k + 1])) << 16;
+  *reinterpret_cast<u32x4_any*>(p) = a;
+}
+// The same for the columns c .. c + 7 of a row of H: fewer at its end (zeros are read there).
+template <typename E>
+__device__ __forceinline__ void get8(const E* row, int c, int H, float (&v)[8]) {
+  if (c + 8 <= H) {
+    load8(row + c, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < H ? to_f(row[c + k]) : 0.0f;
+  }
+}
+template <typename E>
+__device__ __forceinline__ void put8(E* row, int c, int H, const float (&v)[8]) {
+  if (c + 8 <= H) {
+    store8(row + c, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < H) row[c + k] = from_f<E>(v[k]);
+  }
+}
+
+// A wave takes 64 / lanes rows at a time, `lanes` (a power of two) lanes a row.
+template <typename E>
+__global__ void __launch_bounds__(256) lookup_kernel(int64_t n, int64_t V, int H, int lanes_log2,
+                                                     const int64_t* __restrict__ ids,
+                                                     const E* __restrict__ weight, int64_t ldw,
+                                                     float scale, E* __restrict__ out,
+                                                     uint32_t* err) {
+  const int lanes = 1 << lanes_log2;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1);
+  if (i >= n) return;
+  const int64_t id = ids[i];
+  const bool ok = id >= 0 && id < V;
+  if (!ok && lane == 0) atomicOr(err, kErrToken);
+  const E* w = weight + (ok ? id : 0) * ldw;
+  const float s = ok ? scale : NAN;
+  E* o = out + i * H;
+#pragma unroll 4
+  for (int c = lane * 8; c < H; c += lanes * 8) {
+    float v[8];
+    get8(w, c, H, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= s;
+    put8(o, c, H, v);
+  }
+}
+
+// ---- stable sort of the tokens by word -----------------------------------------------------
+// Tokens that give no gradient (out of range, the padding word) get the key V and come last.
+__device__ __forceinline__ uint32_t key_of(int64_t id, int64_t V, int64_t padding) {
+  return id < 0 || id >= V || id == padding ? static_cast<uint32_t>(V) : static_cast<uint32_t>(id);
+}
+
+// Few tokens: a token's place is the number of tokens before it in the order (key, index),
+// counted against all of them in shared memory; four threads share a token's count.
+constexpr int kRankTokens = 4096;
+__global__ void __launch_bounds__(256) rank_kernel(int n, int64_t V, int64_t padding,
+                                                   const int64_t* __restrict__ ids,
+                                                   uint32_t* __restrict__ keys,
+                                                   uint32_t* __restrict__ pos) {
+  __shared__ uint32_t all[kRankTokens];
+  for (int j = threadIdx.x; j < n; j += 256) all[j] = key_of(ids[j], V, padding);
+  __syncthreads();
+  const int i = blockIdx.x * 64 + (threadIdx.x >> 2), part = threadIdx.x & 3;
+  const uint32_t mine = i < n ? all[i] : 0;
+  int rank = 0;
+  for (int j = part; j < n; j += 4) rank += all[j] < mine + (j < i);  // equal and earlier, or less
+  rank += __shfl_xor(rank, 1, 64);
+  rank += __shfl_xor(rank, 2, 64);
+  if (part == 0 && i < n) {
+    keys[rank] = mine;
+    pos[rank] = static_cast<uint32_t>(i);
+  }
+}
+
+// Many tokens: passes over digits of `bits` bits, the lowest first. A block counts its tile's
+// digits; then each block finds where its tile's digits start (all smaller digits, and the same
+// digit in earlier tiles) and places its tokens, 64 at a time a wave, by their rank among equal
+// digits: bits ballots.
+constexpr int kMaxBits = 10;
+template <bool FIRST>
+__device__ __forceinline__ uint32_t sort_key(int64_t i, int64_t V, int64_t padding,
+                                             const int64_t* ids, const uint32_t* keys) {
+  if constexpr (FIRST) return key_of(ids[i], V, padding);
+  return keys[i];
+}
+template <bool FIRST>
+__global__ void __launch_bounds__(256) digits_kernel(int64_t n, int64_t V, int64_t padding, int tile,
+                                                     int shift, int bits,
+                                                     const int64_t* __restrict__ ids,
+                                                     const uint32_t* __restrict__ keys,
+                                                     uint32_t* __restrict__ counts) {
+  __shared__ uint32_t h[1 << kMaxBits];
+  const int bins = 1 << bits;
+  for (int b = threadIdx.x; b < bins; b += 256) h[b] = 0;
+  __syncthreads();
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * tile, i1 = min(n, i0 + tile);
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += 256)
+    atomicAdd(&h[sort_key<FIRST>(i, V, padding, ids, keys) >> shift & (bins - 1)], 1u);
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += 256)
+    counts[static_cast<size_t>(blockIdx.x) * bins + b] = h[b];
+}
+template <bool FIRST>
+__global__ void __launch_bounds__(256) place_kernel(int64_t n, int64_t V, int64_t padding, int tile,
+                                                    int shift, int bits, int tiles,
+                                                    const int64_t* __restrict__ ids,
+                                                    const uint32_t* __restrict__ keys,
+                                                    const uint32_t* __restrict__ pos,
+                                                    const uint32_t* __restrict__ counts,
+                                                    uint32_t* __restrict__ keys_out,
+                                                    uint32_t* __restrict__ pos_out) {
+  __shared__ uint32_t at[4][1 << kMaxBits];
+  __shared__ uint32_t total[1 << kMaxBits];
+  __shared__ uint32_t waves[4];
+  const int bins = 1 << bits, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  for (int b = tid; b < bins; b += 256) {
+    uint32_t before = 0, all = 0;
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) {
+      const uint32_t x = counts[static_cast<size_t>(t) * bins + b];
+      before += t < static_cast<int>(blockIdx.x) ? x : 0;
+      all += x;
+    }
+    at[0][b] = before;
+    at[1][b] = at[2][b] = at[3][b] = 0;
+    total[b] = all;
+  }
+  __syncthreads();
+  // Exclusive sums of the digits' totals: a thread's run of bins, then over lanes and waves.
+  const int run = (bins + 255) / 256, b0 = tid * run;
+  uint32_t mine = 0;
+  for (int b = b0; b < min(b0 + run, bins); ++b) mine += total[b];
+  uint32_t up = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t x = __shfl_up(up, o, 64);
+    up += lane >= o ? x : 0;
+  }
+  if (lane == 63) waves[wave] = up;
+  __syncthreads();
+  uint32_t start = up - mine;
+  for (int w = 0; w < wave; ++w) start += waves[w];
+  for (int b = b0; b < min(b0 + run, bins); ++b) {
+    at[0][b] += start;
+    start += total[b];
+  }
+  // The waves' quarters of the tile: counts of the quarters before a wave's own.
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * tile, i1 = min(n, i0 + tile);
+  const int quarter = tile / 4;
+  const int64_t q0 = i0 + static_cast<int64_t>(wave) * quarter, q1 = min(i1, q0 + quarter);
+  if (wave < 3) {
+    for (int64_t i = q0 + lane; i < q1; i += 64)
+      atomicAdd(&at[wave + 1][sort_key<FIRST>(i, V, padding, ids, keys) >> shift & (bins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int b = tid; b < bins; b += 256) {
+    uint32_t s = at[0][b];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      s += at[w][b];
+      at[w][b] = s;
+    }
+  }
+  __syncthreads();
+  for (int64_t i = q0; i < q1; i += 64) {
+    const bool live = i + lane < q1;
+    const uint32_t key = live ? sort_key<FIRST>(i + lane, V, padding, ids, keys) : 0;
+    const uint32_t d = key >> shift & (bins - 1);
+    uint64_t same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+      const bool one = d >> b & 1;
+      const uint64_t with = __ballot(one);
+      same &= one ? with : ~with;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    const uint32_t from = live ? at[wave][d] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // all lanes have read
+    if (live && rank == 0) at[wave][d] = from + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    if (live) {
+      keys_out[from + rank] = key;
+      pos_out[from + rank] = FIRST ? static_cast<uint32_t>(i + lane) : pos[i + lane];
+    }
+  }
+}
+
+// starts[v] = the first sorted token of a word >= v, v = 0 .. V.
+__global__ void __launch_bounds__(256) starts_kernel(uint32_t n, uint32_t V,
+                                                     const uint32_t* __restrict__ keys,
+                                                     uint32_t* __restrict__ starts) {
+  const uint32_t v = blockIdx.x * 256 + threadIdx.x;
+  if (v > V) return;
+  uint32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (keys[mid] < v) lo = mid + 1; else hi = mid;
+  }
+  starts[v] = lo;
+}
+
+// ---- sums ----------------------------------------------------------------------------------
+// A wave sums the rows of the sorted tokens [piece * P, + P) over 64 * 8 columns. A word that
+// begins and ends in the piece is written; one that began in an earlier piece leaves its partial
+// sum in slot 2 piece, one that only begins here in slot 2 piece + 1.
+template <typename E>
+__global__ void __launch_bounds__(256) pieces_kernel(int H, int P, int strips, int64_t tasks,
+                                                     uint32_t V, const uint32_t* __restrict__ starts,
+                                                     const uint32_t* __restrict__ keys,
+                                                     const uint32_t* __restrict__ pos,
+                                                     const E* __restrict__ grad, float scale,
+                                                     E* __restrict__ dweight,
+                                                     float* __restrict__ partial) {
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (task >= tasks) return;
+  const int lane = threadIdx.x & 63;
+  const uint32_t piece = static_cast<uint32_t>(task / strips);
+  const int c = (static_cast<int>(task - static_cast<int64_t>(piece) * strips) * 64 + lane) * 8;
+  const uint32_t n = starts[V];  // tokens that give a gradient
+  const uint32_t lo = piece * P, hi = min(n, lo + P);
+  if (lo >= n) return;
+  const int count = static_cast<int>(hi - lo);
+  const uint32_t key = keys[min(lo + lane, n - 1)], row = pos[min(lo + lane, n - 1)];
+  const uint32_t before = lo > 0 ? keys[lo - 1] : 0xffffffffu;
+  const uint32_t after = hi < n ? keys[hi] : 0xffffffffu;
+  const bool live = c < H;
+  float sum[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
+  bool began = __builtin_amdgcn_readlane(key, 0) != before;
+  constexpr int U = 8;
+  for (int i0 = 0; i0 < count; i0 += U) {
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t r = __builtin_amdgcn_readlane(row, min(i0 + u, count - 1));
+      if (live) get8(grad + static_cast<size_t>(r) * H, c, H, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      if (i >= count) break;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += v[u][k];
+      const uint32_t now = __builtin_amdgcn_readlane(key, i);
+      const bool last = i + 1 == count;
+      const uint32_t next = last ? after : __builtin_amdgcn_readlane(key, min(i + 1, 63));
+      if (last || next != now) {
+        if (live) {
+          if (began && next != now) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k] *= scale;
+            put8(dweight + static_cast<size_t>(now) * H, c, H, sum);
+          } else {
+            put8(partial + (2 * static_cast<size_t>(piece) + (began ? 1 : 0)) * H, c, H, sum);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
+        began = true;
+      }
+    }
+  }
+}
+
+// A block per word: zeros where it has no token, the joined partial sums where it crosses
+// pieces; the others are written.
+template <typename E>
+__global__ void __launch_bounds__(256) words_kernel(int H, int P, const uint32_t* __restrict__ starts,
+                                                    const float* __restrict__ partial, float scale,
+                                                    E* __restrict__ dweight) {
+  const size_t v = blockIdx.x;
+  const uint32_t a = starts[v], b = starts[v + 1];
+  E* o = dweight + v * H;
+  const uint32_t p0 = a / P, p1 = b > a ? (b - 1) / P : p0;
+  if (b > a && p0 == p1) return;
+  for (int c = threadIdx.x * 8; c < H; c += 256 * 8) {
+    float sum[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
+    if (b > a) {
+      get8(partial + (2 * static_cast<size_t>(p0) + 1) * H, c, H, sum);
+#pragma unroll 4
+      for (uint32_t p = p0 + 1; p <= p1; ++p) {
+        float w[8];
+        get8(partial + 2 * static_cast<size_t>(p) * H, c, H, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += w[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] *= scale;
+    }
+    put8(o, c, H, sum);
+  }
+}
+
+constexpr int kPiece = 32;
+
+struct Plan {
+  int bits, passes, tile, tiles;
+  int64_t pieces;
+  size_t keys, pos, keys2, pos2, counts, starts, partial, bytes;
+};
+static size_t up(size_t b) { return (b + 255) / 256 * 256; }
+static Plan plan_of(int64_t n, int64_t V, int64_t H) {
+  Plan p{};
+  int need = 1;
+  while ((1ll << need) <= V) ++need;  // keys 0 .. V
+  const bool rank = n <= kRankTokens;
+  p.passes = rank ? 0 : (need + kMaxBits - 1) / kMaxBits;
+  p.bits = rank ? 0 : (need + p.passes - 1) / p.passes;
+  // At most 128 tiles, whose counts every block adds up; a multiple of 256, the waves' rounds.
+  p.tile = static_cast<int>(std::max<int64_t>(1024, (n + 127) / 128));
+  p.tile = (p.tile + 255) / 256 * 256;
+  p.tiles = static_cast<int>((n + p.tile - 1) / p.tile);
+  p.pieces = (n + kPiece - 1) / kPiece;
+  size_t at = 0;
+  auto take = [&](size_t b) { const size_t o = at; at += up(b); return o; };
+  p.keys = take(4 * n);
+  p.pos = take(4 * n);
+  p.keys2 = p.passes > 1 ? take(4 * n) : p.keys;
+  p.pos2 = p.passes > 1 ? take(4 * n) : p.pos;
+  p.counts = take(p.passes ? 4ull * p.tiles << p.bits : 0);
+  p.starts = take(4 * (V + 1));
+  p.partial = take(8ull * p.pieces * H);
+  p.bytes = at;
+  return p;
+}
+
+static int checks(const char* what, int dtype, int64_t n, int64_t V, int64_t H) {
+  DABSN_REQUIRE(dtype == kF32 || dtype == kBF16, "%s: bad dtype %d", what, dtype);
+  DABSN_REQUIRE(n >= 0 && n < (1ll << 31) && V > 0 && V < (1ll << 31) - 256 && H > 0 && H < (1 << 24),
+                "%s: bad shape (tokens=%lld, V=%lld, H=%lld)", what, (long long)n, (long long)V,
+                (long long)H);
+  return DABSN_OK;
+}
+
+template <typename E>
+static void launch_bwd(const Plan& p, int64_t n, int64_t V, int H, const int64_t* ids, int64_t padding,
+                       const E* grad, float scale, E* dweight, char* ws, hipStream_t stream) {
+  auto* keys = reinterpret_cast<uint32_t*>(ws + p.keys);
+  auto* pos = reinterpret_cast<uint32_t*>(ws + p.pos);
+  auto* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
+  auto* starts = reinterpret_cast<uint32_t*>(ws + p.starts);
+  auto* partial = reinterpret_cast<float*>(ws + p.partial);
+  if (p.passes == 0 && n > 0) {
+    hipLaunchKernelGGL(rank_kernel, dim3(static_cast<unsigned>((n + 63) / 64)), dim3(256), 0, stream,
+                       static_cast<int>(n), V, padding, ids, keys, pos);
+  }
+  // Passes alternate between two buffers and end in the first.
+  uint32_t *ka = keys, *pa = pos;
+  uint32_t *kb = reinterpret_cast<uint32_t*>(ws + p.keys2), *pb = reinterpret_cast<uint32_t*>(ws + p.pos2);
+  if (p.passes % 2 == 0) {
+    std::swap(ka, kb);
+    std::swap(pa, pb);
+  }
+  for (int s = 0; s < p.passes; ++s) {
+    const dim3 grid(static_cast<unsigned>(p.tiles));
+    const int shift = s * p.bits;
+    if (s == 0) {
+      hipLaunchKernelGGL((digits_kernel<true>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
+                         shift, p.bits, ids, nullptr, counts);
+      hipLaunchKernelGGL((place_kernel<true>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
+                         shift, p.bits, p.tiles, ids, nullptr, nullptr, counts, ka, pa);
+    } else {
+      hipLaunchKernelGGL((digits_kernel<false>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
+                         shift, p.bits, ids, kb, counts);
+      hipLaunchKernelGGL((place_kernel<false>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
+                         shift, p.bits, p.tiles, ids, kb, pb, counts, ka, pa);
+    }
+    std::swap(ka, kb);
+    std::swap(pa, pb);
+  }
+  hipLaunchKernelGGL(starts_kernel, dim3(static_cast<unsigned>(V / 256 + 1)), dim3(256), 0, stream,
+                     static_cast<uint32_t>(n), static_cast<uint32_t>(V), keys, starts);
+  const int strips = (H + 511) / 512;
+  const int64_t tasks = p.pieces * strips;
+  if (tasks > 0)
+    hipLaunchKernelGGL((pieces_kernel<E>), dim3(static_cast<unsigned>((tasks + 3) / 4)), dim3(256), 0,
+                       stream, H, kPiece, strips, tasks, static_cast<uint32_t>(V), starts, keys, pos,
+                       grad, scale, dweight, partial);
+  hipLaunchKernelGGL((words_kernel<E>), dim3(static_cast<unsigned>(V)), dim3(256), 0, stream, H,
+                     kPiece, starts, partial, scale, dweight);
+}
+
+}  // namespace embed
+}  // namespace dabsn
+
+using namespace dabsn;
+using namespace dabsn::embed;
+
+extern "C" {
+
+int dabsn_hip_embedding_fwd(int dtype, int64_t n, int64_t V, int64_t H, const int64_t* ids,
+                            const void* weight, int64_t ldw, float scale, void* out, uint32_t* err,
+                            hipStream_t stream) {
+  int rc = checks("embedding", dtype, n, V, H);
+  if (rc != DABSN_OK) return rc;
+  DABSN_REQUIRE(ldw >= H, "embedding: row stride %lld of %lld values", (long long)ldw, (long long)H);
+  if (n == 0) return DABSN_OK;
+  DABSN_REQUIRE(ids && weight && out && err, "embedding: null pointer");
+  int log2 = 0;
+  while (log2 < 6 && (8ll << log2) < H) ++log2;
+  const int64_t blocks = ((n << log2) + 255) / 256;
+  DABSN_REQUIRE(blocks < (1ll << 31), "embedding: %lld tokens in one call", (long long)n);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (dtype == kBF16)
+    hipLaunchKernelGGL((lookup_kernel<bf16>), grid, dim3(256), 0, stream, n, V, (int)H, log2, ids,
+                       static_cast<const bf16*>(weight), ldw, scale, static_cast<bf16*>(out), err);
+  else
+    hipLaunchKernelGGL((lookup_kernel<float>), grid, dim3(256), 0, stream, n, V, (int)H, log2, ids,
+                       static_cast<const float*>(weight), ldw, scale, static_cast<float*>(out), err);
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+size_t dabsn_hip_embedding_workspace_bytes(int64_t n, int64_t V, int64_t H) {
+  if (n < 0 || n >= (1ll << 31) || V <= 0 || V >= (1ll << 31) - 256 || H <= 0 || H >= (1 << 24)) return 0;
+  return plan_of(n, V, H).bytes;
+}
+
+int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const int64_t* ids,
+                            int64_t padding_idx, const void* grad, float scale, void* dweight,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  int rc = checks("embedding backward", dtype, n, V, H);
+  if (rc != DABSN_OK) return rc;
+  const Plan p = plan_of(n, V, H);
+  DABSN_REQUIRE(((ids && grad) || n == 0) && dweight && workspace,
+                "embedding backward: null pointer");
+  DABSN_REQUIRE(workspace_bytes >= p.bytes, "embedding backward: workspace of %zu bytes, %zu needed",
+                workspace_bytes, p.bytes);
+  DABSN_REQUIRE(p.pieces * ((H + 511) / 512) < (1ll << 32),
+                "embedding backward: %lld x %lld values in one call", (long long)n, (long long)H);
+  if (dtype == kBF16)
+    launch_bwd<bf16>(p, n, V, (int)H, ids, padding_idx, static_cast<const bf16*>(grad), scale,
+                     static_cast<bf16*>(dweight), static_cast<char*>(workspace), stream);
+  else
+    launch_bwd<float>(p, n, V, (int)H, ids, padding_idx, static_cast<const float*>(grad), scale,
+                      static_cast<float*>(dweight), static_cast<char*>(workspace), stream);
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+}  // extern "C"

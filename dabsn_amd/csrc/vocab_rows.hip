@@ -1,0 +1,1123 @@
+// Row kernels over a vocabulary: token log probabilities and distillation.
+//
+// Both take rows of logits [rows, V] (or the fp32 logits of a readout before its bias) and a
+// temperature T, z = x / T, and form the row's softmax from its maximum m and the sum
+// s = sum exp(z - m/T) in one pass, fp32, with a running maximum per thread:
+//   log probabilities   logp_t = z_t - m/T - ln s;  H = ln s - sum e (z - m/T) / s;  the K
+//                       largest logits in order (equal ones by index)
+//   distillation        sum q (ln q - logp) over a teacher's listed tokens and, with the
+//                       teacher's normaliser, over the rest of the vocabulary as one event
+// and a backward that reads the logits once more and writes their gradient.
+//
+// Differences x - m are formed before they are scaled, so that masks of the type's lowest value
+// and -inf give exp 0 and never inf - inf. The pass is bound by memory: an element costs about
+// 10 vector instructions (4 of them the exponential's), half the time of its 2 bytes.
+#include <algorithm>
+
+#include "../../include/dabsn_hip.h"
+#include "capi.hpp"
+#include "common.hpp"
+
+namespace dabsn {
+namespace vocab {
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLowest = -3.40282346638528860e38f;
+constexpr int kMaxTop = 128;
+// Candidates of the top selection that fit: all of a vocabulary whose vectors of 8 are fewer
+// than kMaxTop (there the threshold may be below every logit), and some room for equal logits.
+constexpr int kCap = 1152;
+constexpr uint32_t kErrToken = 1u;
+
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+// A row's logits, 8 at a time from any element alignment (global memory takes 16-byte accesses
+// at 2-byte addresses; rows of an odd vocabulary start at such), plus the readout's bias.
+template <typename E, bool BIAS>
+struct Row {
+  const E* x;
+  const bf16* b;
+  struct Raw {
+    u32x4 v[is_bf16<E>::value ? 1 : 2];
+    u32x4 bias;
+  };
+  __device__ __forceinline__ Raw load(int c) const {
+    Raw r;
+    const E* p = x + static_cast<size_t>(c) * 8;
+    r.v[0] = *reinterpret_cast<const u32x4_any*>(p);
+    if constexpr (!is_bf16<E>::value) r.v[1] = *reinterpret_cast<const u32x4_any*>(p + 4);
+    if constexpr (BIAS) r.bias = *reinterpret_cast<const u32x4_any*>(b + static_cast<size_t>(c) * 8);
+    return r;
+  }
+  static __device__ __forceinline__ void halves(const u32x4& u, float (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[2 * k] = __builtin_bit_cast(float, u[k] << 16);
+      v[2 * k + 1] = __builtin_bit_cast(float, u[k] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[8]) {
+    if constexpr (is_bf16<E>::value) {
+      halves(r.v[0], v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t u = r.v[k >> 2][k & 3];  // a cast of the element itself reads element 0
+        v[k] = __builtin_bit_cast(float, u);
+      }
+    }
+    if constexpr (BIAS) {
+      float w[8];
+      halves(r.bias, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += w[k];
+    }
+  }
+  __device__ __forceinline__ float at(int64_t j) const {
+    float v = ld(x, static_cast<size_t>(j));
+    if constexpr (BIAS) v += bf2f(b[j]);
+    return v;
+  }
+};
+
+// f(c, values) for this thread's vectors c = tid, tid + NTH, ... of the row's V / 8, four loads
+// in flight, then g(column, value) for its one element of the last V % 8.
+template <int NTH, typename R, typename F, typename G>
+__device__ __forceinline__ void for_row(const R& row, int V, F f, G g) {
+  constexpr int U = 4;
+  const int nv = V >> 3;
+  for (int c0 = threadIdx.x; c0 < nv; c0 += U * NTH) {
+    typename R::Raw raw[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) raw[k] = row.load(min(c0 + k * NTH, nv - 1));
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (c0 + k * NTH < nv) {
+        float v[8];
+        R::unpack(raw[k], v);
+        f(c0 + k * NTH, v);
+      }
+    }
+  }
+  const int j = nv * 8 + threadIdx.x;
+  if (j < V) g(j, row.at(j));
+}
+
+__device__ __forceinline__ float max8(const float (&v)[8]) {
+  return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])),
+               fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+}
+
+// The sum over the block of N values a thread, to every thread. sh: N * NTH/64 floats.
+template <int NTH, int N>
+__device__ __forceinline__ void block_sums(float (&v)[N], float* sh) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  if constexpr (NTH > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sh[i * (NTH / 64) + (threadIdx.x >> 6)] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NTH / 64; ++w) v[i] += sh[i * (NTH / 64) + w];
+    }
+  }
+}
+template <int NTH>
+__device__ __forceinline__ float block_max(float v, float* sh) {
+  v = wave_max(v);
+  if constexpr (NTH > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NTH / 64; ++w) v = fmaxf(v, sh[w]);
+  }
+  return v;
+}
+
+// A thread's share of a row: the maximum m (kLowest where it has no finite logit), s = sum
+// exp2((x - m) c), u = sum of these times (x - m) (the entropy's sum), r = the share of s at
+// tokens that are not listed. NaN and +inf make s NaN.
+struct Share {
+  float m = kLowest, s = 0.0f, u = 0.0f, r = 0.0f;
+};
+
+template <bool ENT, bool REST>
+__device__ __forceinline__ void raise(Share& a, float to, float c) {
+  const float d = a.m - to;
+  const float f = __builtin_amdgcn_exp2f(d * c);
+  if constexpr (ENT) a.u = f == 0.0f ? 0.0f : f * (a.u + d * a.s);
+  a.s *= f;
+  if constexpr (REST) a.r *= f;
+  a.m = to;
+}
+
+template <bool ENT, bool REST>
+__device__ __forceinline__ void fold8(Share& a, const float (&v)[8], float vm, float c,
+                                      uint32_t listed) {
+  if (vm > a.m) raise<ENT, REST>(a, vm, c);
+  float vs = 0.0f, vr = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float d = v[k] - a.m;
+    const float e = __builtin_amdgcn_exp2f(d * c);
+    vs += e;
+    if constexpr (ENT) a.u += e * fmaxf(d, -1e30f);  // d = -inf has e = 0
+    if constexpr (REST) {
+      if (listed) vr += (listed >> k & 1) ? 0.0f : e;  // few vectors hold a listed token
+    }
+  }
+  a.s += vs;
+  if constexpr (REST) a.r += listed ? vr : vs;
+}
+
+template <bool ENT, bool REST>
+__device__ __forceinline__ void fold1(Share& a, float x, float c, bool listed) {
+  if (x > a.m) raise<ENT, REST>(a, x, c);
+  const float d = x - a.m, e = __builtin_amdgcn_exp2f(d * c);
+  a.s += e;
+  if constexpr (ENT) a.u += e * fmaxf(d, -1e30f);
+  if constexpr (REST) a.r += listed ? 0.0f : e;
+}
+
+// The block's shares as one, to every thread.
+template <int NTH, bool ENT, bool REST>
+__device__ __forceinline__ void join(Share& a, float c, float* sh) {
+  const float M = block_max<NTH>(a.m, sh);
+  raise<ENT, REST>(a, M, c);
+  float v[1 + ENT + REST];
+  v[0] = a.s;
+  if constexpr (ENT) v[1] = a.u;
+  if constexpr (REST) v[ENT + 1] = a.r;
+  block_sums<NTH, 1 + ENT + REST>(v, sh);
+  a.s = v[0];
+  if constexpr (ENT) a.u = v[1];
+  if constexpr (REST) a.r = v[ENT + 1];
+}
+
+// ---- the K largest logits of a row ---------------------------------------------------------
+// Order-preserving integers of floats; -0 counts as 0, and NaN with -inf, below every number.
+constexpr uint32_t kNone = 0x007fffffu;  // key of -inf
+__device__ __forceinline__ uint32_t key_of(float x) {
+  if (!(x > -INFINITY)) return kNone;
+  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// A thread's best two vectors (8 neighbouring logits, by their largest).
+struct Best {
+  float v1 = -INFINITY, v2 = -INFINITY;
+  int c1 = -1;
+  __device__ __forceinline__ void see(float vm, int c) {
+    const bool up = vm > v1;
+    v2 = up ? v1 : fmaxf(v2, vm);
+    c1 = up ? c : c1;
+    v1 = up ? vm : v1;
+  }
+};
+
+template <int NTH>
+struct TopShared {
+  uint64_t cand[kCap];  // key << 32 | ~column: the larger, the earlier
+  float best[NTH];
+  uint32_t tau;
+  int count;
+  int wave[NTH / 64];
+};
+
+__device__ __forceinline__ void push(uint64_t* cand, int* count, uint32_t key, int j) {
+  const int at = atomicAdd(count, 1);
+  if (at < kCap) cand[at] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~j);
+}
+
+// How many of the row's keys are at least `lo`.
+template <int NTH, typename R>
+__device__ int count_from(const R& row, int V, uint32_t lo, TopShared<NTH>& t) {
+  int n = 0;
+  for_row<NTH>(
+      row, V,
+      [&](int, const float (&v)[8]) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) n += key_of(v[k]) >= lo;
+      },
+      [&](int, float x) { n += key_of(x) >= lo; });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) t.wave[threadIdx.x >> 6] = n;
+  __syncthreads();
+  n = 0;
+  for (int w = 0; w < NTH / 64; ++w) n += t.wave[w];
+  return n;
+}
+
+// Appends the first `want` columns (in order) whose key is `key`.
+template <int NTH, typename R>
+__device__ void append_equal(const R& row, int V, uint32_t key, int want, TopShared<NTH>& t) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int j0 = 0; j0 < V && want > 0; j0 += NTH) {
+    const int j = j0 + threadIdx.x;
+    const bool hit = j < V && key_of(row.at(j)) == key;
+    const uint64_t mask = __ballot(hit);
+    __syncthreads();  // the counts of the tile before have been read
+    if (lane == 0) t.wave[wave] = __popcll(mask);
+    __syncthreads();
+    int before = __popcll(mask & ((1ull << lane) - 1)), all = 0;
+    for (int w = 0; w < NTH / 64; ++w) {
+      before += w < wave ? t.wave[w] : 0;
+      all += t.wave[w];
+    }
+    if (hit && before < want) push(t.cand, &t.count, key, j);
+    want -= all;
+  }
+}
+
+// The K largest logits in order (equal ones by column) into lp / idx. Every thread's largest is
+// known from the row's pass; the K-th largest of these is a bound that K logits reach, and few
+// more do (85 on average for K = 64 of 32,000 with 256 threads), so only the vectors that reach
+// it are read again, gathered and ranked against each other. Where more than kCap reach it
+// (rows with many equal logits) the K-th largest key is found by bisection over the row.
+template <int NTH, typename R>
+__device__ void top_k(const R& row, int V, int K, const Best& b, float last, float m, float inv_t,
+                      float lns, TopShared<NTH>& t, float* lp, int64_t* idx) {
+  const int tid = threadIdx.x;
+  const int nv = V >> 3;
+  t.best[tid] = fmaxf(b.v1, last);
+  if (tid == 0) t.count = 0;
+  __syncthreads();
+  if (tid < 64) {  // the upper 16 bits of the bound, bit by bit (the lower ones as zeros)
+    uint32_t k[NTH / 64];
+#pragma unroll
+    for (int i = 0; i < NTH / 64; ++i) k[i] = key_of(t.best[i * 64 + tid]) >> 16;
+    uint32_t tau = 0;
+    if (K <= NTH) {
+      for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t to = tau | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NTH / 64; ++i) n += __popcll(__ballot(k[i] >= to));
+        if (n >= K) tau = to;
+      }
+    }
+    if (tid == 0) t.tau = max(tau << 16, kNone + 1);
+  }
+  __syncthreads();
+  const uint32_t tau = t.tau;
+  auto take = [&](int j, float x) {
+    const uint32_t k = key_of(x);
+    if (k >= tau) push(t.cand, &t.count, k, j);
+  };
+  if (key_of(b.v1) >= tau && b.c1 >= 0) {
+    const bool more = key_of(b.v2) >= tau;
+    for (int c = more ? tid : b.c1; c < nv; c += more ? NTH : nv) {
+      float v[8];
+      R::unpack(row.load(c), v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) take(c * 8 + k, v[k]);
+    }
+  }
+  if (nv * 8 + tid < V) take(nv * 8 + tid, last);
+  __syncthreads();
+  int n = t.count;
+  if (n > kCap) {
+    uint32_t lo = tau, hi = 0xffffffffu;  // K keys are at least lo, fewer at least hi
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (count_from<NTH>(row, V, mid, t) >= K) lo = mid; else hi = mid;
+    }
+    __syncthreads();
+    if (tid == 0) t.count = 0;
+    __syncthreads();
+    for_row<NTH>(
+        row, V,
+        [&](int c, const float (&v)[8]) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (key_of(v[k]) > lo) push(t.cand, &t.count, key_of(v[k]), c * 8 + k);
+        },
+        [&](int j, float x) {
+          if (key_of(x) > lo) push(t.cand, &t.count, key_of(x), j);
+        });
+    __syncthreads();
+    n = t.count;
+    append_equal<NTH>(row, V, lo, K - n, t);
+    __syncthreads();
+    n = t.count;
+  }
+  if (n < K) {  // fewer numbers than K: -inf (and NaN) fill the places
+    append_equal<NTH>(row, V, kNone, K - n, t);
+    __syncthreads();
+    n = t.count;
+  }
+  for (int i = tid; i < n; i += NTH) {
+    const uint64_t mine = t.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += t.cand[j] > mine;
+    if (rank < K) {
+      const float x = of_key(static_cast<uint32_t>(mine >> 32));
+      lp[rank] = lns == -INFINITY ? -INFINITY : (x - m) * inv_t - lns;
+      idx[rank] = static_cast<int64_t>(static_cast<uint32_t>(~static_cast<uint32_t>(mine)));
+    }
+  }
+}
+
+template <typename E, bool BIAS, int NTH, bool TOP>
+__global__ void __launch_bounds__(NTH) logprobs_kernel(
+    int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
+    const int64_t* __restrict__ targets, int64_t ignore, float inv_t, int K,
+    float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ stats,
+    float* __restrict__ top_lp, int64_t* __restrict__ top_idx, uint32_t* err) {
+  __shared__ float sh[2 * (NTH / 64)];
+  const size_t r = blockIdx.x;
+  const Row<E, BIAS> row{logits + r * ldl, bias};
+  const float c = inv_t * kLog2e;
+  Share a;
+  Best best;
+  float last = -INFINITY;
+  for_row<NTH>(
+      row, V,
+      [&](int k, const float (&v)[8]) {
+        const float vm = max8(v);
+        fold8<true, false>(a, v, vm, c, 0);
+        if constexpr (TOP) best.see(vm, k);
+      },
+      [&](int, float x) {
+        fold1<true, false>(a, x, c, false);
+        last = x;
+      });
+  join<NTH, true, false>(a, c, sh);
+  const float lns = a.s == 0.0f ? -INFINITY : logf(a.s);
+  if (threadIdx.x == 0) {
+    const float h = lns - a.u * inv_t / a.s;
+    entropy[r] = a.s == 0.0f || h < 0.0f ? 0.0f : h;
+    if (stats) {
+      stats[2 * r] = a.m;
+      stats[2 * r + 1] = a.s;
+    }
+    if (logprob) {
+      const int64_t t = targets[r];
+      float lp = 0.0f;
+      if (t != ignore) {
+        if (t < 0 || t >= V) {
+          atomicOr(err, kErrToken);
+          lp = NAN;
+        } else {
+          lp = a.s == 0.0f ? -INFINITY : (row.at(t) - a.m) * inv_t - lns;
+        }
+      }
+      logprob[r] = lp;
+    }
+  }
+  if constexpr (TOP) {
+    __shared__ TopShared<NTH> t;
+    top_k<NTH>(row, V, K, best, last, a.m, inv_t, lns, t, top_lp + r * K, top_idx + r * K);
+  }
+}
+
+// ---- where a gradient goes -----------------------------------------------------------------
+// A row of the logits' type, or (planes) two bf16 rows whose sum holds 17 bits of the fp32
+// value: the gradient products of a bf16 readout then run as bf16 matrix products with an
+// error of 2^-18 a term, far below the 2^-9 that their bf16 results are rounded by; one bf16
+// row would add as much as that rounding.
+template <typename E>
+struct RowOut {
+  E* p;
+  __device__ __forceinline__ void put(int64_t j, float v) const { st(p, j, v); }
+  __device__ __forceinline__ void put8(int c, const float (&v)[8]) const {
+    E* q = p + static_cast<size_t>(c) * 8;
+    if constexpr (is_bf16<E>::value) {
+      u32x4 u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        u[k] = static_cast<uint32_t>(f2bf(v[2 * k])) |
+               static_cast<uint32_t>(f2bf(v[2 * k + 1])) << 16;
+      *reinterpret_cast<u32x4_any*>(q) = u;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = __builtin_bit_cast(uint32_t, v[4 * h + k]);
+        *reinterpret_cast<u32x4_any*>(q + 4 * h) = u;
+      }
+    }
+  }
+};
+struct PlanesOut {
+  bf16* p;
+  int64_t plane;
+  __device__ __forceinline__ static float left(float v) {
+    const float r = v - bf2f(f2bf(v));
+    return r == r ? r : 0.0f;  // inf and NaN are the first plane's alone
+  }
+  __device__ __forceinline__ void put(int64_t j, float v) const {
+    p[j] = f2bf(v);
+    p[plane + j] = f2bf(left(v));
+  }
+  __device__ __forceinline__ void put8(int c, const float (&v)[8]) const {
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = left(v[k]);
+    RowOut<bf16>{p}.put8(c, v);
+    RowOut<bf16>{p + plane}.put8(c, w);
+  }
+};
+template <typename E, bool PLANES>
+__device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_t plane) {
+  if constexpr (PLANES) {
+    return PlanesOut{static_cast<bf16*>(out) + r * ldo, plane};
+  } else {
+    return RowOut<E>{static_cast<E*>(out) + r * ldo};
+  }
+}
+
+// d x_j = -(p_j / T) (g_lp + sum g_top + g_H (logp_j + H)), plus g_lp / T at the target and
+// g_top / T at the alternatives. The whole row is written without these, then their places.
+template <typename E, bool BIAS, int NTH, bool PLANES>
+__global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
+    int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
+    const int64_t* __restrict__ targets, int64_t ignore, float inv_t, int K,
+    const int64_t* __restrict__ top_idx, const float* __restrict__ stats,
+    const float* __restrict__ entropy, const float* __restrict__ g_lp,
+    const float* __restrict__ g_ent, const float* __restrict__ g_top, void* out, int64_t ldo,
+    int64_t plane) {
+  __shared__ int taken;
+  const size_t r = blockIdx.x;
+  const Row<E, BIAS> row{logits + r * ldl, bias};
+  const auto o = out_row<E, PLANES>(out, r, ldo, plane);
+  const float c = inv_t * kLog2e, m = stats[2 * r], s = stats[2 * r + 1];
+  int64_t t = targets && g_lp ? targets[r] : -1;
+  const bool off = targets && g_lp && t != ignore && (t < 0 || t >= V);  // a NaN row
+  const bool aim = targets && g_lp && t != ignore && !off;
+  const float gl = aim ? g_lp[r] * inv_t : 0.0f;
+  float sum = gl;
+  if (g_top) {
+    float part = 0.0f;
+    for (int k = threadIdx.x & 63; k < K; k += 64) part += g_top[r * K + k];
+    sum += wave_sum(part) * inv_t;
+  }
+  const float ge = g_ent ? g_ent[r] * inv_t : 0.0f;
+  const float is = s == 0.0f ? 0.0f : 1.0f / s;
+  const float lns = s == 0.0f ? 0.0f : logf(s);
+  const float A = off ? NAN : -(sum + ge * (entropy[r] - lns)) * is, B = -ge * inv_t * is;
+  auto grad = [&](float x) {
+    const float d = x - m;
+    return __builtin_amdgcn_exp2f(d * c) * (A + B * fmaxf(d, -1e30f));
+  };
+  if (threadIdx.x == 0) taken = 0;
+  for_row<NTH>(
+      row, V,
+      [&](int k, const float (&v)[8]) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = grad(v[e]);
+        o.put8(k, w);
+      },
+      [&](int j, float x) { o.put(j, grad(x)); });
+  __syncthreads();
+  if (s == 0.0f) return;  // no finite logit: nothing depends on the row
+  if (g_top) {
+    for (int k = threadIdx.x; k < K; k += NTH) {
+      const int64_t j = top_idx[r * K + k];
+      const bool both = aim && j == t;
+      if (both) taken = 1;
+      o.put(j, grad(row.at(j)) + (g_top[r * K + k] * inv_t + (both ? gl : 0.0f)));
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && aim && !taken) o.put(t, grad(row.at(t)) + gl);
+}
+
+// ---- distillation --------------------------------------------------------------------------
+// One row: the teacher's weights q of its listed tokens (64 bits: one less their sum is what
+// the rest gets), the student's softmax, the loss
+//   sum q (ln q - logp) + q_r (ln q_r - ln p_r),  p_r the student's mass off the list,
+// and the coefficients of its gradient p_j b - q_j at listed and p_j a at other tokens:
+//   b = Q / s, a = b - q_r / r  (Q = sum q + q_r, r = the student's exp-sum off the list).
+// A bit per word (with the rest; else per word modulo kBits) marks the listed tokens: the rest's
+// sum leaves them out one by one, as a difference of sums would lose a small rest, and a bit
+// that was set before shows that a token may be listed twice.
+constexpr int kBits = 32768;
+constexpr int kMaxRestVocab = 480000;  // 60 KB of bits
+
+struct Teacher {
+  int idx[kMaxTop];  // -1: absent
+  float q[kMaxTop];
+  float a, b;
+  int twice;
+};
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_max_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// Writes the row's gradient times sc; a token listed twice has both weights at its place.
+template <int NTH, typename R, typename O>
+__device__ __forceinline__ void distill_grad(const R& row, int V, int K, float m, float c,
+                                             float sc, float a, float b, bool twice,
+                                             const int* idx, const float* q, const O& o) {
+  const float asc = a * sc, bsc = b * sc;
+  for_row<NTH>(
+      row, V,
+      [&](int k, const float (&v)[8]) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f((v[e] - m) * c) * asc;
+        o.put8(k, w);
+      },
+      [&](int j, float x) { o.put(j, __builtin_amdgcn_exp2f((x - m) * c) * asc); });
+  __syncthreads();
+  for (int k = threadIdx.x; k < K; k += NTH) {
+    const int j = idx[k];
+    if (j < 0) continue;
+    float w = q[k];
+    bool first = true;
+    if (twice) {
+      w = 0.0f;
+      for (int i = 0; i < K; ++i) {
+        const bool same = idx[i] == j;
+        first = first && !(same && i < k);
+        w += same ? q[i] : 0.0f;
+      }
+    }
+    if (first) o.put(j, __builtin_amdgcn_exp2f((row.at(j) - m) * c) * bsc - w * sc);
+  }
+}
+
+// GRAD 0: loss and coefficients; 1: and the row's gradient (T / count), as the fused readout
+// takes it while the logits are at hand.
+template <typename E, bool BIAS, int NTH, bool REST, bool GRAD, bool PLANES>
+__global__ void __launch_bounds__(NTH) distill_kernel(
+    int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias, int K,
+    int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
+    int64_t ignore, float inv_t, const float* __restrict__ teacher_lse, int words,
+    float* __restrict__ loss, float* __restrict__ coef, float* __restrict__ weights,
+    const float* __restrict__ scale, void* out, int64_t ldo, int64_t plane, uint32_t* err) {
+  extern __shared__ uint32_t bits[];
+  __shared__ float sh[2 * (NTH / 64)];
+  __shared__ Teacher te;
+  const size_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const Row<E, BIAS> row{logits + r * ldl, bias};
+  const float c = inv_t * kLog2e;
+  for (int i = tid; i < words; i += NTH) bits[i] = 0;
+  if (tid == 0) te.twice = 0;
+  __syncthreads();
+  double q[2], logq[2], rest = 0.0, total = 0.0;
+  float x[2];
+  bool some = false, wrong = false;
+  if (tid < 64) {
+    double u[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = tid + 64 * h;
+      u[h] = -INFINITY;
+      x[h] = 0.0f;
+      int j = -1;
+      if (k < K) {
+        const int64_t at = tokens[r * K + k];
+        const float v = value_type == kBF16 ? ld(static_cast<const bf16*>(values), r * K + k)
+                                            : ld(static_cast<const float*>(values), r * K + k);
+        if (at != ignore) {
+          if (at < 0 || at >= V) {
+            wrong = true;
+          } else if (v != -INFINITY) {
+            j = static_cast<int>(at);
+            u[h] = static_cast<double>(v) * inv_t;
+            x[h] = row.at(at);
+            const uint32_t bit = static_cast<uint32_t>(j) % (static_cast<uint32_t>(words) * 32);
+            if (atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1) te.twice = 1;
+          }
+        }
+        te.idx[k] = j;
+      }
+      some = some || j >= 0;
+    }
+    wrong = __any(wrong);
+    some = __any(some);
+    double norm;
+    if constexpr (REST) {
+      norm = teacher_lse[r];
+    } else {
+      const double top = wave_max_d(fmax(u[0], u[1]));
+      norm = top + log(wave_sum_d(exp(u[0] - top) + exp(u[1] - top)));
+    }
+    double all = 0.0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = tid + 64 * h;
+      logq[h] = u[h] - norm;
+      q[h] = k < K && te.idx[k] >= 0 ? exp(logq[h]) : 0.0;
+      all += q[h];
+    }
+    total = wave_sum_d(all);
+    if constexpr (REST) rest = 1.0 - total;
+  }
+  __syncthreads();
+  Share a;
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
+  for_row<NTH>(
+      row, V,
+      [&](int k, const float (&v)[8]) {
+        fold8<false, REST>(a, v, max8(v), c, REST ? bytes[k] : 0);
+      },
+      [&](int j, float y) {
+        fold1<false, REST>(a, y, c, REST && (bytes[j >> 3] >> (j & 7) & 1));
+      });
+  join<NTH, false, REST>(a, c, sh);
+  if (tid < 64) {
+    const bool empty = a.s == 0.0f;
+    const float lns = empty ? 0.0f : logf(a.s);
+    double part = 0.0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float logp = empty ? -INFINITY : (x[h] - a.m) * inv_t - lns;
+      if (q[h] != 0.0) part += q[h] * (logq[h] - logp);
+    }
+    double l = wave_sum_d(part);
+    if constexpr (REST) {
+      // A rest that the student's mask or a list of all tokens leaves no room for is left out.
+      rest = rest > 0.0 && a.r != 0.0f ? rest : 0.0;
+      if (rest != 0.0) l += rest * (log(rest) - (logf(a.r) - lns));
+      total += rest;
+    }
+    float b = empty ? 0.0f : static_cast<float>(total / a.s);
+    float ca = b;
+    if constexpr (REST) {
+      if (rest != 0.0) ca = static_cast<float>(total / a.s - rest / a.r);
+    }
+    if (!some) b = ca = 0.0f, l = 0.0;
+    if (wrong) b = ca = NAN, l = NAN;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = tid + 64 * h;
+      if (k < K) {
+        // A row without a finite logit has no gradient.
+        const float w = te.idx[k] < 0 ? -1.0f : empty ? 0.0f : static_cast<float>(q[h]);
+        te.q[k] = w;
+        if (weights) weights[r * K + k] = w;
+      }
+    }
+    if (tid == 0) {
+      if (wrong) atomicOr(err, kErrToken);
+      loss[2 * r] = static_cast<float>(l);
+      loss[2 * r + 1] = some || wrong ? 1.0f : 0.0f;
+      if (coef) {
+        coef[4 * r] = a.m;
+        coef[4 * r + 1] = ca;
+        coef[4 * r + 2] = b;
+        coef[4 * r + 3] = te.twice ? 1.0f : 0.0f;
+      }
+      te.a = ca;
+      te.b = b;
+    }
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    distill_grad<NTH>(row, V, K, a.m, c, scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
+                      out_row<E, PLANES>(out, r, ldo, plane));
+  }
+}
+
+template <typename E, int NTH>
+__global__ void __launch_bounds__(NTH) distill_bwd_kernel(
+    int V, int64_t ldl, const E* __restrict__ logits, int K, const int64_t* __restrict__ tokens,
+    float inv_t, const float* __restrict__ coef, const float* __restrict__ weights,
+    const float* __restrict__ scale, const float* __restrict__ grad, E* __restrict__ out) {
+  __shared__ int idx[kMaxTop];
+  __shared__ float q[kMaxTop];
+  const size_t r = blockIdx.x;
+  for (int k = threadIdx.x; k < K; k += NTH) {
+    const float w = weights[r * K + k];
+    q[k] = w;
+    idx[k] = w < 0.0f ? -1 : static_cast<int>(tokens[r * K + k]);  // a NaN weight is listed
+  }
+  distill_grad<NTH>(Row<E, false>{logits + r * ldl, nullptr}, V, K, coef[4 * r], inv_t * kLog2e,
+                    scale[0] * grad[0], coef[4 * r + 1], coef[4 * r + 2], coef[4 * r + 3] != 0.0f,
+                    idx, q, RowOut<E>{out + r * V});
+}
+
+// mean = T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = T / that count; the sums in
+// 64 bits and a fixed order, one block.
+__global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, const float* __restrict__ loss,
+                                                            float t, float* __restrict__ mean,
+                                                            float* __restrict__ factor) {
+  __shared__ double sh[2][16];
+  double l = 0.0, n = 0.0;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    l += loss[2 * r];
+    n += loss[2 * r + 1];
+  }
+  l = wave_sum_d(l);
+  n = wave_sum_d(n);
+  if ((threadIdx.x & 63) == 0) {
+    sh[0][threadIdx.x >> 6] = l;
+    sh[1][threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    l = n = 0.0;
+    for (int w = 0; w < 16; ++w) {
+      l += sh[0][w];
+      n += sh[1][w];
+    }
+    n = n < 1.0 ? 1.0 : n;
+    if (mean) mean[0] = static_cast<float>(static_cast<double>(t) * t * l / n);
+    if (factor) factor[0] = static_cast<float>(t / n);
+  }
+}
+
+// loss[r] = (0, 1) for rows that the mean counts, (0, 0) for the others: with the kernel above
+// the factor T / count before any logits are there. A wave takes a row.
+__global__ void __launch_bounds__(256) distill_rows_kernel(int64_t rows, int V, int K, int value_type,
+                                                           const void* __restrict__ values,
+                                                           const int64_t* __restrict__ tokens,
+                                                           int64_t ignore, float* __restrict__ loss) {
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  bool some = false;
+  for (int k = threadIdx.x & 63; k < K; k += 64) {
+    const int64_t at = tokens[r * K + k];
+    const float v = value_type == kBF16 ? ld(static_cast<const bf16*>(values), r * K + k)
+                                        : ld(static_cast<const float*>(values), r * K + k);
+    some = some || (at != ignore && (v != -INFINITY || at < 0 || at >= V));
+  }
+  some = __any(some);
+  if ((threadIdx.x & 63) == 0) {
+    loss[2 * r] = 0.0f;
+    loss[2 * r + 1] = some ? 1.0f : 0.0f;
+  }
+}
+
+// part[b][c] = the sum over the rows b * kSumRows + 0 .. of column c of bf16 rows x (stride ld).
+constexpr int kSumRows = 64;
+__global__ void __launch_bounds__(256) column_sums_kernel(int64_t rows, int V, int64_t ld,
+                                                          const bf16* __restrict__ x,
+                                                          float* __restrict__ part) {
+  const unsigned strips = (V + 2047) / 2048, b = blockIdx.x / strips;
+  const int c = ((blockIdx.x - b * strips) * 256 + threadIdx.x) * 8;
+  if (c >= V) return;
+  const int64_t r0 = static_cast<int64_t>(b) * kSumRows, r1 = min(rows, r0 + kSumRows);
+  float sum[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
+#pragma unroll 8
+  for (int64_t r = r0; r < r1; ++r) {  // the stride is a multiple of 8: whole vectors
+    const u32x4 u = *reinterpret_cast<const u32x4*>(x + r * ld + c);
+    float v[8];
+    Row<bf16, false>::halves(u, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] += c + k < V ? v[k] : 0.0f;
+  }
+  float* o = part + static_cast<size_t>(b) * V + c;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (c + k < V) o[k] = sum[k];
+}
+__global__ void __launch_bounds__(256) add_parts_kernel(int64_t parts, int V,
+                                                        const float* __restrict__ part, int add,
+                                                        float* __restrict__ out) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= V) return;
+  float s = add ? out[c] : 0.0f;
+#pragma unroll 8
+  for (int64_t p = 0; p < parts; ++p) s += part[p * V + c];
+  out[c] = s;
+}
+
+// out[i] = x[i] * g[0] in the type of out: gradients held in fp32 from the forward, rounded once.
+template <typename E>
+__global__ void __launch_bounds__(256) scaled_kernel(int64_t n, const float* __restrict__ x,
+                                                     const float* __restrict__ g,
+                                                     E* __restrict__ out) {
+  const float s = g[0];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * 8;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += step) {
+    if (i + 8 <= n) {
+      float v[8];
+      Row<float, false>::unpack(Row<float, false>{x + i, nullptr}.load(0), v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= s;
+      RowOut<E>{out + i}.put8(0, v);
+    } else {
+      for (int64_t j = i; j < n; ++j) st(out, j, x[j] * s);
+    }
+  }
+}
+
+static int checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t ldl, float t) {
+  DABSN_REQUIRE(dtype == kF32 || dtype == kBF16, "%s: bad dtype %d", what, dtype);
+  DABSN_REQUIRE(rows >= 0 && rows < (1ll << 31) && V > 0 && V < (1ll << 31) - 4096 && ldl >= V,
+                "%s: bad shape (rows=%lld, V=%lld, ld=%lld)", what, (long long)rows, (long long)V,
+                (long long)ldl);
+  DABSN_REQUIRE(t >= 1e-6f && t <= 1e6f, "%s: temperature %g lies outside [1e-6, 1e6]", what,
+                static_cast<double>(t));
+  return DABSN_OK;
+}
+
+// Threads a row: a wave where the row is a few vectors; the whole of a compute unit where fewer
+// rows than two a unit are there; else 256, of which eight rows share a unit.
+static int threads(int64_t rows, int64_t V) { return V <= 1024 ? 64 : rows < 512 && V >= 8192 ? 1024 : 256; }
+
+}  // namespace vocab
+}  // namespace dabsn
+
+using namespace dabsn;
+using namespace dabsn::vocab;
+
+#define DABSN_BY_THREADS(M)                     \
+  do {                                          \
+    if (nth == 64) { M(64); }                   \
+    else if (nth == 256) { M(256); }            \
+    else { M(1024); }                           \
+  } while (0)
+
+extern "C" {
+
+int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
+                             const void* bias, const int64_t* targets, int64_t ignore_index,
+                             float temperature, int64_t top, float* logprob, float* entropy,
+                             float* stats, float* top_logprobs, int64_t* top_indices,
+                             uint32_t* err, hipStream_t stream) {
+  int rc = checks("token log probabilities", dtype, rows, V, ldl, temperature);
+  if (rc != DABSN_OK) return rc;
+  DABSN_REQUIRE(top >= 0 && top <= kMaxTop && top <= V,
+                "token log probabilities: top %lld of %lld words (at most %d)", (long long)top,
+                (long long)V, kMaxTop);
+  DABSN_REQUIRE(!bias || dtype == kF32, "token log probabilities: a bias goes with fp32 logits");
+  if (rows == 0) return DABSN_OK;
+  DABSN_REQUIRE(logits && entropy && err && (!logprob || targets) &&
+                    (top == 0 || (top_logprobs && top_indices)),
+                "token log probabilities: null pointer");
+  const int nth = threads(rows, V);
+  const dim3 grid(static_cast<unsigned>(rows));
+  const float inv_t = 1.0f / temperature;
+  const bf16* b = static_cast<const bf16*>(bias);
+#define DABSN_LAUNCH(E, BIAS, N, TOP)                                                          \
+  hipLaunchKernelGGL((logprobs_kernel<E, BIAS, N, TOP>), grid, dim3(N), 0, stream, (int)V, ldl, \
+                     static_cast<const E*>(logits), b, targets, ignore_index, inv_t, (int)top,  \
+                     logprob, entropy, stats, top_logprobs, top_indices, err)
+#define DABSN_ROWS(N)                                                                          \
+  if (dtype == kBF16) {                                                                        \
+    if (top) DABSN_LAUNCH(bf16, false, N, true); else DABSN_LAUNCH(bf16, false, N, false);      \
+  } else if (b) {                                                                              \
+    if (top) DABSN_LAUNCH(float, true, N, true); else DABSN_LAUNCH(float, true, N, false);      \
+  } else {                                                                                     \
+    if (top) DABSN_LAUNCH(float, false, N, true); else DABSN_LAUNCH(float, false, N, false);    \
+  }
+  DABSN_BY_THREADS(DABSN_ROWS);
+#undef DABSN_ROWS
+#undef DABSN_LAUNCH
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void* logits,
+                                 int64_t ldl, const void* bias, const int64_t* targets,
+                                 int64_t ignore_index, float temperature, int64_t top,
+                                 const int64_t* top_indices, const float* stats,
+                                 const float* entropy, const float* g_logprob,
+                                 const float* g_entropy, const float* g_top, void* out,
+                                 int64_t ldo, int64_t plane, hipStream_t stream) {
+  int rc = checks("token log probabilities backward", dtype, rows, V, ldl, temperature);
+  if (rc != DABSN_OK) return rc;
+  DABSN_REQUIRE(top >= 0 && top <= kMaxTop && top <= V && ldo >= V && plane >= 0 &&
+                    (plane == 0 || (dtype == kF32 && plane >= rows * ldo)) &&
+                    (!bias || dtype == kF32),
+                "token log probabilities backward: bad arguments");
+  if (rows == 0) return DABSN_OK;
+  DABSN_REQUIRE(logits && stats && entropy && out && (!g_logprob || targets) &&
+                    (!g_top || (top > 0 && top_indices)),
+                "token log probabilities backward: null pointer");
+  const int nth = threads(rows, V);
+  const dim3 grid(static_cast<unsigned>(rows));
+  const float inv_t = 1.0f / temperature;
+  const bf16* b = static_cast<const bf16*>(bias);
+#define DABSN_LAUNCH(E, BIAS, N, PLANES)                                                         \
+  hipLaunchKernelGGL((logprobs_bwd_kernel<E, BIAS, N, PLANES>), grid, dim3(N), 0, stream, (int)V, \
+                     ldl, static_cast<const E*>(logits), b, targets, ignore_index, inv_t,         \
+                     (int)top, top_indices, stats, entropy, g_logprob, g_entropy, g_top, out,     \
+                     ldo, plane)
+#define DABSN_ROWS(N)                                                                             \
+  if (dtype == kBF16) {                                                                           \
+    DABSN_LAUNCH(bf16, false, N, false);                                                          \
+  } else if (b) {                                                                                 \
+    if (plane) DABSN_LAUNCH(float, true, N, true); else DABSN_LAUNCH(float, true, N, false);       \
+  } else {                                                                                        \
+    if (plane) DABSN_LAUNCH(float, false, N, true); else DABSN_LAUNCH(float, false, N, false);     \
+  }
+  DABSN_BY_THREADS(DABSN_ROWS);
+#undef DABSN_ROWS
+#undef DABSN_LAUNCH
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+static int distill_checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t ldl,
+                          int64_t top, float temperature) {
+  int rc = checks(what, dtype, rows, V, ldl, temperature);
+  if (rc != DABSN_OK) return rc;
+  DABSN_REQUIRE(top > 0 && top <= kMaxTop, "%s: %lld listed tokens a row (1 to %d)", what,
+                (long long)top, kMaxTop);
+  return DABSN_OK;
+}
+
+int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype,
+                           const void* values, const int64_t* tokens, int64_t ignore_index,
+                           float* loss, hipStream_t stream) {
+  int rc = distill_checks("distillation rows", kF32, rows, V, V, top, 1.0f);
+  if (rc != DABSN_OK) return rc;
+  DABSN_REQUIRE(value_dtype == kF32 || value_dtype == kBF16, "distillation rows: bad dtype %d",
+                value_dtype);
+  if (rows == 0) return DABSN_OK;
+  DABSN_REQUIRE(values && tokens && loss, "distillation rows: null pointer");
+  hipLaunchKernelGGL(distill_rows_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0,
+                     stream, rows, (int)V, (int)top, value_dtype, values, tokens, ignore_index,
+                     loss);
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float* mean,
+                           float* factor, hipStream_t stream) {
+  DABSN_REQUIRE(rows >= 0 && (rows == 0 || loss) && (mean || factor),
+                "distillation mean: bad arguments");
+  hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, stream, rows, loss, temperature,
+                     mean, factor);
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
+                      const void* bias, int64_t top, int value_dtype, const void* values,
+                      const int64_t* tokens, int64_t ignore_index, float temperature,
+                      const float* teacher_lse, float* loss, float* coef, float* weights,
+                      const float* scale, void* out, int64_t ldo, int64_t plane, uint32_t* err,
+                      hipStream_t stream) {
+  int rc = distill_checks("distillation", dtype, rows, V, ldl, top, temperature);
+  if (rc != DABSN_OK) return rc;
+  DABSN_REQUIRE(value_dtype == kF32 || value_dtype == kBF16, "distillation: bad value dtype %d",
+                value_dtype);
+  DABSN_REQUIRE(!teacher_lse || V <= kMaxRestVocab,
+                "distillation: the rest of more than %d words is not supported (V=%lld)",
+                kMaxRestVocab, (long long)V);
+  DABSN_REQUIRE(!bias || dtype == kF32, "distillation: a bias goes with fp32 logits");
+  DABSN_REQUIRE(!out || (dtype == kF32 && ldo >= V && (plane == 0 || plane >= rows * ldo) && scale),
+                "distillation: bad gradient rows");
+  if (rows == 0) return DABSN_OK;
+  DABSN_REQUIRE(logits && values && tokens && loss && err, "distillation: null pointer");
+  const int nth = threads(rows, V);
+  const dim3 grid(static_cast<unsigned>(rows));
+  const float inv_t = 1.0f / temperature;
+  const bf16* b = static_cast<const bf16*>(bias);
+  const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 31) / 32);
+#define DABSN_LAUNCH(E, BIAS, N, REST, GRAD, PLANES)                                             \
+  hipLaunchKernelGGL((distill_kernel<E, BIAS, N, REST, GRAD, PLANES>), grid, dim3(N), 4 * words,  \
+                     stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype, \
+                     values, tokens, ignore_index, inv_t, teacher_lse, words, loss, coef, weights, \
+                     scale, out, ldo, plane, err)
+#define DABSN_REST(E, BIAS, N, GRAD, PLANES)                    \
+  if (teacher_lse) DABSN_LAUNCH(E, BIAS, N, true, GRAD, PLANES); \
+  else DABSN_LAUNCH(E, BIAS, N, false, GRAD, PLANES)
+#define DABSN_ROWS(N)                                                                        \
+  if (dtype == kBF16) {                                                                      \
+    DABSN_REST(bf16, false, N, false, false);                                                \
+  } else if (!out) {                                                                         \
+    if (b) { DABSN_REST(float, true, N, false, false); }                                     \
+    else { DABSN_REST(float, false, N, false, false); }                                      \
+  } else if (plane) {                                                                        \
+    if (b) { DABSN_REST(float, true, N, true, true); }                                       \
+    else { DABSN_REST(float, false, N, true, true); }                                        \
+  } else {                                                                                   \
+    if (b) { DABSN_REST(float, true, N, true, false); }                                      \
+    else { DABSN_REST(float, false, N, true, false); }                                       \
+  }
+  DABSN_BY_THREADS(DABSN_ROWS);
+#undef DABSN_ROWS
+#undef DABSN_REST
+#undef DABSN_LAUNCH
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
+                          int64_t top, const int64_t* tokens, float temperature, const float* coef,
+                          const float* weights, const float* scale, const float* grad,
+                          void* dlogits, hipStream_t stream) {
+  int rc = distill_checks("distillation backward", dtype, rows, V, ldl, top, temperature);
+  if (rc != DABSN_OK) return rc;
+  if (rows == 0) return DABSN_OK;
+  DABSN_REQUIRE(logits && tokens && coef && weights && scale && grad && dlogits,
+                "distillation backward: null pointer");
+  const int nth = threads(rows, V);
+  const dim3 grid(static_cast<unsigned>(rows));
+  const float inv_t = 1.0f / temperature;
+#define DABSN_LAUNCH(E, N)                                                                       \
+  hipLaunchKernelGGL((distill_bwd_kernel<E, N>), grid, dim3(N), 0, stream, (int)V, ldl,           \
+                     static_cast<const E*>(logits), (int)top, tokens, inv_t, coef, weights, scale, \
+                     grad, static_cast<E*>(dlogits))
+#define DABSN_ROWS(N) \
+  if (dtype == kBF16) { DABSN_LAUNCH(bf16, N); } else { DABSN_LAUNCH(float, N); }
+  DABSN_BY_THREADS(DABSN_ROWS);
+#undef DABSN_ROWS
+#undef DABSN_LAUNCH
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V) {
+  return rows <= 0 || V <= 0 ? 0 : static_cast<size_t>((rows + kSumRows - 1) / kSumRows) * V;
+}
+
+int dabsn_hip_column_sums(int64_t rows, int64_t V, int64_t ld, const void* x, int add,
+                          float* partials, float* out, hipStream_t stream) {
+  const int64_t parts = (rows + kSumRows - 1) / kSumRows, strips = (V + 2047) / 2048;
+  DABSN_REQUIRE(rows >= 0 && V > 0 && V < (1ll << 31) - 4096 && parts * strips < (1ll << 31) && ld >= V &&
+                    ld % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && out &&
+                    (rows == 0 || (x && partials)),
+                "column sums: bad arguments (rows=%lld, V=%lld, ld=%lld)", (long long)rows,
+                (long long)V, (long long)ld);
+  if (rows > 0)
+    hipLaunchKernelGGL(column_sums_kernel,
+                       dim3(static_cast<unsigned>(strips * parts)), dim3(256), 0, stream, rows, (int)V, ld, static_cast<const bf16*>(x), partials);
+  hipLaunchKernelGGL(add_parts_kernel, dim3(static_cast<unsigned>((V + 255) / 256)), dim3(256), 0,
+                     stream, parts, (int)V, partials, add, out);
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* scale, void* out,
+                     hipStream_t stream) {
+  DABSN_REQUIRE((dtype == kF32 || dtype == kBF16) && n >= 0 && (n == 0 || (x && scale && out)),
+                "scaled copy: bad arguments");
+  if (n == 0) return DABSN_OK;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + 2047) / 2048, 1 << 16)));
+  if (dtype == kBF16)
+    hipLaunchKernelGGL((scaled_kernel<bf16>), grid, dim3(256), 0, stream, n, x, scale,
+                       static_cast<bf16*>(out));
+  else
+    hipLaunchKernelGGL((scaled_kernel<float>), grid, dim3(256), 0, stream, n, x, scale,
+                       static_cast<float*>(out));
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,262 @@
+"""Calls of the vocabulary-row and embedding kernels, shared by ``scoring``, ``distill`` and
+``embedding``: argument checks, error words, and the readout products of the chunked forms.
+
+Indices out of range are found by the kernels. These operators run once per token in serving and
+inside captured training steps, so they do not wait for the device: the kernel sets the device's
+sticky error word, which ``check_errors()`` (and the training read) raises, and the row in
+question is NaN. ``DABSN_HIP_ERROR_CHECK=sync`` raises from the call instead.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import math
+import os
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+from . import ops
+
+MAX_TOP = 128
+MAX_REST_VOCAB = 480_000
+MAX_VOCAB = (1 << 31) - 4097
+_CHUNK_BUDGET = 1 << 24
+_TOKEN_ERROR = "a token lies outside [0, V) and is not ignore_index"
+_HERE = contextlib.nullcontext()
+
+
+def on(t: Tensor):
+    """The device of ``t`` as the current one (the library launches on the current device)."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def need_device(what: str, *tensors: Tensor | None) -> None:
+    """All tensors on one ROCm device."""
+    first = None
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.type != "cuda":
+            raise RuntimeError(f"{what}: DABSN HIP operators need ROCm device tensors")
+        if first is None:
+            first = t.device
+        elif t.device != first:
+            raise RuntimeError(f"{what}: tensors on {first} and {t.device}")
+
+
+def need_float(what: str, name: str, t: Tensor) -> None:
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{what}: {name} must be float32 or bfloat16, not {t.dtype}")
+
+
+def need_tokens(what: str, name: str, t: Tensor, shape) -> Tensor:
+    """Token numbers of the given shape as contiguous int64."""
+    if t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: {name} must be int64 or int32, not {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} {tuple(t.shape)} does not match {tuple(shape)}")
+    if t.dtype != torch.int64:
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def need_temperature(what: str, t: float) -> float:
+    t = float(t)
+    if not (math.isfinite(t) and 1e-6 <= t <= 1e6):
+        raise ValueError(f"{what}: temperature must lie in [1e-6, 1e6], not {t}")
+    return t
+
+
+def need_vocab(what: str, v: int) -> int:
+    if not 0 < v <= MAX_VOCAB:
+        raise ValueError(f"{what}: a vocabulary of {v} words")
+    return v
+
+
+def rows_of(x: Tensor) -> Tensor:
+    """x [..., V] as [rows, V] with unit column stride and rows that do not overlap."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if (x.stride(1) != 1 and x.shape[1] > 1) or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
+        x = x.contiguous()
+    return x
+
+
+def row_stride(x: Tensor) -> int:
+    """The row stride of ``rows_of``'s result (a lone row's stride says nothing)."""
+    return max(x.stride(0), x.shape[1])
+
+
+def grads_of(g: Tensor | None) -> Tensor | None:
+    return None if g is None else g.to(torch.float32).contiguous()
+
+
+class ErrorWord:
+    """The int32 word a call's kernels set for tokens out of range (see the module's note)."""
+
+    __slots__ = ("word", "own")
+
+    def __init__(self, device: torch.device):
+        self.own = ops._sync_mode() == "sync"
+        self.word = (torch.zeros(1, device=device, dtype=torch.int32) if self.own
+                     else ops._sticky(device))
+
+    def check(self, what: str) -> None:
+        if self.own:
+            ops._record_error_word(self.word.view(torch.uint8), what, _TOKEN_ERROR)
+
+
+def chunk_rows(rows: int, vocab: int, budget: int | None) -> int:
+    """Rows a chunk, so that its logits stay within the element budget of the readout loss
+    (``DABSN_LOSS_CHUNK_SCORES``, default 2**24; not positive or ``off``: all rows at once)."""
+    if budget is None:
+        env = os.environ.get("DABSN_LOSS_CHUNK_SCORES", "")
+        try:
+            budget = int(env) if env else _CHUNK_BUDGET
+        except ValueError:
+            budget = 0 if env.lower() == "off" else _CHUNK_BUDGET
+    if budget <= 0:
+        return max(rows, 1)
+    return max(1, min(max(rows, 1), int(budget) // max(1, vocab)))
+
+
+class Readout:
+    """The readout of rows ``hidden`` [N, H] by ``weight`` [V, H] and ``bias`` [V]: logits of
+    row ranges in fp32. A bf16 readout's product keeps its fp32 sums (a rounding of the logits to
+    bf16, 2^-9 of values around 10, would show in every log probability) and leaves the bias to
+    the row kernel; adding it in the product took 30% longer (8192 x 2048 x 32000: 846 against
+    1135 TFLOP/s)."""
+
+    def __init__(self, hidden: Tensor, weight: Tensor, bias: Tensor | None):
+        self.hidden, self.weight, self.bias = hidden, weight, bias
+        self.half = hidden.dtype == torch.bfloat16
+        self.row_bias = bias if self.half else None
+        self.V, self.H = int(weight.shape[0]), int(weight.shape[1])
+        self.wt = weight.t()
+
+    def logits(self, s: int, e: int) -> Tensor:
+        h = self.hidden[s:e]
+        if self.half:
+            return torch.mm(h, self.wt, out_dtype=torch.float32)
+        return torch.mm(h, self.wt) if self.bias is None else torch.addmm(self.bias, h, self.wt)
+
+
+def need_readout(what: str, hidden: Tensor, weight: Tensor, bias: Tensor | None):
+    """(hidden [N, H], weight, bias) of one type, contiguous; inside autocast in its type, as
+    ``F.linear`` casts them."""
+    if hidden.dim() < 2 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: hidden [..., H] and weight [V, H] do not match: "
+                         f"{tuple(hidden.shape)}, {tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"{what}: bias {tuple(bias.shape)} does not match {weight.shape[0]} words")
+    need_vocab(what, int(weight.shape[0]))
+    if weight.shape[1] == 0:
+        raise ValueError(f"{what}: hidden rows of width 0")
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(dt), weight.to(dt)
+        bias = None if bias is None else bias.to(dt)
+    need_float(what, "hidden", hidden)
+    if weight.dtype != hidden.dtype or (bias is not None and bias.dtype != hidden.dtype):
+        raise TypeError(f"{what}: hidden, weight and bias must share a type")
+    hidden = hidden.reshape(-1, hidden.shape[-1]).contiguous()
+    return hidden, weight.contiguous(), None if bias is None else bias.contiguous()
+
+
+class ReadoutGrads:
+    """Gradients of a ``Readout`` from gradient rows of its logits, in fp32: the row kernel
+    writes rows where ``rows`` says, and ``done`` adds their products.
+
+    fp32 readouts: fp32 rows and products. bf16 ones: two bf16 planes that hold 17 bits of each
+    value, stacked as twice the rows of one bf16 product with fp32 sums; several chunks share a
+    product, as many rows as the hidden width (the planes then take no more than the weight's fp32
+    gradient): a product of few rows reaches a fifth of the rate (524 rows x 32000 x 2048: 243
+    TFLOP/s, 8192 rows: 1356)."""
+
+    def __init__(self, r: Readout, need, chunk: int):
+        self.r, self.need = r, need
+        n, V, H, dev = int(r.hidden.shape[0]), r.V, r.H, r.hidden.device
+        f32 = torch.float32
+        self.hidden = torch.empty((n, H), device=dev, dtype=f32) if need[0] else None
+        self.weight = None
+        self.bias = torch.zeros(V, device=dev, dtype=f32) if need[2] else None
+        self.ldo = -(-V // 8) * 8 if r.half else V
+        # The products' copies (two fp32 rows and two bf16 rows of H a row) stay within the
+        # weight's fp32 gradient or 512 MB.
+        fit = max(1, max(4 * V * H, 1 << 29) // (12 * H))
+        self.chunk = max(1, min(chunk, n, fit)) if n else 1
+        self.group = min(n, self.chunk * max(1, min(fit, H) // self.chunk)) if r.half else self.chunk
+        shape = (2, self.group, self.ldo) if r.half else (self.group, V)
+        self.buf = torch.empty(shape, device=dev, dtype=r.hidden.dtype) if n else None
+        self.first = True
+
+    def groups(self):
+        n = int(self.r.hidden.shape[0])
+        return [(s, min(n, s + self.group)) for s in range(0, n, max(self.group, 1))]
+
+    def begin(self, g0: int, g1: int) -> None:
+        self.g0, self.g1 = g0, g1
+        if g1 - g0 < self.group:  # the last, shorter group: planes of its own height
+            m = g1 - g0
+            self.buf = (self.buf.reshape(-1)[:2 * m * self.ldo].reshape(2, m, self.ldo)
+                        if self.r.half else self.buf[:m])
+
+    def rows(self, s: int):
+        """(pointer, row stride, plane stride) of the gradient rows from row s on."""
+        if self.r.half:
+            return self.buf[0, s - self.g0].data_ptr(), self.ldo, (self.g1 - self.g0) * self.ldo
+        return self.buf[s - self.g0].data_ptr(), self.ldo, 0
+
+    def end(self) -> None:
+        r, m, f32 = self.r, self.g1 - self.g0, torch.float32
+        rows = r.hidden[self.g0:self.g1]
+        if not r.half:
+            d = self.buf
+            if self.need[0]:
+                torch.mm(d, r.weight, out=self.hidden[self.g0:self.g1])
+            if self.need[1]:
+                self.weight = (torch.mm(d.t(), rows) if self.first
+                               else self.weight.addmm_(d.t(), rows))
+            if self.need[2]:
+                self.bias += d.sum(dim=0)
+            self.first = False
+            return
+        d = self.buf.view(2 * m, self.ldo)[:, :r.V]
+        if self.need[0]:
+            p = torch.mm(d, r.weight, out_dtype=f32)
+            torch.add(p[:m], p[m:], out=self.hidden[self.g0:self.g1])
+            del p
+        if self.need[1]:
+            both = torch.cat((rows, rows))
+            if self.first:
+                self.weight = torch.mm(d.t(), both, out_dtype=f32)
+            else:
+                torch.addmm(self.weight, d.t(), both, out_dtype=f32, out=self.weight)
+            del both
+        if self.need[2]:
+            lib = _lib.load()
+            part = torch.empty(lib.dabsn_hip_column_sums_partials(2 * m, r.V), device=d.device,
+                               dtype=f32)
+            _lib.check(lib.dabsn_hip_column_sums(2 * m, r.V, self.ldo, self.buf.data_ptr(), 1,
+                                                 part.data_ptr(), self.bias.data_ptr(),
+                                                 ops._stream(d)), "readout bias gradient")
+        self.first = False
+
+    def results(self):
+        """(hidden, weight, bias) gradients in fp32, None where not needed."""
+        if self.need[1] and self.weight is None:
+            self.weight = torch.zeros((self.r.V, self.r.H), device=self.r.hidden.device,
+                                      dtype=torch.float32)
+        return self.hidden, self.weight, self.bias
+
+
+def scaled(x: Tensor | None, g: Tensor, like: torch.dtype) -> Tensor | None:
+    """fp32 ``x`` times the device scalar g, rounded once to ``like``."""
+    if x is None:
+        return None
+    out = torch.empty(x.shape, device=x.device, dtype=like)
+    _lib.check(_lib.load().dabsn_hip_scaled(ops._code(like), x.numel(), x.data_ptr(), g.data_ptr(),
+                                            out.data_ptr(), ops._stream(x)), "scaled gradient")
+    return out

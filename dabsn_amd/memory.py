@@ -260,8 +260,11 @@ class DABSNMemory:
 
 def fingerprint_of(model: DABSNSequenceLM) -> dict[str, object]:
     """Architecture identity a memory must match: the reference's dictionary, key for key
-    (memory.py:149-161), so files cross-load in both directions."""
+    (memory.py:149-161), so files cross-load in both directions; a scaled embedding, which the
+    reference has not, adds its scale."""
+    scaled = {} if model.embed_scale is None else {"embed_scale": model.embed_scale}
     return {
+        **scaled,
         "vocab": int(model.vocab),
         "hidden_dim": int(model.hidden_dim),
         "depth": int(model.depth),
@@ -287,8 +290,8 @@ def _check_fingerprint(memory: DABSNMemory, model: DABSNSequenceLM) -> None:
     observed.setdefault("mlp_middle_depth", 0)
     observed.setdefault("mlp_depth_index", 0)
     if observed != expected:
-        bad = [f"{k}: memory={observed.get(k)!r} model={v!r}"
-               for k, v in expected.items() if observed.get(k) != v]
+        bad = [f"{k}: memory={observed.get(k)!r} model={expected.get(k)!r}"
+               for k in {**expected, **observed} if observed.get(k) != expected.get(k)]
         raise ValueError("memory was built by a different architecture: " + "; ".join(bad))
 
 
@@ -368,7 +371,7 @@ def _run(model: DABSNSequenceLM, ids: Tensor, memory: DABSNMemory | None, *,
     outputs = []
     with torch.no_grad(), ops.reuse_parameter_copies():
         for start, stop in _chunks(int(ids.shape[1]), chunk_size):
-            hidden = model.embed(ids[:, start:stop])
+            hidden = model.embed_tokens(ids[:, start:stop])
             for i, block in enumerate(blocks):
                 hidden, state[i] = _block_step(block, hidden, state[i], position)
             outputs.append(hidden)

@@ -22,8 +22,11 @@ from torch import Tensor
 from torch.utils.checkpoint import checkpoint
 
 from .core import DABSNCore
+from .distill import chunked_linear_distillation
+from .embedding import scaled_embedding
 from .kernels import ops, pipeline
 from .read import DABSNRead
+from .scoring import TokenLogprobs, chunked_linear_token_logprobs
 
 
 class MLPRMSNorm(nn.Module):
@@ -259,15 +262,20 @@ class DABSNSequenceLM(nn.Module):
     specs (e.g. ``"seq:2048:2048,seq:2048:2048"``); without it, ``depth`` blocks of
     ``hidden_dim`` (state ``state_dim``) are built. Only the seq read geometry is built
     here; the field/hybrid geometries and the middle MLP stack are outside this backend.
+
+    ``embed_scale`` (None: the plain embedding) multiplies the token embedding, as a model with
+    tied embeddings wants: the table then runs through ``scaled_embedding``.
     """
 
     is_dabsn_sequence_lm = True
+    embed_scale: float | None = None
 
     def __init__(self, vocab: int, hidden_dim: int, depth: int = 1, layer_geometries=None, *,
                  layers=None, state_dim: int | None = None, tie_embeddings: bool = False,
                  grad_checkpoint: bool = False, residual: bool = False,
                  mlp_ratio: float | None = None, mlp_middle_depth: int = 0,
-                 mlp_depth_index: int = 0, block_chunk_t: int | None = None) -> None:
+                 mlp_depth_index: int = 0, block_chunk_t: int | None = None,
+                 embed_scale: float | None = None) -> None:
         super().__init__()
         del grad_checkpoint  # block time-chunking (block_chunk_t) is this backend's checkpoint
         if int(mlp_middle_depth) != 0:
@@ -290,6 +298,7 @@ class DABSNSequenceLM(nn.Module):
         self.layers = specs
         self.depth = len(specs)
         self.layer_geometries = [s.read_geometry for s in specs]
+        self.embed_scale = None if embed_scale is None else float(embed_scale)
         self.embed = nn.Embedding(self.vocab, self.hidden_dim)
         self.backbone = DABSNBackbone(self.hidden_dim, specs, residual=self.residual,
                                       mlp_ratio=self.mlp_ratio, block_chunk_t=block_chunk_t)
@@ -303,8 +312,34 @@ class DABSNSequenceLM(nn.Module):
     def blocks(self) -> nn.ModuleList:
         return self.backbone.blocks
 
+    def embed_tokens(self, ids: Tensor) -> Tensor:
+        if self.embed_scale is None:
+            return self.embed(ids)
+        return scaled_embedding(ids, self.embed.weight, scale=self.embed_scale)
+
     def forward_hidden(self, ids: Tensor) -> Tensor:
-        return self.backbone(self.embed(ids))
+        return self.backbone(self.embed_tokens(ids))
 
     def forward(self, ids: Tensor) -> Tensor:
         return self.readout(self.forward_hidden(ids))
+
+    def token_logprobs(self, ids: Tensor, *, top: int = 0, temperature: float = 1.0,
+                       chunk_budget: int | None = None) -> TokenLogprobs:
+        """Scores of ``ids`` [B, T]: at position t the log probability of token t + 1 given the
+        tokens up to t (0 at the last position), the entropy there and the ``top`` likeliest
+        next tokens; the logits [B, T, V] are never held at once."""
+        targets = torch.full_like(ids, -100)
+        targets[:, :-1] = ids[:, 1:]
+        return chunked_linear_token_logprobs(
+            self.forward_hidden(ids), self.readout.weight, self.readout.bias, targets, top=top,
+            temperature=temperature, ignore_index=-100, chunk_budget=chunk_budget)
+
+    def distillation_loss(self, ids: Tensor, top_logits: Tensor, top_indices: Tensor, *,
+                          temperature: float = 1.0, teacher_lse: Tensor | None = None,
+                          ignore_index: int = -100, chunk_budget: int | None = None) -> Tensor:
+        """Distillation loss of this model's next-token distributions on ``ids`` [B, T] against a
+        teacher's top logits and tokens [B, T, K] (see ``chunked_linear_distillation``)."""
+        return chunked_linear_distillation(
+            self.forward_hidden(ids), self.readout.weight, self.readout.bias, top_logits,
+            top_indices, temperature=temperature, teacher_lse=teacher_lse,
+            ignore_index=ignore_index, chunk_budget=chunk_budget)

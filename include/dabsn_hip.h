@@ -17,7 +17,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#define DABSN_HIP_ABI_VERSION 20
+#define DABSN_HIP_ABI_VERSION 21
 
 /* Status codes returned by every entry point. */
 #define DABSN_OK 0
@@ -679,6 +679,86 @@ int dabsn_hip_ce_split(int64_t rows, int64_t V, const void* logits, int64_t ldl,
 int dabsn_hip_ce_bias(int64_t nparts, int64_t V, const float* part, int add, float* gbias,
                       hipStream_t stream);
 int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t stream);
+
+/* ---- vocabulary rows: token log probabilities and distillation --------------------
+ * New operators beside the readout loss (src/dabsn/runtime/loss.py:52-137), over the same
+ * logits [rows, V] (row stride ldl >= V, any alignment, `dtype` 0 fp32 / 1 bf16). With fp32
+ * logits `bias` (bf16 [V] or NULL) is added to every row: a bf16 readout's product kept in
+ * fp32. z = logits / temperature (1e-6 .. 1e6); softmax sums are fp32.
+ *
+ * dabsn_hip_token_logprobs: logprob [rows] (NULL: none) = log softmax(z)[target], 0 where
+ * target == ignore_index; entropy [rows]; the `top` (0 .. 128, <= V) largest logits' log
+ * probabilities [rows, top] and columns (int64), largest first, equal ones by column. Logits of
+ * -inf have probability 0; a row of only such has log probabilities -inf and entropy 0; a row
+ * with NaN or +inf has NaN. stats ([rows][2] or NULL) keeps what the backward needs. A target
+ * outside [0, V) sets *err to 1 and its log probability to NaN.
+ * _bwd: out = the logits' gradient for the given upstream gradients (each may be NULL), rows of
+ * stride ldo in the logits' type, or with plane > 0 (fp32 logits) two bf16 rows, out and
+ * out + plane, whose sum holds the fp32 value to 17 bits.
+ *
+ * dabsn_hip_distill: `top` (1 .. 128) listed tokens a row with the teacher's logits `values`
+ * (value_dtype 0 fp32 / 1 bf16); entries whose token is ignore_index or whose value is -inf are
+ * absent. q = softmax of values / temperature over the listed ones, or, with teacher_lse (the
+ * log-sum-exp of the teacher's whole row / temperature; V <= 480000), exp(values / temperature -
+ * teacher_lse) with the rest q_r = 1 - sum q on all other tokens as one event. loss [rows][2] =
+ * (KL(q || softmax(z)), 1 if the row has a listed token, else 0). coef [rows][4] and weights
+ * [rows][top] (NULL: none) are for _bwd. With out (fp32 logits) the gradient rows are written
+ * too, times scale[0], as above. A listed token outside [0, V) sets *err to 1 and its row to NaN.
+ * dabsn_hip_distill_rows: loss = (0, 1 or 0) without logits. dabsn_hip_distill_mean: mean[0] =
+ * temperature^2 * mean loss over the counted rows, factor[0] = temperature / their number (each
+ * may be NULL). dabsn_hip_distill_bwd: dlogits [rows, V] = d mean[0] / d logits * grad[0], given
+ * scale = factor. A token listed several times has the sum of its weights.
+ *
+ * dabsn_hip_column_sums: out [V] (added to with `add`) = column sums of bf16 rows x (stride ld,
+ * a multiple of 8), through partials [dabsn_hip_column_sums_partials]. dabsn_hip_scaled: out[i] =
+ * x[i] * scale[0], rounded once to dtype. */
+int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
+                             const void* bias, const int64_t* targets, int64_t ignore_index,
+                             float temperature, int64_t top, float* logprob, float* entropy,
+                             float* stats, float* top_logprobs, int64_t* top_indices,
+                             uint32_t* err, hipStream_t stream);
+int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void* logits,
+                                 int64_t ldl, const void* bias, const int64_t* targets,
+                                 int64_t ignore_index, float temperature, int64_t top,
+                                 const int64_t* top_indices, const float* stats,
+                                 const float* entropy, const float* g_logprob,
+                                 const float* g_entropy, const float* g_top, void* out,
+                                 int64_t ldo, int64_t plane, hipStream_t stream);
+int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype,
+                           const void* values, const int64_t* tokens, int64_t ignore_index,
+                           float* loss, hipStream_t stream);
+int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float* mean,
+                           float* factor, hipStream_t stream);
+int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
+                      const void* bias, int64_t top, int value_dtype, const void* values,
+                      const int64_t* tokens, int64_t ignore_index, float temperature,
+                      const float* teacher_lse, float* loss, float* coef, float* weights,
+                      const float* scale, void* out, int64_t ldo, int64_t plane, uint32_t* err,
+                      hipStream_t stream);
+int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
+                          int64_t top, const int64_t* tokens, float temperature, const float* coef,
+                          const float* weights, const float* scale, const float* grad,
+                          void* dlogits, hipStream_t stream);
+size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V);
+int dabsn_hip_column_sums(int64_t rows, int64_t V, int64_t ld, const void* x, int add,
+                          float* partials, float* out, hipStream_t stream);
+int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* scale, void* out,
+                     hipStream_t stream);
+
+/* ---- scaled token embedding ---------------------------------------------------------
+ * New operator for the language model's embedding (src/dabsn/model.py:804-860 has
+ * nn.Embedding): out [n, H] = scale * weight[ids] (int64 ids; weight rows of stride ldw >= H,
+ * any alignment), one rounding. An id outside [0, V) sets *err to 1 and its row to NaN.
+ * Backward: dweight [V, H] = scale * the sum of grad [n, H] over the tokens of each word, fp32
+ * sums in a fixed order, one rounding; zeros for words without tokens, for padding_idx and for
+ * ids out of range. Workspace: dabsn_hip_embedding_workspace_bytes(n, V, H) (0: refused). */
+int dabsn_hip_embedding_fwd(int dtype, int64_t n, int64_t V, int64_t H, const int64_t* ids,
+                            const void* weight, int64_t ldw, float scale, void* out, uint32_t* err,
+                            hipStream_t stream);
+size_t dabsn_hip_embedding_workspace_bytes(int64_t n, int64_t V, int64_t H);
+int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const int64_t* ids,
+                            int64_t padding_idx, const void* grad, float scale, void* dweight,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }
