@@ -9,9 +9,13 @@
 //                       teacher's normaliser, over the rest of the vocabulary as one event
 // and a backward that reads the logits once more and writes their gradient.
 //
-// Differences x - m are formed before they are scaled, so that masks of the type's lowest value
-// and -inf give exp 0 and never inf - inf. The pass is bound by memory: an element costs about
-// 10 vector instructions (4 of them the exponential's), half the time of its 2 bytes.
+// The pass is bound by memory where an element costs few instructions: 8 to 10 here (4 of them
+// the exponential's), against the 12 that a byte pair's time allows. So the exponent's argument is
+// one fma of the logit, x c - r with c = log2 e / T and r a reference near the thread's maximum
+// (any number does: e = 2^(x c - r) is exact in r), and r moves only when a vector exceeds it by
+// 2^16. c is rounded: the sums u of e (x c - r), which the entropy needs anyhow, give the exact
+// normaliser to first order. Logits so large that x c overflows leave s = 0 and take the row's
+// pass again with differences formed first: rows that hold nothing but a mask's lowest value.
 #include <algorithm>
 
 #include "../../include/dabsn_hip.h"
@@ -21,7 +25,7 @@
 namespace dabsn {
 namespace vocab {
 
-constexpr float kLog2e = 1.44269504088896341f;
+constexpr double kLn2 = 0.693147180559945309417;
 constexpr float kLowest = -3.40282346638528860e38f;
 constexpr int kMaxTop = 128;
 // Candidates of the top selection that fit: all of a vocabulary whose vectors of 8 are fewer
@@ -73,6 +77,11 @@ struct Row {
       for (int k = 0; k < 8; ++k) v[k] += w[k];
     }
   }
+  static __device__ __forceinline__ void keep(Raw& r) {
+    asm volatile("" : "+v"(r.v[0]));
+    if constexpr (!is_bf16<E>::value) asm volatile("" : "+v"(r.v[1]));
+    if constexpr (BIAS) asm volatile("" : "+v"(r.bias));
+  }
   __device__ __forceinline__ float at(int64_t j) const {
     float v = ld(x, static_cast<size_t>(j));
     if constexpr (BIAS) v += bf2f(b[j]);
@@ -86,16 +95,32 @@ template <int NTH, typename R, typename F, typename G>
 __device__ __forceinline__ void for_row(const R& row, int V, F f, G g) {
   constexpr int U = 4;
   const int nv = V >> 3;
-  for (int c0 = threadIdx.x; c0 < nv; c0 += U * NTH) {
+  int b = 0;  // the block's first vector
+  for (; b + U * NTH <= nv; b += U * NTH) {
     typename R::Raw raw[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) raw[k] = row.load(min(c0 + k * NTH, nv - 1));
+    for (int k = 0; k < U; ++k) raw[k] = row.load(b + k * NTH + threadIdx.x);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      if (c0 + k * NTH < nv) {
+      float v[8];
+      R::unpack(raw[k], v);
+      f(b + k * NTH + threadIdx.x, v);
+    }
+  }
+  if (b < nv) {
+    typename R::Raw raw[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) raw[k] = row.load(min(b + k * NTH + static_cast<int>(threadIdx.x), nv - 1));
+    // Without a use out here the compiler moves each load under its condition, one at a time.
+#pragma unroll
+    for (int k = 0; k < U; ++k) R::keep(raw[k]);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int c = b + k * NTH + threadIdx.x;
+      if (c < nv) {
         float v[8];
         R::unpack(raw[k], v);
-        f(c0 + k * NTH, v);
+        f(c, v);
       }
     }
   }
@@ -103,9 +128,14 @@ __device__ __forceinline__ void for_row(const R& row, int V, F f, G g) {
   if (j < V) g(j, row.at(j));
 }
 
+// Of a quiet NaN and a number the number; fmaxf adds an instruction an operand to quiet others.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 __device__ __forceinline__ float max8(const float (&v)[8]) {
-  return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])),
-               fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+  return max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[7]));
 }
 
 // The sum over the block of N values a thread, to every thread. sh: N * NTH/64 floats.
@@ -142,64 +172,135 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
   return v;
 }
 
-// A thread's share of a row: the maximum m (kLowest where it has no finite logit), s = sum
-// exp2((x - m) c), u = sum of these times (x - m) (the entropy's sum), r = the share of s at
-// tokens that are not listed. NaN and +inf make s NaN.
+// A thread's share of a row relative to its reference r: s = sum e, u = sum e arg with
+// e = 2^arg, rest = the share of s at tokens that are not listed. arg = x c - r; SAFE rows have
+// arg = (x - r) c. Logits of -inf give e = 0; NaN and +inf make s NaN.
+template <bool SAFE>
 struct Share {
-  float m = kLowest, s = 0.0f, u = 0.0f, r = 0.0f;
+  float r = SAFE ? kLowest : -3e38f, s = 0.0f, u = 0.0f, rest = 0.0f;
+  float c;
+  __device__ __forceinline__ explicit Share(float c_) : c(c_) {}
+  static __device__ __forceinline__ float arg(float x, float r, float c) {
+    return SAFE ? (x - r) * c : __builtin_fmaf(x, c, -r);
+  }
+  // The reference becomes `to`.
+  template <bool REST>
+  __device__ __forceinline__ void raise(float to) {
+    const float d = r == to ? 0.0f : SAFE ? (r - to) * c : r - to;  // both may be inf
+    const float f = __builtin_amdgcn_exp2f(d);
+    u = f == 0.0f ? 0.0f : f * (u + d * s);
+    s *= f;
+    if constexpr (REST) rest *= f;
+    r = to;
+  }
+  template <bool REST>
+  __device__ __forceinline__ void see(float largest) {
+    const float t = SAFE ? largest : largest * c;
+    if (t > (SAFE ? r : r + 16.0f)) raise<REST>(t);
+  }
+  template <bool REST>
+  __device__ __forceinline__ void fold8(const float (&v)[8], float vm, uint32_t listed) {
+    see<REST>(vm);
+    float vs = 0.0f, vr = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float a = arg(v[k], r, c);
+      const float e = __builtin_amdgcn_exp2f(a);
+      vs += e;
+      u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);  // arg = -inf has e = 0
+      if constexpr (REST) {
+        if (listed) vr += (listed >> k & 1) ? 0.0f : e;  // few vectors hold a listed token
+      }
+    }
+    s += vs;
+    if constexpr (REST) rest += listed ? vr : vs;
+  }
+  template <bool REST>
+  __device__ __forceinline__ void fold1(float x, bool listed) {
+    see<REST>(x);
+    const float a = arg(x, r, c), e = __builtin_amdgcn_exp2f(a);
+    s += e;
+    u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);
+    if constexpr (REST) rest += listed ? 0.0f : e;
+  }
+  // The block's shares as one, to every thread.
+  template <int NTH, bool REST>
+  __device__ __forceinline__ void join(float* sh) {
+    raise<REST>(block_max<NTH>(r, sh));
+    float v[2 + REST];
+    v[0] = s;
+    v[1] = u;
+    if constexpr (REST) v[2] = rest;
+    block_sums<NTH, 2 + REST>(v, sh);
+    s = v[0];
+    u = v[1];
+    if constexpr (REST) rest = v[2];
+  }
 };
 
-template <bool ENT, bool REST>
-__device__ __forceinline__ void raise(Share& a, float to, float c) {
-  const float d = a.m - to;
-  const float f = __builtin_amdgcn_exp2f(d * c);
-  if constexpr (ENT) a.u = f == 0.0f ? 0.0f : f * (a.u + d * a.s);
-  a.s *= f;
-  if constexpr (REST) a.r *= f;
-  a.m = to;
-}
-
-template <bool ENT, bool REST>
-__device__ __forceinline__ void fold8(Share& a, const float (&v)[8], float vm, float c,
-                                      uint32_t listed) {
-  if (vm > a.m) raise<ENT, REST>(a, vm, c);
-  float vs = 0.0f, vr = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float d = v[k] - a.m;
-    const float e = __builtin_amdgcn_exp2f(d * c);
-    vs += e;
-    if constexpr (ENT) a.u += e * fmaxf(d, -1e30f);  // d = -inf has e = 0
-    if constexpr (REST) {
-      if (listed) vr += (listed >> k & 1) ? 0.0f : e;  // few vectors hold a listed token
-    }
+// What a row's pass leaves. Log probabilities are differences of numbers of the size of the
+// logits, so the few of a row are formed in 64 bits.
+struct Norm {
+  float r, s, u, rest;
+  bool safe;
+  // f(arg) with the row's form of the exponent's argument as a function of a logit.
+  template <typename F>
+  __device__ __forceinline__ void with_arg(float c, F f) const {
+    if (safe) f([r = r, c](float x) { return Share<true>::arg(x, r, c); });
+    else f([r = r, c](float x) { return Share<false>::arg(x, r, c); });
   }
-  a.s += vs;
-  if constexpr (REST) a.r += listed ? vr : vs;
+  __device__ __forceinline__ bool empty() const { return s == 0.0f; }  // no finite logit
+  // ln s, corrected for the rounding of c (log2 e / T = c (1 + delta)).
+  __device__ __forceinline__ double ln_s(double delta) const {
+    const double mean = static_cast<double>(u) / s + (safe ? 0.0 : static_cast<double>(r));
+    return log(static_cast<double>(s)) + kLn2 * delta * mean;
+  }
+  // log p of a logit x.
+  __device__ __forceinline__ double logp(float x, double inv_t, double ln_s) const {
+    if (empty()) return -INFINITY;
+    const double z = static_cast<double>(x);
+    return safe ? (z - r) * inv_t - ln_s : z * inv_t - (r * kLn2 + ln_s);
+  }
+};
+// 1 / T, c and its error, from the host.
+struct Scale {
+  double inv_t, delta;
+  float c;
+};
+static Scale scale_of(float t) {
+  Scale k;
+  k.inv_t = 1.0 / static_cast<double>(t);
+  k.c = static_cast<float>(k.inv_t / kLn2);
+  k.delta = k.inv_t / kLn2 / static_cast<double>(k.c) - 1.0;
+  return k;
 }
 
-template <bool ENT, bool REST>
-__device__ __forceinline__ void fold1(Share& a, float x, float c, bool listed) {
-  if (x > a.m) raise<ENT, REST>(a, x, c);
-  const float d = x - a.m, e = __builtin_amdgcn_exp2f(d * c);
-  a.s += e;
-  if constexpr (ENT) a.u += e * fmaxf(d, -1e30f);
-  if constexpr (REST) a.r += listed ? 0.0f : e;
+template <int NTH, bool REST, bool SAFE, typename R, typename See, typename Last>
+__device__ __forceinline__ Norm row_pass(const R& row, int V, float c, const uint8_t* listed,
+                                         float* sh, See see, Last last) {
+  Share<SAFE> a(c);
+  for_row<NTH>(
+      row, V,
+      [&](int k, const float (&v)[8]) {
+        const float vm = max8(v);
+        a.template fold8<REST>(v, vm, REST ? listed[k] : 0);
+        see(k, vm);
+      },
+      [&](int j, float x) {
+        a.template fold1<REST>(x, REST && (listed[j >> 3] >> (j & 7) & 1));
+        last(x);
+      });
+  a.template join<NTH, REST>(sh);
+  return Norm{a.r, a.s, a.u, a.rest, SAFE};
 }
-
-// The block's shares as one, to every thread.
-template <int NTH, bool ENT, bool REST>
-__device__ __forceinline__ void join(Share& a, float c, float* sh) {
-  const float M = block_max<NTH>(a.m, sh);
-  raise<ENT, REST>(a, M, c);
-  float v[1 + ENT + REST];
-  v[0] = a.s;
-  if constexpr (ENT) v[1] = a.u;
-  if constexpr (REST) v[ENT + 1] = a.r;
-  block_sums<NTH, 1 + ENT + REST>(v, sh);
-  a.s = v[0];
-  if constexpr (ENT) a.u = v[1];
-  if constexpr (REST) a.r = v[ENT + 1];
+// The row's norm; `see` gets each vector's number and largest logit, `last` the last logits.
+template <int NTH, bool REST, typename R, typename See, typename Last>
+__device__ __forceinline__ Norm norm_of(const R& row, int V, float c, const uint8_t* listed,
+                                        float* sh, See see, Last last) {
+  const Norm n = row_pass<NTH, REST, false>(row, V, c, listed, sh, see, last);
+  if (n.s != 0.0f) return n;
+  __syncthreads();
+  return row_pass<NTH, REST, true>(row, V, c, listed, sh, [](int, float) {}, [](float) {});
 }
 
 // ---- the K largest logits of a row ---------------------------------------------------------
@@ -282,14 +383,14 @@ __device__ void append_equal(const R& row, int V, uint32_t key, int want, TopSha
   }
 }
 
-// The K largest logits in order (equal ones by column) into lp / idx. Every thread's largest is
-// known from the row's pass; the K-th largest of these is a bound that K logits reach, and few
+// Gathers candidates that hold the K largest logits (equal ones by column). Every thread's
+// largest is known from the row's pass; the K-th largest of these is a bound that K logits reach, and few
 // more do (85 on average for K = 64 of 32,000 with 256 threads), so only the vectors that reach
 // it are read again, gathered and ranked against each other. Where more than kCap reach it
 // (rows with many equal logits) the K-th largest key is found by bisection over the row.
 template <int NTH, typename R>
-__device__ void top_k(const R& row, int V, int K, const Best& b, float last, float m, float inv_t,
-                      float lns, TopShared<NTH>& t, float* lp, int64_t* idx) {
+__device__ void top_k(const R& row, int V, int K, const Best& b, float last, bool nan,
+                      TopShared<NTH>& t) {
   const int tid = threadIdx.x;
   const int nv = V >> 3;
   t.best[tid] = fmaxf(b.v1, last);
@@ -329,8 +430,8 @@ __device__ void top_k(const R& row, int V, int K, const Best& b, float last, flo
   if (nv * 8 + tid < V) take(nv * 8 + tid, last);
   __syncthreads();
   int n = t.count;
-  if (n > kCap) {
-    uint32_t lo = tau, hi = 0xffffffffu;  // K keys are at least lo, fewer at least hi
+  if (n > kCap || nan) {  // a NaN may have hidden its neighbours' maximum
+    uint32_t lo = nan ? 0 : tau, hi = 0xffffffffu;  // K keys are at least lo, fewer at least hi
     while (hi - lo > 1) {
       const uint32_t mid = lo + (hi - lo) / 2;
       if (count_from<NTH>(row, V, mid, t) >= K) lo = mid; else hi = mid;
@@ -359,68 +460,61 @@ __device__ void top_k(const R& row, int V, int K, const Best& b, float last, flo
     __syncthreads();
     n = t.count;
   }
-  for (int i = tid; i < n; i += NTH) {
-    const uint64_t mine = t.cand[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += t.cand[j] > mine;
-    if (rank < K) {
-      const float x = of_key(static_cast<uint32_t>(mine >> 32));
-      lp[rank] = lns == -INFINITY ? -INFINITY : (x - m) * inv_t - lns;
-      idx[rank] = static_cast<int64_t>(static_cast<uint32_t>(~static_cast<uint32_t>(mine)));
-    }
-  }
 }
 
 template <typename E, bool BIAS, int NTH, bool TOP>
 __global__ void __launch_bounds__(NTH) logprobs_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
-    const int64_t* __restrict__ targets, int64_t ignore, float inv_t, int K,
+    const int64_t* __restrict__ targets, int64_t ignore, Scale k, int K,
     float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ stats,
     float* __restrict__ top_lp, int64_t* __restrict__ top_idx, uint32_t* err) {
   __shared__ float sh[2 * (NTH / 64)];
   const size_t r = blockIdx.x;
   const Row<E, BIAS> row{logits + r * ldl, bias};
-  const float c = inv_t * kLog2e;
-  Share a;
   Best best;
   float last = -INFINITY;
-  for_row<NTH>(
-      row, V,
-      [&](int k, const float (&v)[8]) {
-        const float vm = max8(v);
-        fold8<true, false>(a, v, vm, c, 0);
-        if constexpr (TOP) best.see(vm, k);
+  const Norm n = norm_of<NTH, false>(
+      row, V, k.c, nullptr, sh,
+      [&](int c, float vm) {
+        if constexpr (TOP) best.see(vm, c);
       },
-      [&](int, float x) {
-        fold1<true, false>(a, x, c, false);
-        last = x;
-      });
-  join<NTH, true, false>(a, c, sh);
-  const float lns = a.s == 0.0f ? -INFINITY : logf(a.s);
+      [&](float x) { last = x; });
+  const double ln_s = n.ln_s(k.delta);
+  auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (threadIdx.x == 0) {
-    const float h = lns - a.u * inv_t / a.s;
-    entropy[r] = a.s == 0.0f || h < 0.0f ? 0.0f : h;
+    const double h = ln_s - kLn2 * n.u / n.s;
+    entropy[r] = n.empty() || h < 0.0 ? 0.0f : static_cast<float>(h);
     if (stats) {
-      stats[2 * r] = a.m;
-      stats[2 * r + 1] = a.s;
+      stats[2 * r] = n.r;
+      stats[2 * r + 1] = n.safe ? -n.s : n.s;
     }
     if (logprob) {
       const int64_t t = targets[r];
-      float lp = 0.0f;
+      float v = 0.0f;
       if (t != ignore) {
         if (t < 0 || t >= V) {
           atomicOr(err, kErrToken);
-          lp = NAN;
+          v = NAN;
         } else {
-          lp = a.s == 0.0f ? -INFINITY : (row.at(t) - a.m) * inv_t - lns;
+          v = lp(row.at(t));
         }
       }
-      logprob[r] = lp;
+      logprob[r] = v;
     }
   }
   if constexpr (TOP) {
     __shared__ TopShared<NTH> t;
-    top_k<NTH>(row, V, K, best, last, a.m, inv_t, lns, t, top_lp + r * K, top_idx + r * K);
+    top_k<NTH>(row, V, K, best, last, n.s != n.s, t);
+    const int count = t.count;
+    for (int i = threadIdx.x; i < count; i += NTH) {
+      const uint64_t mine = t.cand[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += t.cand[j] > mine;
+      if (rank < K) {
+        top_lp[r * K + rank] = lp(of_key(static_cast<uint32_t>(mine >> 32)));
+        top_idx[r * K + rank] = static_cast<int64_t>(~static_cast<uint32_t>(mine));
+      }
+    }
   }
 }
 
@@ -486,7 +580,7 @@ __device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_
 template <typename E, bool BIAS, int NTH, bool PLANES>
 __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
-    const int64_t* __restrict__ targets, int64_t ignore, float inv_t, int K,
+    const int64_t* __restrict__ targets, int64_t ignore, Scale k, int K,
     const int64_t* __restrict__ top_idx, const float* __restrict__ stats,
     const float* __restrict__ entropy, const float* __restrict__ g_lp,
     const float* __restrict__ g_ent, const float* __restrict__ g_top, void* out, int64_t ldo,
@@ -495,7 +589,8 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
   const size_t r = blockIdx.x;
   const Row<E, BIAS> row{logits + r * ldl, bias};
   const auto o = out_row<E, PLANES>(out, r, ldo, plane);
-  const float c = inv_t * kLog2e, m = stats[2 * r], s = stats[2 * r + 1];
+  const float inv_t = static_cast<float>(k.inv_t), c = k.c;
+  const Norm n{stats[2 * r], fabsf(stats[2 * r + 1]), 0.0f, 0.0f, stats[2 * r + 1] < 0.0f};
   int64_t t = targets && g_lp ? targets[r] : -1;
   const bool off = targets && g_lp && t != ignore && (t < 0 || t >= V);  // a NaN row
   const bool aim = targets && g_lp && t != ignore && !off;
@@ -503,39 +598,42 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
   float sum = gl;
   if (g_top) {
     float part = 0.0f;
-    for (int k = threadIdx.x & 63; k < K; k += 64) part += g_top[r * K + k];
+    for (int i = threadIdx.x & 63; i < K; i += 64) part += g_top[r * K + i];
     sum += wave_sum(part) * inv_t;
   }
   const float ge = g_ent ? g_ent[r] * inv_t : 0.0f;
-  const float is = s == 0.0f ? 0.0f : 1.0f / s;
-  const float lns = s == 0.0f ? 0.0f : logf(s);
-  const float A = off ? NAN : -(sum + ge * (entropy[r] - lns)) * is, B = -ge * inv_t * is;
-  auto grad = [&](float x) {
-    const float d = x - m;
-    return __builtin_amdgcn_exp2f(d * c) * (A + B * fmaxf(d, -1e30f));
-  };
+  const float is = n.empty() ? 0.0f : 1.0f / n.s;
+  const float lns = n.empty() ? 0.0f : logf(n.s);
+  const float A = off ? NAN : -(sum + ge * (entropy[r] - lns)) * is;
+  const float B = -ge * static_cast<float>(kLn2) * is;
   if (threadIdx.x == 0) taken = 0;
-  for_row<NTH>(
-      row, V,
-      [&](int k, const float (&v)[8]) {
-        float w[8];
+  n.with_arg(c, [&](auto arg) {
+    auto grad = [&](float x) {
+      const float a = arg(x);
+      return __builtin_amdgcn_exp2f(a) * __builtin_fmaf(B, fmaxf(a, -1e30f), A);
+    };
+    for_row<NTH>(
+        row, V,
+        [&](int j, const float (&v)[8]) {
+          float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = grad(v[e]);
-        o.put8(k, w);
-      },
-      [&](int j, float x) { o.put(j, grad(x)); });
-  __syncthreads();
-  if (s == 0.0f) return;  // no finite logit: nothing depends on the row
-  if (g_top) {
-    for (int k = threadIdx.x; k < K; k += NTH) {
-      const int64_t j = top_idx[r * K + k];
-      const bool both = aim && j == t;
-      if (both) taken = 1;
-      o.put(j, grad(row.at(j)) + (g_top[r * K + k] * inv_t + (both ? gl : 0.0f)));
-    }
+          for (int e = 0; e < 8; ++e) w[e] = grad(v[e]);
+          o.put8(j, w);
+        },
+        [&](int j, float x) { o.put(j, grad(x)); });
     __syncthreads();
-  }
-  if (threadIdx.x == 0 && aim && !taken) o.put(t, grad(row.at(t)) + gl);
+    if (n.empty()) return;  // nothing depends on the row
+    if (g_top) {
+      for (int i = threadIdx.x; i < K; i += NTH) {
+        const int64_t j = top_idx[r * K + i];
+        const bool both = aim && j == t;
+        if (both) taken = 1;
+        o.put(j, grad(row.at(j)) + (g_top[r * K + i] * inv_t + (both ? gl : 0.0f)));
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0 && aim && !taken) o.put(t, grad(row.at(t)) + gl);
+  });
 }
 
 // ---- distillation --------------------------------------------------------------------------
@@ -570,35 +668,37 @@ __device__ __forceinline__ double wave_max_d(double v) {
 
 // Writes the row's gradient times sc; a token listed twice has both weights at its place.
 template <int NTH, typename R, typename O>
-__device__ __forceinline__ void distill_grad(const R& row, int V, int K, float m, float c,
+__device__ __forceinline__ void distill_grad(const R& row, int V, int K, const Norm& n, float c,
                                              float sc, float a, float b, bool twice,
                                              const int* idx, const float* q, const O& o) {
   const float asc = a * sc, bsc = b * sc;
-  for_row<NTH>(
-      row, V,
-      [&](int k, const float (&v)[8]) {
-        float w[8];
+  n.with_arg(c, [&](auto arg) {
+    for_row<NTH>(
+        row, V,
+        [&](int k, const float (&v)[8]) {
+          float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f((v[e] - m) * c) * asc;
-        o.put8(k, w);
-      },
-      [&](int j, float x) { o.put(j, __builtin_amdgcn_exp2f((x - m) * c) * asc); });
-  __syncthreads();
-  for (int k = threadIdx.x; k < K; k += NTH) {
-    const int j = idx[k];
-    if (j < 0) continue;
-    float w = q[k];
-    bool first = true;
-    if (twice) {
-      w = 0.0f;
-      for (int i = 0; i < K; ++i) {
-        const bool same = idx[i] == j;
-        first = first && !(same && i < k);
-        w += same ? q[i] : 0.0f;
+          for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(arg(v[e])) * asc;
+          o.put8(k, w);
+        },
+        [&](int j, float x) { o.put(j, __builtin_amdgcn_exp2f(arg(x)) * asc); });
+    __syncthreads();
+    for (int k = threadIdx.x; k < K; k += NTH) {
+      const int j = idx[k];
+      if (j < 0) continue;
+      float w = q[k];
+      bool first = true;
+      if (twice) {
+        w = 0.0f;
+        for (int i = 0; i < K; ++i) {
+          const bool same = idx[i] == j;
+          first = first && !(same && i < k);
+          w += same ? q[i] : 0.0f;
+        }
       }
+      if (first) o.put(j, __builtin_amdgcn_exp2f(arg(row.at(j))) * bsc - w * sc);
     }
-    if (first) o.put(j, __builtin_amdgcn_exp2f((row.at(j) - m) * c) * bsc - w * sc);
-  }
+  });
 }
 
 // GRAD 0: loss and coefficients; 1: and the row's gradient (T / count), as the fused readout
@@ -607,16 +707,15 @@ template <typename E, bool BIAS, int NTH, bool REST, bool GRAD, bool PLANES>
 __global__ void __launch_bounds__(NTH) distill_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias, int K,
     int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
-    int64_t ignore, float inv_t, const float* __restrict__ teacher_lse, int words,
+    int64_t ignore, Scale sc, const float* __restrict__ teacher_lse, int words,
     float* __restrict__ loss, float* __restrict__ coef, float* __restrict__ weights,
     const float* __restrict__ scale, void* out, int64_t ldo, int64_t plane, uint32_t* err) {
   extern __shared__ uint32_t bits[];
-  __shared__ float sh[2 * (NTH / 64)];
+  __shared__ float sh[3 * (NTH / 64)];
   __shared__ Teacher te;
   const size_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const Row<E, BIAS> row{logits + r * ldl, bias};
-  const float c = inv_t * kLog2e;
   for (int i = tid; i < words; i += NTH) bits[i] = 0;
   if (tid == 0) te.twice = 0;
   __syncthreads();
@@ -640,7 +739,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
             wrong = true;
           } else if (v != -INFINITY) {
             j = static_cast<int>(at);
-            u[h] = static_cast<double>(v) * inv_t;
+            u[h] = v * sc.inv_t;
             x[h] = row.at(at);
             const uint32_t bit = static_cast<uint32_t>(j) % (static_cast<uint32_t>(words) * 32);
             if (atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1) te.twice = 1;
@@ -671,37 +770,28 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
     if constexpr (REST) rest = 1.0 - total;
   }
   __syncthreads();
-  Share a;
-  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bits);
-  for_row<NTH>(
-      row, V,
-      [&](int k, const float (&v)[8]) {
-        fold8<false, REST>(a, v, max8(v), c, REST ? bytes[k] : 0);
-      },
-      [&](int j, float y) {
-        fold1<false, REST>(a, y, c, REST && (bytes[j >> 3] >> (j & 7) & 1));
-      });
-  join<NTH, false, REST>(a, c, sh);
+  const Norm a = norm_of<NTH, REST>(row, V, sc.c, reinterpret_cast<const uint8_t*>(bits), sh,
+                                    [](int, float) {}, [](float) {});
   if (tid < 64) {
-    const bool empty = a.s == 0.0f;
-    const float lns = empty ? 0.0f : logf(a.s);
+    const bool empty = a.empty();
+    const double ln_s = a.ln_s(sc.delta);
     double part = 0.0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float logp = empty ? -INFINITY : (x[h] - a.m) * inv_t - lns;
+      const double logp = a.logp(x[h], sc.inv_t, ln_s);
       if (q[h] != 0.0) part += q[h] * (logq[h] - logp);
     }
     double l = wave_sum_d(part);
     if constexpr (REST) {
       // A rest that the student's mask or a list of all tokens leaves no room for is left out.
-      rest = rest > 0.0 && a.r != 0.0f ? rest : 0.0;
-      if (rest != 0.0) l += rest * (log(rest) - (logf(a.r) - lns));
+      rest = rest > 0.0 && a.rest != 0.0f ? rest : 0.0;
+      if (rest != 0.0) l += rest * (log(rest) - log(static_cast<double>(a.rest)) + ln_s);
       total += rest;
     }
     float b = empty ? 0.0f : static_cast<float>(total / a.s);
     float ca = b;
     if constexpr (REST) {
-      if (rest != 0.0) ca = static_cast<float>(total / a.s - rest / a.r);
+      if (rest != 0.0) ca = static_cast<float>(total / a.s - rest / a.rest);
     }
     if (!some) b = ca = 0.0f, l = 0.0;
     if (wrong) b = ca = NAN, l = NAN;
@@ -720,10 +810,10 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
       loss[2 * r] = static_cast<float>(l);
       loss[2 * r + 1] = some || wrong ? 1.0f : 0.0f;
       if (coef) {
-        coef[4 * r] = a.m;
+        coef[4 * r] = a.r;
         coef[4 * r + 1] = ca;
         coef[4 * r + 2] = b;
-        coef[4 * r + 3] = te.twice ? 1.0f : 0.0f;
+        coef[4 * r + 3] = (te.twice ? 1.0f : 0.0f) + (a.safe ? 2.0f : 0.0f);
       }
       te.a = ca;
       te.b = b;
@@ -731,7 +821,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   }
   if constexpr (GRAD) {
     __syncthreads();
-    distill_grad<NTH>(row, V, K, a.m, c, scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
+    distill_grad<NTH>(row, V, K, a, sc.c, scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
                       out_row<E, PLANES>(out, r, ldo, plane));
   }
 }
@@ -739,7 +829,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
 template <typename E, int NTH>
 __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, int K, const int64_t* __restrict__ tokens,
-    float inv_t, const float* __restrict__ coef, const float* __restrict__ weights,
+    float c, const float* __restrict__ coef, const float* __restrict__ weights,
     const float* __restrict__ scale, const float* __restrict__ grad, E* __restrict__ out) {
   __shared__ int idx[kMaxTop];
   __shared__ float q[kMaxTop];
@@ -749,9 +839,11 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
     q[k] = w;
     idx[k] = w < 0.0f ? -1 : static_cast<int>(tokens[r * K + k]);  // a NaN weight is listed
   }
-  distill_grad<NTH>(Row<E, false>{logits + r * ldl, nullptr}, V, K, coef[4 * r], inv_t * kLog2e,
-                    scale[0] * grad[0], coef[4 * r + 1], coef[4 * r + 2], coef[4 * r + 3] != 0.0f,
-                    idx, q, RowOut<E>{out + r * V});
+  const int flags = static_cast<int>(coef[4 * r + 3]);
+  const Norm n{coef[4 * r], 1.0f, 0.0f, 0.0f, (flags & 2) != 0};
+  distill_grad<NTH>(Row<E, false>{logits + r * ldl, nullptr}, V, K, n, c, scale[0] * grad[0],
+                    coef[4 * r + 1], coef[4 * r + 2], (flags & 1) != 0, idx, q,
+                    RowOut<E>{out + r * V});
 }
 
 // mean = T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = T / that count; the sums in
@@ -909,11 +1001,11 @@ int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* log
                 "token log probabilities: null pointer");
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
-  const float inv_t = 1.0f / temperature;
+  const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
 #define DABSN_LAUNCH(E, BIAS, N, TOP)                                                          \
   hipLaunchKernelGGL((logprobs_kernel<E, BIAS, N, TOP>), grid, dim3(N), 0, stream, (int)V, ldl, \
-                     static_cast<const E*>(logits), b, targets, ignore_index, inv_t, (int)top,  \
+                     static_cast<const E*>(logits), b, targets, ignore_index, scale_t, (int)top,  \
                      logprob, entropy, stats, top_logprobs, top_indices, err)
 #define DABSN_ROWS(N)                                                                          \
   if (dtype == kBF16) {                                                                        \
@@ -949,11 +1041,11 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
                 "token log probabilities backward: null pointer");
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
-  const float inv_t = 1.0f / temperature;
+  const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
 #define DABSN_LAUNCH(E, BIAS, N, PLANES)                                                         \
   hipLaunchKernelGGL((logprobs_bwd_kernel<E, BIAS, N, PLANES>), grid, dim3(N), 0, stream, (int)V, \
-                     ldl, static_cast<const E*>(logits), b, targets, ignore_index, inv_t,         \
+                     ldl, static_cast<const E*>(logits), b, targets, ignore_index, scale_t,         \
                      (int)top, top_indices, stats, entropy, g_logprob, g_entropy, g_top, out,     \
                      ldo, plane)
 #define DABSN_ROWS(N)                                                                             \
@@ -1020,26 +1112,27 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                 "distillation: the rest of more than %d words is not supported (V=%lld)",
                 kMaxRestVocab, (long long)V);
   DABSN_REQUIRE(!bias || dtype == kF32, "distillation: a bias goes with fp32 logits");
-  DABSN_REQUIRE(!out || (dtype == kF32 && ldo >= V && (plane == 0 || plane >= rows * ldo) && scale),
+  DABSN_REQUIRE(!out || (ldo >= V && (plane == 0 || (dtype == kF32 && plane >= rows * ldo)) && scale),
                 "distillation: bad gradient rows");
   if (rows == 0) return DABSN_OK;
   DABSN_REQUIRE(logits && values && tokens && loss && err, "distillation: null pointer");
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
-  const float inv_t = 1.0f / temperature;
+  const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
   const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 31) / 32);
 #define DABSN_LAUNCH(E, BIAS, N, REST, GRAD, PLANES)                                             \
   hipLaunchKernelGGL((distill_kernel<E, BIAS, N, REST, GRAD, PLANES>), grid, dim3(N), 4 * words,  \
                      stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype, \
-                     values, tokens, ignore_index, inv_t, teacher_lse, words, loss, coef, weights, \
+                     values, tokens, ignore_index, scale_t, teacher_lse, words, loss, coef, weights, \
                      scale, out, ldo, plane, err)
 #define DABSN_REST(E, BIAS, N, GRAD, PLANES)                    \
   if (teacher_lse) DABSN_LAUNCH(E, BIAS, N, true, GRAD, PLANES); \
   else DABSN_LAUNCH(E, BIAS, N, false, GRAD, PLANES)
 #define DABSN_ROWS(N)                                                                        \
   if (dtype == kBF16) {                                                                      \
-    DABSN_REST(bf16, false, N, false, false);                                                \
+    if (out) { DABSN_REST(bf16, false, N, true, false); }                                    \
+    else { DABSN_REST(bf16, false, N, false, false); }                                       \
   } else if (!out) {                                                                         \
     if (b) { DABSN_REST(float, true, N, false, false); }                                     \
     else { DABSN_REST(float, false, N, false, false); }                                      \
@@ -1069,10 +1162,10 @@ int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits
                 "distillation backward: null pointer");
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
-  const float inv_t = 1.0f / temperature;
+  const Scale scale_t = scale_of(temperature);
 #define DABSN_LAUNCH(E, N)                                                                       \
   hipLaunchKernelGGL((distill_bwd_kernel<E, N>), grid, dim3(N), 0, stream, (int)V, ldl,           \
-                     static_cast<const E*>(logits), (int)top, tokens, inv_t, coef, weights, scale, \
+                     static_cast<const E*>(logits), (int)top, tokens, scale_t.c, coef, weights, scale, \
                      grad, static_cast<E*>(dlogits))
 #define DABSN_ROWS(N) \
   if (dtype == kBF16) { DABSN_LAUNCH(bf16, N); } else { DABSN_LAUNCH(float, N); }

@@ -70,7 +70,7 @@ def test_library_refuses_bad_arguments_before_it_launches():
     for kw in (dict(dtype=3), dict(V=0), dict(ld=4), dict(top=0), dict(top=129), dict(vt=2), dict(t=0.0),
                dict(V=480_001, ld=480_001, lse=one), dict(dtype=1, bias=one), dict(out=one, ldo=4),
                dict(out=one, ldo=8, plane=15), dict(out=one, ldo=8, scale=None),
-               dict(dtype=1, out=one, ldo=8)):
+               dict(dtype=1, out=one, ldo=8, plane=16)):
         assert f(**kw) == -2, kw
     assert lib.dabsn_hip_distill_bwd(0, 2, 5, one, 5, 0, one, 1.0, one, one, one, one, one, None) == -2
     assert lib.dabsn_hip_distill_rows(2, 5, 0, 0, one, one, -100, one, None) == -2
