@@ -89,43 +89,85 @@ struct Row {
   }
 };
 
-// f(c, values) for this thread's vectors c = tid, tid + NTH, ... of the row's V / 8, four loads
-// in flight, then g(column, value) for its one element of the last V % 8.
-template <int NTH, typename R, typename F, typename G>
-__device__ __forceinline__ void for_row(const R& row, int V, F f, G g) {
-  constexpr int U = 4;
-  const int nv = V >> 3;
-  int b = 0;  // the block's first vector
-  for (; b + U * NTH <= nv; b += U * NTH) {
-    typename R::Raw raw[U];
+// A row's logits as its threads go through them: each(f, g) calls f(c, values) for this thread's
+// vectors c = tid, tid + NTH, ... of the row's V / 8, then g(column, value) for its one element
+// of the last V % 8. Streamed: from memory each time, four loads in flight.
+template <int NTH, typename R>
+struct Streamed {
+  const R& row;
+  int V;
+  template <typename F, typename G>
+  __device__ __forceinline__ void each(F f, G g) const {
+    constexpr int U = 4;
+    const int nv = V >> 3;
+    int b = 0;  // the block's first vector
+    for (; b + U * NTH <= nv; b += U * NTH) {
+      typename R::Raw raw[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) raw[k] = row.load(b + k * NTH + threadIdx.x);
+      for (int k = 0; k < U; ++k) raw[k] = row.load(b + k * NTH + threadIdx.x);
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      float v[8];
-      R::unpack(raw[k], v);
-      f(b + k * NTH + threadIdx.x, v);
+      for (int k = 0; k < U; ++k) {
+        float v[8];
+        R::unpack(raw[k], v);
+        f(b + k * NTH + threadIdx.x, v);
+      }
     }
+    if (b < nv) {
+      typename R::Raw raw[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) raw[k] = row.load(min(b + k * NTH + static_cast<int>(threadIdx.x), nv - 1));
+      // Without a use out here the compiler moves each load under its condition, one at a time.
+#pragma unroll
+      for (int k = 0; k < U; ++k) R::keep(raw[k]);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int c = b + k * NTH + threadIdx.x;
+        if (c < nv) {
+          float v[8];
+          R::unpack(raw[k], v);
+          f(c, v);
+        }
+      }
+    }
+    const int j = nv * 8 + threadIdx.x;
+    if (j < V) g(j, row.at(j));
   }
-  if (b < nv) {
-    typename R::Raw raw[U];
+};
+// Held: loaded once into NV vectors of registers a thread (V < 8 (NTH NV + 1)), for a row that is
+// read twice and written: the second reading otherwise comes from the memory side, as the rows
+// under way (2,048 of 64 KB) are far more than the L2 caches hold.
+template <int NTH, int NV, typename R>
+struct Held {
+  const R& row;
+  int V;
+  typename R::Raw raw[NV];
+  __device__ __forceinline__ Held(const R& row_, int V_) : row(row_), V(V_) {
+    const int nv = V >> 3;
 #pragma unroll
-    for (int k = 0; k < U; ++k) raw[k] = row.load(min(b + k * NTH + static_cast<int>(threadIdx.x), nv - 1));
-    // Without a use out here the compiler moves each load under its condition, one at a time.
+    for (int k = 0; k < NV; ++k)
+      raw[k] = row.load(max(0, min(k * NTH + static_cast<int>(threadIdx.x), nv - 1)));
+  }
+  template <typename F, typename G>
+  __device__ __forceinline__ void each(F f, G g) const {
+    const int nv = V >> 3;
 #pragma unroll
-    for (int k = 0; k < U; ++k) R::keep(raw[k]);
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int c = b + k * NTH + threadIdx.x;
+    for (int k = 0; k < NV; ++k) {
+      const int c = k * NTH + threadIdx.x;
       if (c < nv) {
         float v[8];
         R::unpack(raw[k], v);
         f(c, v);
       }
     }
+    const int j = nv * 8 + threadIdx.x;
+    if (j < V) g(j, row.at(j));
   }
-  const int j = nv * 8 + threadIdx.x;
-  if (j < V) g(j, row.at(j));
+};
+// NV = 0: streamed.
+template <int NTH, int NV, typename R>
+__device__ __forceinline__ auto source(const R& row, int V) {
+  if constexpr (NV > 0) return Held<NTH, NV, R>(row, V);
+  else return Streamed<NTH, R>{row, V};
 }
 
 // Of a quiet NaN and a number the number; fmaxf adds an instruction an operand to quiet others.
@@ -275,12 +317,11 @@ static Scale scale_of(float t) {
   return k;
 }
 
-template <int NTH, bool REST, bool SAFE, typename R, typename See, typename Last>
-__device__ __forceinline__ Norm row_pass(const R& row, int V, float c, const uint8_t* listed,
-                                         float* sh, See see, Last last) {
+template <int NTH, bool REST, bool SAFE, typename S, typename See, typename Last>
+__device__ __forceinline__ Norm row_pass(const S& src, float c, const uint8_t* listed, float* sh,
+                                         See see, Last last) {
   Share<SAFE> a(c);
-  for_row<NTH>(
-      row, V,
+  src.each(
       [&](int k, const float (&v)[8]) {
         const float vm = max8(v);
         a.template fold8<REST>(v, vm, REST ? listed[k] : 0);
@@ -294,13 +335,13 @@ __device__ __forceinline__ Norm row_pass(const R& row, int V, float c, const uin
   return Norm{a.r, a.s, a.u, a.rest, SAFE};
 }
 // The row's norm; `see` gets each vector's number and largest logit, `last` the last logits.
-template <int NTH, bool REST, typename R, typename See, typename Last>
-__device__ __forceinline__ Norm norm_of(const R& row, int V, float c, const uint8_t* listed,
-                                        float* sh, See see, Last last) {
-  const Norm n = row_pass<NTH, REST, false>(row, V, c, listed, sh, see, last);
+template <int NTH, bool REST, typename S, typename See, typename Last>
+__device__ __forceinline__ Norm norm_of(const S& src, float c, const uint8_t* listed, float* sh,
+                                        See see, Last last) {
+  const Norm n = row_pass<NTH, REST, false>(src, c, listed, sh, see, last);
   if (n.s != 0.0f) return n;
   __syncthreads();
-  return row_pass<NTH, REST, true>(row, V, c, listed, sh, [](int, float) {}, [](float) {});
+  return row_pass<NTH, REST, true>(src, c, listed, sh, [](int, float) {}, [](float) {});
 }
 
 // ---- the K largest logits of a row ---------------------------------------------------------
@@ -345,8 +386,7 @@ __device__ __forceinline__ void push(uint64_t* cand, int* count, uint32_t key, i
 template <int NTH, typename R>
 __device__ int count_from(const R& row, int V, uint32_t lo, TopShared<NTH>& t) {
   int n = 0;
-  for_row<NTH>(
-      row, V,
+  Streamed<NTH, R>{row, V}.each(
       [&](int, const float (&v)[8]) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) n += key_of(v[k]) >= lo;
@@ -439,8 +479,7 @@ __device__ void top_k(const R& row, int V, int K, const Best& b, float last, boo
     __syncthreads();
     if (tid == 0) t.count = 0;
     __syncthreads();
-    for_row<NTH>(
-        row, V,
+    Streamed<NTH, R>{row, V}.each(
         [&](int c, const float (&v)[8]) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -474,7 +513,7 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
   Best best;
   float last = -INFINITY;
   const Norm n = norm_of<NTH, false>(
-      row, V, k.c, nullptr, sh,
+      Streamed<NTH, Row<E, BIAS>>{row, V}, k.c, nullptr, sh,
       [&](int c, float vm) {
         if constexpr (TOP) best.see(vm, c);
       },
@@ -612,8 +651,7 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
       const float a = arg(x);
       return __builtin_amdgcn_exp2f(a) * __builtin_fmaf(B, fmaxf(a, -1e30f), A);
     };
-    for_row<NTH>(
-        row, V,
+    Streamed<NTH, Row<E, BIAS>>{row, V}.each(
         [&](int j, const float (&v)[8]) {
           float w[8];
 #pragma unroll
@@ -667,14 +705,13 @@ __device__ __forceinline__ double wave_max_d(double v) {
 }
 
 // Writes the row's gradient times sc; a token listed twice has both weights at its place.
-template <int NTH, typename R, typename O>
-__device__ __forceinline__ void distill_grad(const R& row, int V, int K, const Norm& n, float c,
+template <int NTH, typename S, typename O>
+__device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n, float c,
                                              float sc, float a, float b, bool twice,
                                              const int* idx, const float* q, const O& o) {
   const float asc = a * sc, bsc = b * sc;
   n.with_arg(c, [&](auto arg) {
-    for_row<NTH>(
-        row, V,
+    src.each(
         [&](int k, const float (&v)[8]) {
           float w[8];
 #pragma unroll
@@ -696,14 +733,14 @@ __device__ __forceinline__ void distill_grad(const R& row, int V, int K, const N
           w += same ? q[i] : 0.0f;
         }
       }
-      if (first) o.put(j, __builtin_amdgcn_exp2f(arg(row.at(j))) * bsc - w * sc);
+      if (first) o.put(j, __builtin_amdgcn_exp2f(arg(src.row.at(j))) * bsc - w * sc);
     }
   });
 }
 
 // GRAD 0: loss and coefficients; 1: and the row's gradient (T / count), as the fused readout
 // takes it while the logits are at hand.
-template <typename E, bool BIAS, int NTH, bool REST, bool GRAD, bool PLANES>
+template <typename E, bool BIAS, int NTH, int NV, bool REST, bool GRAD, bool PLANES>
 __global__ void __launch_bounds__(NTH) distill_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias, int K,
     int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
@@ -716,6 +753,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   const size_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const Row<E, BIAS> row{logits + r * ldl, bias};
+  const auto src = source<NTH, NV>(row, V);
   for (int i = tid; i < words; i += NTH) bits[i] = 0;
   if (tid == 0) te.twice = 0;
   __syncthreads();
@@ -770,7 +808,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
     if constexpr (REST) rest = 1.0 - total;
   }
   __syncthreads();
-  const Norm a = norm_of<NTH, REST>(row, V, sc.c, reinterpret_cast<const uint8_t*>(bits), sh,
+  const Norm a = norm_of<NTH, REST>(src, sc.c, reinterpret_cast<const uint8_t*>(bits), sh,
                                     [](int, float) {}, [](float) {});
   if (tid < 64) {
     const bool empty = a.empty();
@@ -821,7 +859,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   }
   if constexpr (GRAD) {
     __syncthreads();
-    distill_grad<NTH>(row, V, K, a, sc.c, scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
+    distill_grad<NTH>(src, K, a, sc.c, scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
                       out_row<E, PLANES>(out, r, ldo, plane));
   }
 }
@@ -830,7 +868,8 @@ template <typename E, int NTH>
 __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, int K, const int64_t* __restrict__ tokens,
     float c, const float* __restrict__ coef, const float* __restrict__ weights,
-    const float* __restrict__ scale, const float* __restrict__ grad, E* __restrict__ out) {
+    const float* __restrict__ scale, const float* __restrict__ grad, int done, E* __restrict__ out) {
+  if (done && grad[0] == 1.0f) return;  // the rows are there
   __shared__ int idx[kMaxTop];
   __shared__ float q[kMaxTop];
   const size_t r = blockIdx.x;
@@ -841,15 +880,17 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
   }
   const int flags = static_cast<int>(coef[4 * r + 3]);
   const Norm n{coef[4 * r], 1.0f, 0.0f, 0.0f, (flags & 2) != 0};
-  distill_grad<NTH>(Row<E, false>{logits + r * ldl, nullptr}, V, K, n, c, scale[0] * grad[0],
+  const Row<E, false> row{logits + r * ldl, nullptr};
+  distill_grad<NTH>(Streamed<NTH, Row<E, false>>{row, V}, K, n, c, scale[0] * grad[0],
                     coef[4 * r + 1], coef[4 * r + 2], (flags & 1) != 0, idx, q,
                     RowOut<E>{out + r * V});
 }
 
-// mean = T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = T / that count; the sums in
-// 64 bits and a fixed order, one block.
+// mean = weight T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = weight T / that count;
+// the sums in 64 bits and a fixed order, one block.
 __global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, const float* __restrict__ loss,
-                                                            float t, float* __restrict__ mean,
+                                                            float t, float weight,
+                                                            float* __restrict__ mean,
                                                             float* __restrict__ factor) {
   __shared__ double sh[2][16];
   double l = 0.0, n = 0.0;
@@ -872,8 +913,9 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, const 
       n += sh[1][w];
     }
     n = n < 1.0 ? 1.0 : n;
-    if (mean) mean[0] = static_cast<float>(static_cast<double>(t) * t * l / n);
-    if (factor) factor[0] = static_cast<float>(t / n);
+    const double wt = static_cast<double>(weight) * t;
+    if (mean) mean[0] = static_cast<float>(wt * t * l / n);
+    if (factor) factor[0] = static_cast<float>(wt / n);
   }
 }
 
@@ -1088,12 +1130,12 @@ int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype
   return DABSN_OK;
 }
 
-int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float* mean,
-                           float* factor, hipStream_t stream) {
+int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float weight,
+                           float* mean, float* factor, hipStream_t stream) {
   DABSN_REQUIRE(rows >= 0 && (rows == 0 || loss) && (mean || factor),
                 "distillation mean: bad arguments");
   hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, stream, rows, loss, temperature,
-                     mean, factor);
+                     weight, mean, factor);
   DABSN_HIP_CHECK(hipGetLastError());
   return DABSN_OK;
 }
@@ -1121,29 +1163,43 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
   const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 31) / 32);
-#define DABSN_LAUNCH(E, BIAS, N, REST, GRAD, PLANES)                                             \
-  hipLaunchKernelGGL((distill_kernel<E, BIAS, N, REST, GRAD, PLANES>), grid, dim3(N), 4 * words,  \
-                     stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype, \
+#define DABSN_LAUNCH(E, BIAS, N, NV, REST, GRAD, PLANES)                                          \
+  hipLaunchKernelGGL((distill_kernel<E, BIAS, N, NV, REST, GRAD, PLANES>), grid, dim3(N), 4 * words, \
+                     stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype,  \
                      values, tokens, ignore_index, scale_t, teacher_lse, words, loss, coef, weights, \
                      scale, out, ldo, plane, err)
-#define DABSN_REST(E, BIAS, N, GRAD, PLANES)                    \
-  if (teacher_lse) DABSN_LAUNCH(E, BIAS, N, true, GRAD, PLANES); \
-  else DABSN_LAUNCH(E, BIAS, N, false, GRAD, PLANES)
+#define DABSN_REST(E, BIAS, N, NV, GRAD, PLANES)                    \
+  if (teacher_lse) DABSN_LAUNCH(E, BIAS, N, NV, true, GRAD, PLANES); \
+  else DABSN_LAUNCH(E, BIAS, N, NV, false, GRAD, PLANES)
 #define DABSN_ROWS(N)                                                                        \
   if (dtype == kBF16) {                                                                      \
-    if (out) { DABSN_REST(bf16, false, N, true, false); }                                    \
-    else { DABSN_REST(bf16, false, N, false, false); }                                       \
+    if (out) { DABSN_REST(bf16, false, N, 0, true, false); }                                 \
+    else { DABSN_REST(bf16, false, N, 0, false, false); }                                    \
   } else if (!out) {                                                                         \
-    if (b) { DABSN_REST(float, true, N, false, false); }                                     \
-    else { DABSN_REST(float, false, N, false, false); }                                      \
+    if (b) { DABSN_REST(float, true, N, 0, false, false); }                                  \
+    else { DABSN_REST(float, false, N, 0, false, false); }                                   \
   } else if (plane) {                                                                        \
-    if (b) { DABSN_REST(float, true, N, true, true); }                                       \
-    else { DABSN_REST(float, false, N, true, true); }                                        \
+    if (b) { DABSN_REST(float, true, N, 0, true, true); }                                    \
+    else { DABSN_REST(float, false, N, 0, true, true); }                                     \
   } else {                                                                                   \
-    if (b) { DABSN_REST(float, true, N, true, false); }                                      \
-    else { DABSN_REST(float, false, N, true, false); }                                       \
+    if (b) { DABSN_REST(float, true, N, 0, true, false); }                                   \
+    else { DABSN_REST(float, false, N, 0, true, false); }                                    \
   }
-  DABSN_BY_THREADS(DABSN_ROWS);
+  // Held rows: 64 registers a thread, so that four waves share a SIMD.
+  const int64_t nv = V >> 3;
+  if (out && !plane && !b && V > 1024 && dtype == kBF16 && nv <= 256 * 16) {
+    if (nv <= 256 * 8) { DABSN_REST(bf16, false, 256, 8, true, false); }
+    else { DABSN_REST(bf16, false, 256, 16, true, false); }
+  } else if (out && !plane && !b && V > 1024 && dtype == kBF16 && nv <= 512 * 16) {
+    DABSN_REST(bf16, false, 512, 16, true, false);
+  } else if (out && !plane && !b && V > 1024 && dtype == kF32 && nv <= 512 * 8) {
+    if (nv <= 256 * 8) { DABSN_REST(float, false, 256, 8, true, false); }
+    else { DABSN_REST(float, false, 512, 8, true, false); }
+  } else if (out && !plane && !b && V > 1024 && dtype == kF32 && nv <= 1024 * 8) {
+    DABSN_REST(float, false, 1024, 8, true, false);
+  } else {
+    DABSN_BY_THREADS(DABSN_ROWS);
+  }
 #undef DABSN_ROWS
 #undef DABSN_REST
 #undef DABSN_LAUNCH
@@ -1153,7 +1209,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
 
 int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                           int64_t top, const int64_t* tokens, float temperature, const float* coef,
-                          const float* weights, const float* scale, const float* grad,
+                          const float* weights, const float* scale, const float* grad, int done,
                           void* dlogits, hipStream_t stream) {
   int rc = distill_checks("distillation backward", dtype, rows, V, ldl, top, temperature);
   if (rc != DABSN_OK) return rc;
@@ -1166,7 +1222,7 @@ int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits
 #define DABSN_LAUNCH(E, N)                                                                       \
   hipLaunchKernelGGL((distill_bwd_kernel<E, N>), grid, dim3(N), 0, stream, (int)V, ldl,           \
                      static_cast<const E*>(logits), (int)top, tokens, scale_t.c, coef, weights, scale, \
-                     grad, static_cast<E*>(dlogits))
+                     grad, done, static_cast<E*>(dlogits))
 #define DABSN_ROWS(N) \
   if (dtype == kBF16) { DABSN_LAUNCH(bf16, N); } else { DABSN_LAUNCH(float, N); }
   DABSN_BY_THREADS(DABSN_ROWS);

@@ -23,73 +23,102 @@ rows and the readout's weight and bias, whose logits [N, V] never exist at once.
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernels import ops, vocab
-from .scoring import _at
 
 _WHAT = "distillation"
 
 
+# From this many logits on, the gradient is formed with the loss while a row's logits are in
+# registers, and the backward only checks that its upstream factor is 1 (loss.backward()); another
+# factor forms it again. 8192 x 32000 bf16: 230 us forward and backward against 355 in two passes
+# (and 430 for another factor; ``loss_weight`` keeps a mixed objective's share out of it). Below, the
+# two launches that count the rows ahead cost more than the second reading: 2048 x 65 fp32.
+_FUSED_LOGITS = 1 << 24
+
+
 def _rows(x, bias, values, tokens, lse, ignore, t, s, loss, coef, weights, scale, out, ldo, plane,
-          word):
+          word, stream):
     rows, V = x.shape
     tk = ops.KernelTimer.begin("distill", x)
     _lib.check(_lib.load().dabsn_hip_distill(
         ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), ops._p(bias),
-        tokens.shape[1], ops._code(values.dtype), _at(values, s), _at(tokens, s), ignore, t,
-        _at(lse, s), _at(loss, s), _at(coef, s), _at(weights, s), ops._p(scale), out, ldo, plane,
-        word.word.data_ptr(), ops._stream(x)), _WHAT)
+        tokens.shape[1], ops._code(values.dtype), vocab.at(values, s), vocab.at(tokens, s), ignore, t,
+        vocab.at(lse, s), loss, coef, weights, scale, out, ldo, plane, word.word.data_ptr(), stream),
+        _WHAT)
     ops.KernelTimer.end(tk)
 
 
-def _mean(loss: Tensor, t: float) -> tuple[Tensor, Tensor]:
-    """(mean loss, T / counted rows) of the rows' losses."""
-    mean = torch.empty((), device=loss.device, dtype=torch.float32)
-    factor = torch.empty((), device=loss.device, dtype=torch.float32)
-    _lib.check(_lib.load().dabsn_hip_distill_mean(
-        loss.shape[0], loss.data_ptr(), t, mean.data_ptr(), factor.data_ptr(), ops._stream(loss)),
-        _WHAT)
-    return mean, factor
+def _counted(values, tokens, ignore, V, loss, t, weight, factor, stream):
+    """factor = weight T / counted rows, from the lists alone."""
+    n, lib = tokens.shape[0], _lib.load()
+    _lib.check(lib.dabsn_hip_distill_rows(n, V, tokens.shape[1], ops._code(values.dtype),
+                                          values.data_ptr(), tokens.data_ptr(), ignore, loss, stream),
+               _WHAT)
+    _lib.check(lib.dabsn_hip_distill_mean(n, loss, t, weight, None, factor, stream), _WHAT)
 
 
 class _FromLogits(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, values, tokens, lse, ignore, t):
-        n, f32 = int(x.shape[0]), torch.float32
-        need = ctx.needs_input_grad[0]
+    def forward(ctx, x, values, tokens, lse, ignore, t, weight):
+        (n, V), K, dev = x.shape, tokens.shape[1], x.device
+        need, lib = ctx.needs_input_grad[0], _lib.load()
+        fused = need and n * V >= _FUSED_LOGITS
         with vocab.on(x):
-            word = vocab.ErrorWord(x.device)
-            loss = torch.empty((n, 2), device=x.device, dtype=f32)
-            coef = torch.empty((n, 4), device=x.device, dtype=f32) if need else None
-            weights = torch.empty(tokens.shape, device=x.device, dtype=f32) if need else None
-            _rows(x, None, values, tokens, lse, ignore, t, 0, loss, coef, weights, None, None, 0, 0,
-                  word)
+            stream = vocab.stream(x)
+            word = vocab.ErrorWord(dev)
+            mean = torch.empty((), device=dev, dtype=torch.float32)
+            # The rows' losses [n, 2], coefficients [n, 4] and weights [n, K], and the factor.
+            aux = torch.empty(n * (6 + K) + 1 if need else 2 * n, device=dev, dtype=torch.float32)
+            loss = aux.data_ptr()
+            coef = weights = factor = ready = None
+            if need:
+                coef, weights, factor = loss + 8 * n, loss + 24 * n, loss + 4 * n * (6 + K)
+            if fused:
+                _counted(values, tokens, ignore, V, loss, t, weight, factor, stream)
+                ready = torch.empty((n, V), device=dev, dtype=x.dtype)
+            _rows(x, None, values, tokens, lse, ignore, t, 0, loss, coef, weights, factor,
+                  None if ready is None else ready.data_ptr(), V, 0, word, stream)
+            _lib.check(lib.dabsn_hip_distill_mean(n, loss, t, weight, mean.data_ptr(),
+                                                  None if fused else factor, stream), _WHAT)
             word.check(_WHAT)
-            mean, factor = _mean(loss, t)
-        ctx.save_for_backward(x, tokens, coef, weights, factor)
-        ctx.t = t
+        if need:
+            ctx.save_for_backward(x, tokens, aux)
+            ctx.t = t
+            ctx.ready = ready
+            ctx.captured = ready is not None and torch.cuda.is_current_stream_capturing()
         return mean
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, tokens, coef, weights, factor = ctx.saved_tensors
-        rows, V = x.shape
-        g = g.to(torch.float32)
+        x, tokens, aux = ctx.saved_tensors
+        (n, V), K = x.shape, tokens.shape[1]
+        if g.dtype != torch.float32:
+            g = g.float()
+        # The rows formed ahead serve one backward (the caller owns what it returns), of the same
+        # graph if one is being captured.
+        out, ctx.ready = ctx.ready, None
+        if out is not None and ctx.captured != torch.cuda.is_current_stream_capturing():
+            out = None
+        done = out is not None
         with vocab.on(x):
-            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+            if out is None:
+                out = torch.empty((n, V), device=x.device, dtype=x.dtype)
+            aux_p = aux.data_ptr()
             tk = ops.KernelTimer.begin("distill_bwd", x)
             _lib.check(_lib.load().dabsn_hip_distill_bwd(
-                ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), tokens.shape[1],
-                tokens.data_ptr(), ctx.t, coef.data_ptr(), weights.data_ptr(),
-                factor.data_ptr(), g.data_ptr(), out.data_ptr(), ops._stream(x)),
-                _WHAT + " backward")
+                ops._code(x.dtype), n, V, x.data_ptr(), vocab.row_stride(x), K, tokens.data_ptr(),
+                ctx.t, aux_p + 8 * n, aux_p + 24 * n, aux_p + 4 * n * (6 + K), g.data_ptr(), done,
+                out.data_ptr(), vocab.stream(x)), _WHAT + " backward")
             ops.KernelTimer.end(tk)
-        return out, None, None, None, None, None
+        return out, None, None, None, None, None, None
 
 
 class _Linear(torch.autograd.Function):
@@ -98,35 +127,36 @@ class _Linear(torch.autograd.Function):
     rounds them. Forming the logits again there would be a fourth product beside the three."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, bias, values, tokens, lse, ignore, t, chunk):
+    def forward(ctx, hidden, weight, bias, values, tokens, lse, ignore, t, share, chunk):
         n, dev = int(hidden.shape[0]), hidden.device
         need = ctx.needs_input_grad[:3]
-        lib = _lib.load()
         with vocab.on(hidden), torch.autocast("cuda", enabled=False):
+            stream = vocab.stream(hidden)
             r = vocab.Readout(hidden, weight, bias)
             word = vocab.ErrorWord(dev)
-            loss = torch.empty((n, 2), device=dev, dtype=torch.float32)
+            aux = torch.empty(2 * n + 1, device=dev, dtype=torch.float32)
+            loss, factor = aux.data_ptr(), aux.data_ptr() + 8 * n
+            mean = torch.empty((), device=dev, dtype=torch.float32)
+
+            def rows(x, s, scale, out, ldo, plane):
+                _rows(x, r.row_bias, values, tokens, lse, ignore, t, s, loss + 8 * s, None, None,
+                      scale, out, ldo, plane, word, stream)
+
             if any(need):
-                _lib.check(lib.dabsn_hip_distill_rows(
-                    n, r.V, tokens.shape[1], ops._code(values.dtype), values.data_ptr(),
-                    tokens.data_ptr(), ignore, loss.data_ptr(), ops._stream(hidden)), _WHAT)
-                _, scale = _mean(loss, t)
+                _counted(values, tokens, ignore, r.V, loss, t, share, factor, stream)
                 acc = vocab.ReadoutGrads(r, need, chunk)
                 for g0, g1 in acc.groups():
                     acc.begin(g0, g1)
                     for s in range(g0, g1, acc.chunk):
-                        x = r.logits(s, min(g1, s + acc.chunk))
-                        _rows(x, r.row_bias, values, tokens, lse, ignore, t, s, loss, None, None,
-                              scale, *acc.rows(s), word)
-                        del x
+                        rows(r.logits(s, min(g1, s + acc.chunk)), s, factor, *acc.rows(s))
                     acc.end()
                 ctx.save_for_backward(*acc.results())
             else:
                 for s in range(0, n, chunk):
-                    _rows(r.logits(s, min(n, s + chunk)), r.row_bias, values, tokens, lse, ignore, t,
-                          s, loss, None, None, None, None, 0, 0, word)
+                    rows(r.logits(s, min(n, s + chunk)), s, None, None, 0, 0)
             word.check(_WHAT)
-            mean, _ = _mean(loss, t)
+            _lib.check(_lib.load().dabsn_hip_distill_mean(n, loss, t, share, mean.data_ptr(), None,
+                                                          stream), _WHAT)
         ctx.dtype = hidden.dtype
         return mean
 
@@ -136,7 +166,14 @@ class _Linear(torch.autograd.Function):
         g = g.to(torch.float32)
         with vocab.on(g):
             grads = [vocab.scaled(x, g, ctx.dtype) for x in ctx.saved_tensors]
-        return (*grads, None, None, None, None, None, None)
+        return (*grads, None, None, None, None, None, None, None)
+
+
+def _share(weight: float) -> float:
+    weight = float(weight)
+    if not math.isfinite(weight):
+        raise ValueError(f"{_WHAT}: loss_weight must be finite, not {weight}")
+    return weight
 
 
 def _lists(shape, v: int, top_logits: Tensor, top_indices: Tensor, teacher_lse: Tensor | None):
@@ -168,11 +205,14 @@ def _lists(shape, v: int, top_logits: Tensor, top_indices: Tensor, teacher_lse: 
 
 def distillation_from_logits(logits: Tensor, top_logits: Tensor, top_indices: Tensor, *,
                              temperature: float = 1.0, teacher_lse: Tensor | None = None,
-                             ignore_index: int = -100) -> Tensor:
-    """Mean distillation loss (fp32 scalar; see the module's note) of the student's ``logits``
-    [..., V], float32 or bfloat16 of any row stride, against the teacher's ``top_logits`` and
-    ``top_indices`` [..., K], 1 <= K <= 128, and ``teacher_lse`` [...]. The gradient has the
-    logits' type, one rounding; the teacher's arrays get none. A listed token outside [0, V)
+                             ignore_index: int = -100, loss_weight: float = 1.0) -> Tensor:
+    """``loss_weight`` times the mean distillation loss (fp32 scalar; see the module's note) of the
+    student's ``logits`` [..., V], float32 or bfloat16 of any row stride, against the teacher's
+    ``top_logits`` and ``top_indices`` [..., K], 1 <= K <= 128, and ``teacher_lse`` [...]. The
+    gradient has the logits' type, one rounding; the teacher's arrays get none. For many logits it
+    is formed with the loss (and takes their memory from then on): give a share of a mixed
+    objective, or one over the micro-batches, as ``loss_weight``; an upstream factor other than 1 forms
+    it again. A listed token outside [0, V)
     other than ``ignore_index`` makes the loss NaN and sets the error word that
     ``kernels.check_errors()`` raises (``DABSN_HIP_ERROR_CHECK=sync``: raised here)."""
     vocab.need_float(_WHAT, "logits", logits)
@@ -182,13 +222,14 @@ def distillation_from_logits(logits: Tensor, top_logits: Tensor, top_indices: Te
     t = vocab.need_temperature(_WHAT, temperature)
     values, tokens, lse = _lists(logits.shape[:-1], v, top_logits, top_indices, teacher_lse)
     vocab.need_device(_WHAT, logits, values, tokens, lse)
-    return _FromLogits.apply(vocab.rows_of(logits), values, tokens, lse, int(ignore_index), t)
+    return _FromLogits.apply(vocab.rows_of(logits), values, tokens, lse, int(ignore_index), t,
+                             _share(loss_weight))
 
 
 def chunked_linear_distillation(hidden: Tensor, weight: Tensor, bias: Tensor | None,
                                 top_logits: Tensor, top_indices: Tensor, *,
                                 temperature: float = 1.0, teacher_lse: Tensor | None = None,
-                                ignore_index: int = -100,
+                                ignore_index: int = -100, loss_weight: float = 1.0,
                                 chunk_budget: int | None = None) -> Tensor:
     """``distillation_from_logits(F.linear(hidden, weight, bias), ...)`` in chunks of
     ``chunk_budget // V`` rows (``DABSN_LOSS_CHUNK_SCORES``, default 2**24 elements), the logits
@@ -201,4 +242,4 @@ def chunked_linear_distillation(hidden: Tensor, weight: Tensor, bias: Tensor | N
     values, tokens, lse = _lists(shape, int(w.shape[0]), top_logits, top_indices, teacher_lse)
     vocab.need_device(_WHAT, h, w, b, values, tokens, lse)
     chunk = vocab.chunk_rows(int(h.shape[0]), int(w.shape[0]), chunk_budget)
-    return _Linear.apply(h, w, b, values, tokens, lse, int(ignore_index), t, chunk)
+    return _Linear.apply(h, w, b, values, tokens, lse, int(ignore_index), t, _share(loss_weight), chunk)

@@ -28,7 +28,7 @@ def _lookup(ids: Tensor, w: Tensor, scale: float) -> Tensor:
         tk = ops.KernelTimer.begin("embedding", w)
         _lib.check(_lib.load().dabsn_hip_embedding_fwd(
             ops._code(w.dtype), n, V, H, ids.data_ptr(), w.data_ptr(), vocab.row_stride(w), scale,
-            out.data_ptr(), word.word.data_ptr(), ops._stream(w)), _WHAT)
+            out.data_ptr(), word.word.data_ptr(), vocab.stream(w)), _WHAT)
         ops.KernelTimer.end(tk)
         word.check(_WHAT)
     return out
@@ -55,7 +55,7 @@ class _ScaledEmbedding(torch.autograd.Function):
             tk = ops.KernelTimer.begin("embedding_bwd", g)
             _lib.check(lib.dabsn_hip_embedding_bwd(
                 ops._code(dtype), n, V, H, ids.data_ptr(), padding, g.data_ptr(), scale,
-                out.data_ptr(), ws.data_ptr(), nbytes, ops._stream(g)), _WHAT + " backward")
+                out.data_ptr(), ws.data_ptr(), nbytes, vocab.stream(g)), _WHAT + " backward")
             ops.KernelTimer.end(tk)
         return None, out, None, None
 

@@ -32,6 +32,18 @@ def on(t: Tensor):
     return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def stream(t: Tensor) -> int:
+    """The current stream's handle on the device of ``t``."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def at(t: Tensor | None, s: int) -> int | None:
+    """Pointer to row s of a contiguous tensor."""
+    if t is None:
+        return None
+    return t.data_ptr() + s * t.stride(0) * t.element_size() if s else t.data_ptr()
+
+
 def need_device(what: str, *tensors: Tensor | None) -> None:
     """All tensors on one ROCm device."""
     first = None
@@ -241,7 +253,7 @@ class ReadoutGrads:
                                dtype=f32)
             _lib.check(lib.dabsn_hip_column_sums(2 * m, r.V, self.ldo, self.buf.data_ptr(), 1,
                                                  part.data_ptr(), self.bias.data_ptr(),
-                                                 ops._stream(d)), "readout bias gradient")
+                                                 stream(d)), "readout bias gradient")
         self.first = False
 
     def results(self):
@@ -258,5 +270,5 @@ def scaled(x: Tensor | None, g: Tensor, like: torch.dtype) -> Tensor | None:
         return None
     out = torch.empty(x.shape, device=x.device, dtype=like)
     _lib.check(_lib.load().dabsn_hip_scaled(ops._code(like), x.numel(), x.data_ptr(), g.data_ptr(),
-                                            out.data_ptr(), ops._stream(x)), "scaled gradient")
+                                            out.data_ptr(), stream(x)), "scaled gradient")
     return out

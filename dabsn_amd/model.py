@@ -336,10 +336,11 @@ class DABSNSequenceLM(nn.Module):
 
     def distillation_loss(self, ids: Tensor, top_logits: Tensor, top_indices: Tensor, *,
                           temperature: float = 1.0, teacher_lse: Tensor | None = None,
-                          ignore_index: int = -100, chunk_budget: int | None = None) -> Tensor:
+                          ignore_index: int = -100, loss_weight: float = 1.0,
+                          chunk_budget: int | None = None) -> Tensor:
         """Distillation loss of this model's next-token distributions on ``ids`` [B, T] against a
         teacher's top logits and tokens [B, T, K] (see ``chunked_linear_distillation``)."""
         return chunked_linear_distillation(
             self.forward_hidden(ids), self.readout.weight, self.readout.bias, top_logits,
             top_indices, temperature=temperature, teacher_lse=teacher_lse,
-            ignore_index=ignore_index, chunk_budget=chunk_budget)
+            ignore_index=ignore_index, loss_weight=loss_weight, chunk_budget=chunk_budget)

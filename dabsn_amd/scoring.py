@@ -53,18 +53,14 @@ def _outputs(rows: int, top: int, device, targets: bool, stats: bool):
     return lp, ent, st, tl, ti
 
 
-def _at(t: Optional[Tensor], s: int) -> Optional[int]:
-    return None if t is None else t.data_ptr() + s * t.stride(0) * t.element_size()
-
-
 def _forward(x, bias, targets, ignore, temperature, top, outs, s, word, stream):
     lp, ent, st, tl, ti = outs
     rows, V = x.shape
     tk = ops.KernelTimer.begin("token_logprobs", x)
     _lib.check(_lib.load().dabsn_hip_token_logprobs(
         ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), ops._p(bias),
-        _at(targets, s), ignore, temperature, top, _at(lp, s), _at(ent, s), _at(st, s), _at(tl, s),
-        _at(ti, s), word.word.data_ptr(), stream), _WHAT)
+        vocab.at(targets, s), ignore, temperature, top, vocab.at(lp, s), vocab.at(ent, s), vocab.at(st, s), vocab.at(tl, s),
+        vocab.at(ti, s), word.word.data_ptr(), stream), _WHAT)
     ops.KernelTimer.end(tk)
 
 
@@ -75,15 +71,15 @@ def _backward(x, bias, targets, ignore, temperature, top, saved, grads, s, out, 
     tk = ops.KernelTimer.begin("token_logprobs_bwd", x)
     _lib.check(_lib.load().dabsn_hip_token_logprobs_bwd(
         ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), ops._p(bias),
-        _at(targets, s), ignore, temperature, top, _at(ti, s), _at(st, s), _at(ent, s), _at(gl, s),
-        _at(ge, s), _at(gt, s), out, ldo, plane, ops._stream(x)), _WHAT + " backward")
+        vocab.at(targets, s), ignore, temperature, top, vocab.at(ti, s), vocab.at(st, s), vocab.at(ent, s), vocab.at(gl, s),
+        vocab.at(ge, s), vocab.at(gt, s), out, ldo, plane, vocab.stream(x)), _WHAT + " backward")
     ops.KernelTimer.end(tk)
 
 
 def _from_logits(x, targets, ignore, temperature, top, stats):
     word = vocab.ErrorWord(x.device)
     outs = _outputs(x.shape[0], top, x.device, targets is not None, stats)
-    _forward(x, None, targets, ignore, temperature, top, outs, 0, word, ops._stream(x))
+    _forward(x, None, targets, ignore, temperature, top, outs, 0, word, vocab.stream(x))
     word.check(_WHAT)
     return outs
 
@@ -120,7 +116,7 @@ class _LinearTokenLogprobs(torch.autograd.Function):
             r = vocab.Readout(hidden, weight, bias)
             word = vocab.ErrorWord(hidden.device)
             outs = _outputs(n, top, hidden.device, targets is not None, stats)
-            stream = ops._stream(hidden)
+            stream = vocab.stream(hidden)
             for s in range(0, n, chunk):
                 _forward(r.logits(s, min(n, s + chunk)), r.row_bias, targets, ignore, temperature,
                          top, outs, s, word, stream)

@@ -702,12 +702,13 @@ int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t str
  * log-sum-exp of the teacher's whole row / temperature; V <= 480000), exp(values / temperature -
  * teacher_lse) with the rest q_r = 1 - sum q on all other tokens as one event. loss [rows][2] =
  * (KL(q || softmax(z)), 1 if the row has a listed token, else 0). coef [rows][4] and weights
- * [rows][top] (NULL: none) are for _bwd. With out (fp32 logits) the gradient rows are written
- * too, times scale[0], as above. A listed token outside [0, V) sets *err to 1 and its row to NaN.
+ * [rows][top] (NULL: none) are for _bwd. With out the gradient rows are written too,
+ * times scale[0], in the logits' type or (fp32 logits) as two planes as above. A listed token outside [0, V) sets *err to 1 and its row to NaN.
  * dabsn_hip_distill_rows: loss = (0, 1 or 0) without logits. dabsn_hip_distill_mean: mean[0] =
- * temperature^2 * mean loss over the counted rows, factor[0] = temperature / their number (each
- * may be NULL). dabsn_hip_distill_bwd: dlogits [rows, V] = d mean[0] / d logits * grad[0], given
- * scale = factor. A token listed several times has the sum of its weights.
+ * weight * temperature^2 * mean loss over the counted rows, factor[0] = weight * temperature / their
+ * number (each may be NULL). dabsn_hip_distill_bwd: dlogits [rows, V] = d mean[0] / d logits * grad[0], given
+ * scale = factor; with `done` dlogits holds the rows for grad[0] = 1 already and the call writes
+ * only for another factor. A token listed several times has the sum of its weights.
  *
  * dabsn_hip_column_sums: out [V] (added to with `add`) = column sums of bf16 rows x (stride ld,
  * a multiple of 8), through partials [dabsn_hip_column_sums_partials]. dabsn_hip_scaled: out[i] =
@@ -727,8 +728,8 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
 int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype,
                            const void* values, const int64_t* tokens, int64_t ignore_index,
                            float* loss, hipStream_t stream);
-int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float* mean,
-                           float* factor, hipStream_t stream);
+int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float weight,
+                           float* mean, float* factor, hipStream_t stream);
 int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                       const void* bias, int64_t top, int value_dtype, const void* values,
                       const int64_t* tokens, int64_t ignore_index, float temperature,
@@ -737,7 +738,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                       hipStream_t stream);
 int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                           int64_t top, const int64_t* tokens, float temperature, const float* coef,
-                          const float* weights, const float* scale, const float* grad,
+                          const float* weights, const float* scale, const float* grad, int done,
                           void* dlogits, hipStream_t stream);
 size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V);
 int dabsn_hip_column_sums(int64_t rows, int64_t V, int64_t ld, const void* x, int add,

@@ -72,9 +72,9 @@ def test_library_refuses_bad_arguments_before_it_launches():
                dict(out=one, ldo=8, plane=15), dict(out=one, ldo=8, scale=None),
                dict(dtype=1, out=one, ldo=8, plane=16)):
         assert f(**kw) == -2, kw
-    assert lib.dabsn_hip_distill_bwd(0, 2, 5, one, 5, 0, one, 1.0, one, one, one, one, one, None) == -2
+    assert lib.dabsn_hip_distill_bwd(0, 2, 5, one, 5, 0, one, 1.0, one, one, one, one, 0, one, None) == -2
     assert lib.dabsn_hip_distill_rows(2, 5, 0, 0, one, one, -100, one, None) == -2
-    assert lib.dabsn_hip_distill_mean(2, None, 1.0, one, one, None) == -2
+    assert lib.dabsn_hip_distill_mean(2, None, 1.0, 1.0, one, one, None) == -2
 
 
 # ---- the definition in 64 bits ---------------------------------------------------------------
@@ -275,6 +275,86 @@ def test_upstream_factor_scales_the_gradient(cuda_device):
     (g4,) = torch.autograd.grad(loss * 4, leaf, retain_graph=True)
     (g8,) = torch.autograd.grad(loss / 8, leaf)
     assert torch.equal(g1, g2) and torch.equal(g1 * 4, g4) and torch.equal(g1 / 8, g8)
+
+
+FUSED = [(17000, 1001, 5), (8300, 2050, 16), (1030, 16385, 64), (520, 32777, 40), (400, 65000, 20),
+         (150, 131080, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,K", FUSED)
+def test_gradients_formed_with_the_loss(cuda_device, n, V, K, dtype):
+    """Many logits: rows of every way to hold them. The gradient equals the one that a factor of 2
+    forms again, halved (exact), bit for bit, its first rows the definition's, and a second
+    backward gives it again though the first one's result was changed."""
+    assert n * V >= 1 << 24
+    x = (torch.randn(n, V, generator=torch.Generator(device="cuda").manual_seed(V), device="cuda")
+         * 2.5).to(dtype)
+    values, tokens = (x.float() + torch.randn(n, V, device="cuda")).topk(K, dim=1)
+    tokens[8:] = torch.where(torch.arange(n - 8, device="cuda")[:, None] % 7 == 0, -100, tokens[8:])
+    tokens[0, 0] = tokens[0, -1]
+    x[1, tokens[1, 0]] = 30.0
+    lse = torch.logsumexp(x.float(), 1) + 1
+    leaf = x.requires_grad_(True)
+    for rest in (None, lse):
+        loss = distillation_from_logits(leaf, values, tokens, temperature=1.0, teacher_lse=rest)
+        (g2,) = torch.autograd.grad(loss * 2, leaf, retain_graph=True)
+        (g1,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+        assert torch.equal(g2 / 2, g1)
+        loss = distillation_from_logits(leaf, values, tokens, temperature=1.0, teacher_lse=rest)
+        (ga,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+        assert torch.equal(ga, g1)
+        ga.zero_()
+        (gb,) = torch.autograd.grad(loss, leaf)
+        assert torch.equal(gb, g1)
+        with torch.no_grad():
+            assert torch.equal(distillation_from_logits(leaf, values, tokens, teacher_lse=rest), loss)
+        part = None if rest is None else rest[:8]
+        _, grad, _, tol = reference(x[:8], values[:8], tokens[:8], 1.0, part)
+        counted = int((tokens != -100).any(1).sum())
+        small = int((tokens[:8] != -100).any(1).sum())
+        rnd = U if dtype == torch.float32 else 2.0 ** -8
+        want, tol = grad * small / counted, tol * small / counted
+        err = (g1[:8].double().cpu() - want).abs()
+        assert bool((err <= tol + (rnd + 2 * U) * (want.abs() + tol) + 2.0 ** -126).all())
+
+
+@pytest.mark.gpu
+def test_gradients_formed_with_the_loss_in_a_graph(cuda_device):
+    """Loss and backward captured together replay with new inputs."""
+    from test_capture import _capture, _replays
+
+    token_logprobs(torch.zeros(1, 4, device=cuda_device))
+    cases = [case(s, 8300, 2050, 16, torch.bfloat16, True) for s in (1, 2, 3)]
+    static = [v.clone() for v in cases[0]]
+
+    def go(v):
+        leaf = v[0].detach().requires_grad_(True)
+        loss = distillation_from_logits(leaf, v[1], v[2], teacher_lse=v[3])
+        return [loss.detach(), *torch.autograd.grad(loss, leaf)]
+
+    graph, outs = _capture(lambda: go(static))
+    _replays(graph, outs, static, cases[1:] + cases[:1], go)
+
+
+@pytest.mark.gpu
+def test_loss_weight(cuda_device):
+    """A weight of 1/4 is exact in the loss and the gradients of both forms."""
+    x, values, tokens, lse = case(5, 6, 1300, 16, torch.bfloat16, True)
+    for big in (False, True):
+        rep = 2200 if big else 1
+        xs, vs, ts = x.repeat(rep, 1).requires_grad_(True), values.repeat(rep, 1), tokens.repeat(rep, 1)
+        a = distillation_from_logits(xs, vs, ts)
+        b = distillation_from_logits(xs, vs, ts, loss_weight=0.25)
+        assert torch.equal(a / 4, b)
+        assert torch.equal(torch.autograd.grad(a, xs)[0] / 4, torch.autograd.grad(b, xs)[0])
+    h, w, b, values, tokens, lse = linear_case(1, 96, 64, 1000, 16, torch.bfloat16)
+    h.requires_grad_(True)
+    one = chunked_linear_distillation(h, w, b, values, tokens, teacher_lse=lse)
+    part = chunked_linear_distillation(h, w, b, values, tokens, teacher_lse=lse, loss_weight=0.25)
+    assert torch.equal(one / 4, part)
+    assert torch.equal(torch.autograd.grad(one, h)[0] / 4, torch.autograd.grad(part, h)[0])
 
 
 @pytest.mark.gpu
