@@ -4,8 +4,8 @@
 // Backward: dweight[v] = scale * (the sum of the rows grad[i] with id_i = v, in token order),
 // fp32 sums, one rounding; a row of zeros where no token is v. The order is fixed, so the same
 // inputs give the same bits: no float atomics. The tokens are sorted by word (stable, so each
-// word's tokens stay in order), the sorted list is cut into pieces of equal length whatever the
-// words' frequencies, a wave sums a piece's rows word by word, and words that cross pieces are
+// word's tokens stay in order), the sorted list is cut into pieces of about equal length whatever the
+// words' frequencies, a wave sums a piece's rows word by word, and the words of many pieces are
 // joined from partial sums, piece after piece.
 #include <algorithm>
 
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256) place_kernel(int64_t n, int64_t V, int64_
   const int bins = 1 << bits, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   for (int b = tid; b < bins; b += 256) {
     uint32_t before = 0, all = 0;
-#pragma unroll 8
+#pragma unroll 32
     for (int t = 0; t < tiles; ++t) {
       const uint32_t x = counts[static_cast<size_t>(t) * bins + b];
       before += t < static_cast<int>(blockIdx.x) ? x : 0;
@@ -258,12 +258,69 @@ __global__ void __launch_bounds__(256) starts_kernel(uint32_t n, uint32_t V,
 }
 
 // ---- sums ----------------------------------------------------------------------------------
-// A wave sums the rows of the sorted tokens [piece * P, + P) over 64 * 8 columns. A word that
-// begins and ends in the piece is written; one that began in an earlier piece leaves its partial
-// sum in slot 2 piece, one that only begins here in slot 2 piece + 1.
+// The sum of the rows `at(i)`, i = i0 .. i1 - 1 in order, over this lane's 8 columns; U rows' loads
+// in flight.
+template <int U, typename E, typename At>
+__device__ __forceinline__ void add_rows(const E* grad, int H, int c, int i0, int i1, At at,
+                                         float (&sum)[8]) {
+  for (int i = i0; i < i1; i += U) {
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c < H) get8(grad + static_cast<size_t>(at(min(i + u, i1 - 1))) * H, c, H, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u < i1) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += v[u][k];
+      }
+    }
+  }
+}
+
+// Few tokens and words: a wave takes a word and 512 columns, finds the word's tokens among all
+// and sums their rows, zeros included: one launch instead of four.
+constexpr int kDirectTokens = 512;
+constexpr int64_t kDirectWork = 1 << 23;  // tokens * words
 template <typename E>
-__global__ void __launch_bounds__(256) pieces_kernel(int H, int P, int strips, int64_t tasks,
-                                                     uint32_t V, const uint32_t* __restrict__ starts,
+__global__ void __launch_bounds__(256) direct_kernel(int n, int64_t V, int64_t padding, int H,
+                                                     int strips, int64_t tasks,
+                                                     const int64_t* __restrict__ ids,
+                                                     const E* __restrict__ grad, float scale,
+                                                     E* __restrict__ dweight) {
+  __shared__ uint16_t lists[4][kDirectTokens];
+  const int64_t task = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  uint16_t* list = lists[threadIdx.x >> 6];
+  const int64_t word = task / strips;  // no word at all behind the last task
+  const int c = (static_cast<int>(task - word * strips) * 64 + lane) * 8;
+  int count = 0;
+  for (int i = 0; i < n; i += 64) {
+    const bool mine = i + lane < n && ids[i + lane] == word && word != padding && word < V;
+    const uint64_t mask = __ballot(mine);
+    if (mine) list[count + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(i + lane);
+    count += __popcll(mask);
+  }
+  __syncthreads();
+  if (task >= tasks || c >= H) return;
+  float sum[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
+  add_rows<8>(grad, H, c, 0, count, [&](int i) { return list[i]; }, sum);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[k] *= scale;
+  put8(dweight + word * H, c, H, sum);
+}
+
+// The sorted tokens in pieces of kPiece. A word of at most kPiece tokens belongs to the piece in
+// which it begins (so a piece sums fewer than 2 kPiece tokens, and short words, whose sums would
+// cost as much to pass on as their rows, cross no piece). A longer word is cut where pieces end:
+// it leaves the partial sum of its first piece in slot 2 piece + 1 and those of the next ones in
+// slot 2 piece. A wave sums a piece over 512 columns.
+constexpr int kPiece = 32;
+template <typename E>
+__global__ void __launch_bounds__(256) pieces_kernel(int H, int strips, int64_t tasks, uint32_t V,
+                                                     const uint32_t* __restrict__ starts,
                                                      const uint32_t* __restrict__ keys,
                                                      const uint32_t* __restrict__ pos,
                                                      const E* __restrict__ grad, float scale,
@@ -275,86 +332,125 @@ __global__ void __launch_bounds__(256) pieces_kernel(int H, int P, int strips, i
   const uint32_t piece = static_cast<uint32_t>(task / strips);
   const int c = (static_cast<int>(task - static_cast<int64_t>(piece) * strips) * 64 + lane) * 8;
   const uint32_t n = starts[V];  // tokens that give a gradient
-  const uint32_t lo = piece * P, hi = min(n, lo + P);
+  const uint32_t lo = piece * kPiece, hi = min(n, lo + kPiece);
   if (lo >= n) return;
-  const int count = static_cast<int>(hi - lo);
-  const uint32_t key = keys[min(lo + lane, n - 1)], row = pos[min(lo + lane, n - 1)];
-  const uint32_t before = lo > 0 ? keys[lo - 1] : 0xffffffffu;
-  const uint32_t after = hi < n ? keys[hi] : 0xffffffffu;
-  const bool live = c < H;
+  // A lane a token, the first ones of the next piece too: its word and where that begins and ends.
+  const uint32_t at = lo + lane;
+  const uint32_t key = keys[min(at, n - 1)], row = pos[min(at, n - 1)];
+  const uint32_t from = starts[key], to = starts[key + 1];
+  const bool cut = to - from > kPiece;
+  const uint64_t ends = __ballot(at < n && to == at + 1), cuts = __ballot(cut);
+  const uint64_t begun = __ballot(from >= lo);
+  const int tail = static_cast<int>(hi - lo) - 1;
+  const uint32_t first_to = __builtin_amdgcn_readlane(to, 0);
+  const uint32_t last_to = __builtin_amdgcn_readlane(to, tail);
+  // From behind a short word of the piece before, to the end of the last short word.
+  int i = (begun & 1) || (cuts & 1) ? 0 : static_cast<int>(first_to - lo);
+  const int end = (cuts >> tail & 1) ? tail + 1 : static_cast<int>(last_to - lo);
   float sum[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
-  bool began = __builtin_amdgcn_readlane(key, 0) != before;
-  constexpr int U = 8;
-  for (int i0 = 0; i0 < count; i0 += U) {
+  constexpr int U = 8;  // rows' loads in flight, whatever words they belong to
+  for (; i < end; i += U) {
     float v[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t r = __builtin_amdgcn_readlane(row, min(i0 + u, count - 1));
-      if (live) get8(grad + static_cast<size_t>(r) * H, c, H, v[u]);
+      const size_t r = __builtin_amdgcn_readlane(row, min(i + u, end - 1));
+      if (c < H) get8(grad + r * H, c, H, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u;
-      if (i >= count) break;
+      const int j = i + u;
+      if (j >= end) break;
 #pragma unroll
       for (int k = 0; k < 8; ++k) sum[k] += v[u][k];
-      const uint32_t now = __builtin_amdgcn_readlane(key, i);
-      const bool last = i + 1 == count;
-      const uint32_t next = last ? after : __builtin_amdgcn_readlane(key, min(i + 1, 63));
-      if (last || next != now) {
-        if (live) {
-          if (began && next != now) {
+      if ((ends >> j & 1) || j + 1 == end) {
+        const uint32_t word = __builtin_amdgcn_readlane(key, j);
+        if (c < H) {
+          if (cuts >> j & 1) {
+            const size_t slot = 2 * static_cast<size_t>(piece) + (begun >> j & 1);
+            put8(partial + slot * H, c, H, sum);
+          } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) sum[k] *= scale;
-            put8(dweight + static_cast<size_t>(now) * H, c, H, sum);
-          } else {
-            put8(partial + (2 * static_cast<size_t>(piece) + (began ? 1 : 0)) * H, c, H, sum);
+            put8(dweight + static_cast<size_t>(word) * H, c, H, sum);
           }
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
-        began = true;
       }
     }
   }
 }
 
-// A block per word: zeros where it has no token, the joined partial sums where it crosses
-// pieces; the others are written.
+// The first `blanks` blocks write the zeros of words without tokens, 64 / lanes words a wave; then
+// a block a piece and 512 columns joins the partial sums of the cut word that begins in the piece,
+// if one does (a cut word is longer than a piece, so one at most): its waves take ranges of the
+// pieces, added in order.
 template <typename E>
-__global__ void __launch_bounds__(256) words_kernel(int H, int P, const uint32_t* __restrict__ starts,
+__global__ void __launch_bounds__(256) words_kernel(int H, int lanes_log2, int strips, int64_t V,
+                                                    int64_t blanks, const uint32_t* __restrict__ starts,
+                                                    const uint32_t* __restrict__ keys,
                                                     const float* __restrict__ partial, float scale,
                                                     E* __restrict__ dweight) {
-  const size_t v = blockIdx.x;
-  const uint32_t a = starts[v], b = starts[v + 1];
-  E* o = dweight + v * H;
-  const uint32_t p0 = a / P, p1 = b > a ? (b - 1) / P : p0;
-  if (b > a && p0 == p1) return;
-  for (int c = threadIdx.x * 8; c < H; c += 256 * 8) {
-    float sum[8];
+  __shared__ float part[4][512];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (blockIdx.x < blanks) {
+    const int lanes = 1 << lanes_log2;
+    const int64_t v = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> lanes_log2;
+    if (v >= V || starts[v] != starts[v + 1]) return;
+    float zero[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
-    if (b > a) {
-      get8(partial + (2 * static_cast<size_t>(p0) + 1) * H, c, H, sum);
-#pragma unroll 4
-      for (uint32_t p = p0 + 1; p <= p1; ++p) {
-        float w[8];
-        get8(partial + 2 * static_cast<size_t>(p) * H, c, H, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] += w[k];
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] *= scale;
-    }
-    put8(o, c, H, sum);
+    for (int k = 0; k < 8; ++k) zero[k] = 0.0f;
+    for (int c = (threadIdx.x & (lanes - 1)) * 8; c < H; c += lanes * 8) put8(dweight + v * H, c, H, zero);
+    return;
   }
+  const int64_t task = blockIdx.x - blanks;
+  const uint32_t n = starts[V], piece = static_cast<uint32_t>(task / strips);
+  const uint32_t lo = piece * kPiece;
+  if (n <= kPiece || lo >= n - kPiece) return;  // no piece behind this one
+  const uint32_t word = keys[lo + kPiece - 1], a = starts[word], b = starts[word + 1];
+  if (a < lo || b - a <= kPiece) return;
+  const uint32_t pieces = (b - 1) / kPiece - piece;  // behind the first
+  const uint32_t per = (pieces + 3) / 4, p1 = min(pieces, (wave + 1) * per);
+  const int c = (static_cast<int>(task - static_cast<int64_t>(piece) * strips) * 64 + lane) * 8;
+  float sum[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
+  if (c < H) {
+    if (wave == 0) get8(partial + (2 * static_cast<size_t>(piece) + 1) * H, c, H, sum);
+#pragma unroll 8
+    for (uint32_t p = wave * per; p < p1; ++p) {
+      float w[8];
+      get8(partial + 2 * static_cast<size_t>(piece + 1 + p) * H, c, H, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += w[k];
+    }
+    store8(&part[wave][lane * 8], sum);
+  }
+  __syncthreads();
+  if (wave != 0 || c >= H) return;
+#pragma unroll
+  for (int g = 1; g < 4; ++g) {
+    float w[8];
+    load8(&part[g][lane * 8], w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] += w[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[k] *= scale;
+  put8(dweight + static_cast<size_t>(word) * H, c, H, sum);
 }
 
-constexpr int kPiece = 32;
+// Lanes a row where a wave may share rows: 8 columns each, a power of two, at most the wave.
+static int lanes_log2(int64_t H) {
+  int l = 0;
+  while (l < 6 && (8ll << l) < H) ++l;
+  return l;
+}
 
 struct Plan {
+  bool direct;
   int bits, passes, tile, tiles;
   int64_t pieces;
   size_t keys, pos, keys2, pos2, counts, starts, partial, bytes;
@@ -362,6 +458,8 @@ struct Plan {
 static size_t up(size_t b) { return (b + 255) / 256 * 256; }
 static Plan plan_of(int64_t n, int64_t V, int64_t H) {
   Plan p{};
+  p.direct = n <= kDirectTokens && n * V <= kDirectWork;
+  if (p.direct) return p;
   int need = 1;
   while ((1ll << need) <= V) ++need;  // keys 0 .. V
   const bool rank = n <= kRankTokens;
@@ -396,12 +494,20 @@ static int checks(const char* what, int dtype, int64_t n, int64_t V, int64_t H) 
 template <typename E>
 static void launch_bwd(const Plan& p, int64_t n, int64_t V, int H, const int64_t* ids, int64_t padding,
                        const E* grad, float scale, E* dweight, char* ws, hipStream_t stream) {
+  const int strips = (H + 511) / 512;
+  if (p.direct) {
+    const int64_t tasks = V * strips;
+    hipLaunchKernelGGL((direct_kernel<E>), dim3(static_cast<unsigned>((tasks + 3) / 4)), dim3(256), 0,
+                       stream, static_cast<int>(n), V, padding, H, strips, tasks, ids, grad, scale,
+                       dweight);
+    return;
+  }
   auto* keys = reinterpret_cast<uint32_t*>(ws + p.keys);
   auto* pos = reinterpret_cast<uint32_t*>(ws + p.pos);
   auto* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
   auto* starts = reinterpret_cast<uint32_t*>(ws + p.starts);
   auto* partial = reinterpret_cast<float*>(ws + p.partial);
-  if (p.passes == 0 && n > 0) {
+  if (p.passes == 0) {
     hipLaunchKernelGGL(rank_kernel, dim3(static_cast<unsigned>((n + 63) / 64)), dim3(256), 0, stream,
                        static_cast<int>(n), V, padding, ids, keys, pos);
   }
@@ -431,14 +537,14 @@ static void launch_bwd(const Plan& p, int64_t n, int64_t V, int H, const int64_t
   }
   hipLaunchKernelGGL(starts_kernel, dim3(static_cast<unsigned>(V / 256 + 1)), dim3(256), 0, stream,
                      static_cast<uint32_t>(n), static_cast<uint32_t>(V), keys, starts);
-  const int strips = (H + 511) / 512;
   const int64_t tasks = p.pieces * strips;
-  if (tasks > 0)
-    hipLaunchKernelGGL((pieces_kernel<E>), dim3(static_cast<unsigned>((tasks + 3) / 4)), dim3(256), 0,
-                       stream, H, kPiece, strips, tasks, static_cast<uint32_t>(V), starts, keys, pos,
-                       grad, scale, dweight, partial);
-  hipLaunchKernelGGL((words_kernel<E>), dim3(static_cast<unsigned>(V)), dim3(256), 0, stream, H,
-                     kPiece, starts, partial, scale, dweight);
+  hipLaunchKernelGGL((pieces_kernel<E>), dim3(static_cast<unsigned>((tasks + 3) / 4)), dim3(256), 0,
+                     stream, H, strips, tasks, static_cast<uint32_t>(V), starts, keys, pos, grad,
+                     scale, dweight, partial);
+  const int log2 = lanes_log2(H);
+  const int64_t blanks = ((V << log2) + 255) / 256;
+  hipLaunchKernelGGL((words_kernel<E>), dim3(static_cast<unsigned>(blanks + tasks)), dim3(256), 0,
+                     stream, H, log2, strips, V, blanks, starts, keys, partial, scale, dweight);
 }
 
 }  // namespace embed
@@ -457,8 +563,7 @@ int dabsn_hip_embedding_fwd(int dtype, int64_t n, int64_t V, int64_t H, const in
   DABSN_REQUIRE(ldw >= H, "embedding: row stride %lld of %lld values", (long long)ldw, (long long)H);
   if (n == 0) return DABSN_OK;
   DABSN_REQUIRE(ids && weight && out && err, "embedding: null pointer");
-  int log2 = 0;
-  while (log2 < 6 && (8ll << log2) < H) ++log2;
+  const int log2 = lanes_log2(H);
   const int64_t blocks = ((n << log2) + 255) / 256;
   DABSN_REQUIRE(blocks < (1ll << 31), "embedding: %lld tokens in one call", (long long)n);
   const dim3 grid(static_cast<unsigned>(blocks));
@@ -483,11 +588,13 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
   int rc = checks("embedding backward", dtype, n, V, H);
   if (rc != DABSN_OK) return rc;
   const Plan p = plan_of(n, V, H);
-  DABSN_REQUIRE(((ids && grad) || n == 0) && dweight && workspace,
+  DABSN_REQUIRE(((ids && grad) || n == 0) && dweight && (workspace || p.bytes == 0),
                 "embedding backward: null pointer");
   DABSN_REQUIRE(workspace_bytes >= p.bytes, "embedding backward: workspace of %zu bytes, %zu needed",
                 workspace_bytes, p.bytes);
-  DABSN_REQUIRE(p.pieces * ((H + 511) / 512) < (1ll << 32),
+  const int64_t strips = (H + 511) / 512;
+  DABSN_REQUIRE(p.pieces * strips + ((V << lanes_log2(H)) + 255) / 256 < (1ll << 31) &&
+                    (!p.direct || V * strips < (1ll << 32)),
                 "embedding backward: %lld x %lld values in one call", (long long)n, (long long)H);
   if (dtype == kBF16)
     launch_bwd<bf16>(p, n, V, (int)H, ids, padding_idx, static_cast<const bf16*>(grad), scale,

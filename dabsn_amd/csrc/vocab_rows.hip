@@ -28,59 +28,87 @@ namespace vocab {
 constexpr double kLn2 = 0.693147180559945309417;
 constexpr float kLowest = -3.40282346638528860e38f;
 constexpr int kMaxTop = 128;
-// Candidates of the top selection that fit: all of a vocabulary whose vectors of 8 are fewer
-// than kMaxTop (there the threshold may be below every logit), and some room for equal logits.
+// Candidates of the top selection that fit: all of a vocabulary whose vectors are fewer than
+// kMaxTop (there the threshold may be below every logit), and some room for equal logits.
 constexpr int kCap = 1152;
 constexpr uint32_t kErrToken = 1u;
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-// A row's logits, 8 at a time from any element alignment (global memory takes 16-byte accesses
-// at 2-byte addresses; rows of an odd vocabulary start at such), plus the readout's bias.
-template <typename E, bool BIAS>
+// bf16 bits, two to a word, as floats.
+template <int N>
+__device__ __forceinline__ void halves(const uint32_t (&u)[N / 2], float (&v)[N]) {
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) {
+    v[2 * k] = __builtin_bit_cast(float, u[k] << 16);
+    v[2 * k + 1] = __builtin_bit_cast(float, u[k] & 0xffff0000u);
+  }
+}
+
+// A row's logits, W = 8 bf16 or 4 fp32 (16 bytes) at a time, plus the readout's bias. A row of an
+// odd vocabulary starts anywhere in a line of 128 bytes: its vectors begin at the first whole line,
+// column `head`, and the logits before it and behind the last vector are taken one by one.
+// ONCE: the loads are marked as not to be kept in the caches. 8192 x 32000 bf16 are read in 83 us
+// instead of 128 (6.3 TB/s), as the lines that a pass would leave there, and those it would push
+// out to memory, are of no use. Whole lines at a time are needed for this: fp32 lanes that took two
+// neighbouring vectors (each line fetched twice) or vectors across lines lost a third instead,
+// 173 -> 205 and 231 us at 4099 x 50021.
+template <typename E, bool BIAS, bool ONCE>
 struct Row {
+  static constexpr int W = is_bf16<E>::value ? 8 : 4;
   const E* x;
   const bf16* b;
+  int V, head;
+  __device__ __forceinline__ Row(const E* x_, const bf16* b_, int V_) : x(x_), b(b_), V(V_) {
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) & 127) / sizeof(E);
+    head = min(V, static_cast<int>((128 / sizeof(E) - off) & (128 / sizeof(E) - 1)));
+  }
+  __device__ __forceinline__ int vectors() const { return (V - head) / W; }
+  __device__ __forceinline__ int64_t column(int c) const {
+    return head + static_cast<int64_t>(c) * W;
+  }
+  // f(column, value) for this thread's logit before the vectors and the one behind them.
+  template <typename F>
+  __device__ __forceinline__ void singles(F f) const {
+    const int t = threadIdx.x, j = head + vectors() * W + t;
+    if (t < head) f(t, at(t));
+    if (j < V) f(j, at(j));
+  }
   struct Raw {
-    u32x4 v[is_bf16<E>::value ? 1 : 2];
-    u32x4 bias;
+    u32x4 v;
+    uint32_t bias[W / 2];
   };
   __device__ __forceinline__ Raw load(int c) const {
     Raw r;
-    const E* p = x + static_cast<size_t>(c) * 8;
-    r.v[0] = *reinterpret_cast<const u32x4_any*>(p);
-    if constexpr (!is_bf16<E>::value) r.v[1] = *reinterpret_cast<const u32x4_any*>(p + 4);
-    if constexpr (BIAS) r.bias = *reinterpret_cast<const u32x4_any*>(b + static_cast<size_t>(c) * 8);
+    const u32x4* p = reinterpret_cast<const u32x4*>(x + column(c));
+    if constexpr (ONCE) r.v = __builtin_nontemporal_load(p);
+    else r.v = *p;
+    if constexpr (BIAS) __builtin_memcpy(r.bias, b + column(c), 2 * W);
     return r;
   }
-  static __device__ __forceinline__ void halves(const u32x4& u, float (&v)[8]) {
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[W]) {
+    uint32_t u[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[2 * k] = __builtin_bit_cast(float, u[k] << 16);
-      v[2 * k + 1] = __builtin_bit_cast(float, u[k] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[8]) {
+    for (int k = 0; k < 4; ++k) u[k] = r.v[k];
     if constexpr (is_bf16<E>::value) {
-      halves(r.v[0], v);
+      halves<W>(u, v);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t u = r.v[k >> 2][k & 3];  // a cast of the element itself reads element 0
-        v[k] = __builtin_bit_cast(float, u);
-      }
+      for (int k = 0; k < 4; ++k) v[k] = __builtin_bit_cast(float, u[k]);
     }
     if constexpr (BIAS) {
-      float w[8];
-      halves(r.bias, w);
+      float w[W];
+      halves<W>(r.bias, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += w[k];
+      for (int k = 0; k < W; ++k) v[k] += w[k];
     }
   }
   static __device__ __forceinline__ void keep(Raw& r) {
-    asm volatile("" : "+v"(r.v[0]));
-    if constexpr (!is_bf16<E>::value) asm volatile("" : "+v"(r.v[1]));
-    if constexpr (BIAS) asm volatile("" : "+v"(r.bias));
+    asm volatile("" : "+v"(r.v));
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int k = 0; k < W / 2; ++k) asm volatile("" : "+v"(r.bias[k]));
+    }
   }
   __device__ __forceinline__ float at(int64_t j) const {
     float v = ld(x, static_cast<size_t>(j));
@@ -89,85 +117,95 @@ struct Row {
   }
 };
 
-// A row's logits as its threads go through them: each(f, g) calls f(c, values) for this thread's
-// vectors c = tid, tid + NTH, ... of the row's V / 8, then g(column, value) for its one element
-// of the last V % 8. Streamed: from memory each time, four loads in flight.
+// A row's logits as its threads go through them: each(f, g) calls f(c, n, values) for groups of 8
+// values, the vector c and (fp32) the vector c + NTH, of which n are the row's (-inf stands for a
+// missing one's values); then g(column, value) for the logits outside the vectors. What a group
+// costs beside its logits (its largest, the reference's test) is shared by 8 of them.
+template <int NTH, typename R>
+struct Group {
+  static constexpr int W = R::W, G = 8 / W;
+  static __device__ __forceinline__ void values(const typename R::Raw (&raw)[G], int n, float (&v)[8]) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float w[W];
+      R::unpack(raw[g], w);
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[g * W + k] = g < n ? w[k] : -INFINITY;
+    }
+  }
+  // The group that starts at vector c.
+  template <typename F>
+  static __device__ __forceinline__ void last(const typename R::Raw (&raw)[G], int c, int nv, F f) {
+    if (c >= nv) return;
+    const int n = G == 2 && c + NTH >= nv ? 1 : G;
+    float v[8];
+    values(raw, n, v);
+    f(c, n, v);
+  }
+};
+// Streamed: from memory each time, four groups' loads in flight.
 template <int NTH, typename R>
 struct Streamed {
   const R& row;
-  int V;
-  template <typename F, typename G>
-  __device__ __forceinline__ void each(F f, G g) const {
-    constexpr int U = 4;
-    const int nv = V >> 3;
+  static constexpr int W = R::W;
+  template <typename F, typename H>
+  __device__ __forceinline__ void each(F f, H h) const {
+    using Gr = Group<NTH, R>;
+    constexpr int G = Gr::G, U = 4;
+    const int nv = row.vectors(), tid = threadIdx.x;
     int b = 0;  // the block's first vector
-    for (; b + U * NTH <= nv; b += U * NTH) {
-      typename R::Raw raw[U];
+    for (; b + U * G * NTH <= nv; b += U * G * NTH) {
+      typename R::Raw raw[U][G];
 #pragma unroll
-      for (int k = 0; k < U; ++k) raw[k] = row.load(b + k * NTH + threadIdx.x);
+      for (int k = 0; k < U * G; ++k) raw[k / G][k % G] = row.load(b + k * NTH + tid);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         float v[8];
-        R::unpack(raw[k], v);
-        f(b + k * NTH + threadIdx.x, v);
+        Gr::values(raw[k], G, v);
+        f(b + k * G * NTH + tid, G, v);
       }
     }
     if (b < nv) {
-      typename R::Raw raw[U];
+      typename R::Raw raw[U][G];
 #pragma unroll
-      for (int k = 0; k < U; ++k) raw[k] = row.load(min(b + k * NTH + static_cast<int>(threadIdx.x), nv - 1));
+      for (int k = 0; k < U * G; ++k) raw[k / G][k % G] = row.load(min(b + k * NTH + tid, nv - 1));
       // Without a use out here the compiler moves each load under its condition, one at a time.
 #pragma unroll
-      for (int k = 0; k < U; ++k) R::keep(raw[k]);
+      for (int k = 0; k < U * G; ++k) R::keep(raw[k / G][k % G]);
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int c = b + k * NTH + threadIdx.x;
-        if (c < nv) {
-          float v[8];
-          R::unpack(raw[k], v);
-          f(c, v);
-        }
-      }
+      for (int k = 0; k < U; ++k) Gr::last(raw[k], b + k * G * NTH + tid, nv, f);
     }
-    const int j = nv * 8 + threadIdx.x;
-    if (j < V) g(j, row.at(j));
+    row.singles(h);
   }
 };
-// Held: loaded once into NV vectors of registers a thread (V < 8 (NTH NV + 1)), for a row that is
-// read twice and written: the second reading otherwise comes from the memory side, as the rows
+// Held: loaded once into NV vectors of registers a thread (at most NTH NV vectors), for a row that
+// is read twice and written: the second reading otherwise comes from the memory side, as the rows
 // under way (2,048 of 64 KB) are far more than the L2 caches hold.
 template <int NTH, int NV, typename R>
 struct Held {
+  using Gr = Group<NTH, R>;
+  static constexpr int W = R::W, G = Gr::G;
   const R& row;
-  int V;
-  typename R::Raw raw[NV];
-  __device__ __forceinline__ Held(const R& row_, int V_) : row(row_), V(V_) {
-    const int nv = V >> 3;
+  typename R::Raw raw[NV / G][G];
+  __device__ __forceinline__ explicit Held(const R& row_) : row(row_) {
+    const int nv = row.vectors();
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      raw[k] = row.load(max(0, min(k * NTH + static_cast<int>(threadIdx.x), nv - 1)));
+      raw[k / G][k % G] = row.load(max(0, min(k * NTH + static_cast<int>(threadIdx.x), nv - 1)));
   }
-  template <typename F, typename G>
-  __device__ __forceinline__ void each(F f, G g) const {
-    const int nv = V >> 3;
+  template <typename F, typename H>
+  __device__ __forceinline__ void each(F f, H h) const {
+    const int nv = row.vectors();
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = k * NTH + threadIdx.x;
-      if (c < nv) {
-        float v[8];
-        R::unpack(raw[k], v);
-        f(c, v);
-      }
-    }
-    const int j = nv * 8 + threadIdx.x;
-    if (j < V) g(j, row.at(j));
+    for (int k = 0; k < NV / G; ++k) Gr::last(raw[k], k * G * NTH + threadIdx.x, nv, f);
+    row.singles(h);
   }
 };
 // NV = 0: streamed.
 template <int NTH, int NV, typename R>
-__device__ __forceinline__ auto source(const R& row, int V) {
-  if constexpr (NV > 0) return Held<NTH, NV, R>(row, V);
-  else return Streamed<NTH, R>{row, V};
+__device__ __forceinline__ auto source(const R& row) {
+  if constexpr (NV > 0) return Held<NTH, NV, R>(row);
+  else return Streamed<NTH, R>{row};
 }
 
 // Of a quiet NaN and a number the number; fmaxf adds an instruction an operand to quiet others.
@@ -176,7 +214,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-__device__ __forceinline__ float max8(const float (&v)[8]) {
+__device__ __forceinline__ float largest(const float (&v)[8]) {
   return max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[7]));
 }
 
@@ -241,7 +279,7 @@ struct Share {
     if (t > (SAFE ? r : r + 16.0f)) raise<REST>(t);
   }
   template <bool REST>
-  __device__ __forceinline__ void fold8(const float (&v)[8], float vm, uint32_t listed) {
+  __device__ __forceinline__ void fold(const float (&v)[8], float vm, uint32_t listed) {
     see<REST>(vm);
     float vs = 0.0f, vr = 0.0f;
 #pragma unroll
@@ -317,31 +355,45 @@ static Scale scale_of(float t) {
   return k;
 }
 
+__device__ __forceinline__ int pad_of(int head) { return -head & 7; }
+
 template <int NTH, bool REST, bool SAFE, typename S, typename See, typename Last>
 __device__ __forceinline__ Norm row_pass(const S& src, float c, const uint8_t* listed, float* sh,
                                          See see, Last last) {
+  // Bit j + pad of `listed` is column j's: whole vectors start at a multiple of 8 (or 4) bits.
+  const int pad = pad_of(src.row.head);
+  const uint8_t* body = REST ? listed + (src.row.head + pad) / 8 : nullptr;
   Share<SAFE> a(c);
   src.each(
-      [&](int k, const float (&v)[8]) {
-        const float vm = max8(v);
-        a.template fold8<REST>(v, vm, REST ? listed[k] : 0);
+      [&](int k, int n, const float (&v)[8]) {
+        const float vm = largest(v);
+        uint32_t bits = 0;
+        if constexpr (REST) {
+          if constexpr (S::W == 8) {
+            bits = body[k];
+          } else {
+            auto four = [&](int i) { return body[i >> 1] >> (4 * (i & 1)) & 15u; };
+            bits = four(k) | (n == 2 ? four(k + NTH) << 4 : 0u);
+          }
+        }
+        a.template fold<REST>(v, vm, bits);
         see(k, vm);
       },
       [&](int j, float x) {
-        a.template fold1<REST>(x, REST && (listed[j >> 3] >> (j & 7) & 1));
-        last(x);
+        a.template fold1<REST>(x, REST && (listed[(j + pad) >> 3] >> ((j + pad) & 7) & 1));
+        last(j, x);
       });
   a.template join<NTH, REST>(sh);
   return Norm{a.r, a.s, a.u, a.rest, SAFE};
 }
-// The row's norm; `see` gets each vector's number and largest logit, `last` the last logits.
+// The row's norm; `see` gets each group's first vector and largest logit, `last` the logits outside.
 template <int NTH, bool REST, typename S, typename See, typename Last>
 __device__ __forceinline__ Norm norm_of(const S& src, float c, const uint8_t* listed, float* sh,
                                         See see, Last last) {
   const Norm n = row_pass<NTH, REST, false>(src, c, listed, sh, see, last);
   if (n.s != 0.0f) return n;
   __syncthreads();
-  return row_pass<NTH, REST, true>(src, c, listed, sh, [](int, float) {}, [](float) {});
+  return row_pass<NTH, REST, true>(src, c, listed, sh, [](int, float) {}, [](int, float) {});
 }
 
 // ---- the K largest logits of a row ---------------------------------------------------------
@@ -356,15 +408,17 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// A thread's best two vectors (8 neighbouring logits, by their largest).
+// A thread's best groups, by their largest logits: two with their places, the third's value.
 struct Best {
-  float v1 = -INFINITY, v2 = -INFINITY;
-  int c1 = -1;
+  float v1 = -INFINITY, v2 = -INFINITY, v3 = -INFINITY;
+  int c1 = -1, c2 = -1;
   __device__ __forceinline__ void see(float vm, int c) {
-    const bool up = vm > v1;
-    v2 = up ? v1 : fmaxf(v2, vm);
-    c1 = up ? c : c1;
-    v1 = up ? vm : v1;
+    const bool up1 = vm > v1, up2 = vm > v2;
+    v3 = up2 ? v2 : fmaxf(v3, vm);
+    v2 = up1 ? v1 : up2 ? vm : v2;
+    c2 = up1 ? c1 : up2 ? c : c2;
+    v1 = up1 ? vm : v1;
+    c1 = up1 ? c : c1;
   }
 };
 
@@ -372,8 +426,9 @@ template <int NTH>
 struct TopShared {
   uint64_t cand[kCap];  // key << 32 | ~column: the larger, the earlier
   float best[NTH];
+  uint16_t full[NTH];
   uint32_t tau;
-  int count;
+  int count, fulls;
   int wave[NTH / 64];
 };
 
@@ -384,12 +439,12 @@ __device__ __forceinline__ void push(uint64_t* cand, int* count, uint32_t key, i
 
 // How many of the row's keys are at least `lo`.
 template <int NTH, typename R>
-__device__ int count_from(const R& row, int V, uint32_t lo, TopShared<NTH>& t) {
+__device__ int count_from(const R& row, uint32_t lo, TopShared<NTH>& t) {
   int n = 0;
-  Streamed<NTH, R>{row, V}.each(
-      [&](int, const float (&v)[8]) {
+  Streamed<NTH, R>{row}.each(
+      [&](int, int m, const float (&v)[8]) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) n += key_of(v[k]) >= lo;
+        for (int k = 0; k < 8; ++k) n += k < m * R::W && key_of(v[k]) >= lo;
       },
       [&](int, float x) { n += key_of(x) >= lo; });
 #pragma unroll
@@ -404,11 +459,11 @@ __device__ int count_from(const R& row, int V, uint32_t lo, TopShared<NTH>& t) {
 
 // Appends the first `want` columns (in order) whose key is `key`.
 template <int NTH, typename R>
-__device__ void append_equal(const R& row, int V, uint32_t key, int want, TopShared<NTH>& t) {
+__device__ void append_equal(const R& row, uint32_t key, int want, TopShared<NTH>& t) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int j0 = 0; j0 < V && want > 0; j0 += NTH) {
+  for (int j0 = 0; j0 < row.V && want > 0; j0 += NTH) {
     const int j = j0 + threadIdx.x;
-    const bool hit = j < V && key_of(row.at(j)) == key;
+    const bool hit = j < row.V && key_of(row.at(j)) == key;
     const uint64_t mask = __ballot(hit);
     __syncthreads();  // the counts of the tile before have been read
     if (lane == 0) t.wave[wave] = __popcll(mask);
@@ -429,12 +484,13 @@ __device__ void append_equal(const R& row, int V, uint32_t key, int want, TopSha
 // it are read again, gathered and ranked against each other. Where more than kCap reach it
 // (rows with many equal logits) the K-th largest key is found by bisection over the row.
 template <int NTH, typename R>
-__device__ void top_k(const R& row, int V, int K, const Best& b, float last, bool nan,
+__device__ void top_k(const R& row, int K, const Best& b, float outside, bool nan,
                       TopShared<NTH>& t) {
   const int tid = threadIdx.x;
-  const int nv = V >> 3;
-  t.best[tid] = fmaxf(b.v1, last);
-  if (tid == 0) t.count = 0;
+  constexpr int W = R::W;
+  const int nv = row.vectors();
+  t.best[tid] = fmaxf(b.v1, outside);
+  if (tid == 0) t.count = t.fulls = 0;
   __syncthreads();
   if (tid < 64) {  // the upper 16 bits of the bound, bit by bit (the lower ones as zeros)
     uint32_t k[NTH / 64];
@@ -458,44 +514,58 @@ __device__ void top_k(const R& row, int V, int K, const Best& b, float last, boo
     const uint32_t k = key_of(x);
     if (k >= tau) push(t.cand, &t.count, k, j);
   };
-  if (key_of(b.v1) >= tau && b.c1 >= 0) {
-    const bool more = key_of(b.v2) >= tau;
-    for (int c = more ? tid : b.c1; c < nv; c += more ? NTH : nv) {
-      float v[8];
-      R::unpack(row.load(c), v);
+  auto take_vector = [&](int c) {
+    float v[W];
+    R::unpack(row.load(c), v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) take(c * 8 + k, v[k]);
+    for (int k = 0; k < W; ++k) take(static_cast<int>(row.column(c)) + k, v[k]);
+  };
+  // A thread whose third best group reaches the bound too leaves all of its vectors to a wave.
+  if (key_of(b.v3) >= tau) {
+    t.full[atomicAdd(&t.fulls, 1)] = static_cast<uint16_t>(tid);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = i ? b.c2 : b.c1;
+      if (c < 0 || key_of(i ? b.v2 : b.v1) < tau) continue;
+      take_vector(c);
+      if (W == 4 && c + NTH < nv) take_vector(c + NTH);
     }
   }
-  if (nv * 8 + tid < V) take(nv * 8 + tid, last);
+  row.singles(take);
+  __syncthreads();
+  for (int i = tid >> 6; i < t.fulls; i += NTH / 64)
+    for (int c = t.full[i] + (tid & 63) * NTH; c < nv; c += 64 * NTH) take_vector(c);
   __syncthreads();
   int n = t.count;
   if (n > kCap || nan) {  // a NaN may have hidden its neighbours' maximum
     uint32_t lo = nan ? 0 : tau, hi = 0xffffffffu;  // K keys are at least lo, fewer at least hi
     while (hi - lo > 1) {
       const uint32_t mid = lo + (hi - lo) / 2;
-      if (count_from<NTH>(row, V, mid, t) >= K) lo = mid; else hi = mid;
+      if (count_from<NTH>(row, mid, t) >= K) lo = mid; else hi = mid;
     }
     __syncthreads();
     if (tid == 0) t.count = 0;
     __syncthreads();
-    Streamed<NTH, R>{row, V}.each(
-        [&](int c, const float (&v)[8]) {
+    Streamed<NTH, R>{row}.each(
+        [&](int c, int m, const float (&v)[8]) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (key_of(v[k]) > lo) push(t.cand, &t.count, key_of(v[k]), c * 8 + k);
+            if (k < m * W && key_of(v[k]) > lo)
+              push(t.cand, &t.count, key_of(v[k]),
+                   static_cast<int>(row.column(c + k / W * NTH)) + k % W);
         },
         [&](int j, float x) {
           if (key_of(x) > lo) push(t.cand, &t.count, key_of(x), j);
         });
     __syncthreads();
     n = t.count;
-    append_equal<NTH>(row, V, lo, K - n, t);
+    append_equal<NTH>(row, lo, K - n, t);
     __syncthreads();
     n = t.count;
   }
   if (n < K) {  // fewer numbers than K: -inf (and NaN) fill the places
-    append_equal<NTH>(row, V, kNone, K - n, t);
+    append_equal<NTH>(row, kNone, K - n, t);
     __syncthreads();
     n = t.count;
   }
@@ -509,15 +579,15 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
     float* __restrict__ top_lp, int64_t* __restrict__ top_idx, uint32_t* err) {
   __shared__ float sh[2 * (NTH / 64)];
   const size_t r = blockIdx.x;
-  const Row<E, BIAS> row{logits + r * ldl, bias};
+  const Row<E, BIAS, !BIAS> row(logits + r * ldl, bias, V);
   Best best;
-  float last = -INFINITY;
+  float outside = -INFINITY;
   const Norm n = norm_of<NTH, false>(
-      Streamed<NTH, Row<E, BIAS>>{row, V}, k.c, nullptr, sh,
+      source<NTH, 0>(row), k.c, nullptr, sh,
       [&](int c, float vm) {
         if constexpr (TOP) best.see(vm, c);
       },
-      [&](float x) { last = x; });
+      [&](int, float x) { outside = fmaxf(outside, x); });
   const double ln_s = n.ln_s(k.delta);
   auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (threadIdx.x == 0) {
@@ -543,11 +613,12 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
   }
   if constexpr (TOP) {
     __shared__ TopShared<NTH> t;
-    top_k<NTH>(row, V, K, best, last, n.s != n.s, t);
+    top_k<NTH>(row, K, best, outside, n.s != n.s, t);
     const int count = t.count;
     for (int i = threadIdx.x; i < count; i += NTH) {
       const uint64_t mine = t.cand[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < count; ++j) rank += t.cand[j] > mine;
       if (rank < K) {
         top_lp[r * K + rank] = lp(of_key(static_cast<uint32_t>(mine >> 32)));
@@ -562,33 +633,29 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
 // value: the gradient products of a bf16 readout then run as bf16 matrix products with an
 // error of 2^-18 a term, far below the 2^-9 that their bf16 results are rounded by; one bf16
 // row would add as much as that rounding.
+__device__ __forceinline__ uint32_t pair(float a, float b) {
+  return static_cast<uint32_t>(f2bf(a)) | static_cast<uint32_t>(f2bf(b)) << 16;
+}
 template <typename E>
 struct RowOut {
+  static constexpr int W = is_bf16<E>::value ? 8 : 4;
   E* p;
+  int head;
   __device__ __forceinline__ void put(int64_t j, float v) const { st(p, j, v); }
-  __device__ __forceinline__ void put8(int c, const float (&v)[8]) const {
-    E* q = p + static_cast<size_t>(c) * 8;
-    if constexpr (is_bf16<E>::value) {
-      u32x4 u;
+  __device__ __forceinline__ void put(int c, const float (&v)[W]) const {
+    u32x4 u;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        u[k] = static_cast<uint32_t>(f2bf(v[2 * k])) |
-               static_cast<uint32_t>(f2bf(v[2 * k + 1])) << 16;
-      *reinterpret_cast<u32x4_any*>(q) = u;
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 u;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) u[k] = __builtin_bit_cast(uint32_t, v[4 * h + k]);
-        *reinterpret_cast<u32x4_any*>(q + 4 * h) = u;
-      }
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (is_bf16<E>::value) u[k] = pair(v[2 * k], v[2 * k + 1]);
+      else u[k] = __builtin_bit_cast(uint32_t, v[k]);
     }
+    __builtin_nontemporal_store(u, reinterpret_cast<u32x4_any*>(p + head + static_cast<size_t>(c) * W));
   }
 };
 struct PlanesOut {
   bf16* p;
   int64_t plane;
+  int head;
   __device__ __forceinline__ static float left(float v) {
     const float r = v - bf2f(f2bf(v));
     return r == r ? r : 0.0f;  // inf and NaN are the first plane's alone
@@ -597,20 +664,20 @@ struct PlanesOut {
     p[j] = f2bf(v);
     p[plane + j] = f2bf(left(v));
   }
-  __device__ __forceinline__ void put8(int c, const float (&v)[8]) const {
-    float w[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = left(v[k]);
-    RowOut<bf16>{p}.put8(c, v);
-    RowOut<bf16>{p + plane}.put8(c, w);
+  __device__ __forceinline__ void put(int c, const float (&v)[4]) const {
+    const uint32_t hi[2] = {pair(v[0], v[1]), pair(v[2], v[3])};
+    const uint32_t lo[2] = {pair(left(v[0]), left(v[1])), pair(left(v[2]), left(v[3]))};
+    bf16* q = p + head + static_cast<size_t>(c) * 4;
+    __builtin_memcpy(q, hi, 8);
+    __builtin_memcpy(q + plane, lo, 8);
   }
 };
 template <typename E, bool PLANES>
-__device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_t plane) {
+__device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_t plane, int head) {
   if constexpr (PLANES) {
-    return PlanesOut{static_cast<bf16*>(out) + r * ldo, plane};
+    return PlanesOut{static_cast<bf16*>(out) + r * ldo, plane, head};
   } else {
-    return RowOut<E>{static_cast<E*>(out) + r * ldo};
+    return RowOut<E>{static_cast<E*>(out) + r * ldo, head};
   }
 }
 
@@ -624,10 +691,11 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
     const float* __restrict__ entropy, const float* __restrict__ g_lp,
     const float* __restrict__ g_ent, const float* __restrict__ g_top, void* out, int64_t ldo,
     int64_t plane) {
+  constexpr int W = RowOut<E>::W;
   __shared__ int taken;
   const size_t r = blockIdx.x;
-  const Row<E, BIAS> row{logits + r * ldl, bias};
-  const auto o = out_row<E, PLANES>(out, r, ldo, plane);
+  const Row<E, BIAS, !BIAS> row(logits + r * ldl, bias, V);
+  const auto o = out_row<E, PLANES>(out, r, ldo, plane, row.head);
   const float inv_t = static_cast<float>(k.inv_t), c = k.c;
   const Norm n{stats[2 * r], fabsf(stats[2 * r + 1]), 0.0f, 0.0f, stats[2 * r + 1] < 0.0f};
   int64_t t = targets && g_lp ? targets[r] : -1;
@@ -651,14 +719,17 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
       const float a = arg(x);
       return __builtin_amdgcn_exp2f(a) * __builtin_fmaf(B, fmaxf(a, -1e30f), A);
     };
-    Streamed<NTH, Row<E, BIAS>>{row, V}.each(
-        [&](int j, const float (&v)[8]) {
-          float w[8];
+    source<NTH, 0>(row).each(
+        [&](int c, int m, const float (&v)[8]) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = grad(v[e]);
-          o.put8(j, w);
+          for (int g = 0; g < 8 / W; ++g) {
+            float w[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) w[e] = grad(v[g * W + e]);
+            if (g < m) o.put(c + g * NTH, w);
+          }
         },
-        [&](int j, float x) { o.put(j, grad(x)); });
+        [&](int j, float x) { o.put(static_cast<int64_t>(j), grad(x)); });
     __syncthreads();
     if (n.empty()) return;  // nothing depends on the row
     if (g_top) {
@@ -712,13 +783,19 @@ __device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n,
   const float asc = a * sc, bsc = b * sc;
   n.with_arg(c, [&](auto arg) {
     src.each(
-        [&](int k, const float (&v)[8]) {
-          float w[8];
+        [&](int c, int m, const float (&v)[8]) {
+          constexpr int W = S::W;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(arg(v[e])) * asc;
-          o.put8(k, w);
+          for (int g = 0; g < 8 / W; ++g) {
+            float w[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) w[e] = __builtin_amdgcn_exp2f(arg(v[g * W + e])) * asc;
+            if (g < m) o.put(c + g * NTH, w);
+          }
         },
-        [&](int j, float x) { o.put(j, __builtin_amdgcn_exp2f(arg(x)) * asc); });
+        [&](int j, float x) {
+          o.put(static_cast<int64_t>(j), __builtin_amdgcn_exp2f(arg(x)) * asc);
+        });
     __syncthreads();
     for (int k = threadIdx.x; k < K; k += NTH) {
       const int j = idx[k];
@@ -733,7 +810,7 @@ __device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n,
           w += same ? q[i] : 0.0f;
         }
       }
-      if (first) o.put(j, __builtin_amdgcn_exp2f(arg(src.row.at(j))) * bsc - w * sc);
+      if (first) o.put(static_cast<int64_t>(j), __builtin_amdgcn_exp2f(arg(src.row.at(j))) * bsc - w * sc);
     }
   });
 }
@@ -752,8 +829,8 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   __shared__ Teacher te;
   const size_t r = blockIdx.x;
   const int tid = threadIdx.x;
-  const Row<E, BIAS> row{logits + r * ldl, bias};
-  const auto src = source<NTH, NV>(row, V);
+  const Row<E, BIAS, !BIAS && (!GRAD || NV > 0)> row(logits + r * ldl, bias, V);
+  const auto src = source<NTH, NV>(row);
   for (int i = tid; i < words; i += NTH) bits[i] = 0;
   if (tid == 0) te.twice = 0;
   __syncthreads();
@@ -779,7 +856,8 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
             j = static_cast<int>(at);
             u[h] = v * sc.inv_t;
             x[h] = row.at(at);
-            const uint32_t bit = static_cast<uint32_t>(j) % (static_cast<uint32_t>(words) * 32);
+            const uint32_t bit = static_cast<uint32_t>(j + pad_of(row.head)) %
+                                 (static_cast<uint32_t>(words) * 32);
             if (atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1) te.twice = 1;
           }
         }
@@ -809,7 +887,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   }
   __syncthreads();
   const Norm a = norm_of<NTH, REST>(src, sc.c, reinterpret_cast<const uint8_t*>(bits), sh,
-                                    [](int, float) {}, [](float) {});
+                                    [](int, float) {}, [](int, float) {});
   if (tid < 64) {
     const bool empty = a.empty();
     const double ln_s = a.ln_s(sc.delta);
@@ -860,7 +938,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   if constexpr (GRAD) {
     __syncthreads();
     distill_grad<NTH>(src, K, a, sc.c, scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
-                      out_row<E, PLANES>(out, r, ldo, plane));
+                      out_row<E, PLANES>(out, r, ldo, plane, row.head));
   }
 }
 
@@ -880,10 +958,10 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
   }
   const int flags = static_cast<int>(coef[4 * r + 3]);
   const Norm n{coef[4 * r], 1.0f, 0.0f, 0.0f, (flags & 2) != 0};
-  const Row<E, false> row{logits + r * ldl, nullptr};
-  distill_grad<NTH>(Streamed<NTH, Row<E, false>>{row, V}, K, n, c, scale[0] * grad[0],
+  const Row<E, false, true> row(logits + r * ldl, nullptr, V);
+  distill_grad<NTH>(source<NTH, 0>(row), K, n, c, scale[0] * grad[0],
                     coef[4 * r + 1], coef[4 * r + 2], (flags & 1) != 0, idx, q,
-                    RowOut<E>{out + r * V});
+                    RowOut<E>{out + r * V, row.head});
 }
 
 // mean = weight T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = weight T / that count;
@@ -955,9 +1033,10 @@ __global__ void __launch_bounds__(256) column_sums_kernel(int64_t rows, int V, i
   for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
 #pragma unroll 8
   for (int64_t r = r0; r < r1; ++r) {  // the stride is a multiple of 8: whole vectors
-    const u32x4 u = *reinterpret_cast<const u32x4*>(x + r * ld + c);
+    uint32_t u[4];
+    __builtin_memcpy(u, __builtin_assume_aligned(x + r * ld + c, 16), 16);
     float v[8];
-    Row<bf16, false>::halves(u, v);
+    halves<8>(u, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[k] += c + k < V ? v[k] : 0.0f;
   }
@@ -982,15 +1061,16 @@ template <typename E>
 __global__ void __launch_bounds__(256) scaled_kernel(int64_t n, const float* __restrict__ x,
                                                      const float* __restrict__ g,
                                                      E* __restrict__ out) {
+  constexpr int W = RowOut<E>::W;
   const float s = g[0];
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * 8;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += step) {
-    if (i + 8 <= n) {
-      float v[8];
-      Row<float, false>::unpack(Row<float, false>{x + i, nullptr}.load(0), v);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * W;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * W; i < n; i += step) {
+    if (i + W <= n) {
+      float v[W];
+      __builtin_memcpy(v, x + i, 4 * W);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= s;
-      RowOut<E>{out + i}.put8(0, v);
+      for (int k = 0; k < W; ++k) v[k] *= s;
+      RowOut<E>{out + i, 0}.put(0, v);
     } else {
       for (int64_t j = i; j < n; ++j) st(out, j, x[j] * s);
     }
@@ -1162,7 +1242,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
-  const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 31) / 32);
+  const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 7 + 31) / 32);
 #define DABSN_LAUNCH(E, BIAS, N, NV, REST, GRAD, PLANES)                                          \
   hipLaunchKernelGGL((distill_kernel<E, BIAS, N, NV, REST, GRAD, PLANES>), grid, dim3(N), 4 * words, \
                      stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype,  \
@@ -1186,17 +1266,17 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
     else { DABSN_REST(float, false, N, 0, true, false); }                                    \
   }
   // Held rows: 64 registers a thread, so that four waves share a SIMD.
-  const int64_t nv = V >> 3;
-  if (out && !plane && !b && V > 1024 && dtype == kBF16 && nv <= 256 * 16) {
+  const bool hold = out && !plane && !b && V > 1024;
+  const int64_t nv = V / (dtype == kBF16 ? 8 : 4);
+  if (hold && dtype == kBF16 && nv <= 512 * 16) {
     if (nv <= 256 * 8) { DABSN_REST(bf16, false, 256, 8, true, false); }
-    else { DABSN_REST(bf16, false, 256, 16, true, false); }
-  } else if (out && !plane && !b && V > 1024 && dtype == kBF16 && nv <= 512 * 16) {
-    DABSN_REST(bf16, false, 512, 16, true, false);
-  } else if (out && !plane && !b && V > 1024 && dtype == kF32 && nv <= 512 * 8) {
+    else if (nv <= 256 * 16) { DABSN_REST(bf16, false, 256, 16, true, false); }
+    else { DABSN_REST(bf16, false, 512, 16, true, false); }
+  } else if (hold && dtype == kF32 && nv <= 1024 * 16) {
     if (nv <= 256 * 8) { DABSN_REST(float, false, 256, 8, true, false); }
-    else { DABSN_REST(float, false, 512, 8, true, false); }
-  } else if (out && !plane && !b && V > 1024 && dtype == kF32 && nv <= 1024 * 8) {
-    DABSN_REST(float, false, 1024, 8, true, false);
+    else if (nv <= 256 * 16) { DABSN_REST(float, false, 256, 16, true, false); }
+    else if (nv <= 512 * 16) { DABSN_REST(float, false, 512, 16, true, false); }
+    else { DABSN_REST(float, false, 1024, 16, true, false); }
   } else {
     DABSN_BY_THREADS(DABSN_ROWS);
   }

@@ -37,10 +37,14 @@ _WHAT = "distillation"
 
 # From this many logits on, the gradient is formed with the loss while a row's logits are in
 # registers, and the backward only checks that its upstream factor is 1 (loss.backward()); another
-# factor forms it again. 8192 x 32000 bf16: 230 us forward and backward against 355 in two passes
-# (and 430 for another factor; ``loss_weight`` keeps a mixed objective's share out of it). Below, the
-# two launches that count the rows ahead cost more than the second reading: 2048 x 65 fp32.
+# factor forms it again (``loss_weight`` keeps a mixed objective's share out of it). Forward and
+# backward in two passes -> with the gradient formed ahead (and again for another factor), us:
+# 8388 x 32000 bf16 356 -> 240 (466), 16777 x 16000 368 -> 244 (480), 4129 x 65000 373 -> 234 (478),
+# 2097 x 32000 fp32 183 -> 140 (254). A row of few words is read again from the L2 cache (33554 x
+# 2000 bf16 160 -> 176), one of too many is not held in registers (2684 x 100000 373 -> 351, 591),
+# and below 2^24 logits the launches that count the rows ahead cost more than the second reading.
 _FUSED_LOGITS = 1 << 24
+_FUSED_WORDS = (4096, 65536)
 
 
 def _rows(x, bias, values, tokens, lse, ignore, t, s, loss, coef, weights, scale, out, ldo, plane,
@@ -69,7 +73,7 @@ class _FromLogits(torch.autograd.Function):
     def forward(ctx, x, values, tokens, lse, ignore, t, weight):
         (n, V), K, dev = x.shape, tokens.shape[1], x.device
         need, lib = ctx.needs_input_grad[0], _lib.load()
-        fused = need and n * V >= _FUSED_LOGITS
+        fused = need and n * V >= _FUSED_LOGITS and _FUSED_WORDS[0] <= V <= _FUSED_WORDS[1]
         with vocab.on(x):
             stream = vocab.stream(x)
             word = vocab.ErrorWord(dev)

@@ -51,11 +51,11 @@ class _ScaledEmbedding(torch.autograd.Function):
         with vocab.on(g):
             out = torch.empty((V, H), device=g.device, dtype=dtype)
             nbytes = lib.dabsn_hip_embedding_workspace_bytes(n, V, H)
-            ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
+            ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8) if nbytes else None
             tk = ops.KernelTimer.begin("embedding_bwd", g)
             _lib.check(lib.dabsn_hip_embedding_bwd(
                 ops._code(dtype), n, V, H, ids.data_ptr(), padding, g.data_ptr(), scale,
-                out.data_ptr(), ws.data_ptr(), nbytes, vocab.stream(g)), _WHAT + " backward")
+                out.data_ptr(), ops._p(ws), nbytes, vocab.stream(g)), _WHAT + " backward")
             ops.KernelTimer.end(tk)
         return None, out, None, None
 

@@ -752,7 +752,7 @@ int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* scale, v
  * any alignment), one rounding. An id outside [0, V) sets *err to 1 and its row to NaN.
  * Backward: dweight [V, H] = scale * the sum of grad [n, H] over the tokens of each word, fp32
  * sums in a fixed order, one rounding; zeros for words without tokens, for padding_idx and for
- * ids out of range. Workspace: dabsn_hip_embedding_workspace_bytes(n, V, H) (0: refused). */
+ * ids out of range. Workspace: dabsn_hip_embedding_workspace_bytes(n, V, H) (0 for few tokens). */
 int dabsn_hip_embedding_fwd(int dtype, int64_t n, int64_t V, int64_t H, const int64_t* ids,
                             const void* weight, int64_t ldw, float scale, void* out, uint32_t* err,
                             hipStream_t stream);
