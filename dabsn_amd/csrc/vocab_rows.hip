@@ -629,10 +629,15 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
 }
 
 // ---- where a gradient goes -----------------------------------------------------------------
-// A row of the logits' type, or (planes) two bf16 rows whose sum holds 17 bits of the fp32
-// value: the gradient products of a bf16 readout then run as bf16 matrix products with an
-// error of 2^-18 a term, far below the 2^-9 that their bf16 results are rounded by; one bf16
-// row would add as much as that rounding.
+// A row of the logits' type; or, for the gradient products of a bf16 readout, which run as 16-bit
+// matrix products with fp32 sums and round their results to bf16 (2^-9):
+//   planes   two bf16 rows whose sum holds 17 bits of the fp32 value, of any size (the products'
+//            error 2^-18 a term; one bf16 row would add as much as the results' rounding);
+//   half     one fp16 row, for gradients whose size is known (distillation: p and q, at most
+//            kMostWeight, times kHalfScale): 11 bits, an error of 2^-12 a term, an eighth of the
+//            results' rounding, at half the products of the planes.
+enum OutKind : int { kRows = 0, kPlanes = 1, kHalf = 2 };
+constexpr float kMostWeight = 256.0f, kHalfScale = 128.0f;
 __device__ __forceinline__ uint32_t pair(float a, float b) {
   return static_cast<uint32_t>(f2bf(a)) | static_cast<uint32_t>(f2bf(b)) << 16;
 }
@@ -672,18 +677,27 @@ struct PlanesOut {
     __builtin_memcpy(q + plane, lo, 8);
   }
 };
-template <typename E, bool PLANES>
-__device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_t plane, int head) {
-  if constexpr (PLANES) {
-    return PlanesOut{static_cast<bf16*>(out) + r * ldo, plane, head};
-  } else {
-    return RowOut<E>{static_cast<E*>(out) + r * ldo, head};
+struct HalfOut {
+  _Float16* p;
+  int head;
+  __device__ __forceinline__ void put(int64_t j, float v) const { p[j] = static_cast<_Float16>(v); }
+  __device__ __forceinline__ void put(int c, const float (&v)[4]) const {
+    _Float16 h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = static_cast<_Float16>(v[k]);
+    __builtin_memcpy(p + head + static_cast<size_t>(c) * 4, h, 8);
   }
+};
+template <typename E, int KIND>
+__device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_t plane, int head) {
+  if constexpr (KIND == kPlanes) return PlanesOut{static_cast<bf16*>(out) + r * ldo, plane, head};
+  else if constexpr (KIND == kHalf) return HalfOut{static_cast<_Float16*>(out) + r * ldo, head};
+  else return RowOut<E>{static_cast<E*>(out) + r * ldo, head};
 }
 
 // d x_j = -(p_j / T) (g_lp + sum g_top + g_H (logp_j + H)), plus g_lp / T at the target and
 // g_top / T at the alternatives. The whole row is written without these, then their places.
-template <typename E, bool BIAS, int NTH, bool PLANES>
+template <typename E, bool BIAS, int NTH, int KIND>
 __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
     const int64_t* __restrict__ targets, int64_t ignore, Scale k, int K,
@@ -695,7 +709,7 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
   __shared__ int taken;
   const size_t r = blockIdx.x;
   const Row<E, BIAS, !BIAS> row(logits + r * ldl, bias, V);
-  const auto o = out_row<E, PLANES>(out, r, ldo, plane, row.head);
+  const auto o = out_row<E, KIND>(out, r, ldo, plane, row.head);
   const float inv_t = static_cast<float>(k.inv_t), c = k.c;
   const Norm n{stats[2 * r], fabsf(stats[2 * r + 1]), 0.0f, 0.0f, stats[2 * r + 1] < 0.0f};
   int64_t t = targets && g_lp ? targets[r] : -1;
@@ -815,15 +829,15 @@ __device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n,
   });
 }
 
-// GRAD 0: loss and coefficients; 1: and the row's gradient (T / count), as the fused readout
-// takes it while the logits are at hand.
-template <typename E, bool BIAS, int NTH, int NV, bool REST, bool GRAD, bool PLANES>
+// GRAD: the row's gradient too while its logits are at hand, times scale[0] (T / count); as fp16
+// rows (KIND) times kHalfScale.
+template <typename E, bool BIAS, int NTH, int NV, bool REST, bool GRAD, int KIND>
 __global__ void __launch_bounds__(NTH) distill_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias, int K,
     int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
     int64_t ignore, Scale sc, const float* __restrict__ teacher_lse, int words,
     float* __restrict__ loss, float* __restrict__ coef, float* __restrict__ weights,
-    const float* __restrict__ scale, void* out, int64_t ldo, int64_t plane, uint32_t* err) {
+    const float* __restrict__ scale, void* out, int64_t ldo, uint32_t* err) {
   extern __shared__ uint32_t bits[];
   __shared__ float sh[3 * (NTH / 64)];
   __shared__ Teacher te;
@@ -883,6 +897,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
       all += q[h];
     }
     total = wave_sum_d(all);
+    wrong = wrong || total > kMostWeight;
     if constexpr (REST) rest = 1.0 - total;
   }
   __syncthreads();
@@ -937,8 +952,8 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   }
   if constexpr (GRAD) {
     __syncthreads();
-    distill_grad<NTH>(src, K, a, sc.c, scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
-                      out_row<E, PLANES>(out, r, ldo, plane, row.head));
+    distill_grad<NTH>(src, K, a, sc.c, KIND == kHalf ? kHalfScale : scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
+                      out_row<E, KIND>(out, r, ldo, 0, row.head));
   }
 }
 
@@ -1019,10 +1034,11 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(int64_t rows, int V, 
   }
 }
 
-// part[b][c] = the sum over the rows b * kSumRows + 0 .. of column c of bf16 rows x (stride ld).
+// part[b][c] = the sum over the rows b * kSumRows + 0 .. of column c of 16-bit rows x (stride ld).
 constexpr int kSumRows = 64;
+template <bool HALF>
 __global__ void __launch_bounds__(256) column_sums_kernel(int64_t rows, int V, int64_t ld,
-                                                          const bf16* __restrict__ x,
+                                                          const uint16_t* __restrict__ x,
                                                           float* __restrict__ part) {
   const unsigned strips = (V + 2047) / 2048, b = blockIdx.x / strips;
   const int c = ((blockIdx.x - b * strips) * 256 + threadIdx.x) * 8;
@@ -1033,10 +1049,17 @@ __global__ void __launch_bounds__(256) column_sums_kernel(int64_t rows, int V, i
   for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
 #pragma unroll 8
   for (int64_t r = r0; r < r1; ++r) {  // the stride is a multiple of 8: whole vectors
-    uint32_t u[4];
-    __builtin_memcpy(u, __builtin_assume_aligned(x + r * ld + c, 16), 16);
     float v[8];
-    halves<8>(u, v);
+    if constexpr (HALF) {
+      _Float16 u[8];
+      __builtin_memcpy(u, __builtin_assume_aligned(x + r * ld + c, 16), 16);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(u[k]);
+    } else {
+      uint32_t u[4];
+      __builtin_memcpy(u, __builtin_assume_aligned(x + r * ld + c, 16), 16);
+      halves<8>(u, v);
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[k] += c + k < V ? v[k] : 0.0f;
   }
@@ -1056,13 +1079,77 @@ __global__ void __launch_bounds__(256) add_parts_kernel(int64_t parts, int V,
   out[c] = s;
 }
 
-// out[i] = x[i] * g[0] in the type of out: gradients held in fp32 from the forward, rounded once.
+// bf16 values as fp16 ones times a power of two that takes the largest to [2^14, 2^15): those down
+// to 2^-31 of the largest keep their 8 bits, the error of a smaller one is below 2^-39 of it. The
+// first kernel (after the word is cleared) finds the largest finite magnitude, as the bits of a
+// float; the second copies and leaves 1 / the power.
+__global__ void clear_word_kernel(uint32_t* word) { *word = 0; }
+__global__ void __launch_bounds__(256) largest_kernel(int64_t n, const bf16* __restrict__ x,
+                                                      uint32_t* __restrict__ word) {
+  uint32_t m = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * 8;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += step) {
+    bf16 u[8];
+    if (i + 8 <= n) {
+      __builtin_memcpy(u, __builtin_assume_aligned(x + i, 16), 16);
+    } else {
+      for (int k = 0; k < 8; ++k) u[k] = i + k < n ? x[i + k] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t a = u[k] & 0x7fffu;
+      m = a < 0x7f80u ? max(m, a) : m;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o, 64)));
+  // One atomic a block, and only of a larger value (a stale word costs one more): of every wave's
+  // they took 190 us.
+  __shared__ uint32_t sh[4];
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    m = max(max(sh[0], sh[1]), max(sh[2], sh[3])) << 16;
+    if (m > __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(word, m);
+  }
+}
+__global__ void __launch_bounds__(256) half_copy_kernel(int64_t n, const bf16* __restrict__ x,
+                                                        const uint32_t* __restrict__ word,
+                                                        _Float16* __restrict__ out,
+                                                        float* __restrict__ inverse) {
+  // The largest's exponent, a subnormal bf16's as that of the smallest normal one.
+  const int e = max(static_cast<int>(*word >> 23), 1) - 127;
+  const int shift = *word ? min(14 - e, 126) : 0;
+  const float s = ldexpf(1.0f, shift);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *inverse = ldexpf(1.0f, -shift);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * 8;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += step) {
+    if (i + 8 <= n) {
+      bf16 u[8];
+      _Float16 h[8];
+      __builtin_memcpy(u, __builtin_assume_aligned(x + i, 16), 16);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) h[k] = static_cast<_Float16>(bf2f(u[k]) * s);
+      __builtin_memcpy(__builtin_assume_aligned(out + i, 16), h, 16);
+    } else {
+      for (int64_t j = i; j < n; ++j) out[j] = static_cast<_Float16>(bf2f(x[j]) * s);
+    }
+  }
+}
+
+// out[i] = x[i] * the product of up to three device scalars and f, in the type of out: gradients
+// held in fp32 from the forward, rounded once.
+struct Factors {
+  const float* p[3];
+  float f;
+};
 template <typename E>
 __global__ void __launch_bounds__(256) scaled_kernel(int64_t n, const float* __restrict__ x,
-                                                     const float* __restrict__ g,
-                                                     E* __restrict__ out) {
+                                                     Factors g, E* __restrict__ out) {
   constexpr int W = RowOut<E>::W;
-  const float s = g[0];
+  float s = g.f;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) s *= g.p[k] ? g.p[k][0] : 1.0f;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * W;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * W; i < n; i += step) {
     if (i + W <= n) {
@@ -1165,18 +1252,18 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
-#define DABSN_LAUNCH(E, BIAS, N, PLANES)                                                         \
-  hipLaunchKernelGGL((logprobs_bwd_kernel<E, BIAS, N, PLANES>), grid, dim3(N), 0, stream, (int)V, \
+#define DABSN_LAUNCH(E, BIAS, N, KIND)                                                           \
+  hipLaunchKernelGGL((logprobs_bwd_kernel<E, BIAS, N, KIND>), grid, dim3(N), 0, stream, (int)V, \
                      ldl, static_cast<const E*>(logits), b, targets, ignore_index, scale_t,         \
                      (int)top, top_indices, stats, entropy, g_logprob, g_entropy, g_top, out,     \
                      ldo, plane)
 #define DABSN_ROWS(N)                                                                             \
   if (dtype == kBF16) {                                                                           \
-    DABSN_LAUNCH(bf16, false, N, false);                                                          \
+    DABSN_LAUNCH(bf16, false, N, kRows);                                                          \
   } else if (b) {                                                                                 \
-    if (plane) DABSN_LAUNCH(float, true, N, true); else DABSN_LAUNCH(float, true, N, false);       \
+    if (plane) DABSN_LAUNCH(float, true, N, kPlanes); else DABSN_LAUNCH(float, true, N, kRows);    \
   } else {                                                                                        \
-    if (plane) DABSN_LAUNCH(float, false, N, true); else DABSN_LAUNCH(float, false, N, false);     \
+    if (plane) DABSN_LAUNCH(float, false, N, kPlanes); else DABSN_LAUNCH(float, false, N, kRows);  \
   }
   DABSN_BY_THREADS(DABSN_ROWS);
 #undef DABSN_ROWS
@@ -1224,7 +1311,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                       const void* bias, int64_t top, int value_dtype, const void* values,
                       const int64_t* tokens, int64_t ignore_index, float temperature,
                       const float* teacher_lse, float* loss, float* coef, float* weights,
-                      const float* scale, void* out, int64_t ldo, int64_t plane, uint32_t* err,
+                      const float* scale, int half, void* out, int64_t ldo, uint32_t* err,
                       hipStream_t stream) {
   int rc = distill_checks("distillation", dtype, rows, V, ldl, top, temperature);
   if (rc != DABSN_OK) return rc;
@@ -1234,7 +1321,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                 "distillation: the rest of more than %d words is not supported (V=%lld)",
                 kMaxRestVocab, (long long)V);
   DABSN_REQUIRE(!bias || dtype == kF32, "distillation: a bias goes with fp32 logits");
-  DABSN_REQUIRE(!out || (ldo >= V && (plane == 0 || (dtype == kF32 && plane >= rows * ldo)) && scale),
+  DABSN_REQUIRE(!out || (ldo >= V && (half ? dtype == kF32 : scale && !bias)),
                 "distillation: bad gradient rows");
   if (rows == 0) return DABSN_OK;
   DABSN_REQUIRE(logits && values && tokens && loss && err, "distillation: null pointer");
@@ -1243,40 +1330,39 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
   const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 7 + 31) / 32);
-#define DABSN_LAUNCH(E, BIAS, N, NV, REST, GRAD, PLANES)                                          \
-  hipLaunchKernelGGL((distill_kernel<E, BIAS, N, NV, REST, GRAD, PLANES>), grid, dim3(N), 4 * words, \
+#define DABSN_LAUNCH(E, BIAS, N, NV, REST, GRAD, KIND)                                            \
+  hipLaunchKernelGGL((distill_kernel<E, BIAS, N, NV, REST, GRAD, KIND>), grid, dim3(N), 4 * words,  \
                      stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype,  \
                      values, tokens, ignore_index, scale_t, teacher_lse, words, loss, coef, weights, \
-                     scale, out, ldo, plane, err)
-#define DABSN_REST(E, BIAS, N, NV, GRAD, PLANES)                    \
-  if (teacher_lse) DABSN_LAUNCH(E, BIAS, N, NV, true, GRAD, PLANES); \
-  else DABSN_LAUNCH(E, BIAS, N, NV, false, GRAD, PLANES)
+                     scale, out, ldo, err)
+#define DABSN_REST(E, BIAS, N, NV, GRAD, KIND)                    \
+  if (teacher_lse) DABSN_LAUNCH(E, BIAS, N, NV, true, GRAD, KIND); \
+  else DABSN_LAUNCH(E, BIAS, N, NV, false, GRAD, KIND)
 #define DABSN_ROWS(N)                                                                        \
   if (dtype == kBF16) {                                                                      \
-    if (out) { DABSN_REST(bf16, false, N, 0, true, false); }                                 \
-    else { DABSN_REST(bf16, false, N, 0, false, false); }                                    \
+    if (out) { DABSN_REST(bf16, false, N, 0, true, kRows); }                                 \
+    else { DABSN_REST(bf16, false, N, 0, false, kRows); }                                    \
   } else if (!out) {                                                                         \
-    if (b) { DABSN_REST(float, true, N, 0, false, false); }                                  \
-    else { DABSN_REST(float, false, N, 0, false, false); }                                   \
-  } else if (plane) {                                                                        \
-    if (b) { DABSN_REST(float, true, N, 0, true, true); }                                    \
-    else { DABSN_REST(float, false, N, 0, true, true); }                                     \
+    if (b) { DABSN_REST(float, true, N, 0, false, kRows); }                                  \
+    else { DABSN_REST(float, false, N, 0, false, kRows); }                                   \
+  } else if (half) {                                                                         \
+    if (b) { DABSN_REST(float, true, N, 0, true, kHalf); }                                   \
+    else { DABSN_REST(float, false, N, 0, true, kHalf); }                                    \
   } else {                                                                                   \
-    if (b) { DABSN_REST(float, true, N, 0, true, false); }                                   \
-    else { DABSN_REST(float, false, N, 0, true, false); }                                    \
+    DABSN_REST(float, false, N, 0, true, kRows);                                             \
   }
   // Held rows: 64 registers a thread, so that four waves share a SIMD.
-  const bool hold = out && !plane && !b && V > 1024;
+  const bool hold = out && !half && V > 1024;
   const int64_t nv = V / (dtype == kBF16 ? 8 : 4);
   if (hold && dtype == kBF16 && nv <= 512 * 16) {
-    if (nv <= 256 * 8) { DABSN_REST(bf16, false, 256, 8, true, false); }
-    else if (nv <= 256 * 16) { DABSN_REST(bf16, false, 256, 16, true, false); }
-    else { DABSN_REST(bf16, false, 512, 16, true, false); }
+    if (nv <= 256 * 8) { DABSN_REST(bf16, false, 256, 8, true, kRows); }
+    else if (nv <= 256 * 16) { DABSN_REST(bf16, false, 256, 16, true, kRows); }
+    else { DABSN_REST(bf16, false, 512, 16, true, kRows); }
   } else if (hold && dtype == kF32 && nv <= 1024 * 16) {
-    if (nv <= 256 * 8) { DABSN_REST(float, false, 256, 8, true, false); }
-    else if (nv <= 256 * 16) { DABSN_REST(float, false, 256, 16, true, false); }
-    else if (nv <= 512 * 16) { DABSN_REST(float, false, 512, 16, true, false); }
-    else { DABSN_REST(float, false, 1024, 16, true, false); }
+    if (nv <= 256 * 8) { DABSN_REST(float, false, 256, 8, true, kRows); }
+    else if (nv <= 256 * 16) { DABSN_REST(float, false, 256, 16, true, kRows); }
+    else if (nv <= 512 * 16) { DABSN_REST(float, false, 512, 16, true, kRows); }
+    else { DABSN_REST(float, false, 1024, 16, true, kRows); }
   } else {
     DABSN_BY_THREADS(DABSN_ROWS);
   }
@@ -1316,34 +1402,56 @@ size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V) {
   return rows <= 0 || V <= 0 ? 0 : static_cast<size_t>((rows + kSumRows - 1) / kSumRows) * V;
 }
 
-int dabsn_hip_column_sums(int64_t rows, int64_t V, int64_t ld, const void* x, int add,
+int dabsn_hip_column_sums(int half, int64_t rows, int64_t V, int64_t ld, const void* x, int add,
                           float* partials, float* out, hipStream_t stream) {
   const int64_t parts = (rows + kSumRows - 1) / kSumRows, strips = (V + 2047) / 2048;
-  DABSN_REQUIRE(rows >= 0 && V > 0 && V < (1ll << 31) - 4096 && parts * strips < (1ll << 31) && ld >= V &&
-                    ld % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && out &&
+  DABSN_REQUIRE(rows >= 0 && V > 0 && V < (1ll << 31) - 4096 && parts * strips < (1ll << 31) &&
+                    ld >= V && ld % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && out &&
                     (rows == 0 || (x && partials)),
                 "column sums: bad arguments (rows=%lld, V=%lld, ld=%lld)", (long long)rows,
                 (long long)V, (long long)ld);
-  if (rows > 0)
-    hipLaunchKernelGGL(column_sums_kernel,
-                       dim3(static_cast<unsigned>(strips * parts)), dim3(256), 0, stream, rows, (int)V, ld, static_cast<const bf16*>(x), partials);
+  const dim3 grid(static_cast<unsigned>(strips * parts));
+  if (rows > 0 && half)
+    hipLaunchKernelGGL((column_sums_kernel<true>), grid, dim3(256), 0, stream, rows, (int)V, ld,
+                       static_cast<const uint16_t*>(x), partials);
+  else if (rows > 0)
+    hipLaunchKernelGGL((column_sums_kernel<false>), grid, dim3(256), 0, stream, rows, (int)V, ld,
+                       static_cast<const uint16_t*>(x), partials);
   hipLaunchKernelGGL(add_parts_kernel, dim3(static_cast<unsigned>((V + 255) / 256)), dim3(256), 0,
                      stream, parts, (int)V, partials, add, out);
   DABSN_HIP_CHECK(hipGetLastError());
   return DABSN_OK;
 }
 
-int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* scale, void* out,
-                     hipStream_t stream) {
-  DABSN_REQUIRE((dtype == kF32 || dtype == kBF16) && n >= 0 && (n == 0 || (x && scale && out)),
+int dabsn_hip_half_copy(int64_t n, const void* x, uint32_t* word, void* out, float* inverse,
+                        hipStream_t stream) {
+  DABSN_REQUIRE(n >= 0 && word && inverse && (n == 0 || (x && out)) &&
+                    reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(out) % 16 == 0,
+                "half copy: bad arguments");
+  const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((n + 2047) / 2048, 2048))));
+  hipLaunchKernelGGL(clear_word_kernel, dim3(1), dim3(1), 0, stream, word);
+  hipLaunchKernelGGL(largest_kernel, grid, dim3(256), 0, stream, n, static_cast<const bf16*>(x), word);
+  hipLaunchKernelGGL(half_copy_kernel, grid, dim3(256), 0, stream, n, static_cast<const bf16*>(x),
+                     word, static_cast<_Float16*>(out), inverse);
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+float dabsn_hip_distill_half_scale(void) { return kHalfScale; }
+
+int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* s0, const float* s1,
+                     const float* s2, float factor, void* out, hipStream_t stream) {
+  DABSN_REQUIRE((dtype == kF32 || dtype == kBF16) && n >= 0 && (n == 0 || (x && out)),
                 "scaled copy: bad arguments");
   if (n == 0) return DABSN_OK;
+  const Factors g{{s0, s1, s2}, factor};
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + 2047) / 2048, 1 << 16)));
   if (dtype == kBF16)
-    hipLaunchKernelGGL((scaled_kernel<bf16>), grid, dim3(256), 0, stream, n, x, scale,
+    hipLaunchKernelGGL((scaled_kernel<bf16>), grid, dim3(256), 0, stream, n, x, g,
                        static_cast<bf16*>(out));
   else
-    hipLaunchKernelGGL((scaled_kernel<float>), grid, dim3(256), 0, stream, n, x, scale,
+    hipLaunchKernelGGL((scaled_kernel<float>), grid, dim3(256), 0, stream, n, x, g,
                        static_cast<float*>(out));
   DABSN_HIP_CHECK(hipGetLastError());
   return DABSN_OK;

@@ -47,14 +47,14 @@ _FUSED_LOGITS = 1 << 24
 _FUSED_WORDS = (4096, 65536)
 
 
-def _rows(x, bias, values, tokens, lse, ignore, t, s, loss, coef, weights, scale, out, ldo, plane,
+def _rows(x, bias, values, tokens, lse, ignore, t, s, loss, coef, weights, scale, half, out, ldo,
           word, stream):
     rows, V = x.shape
     tk = ops.KernelTimer.begin("distill", x)
     _lib.check(_lib.load().dabsn_hip_distill(
         ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), ops._p(bias),
         tokens.shape[1], ops._code(values.dtype), vocab.at(values, s), vocab.at(tokens, s), ignore, t,
-        vocab.at(lse, s), loss, coef, weights, scale, out, ldo, plane, word.word.data_ptr(), stream),
+        vocab.at(lse, s), loss, coef, weights, scale, half, out, ldo, word.word.data_ptr(), stream),
         _WHAT)
     ops.KernelTimer.end(tk)
 
@@ -87,8 +87,8 @@ class _FromLogits(torch.autograd.Function):
             if fused:
                 _counted(values, tokens, ignore, V, loss, t, weight, factor, stream)
                 ready = torch.empty((n, V), device=dev, dtype=x.dtype)
-            _rows(x, None, values, tokens, lse, ignore, t, 0, loss, coef, weights, factor,
-                  None if ready is None else ready.data_ptr(), V, 0, word, stream)
+            _rows(x, None, values, tokens, lse, ignore, t, 0, loss, coef, weights, factor, False,
+                  None if ready is None else ready.data_ptr(), V, word, stream)
             _lib.check(lib.dabsn_hip_distill_mean(n, loss, t, weight, mean.data_ptr(),
                                                   None if fused else factor, stream), _WHAT)
             word.check(_WHAT)
@@ -142,22 +142,25 @@ class _Linear(torch.autograd.Function):
             loss, factor = aux.data_ptr(), aux.data_ptr() + 8 * n
             mean = torch.empty((), device=dev, dtype=torch.float32)
 
-            def rows(x, s, scale, out, ldo, plane):
+            def rows(x, s, scale, out, ldo):
                 _rows(x, r.row_bias, values, tokens, lse, ignore, t, s, loss + 8 * s, None, None,
-                      scale, out, ldo, plane, word, stream)
+                      scale, r.half, out, ldo, word, stream)
 
             if any(need):
                 _counted(values, tokens, ignore, r.V, loss, t, share, factor, stream)
-                acc = vocab.ReadoutGrads(r, need, chunk)
+                acc = vocab.ReadoutGrads(r, need, chunk, half=True)
                 for g0, g1 in acc.groups():
                     acc.begin(g0, g1)
                     for s in range(g0, g1, acc.chunk):
-                        rows(r.logits(s, min(g1, s + acc.chunk)), s, factor, *acc.rows(s))
+                        rows(r.logits(s, min(g1, s + acc.chunk)), s, factor, acc.rows(s), acc.ldo)
                     acc.end()
-                ctx.save_for_backward(*acc.results())
+                # fp16 rows lack the factor T / counted rows, which would take them out of range.
+                own = aux[2 * n:] if r.half else None
+                ctx.save_for_backward(*acc.results(), own, *acc.scales)
+                ctx.factor = acc.factor
             else:
                 for s in range(0, n, chunk):
-                    rows(r.logits(s, min(n, s + chunk)), s, None, None, 0, 0)
+                    rows(r.logits(s, min(n, s + chunk)), s, None, None, 0)
             word.check(_WHAT)
             _lib.check(_lib.load().dabsn_hip_distill_mean(n, loss, t, share, mean.data_ptr(), None,
                                                           stream), _WHAT)
@@ -168,8 +171,10 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         g = g.to(torch.float32)
+        gh, gw, gb, own, *scales = ctx.saved_tensors
         with vocab.on(g):
-            grads = [vocab.scaled(x, g, ctx.dtype) for x in ctx.saved_tensors]
+            grads = [vocab.scaled(x, ctx.dtype, ctx.factor, g, own, s)
+                     for x, s in zip((gh, gw, gb), scales)]
         return (*grads, None, None, None, None, None, None, None)
 
 
@@ -217,8 +222,8 @@ def distillation_from_logits(logits: Tensor, top_logits: Tensor, top_indices: Te
     is formed with the loss (and takes their memory from then on): give a share of a mixed
     objective, or one over the micro-batches, as ``loss_weight``; an upstream factor other than 1 forms
     it again. A listed token outside [0, V)
-    other than ``ignore_index`` makes the loss NaN and sets the error word that
-    ``kernels.check_errors()`` raises (``DABSN_HIP_ERROR_CHECK=sync``: raised here)."""
+    other than ``ignore_index``, or a ``teacher_lse`` that is not the row's (weights of more than
+    256 in sum), makes the loss NaN and sets the error word that ``kernels.check_errors()`` raises (``DABSN_HIP_ERROR_CHECK=sync``: raised here)."""
     vocab.need_float(_WHAT, "logits", logits)
     if logits.dim() < 2:
         raise ValueError(f"{_WHAT}: expected logits [..., V] of one row or more")
@@ -236,7 +241,7 @@ def chunked_linear_distillation(hidden: Tensor, weight: Tensor, bias: Tensor | N
                                 ignore_index: int = -100, loss_weight: float = 1.0,
                                 chunk_budget: int | None = None) -> Tensor:
     """``distillation_from_logits(F.linear(hidden, weight, bias), ...)`` in chunks of
-    ``chunk_budget // V`` rows (``DABSN_LOSS_CHUNK_SCORES``, default 2**24 elements), the logits
+    ``chunk_budget // V`` rows (``DABSN_LOSS_CHUNK_SCORES``, default 2**25 elements), the logits
     in fp32 whatever the type of ``hidden`` [..., H]. Where a gradient is needed it is formed
     with the loss, chunk by chunk, and held in fp32 until the backward, which scales it and
     rounds it once to the inputs' types."""

@@ -22,8 +22,10 @@ from . import ops
 MAX_TOP = 128
 MAX_REST_VOCAB = 480_000
 MAX_VOCAB = (1 << 31) - 4097
-_CHUNK_BUDGET = 1 << 24
-_TOKEN_ERROR = "a token lies outside [0, V) and is not ignore_index"
+_CHUNK_BUDGET = 1 << 25
+_GROUP_LOGITS = 1 << 28
+_TOKEN_ERROR = ("a token lies outside [0, V) and is not ignore_index, or a teacher_lse is not its "
+                "row's")
 _HERE = contextlib.nullcontext()
 
 
@@ -121,17 +123,24 @@ class ErrorWord:
 
 
 def chunk_rows(rows: int, vocab: int, budget: int | None) -> int:
-    """Rows a chunk, so that its logits stay within the element budget of the readout loss
-    (``DABSN_LOSS_CHUNK_SCORES``, default 2**24; not positive or ``off``: all rows at once)."""
+    """Rows a chunk, so that its logits stay within the element budget (that of the readout loss if
+    one is set, ``DABSN_LOSS_CHUNK_SCORES``, else 2**25; not positive or ``off``: all rows at once):
+    chunks of equal height, of whole tiles of 128 rows where they allow it. The default is twice the
+    loss's: 128 MB of fp32 logits, which the row kernel still finds in the memory-side cache, and
+    products of 1024 rows by 32000 words (4096 rows scored in 548 us; 580 with 2**24 and 2**26)."""
     if budget is None:
         env = os.environ.get("DABSN_LOSS_CHUNK_SCORES", "")
         try:
             budget = int(env) if env else _CHUNK_BUDGET
         except ValueError:
             budget = 0 if env.lower() == "off" else _CHUNK_BUDGET
+    rows = max(rows, 1)
     if budget <= 0:
-        return max(rows, 1)
-    return max(1, min(max(rows, 1), int(budget) // max(1, vocab)))
+        return rows
+    most = max(1, min(rows, int(budget) // max(1, vocab)))
+    even = -(-rows // -(-rows // most))
+    tiles = -(-even // 128) * 128
+    return tiles if tiles <= most else even
 
 
 class Readout:
@@ -177,83 +186,123 @@ def need_readout(what: str, hidden: Tensor, weight: Tensor, bias: Tensor | None)
     return hidden, weight.contiguous(), None if bias is None else bias.contiguous()
 
 
+def half_copy(x: Tensor) -> tuple[Tensor, Tensor]:
+    """bf16 ``x`` as fp16 times a power of two (see ``dabsn_hip_half_copy``), and its inverse."""
+    if x.data_ptr() % 16:
+        x = x.clone()
+    out = torch.empty(x.shape, device=x.device, dtype=torch.float16)
+    aux = torch.empty(2, device=x.device, dtype=torch.float32)
+    _lib.check(_lib.load().dabsn_hip_half_copy(x.numel(), x.data_ptr(), aux.data_ptr(),
+                                               out.data_ptr(), aux.data_ptr() + 4, stream(x)),
+               "half copy")
+    return out, aux[1]
+
+
 class ReadoutGrads:
     """Gradients of a ``Readout`` from gradient rows of its logits, in fp32: the row kernel
-    writes rows where ``rows`` says, and ``done`` adds their products.
+    writes rows where ``rows`` says, and ``end`` adds the products of a group of chunks (a product
+    of few rows reaches a fifth of the rate: 524 rows x 32000 x 2048 243 TFLOP/s, 8192 rows 1356).
 
-    fp32 readouts: fp32 rows and products. bf16 ones: two bf16 planes that hold 17 bits of each
-    value, stacked as twice the rows of one bf16 product with fp32 sums; several chunks share a
-    product, as many rows as the hidden width (the planes then take no more than the weight's fp32
-    gradient): a product of few rows reaches a fifth of the rate (524 rows x 32000 x 2048: 243
-    TFLOP/s, 8192 rows: 1356)."""
+    fp32 readouts: fp32 rows and products, a chunk a group. bf16 ones:
+      planes  two bf16 rows that hold 17 bits of each value, stacked as twice the rows of one bf16
+              product; as many rows as the hidden width (the planes then take no more than the
+              weight's fp32 gradient)
+      half    one fp16 row of values of known size, and fp16 copies of the hidden rows and the
+              weight that hold all of their bits, times powers of two; up to 2**28 values
+    """
 
-    def __init__(self, r: Readout, need, chunk: int):
+    def __init__(self, r: Readout, need, chunk: int, half: bool = False):
         self.r, self.need = r, need
         n, V, H, dev = int(r.hidden.shape[0]), r.V, r.H, r.hidden.device
         f32 = torch.float32
-        self.hidden = torch.empty((n, H), device=dev, dtype=f32) if need[0] else None
-        self.weight = None
+        self.kind = "fp32" if not r.half else "half" if half else "planes"
+        self.hidden = self.weight = None
         self.bias = torch.zeros(V, device=dev, dtype=f32) if need[2] else None
         self.ldo = -(-V // 8) * 8 if r.half else V
-        # The products' copies (two fp32 rows and two bf16 rows of H a row) stay within the
-        # weight's fp32 gradient or 512 MB.
-        fit = max(1, max(4 * V * H, 1 << 29) // (12 * H))
-        self.chunk = max(1, min(chunk, n, fit)) if n else 1
-        self.group = min(n, self.chunk * max(1, min(fit, H) // self.chunk)) if r.half else self.chunk
-        shape = (2, self.group, self.ldo) if r.half else (self.group, V)
-        self.buf = torch.empty(shape, device=dev, dtype=r.hidden.dtype) if n else None
+        # Device scalars that the three results have to be multiplied by, besides `factor`.
+        self.scales: list[Tensor | None] = [None, None, None]
+        self.factor = 1.0
+        if self.kind == "planes":
+            # The products' copies (two fp32 rows and two bf16 rows of H a row) stay within the
+            # weight's fp32 gradient or 512 MB.
+            fit = max(1, max(4 * V * H, 1 << 29) // (12 * H))
+            self.chunk = max(1, min(chunk, n, fit))
+            self.group = self.chunk * max(1, min(fit, H) // self.chunk)
+        elif self.kind == "half":
+            self.chunk = chunk
+            self.group = chunk * max(1, _GROUP_LOGITS // (self.ldo * chunk))
+            self.factor = 1.0 / _lib.load().dabsn_hip_distill_half_scale()
+            if need[0] and n:
+                self.half_weight, self.scales[0] = half_copy(r.weight)
+            if need[1] and n:
+                self.half_hidden, self.scales[1] = half_copy(r.hidden)
+        else:
+            self.chunk = self.group = chunk
+        self.group = max(1, min(n, self.group))
+        if need[0] and (self.kind != "half" or self.group < n or n == 0):
+            self.hidden = torch.empty((n, H), device=dev, dtype=f32)
+        dtype = torch.float16 if self.kind == "half" else r.hidden.dtype
+        planes = 2 if self.kind == "planes" else 1
+        self.buf = torch.empty(planes * self.group * self.ldo, device=dev, dtype=dtype)
         self.first = True
 
     def groups(self):
         n = int(self.r.hidden.shape[0])
-        return [(s, min(n, s + self.group)) for s in range(0, n, max(self.group, 1))]
+        return [(s, min(n, s + self.group)) for s in range(0, n, self.group)]
 
     def begin(self, g0: int, g1: int) -> None:
         self.g0, self.g1 = g0, g1
-        if g1 - g0 < self.group:  # the last, shorter group: planes of its own height
-            m = g1 - g0
-            self.buf = (self.buf.reshape(-1)[:2 * m * self.ldo].reshape(2, m, self.ldo)
-                        if self.r.half else self.buf[:m])
 
-    def rows(self, s: int):
-        """(pointer, row stride, plane stride) of the gradient rows from row s on."""
-        if self.r.half:
-            return self.buf[0, s - self.g0].data_ptr(), self.ldo, (self.g1 - self.g0) * self.ldo
-        return self.buf[s - self.g0].data_ptr(), self.ldo, 0
+    def rows(self, s: int) -> int:
+        """Pointer to the gradient rows from row s on; their stride is ``ldo`` and the planes'
+        ``plane()``."""
+        return self.buf.data_ptr() + (s - self.g0) * self.ldo * self.buf.element_size()
+
+    def plane(self) -> int:
+        return (self.g1 - self.g0) * self.ldo if self.kind == "planes" else 0
 
     def end(self) -> None:
         r, m, f32 = self.r, self.g1 - self.g0, torch.float32
         rows = r.hidden[self.g0:self.g1]
-        if not r.half:
-            d = self.buf
-            if self.need[0]:
+        high = 2 * m if self.kind == "planes" else m
+        d = self.buf[:high * self.ldo].view(high, self.ldo)[:, :r.V]
+        if self.need[0]:
+            if self.kind == "fp32":
                 torch.mm(d, r.weight, out=self.hidden[self.g0:self.g1])
-            if self.need[1]:
+            elif self.kind == "half":
+                p = torch.mm(d, self.half_weight, out_dtype=f32)
+                if self.hidden is None:
+                    self.hidden = p
+                else:
+                    self.hidden[self.g0:self.g1] = p
+                del p
+            else:
+                p = torch.mm(d, r.weight, out_dtype=f32)
+                torch.add(p[:m], p[m:], out=self.hidden[self.g0:self.g1])
+                del p
+        if self.need[1]:
+            if self.kind == "half":
+                rows = self.half_hidden[self.g0:self.g1]
+            elif self.kind == "planes":
+                rows = torch.cat((rows, rows))
+            if self.kind == "fp32":
                 self.weight = (torch.mm(d.t(), rows) if self.first
                                else self.weight.addmm_(d.t(), rows))
-            if self.need[2]:
-                self.bias += d.sum(dim=0)
-            self.first = False
-            return
-        d = self.buf.view(2 * m, self.ldo)[:, :r.V]
-        if self.need[0]:
-            p = torch.mm(d, r.weight, out_dtype=f32)
-            torch.add(p[:m], p[m:], out=self.hidden[self.g0:self.g1])
-            del p
-        if self.need[1]:
-            both = torch.cat((rows, rows))
-            if self.first:
-                self.weight = torch.mm(d.t(), both, out_dtype=f32)
+            elif self.first:
+                self.weight = torch.mm(d.t(), rows, out_dtype=f32)
             else:
-                torch.addmm(self.weight, d.t(), both, out_dtype=f32, out=self.weight)
-            del both
+                torch.addmm(self.weight, d.t(), rows, out_dtype=f32, out=self.weight)
+            del rows
         if self.need[2]:
-            lib = _lib.load()
-            part = torch.empty(lib.dabsn_hip_column_sums_partials(2 * m, r.V), device=d.device,
-                               dtype=f32)
-            _lib.check(lib.dabsn_hip_column_sums(2 * m, r.V, self.ldo, self.buf.data_ptr(), 1,
-                                                 part.data_ptr(), self.bias.data_ptr(),
-                                                 stream(d)), "readout bias gradient")
+            if self.kind == "fp32":
+                self.bias += d.sum(dim=0)
+            else:
+                lib = _lib.load()
+                part = torch.empty(lib.dabsn_hip_column_sums_partials(high, r.V), device=d.device,
+                                   dtype=f32)
+                _lib.check(lib.dabsn_hip_column_sums(
+                    self.kind == "half", high, r.V, self.ldo, self.buf.data_ptr(), 1,
+                    part.data_ptr(), self.bias.data_ptr(), stream(d)), "readout bias gradient")
         self.first = False
 
     def results(self):
@@ -264,11 +313,12 @@ class ReadoutGrads:
         return self.hidden, self.weight, self.bias
 
 
-def scaled(x: Tensor | None, g: Tensor, like: torch.dtype) -> Tensor | None:
-    """fp32 ``x`` times the device scalar g, rounded once to ``like``."""
+def scaled(x: Tensor | None, like: torch.dtype, factor: float, *scales: Tensor | None) -> Tensor | None:
+    """fp32 ``x`` times ``factor`` and up to three device scalars, rounded once to ``like``."""
     if x is None:
         return None
     out = torch.empty(x.shape, device=x.device, dtype=like)
-    _lib.check(_lib.load().dabsn_hip_scaled(ops._code(like), x.numel(), x.data_ptr(), g.data_ptr(),
+    p = [ops._p(s) for s in scales] + [None] * (3 - len(scales))
+    _lib.check(_lib.load().dabsn_hip_scaled(ops._code(like), x.numel(), x.data_ptr(), *p, factor,
                                             out.data_ptr(), stream(x)), "scaled gradient")
     return out

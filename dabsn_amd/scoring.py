@@ -142,7 +142,7 @@ class _LinearTokenLogprobs(torch.autograd.Function):
                 for s in range(g0, g1, acc.chunk):
                     x = r.logits(s, min(g1, s + acc.chunk))
                     _backward(x, r.row_bias, targets, *ctx.args, (st, ent, ti), grads, s,
-                              *acc.rows(s))
+                              acc.rows(s), acc.ldo, acc.plane())
                     del x
                 acc.end()
             gh, gw, gb = acc.results()
@@ -196,7 +196,7 @@ def chunked_linear_token_logprobs(hidden: Tensor, weight: Tensor, bias: Tensor |
                                   temperature: float = 1.0, ignore_index: int = -100,
                                   chunk_budget: int | None = None) -> TokenLogprobs:
     """``token_logprobs(F.linear(hidden, weight, bias), targets, ...)`` in chunks of
-    ``chunk_budget // V`` rows (``DABSN_LOSS_CHUNK_SCORES``, default 2**24 elements), the logits
+    ``chunk_budget // V`` rows (``DABSN_LOSS_CHUNK_SCORES``, default 2**25 elements), the logits
     in fp32 whatever the type of ``hidden`` [..., H]. The backward forms each chunk's logits
     again and adds the gradient products in fp32, rounded once to the inputs' types."""
     shape = hidden.shape[:-1]

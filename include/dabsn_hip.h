@@ -702,17 +702,21 @@ int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t str
  * log-sum-exp of the teacher's whole row / temperature; V <= 480000), exp(values / temperature -
  * teacher_lse) with the rest q_r = 1 - sum q on all other tokens as one event. loss [rows][2] =
  * (KL(q || softmax(z)), 1 if the row has a listed token, else 0). coef [rows][4] and weights
- * [rows][top] (NULL: none) are for _bwd. With out the gradient rows are written too,
- * times scale[0], in the logits' type or (fp32 logits) as two planes as above. A listed token outside [0, V) sets *err to 1 and its row to NaN.
+ * [rows][top] (NULL: none) are for _bwd. With out the gradient rows (stride ldo) are written too:
+ * in the logits' type times scale[0] (no bias), or with `half` (fp32 logits) as fp16 times
+ * dabsn_hip_distill_half_scale(). A row whose weights sum to more than 256 (a teacher_lse that is
+ * not the row's) counts as one with a token out of range. A listed token outside [0, V) sets *err to 1 and its row to NaN.
  * dabsn_hip_distill_rows: loss = (0, 1 or 0) without logits. dabsn_hip_distill_mean: mean[0] =
  * weight * temperature^2 * mean loss over the counted rows, factor[0] = weight * temperature / their
  * number (each may be NULL). dabsn_hip_distill_bwd: dlogits [rows, V] = d mean[0] / d logits * grad[0], given
  * scale = factor; with `done` dlogits holds the rows for grad[0] = 1 already and the call writes
  * only for another factor. A token listed several times has the sum of its weights.
  *
- * dabsn_hip_column_sums: out [V] (added to with `add`) = column sums of bf16 rows x (stride ld,
- * a multiple of 8), through partials [dabsn_hip_column_sums_partials]. dabsn_hip_scaled: out[i] =
- * x[i] * scale[0], rounded once to dtype. */
+ * dabsn_hip_column_sums: out [V] (added to with `add`) = column sums of bf16 or fp16 (`half`) rows
+ * x (stride ld, a multiple of 8), through partials [dabsn_hip_column_sums_partials].
+ * dabsn_hip_half_copy: fp16 out = bf16 x times a power of two that takes the largest magnitude to
+ * [2^14, 2^15); inverse = 1 / that power, word: scratch. dabsn_hip_scaled: out[i] = x[i] * factor *
+ * s0[0] * s1[0] * s2[0] (NULL: 1), rounded once to dtype. */
 int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                              const void* bias, const int64_t* targets, int64_t ignore_index,
                              float temperature, int64_t top, float* logprob, float* entropy,
@@ -734,17 +738,20 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                       const void* bias, int64_t top, int value_dtype, const void* values,
                       const int64_t* tokens, int64_t ignore_index, float temperature,
                       const float* teacher_lse, float* loss, float* coef, float* weights,
-                      const float* scale, void* out, int64_t ldo, int64_t plane, uint32_t* err,
+                      const float* scale, int half, void* out, int64_t ldo, uint32_t* err,
                       hipStream_t stream);
 int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                           int64_t top, const int64_t* tokens, float temperature, const float* coef,
                           const float* weights, const float* scale, const float* grad, int done,
                           void* dlogits, hipStream_t stream);
 size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V);
-int dabsn_hip_column_sums(int64_t rows, int64_t V, int64_t ld, const void* x, int add,
+int dabsn_hip_column_sums(int half, int64_t rows, int64_t V, int64_t ld, const void* x, int add,
                           float* partials, float* out, hipStream_t stream);
-int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* scale, void* out,
-                     hipStream_t stream);
+int dabsn_hip_half_copy(int64_t n, const void* x, uint32_t* word, void* out, float* inverse,
+                        hipStream_t stream);
+float dabsn_hip_distill_half_scale(void);
+int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* s0, const float* s1,
+                     const float* s2, float factor, void* out, hipStream_t stream);
 
 /* ---- scaled token embedding ---------------------------------------------------------
  * New operator for the language model's embedding (src/dabsn/model.py:804-860 has

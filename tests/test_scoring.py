@@ -75,8 +75,9 @@ def test_library_refuses_bad_arguments_before_it_launches():
         None)
     for kw in (dict(ldo=4), dict(plane=9), dict(dtype=1, plane=16), dict(top=6)):
         assert bwd(**kw) == -2, kw
-    assert lib.dabsn_hip_column_sums(4, 10, 12, one, 0, one, one, None) == -2  # stride not of 8
-    assert lib.dabsn_hip_scaled(3, 4, one, one, one, None) == -2
+    assert lib.dabsn_hip_column_sums(0, 4, 10, 12, one, 0, one, one, None) == -2  # stride not of 8
+    assert lib.dabsn_hip_scaled(3, 4, one, one, None, None, 1.0, one, None) == -2
+    assert lib.dabsn_hip_half_copy(4, one + 2, one, one, one, None) == -2  # not aligned
 
 
 # ---- the definition in 64 bits ---------------------------------------------------------------
