@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(256) place_kernel(int64_t n, int64_t V, int64_
                                                     const uint32_t* __restrict__ pos,
                                                     const uint32_t* __restrict__ counts,
                                                     uint32_t* __restrict__ keys_out,
-                                                    uint32_t* __restrict__ pos_out) {
+                                                    uint32_t* __restrict__ pos_out,
+                                                    uint32_t* __restrict__ starts) {
   __shared__ uint32_t at[4][1 << kMaxBits];
   __shared__ uint32_t total[1 << kMaxBits];
   __shared__ uint32_t waves[4];
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(256) place_kernel(int64_t n, int64_t V, int64_
   for (int w = 0; w < wave; ++w) start += waves[w];
   for (int b = b0; b < min(b0 + run, bins); ++b) {
     at[0][b] += start;
+    if (starts && blockIdx.x == 0 && b <= V) starts[b] = start;  // the only pass: digits are words
     start += total[b];
   }
   // The waves' quarters of the tile: counts of the quarters before a wave's own.
@@ -570,18 +572,20 @@ static void launch_bwd(const Plan& p, int64_t n, int64_t V, int H, const int64_t
       hipLaunchKernelGGL((digits_kernel<true>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
                          shift, p.bits, ids, nullptr, counts);
       hipLaunchKernelGGL((place_kernel<true>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
-                         shift, p.bits, p.tiles, ids, nullptr, nullptr, counts, ka, pa);
+                         shift, p.bits, p.tiles, ids, nullptr, nullptr, counts, ka, pa,
+                         p.passes == 1 ? starts : nullptr);
     } else {
       hipLaunchKernelGGL((digits_kernel<false>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
                          shift, p.bits, ids, kb, counts);
       hipLaunchKernelGGL((place_kernel<false>), grid, dim3(256), 0, stream, n, V, padding, p.tile,
-                         shift, p.bits, p.tiles, ids, kb, pb, counts, ka, pa);
+                         shift, p.bits, p.tiles, ids, kb, pb, counts, ka, pa, nullptr);
     }
     std::swap(ka, kb);
     std::swap(pa, pb);
   }
-  hipLaunchKernelGGL(starts_kernel, dim3(static_cast<unsigned>(V / 256 + 1)), dim3(256), 0, stream,
-                     static_cast<uint32_t>(n), static_cast<uint32_t>(V), keys, starts);
+  if (p.passes != 1)
+    hipLaunchKernelGGL(starts_kernel, dim3(static_cast<unsigned>(V / 256 + 1)), dim3(256), 0, stream,
+                       static_cast<uint32_t>(n), static_cast<uint32_t>(V), keys, starts);
   const int64_t tasks = p.pieces * strips;
   hipLaunchKernelGGL((pieces_kernel<E>), dim3(static_cast<unsigned>((tasks + 3) / 4)), dim3(256), 0,
                      stream, H, strips, tasks, static_cast<uint32_t>(V), starts, keys, pos, grad,

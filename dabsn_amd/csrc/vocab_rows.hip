@@ -591,7 +591,8 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
   const double ln_s = n.ln_s(k.delta);
   auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (threadIdx.x == 0) {
-    const double h = ln_s - kLn2 * n.u / n.s;
+    // The correction of ln s and that of the mean of z are the same and cancel.
+    const double h = log(static_cast<double>(n.s)) - kLn2 * n.u / n.s;
     entropy[r] = n.empty() || h < 0.0 ? 0.0f : static_cast<float>(h);
     if (stats) {
       stats[2 * r] = n.r;

@@ -27,7 +27,6 @@ import math
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernels import ops, vocab
@@ -100,7 +99,7 @@ class _FromLogits(torch.autograd.Function):
         return mean
 
     @staticmethod
-    @once_differentiable
+    @vocab.once
     def backward(ctx, g):
         x, tokens, aux = ctx.saved_tensors
         (n, V), K = x.shape, tokens.shape[1]
@@ -168,7 +167,7 @@ class _Linear(torch.autograd.Function):
         return mean
 
     @staticmethod
-    @once_differentiable
+    @vocab.once
     def backward(ctx, g):
         g = g.to(torch.float32)
         gh, gw, gb, own, *scales = ctx.saved_tensors

@@ -11,7 +11,6 @@ import math
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernels import ops, vocab
@@ -42,7 +41,7 @@ class _ScaledEmbedding(torch.autograd.Function):
         return _lookup(ids, weight, scale)
 
     @staticmethod
-    @once_differentiable
+    @vocab.once
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
         (V, H), dtype, scale, padding = ctx.args

@@ -46,6 +46,20 @@ def at(t: Tensor | None, s: int) -> int | None:
     return t.data_ptr() + s * t.stride(0) * t.element_size() if s else t.data_ptr()
 
 
+def once(backward):
+    """A Function's backward that refuses to be differentiated itself. (``once_differentiable``
+    takes a gradient whose upstream needs none for a constant, though it depends on the inputs, and
+    costs 4 us of a small call's 25.)"""
+
+    def run(ctx, *grads):
+        if torch.is_grad_enabled():  # create_graph=True
+            raise RuntimeError("DABSN HIP operators of the vocabulary have no second derivative: "
+                               "run the backward without create_graph")
+        return backward(ctx, *grads)
+
+    return run
+
+
 def need_device(what: str, *tensors: Tensor | None) -> None:
     """All tensors on one ROCm device."""
     first = None

@@ -25,7 +25,6 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernels import ops, vocab
@@ -97,7 +96,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp, ent, tl, ti
 
     @staticmethod
-    @once_differentiable
+    @vocab.once
     def backward(ctx, gl, ge, gt, _):
         x, targets, st, ent, ti = ctx.saved_tensors
         grads = vocab.grads_of(gl), vocab.grads_of(ge), vocab.grads_of(gt)
@@ -130,7 +129,7 @@ class _LinearTokenLogprobs(torch.autograd.Function):
         return lp, ent, tl, ti
 
     @staticmethod
-    @once_differentiable
+    @vocab.once
     def backward(ctx, gl, ge, gt, _):
         hidden, weight, bias, targets, st, ent, ti = ctx.saved_tensors
         grads = vocab.grads_of(gl), vocab.grads_of(ge), vocab.grads_of(gt)

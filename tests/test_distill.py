@@ -228,6 +228,28 @@ def test_masked_students(cuda_device, dtype):
 
 
 @pytest.mark.gpu
+def test_the_rest_of_the_largest_vocabulary(cuda_device):
+    x, values, tokens, lse = case(2, 2, 480_000, 30, torch.bfloat16, True)
+    tokens[0, 0], tokens[1, 0] = 479_999, 0
+    check(*run(x, values, tokens, lse), reference(x, values, tokens, 1.0, lse), torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_gradients_formed_with_the_loss_of_strided_rows(cuda_device):
+    """Rows of a wider tensor, whose gradient rows lie at other addresses modulo a line."""
+    wide = torch.randn(2100, 8200, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    base = (wide * 2.5).requires_grad_(True)
+    values, tokens = base.detach()[:, 5:8196].topk(9, dim=1)
+    loss = distillation_from_logits(base[:, 5:8196], values, tokens)
+    (g,) = torch.autograd.grad(loss, base)
+    dense = base.detach()[:, 5:8196].contiguous().requires_grad_(True)
+    (want,) = torch.autograd.grad(distillation_from_logits(dense, values, tokens), dense)
+    # the same terms in other groups: the softmax's sums differ by their roundings
+    assert float((g[:, 5:8196] - want).abs().max()) <= 4 * sum_error(8191) * U * float(want.abs().max())
+    assert float(g[:, :5].abs().max()) == 0 == float(g[:, 8196:].abs().max())
+
+
+@pytest.mark.gpu
 def test_only_padding_and_no_rows(cuda_device):
     x, values, tokens, lse = case(3, 5, 40, 6, torch.float32, True)
     tokens.fill_(-100)

@@ -217,6 +217,30 @@ def test_strides_shapes_and_index_types(cuda_device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1e-6, 0.013, 37.0, 1e6])
+def test_temperatures_from_end_to_end(cuda_device, T):
+    """Forward and gradients; at 1e-6 a row is its largest logit (two equal ones share it)."""
+    x, t = logits_of(4, 6, 2050, torch.float32)
+    x[0, 7] = x[0, 1900] = 20.0
+    t[1] = 7
+    check_forward(token_logprobs(x, t, top=5, temperature=T), x, t, 5, T)
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t, top=5, temperature=T)
+    g = torch.rand(6, generator=torch.Generator().manual_seed(1)).cuda()
+    (got,) = torch.autograd.grad((r.logprobs, r.entropy), leaf, (g, g))
+    want, F, points = reference_grad(x, t, 0, T, g, g, None)
+    check_grad(got, want, F, points, 2050, torch.float32)
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_gradient_is_refused(cuda_device):
+    x, t = logits_of(4, 3, 50, torch.float32)
+    leaf = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(token_logprobs(leaf, t).logprobs.sum(), leaf, create_graph=True)
+
+
+@pytest.mark.gpu
 def test_rows_past_32_bit_offsets(cuda_device):
     """2,200 rows of a million bf16 words: 4.4 GB, so element offsets pass 2^31 and byte offsets
     2^32; the last rows against the definition."""
@@ -271,7 +295,10 @@ def reference_grad(x, targets, top, T, gl, ge, gt, ignore=-100):
         size = size + d(gt).abs().sum(1)
     if gl is not None:
         size = size + d(gl).abs()
-    F = p * (size[:, None] + h.abs() * (lq.abs() + ent[:, None] + 1)) / T
+    # Exponentials below 2^-126 are 0, so p may lack that much: it enters F by as much as check_grad
+    # multiplies F by at least, u 328, leaves of it; |logp| <= 104 there.
+    factor = size[:, None] + h.abs() * (lq.abs().clamp(max=104) + ent[:, None] + 1)
+    F = (p + 2.0 ** -126 / (328 * U)) * factor / T
     live = (p.sum(1) > 0)[:, None]
     return torch.where(live, (dense + points) / T, 0.0), F, points.abs() / T
 
