@@ -133,7 +133,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, values, tokens, lse, ignore, t, share, chunk):
         n, dev = int(hidden.shape[0]), hidden.device
         need = ctx.needs_input_grad[:3]
-        with vocab.on(hidden), torch.autocast("cuda", enabled=False):
+        with vocab.on(hidden), vocab.no_autocast():
             stream = vocab.stream(hidden)
             r = vocab.Readout(hidden, weight, bias)
             word = vocab.ErrorWord(dev)

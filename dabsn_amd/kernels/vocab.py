@@ -34,6 +34,11 @@ def on(t: Tensor):
     return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def no_autocast():
+    """Products in the operands' own types (the context costs 5 us, so only where one is on)."""
+    return torch.autocast("cuda", enabled=False) if torch.is_autocast_enabled("cuda") else _HERE
+
+
 def stream(t: Tensor) -> int:
     """The current stream's handle on the device of ``t``."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
@@ -230,8 +235,7 @@ class ReadoutGrads:
         n, V, H, dev = int(r.hidden.shape[0]), r.V, r.H, r.hidden.device
         f32 = torch.float32
         self.kind = "fp32" if not r.half else "half" if half else "planes"
-        self.hidden = self.weight = None
-        self.bias = torch.zeros(V, device=dev, dtype=f32) if need[2] else None
+        self.hidden = self.weight = self.bias = None
         self.ldo = -(-V // 8) * 8 if r.half else V
         # Device scalars that the three results have to be multiplied by, besides `factor`.
         self.scales: list[Tensor | None] = [None, None, None]
@@ -309,21 +313,25 @@ class ReadoutGrads:
             del rows
         if self.need[2]:
             if self.kind == "fp32":
-                self.bias += d.sum(dim=0)
+                self.bias = d.sum(dim=0) if self.first else self.bias.add_(d.sum(dim=0))
             else:
                 lib = _lib.load()
+                if self.first:
+                    self.bias = torch.empty(r.V, device=d.device, dtype=f32)
                 part = torch.empty(lib.dabsn_hip_column_sums_partials(high, r.V), device=d.device,
                                    dtype=f32)
                 _lib.check(lib.dabsn_hip_column_sums(
-                    self.kind == "half", high, r.V, self.ldo, self.buf.data_ptr(), 1,
+                    self.kind == "half", high, r.V, self.ldo, self.buf.data_ptr(), not self.first,
                     part.data_ptr(), self.bias.data_ptr(), stream(d)), "readout bias gradient")
         self.first = False
 
     def results(self):
         """(hidden, weight, bias) gradients in fp32, None where not needed."""
-        if self.need[1] and self.weight is None:
-            self.weight = torch.zeros((self.r.V, self.r.H), device=self.r.hidden.device,
-                                      dtype=torch.float32)
+        r = self.r
+        if self.first:  # no rows
+            zeros = lambda *s: torch.zeros(s, device=r.hidden.device, dtype=torch.float32)  # noqa: E731
+            self.weight = zeros(r.V, r.H) if self.need[1] else None
+            self.bias = zeros(r.V) if self.need[2] else None
         return self.hidden, self.weight, self.bias
 
 

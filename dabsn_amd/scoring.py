@@ -111,7 +111,7 @@ class _LinearTokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, targets, ignore, temperature, top, chunk, stats):
         n = int(hidden.shape[0])
-        with vocab.on(hidden), torch.autocast("cuda", enabled=False):
+        with vocab.on(hidden), vocab.no_autocast():
             r = vocab.Readout(hidden, weight, bias)
             word = vocab.ErrorWord(hidden.device)
             outs = _outputs(n, top, hidden.device, targets is not None, stats)
@@ -133,7 +133,7 @@ class _LinearTokenLogprobs(torch.autograd.Function):
     def backward(ctx, gl, ge, gt, _):
         hidden, weight, bias, targets, st, ent, ti = ctx.saved_tensors
         grads = vocab.grads_of(gl), vocab.grads_of(ge), vocab.grads_of(gt)
-        with vocab.on(hidden), torch.autocast("cuda", enabled=False):
+        with vocab.on(hidden), vocab.no_autocast():
             r = vocab.Readout(hidden, weight, bias)
             acc = vocab.ReadoutGrads(r, ctx.needs_input_grad[:3], ctx.chunk)
             for g0, g1 in acc.groups():
