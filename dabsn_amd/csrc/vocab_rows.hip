@@ -330,10 +330,17 @@ struct Norm {
     else f([r = r, c](float x) { return Share<false>::arg(x, r, c); });
   }
   __device__ __forceinline__ bool empty() const { return s == 0.0f; }  // no finite logit
-  // ln s, corrected for the rounding of c (log2 e / T = c (1 + delta)).
+  // What ln s lacks for the rounding of c (log2 e / T = c (1 + delta)).
+  __device__ __forceinline__ double correction(double delta) const {
+    return kLn2 * delta * (static_cast<double>(u) / s + (safe ? 0.0 : static_cast<double>(r)));
+  }
   __device__ __forceinline__ double ln_s(double delta) const {
-    const double mean = static_cast<double>(u) / s + (safe ? 0.0 : static_cast<double>(r));
-    return log(static_cast<double>(s)) + kLn2 * delta * mean;
+    return log(static_cast<double>(s)) + correction(delta);
+  }
+  // The correction of ln s and that of the mean of z are the same and cancel.
+  __device__ __forceinline__ float entropy(double log_s) const {
+    const double h = log_s - kLn2 * u / s;
+    return empty() || h < 0.0 ? 0.0f : static_cast<float>(h);
   }
   // log p of a logit x.
   __device__ __forceinline__ double logp(float x, double inv_t, double ln_s) const {
@@ -588,12 +595,10 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
         if constexpr (TOP) best.see(vm, c);
       },
       [&](int, float x) { outside = fmaxf(outside, x); });
-  const double ln_s = n.ln_s(k.delta);
+  const double log_s = log(static_cast<double>(n.s)), ln_s = log_s + n.correction(k.delta);
   auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (threadIdx.x == 0) {
-    // The correction of ln s and that of the mean of z are the same and cancel.
-    const double h = log(static_cast<double>(n.s)) - kLn2 * n.u / n.s;
-    entropy[r] = n.empty() || h < 0.0 ? 0.0f : static_cast<float>(h);
+    entropy[r] = n.entropy(log_s);
     if (stats) {
       stats[2 * r] = n.r;
       stats[2 * r + 1] = n.safe ? -n.s : n.s;
@@ -980,6 +985,352 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
                     RowOut<E>{out + r * V, row.head});
 }
 
+// ---- rows of few words ---------------------------------------------------------------------
+// Vocabularies of up to kNarrow words (tens of them in character and group workloads): 16 lanes
+// take a row, NV values a lane in registers, 16 rows a block. What a row costs beside its logits
+// (reductions of 4 lane exchanges, the teacher's exponentials, the logarithms) is shared by the
+// four rows of a wave, and each lane finds its words in the row's list, in the list's order. A
+// wave a row, as above, took %NARROW%.
+constexpr int kNarrow = 128;
+
+template <typename Op>
+__device__ __forceinline__ float reduce16(float v, Op op) {
+  v = op(v, dpp_mov<0xB1, 0xF>(v, v));   // quad_perm [1,0,3,2]
+  v = op(v, dpp_mov<0x4E, 0xF>(v, v));   // quad_perm [2,3,0,1]
+  v = op(v, dpp_mov<0x141, 0xF>(v, v));  // row_half_mirror
+  return op(v, dpp_mov<0x140, 0xF>(v, v));  // row_mirror
+}
+__device__ __forceinline__ float sum16(float v) {
+  return reduce16(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float max16(float v) {
+  return reduce16(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_mov_d(double x) {
+  uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xF, 0xF, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xF, 0xF, false);
+  u = static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo);
+  return __builtin_bit_cast(double, u);
+}
+template <typename Op>
+__device__ __forceinline__ double reduce16_d(double v, Op op) {
+  v = op(v, dpp_mov_d<0xB1>(v));
+  v = op(v, dpp_mov_d<0x4E>(v));
+  v = op(v, dpp_mov_d<0x141>(v));
+  return op(v, dpp_mov_d<0x140>(v));
+}
+__device__ __forceinline__ double sum16_d(double v) {
+  return reduce16_d(v, [](double a, double b) { return a + b; });
+}
+
+// A lane's values of its row, words lane, lane + 16, ...; -inf behind the last.
+template <typename E, int NV>
+struct Narrow {
+  int lane;
+  size_t r;
+  bool live;
+  float x[NV];
+  __device__ __forceinline__ Narrow(int64_t rows, int V, int64_t ldl, const E* logits,
+                                    const bf16* bias) {
+    lane = threadIdx.x & 15;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+    live = row < rows;
+    r = static_cast<size_t>(live ? row : rows - 1);  // all lanes take part in the exchanges
+    const E* p = logits + r * ldl;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = lane + 16 * i;
+      x[i] = j < V ? ld(p, j) + (bias ? bf2f(bias[j]) : 0.0f) : -INFINITY;
+    }
+  }
+  // The exponentials (in place of the values), their sums relative to the row's largest logit.
+  __device__ __forceinline__ Norm norm(float c, float (&e)[NV]) const {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
+    m = fmaxf(max16(m), kLowest);
+    float s = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float a = Share<true>::arg(x[i], m, c);
+      e[i] = __builtin_amdgcn_exp2f(a);
+      s += e[i];
+      u = __builtin_fmaf(e[i], fmaxf(a, -1e30f), u);
+    }
+    return Norm{m, sum16(s), sum16(u), 0.0f, true};
+  }
+};
+
+template <typename E, int NV>
+__global__ void __launch_bounds__(256) logprobs_narrow_kernel(
+    int64_t rows, int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
+    const int64_t* __restrict__ targets, int64_t ignore, Scale k, int K,
+    float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ stats,
+    float* __restrict__ top_lp, int64_t* __restrict__ top_idx, uint32_t* err) {
+  __shared__ __attribute__((aligned(16))) uint32_t keys[16][16 * NV];
+  const Narrow<E, NV> w(rows, V, ldl, logits, bias);
+  float e[NV];
+  const Norm n = w.norm(k.c, e);
+  const double log_s = log(static_cast<double>(n.s)), ln_s = log_s + n.correction(k.delta);
+  auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
+  if (w.live && w.lane == 0) {
+    entropy[w.r] = n.entropy(log_s);
+    if (stats) {
+      stats[2 * w.r] = n.r;
+      stats[2 * w.r + 1] = -n.s;
+    }
+  }
+  if (logprob) {
+    const int64_t t = targets[w.r];
+    const bool inside = t >= 0 && t < V && t != ignore;
+    if (w.live && w.lane == 0 && !inside) {
+      if (t != ignore) atomicOr(err, kErrToken);
+      logprob[w.r] = t == ignore ? 0.0f : NAN;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (w.live && inside && t == w.lane + 16 * i) logprob[w.r] = lp(w.x[i]);
+  }
+  if (K == 0) return;
+  // A word's place is the number of words before it: of larger logits, or equal and earlier.
+  uint32_t mine[NV];
+  int rank[NV];
+  const int g = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = w.lane + 16 * i;
+    mine[i] = j < V ? key_of(w.x[i]) : 0;  // below every word's
+    rank[i] = 0;
+    keys[g][j] = mine[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < NV; ++h) {  // words 16 h .. 16 h + 15, all before or behind the others' own
+    if (16 * h >= V) break;
+#pragma unroll
+    for (int j0 = 0; j0 < 16; j0 += 4) {
+      const u32x4 four = *reinterpret_cast<const u32x4*>(&keys[g][16 * h + j0]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t key = four[q];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (h < i) rank[i] += key >= mine[i];
+          else if (h > i) rank[i] += key > mine[i];
+          else rank[i] += key + (j0 + q < w.lane) > mine[i];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = w.lane + 16 * i;
+    if (w.live && j < V && rank[i] < K) {
+      const float x = w.x[i] > -INFINITY ? w.x[i] : -INFINITY;
+      top_lp[w.r * K + rank[i]] = lp(x);
+      top_idx[w.r * K + rank[i]] = j;
+    }
+  }
+}
+
+template <typename E, int NV, int KIND>
+__global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
+    int64_t rows, int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
+    const int64_t* __restrict__ targets, int64_t ignore, Scale k, int K,
+    const int64_t* __restrict__ top_idx, const float* __restrict__ stats,
+    const float* __restrict__ entropy, const float* __restrict__ g_lp,
+    const float* __restrict__ g_ent, const float* __restrict__ g_top, void* out, int64_t ldo,
+    int64_t plane) {
+  const Narrow<E, NV> w(rows, V, ldl, logits, bias);
+  const float inv_t = static_cast<float>(k.inv_t);
+  const Norm n{stats[2 * w.r], fabsf(stats[2 * w.r + 1]), 0.0f, 0.0f, stats[2 * w.r + 1] < 0.0f};
+  const int64_t t = targets && g_lp ? targets[w.r] : ignore;
+  const bool off = t != ignore && (t < 0 || t >= V), aim = t != ignore && !off;
+  const float gl = aim ? g_lp[w.r] * inv_t : 0.0f;
+  float point[NV];
+  float sum = gl;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) point[i] = aim && t == w.lane + 16 * i ? gl : 0.0f;
+  if (g_top) {
+    for (int q = 0; q < K; ++q) {
+      const float g = g_top[w.r * K + q] * inv_t;
+      const int64_t j = top_idx[w.r * K + q];
+      sum += g;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) point[i] += j == w.lane + 16 * i ? g : 0.0f;
+    }
+  }
+  const float ge = g_ent ? g_ent[w.r] * inv_t : 0.0f;
+  const float is = n.empty() ? 0.0f : 1.0f / n.s;
+  const float lns = n.empty() ? 0.0f : logf(n.s);
+  const float A = off ? NAN : -(sum + ge * (entropy[w.r] - lns)) * is;
+  const float B = -ge * static_cast<float>(kLn2) * is;
+  const auto o = out_row<E, KIND>(out, w.r, ldo, plane, 0);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = w.lane + 16 * i;
+    const float a = n.safe ? Share<true>::arg(w.x[i], n.r, k.c) : Share<false>::arg(w.x[i], n.r, k.c);
+    const float d = __builtin_amdgcn_exp2f(a) * __builtin_fmaf(B, fmaxf(a, -1e30f), A);
+    if (w.live && j < V) o.put(static_cast<int64_t>(j), n.empty() ? (off ? NAN : 0.0f) : d + point[i]);
+  }
+}
+
+// The list of a row: its words and weights, in shared memory.
+struct NarrowList {
+  int idx[kMaxTop];  // -1: absent
+  float q[kMaxTop];
+};
+// Which of a lane's words are listed, and with what weights in sum.
+template <int NV>
+__device__ __forceinline__ void listed16(const NarrowList& l, int K, int lane, bool (&hit)[NV],
+                                         float (&q)[NV]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    hit[i] = false;
+    q[i] = 0.0f;
+  }
+  for (int k = 0; k < K; ++k) {
+    const int j = l.idx[k];
+    const float w = l.q[k];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const bool same = j == lane + 16 * i;
+      hit[i] = hit[i] || same;
+      q[i] += same ? w : 0.0f;
+    }
+  }
+}
+
+template <typename E, int NV, bool REST>
+__global__ void __launch_bounds__(256) distill_narrow_kernel(
+    int64_t rows, int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
+    int K, int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
+    int64_t ignore, Scale sc, const float* __restrict__ teacher_lse, float* __restrict__ loss,
+    float* __restrict__ coef, float* __restrict__ weights, uint32_t* err) {
+  __shared__ NarrowList lists[16];
+  __shared__ float xs[16][16 * NV];
+  const Narrow<E, NV> w(rows, V, ldl, logits, bias);
+  const int g = threadIdx.x >> 4;
+  NarrowList& l = lists[g];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) xs[g][w.lane + 16 * i] = w.x[i];
+  // The row's entries lane, lane + 16, ...: the largest value, then the weights.
+  float top = -INFINITY;
+  float flags = 0.0f;  // 1: an entry, 1024: one out of range
+  for (int k = w.lane; k < K; k += 16) {
+    const int64_t at = tokens[w.r * K + k];
+    const float v = value_type == kBF16 ? ld(static_cast<const bf16*>(values), w.r * K + k)
+                                        : ld(static_cast<const float*>(values), w.r * K + k);
+    int j = -1;
+    if (at != ignore) {
+      if (at < 0 || at >= V) {
+        flags += 1024.0f;
+      } else if (v != -INFINITY) {
+        j = static_cast<int>(at);
+        flags += 1.0f;
+        top = fmaxf(top, v);
+      }
+    }
+    l.idx[k] = j;
+    l.q[k] = v;
+  }
+  flags = sum16(flags);
+  top = max16(top);
+  float e[NV];
+  Norm n = w.norm(sc.c, e);
+  double norm;
+  if constexpr (REST) {
+    norm = teacher_lse[w.r];
+  } else {
+    double all = 0.0;
+    for (int k = w.lane; k < K; k += 16)
+      if (l.idx[k] >= 0) all += exp((static_cast<double>(l.q[k]) - top) * sc.inv_t);
+    norm = top * sc.inv_t + log(sum16_d(all));
+  }
+  __syncthreads();  // xs
+  const double ln_s = n.ln_s(sc.delta);
+  double part = 0.0, total = 0.0;
+  for (int k = w.lane; k < K; k += 16) {
+    const int j = l.idx[k];
+    float q32 = -1.0f;
+    if (j >= 0) {
+      const double logq = l.q[k] * sc.inv_t - norm, q = exp(logq);
+      if (q != 0.0) part += q * (logq - n.logp(xs[g][j], sc.inv_t, ln_s));
+      total += q;
+      q32 = n.empty() ? 0.0f : static_cast<float>(q);  // no finite logit: no gradient
+    }
+    l.q[k] = q32;
+    if (weights && w.live) weights[w.r * K + k] = q32;
+  }
+  part = sum16_d(part);
+  total = sum16_d(total);
+  const bool wrong = flags >= 1024.0f || total > kMostWeight, some = flags > 0.0f;
+  double rest = 0.0;
+  if constexpr (REST) {
+    __syncthreads();  // the list
+    bool hit[NV];
+    float q[NV];
+    listed16<NV>(l, K, w.lane, hit, q);
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) off += hit[i] ? 0.0f : e[i];
+    n.rest = sum16(off);
+    rest = 1.0 - total;
+    rest = rest > 0.0 && n.rest != 0.0f ? rest : 0.0;
+    if (rest != 0.0) part += rest * (log(rest) - log(static_cast<double>(n.rest)) + ln_s);
+    total += rest;
+  }
+  if (!w.live || w.lane != 0) return;
+  float b = n.empty() ? 0.0f : static_cast<float>(total / n.s), a = b;
+  if (REST && rest != 0.0) a = static_cast<float>(total / n.s - rest / n.rest);
+  if (!some) a = b = 0.0f, part = 0.0;
+  if (wrong) {
+    a = b = NAN, part = NAN;
+    atomicOr(err, kErrToken);
+  }
+  loss[2 * w.r] = static_cast<float>(part);
+  loss[2 * w.r + 1] = some || wrong ? 1.0f : 0.0f;
+  if (coef) {
+    coef[4 * w.r] = n.r;
+    coef[4 * w.r + 1] = a;
+    coef[4 * w.r + 2] = b;
+    coef[4 * w.r + 3] = 2.0f;  // differences first; the list's order serves words listed twice
+  }
+}
+
+template <typename E, int NV>
+__global__ void __launch_bounds__(256) distill_narrow_bwd_kernel(
+    int64_t rows, int V, int64_t ldl, const E* __restrict__ logits, int K,
+    const int64_t* __restrict__ tokens, float c, const float* __restrict__ coef,
+    const float* __restrict__ weights, const float* __restrict__ scale,
+    const float* __restrict__ grad, E* __restrict__ out) {
+  __shared__ NarrowList lists[16];
+  const Narrow<E, NV> w(rows, V, ldl, logits, nullptr);
+  NarrowList& l = lists[threadIdx.x >> 4];
+  for (int k = w.lane; k < K; k += 16) {
+    const float q = weights[w.r * K + k];
+    l.q[k] = q;
+    l.idx[k] = q < 0.0f ? -1 : static_cast<int>(tokens[w.r * K + k]);
+  }
+  __syncthreads();
+  bool hit[NV];
+  float q[NV];
+  listed16<NV>(l, K, w.lane, hit, q);
+  const float r = coef[4 * w.r], a = coef[4 * w.r + 1], b = coef[4 * w.r + 2];
+  const bool safe = (static_cast<int>(coef[4 * w.r + 3]) & 2) != 0;
+  const float sc = scale[0] * grad[0];
+  if (!w.live) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = w.lane + 16 * i;
+    const float arg = safe ? Share<true>::arg(w.x[i], r, c) : Share<false>::arg(w.x[i], r, c);
+    const float e = __builtin_amdgcn_exp2f(arg);
+    if (j < V) st(out, w.r * V + j, hit[i] ? e * (b * sc) - q[i] * sc : e * (a * sc));
+  }
+}
+
 // mean = weight T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = weight T / that count;
 // the sums in 64 bits and a fixed order, one block.
 __global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, const float* __restrict__ loss,
@@ -988,10 +1339,12 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, const 
                                                             float* __restrict__ factor) {
   __shared__ double sh[2][16];
   double l = 0.0, n = 0.0;
-#pragma unroll 4
+  const float2* pairs = reinterpret_cast<const float2*>(loss);
+#pragma unroll 16
   for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-    l += loss[2 * r];
-    n += loss[2 * r + 1];
+    const float2 p = pairs[r];
+    l += p.x;
+    n += p.y;
   }
   l = wave_sum_d(l);
   n = wave_sum_d(n);
@@ -1213,6 +1566,21 @@ int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* log
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
+  if (V <= kNarrow) {
+#define DABSN_NARROW(E, NV)                                                                        \
+  hipLaunchKernelGGL((logprobs_narrow_kernel<E, NV>), dim3(static_cast<unsigned>((rows + 15) / 16)), \
+                     dim3(256), 0, stream, rows, (int)V, ldl, static_cast<const E*>(logits), b,      \
+                     targets, ignore_index, scale_t, (int)top, logprob, entropy, stats,              \
+                     top_logprobs, top_indices, err)
+    if (dtype == kBF16) {
+      if (V <= 64) DABSN_NARROW(bf16, 4); else DABSN_NARROW(bf16, 8);
+    } else {
+      if (V <= 64) DABSN_NARROW(float, 4); else DABSN_NARROW(float, 8);
+    }
+#undef DABSN_NARROW
+    DABSN_HIP_CHECK(hipGetLastError());
+    return DABSN_OK;
+  }
 #define DABSN_LAUNCH(E, BIAS, N, TOP)                                                          \
   hipLaunchKernelGGL((logprobs_kernel<E, BIAS, N, TOP>), grid, dim3(N), 0, stream, (int)V, ldl, \
                      static_cast<const E*>(logits), b, targets, ignore_index, scale_t, (int)top,  \
@@ -1253,6 +1621,24 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
+  if (V <= kNarrow) {
+#define DABSN_NARROW(E, NV, KIND)                                                                  \
+  hipLaunchKernelGGL((logprobs_narrow_bwd_kernel<E, NV, KIND>),                                    \
+                     dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, stream, rows,    \
+                     (int)V, ldl, static_cast<const E*>(logits), b, targets, ignore_index, scale_t, \
+                     (int)top, top_indices, stats, entropy, g_logprob, g_entropy, g_top, out, ldo,  \
+                     plane)
+    if (dtype == kBF16) {
+      if (V <= 64) DABSN_NARROW(bf16, 4, kRows); else DABSN_NARROW(bf16, 8, kRows);
+    } else if (plane) {
+      if (V <= 64) DABSN_NARROW(float, 4, kPlanes); else DABSN_NARROW(float, 8, kPlanes);
+    } else {
+      if (V <= 64) DABSN_NARROW(float, 4, kRows); else DABSN_NARROW(float, 8, kRows);
+    }
+#undef DABSN_NARROW
+    DABSN_HIP_CHECK(hipGetLastError());
+    return DABSN_OK;
+  }
 #define DABSN_LAUNCH(E, BIAS, N, KIND)                                                           \
   hipLaunchKernelGGL((logprobs_bwd_kernel<E, BIAS, N, KIND>), grid, dim3(N), 0, stream, (int)V, \
                      ldl, static_cast<const E*>(logits), b, targets, ignore_index, scale_t,         \
@@ -1331,6 +1717,24 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
   const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 7 + 31) / 32);
+  if (V <= kNarrow && !out) {
+#define DABSN_NARROW(E, NV, REST)                                                                  \
+  hipLaunchKernelGGL((distill_narrow_kernel<E, NV, REST>),                                         \
+                     dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, stream, rows,    \
+                     (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype, values,  \
+                     tokens, ignore_index, scale_t, teacher_lse, loss, coef, weights, err)
+#define DABSN_NV(E, REST) \
+  if (V <= 64) DABSN_NARROW(E, 4, REST); else DABSN_NARROW(E, 8, REST)
+    if (dtype == kBF16) {
+      if (teacher_lse) { DABSN_NV(bf16, true); } else { DABSN_NV(bf16, false); }
+    } else {
+      if (teacher_lse) { DABSN_NV(float, true); } else { DABSN_NV(float, false); }
+    }
+#undef DABSN_NV
+#undef DABSN_NARROW
+    DABSN_HIP_CHECK(hipGetLastError());
+    return DABSN_OK;
+  }
 #define DABSN_LAUNCH(E, BIAS, N, NV, REST, GRAD, KIND)                                            \
   hipLaunchKernelGGL((distill_kernel<E, BIAS, N, NV, REST, GRAD, KIND>), grid, dim3(N), 4 * words,  \
                      stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype,  \
@@ -1386,6 +1790,21 @@ int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
+  if (V <= kNarrow) {
+#define DABSN_NARROW(E, NV)                                                                        \
+  hipLaunchKernelGGL((distill_narrow_bwd_kernel<E, NV>),                                           \
+                     dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, stream, rows,    \
+                     (int)V, ldl, static_cast<const E*>(logits), (int)top, tokens, scale_t.c, coef, \
+                     weights, scale, grad, static_cast<E*>(dlogits))
+    if (dtype == kBF16) {
+      if (V <= 64) DABSN_NARROW(bf16, 4); else DABSN_NARROW(bf16, 8);
+    } else {
+      if (V <= 64) DABSN_NARROW(float, 4); else DABSN_NARROW(float, 8);
+    }
+#undef DABSN_NARROW
+    DABSN_HIP_CHECK(hipGetLastError());
+    return DABSN_OK;
+  }
 #define DABSN_LAUNCH(E, N)                                                                       \
   hipLaunchKernelGGL((distill_bwd_kernel<E, N>), grid, dim3(N), 0, stream, (int)V, ldl,           \
                      static_cast<const E*>(logits), (int)top, tokens, scale_t.c, coef, weights, scale, \

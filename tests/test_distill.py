@@ -160,7 +160,8 @@ def run(x, values, tokens, lse, T=1.0, up=1.0):
     return loss, g / up if up != 1.0 else g
 
 
-SIZES = [(1, 1, 1), (3, 2, 2), (5, 7, 3), (600, 65, 8), (9, 1024, 128), (9, 1025, 128), (4, 1031, 1),
+SIZES = [(1, 1, 1), (3, 2, 2), (5, 7, 3), (33, 60, 8), (18, 64, 64), (600, 65, 8), (19, 128, 128), (19, 129, 20),
+         (9, 300, 17), (9, 1024, 128), (9, 1025, 128), (4, 1031, 1),
          (5, 2049, 64), (3, 4099, 33), (2, 9001, 65), (1, 32000, 64), (2, 50021, 37)]
 
 
@@ -177,7 +178,7 @@ def test_loss_and_gradient_match_the_definition(cuda_device, rows, V, K, rest, d
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rest", [False, True])
-@pytest.mark.parametrize("V,K", [(50, 20), (1031, 128), (9001, 40)])
+@pytest.mark.parametrize("V,K", [(50, 20), (128, 128), (200, 100), (1031, 128), (9001, 40)])
 def test_tokens_listed_twice_and_absent_entries(cuda_device, V, K, rest):
     """The same token at several places of a row (its weights add), in neighbouring and far
     places; entries with the value -inf; a row with one entry; rows with none."""

@@ -141,7 +141,8 @@ def logits_of(seed, rows, V, dtype, spread=3.0, device="cuda"):
     return x.to(device), t.to(device)
 
 
-SIZES = [(1, 1, 1), (3, 2, 2), (5, 7, 3), (4, 8, 8), (700, 65, 20), (9, 1024, 128), (9, 1025, 128),
+SIZES = [(1, 1, 1), (3, 2, 2), (5, 7, 3), (4, 8, 8), (17, 16, 16), (33, 60, 5), (18, 64, 64), (700, 65, 20),
+         (19, 128, 128), (19, 129, 100), (9, 1024, 128), (9, 1025, 128),
          (3, 1023, 127), (5, 2049, 5), (3, 4099, 33), (2, 8192, 1), (600, 9001, 7), (1, 32000, 5),
          (2, 50021, 128), (1, 150001, 20)]
 
@@ -158,7 +159,7 @@ def test_forward_matches_the_definition(cuda_device, rows, V, top, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [61, 1031, 9001])
+@pytest.mark.parametrize("V", [61, 127, 300, 1031, 9001])
 def test_masks_infinities_and_equal_logits(cuda_device, V, dtype):
     """Rows: most words ruled out by -inf, by the type's lowest value; only one word left; none
     left; all at the lowest; all equal; two levels (more equal logits than candidates fit);
@@ -314,7 +315,8 @@ def check_grad(got, want, F, points, V, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,V,top,T", [(1, 1, 1, 1.0), (5, 7, 3, 0.7), (600, 65, 20, 1.0),
+@pytest.mark.parametrize("rows,V,top,T", [(1, 1, 1, 1.0), (5, 7, 3, 0.7), (33, 60, 5, 1.0), (600, 65, 20, 1.0), (20, 128, 128, 3.0),
+                                          (20, 200, 9, 1.0),
                                           (4, 1031, 128, 2.0), (3, 4099, 33, 1.0), (2, 9001, 5, 0.5),
                                           (1, 50021, 2, 1.0)])
 def test_gradients_match_the_formula(cuda_device, rows, V, top, T, dtype):
@@ -410,6 +412,7 @@ def logit_error(h, w, b):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,H,V,budget,bias", [(1, 3, 5, None, True), (70, 48, 33, 16 * 33, True),
+                                               (90, 24, 128, None, False), (50, 24, 200, None, True),
                                                (300, 200, 1001, 40 * 1001, False),
                                                (130, 72, 4099, 1 << 18, True)])
 def test_linear_form_matches_the_definition(cuda_device, n, H, V, budget, bias, dtype):
