@@ -21,9 +21,10 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 // The W = 8 bf16 or 4 fp32 (16 bytes) of a row that a lane takes at a time, at any element alignment:
 // raw, as loaded, and as floats. ONCE: the access is marked as not to be kept in the caches, which
-// then hold what is read again (the table's rows) and are not written out for what is not: 65536
-// rows of 4096 bf16 are looked up in 94 us instead of 132, and their gradients summed in 107
-// instead of 140. Lanes take neighbouring 16 bytes, so that such accesses are whole lines.
+// then hold what is read again (the table's rows) and are not written out for what is not: each
+// called in a loop of its own, 65536 rows of 4096 bf16 are looked up in 94 us instead of 132 and
+// their gradients summed in 107 instead of 140 (called in turn with each other: 131 and 128). Lanes
+// take neighbouring 16 bytes, so that such accesses are whole lines.
 template <typename E>
 struct Vec {
   static constexpr int W = 16 / sizeof(E);

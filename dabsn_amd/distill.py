@@ -38,10 +38,11 @@ _WHAT = "distillation"
 # registers, and the backward only checks that its upstream factor is 1 (loss.backward()); another
 # factor forms it again (``loss_weight`` keeps a mixed objective's share out of it). Forward and
 # backward in two passes -> with the gradient formed ahead (and again for another factor), us:
-# 8388 x 32000 bf16 356 -> 240 (466), 16777 x 16000 368 -> 244 (480), 4129 x 65000 373 -> 234 (478),
-# 2097 x 32000 fp32 183 -> 140 (254). A row of few words is read again from the L2 cache (33554 x
-# 2000 bf16 160 -> 176), one of too many is not held in registers (2684 x 100000 373 -> 351, 591),
-# and below 2^24 logits the launches that count the rows ahead cost more than the second reading.
+# 8388 x 32000 bf16 317 -> 217 (426), 16777 x 16000 338 -> 220 (431), 4129 x 65000 320 -> 221 (435),
+# 33554 x 8000 357 -> 262 (458), 2097 x 32000 fp32 156 -> 138 (220). Rows of few words are read again
+# from the caches (33554 x 2000 bf16 160 -> 176), rows of more do not fit the registers (2684 x 100000
+# 373 -> 351, and 591 for another factor), and below 2^24 logits the launches that count the rows
+# ahead cost as much as the second reading.
 _FUSED_LOGITS = 1 << 24
 _FUSED_WORDS = (4096, 65536)
 

@@ -73,6 +73,14 @@ PRIMITIVES = (
     Primitive("local_field_gather", "inputs[:, patch]", "HIP 16-byte row gather",
               "HIP inverse-index scatter-add in the reference loop's order", ("field", "hybrid"),
               "bit-exact against the oracle gather/scatter"),
+    Primitive("token_logprobs", "none (beside runtime/loss.py:52-137)",
+              "HIP rows: one streaming pass for the softmax, entropy and alternatives",
+              "HIP rows from the saved normaliser", ("seq",), "64-bit definition"),
+    Primitive("distillation", "none (beside runtime/loss.py:52-137)",
+              "HIP rows against a teacher's listed tokens, gradient formed while a row is held",
+              "the same pass, or HIP rows from saved coefficients", ("seq",), "64-bit definition"),
+    Primitive("scaled_embedding", "none (beside model.py:804-860)", "HIP row lookup",
+              "stable HIP sort by word + ordered fp32 sums of pieces", ("seq",), "64-bit definition"),
 )
 
 _PRIMITIVE_HITS = {"permanent_delta_scan": 0, "local_field_gather": 0}
