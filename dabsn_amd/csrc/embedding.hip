@@ -505,7 +505,8 @@ struct Plan {
 static size_t up(size_t b) { return (b + 255) / 256 * 256; }
 static Plan plan_of(int64_t n, int64_t V, int64_t H) {
   Plan p{};
-  p.direct = n <= kDirectTokens && n * V <= kDirectWork;
+  // (A launch holds fewer than 2^32 threads.)
+  p.direct = n <= kDirectTokens && n * V <= kDirectWork && V * strips_of(kF32, H) < (1ll << 25);
   if (p.direct) return p;
   int need = 1;
   while ((1ll << need) <= V) ++need;  // keys 0 .. V
@@ -555,7 +556,7 @@ static void launch_bwd(const Plan& p, int64_t n, int64_t V, int H, const int64_t
   auto* counts = reinterpret_cast<uint32_t*>(ws + p.counts);
   auto* starts = reinterpret_cast<uint32_t*>(ws + p.starts);
   auto* partial = reinterpret_cast<float*>(ws + p.partial);
-  if (p.passes == 0) {
+  if (p.passes == 0 && n > 0) {
     hipLaunchKernelGGL(rank_kernel, dim3(static_cast<unsigned>((n + 63) / 64)), dim3(256), 0, stream,
                        static_cast<int>(n), V, padding, ids, keys, pos);
   }
@@ -588,9 +589,10 @@ static void launch_bwd(const Plan& p, int64_t n, int64_t V, int H, const int64_t
     hipLaunchKernelGGL(starts_kernel, dim3(static_cast<unsigned>(V / 256 + 1)), dim3(256), 0, stream,
                        static_cast<uint32_t>(n), static_cast<uint32_t>(V), keys, starts);
   const int64_t tasks = p.pieces * strips;
-  hipLaunchKernelGGL((pieces_kernel<E>), dim3(static_cast<unsigned>((tasks + 3) / 4)), dim3(256), 0,
-                     stream, H, strips, tasks, static_cast<uint32_t>(V), starts, keys, pos, grad,
-                     scale, dweight, partial);
+  if (tasks > 0)
+    hipLaunchKernelGGL((pieces_kernel<E>), dim3(static_cast<unsigned>((tasks + 3) / 4)), dim3(256), 0,
+                       stream, H, strips, tasks, static_cast<uint32_t>(V), starts, keys, pos, grad,
+                       scale, dweight, partial);
   const int log2 = lanes_log2(dtype, H);
   const int64_t blanks = ((V << log2) + 255) / 256;
   hipLaunchKernelGGL((words_kernel<E>), dim3(static_cast<unsigned>(blanks + tasks)), dim3(256), 0,
@@ -615,7 +617,7 @@ int dabsn_hip_embedding_fwd(int dtype, int64_t n, int64_t V, int64_t H, const in
   DABSN_REQUIRE(ids && weight && out && err, "embedding: null pointer");
   const int log2 = lanes_log2(dtype, H);
   const int64_t blocks = ((n << log2) + 255) / 256;
-  DABSN_REQUIRE(blocks < (1ll << 31), "embedding: %lld tokens in one call", (long long)n);
+  DABSN_REQUIRE(blocks < (1ll << 24), "embedding: %lld tokens in one call", (long long)n);
   const dim3 grid(static_cast<unsigned>(blocks));
   if (dtype == kBF16)
     hipLaunchKernelGGL((lookup_kernel<bf16>), grid, dim3(256), 0, stream, n, V, (int)H, log2, ids,
@@ -643,8 +645,7 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
   DABSN_REQUIRE(workspace_bytes >= p.bytes, "embedding backward: workspace of %zu bytes, %zu needed",
                 workspace_bytes, p.bytes);
   const int64_t strips = strips_of(dtype, H);
-  DABSN_REQUIRE(p.pieces * strips + ((V << lanes_log2(dtype, H)) + 255) / 256 < (1ll << 31) &&
-                    (!p.direct || V * strips < (1ll << 32)),
+  DABSN_REQUIRE(p.pieces * strips + ((V << lanes_log2(dtype, H)) + 255) / 256 < (1ll << 24),
                 "embedding backward: %lld x %lld values in one call", (long long)n, (long long)H);
   if (dtype == kBF16)
     launch_bwd<bf16>(p, n, V, (int)H, ids, padding_idx, static_cast<const bf16*>(grad), scale,

@@ -1335,9 +1335,37 @@ __global__ void __launch_bounds__(256) distill_narrow_bwd_kernel(
   }
 }
 
-// mean = weight T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = weight T / that count;
-// the sums in 64 bits and a fixed order, one block.
-__global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, const float* __restrict__ loss,
+// Many rows: loss[b kMeanRows] = the sums of the rows' losses and marks from there on to the next
+// one's, summed in 64 bits; the result, a mean in fp32, bears the one rounding of each. 262144 rows
+// take 9 us in both kernels, 30 in the one block below alone.
+constexpr int64_t kMeanRows = 4096;
+__global__ void __launch_bounds__(256) distill_parts_kernel(int64_t rows, float* loss) {
+  __shared__ double sh[2][4];
+  float2* pairs = reinterpret_cast<float2*>(loss) + blockIdx.x * kMeanRows;
+  const int n = static_cast<int>(min(kMeanRows, rows - blockIdx.x * kMeanRows));
+  double l = 0.0, m = 0.0;
+#pragma unroll 16
+  for (int r = threadIdx.x; r < n; r += 256) {
+    const float2 p = pairs[r];
+    l += p.x;
+    m += p.y;
+  }
+  l = wave_sum_d(l);
+  m = wave_sum_d(m);
+  if ((threadIdx.x & 63) == 0) {
+    sh[0][threadIdx.x >> 6] = l;
+    sh[1][threadIdx.x >> 6] = m;
+  }
+  __syncthreads();  // all rows have been read
+  if (threadIdx.x == 0)
+    pairs[0] = make_float2(static_cast<float>(sh[0][0] + sh[0][1] + sh[0][2] + sh[0][3]),
+                           static_cast<float>(sh[1][0] + sh[1][1] + sh[1][2] + sh[1][3]));
+}
+
+// mean = weight T^2 * sum of loss[r][0] / max(1, sum of loss[r][1]), factor = weight T / that count,
+// over the rows r = 0, step, ...; the sums in 64 bits and a fixed order, one block.
+__global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, int64_t step,
+                                                            const float* __restrict__ loss,
                                                             float t, float weight,
                                                             float* __restrict__ mean,
                                                             float* __restrict__ factor) {
@@ -1345,7 +1373,7 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, const 
   double l = 0.0, n = 0.0;
   const float2* pairs = reinterpret_cast<const float2*>(loss);
 #pragma unroll 16
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+  for (int64_t r = threadIdx.x * step; r < rows; r += 1024 * step) {
     const float2 p = pairs[r];
     l += p.x;
     n += p.y;
@@ -1536,6 +1564,27 @@ static int checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t 
 // rows than two a unit are there; else 256, of which eight rows share a unit.
 static int threads(int64_t rows, int64_t V) { return V <= 1024 ? 64 : rows < 512 && V >= 8192 ? 1024 : 256; }
 
+// A launch holds fewer than 2^32 threads: more rows than these run as launches of that many.
+constexpr int64_t kMostRows = 1 << 21;
+template <typename T>
+static T* past(T* p, int64_t n) {
+  return p ? p + n : nullptr;
+}
+static const void* past(const void* p, int dtype, int64_t n) {
+  return past(static_cast<const char*>(p), n * (dtype == kBF16 ? 2 : 4));
+}
+static void* past(void* p, int dtype, int64_t n) {
+  return past(static_cast<char*>(p), n * (dtype == kBF16 ? 2 : 4));
+}
+// launch(first row, rows) for each of them.
+template <typename F>
+static int in_launches(int64_t rows, F launch) {
+  int rc = DABSN_OK;
+  for (int64_t s = 0; s < rows && rc == DABSN_OK; s += kMostRows)
+    rc = launch(s, std::min(kMostRows, rows - s));
+  return rc;
+}
+
 }  // namespace vocab
 }  // namespace dabsn
 
@@ -1566,6 +1615,14 @@ int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* log
   DABSN_REQUIRE(logits && entropy && err && (!logprob || targets) &&
                     (top == 0 || (top_logprobs && top_indices)),
                 "token log probabilities: null pointer");
+  if (rows > kMostRows)
+    return in_launches(rows, [&](int64_t s, int64_t n) {
+      return dabsn_hip_token_logprobs(dtype, n, V, past(logits, dtype, s * ldl), ldl, bias,
+                                      past(targets, s), ignore_index, temperature, top,
+                                      past(logprob, s), past(entropy, s), past(stats, 2 * s),
+                                      past(top_logprobs, s * top), past(top_indices, s * top), err,
+                                      stream);
+    });
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
@@ -1621,6 +1678,14 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
   DABSN_REQUIRE(logits && stats && entropy && out && (!g_logprob || targets) &&
                     (!g_top || (top > 0 && top_indices)),
                 "token log probabilities backward: null pointer");
+  if (rows > kMostRows)
+    return in_launches(rows, [&](int64_t s, int64_t n) {
+      return dabsn_hip_token_logprobs_bwd(
+          dtype, n, V, past(logits, dtype, s * ldl), ldl, bias, past(targets, s), ignore_index,
+          temperature, top, past(top_indices, s * top), past(stats, 2 * s), past(entropy, s),
+          past(g_logprob, s), past(g_entropy, s), past(g_top, s * top),
+          past(out, plane ? kBF16 : dtype, s * ldo), ldo, plane, stream);
+    });
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
@@ -1681,6 +1746,11 @@ int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype
                 value_dtype);
   if (rows == 0) return DABSN_OK;
   DABSN_REQUIRE(values && tokens && loss, "distillation rows: null pointer");
+  if (rows > kMostRows)
+    return in_launches(rows, [&](int64_t s, int64_t n) {
+      return dabsn_hip_distill_rows(n, V, top, value_dtype, past(values, value_dtype, s * top),
+                                    past(tokens, s * top), ignore_index, past(loss, 2 * s), stream);
+    });
   hipLaunchKernelGGL(distill_rows_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0,
                      stream, rows, (int)V, (int)top, value_dtype, values, tokens, ignore_index,
                      loss);
@@ -1688,12 +1758,17 @@ int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype
   return DABSN_OK;
 }
 
-int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float weight,
-                           float* mean, float* factor, hipStream_t stream) {
-  DABSN_REQUIRE(rows >= 0 && (rows == 0 || loss) && (mean || factor),
+int dabsn_hip_distill_mean(int64_t rows, float* loss, float temperature, float weight, float* mean,
+                           float* factor, hipStream_t stream) {
+  DABSN_REQUIRE(rows >= 0 && rows < (1ll << 31) && (rows == 0 || loss) && (mean || factor),
                 "distillation mean: bad arguments");
-  hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, stream, rows, loss, temperature,
-                     weight, mean, factor);
+  const bool parts = rows > 4 * kMeanRows;
+  if (parts)
+    hipLaunchKernelGGL(distill_parts_kernel,
+                       dim3(static_cast<unsigned>((rows + kMeanRows - 1) / kMeanRows)), dim3(256), 0,
+                       stream, rows, loss);
+  hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, stream, rows,
+                     parts ? kMeanRows : 1, loss, temperature, weight, mean, factor);
   DABSN_HIP_CHECK(hipGetLastError());
   return DABSN_OK;
 }
@@ -1716,6 +1791,14 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                 "distillation: bad gradient rows");
   if (rows == 0) return DABSN_OK;
   DABSN_REQUIRE(logits && values && tokens && loss && err, "distillation: null pointer");
+  if (rows > kMostRows)
+    return in_launches(rows, [&](int64_t s, int64_t n) {
+      return dabsn_hip_distill(dtype, n, V, past(logits, dtype, s * ldl), ldl, bias, top, value_dtype,
+                               past(values, value_dtype, s * top), past(tokens, s * top),
+                               ignore_index, temperature, past(teacher_lse, s), past(loss, 2 * s),
+                               past(coef, 4 * s), past(weights, s * top), scale, half,
+                               past(out, half ? kBF16 : dtype, s * ldo), ldo, err, stream);
+    });
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
@@ -1791,6 +1874,13 @@ int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits
   if (rows == 0) return DABSN_OK;
   DABSN_REQUIRE(logits && tokens && coef && weights && scale && grad && dlogits,
                 "distillation backward: null pointer");
+  if (rows > kMostRows)
+    return in_launches(rows, [&](int64_t s, int64_t n) {
+      return dabsn_hip_distill_bwd(dtype, n, V, past(logits, dtype, s * ldl), ldl, top,
+                                   past(tokens, s * top), temperature, past(coef, 4 * s),
+                                   past(weights, s * top), scale, grad, done,
+                                   past(dlogits, dtype, s * V), stream);
+    });
   const int nth = threads(rows, V);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);

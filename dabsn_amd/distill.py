@@ -70,9 +70,9 @@ def _counted(values, tokens, ignore, V, loss, t, weight, factor, stream):
 
 class _FromLogits(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, values, tokens, lse, ignore, t, weight):
+    def forward(ctx, x, values, tokens, lse, ignore, t, weight, train):
         (n, V), K, dev = x.shape, tokens.shape[1], x.device
-        need, lib = ctx.needs_input_grad[0], _lib.load()
+        need, lib = train and ctx.needs_input_grad[0], _lib.load()
         fused = need and n * V >= _FUSED_LOGITS and _FUSED_WORDS[0] <= V <= _FUSED_WORDS[1]
         with vocab.on(x):
             stream = vocab.stream(x)
@@ -122,7 +122,7 @@ class _FromLogits(torch.autograd.Function):
                 ctx.t, aux_p + 8 * n, aux_p + 24 * n, aux_p + 4 * n * (6 + K), g.data_ptr(), done,
                 out.data_ptr(), vocab.stream(x)), _WHAT + " backward")
             ops.KernelTimer.end(tk)
-        return out, None, None, None, None, None, None
+        return out, None, None, None, None, None, None, None
 
 
 class _Linear(torch.autograd.Function):
@@ -131,9 +131,10 @@ class _Linear(torch.autograd.Function):
     rounds them. Forming the logits again there would be a fourth product beside the three."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, bias, values, tokens, lse, ignore, t, share, chunk):
+    def forward(ctx, hidden, weight, bias, values, tokens, lse, ignore, t, share, chunk, train):
         n, dev = int(hidden.shape[0]), hidden.device
-        need = ctx.needs_input_grad[:3]
+        # (Under no_grad needs_input_grad tells of a parameter all the same.)
+        need = [train and x for x in ctx.needs_input_grad[:3]]
         with vocab.on(hidden), vocab.no_autocast():
             stream = vocab.stream(hidden)
             r = vocab.Readout(hidden, weight, bias)
@@ -175,7 +176,7 @@ class _Linear(torch.autograd.Function):
         with vocab.on(g):
             grads = [vocab.scaled(x, ctx.dtype, ctx.factor, g, own, s)
                      for x, s in zip((gh, gw, gb), scales)]
-        return (*grads, None, None, None, None, None, None, None)
+        return (*grads, None, None, None, None, None, None, None, None)
 
 
 def _share(weight: float) -> float:
@@ -232,7 +233,7 @@ def distillation_from_logits(logits: Tensor, top_logits: Tensor, top_indices: Te
     values, tokens, lse = _lists(logits.shape[:-1], v, top_logits, top_indices, teacher_lse)
     vocab.need_device(_WHAT, logits, values, tokens, lse)
     return _FromLogits.apply(vocab.rows_of(logits), values, tokens, lse, int(ignore_index), t,
-                             _share(loss_weight))
+                             _share(loss_weight), torch.is_grad_enabled())
 
 
 def chunked_linear_distillation(hidden: Tensor, weight: Tensor, bias: Tensor | None,
@@ -251,4 +252,5 @@ def chunked_linear_distillation(hidden: Tensor, weight: Tensor, bias: Tensor | N
     values, tokens, lse = _lists(shape, int(w.shape[0]), top_logits, top_indices, teacher_lse)
     vocab.need_device(_WHAT, h, w, b, values, tokens, lse)
     chunk = vocab.chunk_rows(int(h.shape[0]), int(w.shape[0]), chunk_budget)
-    return _Linear.apply(h, w, b, values, tokens, lse, int(ignore_index), t, _share(loss_weight), chunk)
+    return _Linear.apply(h, w, b, values, tokens, lse, int(ignore_index), t, _share(loss_weight),
+                         chunk, torch.is_grad_enabled())

@@ -708,7 +708,7 @@ int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t str
  * not the row's) counts as one with a token out of range. A listed token outside [0, V) sets *err to 1 and its row to NaN.
  * dabsn_hip_distill_rows: loss = (0, 1 or 0) without logits. dabsn_hip_distill_mean: mean[0] =
  * weight * temperature^2 * mean loss over the counted rows, factor[0] = weight * temperature / their
- * number (each may be NULL). dabsn_hip_distill_bwd: dlogits [rows, V] = d mean[0] / d logits * grad[0], given
+ * number (each may be NULL); loss is scratch to it. dabsn_hip_distill_bwd: dlogits [rows, V] = d mean[0] / d logits * grad[0], given
  * scale = factor; with `done` dlogits holds the rows for grad[0] = 1 already and the call writes
  * only for another factor. A token listed several times has the sum of its weights.
  *
@@ -732,8 +732,8 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
 int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype,
                            const void* values, const int64_t* tokens, int64_t ignore_index,
                            float* loss, hipStream_t stream);
-int dabsn_hip_distill_mean(int64_t rows, const float* loss, float temperature, float weight,
-                           float* mean, float* factor, hipStream_t stream);
+int dabsn_hip_distill_mean(int64_t rows, float* loss, float temperature, float weight, float* mean,
+                           float* factor, hipStream_t stream);
 int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                       const void* bias, int64_t top, int value_dtype, const void* values,
                       const int64_t* tokens, int64_t ignore_index, float temperature,

@@ -332,7 +332,12 @@ def test_gradients_formed_with_the_loss(cuda_device, n, V, K, dtype):
         (gb,) = torch.autograd.grad(loss, leaf)
         assert torch.equal(gb, g1)
         with torch.no_grad():
-            assert torch.equal(distillation_from_logits(leaf, values, tokens, teacher_lse=rest), loss)
+            plain = distillation_from_logits(leaf, values, tokens, teacher_lse=rest)
+        # Without a gradient the rows' sums are of other groups: ln s and the rest's logarithm
+        # differ by at most 2 S U each, both times weights of at most 1 in sum; rows and mean are
+        # rounded once in each.
+        off = abs(float(plain) - float(loss.detach()))
+        assert off <= U * (4 * sum_error(V) + 8 * (1 + abs(float(loss.detach()))))
         part = None if rest is None else rest[:8]
         _, grad, _, tol = reference(x[:8], values[:8], tokens[:8], 1.0, part)
         counted = int((tokens != -100).any(1).sum())
@@ -378,6 +383,63 @@ def test_loss_weight(cuda_device):
     part = chunked_linear_distillation(h, w, b, values, tokens, teacher_lse=lse, loss_weight=0.25)
     assert torch.equal(one / 4, part)
     assert torch.equal(torch.autograd.grad(one, h)[0] / 4, torch.autograd.grad(part, h)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+def test_many_rows(cuda_device, rest):
+    """Rows whose losses are summed by many workgroups, the last of them one row long."""
+    rows = 5 * 4096 + 1
+    x, values, tokens, lse = case(3, rows, 9, 3, torch.float32, rest)
+    check(*run(x, values, tokens, lse), reference(x, values, tokens, 1.0, lse), torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 130])
+def test_rows_of_several_launches(cuda_device, V):
+    """More rows than one launch takes: the gradient rows are those of its two parts (times their
+    counts), and the mean that of their means. Each part's mean is off by U of itself (its last
+    rounding) and U (those of its partial sums, all of one sign), the whole's as well."""
+    rows, cut, K = (1 << 21) + 21, 1 << 21, 2
+    g = torch.Generator(device=cuda_device).manual_seed(V)
+    x = torch.randn(rows, V, generator=g, device=cuda_device).to(torch.bfloat16)
+    values = torch.randn(rows, K, generator=g, device=cuda_device)
+    tokens = torch.randint(0, V, (rows, K), generator=g, device=cuda_device)
+    loss, grad = run(x, values, tokens, None)
+    head, gh = run(x[:cut], values[:cut], tokens[:cut], None)
+    tail, gt = run(x[cut:], values[cut:], tokens[cut:], None)
+    want = (float(head.detach()) * cut + float(tail.detach()) * (rows - cut)) / rows
+    assert abs(float(loss.detach()) - want) <= 4 * U * want
+    # Each side times its count: a half step of bf16 each (and of the factor's and the value's fp32,
+    # within 1 + 2^-7), and at listed words, where the value is the difference p f - q f of terms of
+    # at most 1, U for each of the products and the difference whose factors f differ: 4 U a side.
+    for s, e, part, n in ((0, cut, gh, cut), (cut, rows, gt, rows - cut)):
+        for a in range(s, e, 1 << 18):
+            got = grad[a:min(e, a + (1 << 18))].double() * rows
+            ref = part[a - s:min(e, a + (1 << 18)) - s].double() * n
+            err = (got - ref).abs() - 2.0 ** -8 * (got.abs() + ref.abs()) * (1 + 2.0 ** -7)
+            assert float(err.max()) <= 8 * U
+
+
+@pytest.mark.gpu
+def test_no_gradient_is_formed_where_none_is_recorded(cuda_device):
+    """An evaluation of a model's parameters under no_grad: no room for the weight's gradient
+    (32 MB in fp32) is taken, the logits' chunk and small arrays apart."""
+    h, w, b, values, tokens, lse = linear_case(2, 32, 512, 16384, 4, torch.bfloat16)
+    w, b = torch.nn.Parameter(w), torch.nn.Parameter(b)
+    with torch.no_grad():
+        chunked_linear_distillation(h, w, b, values, tokens, teacher_lse=lse)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        chunked_linear_distillation(h, w, b, values, tokens, teacher_lse=lse)
+        assert torch.cuda.max_memory_allocated() - before < 32 * 16384 * 4 + (1 << 20)
+        x = torch.nn.Parameter(torch.randn(4096, 5000, device=cuda_device))  # formed ahead otherwise
+        k = torch.zeros(4096, 1, device=cuda_device, dtype=torch.int64)
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        distillation_from_logits(x, torch.zeros(4096, 1, device=cuda_device), k)
+        assert torch.cuda.max_memory_allocated() - before < 1 << 20
 
 
 @pytest.mark.gpu

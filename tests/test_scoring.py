@@ -257,6 +257,40 @@ def test_rows_past_32_bit_offsets(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V,top", [(3, 2), (130, 0)])
+def test_rows_of_several_launches(cuda_device, V, top):
+    """More rows than one launch takes give the bits of their two parts."""
+    rows, cut = (1 << 21) + 21, 1 << 21
+    g = torch.Generator(device=cuda_device).manual_seed(V)
+    x = torch.randn(rows, V, generator=g, device=cuda_device).to(torch.bfloat16).requires_grad_(True)
+    t = torch.randint(0, V, (rows,), generator=g, device=cuda_device)
+    up = torch.randn(rows, generator=g, device=cuda_device)
+
+    def call(s, e):
+        r = token_logprobs(x[s:e], t[s:e], top=top)
+        total = (r.logprobs * up[s:e]).sum() + (r.entropy * up[s:e]).sum()
+        if top:
+            total = total + (r.top_logprobs * up[s:e, None]).sum()
+        return [f.detach() for f in r if f is not None], torch.autograd.grad(total, x)[0][s:e]
+
+    whole, grad = call(0, rows)
+    for s, e in ((0, cut), (cut, rows)):
+        part, g = call(s, e)
+        assert all(torch.equal(a[s:e], b) for a, b in zip(whole, part))
+        assert torch.equal(grad[s:e], g)
+
+
+@pytest.mark.gpu
+def test_the_first_call_is_not_captured(cuda_device, monkeypatch):
+    """Its error word would be made, and cleared on every replay, by the graph."""
+    x, t = logits_of(2, 4, 30, torch.float32)
+    monkeypatch.setattr(dabsn_amd.kernels.ops, "_STICKY", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="once before the capture"):
+        token_logprobs(x, t)
+
+
+@pytest.mark.gpu
 def test_bad_targets_are_reported(cuda_device, monkeypatch):
     x, t = logits_of(1, 4, 30, torch.float32)
     t[1], t[2] = 30, -1
