@@ -446,7 +446,8 @@ __global__ void __launch_bounds__(256) words_kernel(int H, int lanes_log2, int s
     float zero[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) zero[k] = 0.0f;
-    for (int c = (threadIdx.x & (lanes - 1)) * W; c < H; c += lanes * W) put<E, true>(dweight + v * H, c, H, zero);
+    for (int c = (threadIdx.x & (lanes - 1)) * W; c < H; c += lanes * W)
+      put<E, true>(dweight + v * H, c, H, zero);
     return;
   }
   const int64_t task = blockIdx.x - blanks;

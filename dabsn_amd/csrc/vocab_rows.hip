@@ -13,9 +13,10 @@
 // (counted at 8192 x 32000 bf16), against the 12 that the time of its 2 bytes allows. So the
 // exponent's argument is one fma of the logit, x c - r with c = log2 e / T and r, in units of ln 2,
 // near the thread's maximum (any number does: the result is exact in r); r moves only when a
-// vector exceeds it by 16. c is rounded: the sums u of e (x c - r), which the entropy needs anyhow, give the exact
-// normaliser to first order. Logits so large that x c overflows leave s = 0 and take the row's
-// pass again with differences formed first: rows that hold nothing but a mask's lowest value.
+// vector exceeds it by 16. c is rounded: the sums u of e (x c - r), which the entropy needs
+// anyhow, give the exact normaliser to first order. Logits so large that x c overflows leave s =
+// 0 and take the row's pass again with differences formed first: rows that hold nothing but a
+// mask's lowest value.
 #include <algorithm>
 
 #include "../../include/dabsn_hip.h"
@@ -485,36 +486,63 @@ __device__ void append_equal(const R& row, uint32_t key, int want, TopShared<NTH
   }
 }
 
+// The upper 16 bits of the K-th largest of 64 N keys, N a lane, bit by bit: a bound that K reach.
+template <int N>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t (&k)[N], int K) {
+  uint32_t tau = 0;
+  for (int bit = 15; bit >= 0; --bit) {
+    const uint32_t to = tau | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += __popcll(__ballot(k[i] >= to));
+    if (n >= K) tau = to;
+  }
+  return tau << 16;
+}
+template <int N, int M>
+__device__ __forceinline__ uint32_t bound_of_largest(const uint32_t (&k)[N], int K) {
+  uint32_t m[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) m[i] = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m[i % M] = max(m[i % M], k[i]);
+  return bound_of<M>(m, K);
+}
+
 // Gathers candidates that hold the K largest logits (equal ones by column). Every thread's
-// largest is known from the row's pass; the K-th largest of these is a bound that K logits reach, and few
-// more do (74 on average for K = 64 of 32,000 normal logits with 256 threads, 177 for K = 128), so
-// only the groups that reach it are read again, gathered and ranked against each other (4099 x 50021
-// fp32: 122 us without alternatives, 133 with 1, 136 with 20, 149 with 64, 182 with 128; bf16 66, 77,
-// 82, 91, 110). Where more than kCap reach it (rows with many equal logits) the K-th largest key is found by bisection over the row.
+// largest is known from the row's pass; the K-th largest of these, or of the largest of G of their
+// groups, is a bound that K logits reach, and few more do: of well mixed logits G ln(G / (G - K)), 74
+// for K = 64 of 256. So only the groups that reach it are read again, gathered and ranked against
+// each other (4099 x 50021 fp32: 122 us without alternatives, 133 with 1, 137 with 20, 148 with 64, 183
+// with 128; bf16 66, 75, 81, 90, 111). Where more than kCap reach it (rows with many equal logits)
+// the K-th largest key is found by bisection over the row. first, last: the thread's logits outside
+// the vectors (-inf: none). With a workgroup a compute unit, whose time is that of one load after
+// another, the threads load their best groups before the bound is known (1 x 32000 bf16 with 5
+// alternatives, with this and the bound of 64 groups: 7.7 us instead of 10.7; without any 4.7).
 template <int NTH, typename R>
-__device__ void top_k(const R& row, int K, const Best& b, float outside, bool nan,
+__device__ void top_k(const R& row, int K, const Best& b, float first, float last, bool nan,
                       TopShared<NTH>& t) {
   const int tid = threadIdx.x;
-  constexpr int W = R::W;
+  constexpr int W = R::W, N = NTH / 64;
+  constexpr bool AHEAD = NTH == 1024;
   const int nv = row.vectors();
-  t.best[tid] = fmaxf(b.v1, outside);
+  typename R::Raw ahead[8 / W];
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int g = 0; g < 8 / W; ++g) ahead[g] = row.load(max(0, min(b.c1 + g * NTH, nv - 1)));
+  }
+  t.best[tid] = fmaxf(b.v1, fmaxf(first, last));
   if (tid == 0) t.count = t.fulls = 0;
   __syncthreads();
-  if (tid < 64) {  // the upper 16 bits of the bound, bit by bit (the lower ones as zeros)
-    uint32_t k[NTH / 64];
+  if (tid < 64) {
+    uint32_t k[N];
 #pragma unroll
-    for (int i = 0; i < NTH / 64; ++i) k[i] = key_of(t.best[i * 64 + tid]) >> 16;
+    for (int i = 0; i < N; ++i) k[i] = key_of(t.best[i * 64 + tid]) >> 16;
     uint32_t tau = 0;
-    if (K <= NTH) {
-      for (int bit = 15; bit >= 0; --bit) {
-        const uint32_t to = tau | 1u << bit;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < NTH / 64; ++i) n += __popcll(__ballot(k[i] >= to));
-        if (n >= K) tau = to;
-      }
-    }
-    if (tid == 0) t.tau = max(tau << 16, kNone + 1);
+    if (K <= 16) tau = bound_of_largest<N, 1>(k, K);
+    else if (N > 4 && K <= 64) tau = bound_of_largest<N, N < 4 ? N : 4>(k, K);
+    else if (K <= NTH) tau = bound_of<N>(k, K);
+    if (tid == 0) t.tau = max(tau, kNone + 1);
   }
   __syncthreads();
   const uint32_t tau = t.tau;
@@ -522,12 +550,13 @@ __device__ void top_k(const R& row, int K, const Best& b, float outside, bool na
     const uint32_t k = key_of(x);
     if (k >= tau) push(t.cand, &t.count, k, j);
   };
-  auto take_vector = [&](int c) {
+  auto take_raw = [&](int c, const typename R::Raw& raw) {
     float v[W];
-    R::unpack(row.load(c), v);
+    R::unpack(raw, v);
 #pragma unroll
     for (int k = 0; k < W; ++k) take(static_cast<int>(row.column(c)) + k, v[k]);
   };
+  auto take_vector = [&](int c) { take_raw(c, row.load(c)); };
   // A thread whose third best group reaches the bound too leaves all of its vectors to a wave.
   if (key_of(b.v3) >= tau) {
     t.full[atomicAdd(&t.fulls, 1)] = static_cast<uint16_t>(tid);
@@ -536,11 +565,18 @@ __device__ void top_k(const R& row, int K, const Best& b, float outside, bool na
     for (int i = 0; i < 2; ++i) {
       const int c = i ? b.c2 : b.c1;
       if (c < 0 || key_of(i ? b.v2 : b.v1) < tau) continue;
+      if (AHEAD && i == 0) {
+#pragma unroll
+        for (int g = 0; g < 8 / W; ++g)
+          if (c + g * NTH < nv) take_raw(c + g * NTH, ahead[g]);
+        continue;
+      }
       take_vector(c);
       if (W == 4 && c + NTH < nv) take_vector(c + NTH);
     }
   }
-  row.singles(take);
+  take(tid, first);
+  take(row.head + nv * W + tid, last);
   __syncthreads();
   for (int i = tid >> 6; i < t.fulls; i += NTH / 64)
     for (int c = t.full[i] + (tid & 63) * NTH; c < nv; c += 64 * NTH) take_vector(c);
@@ -589,13 +625,13 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
   const size_t r = blockIdx.x;
   const Row<E, BIAS, !BIAS> row(logits + r * ldl, bias, V);
   Best best;
-  float outside = -INFINITY;
+  float first = -INFINITY, last = -INFINITY;  // this thread's logits outside the vectors
   const Norm n = norm_of<NTH, false>(
       source<NTH, 0>(row), k.c, nullptr, sh,
       [&](int c, float vm) {
         if constexpr (TOP) best.see(vm, c);
       },
-      [&](int, float x) { outside = fmaxf(outside, x); });
+      [&](int j, float x) { (j < row.head ? first : last) = x; });
   const double log_s = log(static_cast<double>(n.s)), ln_s = log_s + n.correction(k.delta);
   auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (threadIdx.x == 0) {
@@ -620,7 +656,7 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
   }
   if constexpr (TOP) {
     __shared__ TopShared<NTH> t;
-    top_k<NTH>(row, K, best, outside, n.s != n.s, t);
+    top_k<NTH>(row, K, best, first, last, n.s != n.s, t);
     const int count = t.count;
     for (int i = threadIdx.x; i < count; i += NTH) {
       const uint64_t mine = t.cand[i];
@@ -831,7 +867,9 @@ __device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n,
           w += same ? q[i] : 0.0f;
         }
       }
-      if (first) o.put(static_cast<int64_t>(j), __builtin_amdgcn_exp2f(arg(src.row.at(j))) * bsc - w * sc);
+      if (first)
+        o.put(static_cast<int64_t>(j),
+              __builtin_amdgcn_exp2f(arg(src.row.at(j))) * bsc - w * sc);
     }
   });
 }
@@ -959,8 +997,8 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   }
   if constexpr (GRAD) {
     __syncthreads();
-    distill_grad<NTH>(src, K, a, sc.c, KIND == kHalf ? kHalfScale : scale[0], te.a, te.b, te.twice != 0, te.idx, te.q,
-                      out_row<E, KIND>(out, r, ldo, 0, row.head));
+    distill_grad<NTH>(src, K, a, sc.c, KIND == kHalf ? kHalfScale : scale[0], te.a, te.b,
+                      te.twice != 0, te.idx, te.q, out_row<E, KIND>(out, r, ldo, 0, row.head));
   }
 }
 
@@ -1560,9 +1598,16 @@ static int checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t 
   return DABSN_OK;
 }
 
-// Threads a row: a wave where the row is a few vectors; the whole of a compute unit where fewer
-// rows than two a unit are there; else 256, of which eight rows share a unit.
-static int threads(int64_t rows, int64_t V) { return V <= 1024 ? 64 : rows < 512 && V >= 8192 ? 1024 : 256; }
+// Threads a row: a wave where the row is a few vectors; the whole of a compute unit where no more
+// rows than units are there; else 256, of which eight rows share a unit. With 1024 threads (of
+// which a unit holds one row or two) against 256, us: 384 rows of 8200 bf16, distillation 13.4 and
+// 9.3, log probabilities and their gradient 10.9 and 9.7; of 32000 15.8 and 13.2, 19.8 and 20.9,
+// log probabilities with 5 alternatives 21.7 and 12.6; of 128000 29.7 and 34.3, 57 and 67. So
+// plain passes (no alternatives, no list) over long rows keep 1024 up to two rows a unit.
+static int threads(int64_t rows, int64_t V, bool plain) {
+  const int64_t most = plain && V >= 65536 ? 511 : 256;
+  return V <= 1024 ? 64 : V >= 8192 && rows <= most ? 1024 : 256;
+}
 
 // A launch holds fewer than 2^32 threads: more rows than these run as launches of that many.
 constexpr int64_t kMostRows = 1 << 21;
@@ -1623,7 +1668,7 @@ int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* log
                                       past(top_logprobs, s * top), past(top_indices, s * top), err,
                                       stream);
     });
-  const int nth = threads(rows, V);
+  const int nth = threads(rows, V, top == 0);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
@@ -1686,7 +1731,7 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
           past(g_logprob, s), past(g_entropy, s), past(g_top, s * top),
           past(out, plane ? kBF16 : dtype, s * ldo), ldo, plane, stream);
     });
-  const int nth = threads(rows, V);
+  const int nth = threads(rows, V, true);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
@@ -1799,7 +1844,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                                past(coef, 4 * s), past(weights, s * top), scale, half,
                                past(out, half ? kBF16 : dtype, s * ldo), ldo, err, stream);
     });
-  const int nth = threads(rows, V);
+  const int nth = threads(rows, V, false);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   const bf16* b = static_cast<const bf16*>(bias);
@@ -1881,7 +1926,7 @@ int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits
                                    past(weights, s * top), scale, grad, done,
                                    past(dlogits, dtype, s * V), stream);
     });
-  const int nth = threads(rows, V);
+  const int nth = threads(rows, V, false);
   const dim3 grid(static_cast<unsigned>(rows));
   const Scale scale_t = scale_of(temperature);
   if (V <= kNarrow) {

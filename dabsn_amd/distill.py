@@ -219,12 +219,13 @@ def distillation_from_logits(logits: Tensor, top_logits: Tensor, top_indices: Te
     """``loss_weight`` times the mean distillation loss (fp32 scalar; see the module's note) of the
     student's ``logits`` [..., V], float32 or bfloat16 of any row stride, against the teacher's
     ``top_logits`` and ``top_indices`` [..., K], 1 <= K <= 128, and ``teacher_lse`` [...]. The
-    gradient has the logits' type, one rounding; the teacher's arrays get none. For many logits it
-    is formed with the loss (and takes their memory from then on): give a share of a mixed
-    objective, or one over the micro-batches, as ``loss_weight``; an upstream factor other than 1 forms
-    it again. A listed token outside [0, V)
-    other than ``ignore_index``, or a ``teacher_lse`` that is not the row's (weights of more than
-    256 in sum), makes the loss NaN and sets the error word that ``kernels.check_errors()`` raises (``DABSN_HIP_ERROR_CHECK=sync``: raised here)."""
+    gradient has the logits' type, one rounding; the teacher's arrays get none. For many logits
+    it is formed with the loss (and takes their memory from then on): give a share of a mixed
+    objective, or one over the micro-batches, as ``loss_weight``; an upstream factor other than
+    1 forms it again. A listed token outside [0, V) other than ``ignore_index``, or a
+    ``teacher_lse`` that is not the row's (weights of more than 256 in sum), makes the loss NaN
+    and sets the error word that ``kernels.check_errors()`` raises
+    (``DABSN_HIP_ERROR_CHECK=sync``: raised here)."""
     vocab.need_float(_WHAT, "logits", logits)
     if logits.dim() < 2:
         raise ValueError(f"{_WHAT}: expected logits [..., V] of one row or more")

@@ -58,8 +58,8 @@ def _forward(x, bias, targets, ignore, temperature, top, outs, s, word, stream):
     tk = ops.KernelTimer.begin("token_logprobs", x)
     _lib.check(_lib.load().dabsn_hip_token_logprobs(
         ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), ops._p(bias),
-        vocab.at(targets, s), ignore, temperature, top, vocab.at(lp, s), vocab.at(ent, s), vocab.at(st, s), vocab.at(tl, s),
-        vocab.at(ti, s), word.word.data_ptr(), stream), _WHAT)
+        vocab.at(targets, s), ignore, temperature, top, vocab.at(lp, s), vocab.at(ent, s),
+        vocab.at(st, s), vocab.at(tl, s), vocab.at(ti, s), word.word.data_ptr(), stream), _WHAT)
     ops.KernelTimer.end(tk)
 
 
@@ -70,8 +70,9 @@ def _backward(x, bias, targets, ignore, temperature, top, saved, grads, s, out, 
     tk = ops.KernelTimer.begin("token_logprobs_bwd", x)
     _lib.check(_lib.load().dabsn_hip_token_logprobs_bwd(
         ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), ops._p(bias),
-        vocab.at(targets, s), ignore, temperature, top, vocab.at(ti, s), vocab.at(st, s), vocab.at(ent, s), vocab.at(gl, s),
-        vocab.at(ge, s), vocab.at(gt, s), out, ldo, plane, vocab.stream(x)), _WHAT + " backward")
+        vocab.at(targets, s), ignore, temperature, top, vocab.at(ti, s), vocab.at(st, s),
+        vocab.at(ent, s), vocab.at(gl, s), vocab.at(ge, s), vocab.at(gt, s), out, ldo, plane,
+        vocab.stream(x)), _WHAT + " backward")
     ops.KernelTimer.end(tk)
 
 
