@@ -133,13 +133,14 @@ class ErrorWord:
 
     def __init__(self, device: torch.device):
         self.own = ops._sync_mode() == "sync"
-        if (not self.own and device.index not in ops._STICKY
-                and torch.cuda.is_current_stream_capturing()):
-            # The word would be made, and cleared on every replay, by the graph.
-            raise RuntimeError("the first DABSN HIP call on a device cannot be captured into a "
-                               "graph: call the operator once before the capture")
-        self.word = (torch.zeros(1, device=device, dtype=torch.int32) if self.own
-                     else ops._sticky(device))
+        sticky = ops._STICKY.get(device.index)
+        if sticky is None:
+            # The graph would make the word, and clear it on every replay.
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first DABSN HIP call on a device cannot be captured into a "
+                                   "graph: call the operator once before the capture")
+            sticky = ops._sticky(device)
+        self.word = torch.zeros(1, device=device, dtype=torch.int32) if self.own else sticky
 
     def check(self, what: str) -> None:
         if self.own:

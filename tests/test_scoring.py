@@ -282,12 +282,18 @@ def test_rows_of_several_launches(cuda_device, V, top):
 
 @pytest.mark.gpu
 def test_the_first_call_is_not_captured(cuda_device, monkeypatch):
-    """Its error word would be made, and cleared on every replay, by the graph."""
+    """Its error word would be made, and cleared on every replay, by the graph. A call before it
+    makes the word, also one that reads its own."""
     x, t = logits_of(2, 4, 30, torch.float32)
     monkeypatch.setattr(dabsn_amd.kernels.ops, "_STICKY", {})
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="once before the capture"):
+            token_logprobs(x, t)
+    monkeypatch.setenv("DABSN_HIP_ERROR_CHECK", "sync")
+    eager = token_logprobs(x, t).logprobs
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
-    with pytest.raises(RuntimeError, match="once before the capture"):
-        token_logprobs(x, t)
+    assert torch.equal(token_logprobs(x, t).logprobs, eager)
 
 
 @pytest.mark.gpu
