@@ -77,16 +77,16 @@ class _FromLogits(torch.autograd.Function):
         with vocab.on(x):
             stream = vocab.stream(x)
             word = vocab.ErrorWord(dev)
-            mean = torch.empty((), device=dev, dtype=torch.float32)
             # The rows' losses [n, 2], coefficients [n, 4] and weights [n, K], and the factor.
             aux = torch.empty(n * (6 + K) + 1 if need else 2 * n, device=dev, dtype=torch.float32)
+            mean = aux.new_empty(())
             loss = aux.data_ptr()
             coef = weights = factor = ready = None
             if need:
                 coef, weights, factor = loss + 8 * n, loss + 24 * n, loss + 4 * n * (6 + K)
             if fused:
                 _counted(values, tokens, ignore, V, loss, t, weight, factor, stream)
-                ready = torch.empty((n, V), device=dev, dtype=x.dtype)
+                ready = x.new_empty((n, V))
             _rows(x, None, values, tokens, lse, ignore, t, 0, loss, coef, weights, factor, False,
                   None if ready is None else ready.data_ptr(), V, word, stream)
             _lib.check(lib.dabsn_hip_distill_mean(n, loss, t, weight, mean.data_ptr(),
@@ -114,7 +114,7 @@ class _FromLogits(torch.autograd.Function):
         done = out is not None
         with vocab.on(x):
             if out is None:
-                out = torch.empty((n, V), device=x.device, dtype=x.dtype)
+                out = x.new_empty((n, V))
             aux_p = aux.data_ptr()
             tk = ops.KernelTimer.begin("distill_bwd", x)
             _lib.check(_lib.load().dabsn_hip_distill_bwd(

@@ -22,7 +22,7 @@ _NO_PADDING = -1  # not a word
 def _lookup(ids: Tensor, w: Tensor, scale: float) -> Tensor:
     (V, H), n = w.shape, ids.numel()
     with vocab.on(w):
-        out = torch.empty((*ids.shape, H), device=w.device, dtype=w.dtype)
+        out = w.new_empty((*ids.shape, H))
         word = vocab.ErrorWord(w.device)
         tk = ops.KernelTimer.begin("embedding", w)
         _lib.check(_lib.load().dabsn_hip_embedding_fwd(
@@ -45,12 +45,12 @@ class _ScaledEmbedding(torch.autograd.Function):
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
         (V, H), dtype, scale, padding = ctx.args
-        g = grad.to(dtype).contiguous()
+        g = (grad if grad.dtype == dtype else grad.to(dtype)).contiguous()
         n, lib = ids.numel(), _lib.load()
         with vocab.on(g):
-            out = torch.empty((V, H), device=g.device, dtype=dtype)
+            out = g.new_empty((V, H))
             nbytes = lib.dabsn_hip_embedding_workspace_bytes(n, V, H)
-            ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8) if nbytes else None
+            ws = g.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
             tk = ops.KernelTimer.begin("embedding_bwd", g)
             _lib.check(lib.dabsn_hip_embedding_bwd(
                 ops._code(dtype), n, V, H, ids.data_ptr(), padding, g.data_ptr(), scale,

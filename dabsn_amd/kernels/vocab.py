@@ -10,7 +10,6 @@ question is NaN. ``DABSN_HIP_ERROR_CHECK=sync`` raises from the call instead.
 from __future__ import annotations
 
 import contextlib
-import math
 import os
 
 import torch
@@ -31,7 +30,7 @@ _HERE = contextlib.nullcontext()
 
 def on(t: Tensor):
     """The device of ``t`` as the current one (the library launches on the current device)."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def no_autocast():
@@ -41,7 +40,7 @@ def no_autocast():
 
 def stream(t: Tensor) -> int:
     """The current stream's handle on the device of ``t``."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def at(t: Tensor | None, s: int) -> int | None:
@@ -71,12 +70,12 @@ def need_device(what: str, *tensors: Tensor | None) -> None:
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError(f"{what}: DABSN HIP operators need ROCm device tensors")
         if first is None:
-            first = t.device
-        elif t.device != first:
-            raise RuntimeError(f"{what}: tensors on {first} and {t.device}")
+            first = t
+        elif t.get_device() != first.get_device():
+            raise RuntimeError(f"{what}: tensors on {first.device} and {t.device}")
 
 
 def need_float(what: str, name: str, t: Tensor) -> None:
@@ -88,7 +87,7 @@ def need_tokens(what: str, name: str, t: Tensor, shape) -> Tensor:
     """Token numbers of the given shape as contiguous int64."""
     if t.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{what}: {name} must be int64 or int32, not {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} {tuple(t.shape)} does not match {tuple(shape)}")
     if t.dtype != torch.int64:
         t = t.to(torch.int64)
@@ -97,7 +96,7 @@ def need_tokens(what: str, name: str, t: Tensor, shape) -> Tensor:
 
 def need_temperature(what: str, t: float) -> float:
     t = float(t)
-    if not (math.isfinite(t) and 1e-6 <= t <= 1e6):
+    if not 1e-6 <= t <= 1e6:  # nor NaN
         raise ValueError(f"{what}: temperature must lie in [1e-6, 1e6], not {t}")
     return t
 
@@ -123,7 +122,9 @@ def row_stride(x: Tensor) -> int:
 
 
 def grads_of(g: Tensor | None) -> Tensor | None:
-    return None if g is None else g.to(torch.float32).contiguous()
+    if g is None:
+        return None
+    return (g if g.dtype == torch.float32 else g.float()).contiguous()
 
 
 class ErrorWord:

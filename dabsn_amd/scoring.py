@@ -43,12 +43,11 @@ _WHAT = "token log probabilities"
 
 
 def _outputs(rows: int, top: int, device, targets: bool, stats: bool):
-    f32 = torch.float32
-    lp = torch.empty(rows, device=device, dtype=f32) if targets else None
-    ent = torch.empty(rows, device=device, dtype=f32)
-    st = torch.empty((rows, 2), device=device, dtype=f32) if stats else None
-    tl = torch.empty((rows, top), device=device, dtype=f32) if top else None
-    ti = torch.empty((rows, top), device=device, dtype=torch.int64) if top else None
+    ent = torch.empty(rows, device=device, dtype=torch.float32)
+    lp = torch.empty_like(ent) if targets else None
+    st = ent.new_empty((rows, 2)) if stats else None
+    tl = ent.new_empty((rows, top)) if top else None
+    ti = ent.new_empty((rows, top), dtype=torch.int64) if top else None
     return lp, ent, st, tl, ti
 
 
@@ -102,7 +101,7 @@ class _TokenLogprobs(torch.autograd.Function):
         x, targets, st, ent, ti = ctx.saved_tensors
         grads = vocab.grads_of(gl), vocab.grads_of(ge), vocab.grads_of(gt)
         with vocab.on(x):
-            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+            out = x.new_empty(x.shape)
             _backward(x, None, targets, *ctx.args, (st, ent, ti), grads, 0, out.data_ptr(),
                       x.shape[1], 0)
         return out, None, None, None, None
