@@ -219,11 +219,12 @@ __device__ __forceinline__ float largest(const float (&v)[8]) {
   return max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[7]));
 }
 
-// The sum over the block of N values a thread, to every thread. sh: N * NTH/64 floats.
+// The sum over the block of N values a thread, to every thread; the waves' sums are added in 64
+// bits (16 roundings to fp32 of a sum that grows would be most of its error). sh: N * NTH/64 floats.
 template <int NTH, int N>
-__device__ __forceinline__ void block_sums(float (&v)[N], float* sh) {
+__device__ __forceinline__ void block_sums(float (&v)[N], double (&sum)[N], float* sh) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  for (int i = 0; i < N; ++i) sum[i] = v[i] = wave_sum(v[i]);
   if constexpr (NTH > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
@@ -233,9 +234,9 @@ __device__ __forceinline__ void block_sums(float (&v)[N], float* sh) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = 0.0f;
+      sum[i] = 0.0;
 #pragma unroll
-      for (int w = 0; w < NTH / 64; ++w) v[i] += sh[i * (NTH / 64) + w];
+      for (int w = 0; w < NTH / 64; ++w) sum[i] += sh[i * (NTH / 64) + w];
     }
   }
 }
@@ -304,25 +305,23 @@ struct Share {
     u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);
     if constexpr (REST) rest += listed ? 0.0f : e;
   }
-  // The block's shares as one, to every thread.
+  // The block's shares as one: s, u and with REST rest.
   template <int NTH, bool REST>
-  __device__ __forceinline__ void join(float* sh) {
+  __device__ __forceinline__ void join(double (&sum)[2 + REST], float* sh) {
     raise<REST>(block_max<NTH>(r, sh));
     float v[2 + REST];
     v[0] = s;
     v[1] = u;
     if constexpr (REST) v[2] = rest;
-    block_sums<NTH, 2 + REST>(v, sh);
-    s = v[0];
-    u = v[1];
-    if constexpr (REST) rest = v[2];
+    block_sums<NTH, 2 + REST>(v, sum, sh);
   }
 };
 
 // What a row's pass leaves. Log probabilities are differences of numbers of the size of the
 // logits, so the few of a row are formed in 64 bits.
 struct Norm {
-  float r, s, u, rest;
+  float r;
+  double s, u, rest;
   bool safe;
   // f(arg) with the row's form of the exponent's argument as a function of a logit.
   template <typename F>
@@ -330,13 +329,13 @@ struct Norm {
     if (safe) f([r = r, c](float x) { return Share<true>::arg(x, r, c); });
     else f([r = r, c](float x) { return Share<false>::arg(x, r, c); });
   }
-  __device__ __forceinline__ bool empty() const { return s == 0.0f; }  // no finite logit
+  __device__ __forceinline__ bool empty() const { return s == 0.0; }  // no finite logit
   // What ln s lacks for the rounding of c (log2 e / T = c (1 + delta)).
   __device__ __forceinline__ double correction(double delta) const {
-    return kLn2 * delta * (static_cast<double>(u) / s + (safe ? 0.0 : static_cast<double>(r)));
+    return kLn2 * delta * (u / s + (safe ? 0.0 : static_cast<double>(r)));
   }
   __device__ __forceinline__ double ln_s(double delta) const {
-    return log(static_cast<double>(s)) + correction(delta);
+    return log(s) + correction(delta);
   }
   // The correction of ln s and that of the mean of z are the same and cancel.
   __device__ __forceinline__ float entropy(double log_s) const {
@@ -391,15 +390,18 @@ __device__ __forceinline__ Norm row_pass(const S& src, float c, const uint8_t* l
         a.template fold1<REST>(x, REST && (listed[(j + pad) >> 3] >> ((j + pad) & 7) & 1));
         last(j, x);
       });
-  a.template join<NTH, REST>(sh);
-  return Norm{a.r, a.s, a.u, a.rest, SAFE};
+  double sum[2 + REST];
+  a.template join<NTH, REST>(sum, sh);
+  double rest = 0.0;
+  if constexpr (REST) rest = sum[2];
+  return Norm{a.r, sum[0], sum[1], rest, SAFE};
 }
 // The row's norm; `see` gets each group's first vector and largest logit, `last` the logits outside.
 template <int NTH, bool REST, typename S, typename See, typename Last>
 __device__ __forceinline__ Norm norm_of(const S& src, float c, const uint8_t* listed, float* sh,
                                         See see, Last last) {
   const Norm n = row_pass<NTH, REST, false>(src, c, listed, sh, see, last);
-  if (n.s != 0.0f) return n;
+  if (n.s != 0.0) return n;
   __syncthreads();
   return row_pass<NTH, REST, true>(src, c, listed, sh, [](int, float) {}, [](int, float) {});
 }
@@ -632,13 +634,13 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
         if constexpr (TOP) best.see(vm, c);
       },
       [&](int j, float x) { (j < row.head ? first : last) = x; });
-  const double log_s = log(static_cast<double>(n.s)), ln_s = log_s + n.correction(k.delta);
+  const double log_s = log(n.s), ln_s = log_s + n.correction(k.delta);
   auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (threadIdx.x == 0) {
     entropy[r] = n.entropy(log_s);
     if (stats) {
       stats[2 * r] = n.r;
-      stats[2 * r + 1] = n.safe ? -n.s : n.s;
+      stats[2 * r + 1] = static_cast<float>(n.safe ? -n.s : n.s);
     }
     if (logprob) {
       const int64_t t = targets[r];
@@ -766,8 +768,8 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
     sum += wave_sum(part) * inv_t;
   }
   const float ge = g_ent ? g_ent[r] * inv_t : 0.0f;
-  const float is = n.empty() ? 0.0f : 1.0f / n.s;
-  const float lns = n.empty() ? 0.0f : logf(n.s);
+  const float s = static_cast<float>(n.s), is = n.empty() ? 0.0f : 1.0f / s;
+  const float lns = n.empty() ? 0.0f : logf(s);
   const float A = off ? NAN : -(sum + ge * (entropy[r] - lns)) * is;
   const float B = -ge * static_cast<float>(kLn2) * is;
   if (threadIdx.x == 0) taken = 0;
@@ -960,8 +962,8 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
     double l = wave_sum_d(part);
     if constexpr (REST) {
       // A rest that the student's mask or a list of all tokens leaves no room for is left out.
-      rest = rest > 0.0 && a.rest != 0.0f ? rest : 0.0;
-      if (rest != 0.0) l += rest * (log(rest) - log(static_cast<double>(a.rest)) + ln_s);
+      rest = rest > 0.0 && a.rest != 0.0 ? rest : 0.0;
+      if (rest != 0.0) l += rest * (log(rest) - log(a.rest) + ln_s);
       total += rest;
     }
     float b = empty ? 0.0f : static_cast<float>(total / a.s);
@@ -1115,13 +1117,13 @@ __global__ void __launch_bounds__(256) logprobs_narrow_kernel(
   const Narrow<E, NV> w(rows, V, ldl, logits, bias);
   float e[NV];
   const Norm n = w.norm(k.c, e);
-  const double log_s = log(static_cast<double>(n.s)), ln_s = log_s + n.correction(k.delta);
+  const double log_s = log(n.s), ln_s = log_s + n.correction(k.delta);
   auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (w.live && w.lane == 0) {
     entropy[w.r] = n.entropy(log_s);
     if (stats) {
       stats[2 * w.r] = n.r;
-      stats[2 * w.r + 1] = -n.s;
+      stats[2 * w.r + 1] = static_cast<float>(-n.s);
     }
   }
   if (logprob) {
@@ -1205,8 +1207,8 @@ __global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
     }
   }
   const float ge = g_ent ? g_ent[w.r] * inv_t : 0.0f;
-  const float is = n.empty() ? 0.0f : 1.0f / n.s;
-  const float lns = n.empty() ? 0.0f : logf(n.s);
+  const float s = static_cast<float>(n.s), is = n.empty() ? 0.0f : 1.0f / s;
+  const float lns = n.empty() ? 0.0f : logf(s);
   const float A = off ? NAN : -(sum + ge * (entropy[w.r] - lns)) * is;
   const float B = -ge * static_cast<float>(kLn2) * is;
   const auto o = out_row<E, KIND>(out, w.r, ldo, plane, 0);
@@ -1320,8 +1322,8 @@ __global__ void __launch_bounds__(256) distill_narrow_kernel(
     for (int i = 0; i < NV; ++i) off += hit[i] ? 0.0f : e[i];
     n.rest = sum16(off);
     rest = 1.0 - total;
-    rest = rest > 0.0 && n.rest != 0.0f ? rest : 0.0;
-    if (rest != 0.0) part += rest * (log(rest) - log(static_cast<double>(n.rest)) + ln_s);
+    rest = rest > 0.0 && n.rest != 0.0 ? rest : 0.0;
+    if (rest != 0.0) part += rest * (log(rest) - log(n.rest) + ln_s);
     total += rest;
   }
   if (!w.live || w.lane != 0) return;
