@@ -16,7 +16,7 @@ entropy bonus needs the first two, and a teacher's alternatives are what ``disti
 Words whose logit is -inf (or the type's lowest value, as masks use) have probability 0 and take
 no part. A row of -inf only has log probabilities -inf, entropy 0, its first words as
 alternatives and no gradient. A row with a NaN or +inf gives NaN. One kernel reads the logits
-once (and the few vectors that hold an alternative again); all sums are fp32.
+once (and the few vectors that hold an alternative again); sums are fp32, joined in 64 bits.
 """
 
 from __future__ import annotations
