@@ -14,9 +14,11 @@
 // exponent's argument is one fma of the logit, x c - r with c = log2 e / T and r, in units of ln 2,
 // near the thread's maximum (any number does: the result is exact in r); r moves only when a
 // vector exceeds it by 16. c is rounded: the sums u of e (x c - r), which the entropy needs
-// anyhow, give the exact normaliser to first order. Logits so large that x c overflows leave s =
-// 0 and take the row's pass again with differences formed first: rows that hold nothing but a
-// mask's lowest value.
+// anyhow, give the exact normaliser to first order. The fma leaves what r = x c lost in its own
+// rounding, half an ulp of x c: below 4 up to 2^26, and 2^100 of a mask's -1e30, so r is kept in
+// +-2^26. It starts at the lower end, from where the words that a mask rules out with any large
+// negative number add 0 and move nothing. A row that holds nothing else (s = 0), or whose largest
+// logit passes the upper end, takes the pass again with differences formed first.
 #include <algorithm>
 
 #include "../../include/dabsn_hip.h"
@@ -257,9 +259,10 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
 // A thread's share of a row relative to its reference r: s = sum e, u = sum e arg with
 // e = 2^arg, rest = the share of s at tokens that are not listed. arg = x c - r; SAFE rows have
 // arg = (x - r) c. Logits of -inf give e = 0; NaN and +inf make s NaN.
+constexpr float kFar = 67108864.0f;  // 2^26
 template <bool SAFE>
 struct Share {
-  float r = SAFE ? kLowest : -3e38f, s = 0.0f, u = 0.0f, rest = 0.0f;
+  float r = SAFE ? kLowest : -kFar, s = 0.0f, u = 0.0f, rest = 0.0f;
   float c;
   __device__ __forceinline__ explicit Share(float c_) : c(c_) {}
   static __device__ __forceinline__ float arg(float x, float r, float c) {
@@ -401,7 +404,7 @@ template <int NTH, bool REST, typename S, typename See, typename Last>
 __device__ __forceinline__ Norm norm_of(const S& src, float c, const uint8_t* listed, float* sh,
                                         See see, Last last) {
   const Norm n = row_pass<NTH, REST, false>(src, c, listed, sh, see, last);
-  if (n.s != 0.0) return n;
+  if (n.s != 0.0 && n.r <= kFar) return n;
   __syncthreads();
   return row_pass<NTH, REST, true>(src, c, listed, sh, [](int, float) {}, [](int, float) {});
 }

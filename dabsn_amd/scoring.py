@@ -13,8 +13,8 @@ readout's weight and bias, whose logits [N, V] never exist at once (chunks as in
 probabilities, the entropy and the alternatives' log probabilities: a policy gradient with an
 entropy bonus needs the first two, and a teacher's alternatives are what ``distill`` learns from.
 
-Words whose logit is -inf (or the type's lowest value, as masks use) have probability 0 and take
-no part. A row of -inf only has log probabilities -inf, entropy 0, its first words as
+Words whose logit is -inf, or as low as masks set it (-1e9, the type's lowest value), have
+probability 0 and take no part. A row of -inf only has log probabilities -inf, entropy 0, its first words as
 alternatives and no gradient. A row with a NaN or +inf gives NaN. One kernel reads the logits
 once (and the few vectors that hold an alternative again); sums are fp32, joined in 64 bits.
 """

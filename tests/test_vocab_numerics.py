@@ -1,0 +1,111 @@
+"""Rows of a vocabulary where 32 bits are short: masks of large finite numbers, against the
+definitions in 64 bits of test_scoring.py and test_distill.py, with the tolerances derived there."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from dabsn_amd import distillation_from_logits, token_logprobs
+from test_distill import check, reference as distill_reference
+from test_scoring import check_forward, check_grad, logits_of, reference_grad
+
+INF = math.inf
+FILLS = [-1e9, -1e10, -1e20, -1e30, "lowest", -6e7, -4e7]
+TEMPERATURES = [0.5, 1.0, 1.5, 2.0, 2.5, 3.0, 5.0, 8.0]
+
+
+def masked_rows(V, dtype, fill, seed):
+    """Rows: nine words of ten at the fill; all but the last; all; the fill beside -inf; all but
+    word 3 of those before the row's second half; an unmasked one."""
+    fill = torch.finfo(dtype).min if fill == "lowest" else fill
+    x, _ = logits_of(seed, 6, V, dtype, device="cpu")
+    drop = torch.rand(V, generator=torch.Generator().manual_seed(seed)) < 0.9
+    drop[5] = False
+    x[0, drop] = fill
+    x[1, :-1] = fill
+    x[2] = fill
+    x[3, drop] = fill
+    x[3, ::3] = -INF
+    x[4, :V // 2] = fill
+    x[4, 3] = 1.0
+    return x.cuda(), torch.tensor([5, V - 1, 2, 5, 3, 7]).cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fill", FILLS)
+@pytest.mark.parametrize("V", [61, 300, 9001])
+def test_scores_of_rows_masked_by_large_numbers(cuda_device, V, fill, dtype):
+    x, t = masked_rows(V, dtype, fill, V)
+    g = torch.Generator().manual_seed(1)
+    gl, ge = torch.randn(6, generator=g).cuda(), torch.randn(6, generator=g).cuda()
+    for T in TEMPERATURES:
+        check_forward(token_logprobs(x, t, top=9, temperature=T), x, t, 9, T)
+        leaf = x.clone().requires_grad_(True)
+        r = token_logprobs(leaf, t, top=9, temperature=T)
+        (got,) = torch.autograd.grad((r.logprobs, r.entropy), leaf, (gl, ge))
+        check_grad(got, *reference_grad(x, t, 0, T, gl, ge, None), V, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [61, 300, 9001])
+def test_scores_of_large_positive_logits(cuda_device, V, dtype):
+    """Logits around 1e8, 1e10 and 1e30, all of a row or one word in seven."""
+    for k, big in enumerate((1e8, 1e10, 1e30)):
+        x, t = logits_of(k, 5, V, dtype)
+        x[0] = (x[0].float() * big / 100 + big).to(dtype)
+        x[1, ::7] = (x[1, ::7].float() * big / 100 + big).to(dtype)
+        x[2, 4] = big
+        x[3] = big
+        t[:] = torch.tensor([1, 7, 4, 0, 3])
+        for T in (0.5, 1.0, 2.5):
+            check_forward(token_logprobs(x, t, top=3, temperature=T), x, t, 3, T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("fill", FILLS)
+@pytest.mark.parametrize("V", [61, 300, 9001])
+def test_distillation_of_rows_masked_by_large_numbers(cuda_device, V, fill, rest, dtype):
+    """A listed word is ruled out in no row (its loss would be the fill itself); row 4 has no list."""
+    x, _ = masked_rows(V, dtype, fill, V)
+    x = x[[0, 1, 3, 4, 2, 5]]
+    words = [(x[r].float() > -1e4).nonzero()[:, 0] for r in range(6)]
+    words[4] = torch.arange(3, device=x.device)
+    K = 4
+    tokens = torch.full((6, K), -100, device=x.device)
+    for r, w in enumerate(words):
+        if r != 4:
+            tokens[r, :min(K, len(w))] = w[:K]
+    values = torch.randn(6, K, generator=torch.Generator().manual_seed(3)).cuda()
+    for T in TEMPERATURES:
+        lse = (torch.logsumexp(values.double() / T, 1) + 0.4).float() if rest else None
+        leaf = x.clone().requires_grad_(True)
+        loss = distillation_from_logits(leaf, values, tokens, temperature=T, teacher_lse=lse)
+        (got,) = torch.autograd.grad(loss, leaf)
+        check(loss, got, distill_reference(x, values, tokens, T, lse), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [-1e10, -1e30])
+def test_many_masked_rows_with_the_gradient_formed_ahead(cuda_device, fill):
+    """Enough logits that loss and gradient are formed together (2100 x 8200): bit for bit what a
+    factor of 2 forms again, its first rows the definition's."""
+    x, t = logits_of(5, 2100, 8200, torch.bfloat16)
+    keep = torch.rand(2100, 8200, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < 0.1
+    x = torch.where(keep, x, fill).to(torch.bfloat16)
+    values, tokens = x.float().topk(6, dim=1)
+    leaf = x.requires_grad_(True)
+    loss = distillation_from_logits(leaf, values, tokens, temperature=2.0)
+    (g1,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+    (g2,) = torch.autograd.grad(loss * 2, leaf)
+    assert math.isfinite(float(loss.detach())) and torch.equal(g2 / 2, g1)
+    _, grad, _, tol = distill_reference(x[:6], values[:6], tokens[:6], 2.0)
+    grad, tol = grad * 6 / 2100, tol * 6 / 2100
+    err = (g1[:6].double().cpu() - grad).abs()
+    assert bool((err <= tol + 2.0 ** -8 * (grad.abs() + tol) * (1 + 2.0 ** -10) + 2.0 ** -126).all())
