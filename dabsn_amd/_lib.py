@@ -13,7 +13,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_build" / "libdabsn_hip.so"
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 _lock = threading.Lock()
 _lib = None

@@ -257,66 +257,53 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
 }
 
 // A thread's share of a row relative to its reference r: s = sum e, u = sum e arg with
-// e = 2^arg, rest = the share of s at tokens that are not listed. arg = x c - r; SAFE rows have
-// arg = (x - r) c. Logits of -inf give e = 0; NaN and +inf make s NaN.
+// e = 2^arg. arg = x c - r; SAFE rows have arg = (x - r) c. Logits of -inf give e = 0; NaN and +inf
+// make s NaN.
 constexpr float kFar = 67108864.0f;  // 2^26
 template <bool SAFE>
 struct Share {
-  float r = SAFE ? kLowest : -kFar, s = 0.0f, u = 0.0f, rest = 0.0f;
+  float r = SAFE ? kLowest : -kFar, s = 0.0f, u = 0.0f;
   float c;
   __device__ __forceinline__ explicit Share(float c_) : c(c_) {}
   static __device__ __forceinline__ float arg(float x, float r, float c) {
     return SAFE ? (x - r) * c : __builtin_fmaf(x, c, -r);
   }
   // The reference becomes `to`.
-  template <bool REST>
   __device__ __forceinline__ void raise(float to) {
     const float d = r == to ? 0.0f : SAFE ? (r - to) * c : r - to;  // both may be inf
     const float f = __builtin_amdgcn_exp2f(d);
     u = f == 0.0f ? 0.0f : f * (u + d * s);
     s *= f;
-    if constexpr (REST) rest *= f;
     r = to;
   }
-  template <bool REST>
   __device__ __forceinline__ void see(float largest) {
     const float t = SAFE ? largest : largest * c;
-    if (t > (SAFE ? r : r + 16.0f)) raise<REST>(t);
+    if (t > (SAFE ? r : r + 16.0f)) raise(t);
   }
-  template <bool REST>
-  __device__ __forceinline__ void fold(const float (&v)[8], float vm, uint32_t listed) {
-    see<REST>(vm);
-    float vs = 0.0f, vr = 0.0f;
+  __device__ __forceinline__ void fold(const float (&v)[8], float vm) {
+    see(vm);
+    float vs = 0.0f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float a = arg(v[k], r, c);
       const float e = __builtin_amdgcn_exp2f(a);
       vs += e;
       u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);  // arg = -inf has e = 0
-      if constexpr (REST) {
-        if (listed) vr += (listed >> k & 1) ? 0.0f : e;  // few vectors hold a listed token
-      }
     }
     s += vs;
-    if constexpr (REST) rest += listed ? vr : vs;
   }
-  template <bool REST>
-  __device__ __forceinline__ void fold1(float x, bool listed) {
-    see<REST>(x);
+  __device__ __forceinline__ void fold1(float x) {
+    see(x);
     const float a = arg(x, r, c), e = __builtin_amdgcn_exp2f(a);
     s += e;
     u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);
-    if constexpr (REST) rest += listed ? 0.0f : e;
   }
-  // The block's shares as one: s, u and with REST rest.
-  template <int NTH, bool REST>
-  __device__ __forceinline__ void join(double (&sum)[2 + REST], float* sh) {
-    raise<REST>(block_max<NTH>(r, sh));
-    float v[2 + REST];
-    v[0] = s;
-    v[1] = u;
-    if constexpr (REST) v[2] = rest;
-    block_sums<NTH, 2 + REST>(v, sum, sh);
+  // The block's shares as one: s and u.
+  template <int NTH>
+  __device__ __forceinline__ void join(double (&sum)[2], float* sh) {
+    raise(block_max<NTH>(r, sh));
+    float v[2] = {s, u};
+    block_sums<NTH, 2>(v, sum, sh);
   }
 };
 
@@ -324,7 +311,7 @@ struct Share {
 // logits, so the few of a row are formed in 64 bits.
 struct Norm {
   float r;
-  double s, u, rest;
+  double s, u;
   bool safe;
   // f(arg) with the row's form of the exponent's argument as a function of a logit.
   template <typename F>
@@ -345,11 +332,14 @@ struct Norm {
     const double h = log_s - kLn2 * u / s;
     return empty() || h < 0.0 ? 0.0f : static_cast<float>(h);
   }
+  // ln of the sum of exp((x - at) / T) over the row's logits x.
+  __device__ __forceinline__ double ln_sum(double at, double inv_t, double ln_s) const {
+    if (empty()) return -INFINITY;
+    return safe ? (r - at) * inv_t + ln_s : r * kLn2 - at * inv_t + ln_s;
+  }
   // log p of a logit x.
   __device__ __forceinline__ double logp(float x, double inv_t, double ln_s) const {
-    if (empty()) return -INFINITY;
-    const double z = static_cast<double>(x);
-    return safe ? (z - r) * inv_t - ln_s : z * inv_t - (r * kLn2 + ln_s);
+    return empty() ? -INFINITY : -ln_sum(static_cast<double>(x), inv_t, ln_s);
   }
 };
 // 1 / T, c and its error, from the host.
@@ -367,6 +357,7 @@ static Scale scale_of(float t) {
 
 __device__ __forceinline__ int pad_of(int head) { return -head & 7; }
 
+// REST: over the words whose bit in `listed` is not set.
 template <int NTH, bool REST, bool SAFE, typename S, typename See, typename Last>
 __device__ __forceinline__ Norm row_pass(const S& src, float c, const uint8_t* listed, float* sh,
                                          See see, Last last) {
@@ -376,28 +367,33 @@ __device__ __forceinline__ Norm row_pass(const S& src, float c, const uint8_t* l
   Share<SAFE> a(c);
   src.each(
       [&](int k, int n, const float (&v)[8]) {
-        const float vm = largest(v);
-        uint32_t bits = 0;
         if constexpr (REST) {
+          uint32_t bits = 0;
           if constexpr (S::W == 8) {
             bits = body[k];
           } else {
             auto four = [&](int i) { return body[i >> 1] >> (4 * (i & 1)) & 15u; };
             bits = four(k) | (n == 2 ? four(k + NTH) << 4 : 0u);
           }
+          if (bits) {  // few vectors hold a listed word
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = (bits >> i & 1) ? -INFINITY : v[i];
+            a.fold(w, largest(w));
+            return;
+          }
         }
-        a.template fold<REST>(v, vm, bits);
+        const float vm = largest(v);
+        a.fold(v, vm);
         see(k, vm);
       },
       [&](int j, float x) {
-        a.template fold1<REST>(x, REST && (listed[(j + pad) >> 3] >> ((j + pad) & 7) & 1));
+        a.fold1(REST && (listed[(j + pad) >> 3] >> ((j + pad) & 7) & 1) ? -INFINITY : x);
         last(j, x);
       });
-  double sum[2 + REST];
-  a.template join<NTH, REST>(sum, sh);
-  double rest = 0.0;
-  if constexpr (REST) rest = sum[2];
-  return Norm{a.r, sum[0], sum[1], rest, SAFE};
+  double sum[2];
+  a.template join<NTH>(sum, sh);
+  return Norm{a.r, sum[0], sum[1], SAFE};
 }
 // The row's norm; `see` gets each group's first vector and largest logit, `last` the logits outside.
 template <int NTH, bool REST, typename S, typename See, typename Last>
@@ -759,7 +755,7 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
   const Row<E, BIAS, !BIAS> row(logits + r * ldl, bias, V);
   const auto o = out_row<E, KIND>(out, r, ldo, plane, row.head);
   const float inv_t = static_cast<float>(k.inv_t), c = k.c;
-  const Norm n{stats[2 * r], fabsf(stats[2 * r + 1]), 0.0f, 0.0f, stats[2 * r + 1] < 0.0f};
+  const Norm n{stats[2 * r], fabsf(stats[2 * r + 1]), 0.0f, stats[2 * r + 1] < 0.0f};
   int64_t t = targets && g_lp ? targets[r] : -1;
   const bool off = targets && g_lp && t != ignore && (t < 0 || t >= V);  // a NaN row
   const bool aim = targets && g_lp && t != ignore && !off;
@@ -811,18 +807,24 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
 // One row: the teacher's weights q of its listed tokens (64 bits: one less their sum is what
 // the rest gets), the student's softmax, the loss
 //   sum q (ln q - logp) + q_r (ln q_r - ln p_r),  p_r the student's mass off the list,
-// and the coefficients of its gradient p_j b - q_j at listed and p_j a at other tokens:
-//   b = Q / s, a = b - q_r / r  (Q = sum q + q_r, r = the student's exp-sum off the list).
-// A bit per word (with the rest; else per word modulo kBits) marks the listed tokens: the rest's
-// sum leaves them out one by one, as a difference of sums would lose a small rest, and a bit
-// that was set before shows that a token may be listed twice.
+// and its gradient, with Q = sum q + q_r: p_j Q - q_j at listed words, formed here in 64 bits (a
+// student near its teacher leaves a small difference), and at the others
+//   p_j Q - q_r p_j / p_r = e_j a,  a = (p_r Q - q_r) / sum of e off the list.
+// With the rest the pass goes over the words off the list alone, relative to the largest of these:
+// p_r may be smaller than fp32 holds beside the listed words, which join in 64 bits. A student
+// that has no word for the rest, by -inf or by a mass that 64 bits hold as 0, is not asked for it.
+// A bit per word (with the rest; else per word modulo kBits) marks the listed tokens; one that
+// was set before shows that a token may be listed twice.
 constexpr int kBits = 32768;
 constexpr int kMaxRestVocab = 480000;  // 60 KB of bits
+constexpr float kAbsent = 3e38f;       // in the place of a listed word's gradient: not written
+constexpr double kLeast = -745.0;      // ln of the smallest positive number of 64 bits
 
 struct Teacher {
   int idx[kMaxTop];  // -1: absent
-  float q[kMaxTop];
-  float a, b;
+  double q[kMaxTop];
+  float g[kMaxTop];
+  float a;
   int twice;
 };
 
@@ -837,12 +839,12 @@ __device__ __forceinline__ double wave_max_d(double v) {
   return v;
 }
 
-// Writes the row's gradient times sc; a token listed twice has both weights at its place.
-template <int NTH, typename S, typename O>
-__device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n, float c,
-                                             float sc, float a, float b, bool twice,
-                                             const int* idx, const float* q, const O& o) {
-  const float asc = a * sc, bsc = b * sc;
+// Writes the row's gradient times sc; g: of the listed words, kAbsent where there is none or an
+// earlier place has the word's.
+template <int NTH, typename S, typename O, typename T>
+__device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n, float c, float sc,
+                                             float a, const T* idx, const float* g, const O& o) {
+  const float asc = a * sc;
   n.with_arg(c, [&](auto arg) {
     src.each(
         [&](int c, int m, const float (&v)[8]) {
@@ -858,25 +860,12 @@ __device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n,
         [&](int j, float x) {
           o.put(static_cast<int64_t>(j), __builtin_amdgcn_exp2f(arg(x)) * asc);
         });
-    __syncthreads();
-    for (int k = threadIdx.x; k < K; k += NTH) {
-      const int j = idx[k];
-      if (j < 0) continue;
-      float w = q[k];
-      bool first = true;
-      if (twice) {
-        w = 0.0f;
-        for (int i = 0; i < K; ++i) {
-          const bool same = idx[i] == j;
-          first = first && !(same && i < k);
-          w += same ? q[i] : 0.0f;
-        }
-      }
-      if (first)
-        o.put(static_cast<int64_t>(j),
-              __builtin_amdgcn_exp2f(arg(src.row.at(j))) * bsc - w * sc);
-    }
   });
+  __syncthreads();
+  for (int k = threadIdx.x; k < K; k += NTH) {
+    const float w = g[k];
+    if (w != kAbsent) o.put(static_cast<int64_t>(idx[k]), w * sc);
+  }
 }
 
 // GRAD: the row's gradient too while its logits are at hand, times scale[0] (T / count); as fp16
@@ -900,6 +889,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   __syncthreads();
   double q[2], logq[2], rest = 0.0, total = 0.0;
   float x[2];
+  bool only[2];  // a listed word's first mark, where marks are exact
   bool some = false, wrong = false;
   if (tid < 64) {
     double u[2];
@@ -908,6 +898,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
       const int k = tid + 64 * h;
       u[h] = -INFINITY;
       x[h] = 0.0f;
+      only[h] = false;
       int j = -1;
       if (k < K) {
         const int64_t at = tokens[r * K + k];
@@ -922,7 +913,8 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
             x[h] = row.at(at);
             const uint32_t bit = static_cast<uint32_t>(j + pad_of(row.head)) %
                                  (static_cast<uint32_t>(words) * 32);
-            if (atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1) te.twice = 1;
+            only[h] = !(atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1);
+            if (!only[h]) te.twice = 1;
           }
         }
         te.idx[k] = j;
@@ -944,6 +936,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
       const int k = tid + 64 * h;
       logq[h] = u[h] - norm;
       q[h] = k < K && te.idx[k] >= 0 ? exp(logq[h]) : 0.0;
+      if (k < K) te.q[k] = q[h];
       all += q[h];
     }
     total = wave_sum_d(all);
@@ -954,56 +947,89 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   const Norm a = norm_of<NTH, REST>(src, sc.c, reinterpret_cast<const uint8_t*>(bits), sh,
                                     [](int, float) {}, [](int, float) {});
   if (tid < 64) {
-    const bool empty = a.empty();
-    const double ln_s = a.ln_s(sc.delta);
+    bool empty = a.empty();
+    const double ln_s = empty ? 0.0 : a.ln_s(sc.delta);
+    // Of the whole row's sum: the logit it is relative to and its logarithm.
+    double at = 0.0, ln_all = 0.0, ln_rest = 0.0;
+    if constexpr (REST) {
+      at = empty ? -INFINITY : a.safe ? a.r : a.r * kLn2 / sc.inv_t;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (only[h]) at = fmax(at, static_cast<double>(x[h]));
+      at = wave_max_d(at);
+      const double off = a.ln_sum(at, sc.inv_t, ln_s);
+      double sum = 0.0;
+      bool nan = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!only[h]) continue;
+        sum += exp((x[h] - at) * sc.inv_t);
+        nan = nan || x[h] != x[h];
+      }
+      sum = wave_sum_d(sum) + exp(off);
+      empty = at == -INFINITY && !__any(nan);
+      ln_all = log(sum);
+      ln_rest = off - ln_all;
+    }
+    double logp[2];
     double part = 0.0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const double logp = a.logp(x[h], sc.inv_t, ln_s);
-      if (q[h] != 0.0) part += q[h] * (logq[h] - logp);
+      if constexpr (REST) logp[h] = empty ? -INFINITY : (x[h] - at) * sc.inv_t - ln_all;
+      else logp[h] = a.logp(x[h], sc.inv_t, ln_s);
+      if (q[h] != 0.0) part += q[h] * (logq[h] - logp[h]);
     }
     double l = wave_sum_d(part);
+    // e_j a at the words off the list (without the rest: at all).
+    float ca = 0.0f;
     if constexpr (REST) {
-      // A rest that the student's mask or a list of all tokens leaves no room for is left out.
-      rest = rest > 0.0 && a.rest != 0.0 ? rest : 0.0;
-      if (rest != 0.0) l += rest * (log(rest) - log(a.rest) + ln_s);
+      rest = rest > 0.0 && !a.empty() && !(ln_rest <= kLeast) ? rest : 0.0;
+      if (rest != 0.0) l += rest * (log(rest) - ln_rest);
       total += rest;
+      if (!a.empty()) ca = static_cast<float>(exp(-ln_s) * (exp(ln_rest) * total - rest));
+    } else {
+      if (!empty) ca = static_cast<float>(exp(-ln_s) * total);
     }
-    float b = empty ? 0.0f : static_cast<float>(total / a.s);
-    float ca = b;
-    if constexpr (REST) {
-      if (rest != 0.0) ca = static_cast<float>(total / a.s - rest / a.rest);
-    }
-    if (!some) b = ca = 0.0f, l = 0.0;
-    if (wrong) b = ca = NAN, l = NAN;
+    if (!some) ca = 0.0f, l = 0.0;
+    if (wrong) ca = NAN, l = NAN;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = tid + 64 * h;
-      if (k < K) {
-        // A row without a finite logit has no gradient.
-        const float w = te.idx[k] < 0 ? -1.0f : empty ? 0.0f : static_cast<float>(q[h]);
-        te.q[k] = w;
-        if (weights) weights[r * K + k] = w;
+      if (k >= K) continue;
+      const int j = te.idx[k];
+      double w = q[h];
+      bool first = j >= 0;
+      if (te.twice) {
+        w = 0.0;
+        for (int i = 0; i < K; ++i) {
+          const bool same = te.idx[i] == j;
+          first = first && !(same && i < k);
+          w += same ? te.q[i] : 0.0;
+        }
       }
+      // A row without a finite logit has no gradient.
+      te.g[k] = !first  ? kAbsent
+                : wrong ? NAN
+                : empty ? 0.0f
+                        : static_cast<float>(exp(logp[h]) * total - w);
+      if (weights) weights[r * K + k] = te.g[k];
     }
     if (tid == 0) {
       if (wrong) atomicOr(err, kErrToken);
       loss[2 * r] = static_cast<float>(l);
       loss[2 * r + 1] = some || wrong ? 1.0f : 0.0f;
       if (coef) {
-        coef[4 * r] = a.r;
-        coef[4 * r + 1] = ca;
-        coef[4 * r + 2] = b;
-        coef[4 * r + 3] = (te.twice ? 1.0f : 0.0f) + (a.safe ? 2.0f : 0.0f);
+        coef[3 * r] = a.r;
+        coef[3 * r + 1] = ca;
+        coef[3 * r + 2] = a.safe ? 1.0f : 0.0f;
       }
       te.a = ca;
-      te.b = b;
     }
   }
   if constexpr (GRAD) {
     __syncthreads();
-    distill_grad<NTH>(src, K, a, sc.c, KIND == kHalf ? kHalfScale : scale[0], te.a, te.b,
-                      te.twice != 0, te.idx, te.q, out_row<E, KIND>(out, r, ldo, 0, row.head));
+    distill_grad<NTH>(src, K, a, sc.c, KIND == kHalf ? kHalfScale : scale[0], te.a, te.idx, te.g,
+                      out_row<E, KIND>(out, r, ldo, 0, row.head));
   }
 }
 
@@ -1013,20 +1039,11 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
     float c, const float* __restrict__ coef, const float* __restrict__ weights,
     const float* __restrict__ scale, const float* __restrict__ grad, int done, E* __restrict__ out) {
   if (done && grad[0] == 1.0f) return;  // the rows are there
-  __shared__ int idx[kMaxTop];
-  __shared__ float q[kMaxTop];
   const size_t r = blockIdx.x;
-  for (int k = threadIdx.x; k < K; k += NTH) {
-    const float w = weights[r * K + k];
-    q[k] = w;
-    idx[k] = w < 0.0f ? -1 : static_cast<int>(tokens[r * K + k]);  // a NaN weight is listed
-  }
-  const int flags = static_cast<int>(coef[4 * r + 3]);
-  const Norm n{coef[4 * r], 1.0f, 0.0f, 0.0f, (flags & 2) != 0};
+  const Norm n{coef[3 * r], 1.0f, 0.0f, coef[3 * r + 2] != 0.0f};
   const Row<E, false, true> row(logits + r * ldl, nullptr, V);
-  distill_grad<NTH>(source<NTH, 0>(row), K, n, c, scale[0] * grad[0],
-                    coef[4 * r + 1], coef[4 * r + 2], (flags & 1) != 0, idx, q,
-                    RowOut<E>{out + r * V, row.head});
+  distill_grad<NTH>(source<NTH, 0>(row), K, n, c, scale[0] * grad[0], coef[3 * r + 1],
+                    tokens + r * K, weights + r * K, RowOut<E>{out + r * V, row.head});
 }
 
 // ---- rows of few words ---------------------------------------------------------------------
@@ -1092,21 +1109,26 @@ struct Narrow {
       x[i] = j < V ? ld(p, j) + (bias ? bf2f(bias[j]) : 0.0f) : -INFINITY;
     }
   }
-  // The exponentials (in place of the values), their sums relative to the row's largest logit.
-  __device__ __forceinline__ Norm norm(float c, float (&e)[NV]) const {
-    float m = x[0];
+  // The sums of the exponentials relative to the row's largest logit; off: of the words that are
+  // not listed.
+  template <typename Off>
+  __device__ __forceinline__ Norm norm(float c, Off off) const {
+    float m = kLowest;
 #pragma unroll
-    for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
-    m = fmaxf(max16(m), kLowest);
+    for (int i = 0; i < NV; ++i) m = off(i) ? fmaxf(m, x[i]) : m;
+    m = max16(m);
     float s = 0.0f, u = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float a = Share<true>::arg(x[i], m, c);
-      e[i] = __builtin_amdgcn_exp2f(a);
-      s += e[i];
-      u = __builtin_fmaf(e[i], fmaxf(a, -1e30f), u);
+      const float a = Share<true>::arg(off(i) ? x[i] : -INFINITY, m, c);
+      const float e = __builtin_amdgcn_exp2f(a);
+      s += e;
+      u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);
     }
-    return Norm{m, sum16(s), sum16(u), 0.0f, true};
+    return Norm{m, sum16(s), sum16(u), true};
+  }
+  __device__ __forceinline__ Norm norm(float c) const {
+    return norm(c, [](int) { return true; });
   }
 };
 
@@ -1118,8 +1140,7 @@ __global__ void __launch_bounds__(256) logprobs_narrow_kernel(
     float* __restrict__ top_lp, int64_t* __restrict__ top_idx, uint32_t* err) {
   __shared__ __attribute__((aligned(16))) uint32_t keys[16][16 * NV];
   const Narrow<E, NV> w(rows, V, ldl, logits, bias);
-  float e[NV];
-  const Norm n = w.norm(k.c, e);
+  const Norm n = w.norm(k.c);
   const double log_s = log(n.s), ln_s = log_s + n.correction(k.delta);
   auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
   if (w.live && w.lane == 0) {
@@ -1192,7 +1213,7 @@ __global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
     int64_t plane) {
   const Narrow<E, NV> w(rows, V, ldl, logits, bias);
   const float inv_t = static_cast<float>(k.inv_t);
-  const Norm n{stats[2 * w.r], fabsf(stats[2 * w.r + 1]), 0.0f, 0.0f, stats[2 * w.r + 1] < 0.0f};
+  const Norm n{stats[2 * w.r], fabsf(stats[2 * w.r + 1]), 0.0f, stats[2 * w.r + 1] < 0.0f};
   const int64_t t = targets && g_lp ? targets[w.r] : ignore;
   const bool off = t != ignore && (t < 0 || t >= V), aim = t != ignore && !off;
   const float gl = aim ? g_lp[w.r] * inv_t : 0.0f;
@@ -1224,126 +1245,137 @@ __global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
   }
 }
 
-// The list of a row: its words and weights, in shared memory.
-struct NarrowList {
-  int idx[kMaxTop];  // -1: absent
-  float q[kMaxTop];
-};
-// Which of a lane's words are listed, and with what weights in sum.
-template <int NV>
-__device__ __forceinline__ void listed16(const NarrowList& l, int K, int lane, bool (&hit)[NV],
-                                         float (&q)[NV]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    hit[i] = false;
-    q[i] = 0.0f;
-  }
-  for (int k = 0; k < K; ++k) {
-    const int j = l.idx[k];
-    const float w = l.q[k];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool same = j == lane + 16 * i;
-      hit[i] = hit[i] || same;
-      q[i] += same ? w : 0.0f;
-    }
-  }
-}
-
+// A listed word twice is found by its bit; then the list is gone through for each of its places.
 template <typename E, int NV, bool REST>
 __global__ void __launch_bounds__(256) distill_narrow_kernel(
     int64_t rows, int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
     int K, int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
     int64_t ignore, Scale sc, const float* __restrict__ teacher_lse, float* __restrict__ loss,
     float* __restrict__ coef, float* __restrict__ weights, uint32_t* err) {
-  __shared__ NarrowList lists[16];
+  constexpr int kEntries = kMaxTop / 16;  // a lane's: lane, lane + 16, ...
+  __shared__ int lists[16][kMaxTop];      // -1: absent
   __shared__ float xs[16][16 * NV];
+  __shared__ uint32_t marks[16][kNarrow / 32];
   const Narrow<E, NV> w(rows, V, ldl, logits, bias);
   const int g = threadIdx.x >> 4;
-  NarrowList& l = lists[g];
 #pragma unroll
   for (int i = 0; i < NV; ++i) xs[g][w.lane + 16 * i] = w.x[i];
-  // The row's entries lane, lane + 16, ...: the largest value, then the weights.
+  if (w.lane < kNarrow / 32) marks[g][w.lane] = 0;
+  __syncthreads();
+  auto value = [&](int k) {
+    return value_type == kBF16 ? ld(static_cast<const bf16*>(values), w.r * K + k)
+                               : ld(static_cast<const float*>(values), w.r * K + k);
+  };
   float top = -INFINITY;
   float flags = 0.0f;  // 1: an entry, 1024: one out of range
-  for (int k = w.lane; k < K; k += 16) {
+  float twice = 0.0f;
+  float val[kEntries];
+  int word[kEntries];
+#pragma unroll
+  for (int i = 0; i < kEntries; ++i) {
+    const int k = w.lane + 16 * i;
+    word[i] = -1;
+    val[i] = 0.0f;
+    if (k >= K) continue;
     const int64_t at = tokens[w.r * K + k];
-    const float v = value_type == kBF16 ? ld(static_cast<const bf16*>(values), w.r * K + k)
-                                        : ld(static_cast<const float*>(values), w.r * K + k);
-    int j = -1;
+    val[i] = value(k);
     if (at != ignore) {
       if (at < 0 || at >= V) {
         flags += 1024.0f;
-      } else if (v != -INFINITY) {
-        j = static_cast<int>(at);
+      } else if (val[i] != -INFINITY) {
+        const int j = static_cast<int>(at);
+        word[i] = j;
         flags += 1.0f;
-        top = fmaxf(top, v);
+        top = fmaxf(top, val[i]);
+        if (atomicOr(&marks[g][j >> 5], 1u << (j & 31)) >> (j & 31) & 1) twice = 1.0f;
       }
     }
-    l.idx[k] = j;
-    l.q[k] = v;
+    lists[g][k] = word[i];
   }
   flags = sum16(flags);
   top = max16(top);
-  float e[NV];
-  Norm n = w.norm(sc.c, e);
+  twice = max16(twice);
+  __syncthreads();  // the words, their marks
+  const Norm n = w.norm(sc.c);
   double norm;
   if constexpr (REST) {
     norm = teacher_lse[w.r];
   } else {
     double all = 0.0;
-    for (int k = w.lane; k < K; k += 16)
-      if (l.idx[k] >= 0) all += exp((static_cast<double>(l.q[k]) - top) * sc.inv_t);
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i)
+      if (word[i] >= 0) all += exp((static_cast<double>(val[i]) - top) * sc.inv_t);
     norm = top * sc.inv_t + log(sum16_d(all));
   }
-  __syncthreads();  // xs
   const double ln_s = n.ln_s(sc.delta);
   double part = 0.0, total = 0.0;
-  for (int k = w.lane; k < K; k += 16) {
-    const int j = l.idx[k];
-    float q32 = -1.0f;
-    if (j >= 0) {
-      const double logq = l.q[k] * sc.inv_t - norm, q = exp(logq);
-      if (q != 0.0) part += q * (logq - n.logp(xs[g][j], sc.inv_t, ln_s));
-      total += q;
-      q32 = n.empty() ? 0.0f : static_cast<float>(q);  // no finite logit: no gradient
-    }
-    l.q[k] = q32;
-    if (weights && w.live) weights[w.r * K + k] = q32;
+  double q[kEntries], logp[kEntries];
+#pragma unroll
+  for (int i = 0; i < kEntries; ++i) {
+    q[i] = logp[i] = 0.0;
+    if (word[i] < 0) continue;
+    const double logq = val[i] * sc.inv_t - norm;
+    q[i] = exp(logq);
+    logp[i] = n.logp(xs[g][word[i]], sc.inv_t, ln_s);
+    if (q[i] != 0.0) part += q[i] * (logq - logp[i]);
+    total += q[i];
   }
   part = sum16_d(part);
   total = sum16_d(total);
   const bool wrong = flags >= 1024.0f || total > kMostWeight, some = flags > 0.0f;
-  double rest = 0.0;
+  float r = n.r;
+  double a = n.empty() ? 0.0 : exp(-ln_s) * total;
   if constexpr (REST) {
-    __syncthreads();  // the list
-    bool hit[NV];
-    float q[NV];
-    listed16<NV>(l, K, w.lane, hit, q);
-    float off = 0.0f;
+    uint32_t listed = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) off += hit[i] ? 0.0f : e[i];
-    n.rest = sum16(off);
-    rest = 1.0 - total;
-    rest = rest > 0.0 && n.rest != 0.0 ? rest : 0.0;
-    if (rest != 0.0) part += rest * (log(rest) - log(n.rest) + ln_s);
+    for (int i = 0; i < NV; ++i) {
+      const int j = w.lane + 16 * i;
+      listed |= (marks[g][j >> 5] >> (j & 31) & 1) << i;
+    }
+    const Norm off = w.norm(sc.c, [&](int i) { return !(listed >> i & 1); });
+    const double ln_off = off.ln_s(sc.delta);
+    const double ln_rest = off.ln_sum(n.r, sc.inv_t, ln_off) - ln_s;
+    double rest = 1.0 - total;
+    rest = rest > 0.0 && !off.empty() && !(ln_rest <= kLeast) ? rest : 0.0;
+    if (rest != 0.0) part += rest * (log(rest) - ln_rest);
     total += rest;
+    r = off.r;
+    a = off.empty() ? 0.0 : exp(-ln_off) * (exp(ln_rest) * total - rest);
+  }
+  if (weights && w.live) {
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      const int k = w.lane + 16 * i;
+      if (k >= K) continue;
+      double sum = q[i];
+      bool first = word[i] >= 0;
+      if (first && twice != 0.0f) {
+        sum = 0.0;
+        for (int h = 0; h < K; ++h) {
+          if (lists[g][h] != word[i]) continue;
+          first = first && h >= k;
+          sum += exp(value(h) * sc.inv_t - norm);
+        }
+      }
+      // A row without a finite logit has no gradient.
+      weights[w.r * K + k] = !first      ? kAbsent
+                             : wrong     ? NAN
+                             : n.empty() ? 0.0f
+                                         : static_cast<float>(exp(logp[i]) * total - sum);
+    }
   }
   if (!w.live || w.lane != 0) return;
-  float b = n.empty() ? 0.0f : static_cast<float>(total / n.s), a = b;
-  if (REST && rest != 0.0) a = static_cast<float>(total / n.s - rest / n.rest);
-  if (!some) a = b = 0.0f, part = 0.0;
+  if (!some) a = 0.0, part = 0.0;
   if (wrong) {
-    a = b = NAN, part = NAN;
+    a = NAN, part = NAN;
     atomicOr(err, kErrToken);
   }
   loss[2 * w.r] = static_cast<float>(part);
   loss[2 * w.r + 1] = some || wrong ? 1.0f : 0.0f;
   if (coef) {
-    coef[4 * w.r] = n.r;
-    coef[4 * w.r + 1] = a;
-    coef[4 * w.r + 2] = b;
-    coef[4 * w.r + 3] = 2.0f;  // differences first; the list's order serves words listed twice
+    coef[3 * w.r] = r;
+    coef[3 * w.r + 1] = static_cast<float>(a);
+    coef[3 * w.r + 2] = 1.0f;  // differences first
   }
 }
 
@@ -1353,28 +1385,26 @@ __global__ void __launch_bounds__(256) distill_narrow_bwd_kernel(
     const int64_t* __restrict__ tokens, float c, const float* __restrict__ coef,
     const float* __restrict__ weights, const float* __restrict__ scale,
     const float* __restrict__ grad, E* __restrict__ out) {
-  __shared__ NarrowList lists[16];
+  __shared__ float point[16][16 * NV];  // the listed words' gradients
   const Narrow<E, NV> w(rows, V, ldl, logits, nullptr);
-  NarrowList& l = lists[threadIdx.x >> 4];
+  float* mine = point[threadIdx.x >> 4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) mine[w.lane + 16 * i] = kAbsent;
+  __syncthreads();
   for (int k = w.lane; k < K; k += 16) {
-    const float q = weights[w.r * K + k];
-    l.q[k] = q;
-    l.idx[k] = q < 0.0f ? -1 : static_cast<int>(tokens[w.r * K + k]);
+    const float g = weights[w.r * K + k];
+    if (g != kAbsent) mine[tokens[w.r * K + k]] = g;
   }
   __syncthreads();
-  bool hit[NV];
-  float q[NV];
-  listed16<NV>(l, K, w.lane, hit, q);
-  const float r = coef[4 * w.r], a = coef[4 * w.r + 1], b = coef[4 * w.r + 2];
-  const bool safe = (static_cast<int>(coef[4 * w.r + 3]) & 2) != 0;
+  const float r = coef[3 * w.r], a = coef[3 * w.r + 1];
   const float sc = scale[0] * grad[0];
   if (!w.live) return;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = w.lane + 16 * i;
-    const float arg = safe ? Share<true>::arg(w.x[i], r, c) : Share<false>::arg(w.x[i], r, c);
-    const float e = __builtin_amdgcn_exp2f(arg);
-    if (j < V) st(out, w.r * V + j, hit[i] ? e * (b * sc) - q[i] * sc : e * (a * sc));
+    const float e = __builtin_amdgcn_exp2f(Share<true>::arg(w.x[i], r, c));
+    const float g = mine[j];
+    if (j < V) st(out, w.r * V + j, g != kAbsent ? g * sc : e * (a * sc));
   }
 }
 
@@ -1846,7 +1876,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
       return dabsn_hip_distill(dtype, n, V, past(logits, dtype, s * ldl), ldl, bias, top, value_dtype,
                                past(values, value_dtype, s * top), past(tokens, s * top),
                                ignore_index, temperature, past(teacher_lse, s), past(loss, 2 * s),
-                               past(coef, 4 * s), past(weights, s * top), scale, half,
+                               past(coef, 3 * s), past(weights, s * top), scale, half,
                                past(out, half ? kBF16 : dtype, s * ldo), ldo, err, stream);
     });
   const int nth = threads(rows, V, false);
@@ -1927,7 +1957,7 @@ int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits
   if (rows > kMostRows)
     return in_launches(rows, [&](int64_t s, int64_t n) {
       return dabsn_hip_distill_bwd(dtype, n, V, past(logits, dtype, s * ldl), ldl, top,
-                                   past(tokens, s * top), temperature, past(coef, 4 * s),
+                                   past(tokens, s * top), temperature, past(coef, 3 * s),
                                    past(weights, s * top), scale, grad, done,
                                    past(dlogits, dtype, s * V), stream);
     });

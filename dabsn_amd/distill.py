@@ -14,8 +14,9 @@ p = softmax(x / T), a row's loss is T^2 KL(q || p):
 and the result the mean over the rows that have a listed token. The factor T^2 keeps the
 gradient's size as T grows. Entries whose token is ``ignore_index`` or whose value is -inf are
 absent, so rows of different lists, and padding rows, share one array; a token listed twice
-counts with both weights. The student may rule words out with -inf; the rest is left out where
-the student has no word for it, and a listed word with probability 0 makes the loss inf.
+counts with both weights. The student may rule words out with -inf or a large negative number; the
+rest is left out where the student has no word for it (a mass off the list of 0 in 64 bits, below
+e^-745), and a listed word with probability 0 makes the loss inf.
 
 ``distillation_from_logits`` takes the student's logits, ``chunked_linear_distillation`` the hidden
 rows and the readout's weight and bias, whose logits [N, V] never exist at once.
@@ -77,13 +78,13 @@ class _FromLogits(torch.autograd.Function):
         with vocab.on(x):
             stream = vocab.stream(x)
             word = vocab.ErrorWord(dev)
-            # The rows' losses [n, 2], coefficients [n, 4] and weights [n, K], and the factor.
-            aux = torch.empty(n * (6 + K) + 1 if need else 2 * n, device=dev, dtype=torch.float32)
+            # The rows' losses [n, 2], coefficients [n, 3], listed words' gradients [n, K], and the factor.
+            aux = torch.empty(n * (5 + K) + 1 if need else 2 * n, device=dev, dtype=torch.float32)
             mean = aux.new_empty(())
             loss = aux.data_ptr()
             coef = weights = factor = ready = None
             if need:
-                coef, weights, factor = loss + 8 * n, loss + 24 * n, loss + 4 * n * (6 + K)
+                coef, weights, factor = loss + 8 * n, loss + 20 * n, loss + 4 * n * (5 + K)
             if fused:
                 _counted(values, tokens, ignore, V, loss, t, weight, factor, stream)
                 ready = x.new_empty((n, V))
@@ -119,7 +120,7 @@ class _FromLogits(torch.autograd.Function):
             tk = ops.KernelTimer.begin("distill_bwd", x)
             _lib.check(_lib.load().dabsn_hip_distill_bwd(
                 ops._code(x.dtype), n, V, x.data_ptr(), vocab.row_stride(x), K, tokens.data_ptr(),
-                ctx.t, aux_p + 8 * n, aux_p + 24 * n, aux_p + 4 * n * (6 + K), g.data_ptr(), done,
+                ctx.t, aux_p + 8 * n, aux_p + 20 * n, aux_p + 4 * n * (5 + K), g.data_ptr(), done,
                 out.data_ptr(), vocab.stream(x)), _WHAT + " backward")
             ops.KernelTimer.end(tk)
         return out, None, None, None, None, None, None, None

@@ -17,7 +17,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#define DABSN_HIP_ABI_VERSION 21
+#define DABSN_HIP_ABI_VERSION 22
 
 /* Status codes returned by every entry point. */
 #define DABSN_OK 0
@@ -701,8 +701,9 @@ int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t str
  * absent. q = softmax of values / temperature over the listed ones, or, with teacher_lse (the
  * log-sum-exp of the teacher's whole row / temperature; V <= 480000), exp(values / temperature -
  * teacher_lse) with the rest q_r = 1 - sum q on all other tokens as one event. loss [rows][2] =
- * (KL(q || softmax(z)), 1 if the row has a listed token, else 0). coef [rows][4] and weights
- * [rows][top] (NULL: none) are for _bwd. With out the gradient rows (stride ldo) are written too:
+ * (KL(q || softmax(z)), 1 if the row has a listed token, else 0); q_r is left out where the
+ * student's mass off the list is below e^-745. coef [rows][3] and weights [rows][top] (the listed
+ * words' gradients; NULL: none) are for _bwd. With out the gradient rows (stride ldo) are written too:
  * in the logits' type times scale[0] (no bias), or with `half` (fp32 logits) as fp16 times
  * dabsn_hip_distill_half_scale(). A row whose weights sum to more than 256 (a teacher_lse that is
  * not the row's) counts as one with a token out of range. A listed token outside [0, V) sets *err to 1 and its row to NaN.

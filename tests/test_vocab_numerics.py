@@ -109,3 +109,30 @@ def test_many_masked_rows_with_the_gradient_formed_ahead(cuda_device, fill):
     grad, tol = grad * 6 / 2100, tol * 6 / 2100
     err = (g1[:6].double().cpu() - grad).abs()
     assert bool((err <= tol + 2.0 ** -8 * (grad.abs() + tol) * (1 + 2.0 ** -10) + 2.0 ** -126).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [60, 128, 300, 9001])
+@pytest.mark.parametrize("margin,T", [(80.0, 1.0), (100.0, 1.0), (200.0, 1.0), (600.0, 1.0), (10.0, 0.05),
+                                      (150.0, 0.7)])
+def test_a_student_far_from_the_rest(cuda_device, V, margin, T, dtype):
+    """The words off the list lie ``margin`` logits below the listed ones, where fp32 holds no mass
+    of theirs beside the listed words': the loss still grows with the distance, and their gradient
+    is theirs. Nothing is left out until 64 bits hold the mass as 0 (row 3, 2000 below)."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(5, V, generator=g)
+    tokens = torch.stack([torch.randperm(V, generator=g)[:7] for _ in range(5)])
+    x.scatter_(1, tokens, x.gather(1, tokens) + margin)
+    x[3].scatter_(0, tokens[3], 2000.0 * T)
+    x[4, tokens[4, 0]] = 3 * margin
+    tokens[1, 3] = tokens[1, 2]
+    tokens[2, 4:] = -100
+    x = x.to(dtype).cuda()
+    values = torch.randn(5, 7, generator=g)
+    lse = (torch.logsumexp(values.double() / T, 1) + 0.5).float().cuda()
+    values, tokens = values.cuda(), tokens.cuda()
+    leaf = x.clone().requires_grad_(True)
+    loss = distillation_from_logits(leaf, values, tokens, temperature=T, teacher_lse=lse)
+    (got,) = torch.autograd.grad(loss, leaf)
+    check(loss, got, distill_reference(x, values, tokens, T, lse), dtype)
