@@ -327,6 +327,11 @@ struct Norm {
   __device__ __forceinline__ double ln_s(double delta) const {
     return log(s) + correction(delta);
   }
+  // ln of the sum of e as they are, each 2^(arg delta) short of its own: without what r lacks, which
+  // the factors of e in a gradient have in common.
+  __device__ __forceinline__ double ln_e(double delta) const {
+    return log(s) + kLn2 * delta * u / s;
+  }
   // The correction of ln s and that of the mean of z are the same and cancel.
   __device__ __forceinline__ float entropy(double log_s) const {
     const double h = log_s - kLn2 * u / s;
@@ -986,9 +991,9 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
       rest = rest > 0.0 && !a.empty() && !(ln_rest <= kLeast) ? rest : 0.0;
       if (rest != 0.0) l += rest * (log(rest) - ln_rest);
       total += rest;
-      if (!a.empty()) ca = static_cast<float>(exp(-ln_s) * (exp(ln_rest) * total - rest));
+      if (!a.empty()) ca = static_cast<float>(exp(-a.ln_e(sc.delta)) * (exp(ln_rest) * total - rest));
     } else {
-      if (!empty) ca = static_cast<float>(exp(-ln_s) * total);
+      if (!empty) ca = static_cast<float>(exp(-a.ln_e(sc.delta)) * total);
     }
     if (!some) ca = 0.0f, l = 0.0;
     if (wrong) ca = NAN, l = NAN;

@@ -10,7 +10,7 @@ import torch
 
 from dabsn_amd import distillation_from_logits, token_logprobs
 from test_distill import check, reference as distill_reference
-from test_scoring import check_forward, check_grad, logits_of, reference_grad
+from test_scoring import U, check_forward, check_grad, logits_of, reference_grad, sum_error
 
 INF = math.inf
 FILLS = [-1e9, -1e10, -1e20, -1e30, "lowest", -6e7, -4e7]
@@ -136,3 +136,37 @@ def test_a_student_far_from_the_rest(cuda_device, V, margin, T, dtype):
     loss = distillation_from_logits(leaf, values, tokens, temperature=T, teacher_lse=lse)
     (got,) = torch.autograd.grad(loss, leaf)
     check(loss, got, distill_reference(x, values, tokens, T, lse), dtype)
+
+
+def far_case(V, T, rest):
+    """Logits around 3000 and a teacher near them."""
+    g = torch.Generator().manual_seed(V)
+    x = 3000 + torch.randn(4, V, generator=g)
+    teacher = x + 0.5 * torch.randn(4, V, generator=g)
+    values, tokens = teacher.topk(8, dim=1)
+    lse = (torch.logsumexp(teacher.double() / T, 1).float() + 0.01).cuda() if rest else None
+    return x.cuda(), values.cuda(), tokens.cuda(), lse
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("T", [1.0, 2.0])
+@pytest.mark.parametrize("V", [50, 300, 9001])
+def test_gradients_of_logits_far_from_zero(cuda_device, V, T, rest):
+    """Off the list p_j a, p off by u (3 spread + S + 32) of itself (S = ``sum_error``) wherever the
+    logits lie: log2 e / T is rounded by 1e-8 of itself, which at 3000 alone would be 4e-5."""
+    x, values, tokens, lse = far_case(V, T, rest)
+    leaf = x.clone().requires_grad_(True)
+    loss = distillation_from_logits(leaf, values, tokens, temperature=T, teacher_lse=lse)
+    (got,) = torch.autograd.grad(loss, leaf)
+    _, grad, _, _ = distill_reference(x, values, tokens, T, lse)
+    z = x.double().cpu() / T
+    tol = U * (3 * float(z.amax() - z.amin()) + sum_error(V) + 32)
+    err = (got.double().cpu() - grad).abs() / (T / 4)
+    p = torch.softmax(z, 1)
+    scale = grad.abs() / (T / 4)
+    listed = torch.zeros_like(p, dtype=torch.bool).scatter_(1, tokens.cpu(), True)
+    if rest:  # a = Q - q_r / p_r, a difference
+        left = torch.where(listed, 0.0, p).sum(1, keepdim=True)
+        scale = scale + 2 * p / left
+    assert bool((err <= tol * scale + 2 * U * scale)[~listed].all())
