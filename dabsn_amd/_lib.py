@@ -168,17 +168,17 @@ _SIGNATURES = {
     "dabsn_hip_ce_bias": ([i64, i64, vp, i32, vp, vp], i32),
     "dabsn_hip_ce_join": ([i64, vp, vp, vp], i32),
     "dabsn_hip_token_logprobs": (
-        [i32, i64, i64, vp, i64, vp, vp, i64, ctypes.c_float, i64] + [vp] * 7, i32),
+        [i32, i64, i64, vp, i64, vp, vp, i64, ctypes.c_double, i64] + [vp] * 7, i32),
     "dabsn_hip_token_logprobs_bwd": (
-        [i32, i64, i64, vp, i64, vp, vp, i64, ctypes.c_float, i64] + [vp] * 7 + [i64, i64, vp],
+        [i32, i64, i64, vp, i64, vp, vp, i64, ctypes.c_double, i64] + [vp] * 7 + [i64, i64, vp],
         i32),
     "dabsn_hip_distill_rows": ([i64, i64, i64, i32, vp, vp, i64, vp, vp], i32),
-    "dabsn_hip_distill_mean": ([i64, vp, ctypes.c_float, ctypes.c_float, vp, vp, vp], i32),
+    "dabsn_hip_distill_mean": ([i64, vp, ctypes.c_double, ctypes.c_double, vp, vp, vp], i32),
     "dabsn_hip_distill": (
-        [i32, i64, i64, vp, i64, vp, i64, i32, vp, vp, i64, ctypes.c_float, vp, vp, vp, vp, vp, i32,
+        [i32, i64, i64, vp, i64, vp, i64, i32, vp, vp, i64, ctypes.c_double, vp, vp, vp, vp, vp, i32,
          vp, i64, vp, vp], i32),
     "dabsn_hip_distill_bwd": (
-        [i32, i64, i64, vp, i64, i64, vp, ctypes.c_float, vp, vp, vp, vp, i32, vp, vp], i32),
+        [i32, i64, i64, vp, i64, i64, vp, ctypes.c_double, vp, vp, vp, vp, i32, vp, vp], i32),
     "dabsn_hip_column_sums_partials": ([i64, i64], sz),
     "dabsn_hip_column_sums": ([i32, i64, i64, i64, vp, i32, vp, vp, vp], i32),
     "dabsn_hip_half_copy": ([i64, vp, vp, vp, vp, vp], i32),

@@ -352,9 +352,9 @@ struct Scale {
   double inv_t, delta;
   float c;
 };
-static Scale scale_of(float t) {
+static Scale scale_of(double t) {
   Scale k;
-  k.inv_t = 1.0 / static_cast<double>(t);
+  k.inv_t = 1.0 / t;
   k.c = static_cast<float>(k.inv_t / kLn2);
   k.delta = k.inv_t / kLn2 / static_cast<double>(k.c) - 1.0;
   return k;
@@ -1444,7 +1444,7 @@ __global__ void __launch_bounds__(256) distill_parts_kernel(int64_t rows, float*
 // over the rows r = 0, step, ...; the sums in 64 bits and a fixed order, one block.
 __global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, int64_t step,
                                                             const float* __restrict__ loss,
-                                                            float t, float weight,
+                                                            double t, double weight,
                                                             float* __restrict__ mean,
                                                             float* __restrict__ factor) {
   __shared__ double sh[2][16];
@@ -1470,7 +1470,7 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(int64_t rows, int64_
       n += sh[1][w];
     }
     n = n < 1.0 ? 1.0 : n;
-    const double wt = static_cast<double>(weight) * t;
+    const double wt = weight * t;
     if (mean) mean[0] = static_cast<float>(wt * t * l / n);
     if (factor) factor[0] = static_cast<float>(wt / n);
   }
@@ -1628,13 +1628,12 @@ __global__ void __launch_bounds__(256) scaled_kernel(int64_t n, const float* __r
   }
 }
 
-static int checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t ldl, float t) {
+static int checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t ldl, double t) {
   DABSN_REQUIRE(dtype == kF32 || dtype == kBF16, "%s: bad dtype %d", what, dtype);
   DABSN_REQUIRE(rows >= 0 && rows < (1ll << 31) && V > 0 && V < (1ll << 31) - 4096 && ldl >= V,
                 "%s: bad shape (rows=%lld, V=%lld, ld=%lld)", what, (long long)rows, (long long)V,
                 (long long)ldl);
-  DABSN_REQUIRE(t >= 1e-6f && t <= 1e6f, "%s: temperature %g lies outside [1e-6, 1e6]", what,
-                static_cast<double>(t));
+  DABSN_REQUIRE(t >= 1e-6 && t <= 1e6, "%s: temperature %g lies outside [1e-6, 1e6]", what, t);
   return DABSN_OK;
 }
 
@@ -1687,7 +1686,7 @@ extern "C" {
 
 int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                              const void* bias, const int64_t* targets, int64_t ignore_index,
-                             float temperature, int64_t top, float* logprob, float* entropy,
+                             double temperature, int64_t top, float* logprob, float* entropy,
                              float* stats, float* top_logprobs, int64_t* top_indices,
                              uint32_t* err, hipStream_t stream) {
   int rc = checks("token log probabilities", dtype, rows, V, ldl, temperature);
@@ -1748,7 +1747,7 @@ int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* log
 
 int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void* logits,
                                  int64_t ldl, const void* bias, const int64_t* targets,
-                                 int64_t ignore_index, float temperature, int64_t top,
+                                 int64_t ignore_index, double temperature, int64_t top,
                                  const int64_t* top_indices, const float* stats,
                                  const float* entropy, const float* g_logprob,
                                  const float* g_entropy, const float* g_top, void* out,
@@ -1814,7 +1813,7 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
 }
 
 static int distill_checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t ldl,
-                          int64_t top, float temperature) {
+                          int64_t top, double temperature) {
   int rc = checks(what, dtype, rows, V, ldl, temperature);
   if (rc != DABSN_OK) return rc;
   DABSN_REQUIRE(top > 0 && top <= kMaxTop, "%s: %lld listed tokens a row (1 to %d)", what,
@@ -1825,7 +1824,7 @@ static int distill_checks(const char* what, int dtype, int64_t rows, int64_t V, 
 int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype,
                            const void* values, const int64_t* tokens, int64_t ignore_index,
                            float* loss, hipStream_t stream) {
-  int rc = distill_checks("distillation rows", kF32, rows, V, V, top, 1.0f);
+  int rc = distill_checks("distillation rows", kF32, rows, V, V, top, 1.0);
   if (rc != DABSN_OK) return rc;
   DABSN_REQUIRE(value_dtype == kF32 || value_dtype == kBF16, "distillation rows: bad dtype %d",
                 value_dtype);
@@ -1843,7 +1842,7 @@ int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype
   return DABSN_OK;
 }
 
-int dabsn_hip_distill_mean(int64_t rows, float* loss, float temperature, float weight, float* mean,
+int dabsn_hip_distill_mean(int64_t rows, float* loss, double temperature, double weight, float* mean,
                            float* factor, hipStream_t stream) {
   DABSN_REQUIRE(rows >= 0 && rows < (1ll << 31) && (rows == 0 || loss) && (mean || factor),
                 "distillation mean: bad arguments");
@@ -1860,7 +1859,7 @@ int dabsn_hip_distill_mean(int64_t rows, float* loss, float temperature, float w
 
 int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                       const void* bias, int64_t top, int value_dtype, const void* values,
-                      const int64_t* tokens, int64_t ignore_index, float temperature,
+                      const int64_t* tokens, int64_t ignore_index, double temperature,
                       const float* teacher_lse, float* loss, float* coef, float* weights,
                       const float* scale, int half, void* out, int64_t ldo, uint32_t* err,
                       hipStream_t stream) {
@@ -1951,7 +1950,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
 }
 
 int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
-                          int64_t top, const int64_t* tokens, float temperature, const float* coef,
+                          int64_t top, const int64_t* tokens, double temperature, const float* coef,
                           const float* weights, const float* scale, const float* grad, int done,
                           void* dlogits, hipStream_t stream) {
   int rc = distill_checks("distillation backward", dtype, rows, V, ldl, top, temperature);

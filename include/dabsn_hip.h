@@ -720,12 +720,12 @@ int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t str
  * s0[0] * s1[0] * s2[0] (NULL: 1), rounded once to dtype. */
 int dabsn_hip_token_logprobs(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                              const void* bias, const int64_t* targets, int64_t ignore_index,
-                             float temperature, int64_t top, float* logprob, float* entropy,
+                             double temperature, int64_t top, float* logprob, float* entropy,
                              float* stats, float* top_logprobs, int64_t* top_indices,
                              uint32_t* err, hipStream_t stream);
 int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void* logits,
                                  int64_t ldl, const void* bias, const int64_t* targets,
-                                 int64_t ignore_index, float temperature, int64_t top,
+                                 int64_t ignore_index, double temperature, int64_t top,
                                  const int64_t* top_indices, const float* stats,
                                  const float* entropy, const float* g_logprob,
                                  const float* g_entropy, const float* g_top, void* out,
@@ -733,16 +733,16 @@ int dabsn_hip_token_logprobs_bwd(int dtype, int64_t rows, int64_t V, const void*
 int dabsn_hip_distill_rows(int64_t rows, int64_t V, int64_t top, int value_dtype,
                            const void* values, const int64_t* tokens, int64_t ignore_index,
                            float* loss, hipStream_t stream);
-int dabsn_hip_distill_mean(int64_t rows, float* loss, float temperature, float weight, float* mean,
+int dabsn_hip_distill_mean(int64_t rows, float* loss, double temperature, double weight, float* mean,
                            float* factor, hipStream_t stream);
 int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                       const void* bias, int64_t top, int value_dtype, const void* values,
-                      const int64_t* tokens, int64_t ignore_index, float temperature,
+                      const int64_t* tokens, int64_t ignore_index, double temperature,
                       const float* teacher_lse, float* loss, float* coef, float* weights,
                       const float* scale, int half, void* out, int64_t ldo, uint32_t* err,
                       hipStream_t stream);
 int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
-                          int64_t top, const int64_t* tokens, float temperature, const float* coef,
+                          int64_t top, const int64_t* tokens, double temperature, const float* coef,
                           const float* weights, const float* scale, const float* grad, int done,
                           void* dlogits, hipStream_t stream);
 size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V);

@@ -170,3 +170,24 @@ def test_gradients_of_logits_far_from_zero(cuda_device, V, T, rest):
         left = torch.where(listed, 0.0, p).sum(1, keepdim=True)
         scale = scale + 2 * p / left
     assert bool((err <= tol * scale + 2 * U * scale)[~listed].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("T", [0.7, 1.1, 3.3])
+@pytest.mark.parametrize("V", [50, 300, 9001])
+def test_the_temperature_has_64_bits(cuda_device, V, T, rest):
+    """Logits around 3000: a temperature rounded to 32 bits (0.7 by 1.7e-8 of itself) would take the
+    teacher's weights off by 1e-5 to 7e-5 of themselves against its normaliser. They are 64-bit values
+    here; the student's log probabilities are off by u (3 spread + S + 32) (S = ``sum_error``)."""
+    x, values, tokens, lse = far_case(V, T, rest)
+    leaf = x.clone().requires_grad_(True)
+    loss = distillation_from_logits(leaf, values, tokens, temperature=T, teacher_lse=lse)
+    (got,) = torch.autograd.grad(loss, leaf)
+    ref, grad, _, _ = distill_reference(x, values, tokens, T, lse)
+    z = x.double().cpu() / T
+    tol = U * (3 * float(z.amax() - z.amin()) + sum_error(V) + 32)
+    assert abs(float(loss.detach()) - ref) <= T * T * tol + 2 * U * ref
+    p = torch.softmax(z, 1)
+    bound = T / 4 * tol * (p + (p - grad * 4 / T).abs()) + 2 * U * grad.abs()
+    assert bool(((got.double().cpu() - grad).abs() <= bound).all())
