@@ -2,23 +2,32 @@
 //
 // Both take rows of logits [rows, V] (or the fp32 logits of a readout before its bias) and a
 // temperature T, z = x / T, and form the row's softmax in one pass, fp32, with a running reference r
-// per thread, e = exp(z - r), s = sum e:
-//   log probabilities   logp_t = z_t - r - ln s;  H = ln s - sum e (z - r) / s;  the K largest
-//                       logits in order (equal ones by index)
+// per thread, e = exp(z - r). With M the row's largest logit:
+//   R = the sum of exp((x - M) / T) over all logits but M itself
+//   log probabilities   logp_t = (x_t - M) / T - ln(1 + R);  H = ln(1 + R) - sum p (z - M / T);
+//                       the K largest logits in order (equal ones by index)
 //   distillation        sum q (ln q - logp) over a teacher's listed tokens and, with the
 //                       teacher's normaliser, over the rest of the vocabulary as one event
 // and a backward that reads the logits once more and writes their gradient.
 //
-// The pass is bound by memory where an element costs few instructions: 8.4 vector instructions here
+// M stays out of the sums: of a token with nearly all the mass log p is
+// -ln(1 + R) with R small, and in a sum that holds the 1 too fp32 would keep R to 2^-24 of 1, not of
+// itself (log p = -1e-4 was off by 1e-3 of itself). So each thread keeps the sums of the group with
+// its largest logit apart from the others', and where R turns out below 1/4 the thread that has M
+// takes that group's again without it. 8192 x 32000 bf16 take 87 us with this and groups of 16, 89 with
+// groups of 8, 82 without; with that group taken again in every row, or the logit itself kept apart
+// and swapped for each larger one, 90 and 93.
+//
+// The pass is bound by memory where an element costs few instructions: 10.2 vector instructions here
 // (counted at 8192 x 32000 bf16), against the 12 that the time of its 2 bytes allows. So the
 // exponent's argument is one fma of the logit, x c - r with c = log2 e / T and r, in units of ln 2,
-// near the thread's maximum (any number does: the result is exact in r); r moves only when a
-// vector exceeds it by 16. c is rounded: the sums u of e (x c - r), which the entropy needs
-// anyhow, give the exact normaliser to first order. The fma leaves what r = x c lost in its own
-// rounding, half an ulp of x c: below 4 up to 2^26, and 2^100 of a mask's -1e30, so r is kept in
-// +-2^26. It starts at the lower end, from where the words that a mask rules out with any large
-// negative number add 0 and move nothing. A row that holds nothing else (s = 0), or whose largest
-// logit passes the upper end, takes the pass again with differences formed first.
+// near the thread's maximum; r moves only when a group exceeds it by 8. c is rounded: the sums u of
+// e (x c - r), which the entropy needs anyhow, give the exact normaliser to first order. The fma
+// leaves what r = x c lost in its own rounding, half an ulp of x c: below 4 up to 2^26, and 2^100 of
+// a mask's -1e30, so r is kept in +-2^26. It starts at the lower end, from where the words that a
+// mask rules out with any large negative number add 0 and move nothing. A row whose largest logit
+// lies beyond half of the lower end or beyond the upper one takes the pass again with differences
+// formed first.
 #include <algorithm>
 
 #include "../../include/dabsn_hip.h"
@@ -120,14 +129,14 @@ struct Row {
   }
 };
 
-// A row's logits as its threads go through them: each(f, g) calls f(c, n, values) for groups of 8
-// values, the vector c and (fp32) the vector c + NTH, of which n are the row's (-inf stands for a
+// A row's logits as its threads go through them: each(f, g) calls f(c, n, values) for groups of P =
+// 8 or 16 values, the vectors c, c + NTH, ... of which the first n are the row's (-inf stands for a
 // missing one's values); then g(column, value) for the logits outside the vectors. What a group
-// costs beside its logits (its largest, the reference's test) is shared by 8 of them.
-template <int NTH, typename R>
+// costs beside its logits (its largest, the reference's test) is shared by P of them.
+template <int NTH, int P_, typename R>
 struct Group {
-  static constexpr int W = R::W, G = 8 / W;
-  static __device__ __forceinline__ void values(const typename R::Raw (&raw)[G], int n, float (&v)[8]) {
+  static constexpr int P = P_, W = R::W, G = P / W;
+  static __device__ __forceinline__ void values(const typename R::Raw (&raw)[G], int n, float (&v)[P]) {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float w[W];
@@ -136,25 +145,33 @@ struct Group {
       for (int k = 0; k < W; ++k) v[g * W + k] = g < n ? w[k] : -INFINITY;
     }
   }
+  // How many of the group's vectors are among nv.
+  static __device__ __forceinline__ int count(int c, int nv) {
+    int n = 1;
+#pragma unroll
+    for (int g = 1; g < G; ++g) n += c + g * NTH < nv;
+    return n;
+  }
   // The group that starts at vector c.
   template <typename F>
   static __device__ __forceinline__ void last(const typename R::Raw (&raw)[G], int c, int nv, F f) {
     if (c >= nv) return;
-    const int n = G == 2 && c + NTH >= nv ? 1 : G;
-    float v[8];
+    const int n = count(c, nv);
+    float v[P];
     values(raw, n, v);
     f(c, n, v);
   }
 };
-// Streamed: from memory each time, four groups' loads in flight.
-template <int NTH, typename R>
+// Streamed: from memory each time, 32 values' loads in flight.
+template <int NTH, int P_, typename R_>
 struct Streamed {
+  using R = R_;
   const R& row;
-  static constexpr int W = R::W;
+  static constexpr int P = P_, W = R::W;
   template <typename F, typename H>
   __device__ __forceinline__ void each(F f, H h) const {
-    using Gr = Group<NTH, R>;
-    constexpr int G = Gr::G, U = 4;
+    using Gr = Group<NTH, P, R>;
+    constexpr int G = Gr::G, U = 32 / P;
     const int nv = row.vectors(), tid = threadIdx.x;
     int b = 0;  // the block's first vector
     for (; b + U * G * NTH <= nv; b += U * G * NTH) {
@@ -163,7 +180,7 @@ struct Streamed {
       for (int k = 0; k < U * G; ++k) raw[k / G][k % G] = row.load(b + k * NTH + tid);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        float v[8];
+        float v[P];
         Gr::values(raw[k], G, v);
         f(b + k * G * NTH + tid, G, v);
       }
@@ -184,10 +201,11 @@ struct Streamed {
 // Held: loaded once into NV vectors of registers a thread (at most NTH NV vectors), for a row that
 // is read twice and written: the second reading otherwise comes from the memory side, as the rows
 // under way (2,048 of 64 KB) are far more than the L2 caches hold.
-template <int NTH, int NV, typename R>
+template <int NTH, int NV, typename R_>
 struct Held {
-  using Gr = Group<NTH, R>;
-  static constexpr int W = R::W, G = Gr::G;
+  using R = R_;
+  using Gr = Group<NTH, 8, R>;
+  static constexpr int P = 8, W = R::W, G = Gr::G;
   const R& row;
   typename R::Raw raw[NV / G][G];
   __device__ __forceinline__ explicit Held(const R& row_) : row(row_) {
@@ -205,10 +223,10 @@ struct Held {
   }
 };
 // NV = 0: streamed.
-template <int NTH, int NV, typename R>
+template <int NTH, int NV, int P = 8, typename R>
 __device__ __forceinline__ auto source(const R& row) {
   if constexpr (NV > 0) return Held<NTH, NV, R>(row);
-  else return Streamed<NTH, R>{row};
+  else return Streamed<NTH, P, R>{row};
 }
 
 // Of a quiet NaN and a number the number; fmaxf adds an instruction an operand to quiet others.
@@ -217,8 +235,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-__device__ __forceinline__ float largest(const float (&v)[8]) {
-  return max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[7]));
+template <int P>
+__device__ __forceinline__ float largest(const float (&v)[P]) {
+  float m = max3(v[0], v[1], v[2]);
+#pragma unroll
+  for (int k = 3; k + 1 < P; k += 2) m = max3(m, v[k], v[k + 1]);
+  return max3(m, v[P - 1], v[P - 1]);
 }
 
 // The sum over the block of N values a thread, to every thread; the waves' sums are added in 64
@@ -255,63 +277,114 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
   }
   return v;
 }
+// The first thread of the block for which `mine` is true.
+template <int NTH>
+__device__ __forceinline__ int block_first(bool mine, float* sh) {
+  if constexpr (NTH == 64) return __ffsll(static_cast<unsigned long long>(__ballot(mine))) - 1;
+  int* word = reinterpret_cast<int*>(sh);
+  __syncthreads();
+  if (threadIdx.x == 0) *word = NTH;
+  __syncthreads();
+  if (mine) atomicMin(word, static_cast<int>(threadIdx.x));
+  __syncthreads();
+  return *word;
+}
 
-// A thread's share of a row relative to its reference r: s = sum e, u = sum e arg with
-// e = 2^arg. arg = x c - r; SAFE rows have arg = (x - r) c. Logits of -inf give e = 0; NaN and +inf
-// make s NaN.
+// A thread's share of a row, relative to its reference r: sums of e = 2^arg and of e arg, of the
+// group with its largest logit (at: its first vector, -1: a logit of its own) apart from the others.
+// arg = x c - r; SAFE rows have arg = (x - r) c. Logits of -inf give e = 0; NaN makes a sum NaN.
 constexpr float kFar = 67108864.0f;  // 2^26
 template <bool SAFE>
 struct Share {
-  float r = SAFE ? kLowest : -kFar, s = 0.0f, u = 0.0f;
+  static constexpr float kFloor = SAFE ? kLowest : -kFar;
+  float best = -INFINITY, r = kFloor;
+  float s = 0.0f, u = 0.0f, sb = 0.0f, ub = 0.0f;
+  int at = -1;
   float c;
   __device__ __forceinline__ explicit Share(float c_) : c(c_) {}
   static __device__ __forceinline__ float arg(float x, float r, float c) {
     return SAFE ? (x - r) * c : __builtin_fmaf(x, c, -r);
   }
-  // The reference becomes `to`.
-  __device__ __forceinline__ void raise(float to) {
-    const float d = r == to ? 0.0f : SAFE ? (r - to) * c : r - to;  // both may be inf
+  // The reference of a largest logit.
+  __device__ __forceinline__ float place(float x) const { return fmaxf(SAFE ? x : x * c, kFloor); }
+  // From the reference `from` to a larger one.
+  __device__ __forceinline__ float shift(float from, float to) const {
+    return from == to ? 0.0f : SAFE ? (from - to) * c : from - to;  // both may be inf
+  }
+  static __device__ __forceinline__ void scale(float d, float& s, float& u) {
     const float f = __builtin_amdgcn_exp2f(d);
     u = f == 0.0f ? 0.0f : f * (u + d * s);
     s *= f;
+  }
+  __device__ __forceinline__ void raise(float to) {
+    const float d = shift(r, to);
+    scale(d, s, u);
+    scale(d, sb, ub);
     r = to;
   }
-  __device__ __forceinline__ void see(float largest) {
-    const float t = SAFE ? largest : largest * c;
-    if (t > (SAFE ? r : r + 16.0f)) raise(t);
+  template <int N>
+  __device__ __forceinline__ void fold(const float (&v)[N], float vm, int k) {
+    const float t = SAFE ? vm : vm * c;
+    if (t > (SAFE ? r : r + 8.0f)) raise(t);
+    float vs = 0.0f, vu = 0.0f;
+    add<N>(v, -1, vs, vu);
+    const bool up = vm > best;
+    s += up ? sb : vs;
+    u += up ? ub : vu;
+    sb = up ? vs : sb;
+    ub = up ? vu : ub;
+    at = up ? k : at;
+    best = up ? vm : best;
   }
-  __device__ __forceinline__ void fold(const float (&v)[8], float vm) {
-    see(vm);
-    float vs = 0.0f;
+  // Adds all but the `without`th.
+  template <int N>
+  __device__ __forceinline__ void add(const float (&v)[N], int without, float& vs, float& vu) const {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float a = arg(v[k], r, c);
+    for (int k = 0; k < N; ++k) {
+      const float a = arg(k == without ? -INFINITY : v[k], r, c);
       const float e = __builtin_amdgcn_exp2f(a);
       vs += e;
-      u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);  // arg = -inf has e = 0
+      vu = __builtin_fmaf(e, fmaxf(a, -1e30f), vu);  // arg = -inf has e = 0
     }
-    s += vs;
   }
   __device__ __forceinline__ void fold1(float x) {
-    see(x);
-    const float a = arg(x, r, c), e = __builtin_amdgcn_exp2f(a);
-    s += e;
-    u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);
+    const float v[1] = {x};
+    fold(v, x, -1);
   }
-  // The block's shares as one: s and u.
-  template <int NTH>
-  __device__ __forceinline__ void join(double (&sum)[2], float* sh) {
-    raise(block_max<NTH>(r, sh));
-    float v[2] = {s, u};
-    block_sums<NTH, 2>(v, sum, sh);
+  // The block's shares as one: m, the row's largest logit, r its place, and the sums of the others.
+  // group(k, v): the group whose first vector is k. sh: 2 * NTH/64 floats.
+  template <int NTH, int P, typename Group>
+  __device__ __forceinline__ void join(Group group, float& m, double (&sum)[2], float* sh) {
+    m = block_max<NTH>(best, sh);
+    raise(place(m));
+    float all[2] = {s + sb, u + ub};
+    block_sums<NTH, 2>(all, sum, sh);
+    const float am = SAFE ? 0.0f : arg(m, r, c), em = __builtin_amdgcn_exp2f(am);  // m's own
+    sum[0] -= em;
+    sum[1] -= static_cast<double>(em) * am;
+    if (sum[0] >= 0.25 || m == -INFINITY) return;
+    if (block_first<NTH>(best == m, sh) == static_cast<int>(threadIdx.x)) {
+      sb = ub = 0.0f;
+      if (at >= 0) {
+        float v[P];
+        group(at, v);
+        int k = P - 1;
+#pragma unroll
+        for (int i = P - 2; i >= 0; --i) k = v[i] == m ? i : k;
+        add<P>(v, k, sb, ub);
+      }
+    }
+    all[0] = s + sb;
+    all[1] = u + ub;
+    block_sums<NTH, 2>(all, sum, sh);
   }
 };
 
 // What a row's pass leaves. Log probabilities are differences of numbers of the size of the
 // logits, so the few of a row are formed in 64 bits.
 struct Norm {
-  float r;
-  double s, u;
+  float m, r;   // the largest logit and its place
+  double s, u;  // sums of the others
   bool safe;
   // f(arg) with the row's form of the exponent's argument as a function of a logit.
   template <typename F>
@@ -319,32 +392,11 @@ struct Norm {
     if (safe) f([r = r, c](float x) { return Share<true>::arg(x, r, c); });
     else f([r = r, c](float x) { return Share<false>::arg(x, r, c); });
   }
-  __device__ __forceinline__ bool empty() const { return s == 0.0; }  // no finite logit
-  // What ln s lacks for the rounding of c (log2 e / T = c (1 + delta)).
-  __device__ __forceinline__ double correction(double delta) const {
-    return kLn2 * delta * (u / s + (safe ? 0.0 : static_cast<double>(r)));
-  }
-  __device__ __forceinline__ double ln_s(double delta) const {
-    return log(s) + correction(delta);
-  }
-  // ln of the sum of e as they are, each 2^(arg delta) short of its own: without what r lacks, which
-  // the factors of e in a gradient have in common.
-  __device__ __forceinline__ double ln_e(double delta) const {
-    return log(s) + kLn2 * delta * u / s;
-  }
-  // The correction of ln s and that of the mean of z are the same and cancel.
-  __device__ __forceinline__ float entropy(double log_s) const {
-    const double h = log_s - kLn2 * u / s;
-    return empty() || h < 0.0 ? 0.0f : static_cast<float>(h);
-  }
-  // ln of the sum of exp((x - at) / T) over the row's logits x.
-  __device__ __forceinline__ double ln_sum(double at, double inv_t, double ln_s) const {
-    if (empty()) return -INFINITY;
-    return safe ? (r - at) * inv_t + ln_s : r * kLn2 - at * inv_t + ln_s;
-  }
-  // log p of a logit x.
-  __device__ __forceinline__ double logp(float x, double inv_t, double ln_s) const {
-    return empty() ? -INFINITY : -ln_sum(static_cast<double>(x), inv_t, ln_s);
+  __device__ __forceinline__ bool nan() const { return s != s || m == INFINITY; }
+  __device__ __forceinline__ bool empty() const { return m == -INFINITY && s == s; }  // no finite logit
+  // arg of the largest: what its place lost in its rounding, exactly.
+  __device__ __forceinline__ float left(float c) const {
+    return safe ? 0.0f : Share<false>::arg(m, r, c);
   }
 };
 // 1 / T, c and its error, from the host.
@@ -359,6 +411,37 @@ static Scale scale_of(double t) {
   k.delta = k.inv_t / kLn2 / static_cast<double>(k.c) - 1.0;
   return k;
 }
+// A row's sums with 1 / T at its full precision, log2 e / T = c (1 + delta): to first order each e is
+// short of the factor 2^(arg delta), and all of 2^-left as M's own e is to be 1.
+struct Sums {
+  double at, inv_t;  // M; 1 / T
+  double ln;         // ln(1 + R)
+  double h;          // the entropy
+  float left;
+  bool empty;
+  __device__ __forceinline__ Sums(const Norm& n, const Scale& k)
+      : at(n.m), inv_t(k.inv_t), left(n.left(k.c)), empty(n.empty()) {
+    const double f = __builtin_amdgcn_exp2f(-left);
+    const double R = n.nan() ? NAN : empty ? 0.0 : f * (n.s + kLn2 * k.delta * n.u);
+    const double one = 1.0 + R;
+    ln = one == 1.0 ? R : log(one) * (R / (one - 1.0));  // ln(1 + R) for small R too, after Kahan
+    // sum p (z - M / T) (1 + R); its own correction would need the sum of e arg^2, and what it
+    // lacks, delta |arg| of itself, is an argument's rounding.
+    const double w = empty ? 0.0 : kLn2 * f * (n.u - left * n.s);
+    h = ln - w / one;
+    h = h < 0.0 ? 0.0 : h;
+  }
+  // ln of the sum of exp((x - y) / T) over the row's logits x.
+  __device__ __forceinline__ double ln_sum(double y) const {
+    return empty ? -INFINITY : (at - y) * inv_t + ln;
+  }
+  // log p of a logit x.
+  __device__ __forceinline__ double logp(float x) const {
+    return empty ? -INFINITY : -ln_sum(static_cast<double>(x));
+  }
+  // ln of the sum of all e = 2^arg.
+  __device__ __forceinline__ double ln_e() const { return ln + kLn2 * left; }
+};
 
 __device__ __forceinline__ int pad_of(int head) { return -head & 7; }
 
@@ -369,43 +452,67 @@ __device__ __forceinline__ Norm row_pass(const S& src, float c, const uint8_t* l
   // Bit j + pad of `listed` is column j's: whole vectors start at a multiple of 8 (or 4) bits.
   const int pad = pad_of(src.row.head);
   const uint8_t* body = REST ? listed + (src.row.head + pad) / 8 : nullptr;
+  constexpr int P = S::P;
   Share<SAFE> a(c);
-  src.each(
-      [&](int k, int n, const float (&v)[8]) {
-        if constexpr (REST) {
-          uint32_t bits = 0;
-          if constexpr (S::W == 8) {
-            bits = body[k];
-          } else {
-            auto four = [&](int i) { return body[i >> 1] >> (4 * (i & 1)) & 15u; };
-            bits = four(k) | (n == 2 ? four(k + NTH) << 4 : 0u);
-          }
-          if (bits) {  // few vectors hold a listed word
-            float w[8];
+  // Listed words out of a group's values; whether there is one.
+  static_assert(!REST || P == 8, "a byte of marks a group");
+  auto mask = [&](int k, int n, const float (&v)[P], float (&w)[P]) {
+    uint32_t bits = 0;
+    if constexpr (S::W == 8) {
+      bits = body[k];
+    } else {
+      auto four = [&](int i) { return body[i >> 1] >> (4 * (i & 1)) & 15u; };
+      bits = four(k) | (n == 2 ? four(k + NTH) << 4 : 0u);
+    }
+    if (!bits) return false;  // few vectors hold one
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = (bits >> i & 1) ? -INFINITY : v[i];
-            a.fold(w, largest(w));
+    for (int i = 0; i < P; ++i) w[i] = (bits >> i & 1) ? -INFINITY : v[i];
+    return true;
+  };
+  src.each(
+      [&](int k, int n, const float (&v)[P]) {
+        if constexpr (REST) {
+          float w[P];
+          if (mask(k, n, v, w)) {
+            a.fold(w, largest(w), k);
             return;
           }
         }
         const float vm = largest(v);
-        a.fold(v, vm);
+        a.fold(v, vm, k);
         see(k, vm);
       },
       [&](int j, float x) {
         a.fold1(REST && (listed[(j + pad) >> 3] >> ((j + pad) & 7) & 1) ? -INFINITY : x);
         last(j, x);
       });
+  float m;
   double sum[2];
-  a.template join<NTH>(sum, sh);
-  return Norm{a.r, sum[0], sum[1], SAFE};
+  a.template join<NTH, P>(
+      [&](int k, float (&v)[P]) {
+        using Gr = Group<NTH, P, typename S::R>;
+        typename S::R::Raw raw[Gr::G];
+        const int nv = src.row.vectors(), n = Gr::count(k, nv);
+#pragma unroll
+        for (int g = 0; g < Gr::G; ++g) raw[g] = src.row.load(min(k + g * NTH, nv - 1));
+        Gr::values(raw, n, v);
+        if constexpr (REST) {
+          float w[P];
+          if (mask(k, n, v, w)) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) v[i] = w[i];
+          }
+        }
+      },
+      m, sum, sh);
+  return Norm{m, a.r, sum[0], sum[1], SAFE};
 }
 // The row's norm; `see` gets each group's first vector and largest logit, `last` the logits outside.
 template <int NTH, bool REST, typename S, typename See, typename Last>
 __device__ __forceinline__ Norm norm_of(const S& src, float c, const uint8_t* listed, float* sh,
                                         See see, Last last) {
   const Norm n = row_pass<NTH, REST, false>(src, c, listed, sh, see, last);
-  if (n.s != 0.0 && n.r <= kFar) return n;
+  if (n.r >= -0.5f * kFar && n.r <= kFar) return n;
   __syncthreads();
   return row_pass<NTH, REST, true>(src, c, listed, sh, [](int, float) {}, [](int, float) {});
 }
@@ -455,7 +562,7 @@ __device__ __forceinline__ void push(uint64_t* cand, int* count, uint32_t key, i
 template <int NTH, typename R>
 __device__ int count_from(const R& row, uint32_t lo, TopShared<NTH>& t) {
   int n = 0;
-  Streamed<NTH, R>{row}.each(
+  Streamed<NTH, 8, R>{row}.each(
       [&](int, int m, const float (&v)[8]) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) n += k < m * R::W && key_of(v[k]) >= lo;
@@ -597,7 +704,7 @@ __device__ void top_k(const R& row, int K, const Best& b, float first, float las
     __syncthreads();
     if (tid == 0) t.count = 0;
     __syncthreads();
-    Streamed<NTH, R>{row}.each(
+    Streamed<NTH, 8, R>{row}.each(
         [&](int c, int m, const float (&v)[8]) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -621,8 +728,26 @@ __device__ void top_k(const R& row, int K, const Best& b, float first, float las
   }
 }
 
+// What the backward needs of a row: M, and ln(1 + R) with the sign bit of a row of differences.
+__device__ __forceinline__ void put_stats(float* stats, const Norm& n, const Sums& sums) {
+  stats[0] = n.m;
+  stats[1] = copysignf(static_cast<float>(sums.ln), n.safe ? -1.0f : 1.0f);
+}
+struct Stats {
+  Norm n;  // without its sums
+  float ln;
+  __device__ __forceinline__ Stats(const float* stats, float c) {
+    const bool safe = signbit(stats[1]);
+    const float m = stats[0];
+    n = Norm{m, fmaxf(safe ? m : m * c, kLowest), 0.0, 0.0, safe};
+    ln = fabsf(stats[1]);
+  }
+};
+
+// (With alternatives at most 84 registers: six waves share a SIMD, 146 us at 4099 x 50021 fp32, top 64,
+// instead of 154 with five.)
 template <typename E, bool BIAS, int NTH, bool TOP>
-__global__ void __launch_bounds__(NTH) logprobs_kernel(
+__global__ void __launch_bounds__(NTH, !TOP ? 1 : NTH == 256 ? (BIAS ? 5 : 6) : 4) logprobs_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
     const int64_t* __restrict__ targets, int64_t ignore, Scale k, int K,
     float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ stats,
@@ -633,19 +758,16 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
   Best best;
   float first = -INFINITY, last = -INFINITY;  // this thread's logits outside the vectors
   const Norm n = norm_of<NTH, false>(
-      source<NTH, 0>(row), k.c, nullptr, sh,
+      source<NTH, 0, TOP ? 8 : 16>(row), k.c, nullptr, sh,
       [&](int c, float vm) {
         if constexpr (TOP) best.see(vm, c);
       },
       [&](int j, float x) { (j < row.head ? first : last) = x; });
-  const double log_s = log(n.s), ln_s = log_s + n.correction(k.delta);
-  auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
+  const Sums sums(n, k);
+  auto lp = [&](float x) { return static_cast<float>(sums.logp(x)); };
   if (threadIdx.x == 0) {
-    entropy[r] = n.entropy(log_s);
-    if (stats) {
-      stats[2 * r] = n.r;
-      stats[2 * r + 1] = static_cast<float>(n.safe ? -n.s : n.s);
-    }
+    entropy[r] = static_cast<float>(sums.h);
+    if (stats) put_stats(stats + 2 * r, n, sums);
     if (logprob) {
       const int64_t t = targets[r];
       float v = 0.0f;
@@ -662,7 +784,7 @@ __global__ void __launch_bounds__(NTH) logprobs_kernel(
   }
   if constexpr (TOP) {
     __shared__ TopShared<NTH> t;
-    top_k<NTH>(row, K, best, first, last, n.s != n.s, t);
+    top_k<NTH>(row, K, best, first, last, n.nan(), t);
     const int count = t.count;
     for (int i = threadIdx.x; i < count; i += NTH) {
       const uint64_t mine = t.cand[i];
@@ -745,7 +867,27 @@ __device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_
 }
 
 // d x_j = -(p_j / T) (g_lp + sum g_top + g_H (logp_j + H)), plus g_lp / T at the target and
-// g_top / T at the alternatives. The whole row is written without these, then their places.
+// g_top / T at the alternatives. The whole row is written without these, then their places, where
+// g (1 - p) comes from log p: the difference of g and g p would lose a small 1 - p.
+struct LogprobGrad {
+  float A, B;  // e_j (B arg_j + A) off these places
+  float sum, ge, h, ln, inv_t;
+  __device__ __forceinline__ LogprobGrad(const Stats& st, float c, float sum_, float ge_, float h_,
+                                         float inv_t_, bool off)
+      : sum(sum_), ge(ge_), h(h_), ln(st.ln), inv_t(inv_t_) {
+    const float left = st.n.left(c), is = st.n.empty() ? 0.0f : expf(-ln) * __builtin_amdgcn_exp2f(-left);
+    A = off ? NAN : -(sum + ge * (h - ln - static_cast<float>(kLn2) * left)) * is;
+    B = -ge * static_cast<float>(kLn2) * is;
+  }
+  __device__ __forceinline__ float at(float e, float arg) const {
+    return e * __builtin_fmaf(B, fmaxf(arg, -1e30f), A);
+  }
+  // At a logit x whose log probability, in these places, has the gradient g.
+  __device__ __forceinline__ float point(float x, float m, float g) const {
+    const float logp = fmaxf((x - m) * inv_t - ln, -1e30f);
+    return -g * expm1f(logp) - expf(logp) * (sum - g + ge * (logp + h));
+  }
+};
 template <typename E, bool BIAS, int NTH, int KIND>
 __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
@@ -760,7 +902,7 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
   const Row<E, BIAS, !BIAS> row(logits + r * ldl, bias, V);
   const auto o = out_row<E, KIND>(out, r, ldo, plane, row.head);
   const float inv_t = static_cast<float>(k.inv_t), c = k.c;
-  const Norm n{stats[2 * r], fabsf(stats[2 * r + 1]), 0.0f, stats[2 * r + 1] < 0.0f};
+  const Stats st(stats + 2 * r, c);
   int64_t t = targets && g_lp ? targets[r] : -1;
   const bool off = targets && g_lp && t != ignore && (t < 0 || t >= V);  // a NaN row
   const bool aim = targets && g_lp && t != ignore && !off;
@@ -772,15 +914,12 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
     sum += wave_sum(part) * inv_t;
   }
   const float ge = g_ent ? g_ent[r] * inv_t : 0.0f;
-  const float s = static_cast<float>(n.s), is = n.empty() ? 0.0f : 1.0f / s;
-  const float lns = n.empty() ? 0.0f : logf(s);
-  const float A = off ? NAN : -(sum + ge * (entropy[r] - lns)) * is;
-  const float B = -ge * static_cast<float>(kLn2) * is;
+  const LogprobGrad d(st, c, sum, ge, entropy[r], inv_t, off);
   if (threadIdx.x == 0) taken = 0;
-  n.with_arg(c, [&](auto arg) {
+  st.n.with_arg(c, [&](auto arg) {
     auto grad = [&](float x) {
       const float a = arg(x);
-      return __builtin_amdgcn_exp2f(a) * __builtin_fmaf(B, fmaxf(a, -1e30f), A);
+      return d.at(__builtin_amdgcn_exp2f(a), a);
     };
     source<NTH, 0>(row).each(
         [&](int c, int m, const float (&v)[8]) {
@@ -793,19 +932,20 @@ __global__ void __launch_bounds__(NTH) logprobs_bwd_kernel(
           }
         },
         [&](int j, float x) { o.put(static_cast<int64_t>(j), grad(x)); });
-    __syncthreads();
-    if (n.empty()) return;  // nothing depends on the row
-    if (g_top) {
-      for (int i = threadIdx.x; i < K; i += NTH) {
-        const int64_t j = top_idx[r * K + i];
-        const bool both = aim && j == t;
-        if (both) taken = 1;
-        o.put(j, grad(row.at(j)) + (g_top[r * K + i] * inv_t + (both ? gl : 0.0f)));
-      }
-      __syncthreads();
-    }
-    if (threadIdx.x == 0 && aim && !taken) o.put(t, grad(row.at(t)) + gl);
   });
+  __syncthreads();
+  if (st.n.empty()) return;  // nothing depends on the row
+  if (g_top) {
+    for (int i = threadIdx.x; i < K; i += NTH) {
+      const int64_t j = top_idx[r * K + i];
+      const bool both = aim && j == t;
+      if (both) taken = 1;
+      const float g = d.point(row.at(j), st.n.m, g_top[r * K + i] * inv_t + (both ? gl : 0.0f));
+      o.put(j, off ? NAN : g);
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && aim && !taken) o.put(t, d.point(row.at(t), st.n.m, gl));
 }
 
 // ---- distillation --------------------------------------------------------------------------
@@ -883,7 +1023,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
     float* __restrict__ loss, float* __restrict__ coef, float* __restrict__ weights,
     const float* __restrict__ scale, void* out, int64_t ldo, uint32_t* err) {
   extern __shared__ uint32_t bits[];
-  __shared__ float sh[3 * (NTH / 64)];
+  __shared__ float sh[2 * (NTH / 64)];
   __shared__ Teacher te;
   const size_t r = blockIdx.x;
   const int tid = threadIdx.x;
@@ -952,17 +1092,17 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   const Norm a = norm_of<NTH, REST>(src, sc.c, reinterpret_cast<const uint8_t*>(bits), sh,
                                     [](int, float) {}, [](int, float) {});
   if (tid < 64) {
-    bool empty = a.empty();
-    const double ln_s = empty ? 0.0 : a.ln_s(sc.delta);
+    const Sums sums(a, sc);
+    bool empty = sums.empty;
     // Of the whole row's sum: the logit it is relative to and its logarithm.
     double at = 0.0, ln_all = 0.0, ln_rest = 0.0;
     if constexpr (REST) {
-      at = empty ? -INFINITY : a.safe ? a.r : a.r * kLn2 / sc.inv_t;
+      at = sums.at;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (only[h]) at = fmax(at, static_cast<double>(x[h]));
       at = wave_max_d(at);
-      const double off = a.ln_sum(at, sc.inv_t, ln_s);
+      const double off = sums.ln_sum(at);
       double sum = 0.0;
       bool nan = false;
 #pragma unroll
@@ -981,19 +1121,19 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if constexpr (REST) logp[h] = empty ? -INFINITY : (x[h] - at) * sc.inv_t - ln_all;
-      else logp[h] = a.logp(x[h], sc.inv_t, ln_s);
+      else logp[h] = sums.logp(x[h]);
       if (q[h] != 0.0) part += q[h] * (logq[h] - logp[h]);
     }
     double l = wave_sum_d(part);
     // e_j a at the words off the list (without the rest: at all).
     float ca = 0.0f;
     if constexpr (REST) {
-      rest = rest > 0.0 && !a.empty() && !(ln_rest <= kLeast) ? rest : 0.0;
+      rest = rest > 0.0 && !sums.empty && !(ln_rest <= kLeast) ? rest : 0.0;
       if (rest != 0.0) l += rest * (log(rest) - ln_rest);
       total += rest;
-      if (!a.empty()) ca = static_cast<float>(exp(-a.ln_e(sc.delta)) * (exp(ln_rest) * total - rest));
+      if (!sums.empty) ca = static_cast<float>(exp(-sums.ln_e()) * (exp(ln_rest) * total - rest));
     } else {
-      if (!empty) ca = static_cast<float>(exp(-a.ln_e(sc.delta)) * total);
+      if (!empty) ca = static_cast<float>(exp(-sums.ln_e()) * total);
     }
     if (!some) ca = 0.0f, l = 0.0;
     if (wrong) ca = NAN, l = NAN;
@@ -1045,7 +1185,7 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
     const float* __restrict__ scale, const float* __restrict__ grad, int done, E* __restrict__ out) {
   if (done && grad[0] == 1.0f) return;  // the rows are there
   const size_t r = blockIdx.x;
-  const Norm n{coef[3 * r], 1.0f, 0.0f, coef[3 * r + 2] != 0.0f};
+  const Norm n{0.0f, coef[3 * r], 0.0, 0.0, coef[3 * r + 2] != 0.0f};
   const Row<E, false, true> row(logits + r * ldl, nullptr, V);
   distill_grad<NTH>(source<NTH, 0>(row), K, n, c, scale[0] * grad[0], coef[3 * r + 1],
                     tokens + r * K, weights + r * K, RowOut<E>{out + r * V, row.head});
@@ -1114,23 +1254,26 @@ struct Narrow {
       x[i] = j < V ? ld(p, j) + (bias ? bf2f(bias[j]) : 0.0f) : -INFINITY;
     }
   }
-  // The sums of the exponentials relative to the row's largest logit; off: of the words that are
-  // not listed.
+  // The sums beside the row's largest logit; off: of the words that are not listed.
   template <typename Off>
   __device__ __forceinline__ Norm norm(float c, Off off) const {
     float m = kLowest;
 #pragma unroll
     for (int i = 0; i < NV; ++i) m = off(i) ? fmaxf(m, x[i]) : m;
     m = max16(m);
-    float s = 0.0f, u = 0.0f;
+    float s = 0.0f, u = 0.0f, ties = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float a = Share<true>::arg(off(i) ? x[i] : -INFINITY, m, c);
+      const bool tie = off(i) && x[i] == m;
+      const float a = Share<true>::arg(off(i) && !tie ? x[i] : -INFINITY, m, c);
       const float e = __builtin_amdgcn_exp2f(a);
+      ties += tie ? 1.0f : 0.0f;
       s += e;
       u = __builtin_fmaf(e, fmaxf(a, -1e30f), u);
     }
-    return Norm{m, sum16(s), sum16(u), true};
+    ties = sum16(ties);
+    return Norm{ties > 0.0f ? m : -INFINITY, m,
+                static_cast<double>(sum16(s)) + fmaxf(ties - 1.0f, 0.0f), sum16(u), true};
   }
   __device__ __forceinline__ Norm norm(float c) const {
     return norm(c, [](int) { return true; });
@@ -1146,14 +1289,11 @@ __global__ void __launch_bounds__(256) logprobs_narrow_kernel(
   __shared__ __attribute__((aligned(16))) uint32_t keys[16][16 * NV];
   const Narrow<E, NV> w(rows, V, ldl, logits, bias);
   const Norm n = w.norm(k.c);
-  const double log_s = log(n.s), ln_s = log_s + n.correction(k.delta);
-  auto lp = [&](float x) { return static_cast<float>(n.logp(x, k.inv_t, ln_s)); };
+  const Sums sums(n, k);
+  auto lp = [&](float x) { return static_cast<float>(sums.logp(x)); };
   if (w.live && w.lane == 0) {
-    entropy[w.r] = n.entropy(log_s);
-    if (stats) {
-      stats[2 * w.r] = n.r;
-      stats[2 * w.r + 1] = static_cast<float>(-n.s);
-    }
+    entropy[w.r] = static_cast<float>(sums.h);
+    if (stats) put_stats(stats + 2 * w.r, n, sums);
   }
   if (logprob) {
     const int64_t t = targets[w.r];
@@ -1218,7 +1358,7 @@ __global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
     int64_t plane) {
   const Narrow<E, NV> w(rows, V, ldl, logits, bias);
   const float inv_t = static_cast<float>(k.inv_t);
-  const Norm n{stats[2 * w.r], fabsf(stats[2 * w.r + 1]), 0.0f, stats[2 * w.r + 1] < 0.0f};
+  const Stats st(stats + 2 * w.r, k.c);
   const int64_t t = targets && g_lp ? targets[w.r] : ignore;
   const bool off = t != ignore && (t < 0 || t >= V), aim = t != ignore && !off;
   const float gl = aim ? g_lp[w.r] * inv_t : 0.0f;
@@ -1236,17 +1376,17 @@ __global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
     }
   }
   const float ge = g_ent ? g_ent[w.r] * inv_t : 0.0f;
-  const float s = static_cast<float>(n.s), is = n.empty() ? 0.0f : 1.0f / s;
-  const float lns = n.empty() ? 0.0f : logf(s);
-  const float A = off ? NAN : -(sum + ge * (entropy[w.r] - lns)) * is;
-  const float B = -ge * static_cast<float>(kLn2) * is;
+  const LogprobGrad d(st, k.c, sum, ge, entropy[w.r], inv_t, off);
   const auto o = out_row<E, KIND>(out, w.r, ldo, plane, 0);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = w.lane + 16 * i;
-    const float a = n.safe ? Share<true>::arg(w.x[i], n.r, k.c) : Share<false>::arg(w.x[i], n.r, k.c);
-    const float d = __builtin_amdgcn_exp2f(a) * __builtin_fmaf(B, fmaxf(a, -1e30f), A);
-    if (w.live && j < V) o.put(static_cast<int64_t>(j), n.empty() ? (off ? NAN : 0.0f) : d + point[i]);
+    const float a = Share<true>::arg(w.x[i], st.n.r, k.c);
+    float g = d.at(__builtin_amdgcn_exp2f(a), a);
+    if (point[i] != 0.0f) g = d.point(w.x[i], st.n.m, point[i]);
+    if (off) g = NAN;
+    else if (st.n.empty()) g = 0.0f;
+    if (w.live && j < V) o.put(static_cast<int64_t>(j), g);
   }
 }
 
@@ -1312,7 +1452,7 @@ __global__ void __launch_bounds__(256) distill_narrow_kernel(
       if (word[i] >= 0) all += exp((static_cast<double>(val[i]) - top) * sc.inv_t);
     norm = top * sc.inv_t + log(sum16_d(all));
   }
-  const double ln_s = n.ln_s(sc.delta);
+  const Sums sums(n, sc);
   double part = 0.0, total = 0.0;
   double q[kEntries], logp[kEntries];
 #pragma unroll
@@ -1321,7 +1461,7 @@ __global__ void __launch_bounds__(256) distill_narrow_kernel(
     if (word[i] < 0) continue;
     const double logq = val[i] * sc.inv_t - norm;
     q[i] = exp(logq);
-    logp[i] = n.logp(xs[g][word[i]], sc.inv_t, ln_s);
+    logp[i] = sums.logp(xs[g][word[i]]);
     if (q[i] != 0.0) part += q[i] * (logq - logp[i]);
     total += q[i];
   }
@@ -1329,7 +1469,7 @@ __global__ void __launch_bounds__(256) distill_narrow_kernel(
   total = sum16_d(total);
   const bool wrong = flags >= 1024.0f || total > kMostWeight, some = flags > 0.0f;
   float r = n.r;
-  double a = n.empty() ? 0.0 : exp(-ln_s) * total;
+  double a = sums.empty ? 0.0 : exp(-sums.ln_e()) * total;
   if constexpr (REST) {
     uint32_t listed = 0;
 #pragma unroll
@@ -1338,14 +1478,14 @@ __global__ void __launch_bounds__(256) distill_narrow_kernel(
       listed |= (marks[g][j >> 5] >> (j & 31) & 1) << i;
     }
     const Norm off = w.norm(sc.c, [&](int i) { return !(listed >> i & 1); });
-    const double ln_off = off.ln_s(sc.delta);
-    const double ln_rest = off.ln_sum(n.r, sc.inv_t, ln_off) - ln_s;
+    const Sums others(off, sc);
+    const double ln_rest = others.ln_sum(sums.at) - sums.ln;
     double rest = 1.0 - total;
-    rest = rest > 0.0 && !off.empty() && !(ln_rest <= kLeast) ? rest : 0.0;
+    rest = rest > 0.0 && !others.empty && !(ln_rest <= kLeast) ? rest : 0.0;
     if (rest != 0.0) part += rest * (log(rest) - ln_rest);
     total += rest;
     r = off.r;
-    a = off.empty() ? 0.0 : exp(-ln_off) * (exp(ln_rest) * total - rest);
+    a = others.empty ? 0.0 : exp(-others.ln_e()) * (exp(ln_rest) * total - rest);
   }
   if (weights && w.live) {
 #pragma unroll
@@ -1365,7 +1505,7 @@ __global__ void __launch_bounds__(256) distill_narrow_kernel(
       // A row without a finite logit has no gradient.
       weights[w.r * K + k] = !first      ? kAbsent
                              : wrong     ? NAN
-                             : n.empty() ? 0.0f
+                             : sums.empty ? 0.0f
                                          : static_cast<float>(exp(logp[i]) * total - sum);
     }
   }

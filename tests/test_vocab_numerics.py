@@ -1,5 +1,14 @@
-"""Rows of a vocabulary where 32 bits are short: masks of large finite numbers, against the
-definitions in 64 bits of test_scoring.py and test_distill.py, with the tolerances derived there."""
+"""Rows of a vocabulary where 32 bits are short: masks of large finite numbers, students far from
+their teacher, tokens that are nearly certain, against the definitions in 64 bits of test_scoring.py
+and test_distill.py, with the tolerances derived there.
+
+Where a token is nearly certain the tolerance is relative (``sure``), u = 2^-24: with R = the other
+words' mass over its own, log p = -ln(1 + R). A term of R carries the rounding of its exponent's
+argument, u |z - max z| of itself, the same again from the steps of the running reference, 3 u of
+exponential and product, and the sum S u (``sum_error``); the rounding of 1 / T is taken out of R, and
+stays in the entropy's -sum p log p once more, u |z - max z|. So log p and 1 - p are off by at most
+u (3 spread + S + 32) of themselves, and so is the entropy, a sum of terms of one sign.
+"""
 
 from __future__ import annotations
 
@@ -10,7 +19,7 @@ import torch
 
 from dabsn_amd import distillation_from_logits, token_logprobs
 from test_distill import check, reference as distill_reference
-from test_scoring import U, check_forward, check_grad, logits_of, reference_grad, sum_error
+from test_scoring import U, check_forward, check_grad, logits_of, reference, reference_grad, sum_error
 
 INF = math.inf
 FILLS = [-1e9, -1e10, -1e20, -1e30, "lowest", -6e7, -4e7]
@@ -191,3 +200,90 @@ def test_the_temperature_has_64_bits(cuda_device, V, T, rest):
     p = torch.softmax(z, 1)
     bound = T / 4 * tol * (p + (p - grad * 4 / T).abs()) + 2 * U * grad.abs()
     assert bool(((got.double().cpu() - grad).abs() <= bound).all())
+
+
+GAPS = [3.0, 5.0, 7.0, 9.0, 11.0, 13.0, 15.0, 17.0]  # log p from -5e-2 to -4e-8
+
+
+def sure_rows(V, dtype, seed):
+    """Rows whose token t lies a gap above the others' log-sum-exp."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(8, V, generator=g) * 1.5).to(dtype).float()
+    t = torch.randint(0, V, (8,), generator=g)
+    t[0], t[1] = 0, V - 1
+    x.scatter_(1, t[:, None], -INF)
+    x.scatter_(1, t[:, None], (torch.logsumexp(x, 1) + torch.tensor(GAPS))[:, None])
+    return x.to(dtype).cuda(), t.cuda()
+
+
+def sure(x, T):
+    z = x.double().cpu() / T
+    return U * (3 * (z.amax(1) - z.amin(1)) + sum_error(x.shape[1]) + 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [1.0, 0.7])
+@pytest.mark.parametrize("V", [50, 128, 300, 2050, 9001, 40000])
+def test_scores_of_nearly_certain_tokens(cuda_device, V, T, dtype):
+    x, t = sure_rows(V, dtype, V)
+    lp, ent, _, _, _, p, logp = reference(x, t, 0, T)
+    exact = -torch.log1p(torch.exp((x.double().cpu() - x.double().cpu().amax(1, keepdim=True)) / T)
+                         .scatter(1, t.cpu()[:, None], 0.0).sum(1))  # the same, without cancellation
+    tol = sure(x, T)
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, t, top=1, temperature=T)
+    for got in (r.logprobs, r.top_logprobs[:, 0]):
+        assert bool(((got.detach().double().cpu() - exact).abs() <= tol * exact.abs()).all())
+    assert bool(((r.entropy.detach().double().cpu() - ent).abs() <= tol * ent + 1e-15).all())
+    # The gradient at the token: (1 - p) / T of its log probability's, p (-log p - H) / T of the entropy's.
+    rows = torch.arange(8)
+    (g,) = torch.autograd.grad(r.logprobs.sum(), leaf, retain_graph=True)
+    rnd = U if dtype == torch.float32 else 2.0 ** -8
+    want = -torch.expm1(exact) / T
+    assert bool(((g.double().cpu()[rows, t.cpu()] - want).abs() <= (tol + rnd * (1 + tol)) * want).all())
+    (g,) = torch.autograd.grad(r.top_logprobs.sum(), leaf, retain_graph=True)
+    assert bool(((g.double().cpu()[rows, t.cpu()] - want).abs() <= (tol + rnd * (1 + tol)) * want).all())
+    (g,) = torch.autograd.grad(r.entropy.sum(), leaf)
+    want = -exact.exp() * (exact + ent) / T
+    size = exact.abs() + ent
+    # (the factor's own rounding goes by the place of the largest logit, 2^-20 of 1, in fp32)
+    assert bool(((g.double().cpu()[rows, t.cpu()] - want).abs()
+                 <= (tol * size + 2.0 ** -43) / T + rnd * want.abs() * (1 + tol)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("T", [1.0, 0.7])
+@pytest.mark.parametrize("V", [50, 128, 300, 2050, 9001, 40000])
+def test_distillation_of_nearly_certain_tokens(cuda_device, V, T, rest):
+    """A student near its teacher, both sure of a token: the gradient there is p - q, a difference of
+    numbers near 1 that each hold an error of ``sure`` times 1 - p (q of the fp32 values' own)."""
+    x, t = sure_rows(V, torch.float32, V)
+    g = torch.Generator().manual_seed(V + 1)
+    teacher = x.cpu() + 0.3 * torch.randn(8, V, generator=g)
+    values, tokens = teacher.topk(6, dim=1)
+    lse = torch.logsumexp(teacher.double() / T, 1).float().cuda() if rest else None
+    values, tokens = values.cuda(), tokens.cuda()
+    tol = sure(x, T)
+    for r in range(8):  # a row each, so that each has its loss
+        row = slice(r, r + 1)
+        part = None if lse is None else lse[row]
+        leaf = x[row].clone().requires_grad_(True)
+        loss = distillation_from_logits(leaf, values[row], tokens[row], temperature=T, teacher_lse=part)
+        (got,) = torch.autograd.grad(loss, leaf)
+        ref, grad, _, _ = distill_reference(x[row], values[row], tokens[row], T, part)
+        u = values[row].double().cpu() / T
+        q = torch.exp(u - (torch.logsumexp(u, 1) if part is None else part.double().cpu())[:, None])
+        z = x[row].double().cpu() / T
+        p = torch.softmax(z, 1)
+        w = p.gather(1, tokens[row].cpu())  # listed
+        other = 1 - p.amax().item()  # 64 bits: to 1e-16
+        # Loss: sum q (ln q - ln p): each ln p off by tol (1 - p) for the sure one, tol (|ln p| + 1) others.
+        off = (q * torch.where(w > 0.5, other, w.log().abs() + 1)).sum() + max(0.0, 1 - float(q.sum())) * (
+            1 + (w.log().abs().max() if rest else 0.0))
+        assert abs(float(loss.detach()) - ref) <= T * T * (float(tol[r]) * float(off) + 1e-12) + U * ref * 2
+        at = tokens[row].cpu()
+        err = (got.double().cpu() - grad).abs().gather(1, at)
+        bound = T * (float(tol[r]) * torch.where(w > 0.5, other, w) + 1e-15) + 2 * U * grad.abs().gather(1, at)
+        assert bool((err <= bound).all()), (r, err, bound)
