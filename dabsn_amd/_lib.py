@@ -182,7 +182,6 @@ _SIGNATURES = {
     "dabsn_hip_column_sums_partials": ([i64, i64], sz),
     "dabsn_hip_column_sums": ([i32, i64, i64, i64, vp, i32, vp, vp, vp], i32),
     "dabsn_hip_half_copy": ([i64, vp, vp, vp, vp, vp], i32),
-    "dabsn_hip_distill_half_scale": ([], ctypes.c_float),
     "dabsn_hip_scaled": ([i32, i64, vp, vp, vp, vp, ctypes.c_float, vp, vp], i32),
     "dabsn_hip_embedding_fwd": (
         [i32, i64, i64, i64, vp, vp, i64, ctypes.c_float, vp, vp, vp], i32),

@@ -804,11 +804,14 @@ __global__ void __launch_bounds__(NTH, !TOP ? 1 : NTH == 256 ? (BIAS ? 5 : 6) : 
 // matrix products with fp32 sums and round their results to bf16 (2^-9):
 //   planes   two bf16 rows whose sum holds 17 bits of the fp32 value, of any size (the products'
 //            error 2^-18 a term; one bf16 row would add as much as the results' rounding);
-//   half     one fp16 row, for gradients whose size is known (distillation: p and q, at most
-//            kMostWeight, times kHalfScale): 11 bits, an error of 2^-12 a term, an eighth of the
-//            results' rounding, at half the products of the planes.
-enum OutKind : int { kRows = 0, kPlanes = 1, kHalf = 2 };
-constexpr float kMostWeight = 256.0f, kHalfScale = 128.0f;
+//   split    these two, for the products that sum over rows, where a word's values may all be small
+//            (a third of a softmax over 32000 words lies below 1e-7), and an fp16 row, for the one
+//            that sums over the row's words: times a power of two by a bound of the row's values,
+//            so it holds 11 bits of values down to 2^-29 of that (an error of 2^-12 a term, an
+//            eighth of the results' rounding) and costs half of the planes' products.
+enum OutKind : int { kRows = 0, kPlanes = 1, kSplit = 2 };
+enum Parts : int { kPartPlanes = 1, kPartHalf = 2 };  // of a split row
+constexpr float kMostWeight = 256.0f;
 __device__ __forceinline__ uint32_t pair(float a, float b) {
   return static_cast<uint32_t>(f2bf(a)) | static_cast<uint32_t>(f2bf(b)) << 16;
 }
@@ -848,21 +851,28 @@ struct PlanesOut {
     __builtin_memcpy(q + plane, lo, 8);
   }
 };
-struct HalfOut {
-  _Float16* p;
-  int head;
-  __device__ __forceinline__ void put(int64_t j, float v) const { p[j] = static_cast<_Float16>(v); }
+struct SplitOut {
+  PlanesOut planes;  // the second row one stride behind the first
+  _Float16* half;    // and the fp16 one behind that
+  int parts;
+  float scale;
+  __device__ __forceinline__ void put(int64_t j, float v) const {
+    if (parts & kPartPlanes) planes.put(j, v);
+    if (parts & kPartHalf) half[j] = static_cast<_Float16>(v * scale);
+  }
   __device__ __forceinline__ void put(int c, const float (&v)[4]) const {
-    _Float16 h[4];
+    if (parts & kPartPlanes) planes.put(c, v);
+    if (parts & kPartHalf) {
+      _Float16 h[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = static_cast<_Float16>(v[k]);
-    __builtin_memcpy(p + head + static_cast<size_t>(c) * 4, h, 8);
+      for (int k = 0; k < 4; ++k) h[k] = static_cast<_Float16>(v[k] * scale);
+      __builtin_memcpy(half + planes.head + static_cast<size_t>(c) * 4, h, 8);
+    }
   }
 };
 template <typename E, int KIND>
 __device__ __forceinline__ auto out_row(void* out, size_t r, int64_t ldo, int64_t plane, int head) {
   if constexpr (KIND == kPlanes) return PlanesOut{static_cast<bf16*>(out) + r * ldo, plane, head};
-  else if constexpr (KIND == kHalf) return HalfOut{static_cast<_Float16*>(out) + r * ldo, head};
   else return RowOut<E>{static_cast<E*>(out) + r * ldo, head};
 }
 
@@ -970,6 +980,7 @@ struct Teacher {
   double q[kMaxTop];
   float g[kMaxTop];
   float a;
+  float scale;  // of an fp16 row
   int twice;
 };
 
@@ -1013,15 +1024,15 @@ __device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n,
   }
 }
 
-// GRAD: the row's gradient too while its logits are at hand, times scale[0] (T / count); as fp16
-// rows (KIND) times kHalfScale.
+// GRAD: the row's gradient too while its logits are at hand, times scale[0] (T / count), which
+// split rows go without.
 template <typename E, bool BIAS, int NTH, int NV, bool REST, bool GRAD, int KIND>
 __global__ void __launch_bounds__(NTH) distill_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias, int K,
     int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
     int64_t ignore, Scale sc, const float* __restrict__ teacher_lse, int words,
     float* __restrict__ loss, float* __restrict__ coef, float* __restrict__ weights,
-    const float* __restrict__ scale, void* out, int64_t ldo, uint32_t* err) {
+    const float* __restrict__ scale, int parts, void* out, int64_t ldo, uint32_t* err) {
   extern __shared__ uint32_t bits[];
   __shared__ float sh[2 * (NTH / 64)];
   __shared__ Teacher te;
@@ -1137,6 +1148,9 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
     }
     if (!some) ca = 0.0f, l = 0.0;
     if (wrong) ca = NAN, l = NAN;
+    float most = 0.0f;  // of the gradient's magnitudes at listed words
+    double mass = 0.0;  // the student's on them
+    double sure = -INFINITY;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = tid + 64 * h;
@@ -1158,12 +1172,38 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
                 : empty ? 0.0f
                         : static_cast<float>(exp(logp[h]) * total - w);
       if (weights) weights[r * K + k] = te.g[k];
+      if (KIND == kSplit && first) {
+        most = fmaxf(most, fabsf(te.g[k]));
+        if (!REST) {
+          mass += exp(logp[h]);
+          sure = fmax(sure, logp[h]);
+        }
+      }
+    }
+    if constexpr (KIND == kSplit) {
+      most = wave_max(most);
+      if constexpr (REST) {
+        most = fmaxf(most, fabsf(ca) * __builtin_amdgcn_exp2f(sums.left));
+      } else {
+        // At the others p Q, p at most their mass: one less the listed words', of which the surest
+        // may hold nearly all.
+        sure = wave_max_d(sure);
+        const double left = -expm1(sure);
+        const double others = fmax(left - (wave_sum_d(mass) - exp(sure)), 0.0) + 1e-6 * left;
+        if (some && !empty) most = fmaxf(most, static_cast<float>(others * total));
+      }
+      // The largest below 2^15.
+      const int up = min(15 - __builtin_amdgcn_frexp_expf(most), 126);
+      if (tid == 0) {
+        te.scale = ldexpf(1.0f, up);
+        if (coef) coef[r] = ldexpf(1.0f, -up);
+      }
     }
     if (tid == 0) {
       if (wrong) atomicOr(err, kErrToken);
       loss[2 * r] = static_cast<float>(l);
       loss[2 * r + 1] = some || wrong ? 1.0f : 0.0f;
-      if (coef) {
+      if (KIND != kSplit && coef) {
         coef[3 * r] = a.r;
         coef[3 * r + 1] = ca;
         coef[3 * r + 2] = a.safe ? 1.0f : 0.0f;
@@ -1173,8 +1213,15 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   }
   if constexpr (GRAD) {
     __syncthreads();
-    distill_grad<NTH>(src, K, a, sc.c, KIND == kHalf ? kHalfScale : scale[0], te.a, te.idx, te.g,
-                      out_row<E, KIND>(out, r, ldo, 0, row.head));
+    if constexpr (KIND == kSplit) {
+      bf16* o = static_cast<bf16*>(out) + r * 3 * ldo;
+      distill_grad<NTH>(src, K, a, sc.c, 1.0f, te.a, te.idx, te.g,
+                        SplitOut{PlanesOut{o, ldo, row.head}, reinterpret_cast<_Float16*>(o + 2 * ldo),
+                                 parts, te.scale});
+    } else {
+      distill_grad<NTH>(src, K, a, sc.c, scale[0], te.a, te.idx, te.g,
+                        out_row<E, KIND>(out, r, ldo, 0, row.head));
+    }
   }
 }
 
@@ -1638,9 +1685,10 @@ __global__ void __launch_bounds__(256) distill_rows_kernel(int64_t rows, int V, 
   }
 }
 
-// part[b][c] = the sum over the rows b * kSumRows + 0 .. of column c of 16-bit rows x (stride ld).
+// part[b][c] = the sum over the rows b * kSumRows + 0 .. of column c of bf16 rows x (stride ld), or of
+// the two planes of split rows.
 constexpr int kSumRows = 64;
-template <bool HALF>
+template <bool SPLIT>
 __global__ void __launch_bounds__(256) column_sums_kernel(int64_t rows, int V, int64_t ld,
                                                           const uint16_t* __restrict__ x,
                                                           float* __restrict__ part) {
@@ -1654,15 +1702,16 @@ __global__ void __launch_bounds__(256) column_sums_kernel(int64_t rows, int V, i
 #pragma unroll 8
   for (int64_t r = r0; r < r1; ++r) {  // the stride is a multiple of 8: whole vectors
     float v[8];
-    if constexpr (HALF) {
-      _Float16 u[8];
-      __builtin_memcpy(u, __builtin_assume_aligned(x + r * ld + c, 16), 16);
+    uint32_t u[4];
+    const uint16_t* p = x + r * ld * (SPLIT ? 3 : 1) + c;
+    __builtin_memcpy(u, __builtin_assume_aligned(p, 16), 16);
+    halves<8>(u, v);
+    if constexpr (SPLIT) {
+      float w[8];
+      __builtin_memcpy(u, __builtin_assume_aligned(p + ld, 16), 16);
+      halves<8>(u, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(u[k]);
-    } else {
-      uint32_t u[4];
-      __builtin_memcpy(u, __builtin_assume_aligned(x + r * ld + c, 16), 16);
-      halves<8>(u, v);
+      for (int k = 0; k < 8; ++k) v[k] += w[k];
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[k] += c + k < V ? v[k] : 0.0f;
@@ -2001,7 +2050,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                       const void* bias, int64_t top, int value_dtype, const void* values,
                       const int64_t* tokens, int64_t ignore_index, double temperature,
                       const float* teacher_lse, float* loss, float* coef, float* weights,
-                      const float* scale, int half, void* out, int64_t ldo, uint32_t* err,
+                      const float* scale, int split, void* out, int64_t ldo, uint32_t* err,
                       hipStream_t stream) {
   int rc = distill_checks("distillation", dtype, rows, V, ldl, top, temperature);
   if (rc != DABSN_OK) return rc;
@@ -2011,7 +2060,8 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                 "distillation: the rest of more than %d words is not supported (V=%lld)",
                 kMaxRestVocab, (long long)V);
   DABSN_REQUIRE(!bias || dtype == kF32, "distillation: a bias goes with fp32 logits");
-  DABSN_REQUIRE(!out || (ldo >= V && (half ? dtype == kF32 : scale && !bias)),
+  DABSN_REQUIRE(!out || (ldo >= V && split >= 0 && split <= 3 &&
+                         (split ? dtype == kF32 && (coef || !(split & kPartHalf)) : scale && !bias)),
                 "distillation: bad gradient rows");
   if (rows == 0) return DABSN_OK;
   DABSN_REQUIRE(logits && values && tokens && loss && err, "distillation: null pointer");
@@ -2020,8 +2070,9 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
       return dabsn_hip_distill(dtype, n, V, past(logits, dtype, s * ldl), ldl, bias, top, value_dtype,
                                past(values, value_dtype, s * top), past(tokens, s * top),
                                ignore_index, temperature, past(teacher_lse, s), past(loss, 2 * s),
-                               past(coef, 3 * s), past(weights, s * top), scale, half,
-                               past(out, half ? kBF16 : dtype, s * ldo), ldo, err, stream);
+                               past(coef, split ? s : 3 * s), past(weights, s * top), scale, split,
+                               split ? past(out, kBF16, 3 * s * ldo) : past(out, dtype, s * ldo), ldo,
+                               err, stream);
     });
   const int nth = threads(rows, V, false);
   const dim3 grid(static_cast<unsigned>(rows));
@@ -2050,7 +2101,7 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
   hipLaunchKernelGGL((distill_kernel<E, BIAS, N, NV, REST, GRAD, KIND>), grid, dim3(N), 4 * words,  \
                      stream, (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype,  \
                      values, tokens, ignore_index, scale_t, teacher_lse, words, loss, coef, weights, \
-                     scale, out, ldo, err)
+                     scale, split, out, ldo, err)
 #define DABSN_REST(E, BIAS, N, NV, GRAD, KIND)                    \
   if (teacher_lse) DABSN_LAUNCH(E, BIAS, N, NV, true, GRAD, KIND); \
   else DABSN_LAUNCH(E, BIAS, N, NV, false, GRAD, KIND)
@@ -2061,14 +2112,14 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
   } else if (!out) {                                                                         \
     if (b) { DABSN_REST(float, true, N, 0, false, kRows); }                                  \
     else { DABSN_REST(float, false, N, 0, false, kRows); }                                   \
-  } else if (half) {                                                                         \
-    if (b) { DABSN_REST(float, true, N, 0, true, kHalf); }                                   \
-    else { DABSN_REST(float, false, N, 0, true, kHalf); }                                    \
+  } else if (split) {                                                                        \
+    if (b) { DABSN_REST(float, true, N, 0, true, kSplit); }                                  \
+    else { DABSN_REST(float, false, N, 0, true, kSplit); }                                   \
   } else {                                                                                   \
     DABSN_REST(float, false, N, 0, true, kRows);                                             \
   }
   // Held rows: 64 registers a thread, so that four waves share a SIMD.
-  const bool hold = out && !half && V > 1024;
+  const bool hold = out && !split && V > 1024;
   const int64_t nv = V / (dtype == kBF16 ? 8 : 4);
   if (hold && dtype == kBF16 && nv <= 512 * 16) {
     if (nv <= 256 * 8) { DABSN_REST(bf16, false, 256, 8, true, kRows); }
@@ -2140,7 +2191,7 @@ size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V) {
   return rows <= 0 || V <= 0 ? 0 : static_cast<size_t>((rows + kSumRows - 1) / kSumRows) * V;
 }
 
-int dabsn_hip_column_sums(int half, int64_t rows, int64_t V, int64_t ld, const void* x, int add,
+int dabsn_hip_column_sums(int split, int64_t rows, int64_t V, int64_t ld, const void* x, int add,
                           float* partials, float* out, hipStream_t stream) {
   const int64_t parts = (rows + kSumRows - 1) / kSumRows, strips = (V + 2047) / 2048;
   DABSN_REQUIRE(rows >= 0 && V > 0 && V < (1ll << 31) - 4096 && parts * strips < (1ll << 31) &&
@@ -2149,7 +2200,7 @@ int dabsn_hip_column_sums(int half, int64_t rows, int64_t V, int64_t ld, const v
                 "column sums: bad arguments (rows=%lld, V=%lld, ld=%lld)", (long long)rows,
                 (long long)V, (long long)ld);
   const dim3 grid(static_cast<unsigned>(strips * parts));
-  if (rows > 0 && half)
+  if (rows > 0 && split)
     hipLaunchKernelGGL((column_sums_kernel<true>), grid, dim3(256), 0, stream, rows, (int)V, ld,
                        static_cast<const uint16_t*>(x), partials);
   else if (rows > 0)
@@ -2175,8 +2226,6 @@ int dabsn_hip_half_copy(int64_t n, const void* x, uint32_t* word, void* out, flo
   DABSN_HIP_CHECK(hipGetLastError());
   return DABSN_OK;
 }
-
-float dabsn_hip_distill_half_scale(void) { return kHalfScale; }
 
 int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* s0, const float* s1,
                      const float* s2, float factor, void* out, hipStream_t stream) {

@@ -48,14 +48,14 @@ _FUSED_LOGITS = 1 << 24
 _FUSED_WORDS = (4096, 65536)
 
 
-def _rows(x, bias, values, tokens, lse, ignore, t, s, loss, coef, weights, scale, half, out, ldo,
+def _rows(x, bias, values, tokens, lse, ignore, t, s, loss, coef, weights, scale, split, out, ldo,
           word, stream):
     rows, V = x.shape
     tk = ops.KernelTimer.begin("distill", x)
     _lib.check(_lib.load().dabsn_hip_distill(
         ops._code(x.dtype), rows, V, x.data_ptr(), vocab.row_stride(x), ops._p(bias),
         tokens.shape[1], ops._code(values.dtype), vocab.at(values, s), vocab.at(tokens, s), ignore, t,
-        vocab.at(lse, s), loss, coef, weights, scale, half, out, ldo, word.word.data_ptr(), stream),
+        vocab.at(lse, s), loss, coef, weights, scale, split, out, ldo, word.word.data_ptr(), stream),
         _WHAT)
     ops.KernelTimer.end(tk)
 
@@ -88,7 +88,7 @@ class _FromLogits(torch.autograd.Function):
             if fused:
                 _counted(values, tokens, ignore, V, loss, t, weight, factor, stream)
                 ready = x.new_empty((n, V))
-            _rows(x, None, values, tokens, lse, ignore, t, 0, loss, coef, weights, factor, False,
+            _rows(x, None, values, tokens, lse, ignore, t, 0, loss, coef, weights, factor, 0,
                   None if ready is None else ready.data_ptr(), V, word, stream)
             _lib.check(lib.dabsn_hip_distill_mean(n, loss, t, weight, mean.data_ptr(),
                                                   None if fused else factor, stream), _WHAT)
@@ -144,25 +144,25 @@ class _Linear(torch.autograd.Function):
             loss, factor = aux.data_ptr(), aux.data_ptr() + 8 * n
             mean = torch.empty((), device=dev, dtype=torch.float32)
 
-            def rows(x, s, scale, out, ldo):
-                _rows(x, r.row_bias, values, tokens, lse, ignore, t, s, loss + 8 * s, None, None,
-                      scale, r.half, out, ldo, word, stream)
+            def rows(x, s, scale=None, split=0, inverse=None, out=None, ldo=0):
+                _rows(x, r.row_bias, values, tokens, lse, ignore, t, s, loss + 8 * s, inverse, None,
+                      scale, split, out, ldo, word, stream)
 
             if any(need):
                 _counted(values, tokens, ignore, r.V, loss, t, share, factor, stream)
-                acc = vocab.ReadoutGrads(r, need, chunk, half=True)
+                acc = vocab.ReadoutGrads(r, need, chunk, split=True)
                 for g0, g1 in acc.groups():
                     acc.begin(g0, g1)
                     for s in range(g0, g1, acc.chunk):
-                        rows(r.logits(s, min(g1, s + acc.chunk)), s, factor, acc.rows(s), acc.ldo)
+                        rows(r.logits(s, min(g1, s + acc.chunk)), s, factor, acc.split,
+                             acc.inverses(s), acc.rows(s), acc.ldo)
                     acc.end()
-                # fp16 rows lack the factor T / counted rows, which would take them out of range.
+                # Split rows lack the factor T / counted rows.
                 own = aux[2 * n:] if r.half else None
-                ctx.save_for_backward(*acc.results(), own, *acc.scales)
-                ctx.factor = acc.factor
+                ctx.save_for_backward(*acc.results(), own, acc.scale)
             else:
                 for s in range(0, n, chunk):
-                    rows(r.logits(s, min(n, s + chunk)), s, None, None, 0)
+                    rows(r.logits(s, min(n, s + chunk)), s)
             word.check(_WHAT)
             _lib.check(_lib.load().dabsn_hip_distill_mean(n, loss, t, share, mean.data_ptr(), None,
                                                           stream), _WHAT)
@@ -173,10 +173,10 @@ class _Linear(torch.autograd.Function):
     @vocab.once
     def backward(ctx, g):
         g = g.to(torch.float32)
-        gh, gw, gb, own, *scales = ctx.saved_tensors
+        gh, gw, gb, own, scale = ctx.saved_tensors
         with vocab.on(g):
-            grads = [vocab.scaled(x, ctx.dtype, ctx.factor, g, own, s)
-                     for x, s in zip((gh, gw, gb), scales)]
+            grads = [vocab.scaled(x, ctx.dtype, g, own, s)
+                     for x, s in ((gh, scale), (gw, None), (gb, None))]
         return (*grads, None, None, None, None, None, None, None, None)
 
 

@@ -22,7 +22,7 @@ MAX_TOP = 128
 MAX_REST_VOCAB = 480_000
 MAX_VOCAB = (1 << 31) - 4097
 _CHUNK_BUDGET = 1 << 25
-_GROUP_LOGITS = 1 << 28
+_GROUP_LOGITS = 1 << 27
 _TOKEN_ERROR = ("a token lies outside [0, V) and is not ignore_index, or a teacher_lse is not its "
                 "row's")
 _HERE = contextlib.nullcontext()
@@ -233,42 +233,42 @@ class ReadoutGrads:
       planes  two bf16 rows that hold 17 bits of each value, stacked as twice the rows of one bf16
               product; as many rows as the hidden width (the planes then take no more than the
               weight's fp32 gradient)
-      half    one fp16 row of values of known size, and fp16 copies of the hidden rows and the
-              weight that hold all of their bits, times powers of two; up to 2**28 values
+      split   these two bf16 rows for the weight's and the bias's gradients, each a product of its
+              own, and one fp16 row, times a power of two by the row's size, for the hidden rows',
+              with an fp16 copy of the weight that holds all of its bits, times a power of two; up to
+              2**27 values in each, 0.8 GB (8192 x 2048 x 32000: 5.27 ms of kernels, 5.23 with 2**28
+              and 6.27 with 2**26)
     """
 
-    def __init__(self, r: Readout, need, chunk: int, half: bool = False):
+    def __init__(self, r: Readout, need, chunk: int, split: bool = False):
         self.r, self.need = r, need
         n, V, H, dev = int(r.hidden.shape[0]), r.V, r.H, r.hidden.device
         f32 = torch.float32
-        self.kind = "fp32" if not r.half else "half" if half else "planes"
+        self.kind = "fp32" if not r.half else "split" if split else "planes"
+        self.split = (bool(need[1] or need[2]) + 2 * bool(need[0])) if self.kind == "split" else 0
         self.hidden = self.weight = self.bias = None
         self.ldo = -(-V // 8) * 8 if r.half else V
-        # Device scalars that the three results have to be multiplied by, besides `factor`.
-        self.scales: list[Tensor | None] = [None, None, None]
-        self.factor = 1.0
+        # A device scalar that the hidden rows' result has to be multiplied by.
+        self.scale: Tensor | None = None
         if self.kind == "planes":
             # The products' copies (two fp32 rows and two bf16 rows of H a row) stay within the
             # weight's fp32 gradient or 512 MB.
             fit = max(1, max(4 * V * H, 1 << 29) // (12 * H))
             self.chunk = max(1, min(chunk, n, fit))
             self.group = self.chunk * max(1, min(fit, H) // self.chunk)
-        elif self.kind == "half":
+        elif self.kind == "split":
             self.chunk = chunk
             self.group = chunk * max(1, _GROUP_LOGITS // (self.ldo * chunk))
-            self.factor = 1.0 / _lib.load().dabsn_hip_distill_half_scale()
             if need[0] and n:
-                self.half_weight, self.scales[0] = half_copy(r.weight)
-            if need[1] and n:
-                self.half_hidden, self.scales[1] = half_copy(r.hidden)
+                self.half_weight, self.scale = half_copy(r.weight)
         else:
             self.chunk = self.group = chunk
         self.group = max(1, min(n, self.group))
-        if need[0] and (self.kind != "half" or self.group < n or n == 0):
+        if need[0] and (self.kind != "split" or self.group < n or n == 0):
             self.hidden = torch.empty((n, H), device=dev, dtype=f32)
-        dtype = torch.float16 if self.kind == "half" else r.hidden.dtype
-        planes = 2 if self.kind == "planes" else 1
-        self.buf = torch.empty(planes * self.group * self.ldo, device=dev, dtype=dtype)
+        self.parts = {"fp32": 1, "planes": 2, "split": 3}[self.kind]
+        self.buf = torch.empty(self.parts * self.group * self.ldo, device=dev, dtype=r.hidden.dtype)
+        self.inverse = torch.empty(self.group, device=dev, dtype=f32) if self.split & 2 else None
         self.first = True
 
     def groups(self):
@@ -279,9 +279,14 @@ class ReadoutGrads:
         self.g0, self.g1 = g0, g1
 
     def rows(self, s: int) -> int:
-        """Pointer to the gradient rows from row s on; their stride is ``ldo`` and the planes'
-        ``plane()``."""
-        return self.buf.data_ptr() + (s - self.g0) * self.ldo * self.buf.element_size()
+        """Pointer to the gradient rows from row s on; their stride is ``ldo`` (split rows' three
+        times that) and the planes' ``plane()``."""
+        step = self.ldo * (3 if self.kind == "split" else 1)
+        return self.buf.data_ptr() + (s - self.g0) * step * self.buf.element_size()
+
+    def inverses(self, s: int) -> int | None:
+        """Pointer to what undoes the fp16 rows' factors from row s on."""
+        return at(self.inverse, s - self.g0)
 
     def plane(self) -> int:
         return (self.g1 - self.g0) * self.ldo if self.kind == "planes" else 0
@@ -289,26 +294,20 @@ class ReadoutGrads:
     def end(self) -> None:
         r, m, f32 = self.r, self.g1 - self.g0, torch.float32
         rows = r.hidden[self.g0:self.g1]
+        if self.kind == "split":
+            self._end_split(m, rows)
+            return
         high = 2 * m if self.kind == "planes" else m
         d = self.buf[:high * self.ldo].view(high, self.ldo)[:, :r.V]
         if self.need[0]:
             if self.kind == "fp32":
                 torch.mm(d, r.weight, out=self.hidden[self.g0:self.g1])
-            elif self.kind == "half":
-                p = torch.mm(d, self.half_weight, out_dtype=f32)
-                if self.hidden is None:
-                    self.hidden = p
-                else:
-                    self.hidden[self.g0:self.g1] = p
-                del p
             else:
                 p = torch.mm(d, r.weight, out_dtype=f32)
                 torch.add(p[:m], p[m:], out=self.hidden[self.g0:self.g1])
                 del p
         if self.need[1]:
-            if self.kind == "half":
-                rows = self.half_hidden[self.g0:self.g1]
-            elif self.kind == "planes":
+            if self.kind == "planes":
                 rows = torch.cat((rows, rows))
             if self.kind == "fp32":
                 self.weight = (torch.mm(d.t(), rows) if self.first
@@ -322,14 +321,38 @@ class ReadoutGrads:
             if self.kind == "fp32":
                 self.bias = d.sum(dim=0) if self.first else self.bias.add_(d.sum(dim=0))
             else:
-                lib = _lib.load()
-                if self.first:
-                    self.bias = torch.empty(r.V, device=d.device, dtype=f32)
-                part = torch.empty(lib.dabsn_hip_column_sums_partials(high, r.V), device=d.device,
-                                   dtype=f32)
-                _lib.check(lib.dabsn_hip_column_sums(
-                    self.kind == "half", high, r.V, self.ldo, self.buf.data_ptr(), not self.first,
-                    part.data_ptr(), self.bias.data_ptr(), stream(d)), "readout bias gradient")
+                self._add_bias(high)
+        self.first = False
+
+    def _add_bias(self, rows: int) -> None:
+        lib, V, dev = _lib.load(), self.r.V, self.buf.device
+        if self.first:
+            self.bias = torch.empty(V, device=dev, dtype=torch.float32)
+        part = torch.empty(lib.dabsn_hip_column_sums_partials(rows, V), device=dev,
+                           dtype=torch.float32)
+        _lib.check(lib.dabsn_hip_column_sums(
+            self.kind == "split", rows, V, self.ldo, self.buf.data_ptr(), not self.first,
+            part.data_ptr(), self.bias.data_ptr(), stream(self.buf)), "readout bias gradient")
+
+    def _end_split(self, m: int, rows: Tensor) -> None:
+        f32, V = torch.float32, self.r.V
+        d = self.buf[:3 * m * self.ldo].view(m, 3, self.ldo)[:, :, :V]
+        if self.need[0]:
+            p = torch.mm(d[:, 2].view(torch.float16), self.half_weight, out_dtype=f32)
+            inverse = self.inverse[:m, None]
+            if self.hidden is None:
+                self.hidden = p.mul_(inverse)
+            else:
+                torch.mul(p, inverse, out=self.hidden[self.g0:self.g1])
+            del p
+        if self.need[1]:
+            for i in range(2):
+                if self.first and i == 0:
+                    self.weight = torch.mm(d[:, 0].t(), rows, out_dtype=f32)
+                else:
+                    torch.addmm(self.weight, d[:, i].t(), rows, out_dtype=f32, out=self.weight)
+        if self.need[2]:
+            self._add_bias(m)
         self.first = False
 
     def results(self):
@@ -342,12 +365,12 @@ class ReadoutGrads:
         return self.hidden, self.weight, self.bias
 
 
-def scaled(x: Tensor | None, like: torch.dtype, factor: float, *scales: Tensor | None) -> Tensor | None:
-    """fp32 ``x`` times ``factor`` and up to three device scalars, rounded once to ``like``."""
+def scaled(x: Tensor | None, like: torch.dtype, *scales: Tensor | None) -> Tensor | None:
+    """fp32 ``x`` times up to three device scalars, rounded once to ``like``."""
     if x is None:
         return None
     out = torch.empty(x.shape, device=x.device, dtype=like)
     p = [ops._p(s) for s in scales] + [None] * (3 - len(scales))
-    _lib.check(_lib.load().dabsn_hip_scaled(ops._code(like), x.numel(), x.data_ptr(), *p, factor,
+    _lib.check(_lib.load().dabsn_hip_scaled(ops._code(like), x.numel(), x.data_ptr(), *p, 1.0,
                                             out.data_ptr(), stream(x)), "scaled gradient")
     return out

@@ -704,8 +704,10 @@ int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t str
  * (KL(q || softmax(z)), 1 if the row has a listed token, else 0); q_r is left out where the
  * student's mass off the list is below e^-745. coef [rows][3] and weights [rows][top] (the listed
  * words' gradients; NULL: none) are for _bwd. With out the gradient rows (stride ldo) are written too:
- * in the logits' type times scale[0] (no bias), or with `half` (fp32 logits) as fp16 times
- * dabsn_hip_distill_half_scale(). A row whose weights sum to more than 256 (a teacher_lse that is
+ * in the logits' type times scale[0] (no bias), or with `split` (fp32 logits; no factor) as three
+ * 16-bit rows of stride ldo: with split & 1 two bf16 ones whose sum holds the value to 17 bits, and
+ * with split & 2 an fp16 one of the value times a power of two that takes a bound of the row's values
+ * to 2^15, whose inverse goes to coef [rows]. A row whose weights sum to more than 256 (a teacher_lse that is
  * not the row's) counts as one with a token out of range. A listed token outside [0, V) sets *err to 1 and its row to NaN.
  * dabsn_hip_distill_rows: loss = (0, 1 or 0) without logits. dabsn_hip_distill_mean: mean[0] =
  * weight * temperature^2 * mean loss over the counted rows, factor[0] = weight * temperature / their
@@ -713,8 +715,8 @@ int dabsn_hip_ce_join(int64_t n, const float* planes, void* out, hipStream_t str
  * scale = factor; with `done` dlogits holds the rows for grad[0] = 1 already and the call writes
  * only for another factor. A token listed several times has the sum of its weights.
  *
- * dabsn_hip_column_sums: out [V] (added to with `add`) = column sums of bf16 or fp16 (`half`) rows
- * x (stride ld, a multiple of 8), through partials [dabsn_hip_column_sums_partials].
+ * dabsn_hip_column_sums: out [V] (added to with `add`) = column sums of bf16 rows x (stride ld, a
+ * multiple of 8), or with `split` of the bf16 pairs of split rows with ldo = ld, through partials [dabsn_hip_column_sums_partials].
  * dabsn_hip_half_copy: fp16 out = bf16 x times a power of two that takes the largest magnitude to
  * [2^14, 2^15); inverse = 1 / that power, word: scratch. dabsn_hip_scaled: out[i] = x[i] * factor *
  * s0[0] * s1[0] * s2[0] (NULL: 1), rounded once to dtype. */
@@ -739,18 +741,17 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
                       const void* bias, int64_t top, int value_dtype, const void* values,
                       const int64_t* tokens, int64_t ignore_index, double temperature,
                       const float* teacher_lse, float* loss, float* coef, float* weights,
-                      const float* scale, int half, void* out, int64_t ldo, uint32_t* err,
+                      const float* scale, int split, void* out, int64_t ldo, uint32_t* err,
                       hipStream_t stream);
 int dabsn_hip_distill_bwd(int dtype, int64_t rows, int64_t V, const void* logits, int64_t ldl,
                           int64_t top, const int64_t* tokens, double temperature, const float* coef,
                           const float* weights, const float* scale, const float* grad, int done,
                           void* dlogits, hipStream_t stream);
 size_t dabsn_hip_column_sums_partials(int64_t rows, int64_t V);
-int dabsn_hip_column_sums(int half, int64_t rows, int64_t V, int64_t ld, const void* x, int add,
+int dabsn_hip_column_sums(int split, int64_t rows, int64_t V, int64_t ld, const void* x, int add,
                           float* partials, float* out, hipStream_t stream);
 int dabsn_hip_half_copy(int64_t n, const void* x, uint32_t* word, void* out, float* inverse,
                         hipStream_t stream);
-float dabsn_hip_distill_half_scale(void);
 int dabsn_hip_scaled(int dtype, int64_t n, const float* x, const float* s0, const float* s1,
                      const float* s2, float factor, void* out, hipStream_t stream);
 

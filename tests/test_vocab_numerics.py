@@ -17,9 +17,10 @@ import math
 import pytest
 import torch
 
-from dabsn_amd import distillation_from_logits, token_logprobs
+from dabsn_amd import chunked_linear_distillation, distillation_from_logits, token_logprobs
 from test_distill import check, reference as distill_reference
-from test_scoring import U, check_forward, check_grad, logits_of, reference, reference_grad, sum_error
+from test_scoring import (U, check_forward, check_grad, logit_error, logits_of, reference,
+                          reference_grad, sum_error)
 
 INF = math.inf
 FILLS = [-1e9, -1e10, -1e20, -1e30, "lowest", -6e7, -4e7]
@@ -287,3 +288,70 @@ def test_distillation_of_nearly_certain_tokens(cuda_device, V, T, rest):
         err = (got.double().cpu() - grad).abs().gather(1, at)
         bound = T * (float(tol[r]) * torch.where(w > 0.5, other, w) + 1e-15) + 2 * U * grad.abs().gather(1, at)
         assert bool((err <= bound).all()), (r, err, bound)
+
+
+# ---- gradients of a bf16 readout ---------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("budget", [None, 64 * 1003])
+def test_readout_gradients_of_words_that_are_never_likely(cuda_device, budget, rest):
+    """Words whose probability is 1e-9 to 1e-15 in every row, word by word: a gradient's terms are off
+    by the logits' error 2 e (``logit_error``), the softmax's, 2^-17 of the planes and n additions of
+    u, each of the term itself, and the result by its rounding to bf16."""
+    from test_distill import linear_case
+
+    n, H, V = 300, 64, 1003
+    h, w, b, values, tokens, lse = linear_case(3, n, H, V, 16, torch.bfloat16, rest=rest)
+    b[:40] = -torch.linspace(14, 26, 40).to(torch.bfloat16)
+    tokens[tokens < 40] = -100
+    leaves = [v.clone().requires_grad_(True) for v in (h, w, b)]
+    loss = chunked_linear_distillation(*leaves, values, tokens, teacher_lse=lse, chunk_budget=budget)
+    _, gw, gb = torch.autograd.grad(loss, leaves)
+    x = h.double().cpu() @ w.double().cpu().t() + b.double().cpu()
+    _, d, _, _ = distill_reference(x, values, tokens, 1.0, lse)
+    p = torch.softmax(x, 1)
+    # The terms' magnitudes: p Q + p q_r / p_r + q.
+    size = 2 * p / n + d.abs()
+    tol = 4 * float(logit_error(h, w, b).max()) + U * (4 * sum_error(V) + 900 + n) + 2.0 ** -17
+    hd = h.double().cpu()
+    for got, want, terms in ((gw, d.t() @ hd, size.t() @ hd.abs()),
+                             (gb[:, None], d.sum(0)[:, None], size.sum(0)[:, None])):
+        err = (got.double().cpu() - want).norm(dim=1)
+        bound = tol * terms.norm(dim=1) + 2.0 ** -8 * want.norm(dim=1) * (1 + 2.0 ** -8)
+        assert bool((err <= bound)[:40].all()), (err / want.norm(dim=1))[:40]
+        assert bool((err <= bound).all())
+
+
+@pytest.mark.gpu
+def test_readout_gradients_of_rows_that_are_nearly_certain(cuda_device):
+    """Student and teacher sure of a token to 1e-10 and less: hidden gradients that small, row by row.
+    Terms as above; an fp16 row holds them to 2^-11 of the row's size."""
+    n, H, V = 24, 64, 1003
+    g = torch.Generator().manual_seed(5)
+    w = (torch.randn(V, H, generator=g) * 2 / H ** 0.5).to(torch.bfloat16).cuda()
+    t = torch.randint(0, V, (n,), generator=g).cuda()
+    wt = w[t].float()
+    scale = torch.linspace(36, 52, n)[:, None].cuda()
+    h = (wt * scale / wt.square().sum(1, keepdim=True)).to(torch.bfloat16)
+    x = h.double().cpu() @ w.double().cpu().t()
+    values, tokens = (x + 0.1 * torch.randn(n, V, generator=g).double()).float().topk(8, dim=1)
+    leaf = h.clone().requires_grad_(True)
+    loss = chunked_linear_distillation(leaf, w, None, values.cuda(), tokens.cuda())
+    (got,) = torch.autograd.grad(loss, leaf)
+    _, d, _, _ = distill_reference(x, values, tokens, 1.0, None)
+    # p - q at the token itself, 2^-53 of 1 in 64 bits, is the others' sum: a row's gradient sums to 0.
+    at = t.cpu()[:, None]
+    d.scatter_(1, at, 0.0)
+    d.scatter_(1, at, -d.sum(1, keepdim=True))
+    q = torch.zeros_like(x).scatter_(1, tokens, torch.softmax(values.double(), 1))
+    small = lambda v: torch.minimum(v, 1 - v)  # noqa: E731
+    size = (small(torch.softmax(x, 1)) + small(q)) / n
+    want = d @ w.double().cpu()
+    assert float(want.norm(dim=1).max()) < 1e-6 and float(want.norm(dim=1).min()) < 1e-11
+    norms = w.double().cpu().norm(dim=1)
+    tol = 4 * float(logit_error(h, w, None).max()) + U * (4 * sum_error(V) + 900 + V) + 2.0 ** -10
+    err = (got.double().cpu() - want).norm(dim=1)
+    # The operator forms exp(log p) Q - q at the token in 64 bits: an exponential (an ulp, 2^-52), the
+    # sum Q, a product and a difference, each of 2^-53 of numbers at most 1.
+    own = 5 * 2.0 ** -53 / n * norms[t.cpu()]
+    assert bool((err <= tol * (size @ norms) + own + 2.0 ** -8 * want.norm(dim=1)).all()), err / want.norm(dim=1)
