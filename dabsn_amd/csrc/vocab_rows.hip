@@ -1242,11 +1242,12 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
 // Vocabularies of up to kNarrow words (tens of them in character and group workloads): 16 lanes
 // take a row, NV values a lane in registers, 16 rows a block. What a row costs beside its logits
 // (reductions of 4 lane exchanges, the teacher's exponentials, the logarithms) is shared by the
-// four rows of a wave, and each lane finds its words in the row's list, in the list's order.
-// 262144 rows of 60 fp32, a wave a row as above -> 16 lanes a row, us: log probabilities 136 -> 35,
-// with alternatives 354 -> 107, backward 166 -> 31; distillation with 8 listed tokens 304 -> 64,
-// with the rest 351 -> 79, backward 138 -> 34. The logits are 63 MB, 12 us at the rate of a copy (24
-// for a backward): logarithms in 64 bits, the list and the ranking bound them, not memory.
+// four rows of a wave. 262144 rows of 60 fp32, a wave a row as above -> 16 lanes a row, us: log
+// probabilities 202 -> 38, with alternatives 371 -> 112, backward 172 -> 37; distillation with 8
+// listed tokens 347 -> 80, with the rest 421 -> 101, backward 121 -> 30. The logits are 63 MB, 12 us at
+// the rate of a copy (24 for a backward): vector instructions bound the forward kernels, 327 a wave
+// of four rows, 1026 with alternatives, 753 and 941 in distillation, which keep the units busy 90 to
+// 100% of the time (SQ_INSTS_VALU, SQ_ACTIVE_INST_VALU).
 constexpr int kNarrow = 128;
 
 template <typename Op>
@@ -1437,15 +1438,15 @@ __global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
   }
 }
 
-// A listed word twice is found by its bit; then the list is gone through for each of its places.
-template <typename E, int NV, bool REST>
+// A lane takes up to `kEntries` of the list's entries: lane, lane + 16, ... A listed word twice is
+// found by its bit; then the list is gone through for each of its places.
+template <typename E, int NV, int kEntries, bool REST>
 __global__ void __launch_bounds__(256) distill_narrow_kernel(
     int64_t rows, int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias,
     int K, int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
     int64_t ignore, Scale sc, const float* __restrict__ teacher_lse, float* __restrict__ loss,
     float* __restrict__ coef, float* __restrict__ weights, uint32_t* err) {
-  constexpr int kEntries = kMaxTop / 16;  // a lane's: lane, lane + 16, ...
-  __shared__ int lists[16][kMaxTop];      // -1: absent
+  __shared__ int lists[16][16 * kEntries];  // -1: absent
   __shared__ float xs[16][16 * NV];
   __shared__ uint32_t marks[16][kNarrow / 32];
   const Narrow<E, NV> w(rows, V, ldl, logits, bias);
@@ -2080,19 +2081,22 @@ int dabsn_hip_distill(int dtype, int64_t rows, int64_t V, const void* logits, in
   const bf16* b = static_cast<const bf16*>(bias);
   const int words = static_cast<int>(((teacher_lse ? V : std::min<int64_t>(V, kBits)) + 7 + 31) / 32);
   if (V <= kNarrow && !out) {
-#define DABSN_NARROW(E, NV, REST)                                                                  \
-  hipLaunchKernelGGL((distill_narrow_kernel<E, NV, REST>),                                         \
+#define DABSN_NARROW(E, NV, NE, REST)                                                              \
+  hipLaunchKernelGGL((distill_narrow_kernel<E, NV, NE, REST>),                                     \
                      dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, stream, rows,    \
                      (int)V, ldl, static_cast<const E*>(logits), b, (int)top, value_dtype, values,  \
                      tokens, ignore_index, scale_t, teacher_lse, loss, coef, weights, err)
+#define DABSN_NE(E, NV, REST) \
+  if (top <= 16) DABSN_NARROW(E, NV, 1, REST); else DABSN_NARROW(E, NV, kMaxTop / 16, REST)
 #define DABSN_NV(E, REST) \
-  if (V <= 64) DABSN_NARROW(E, 4, REST); else DABSN_NARROW(E, 8, REST)
+  if (V <= 64) { DABSN_NE(E, 4, REST); } else { DABSN_NE(E, 8, REST); }
     if (dtype == kBF16) {
       if (teacher_lse) { DABSN_NV(bf16, true); } else { DABSN_NV(bf16, false); }
     } else {
       if (teacher_lse) { DABSN_NV(float, true); } else { DABSN_NV(float, false); }
     }
 #undef DABSN_NV
+#undef DABSN_NE
 #undef DABSN_NARROW
     DABSN_HIP_CHECK(hipGetLastError());
     return DABSN_OK;
