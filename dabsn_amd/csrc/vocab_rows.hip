@@ -975,13 +975,18 @@ constexpr int kMaxRestVocab = 480000;  // 60 KB of bits
 constexpr float kAbsent = 3e38f;       // in the place of a listed word's gradient: not written
 constexpr double kLeast = -745.0;      // ln of the smallest positive number of 64 bits
 
+// In shared memory: in registers it would be the first wave's all through the pass, whose held rows
+// leave no room for it (128 a thread for four waves a SIMD).
 struct Teacher {
+  double q[kMaxTop], logq[kMaxTop];
+  double total;  // sum q
   int idx[kMaxTop];  // -1: absent
-  double q[kMaxTop];
+  float x[kMaxTop];  // the student's logits
   float g[kMaxTop];
   float a;
   float scale;  // of an fp16 row
-  int twice;
+  int twice, some, wrong;
+  bool only[kMaxTop];  // a listed word's first mark, where marks are exact
 };
 
 __device__ __forceinline__ double wave_sum_d(double v) {
@@ -1027,7 +1032,7 @@ __device__ __forceinline__ void distill_grad(const S& src, int K, const Norm& n,
 // GRAD: the row's gradient too while its logits are at hand, times scale[0] (T / count), which
 // split rows go without.
 template <typename E, bool BIAS, int NTH, int NV, bool REST, bool GRAD, int KIND>
-__global__ void __launch_bounds__(NTH) distill_kernel(
+__global__ void __launch_bounds__(NTH, NV == 8 ? 6 : NV == 16 ? 4 : 1) distill_kernel(
     int V, int64_t ldl, const E* __restrict__ logits, const bf16* __restrict__ bias, int K,
     int value_type, const void* __restrict__ values, const int64_t* __restrict__ tokens,
     int64_t ignore, Scale sc, const float* __restrict__ teacher_lse, int words,
@@ -1043,18 +1048,15 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   for (int i = tid; i < words; i += NTH) bits[i] = 0;
   if (tid == 0) te.twice = 0;
   __syncthreads();
-  double q[2], logq[2], rest = 0.0, total = 0.0;
-  float x[2];
-  bool only[2];  // a listed word's first mark, where marks are exact
-  bool some = false, wrong = false;
   if (tid < 64) {
     double u[2];
+    bool some = false, wrong = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = tid + 64 * h;
       u[h] = -INFINITY;
-      x[h] = 0.0f;
-      only[h] = false;
+      float x = 0.0f;
+      bool only = false;
       int j = -1;
       if (k < K) {
         const int64_t at = tokens[r * K + k];
@@ -1066,15 +1068,17 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
           } else if (v != -INFINITY) {
             j = static_cast<int>(at);
             u[h] = v * sc.inv_t;
-            x[h] = row.at(at);
+            x = row.at(at);
             const uint32_t bit = static_cast<uint32_t>(j + pad_of(row.head)) %
                                  (static_cast<uint32_t>(words) * 32);
-            only[h] = !(atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1);
-            if (!only[h]) te.twice = 1;
+            only = !(atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1);
+            if (!only) te.twice = 1;
           }
         }
-        te.idx[k] = j;
       }
+      te.idx[k] = j;
+      te.x[k] = x;
+      te.only[k] = only;
       some = some || j >= 0;
     }
     wrong = __any(wrong);
@@ -1090,14 +1094,17 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = tid + 64 * h;
-      logq[h] = u[h] - norm;
-      q[h] = k < K && te.idx[k] >= 0 ? exp(logq[h]) : 0.0;
-      if (k < K) te.q[k] = q[h];
-      all += q[h];
+      const double logq = u[h] - norm, q = te.idx[k] >= 0 ? exp(logq) : 0.0;
+      te.logq[k] = logq;
+      te.q[k] = q;
+      all += q;
     }
-    total = wave_sum_d(all);
-    wrong = wrong || total > kMostWeight;
-    if constexpr (REST) rest = 1.0 - total;
+    all = wave_sum_d(all);
+    if (tid == 0) {
+      te.total = all;
+      te.some = some;
+      te.wrong = wrong || all > kMostWeight;
+    }
   }
   __syncthreads();
   const Norm a = norm_of<NTH, REST>(src, sc.c, reinterpret_cast<const uint8_t*>(bits), sh,
@@ -1105,6 +1112,15 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
   if (tid < 64) {
     const Sums sums(a, sc);
     bool empty = sums.empty;
+    const bool some = te.some, wrong = te.wrong;
+    double total = te.total;
+    float x[2];
+    bool only[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      x[h] = te.x[tid + 64 * h];
+      only[h] = te.only[tid + 64 * h];
+    }
     // Of the whole row's sum: the logit it is relative to and its logarithm.
     double at = 0.0, ln_all = 0.0, ln_rest = 0.0;
     if constexpr (REST) {
@@ -1133,12 +1149,14 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
     for (int h = 0; h < 2; ++h) {
       if constexpr (REST) logp[h] = empty ? -INFINITY : (x[h] - at) * sc.inv_t - ln_all;
       else logp[h] = sums.logp(x[h]);
-      if (q[h] != 0.0) part += q[h] * (logq[h] - logp[h]);
+      const double q = te.q[tid + 64 * h];
+      if (q != 0.0) part += q * (te.logq[tid + 64 * h] - logp[h]);
     }
     double l = wave_sum_d(part);
     // e_j a at the words off the list (without the rest: at all).
     float ca = 0.0f;
     if constexpr (REST) {
+      double rest = 1.0 - total;
       rest = rest > 0.0 && !sums.empty && !(ln_rest <= kLeast) ? rest : 0.0;
       if (rest != 0.0) l += rest * (log(rest) - ln_rest);
       total += rest;
@@ -1156,7 +1174,7 @@ __global__ void __launch_bounds__(NTH) distill_kernel(
       const int k = tid + 64 * h;
       if (k >= K) continue;
       const int j = te.idx[k];
-      double w = q[h];
+      double w = te.q[k];
       bool first = j >= 0;
       if (te.twice) {
         w = 0.0;
