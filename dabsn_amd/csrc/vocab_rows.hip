@@ -18,7 +18,7 @@
 // groups of 8, 82 without; with that group taken again in every row, or the logit itself kept apart
 // and swapped for each larger one, 90 and 93.
 //
-// The pass is bound by memory where an element costs few instructions: 10.2 vector instructions here
+// The pass is bound by memory where an element costs few instructions: 10.3 vector instructions here
 // (counted at 8192 x 32000 bf16), against the 12 that the time of its 2 bytes allows. So the
 // exponent's argument is one fma of the logit, x c - r with c = log2 e / T and r, in units of ln 2,
 // near the thread's maximum; r moves only when a group exceeds it by 8. c is rounded: the sums u of
@@ -60,11 +60,11 @@ __device__ __forceinline__ void halves(const uint32_t (&u)[N / 2], float (&v)[N]
 // A row's logits, W = 8 bf16 or 4 fp32 (16 bytes) at a time, plus the readout's bias. A row of an
 // odd vocabulary starts anywhere in a line of 128 bytes: its vectors begin at the first whole line,
 // column `head`, and the logits before it and behind the last vector are taken one by one.
-// ONCE: the loads are marked as not to be kept in the caches. 8192 x 32000 bf16 are read in 83 us
-// instead of 128 (6.3 TB/s), as the lines that a pass would leave there, and those it would push
-// out to memory, are of no use. Whole lines at a time are needed for this: fp32 lanes that took two
-// neighbouring vectors (each line fetched twice) or vectors across lines lost a third instead,
-// 173 -> 205 and 231 us at 4099 x 50021.
+// ONCE: the loads are marked as not to be kept in the caches. 8192 x 32000 bf16 take 89 us instead
+// of 98, beside a backward that writes as much 102 instead of 107, as the lines that a pass would
+// leave there, and those it would push out to memory, are of no use. Whole lines at a time are
+// needed for this: fp32 lanes that took two neighbouring vectors (each line fetched twice) or vectors
+// across lines lost a third instead, 173 -> 205 and 231 us at 4099 x 50021.
 template <typename E, bool BIAS, bool ONCE>
 struct Row {
   static constexpr int W = is_bf16<E>::value ? 8 : 4;
@@ -626,12 +626,12 @@ __device__ __forceinline__ uint32_t bound_of_largest(const uint32_t (&k)[N], int
 // largest is known from the row's pass; the K-th largest of these, or of the largest of G of their
 // groups, is a bound that K logits reach, and few more do: of well mixed logits G ln(G / (G - K)), 74
 // for K = 64 of 256. So only the groups that reach it are read again, gathered and ranked against
-// each other (4099 x 50021 fp32: 122 us without alternatives, 133 with 1, 137 with 20, 148 with 64, 183
-// with 128; bf16 66, 75, 81, 90, 111). Where more than kCap reach it (rows with many equal logits)
+// each other (4099 x 50021 fp32: 120 us without alternatives, 125 with 1, 133 with 20, 145 with 64, 183
+// with 128; bf16 69, 87, 89, 98, 115). Where more than kCap reach it (rows with many equal logits)
 // the K-th largest key is found by bisection over the row. first, last: the thread's logits outside
 // the vectors (-inf: none). With a workgroup a compute unit, whose time is that of one load after
-// another, the threads load their best groups before the bound is known (1 x 32000 bf16 with 5
-// alternatives, with this and the bound of 64 groups: 7.7 us instead of 10.7; without any 4.7).
+// another, the threads load their best groups before the bound is known (256 x 32000 bf16 with 20
+// alternatives 13.0 us instead of 13.6; one row with 5 takes 8.6, without any 5.4).
 template <int NTH, typename R>
 __device__ void top_k(const R& row, int K, const Best& b, float first, float last, bool nan,
                       TopShared<NTH>& t) {
@@ -1847,9 +1847,9 @@ static int checks(const char* what, int dtype, int64_t rows, int64_t V, int64_t 
 
 // Threads a row: a wave where the row is a few vectors; the whole of a compute unit where no more
 // rows than units are there; else 256, of which eight rows share a unit. With 1024 threads (of
-// which a unit holds one row or two) against 256, us: 384 rows of 8200 bf16, distillation 13.4 and
-// 9.3, log probabilities and their gradient 10.9 and 9.7; of 32000 15.8 and 13.2, 19.8 and 20.9,
-// log probabilities with 5 alternatives 21.7 and 12.6; of 128000 29.7 and 34.3, 57 and 67. So
+// which a unit holds one row or two) against 256, us: 384 rows of 8200 bf16, distillation 15.8 and
+// 11.4, log probabilities and their gradient 17.1 and 12.2; of 32000 20.1 and 16.7, 29.1 and 27.8,
+// log probabilities with 5 alternatives 18.4 and 14.4; of 128000 36.6 and 37.4, 69 and 76. So
 // plain passes (no alternatives, no list) over long rows keep 1024 up to two rows a unit.
 static int threads(int64_t rows, int64_t V, bool plain) {
   const int64_t most = plain && V >= 65536 ? 511 : 256;

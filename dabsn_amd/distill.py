@@ -37,13 +37,13 @@ _WHAT = "distillation"
 
 # From this many logits on, the gradient is formed with the loss while a row's logits are in
 # registers, and the backward only checks that its upstream factor is 1 (loss.backward()); another
-# factor forms it again (``loss_weight`` keeps a mixed objective's share out of it). Forward and
-# backward in two passes -> with the gradient formed ahead (and again for another factor), us:
-# 8388 x 32000 bf16 317 -> 217 (426), 16777 x 16000 338 -> 220 (431), 4129 x 65000 320 -> 221 (435),
-# 33554 x 8000 357 -> 262 (458), 2097 x 32000 fp32 156 -> 138 (220). Rows of few words are read again
-# from the caches (33554 x 2000 bf16 160 -> 176), rows of more do not fit the registers (2684 x 100000
-# 373 -> 351, and 591 for another factor), and below 2^24 logits the launches that count the rows
-# ahead cost as much as the second reading.
+# factor forms it again (``loss_weight`` keeps a mixed objective's share out of it). Kernels of
+# forward and backward with 32 listed tokens and the rest, in two passes -> with the gradient formed
+# ahead (and again for another factor), us: 8388 x 32000 bf16 330 -> 230 (440), 16777 x 16000 343 -> 255
+# (466), 4129 x 65000 309 -> 244 (461), 33554 x 8000 365 -> 329 (509), 2097 x 32000 fp32 159 -> 126 (235).
+# Rows of few words are read again from the caches (33554 x 2000 bf16 208 -> 231), rows of more do not
+# fit the registers (2684 x 100000 313 -> 308, and 490 for another factor), and below 2^24 logits the
+# launches that count the rows ahead cost as much as the second reading.
 _FUSED_LOGITS = 1 << 24
 _FUSED_WORDS = (4096, 65536)
 
@@ -78,7 +78,7 @@ class _FromLogits(torch.autograd.Function):
         with vocab.on(x):
             stream = vocab.stream(x)
             word = vocab.ErrorWord(dev)
-            # The rows' losses [n, 2], coefficients [n, 3], listed words' gradients [n, K], and the factor.
+            # The rows' losses [n, 2], coefficients [n, 3], listed words' gradients [n, K], the factor.
             aux = torch.empty(n * (5 + K) + 1 if need else 2 * n, device=dev, dtype=torch.float32)
             mean = aux.new_empty(())
             loss = aux.data_ptr()

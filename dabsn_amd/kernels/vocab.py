@@ -153,7 +153,8 @@ def chunk_rows(rows: int, vocab: int, budget: int | None) -> int:
     one is set, ``DABSN_LOSS_CHUNK_SCORES``, else 2**25; not positive or ``off``: all rows at once):
     chunks of equal height, of whole tiles of 128 rows where they allow it. The default is twice the
     loss's: 128 MB of fp32 logits, which the row kernel still finds in the memory-side cache, and
-    products of 1024 rows by 32000 words (4096 rows scored in 548 us; 580 with 2**24 and 2**26)."""
+    products of 1024 rows by 32000 words (4096 rows scored in 622 us of kernels; 668 with 2**24 and
+    670 with 2**26)."""
     if budget is None:
         env = os.environ.get("DABSN_LOSS_CHUNK_SCORES", "")
         try:
