@@ -262,7 +262,8 @@ def fingerprint_of(model: DABSNSequenceLM) -> dict[str, object]:
     """Architecture identity a memory must match: the reference's dictionary, key for key
     (memory.py:149-161), so files cross-load in both directions; a scaled embedding, which the
     reference has not, adds its scale."""
-    scaled = {} if model.embed_scale is None else {"embed_scale": model.embed_scale}
+    scale = getattr(model, "embed_scale", None)
+    scaled = {} if scale is None else {"embed_scale": scale}
     return {
         **scaled,
         "vocab": int(model.vocab),
@@ -368,10 +369,11 @@ def _run(model: DABSNSequenceLM, ids: Tensor, memory: DABSNMemory | None, *,
         state = list(memory.layers)
         position = memory.position
     lengths = [layer.length for layer in memory.layers] if memory is not None else []
+    embed = getattr(model, "embed_tokens", model.embed)  # a caller's own model has its embedding
     outputs = []
     with torch.no_grad(), ops.reuse_parameter_copies():
         for start, stop in _chunks(int(ids.shape[1]), chunk_size):
-            hidden = model.embed_tokens(ids[:, start:stop])
+            hidden = embed(ids[:, start:stop])
             for i, block in enumerate(blocks):
                 hidden, state[i] = _block_step(block, hidden, state[i], position)
             outputs.append(hidden)

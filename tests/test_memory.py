@@ -361,3 +361,29 @@ def test_incremental_admission_decode_is_bit_identical_to_full_recompute(cuda_de
     finally:
         mem._INCREMENTAL_ADMISSION = True
     assert torch.equal(got, want)
+
+
+def test_a_module_of_the_same_parts_carries_memory_cpu():
+    """A language model of the caller's own with the attributes that the memory reads (``embed``,
+    ``blocks``, ``readout`` and the architecture's), which knows nothing of a scaled embedding."""
+    model = _model("cpu")
+
+    class Own(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.embed, self.readout, self.body = model.embed, model.readout, model.backbone
+            for name in ("vocab", "hidden_dim", "depth", "layers", "tie_embeddings", "residual",
+                         "mlp_ratio", "mlp_middle_depth", "mlp_depth_index"):
+                setattr(self, name, getattr(model, name))
+
+        @property
+        def blocks(self):
+            return self.body.blocks
+
+    ids = _ids(2, 20)
+    want, theirs = mem.forward_with_memory(model, ids, extend=True)
+    got, memory = mem.forward_with_memory(Own(), ids, extend=True)
+    assert torch.equal(got, want) and memory.fingerprint == theirs.fingerprint
+    more = _ids(2, 3, seed=9)
+    assert torch.equal(mem.forward_with_memory(Own(), more, memory)[0],
+                       mem.forward_with_memory(model, more, theirs)[0])
