@@ -17,7 +17,8 @@ import math
 import pytest
 import torch
 
-from dabsn_amd import chunked_linear_distillation, distillation_from_logits, token_logprobs
+from dabsn_amd import (chunked_linear_distillation, chunked_linear_token_logprobs,
+                       distillation_from_logits, token_logprobs)
 from test_distill import check, reference as distill_reference
 from test_scoring import (U, check_forward, check_grad, logit_error, logits_of, reference,
                           reference_grad, sum_error)
@@ -355,3 +356,48 @@ def test_readout_gradients_of_rows_that_are_nearly_certain(cuda_device):
     # sum Q, a product and a difference, each of 2^-53 of numbers at most 1.
     own = 5 * 2.0 ** -53 / n * norms[t.cpu()]
     assert bool((err <= tol * (size @ norms) + own + 2.0 ** -8 * want.norm(dim=1)).all()), err / want.norm(dim=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fill", [-INF, -1e9, -1e30, "lowest"])
+@pytest.mark.parametrize("V", [90, 1003])
+def test_a_readout_whose_bias_rules_words_out(cuda_device, V, fill, dtype):
+    """Scores and distillation from hidden rows with a third of the words ruled out by the bias: the
+    definition's values (errors as in test_scoring.py and test_distill.py, logits off by e), and
+    exact zeros in those words' gradients."""
+    from test_distill import linear_case
+
+    n, H = 70, 48
+    fill = torch.finfo(dtype).min if fill == "lowest" else fill
+    h, w, b, values, tokens, _ = linear_case(7, n, H, V, 8, dtype, rest=False)
+    out = torch.arange(V, device="cuda") % 3 == 1
+    b[out] = fill
+    tokens[out[tokens.clamp(min=0)] & (tokens >= 0)] = -100
+    t = torch.arange(n, device="cuda") % (V // 3) * 3
+    x = h.double().cpu() @ w.double().cpu().t() + b.double().cpu()
+    e = float(logit_error(h, w, torch.where(out, 0.0, b.float())).max())
+    lp, ent, _, _, _, p, _ = reference(x, t, 0, 0.9)
+    leaves = [v.clone().requires_grad_(True) for v in (h, w, b)]
+    r = chunked_linear_token_logprobs(*leaves, t, temperature=0.9, chunk_budget=30 * V)
+    z = x[:, ~out.cpu()] / 0.9
+    spread, ln, S = float(z.amax() - z.amin()), math.log(V), sum_error(V)
+    close = lambda a, c, tol: float((a.detach().double().cpu() - c).abs().max()) <= tol  # noqa: E731
+    assert close(r.logprobs, lp, 2 * e / 0.9 + U * (8 * spread + 8 * ln + S))
+    assert close(r.entropy, ent, 2 * e / 0.9 * (1 + ln) + U * (S * (1 + 2 * ln) + 8 * ln))
+    loss = chunked_linear_distillation(*leaves, values, tokens, chunk_budget=30 * V)
+    ref, d, tol, _ = distill_reference(x, values, tokens, 1.0)
+    assert abs(float(loss.detach()) - ref) <= tol + 2 * e
+    hd, wd = h.double().cpu(), w.double().cpu()
+    _, F, _ = reference_grad(x, t, 0, 0.9, torch.ones(n), torch.ones(n), None)
+    dense = reference_grad(x, t, 0, 0.9, torch.ones(n), torch.ones(n), None)[0]
+    rnd = U if dtype == torch.float32 else 2.0 ** -8
+    for total, g, size in ((r.logprobs.sum() + r.entropy.sum(), dense, F + dense.abs()),
+                           (loss, d, 2 * p / n + d.abs())):
+        got = torch.autograd.grad(total, leaves)
+        rel = 8 * e * (1 + ln) + U * (4 * S + 900 + n + V + H) + (2.0 ** -10 if dtype != torch.float32 else 0)
+        for a, want, terms in ((got[0], g @ wd, size @ wd.abs()), (got[1], g.t() @ hd, size.t() @ hd.abs()),
+                               (got[2], g.sum(0), size.sum(0))):
+            err = (a.double().cpu() - want).abs()
+            assert bool((err <= rel * terms + rnd * want.abs() * (1 + rel) + 2.0 ** -126).all())
+        assert float(got[1][out].float().abs().max()) == 0 == float(got[2][out].float().abs().max())
