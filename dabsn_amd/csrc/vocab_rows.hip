@@ -14,11 +14,10 @@
 // -ln(1 + R) with R small, and in a sum that holds the 1 too fp32 would keep R to 2^-24 of 1, not of
 // itself (log p = -1e-4 was off by 1e-3 of itself). So each thread keeps the sums of the group with
 // its largest logit apart from the others', and where R turns out below 1/4 the thread that has M
-// takes that group's again without it. 8192 x 32000 bf16 take 87 us with this and groups of 16, 89 with
-// groups of 8, 82 without; with that group taken again in every row, or the logit itself kept apart
-// and swapped for each larger one, 90 and 93.
+// takes that group's again without it. 8192 x 32000 bf16 take 83 to 87 us with this and groups of 16, 86
+// to 88 with groups of 8 or with that group taken again in every row, 82 without any of it.
 //
-// The pass is bound by memory where an element costs few instructions: 10.3 vector instructions here
+// The pass is bound by memory where an element costs few instructions: 9.5 vector instructions here
 // (counted at 8192 x 32000 bf16), against the 12 that the time of its 2 bytes allows. So the
 // exponent's argument is one fma of the logit, x c - r with c = log2 e / T and r, in units of ln 2,
 // near the thread's maximum; r moves only when a group exceeds it by 8. c is rounded: the sums u of
@@ -411,6 +410,11 @@ static Scale scale_of(double t) {
   k.delta = k.inv_t / kLn2 / static_cast<double>(k.c) - 1.0;
   return k;
 }
+// 1 / x of a number at least 1: 1 ulp of fp32, doubled in bits by a step of Newton's.
+__device__ __forceinline__ double reciprocal(double x) {
+  const double r = __builtin_amdgcn_rcpf(static_cast<float>(x));
+  return r * __builtin_fma(-x, r, 2.0);
+}
 // A row's sums with 1 / T at its full precision, log2 e / T = c (1 + delta): to first order each e is
 // short of the factor 2^(arg delta), and all of 2^-left as M's own e is to be 1.
 struct Sums {
@@ -423,12 +427,14 @@ struct Sums {
       : at(n.m), inv_t(k.inv_t), left(n.left(k.c)), empty(n.empty()) {
     const double f = __builtin_amdgcn_exp2f(-left);
     const double R = n.nan() ? NAN : empty ? 0.0 : f * (n.s + kLn2 * k.delta * n.u);
+    // ln(1 + R) for small R too: with what the sum lost in its rounding, to first order.
     const double one = 1.0 + R;
-    ln = one == 1.0 ? R : log(one) * (R / (one - 1.0));  // ln(1 + R) for small R too, after Kahan
+    const double inverse = reciprocal(one);
+    ln = log(one) + (R - (one - 1.0)) * inverse;
     // sum p (z - M / T) (1 + R); its own correction would need the sum of e arg^2, and what it
     // lacks, delta |arg| of itself, is an argument's rounding.
     const double w = empty ? 0.0 : kLn2 * f * (n.u - left * n.s);
-    h = ln - w / one;
+    h = ln - w * inverse;
     h = h < 0.0 ? 0.0 : h;
   }
   // ln of the sum of exp((x - y) / T) over the row's logits x.
@@ -1261,10 +1267,10 @@ __global__ void __launch_bounds__(NTH) distill_bwd_kernel(
 // take a row, NV values a lane in registers, 16 rows a block. What a row costs beside its logits
 // (reductions of 4 lane exchanges, the teacher's exponentials, the logarithms) is shared by the
 // four rows of a wave. 262144 rows of 60 fp32, a wave a row as above -> 16 lanes a row, us: log
-// probabilities 202 -> 38, with alternatives 371 -> 112, backward 172 -> 37; distillation with 8
-// listed tokens 347 -> 80, with the rest 421 -> 101, backward 121 -> 30. The logits are 63 MB, 12 us at
-// the rate of a copy (24 for a backward): vector instructions bound the forward kernels, 327 a wave
-// of four rows, 1026 with alternatives, 753 and 941 in distillation, which keep the units busy 90 to
+// probabilities 202 -> 35, with alternatives 371 -> 110, backward 172 -> 35; distillation with 8
+// listed tokens 347 -> 75, with the rest 421 -> 99, backward 121 -> 30. The logits are 63 MB, 12 us at
+// the rate of a copy (24 for a backward): vector instructions bound the forward kernels, 311 a wave
+// of four rows, 1010 with alternatives, 704 and 914 in distillation, which keep the units busy 90 to
 // 100% of the time (SQ_INSTS_VALU, SQ_ACTIVE_INST_VALU).
 constexpr int kNarrow = 128;
 
@@ -1444,12 +1450,23 @@ __global__ void __launch_bounds__(256) logprobs_narrow_bwd_kernel(
   const float ge = g_ent ? g_ent[w.r] * inv_t : 0.0f;
   const LogprobGrad d(st, k.c, sum, ge, entropy[w.r], inv_t, off);
   const auto o = out_row<E, KIND>(out, w.r, ldo, plane, 0);
+  float target = 0.0f;  // the gradient there, once for the four rows of a wave
+  if (!g_top) {
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x = point[i] != 0.0f ? w.x[i] : x;
+    target = d.point(x, st.n.m, gl);
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = w.lane + 16 * i;
     const float a = Share<true>::arg(w.x[i], st.n.r, k.c);
     float g = d.at(__builtin_amdgcn_exp2f(a), a);
-    if (point[i] != 0.0f) g = d.point(w.x[i], st.n.m, point[i]);
+    if (g_top) {
+      if (point[i] != 0.0f) g = d.point(w.x[i], st.n.m, point[i]);
+    } else {
+      g = point[i] != 0.0f ? target : g;
+    }
     if (off) g = NAN;
     else if (st.n.empty()) g = 0.0f;
     if (w.live && j < V) o.put(static_cast<int64_t>(j), g);
