@@ -1210,10 +1210,11 @@ __global__ void __launch_bounds__(NTH, NV == 8 ? 6 : NV == 16 ? 4 : 1) distill_k
         most = fmaxf(most, fabsf(ca) * __builtin_amdgcn_exp2f(sums.left));
       } else {
         // At the others p Q, p at most their mass: one less the listed words', of which the surest
-        // may hold nearly all.
+        // may hold nearly all. The difference of what it leaves (fp32 sums, right to some 2^-20) and
+        // the other listed words' may fall short of the mass, so 2^-10 more: no value may overflow.
         sure = wave_max_d(sure);
         const double left = -expm1(sure);
-        const double others = fmax(left - (wave_sum_d(mass) - exp(sure)), 0.0) + 1e-6 * left;
+        const double others = fmax(left - (wave_sum_d(mass) - exp(sure)), 0.0) + 0x1p-10 * left;
         if (some && !empty) most = fmaxf(most, static_cast<float>(others * total));
       }
       // The largest below 2^15.

@@ -401,3 +401,39 @@ def test_a_readout_whose_bias_rules_words_out(cuda_device, V, fill, dtype):
             err = (a.double().cpu() - want).abs()
             assert bool((err <= rel * terms + rnd * want.abs() * (1 + rel) + 2.0 ** -126).all())
         assert float(got[1][out].float().abs().max()) == 0 == float(got[2][out].float().abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [20.0, 40.0, 60.0, 80.0])
+def test_hidden_gradients_where_the_list_holds_nearly_all(cuda_device, gap):
+    """A sure token and a list that leaves 1e-7 to 1e-5 of what it leaves: the fp16 rows' factor goes
+    by a difference of nearly equal numbers and must not take an unlisted word out of range."""
+    n, H, V = 64, 32, 600
+    g = torch.Generator().manual_seed(int(gap))
+    w = torch.zeros(V, H)
+    w[:8] = torch.eye(8, H)
+    w[8:] = torch.randn(V - 8, H, generator=g) * 0.02
+    h = torch.zeros(n, H)
+    h[:, 0] = gap
+    h[:, 1:8] = -3.0 * torch.rand(n, 7, generator=g)  # listed, far above the rest
+    b = torch.zeros(V)
+    b[8:] = -torch.linspace(19, 23, V - 8)
+    h, w, b = (v.to(torch.bfloat16).cuda() for v in (h, w, b))
+    tokens = torch.arange(8).expand(n, 8).contiguous().cuda()
+    values = (h.float() @ w.float().t())[:, :8] + 0.5 * torch.randn(n, 8, generator=g).cuda()
+    leaf = h.clone().requires_grad_(True)
+    loss = chunked_linear_distillation(leaf, w, b, values, tokens)
+    (got,) = torch.autograd.grad(loss, leaf)
+    x = h.double().cpu() @ w.double().cpu().t() + b.double().cpu()
+    _, d, _, _ = distill_reference(x, values, tokens, 1.0, None)
+    d[:, 0] = -d[:, 1:].sum(1)  # a row sums to 0; the difference p - q near 1 would not be exact here
+    want = d @ w.double().cpu()
+    q = torch.zeros_like(x).scatter_(1, tokens.cpu(), torch.softmax(values.double().cpu(), 1))
+    small = lambda v: torch.minimum(v, 1 - v)  # noqa: E731
+    size = (small(torch.softmax(x, 1)) + small(q)) / n
+    norms = w.double().cpu().norm(dim=1)
+    tol = 4 * float(logit_error(h, w, b).max()) + U * (4 * sum_error(V) + 900 + V) + 2.0 ** -10
+    err = (got.double().cpu() - want).norm(dim=1)
+    own = 5 * 2.0 ** -53 / n * norms[0]
+    assert bool(torch.isfinite(got).all())
+    assert bool((err <= tol * (size @ norms) + own + 2.0 ** -8 * want.norm(dim=1)).all()), err / want.norm(dim=1)
