@@ -19,9 +19,11 @@ from .events import (
     remove_event_listener,
     strict_events,
 )
+from .linear import fused_linear, fused_mlp
 from .loss import chunked_cross_entropy_from_logits, chunked_linear_cross_entropy
 from .memory import DABSNMemory, LayerMemory, forward_with_memory, ingest
 from .model import DABSNBlock, DABSNSequenceLM
+from .norm import layer_norm, rms_norm
 from .read import DABSNRead
 from .scoring import TokenLogprobs, chunked_linear_token_logprobs, token_logprobs
 
@@ -42,9 +44,13 @@ __all__ = [
     "add_event_listener",
     "distillation_from_logits",
     "forward_with_memory",
+    "fused_linear",
+    "fused_mlp",
     "ingest",
     "kernels",
+    "layer_norm",
     "remove_event_listener",
+    "rms_norm",
     "scaled_embedding",
     "strict_events",
     "token_logprobs",

@@ -13,7 +13,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_build" / "libdabsn_hip.so"
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 _lock = threading.Lock()
 _lib = None
@@ -56,6 +56,17 @@ class CoreBwdCall(ctypes.Structure):
                                      "gcF", "gWx", "gWgx", "day", "part_vec", "part_scal", "gb0",
                                      "ge0", "gc0", "workspace")]
                 + [("workspace_bytes", sz), ("coresident_cus", i32)])
+
+
+class LinearCall(ctypes.Structure):
+    """Mirror of ``dabsn_linear_call``."""
+
+    _fields_ = ([(n, i32) for n in ("dtype", "transA", "transB", "act", "slope_kind")]
+                + [(n, i64) for n in ("M", "N", "K")]
+                + [(n, vp) for n in ("A", "B", "bias", "slope", "residual")]
+                + [(n, i64) for n in ("lda", "ldb", "lds", "ldr", "ldc", "ldk")]
+                + [(n, vp) for n in ("C", "keep", "workspace")] + [("workspace_bytes", sz)])
+
 
 _SIGNATURES = {
     "dabsn_hip_abi_version": ([], i32),
@@ -188,6 +199,16 @@ _SIGNATURES = {
     "dabsn_hip_embedding_workspace_bytes": ([i64, i64, i64], sz),
     "dabsn_hip_embedding_bwd": (
         [i32, i64, i64, i64, vp, i64, vp, ctypes.c_float, vp, vp, sz, vp], i32),
+    "dabsn_hip_norm_fwd": (
+        [i32, i32, i32, i64, i64, vp, i64, vp, vp, ctypes.c_float, vp, vp, vp], i32),
+    "dabsn_hip_norm_workspace_bytes": ([i32, i64, i64], sz),
+    "dabsn_hip_norm_bwd": (
+        [i32, i32, i32, i64, i64, vp, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp, sz, vp], i32),
+    "dabsn_hip_linear_workspace_bytes": ([i32, i64, i64, i64], sz),
+    "dabsn_hip_linear": ([ctypes.POINTER(LinearCall), vp], i32),
+    "dabsn_hip_linear_slope_workspace_bytes": ([i32, i64, i64], sz),
+    "dabsn_hip_linear_slope": (
+        [i32, i64, i64, vp, i64, vp, i64, i32, vp, i64, vp, vp, sz, vp], i32),
     "dabsn_hip_read3_decode": (
         [i32, i64, i64, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, PTR4,
          vp, vp, sz, vp],

@@ -1,0 +1,196 @@
+"""Linear layers whose bias, activation and residual are the product's epilogue, and the block's
+MLP made of them.
+
+  fused_linear  activation(x W^T + bias) + residual
+  fused_mlp     x + activation(norm(x) W1^T + b1) W2^T + b2
+
+Activations: ``none``, ``relu2`` (the squared ReLU of the reference's MLP), ``gelu`` (by the error
+function) and ``silu``. (A plain ReLU is left out: its slope jumps at 0, so products of 16-bit
+operands would differ by whole terms.) Products are fp32 sums; everything up to the result is fp32
+and is rounded once. Both are differentiable in all their tensors. In the backward the products'
+operands have the inputs' type: dz = g activation'(z) is rounded once to it, from a slope that is
+rounded once too. The squared ReLU's slope is 2 sqrt of its output where that is at hand, so nothing
+more is kept.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from .kernels import dense
+from .norm import layer_norm, rms_norm
+
+_RELU2 = dense.ACTIVATIONS["relu2"]
+
+
+def _cast(*tensors: Tensor | None):
+    """All tensors in autocast's type, as ``F.linear`` casts its own."""
+    dt = torch.get_autocast_dtype("cuda")
+    return tuple(None if t is None else t.to(dt) for t in tensors)
+
+
+def _weight(what: str, name: str, w: Tensor, x: Tensor, width: int) -> Tensor:
+    if w.dim() != 2 or w.shape[1] != width or 0 in w.shape:
+        raise ValueError(f"{what}: {name} {tuple(w.shape)} does not match width {width}")
+    if w.dtype != x.dtype:
+        raise TypeError(f"{what}: {name} must be {x.dtype} as x is, not {w.dtype}")
+    return dense.rows_of(w)
+
+
+def _keeps(x: Tensor, n: int, act: int, residual: bool):
+    """(buffer for the slope or None, its kind) of an activated product's forward in training."""
+    if act == 0:
+        return None, 0
+    if act == _RELU2 and not residual:
+        return None, dense._FROM_SQUARE
+    return dense.padded(x.shape[0], n, x), dense._STORED
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        with dense.on(x):
+            keep, kind = _keeps(x, weight.shape[0], act, residual is not None)
+            out = dense.product(x, weight, bias=bias, act=act, keep=keep, residual=residual)
+        ctx.save_for_backward(x, weight, out if kind == dense._FROM_SQUARE else keep)
+        ctx.kind = kind
+        return out
+
+    @staticmethod
+    @dense.once
+    def backward(ctx, g):
+        x, weight, slope = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = None
+        with dense.on(x):
+            rows = dense.rows_of(g)
+            dz, db = dense.slope_product(rows, slope, ctx.kind, need[0] or need[1], need[2])
+            if need[0]:
+                dx = dense.product(dz, weight, trans_b=True)
+            if need[1]:
+                dw = dense.product(dz, x, trans_a=True, trans_b=True)
+        return dx, dw, db, g if need[3] else None, None
+
+
+def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
+                 activation: str = "none", residual: Tensor | None = None) -> Tensor:
+    """``activation(x @ weight.T + bias) + residual`` (see the module's note) of ``x`` [..., K],
+    ``weight`` [N, K], ``bias`` [N] and ``residual`` [..., N], all float32 or all bfloat16, of any
+    row strides. Inside autocast the product runs in its type, and a residual of another type is
+    added afterwards, as ``F.linear(...) + residual`` would."""
+    what = "fused_linear"
+    act = dense.need_activation(what, activation)
+    if torch.is_autocast_enabled("cuda"):
+        x, weight, bias = _cast(x, weight, bias)
+        if residual is not None and residual.dtype != x.dtype:
+            return fused_linear(x, weight, bias, activation=activation) + residual
+    dense.need_float(what, "x", x)
+    if x.dim() < 1:
+        raise ValueError(f"{what}: expected x [..., K]")
+    w = _weight(what, "weight", weight, x, int(x.shape[-1]))
+    n = int(w.shape[0])
+    bias = dense.need_vector(what, "bias", bias, n, x.dtype)
+    shape = (*x.shape[:-1], n)
+    if residual is not None:
+        if residual.shape != shape:
+            raise ValueError(f"{what}: residual {tuple(residual.shape)} does not match {shape}")
+        if residual.dtype != x.dtype:
+            raise TypeError(f"{what}: residual must be {x.dtype} as x is, not {residual.dtype}")
+    dense.need_device(what, x, w, bias, residual)
+    rows = dense.rows_of(x)
+    res = None if residual is None else dense.rows_of(residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (rows, w, bias, res)):
+        out = _Linear.apply(rows, w, bias, res, act)
+    else:
+        with dense.on(x):
+            out = dense.product(rows, w, bias=bias, act=act, residual=res)
+    return out if x.dim() == 2 else out.view(shape)
+
+
+class _MLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, nw, nb, w1, b1, w2, b2, act, layer, eps):
+        with dense.on(x):
+            normed, stats = dense.norm(x, nw, nb, eps, layer, True)
+            keep, kind = _keeps(x, w1.shape[0], act, False)
+            h = dense.product(normed, w1, bias=b1, act=act, keep=keep,
+                              out=dense.padded(x.shape[0], w1.shape[0], x))
+            out = dense.product(h, w2, bias=b2, residual=x)
+        ctx.save_for_backward(x, nw, stats, normed, w1, h, keep, w2)
+        ctx.kind, ctx.layer = kind, layer
+        ctx.dtype = (x if nw is None and nb is None else nb if nw is None else nw).dtype
+        return out
+
+    @staticmethod
+    @dense.once
+    def backward(ctx, g):
+        x, nw, stats, normed, w1, h, keep, w2 = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dnw = dnb = dw1 = db1 = dw2 = db2 = None
+        with dense.on(x):
+            # Contiguous rows: they are the norm's `add` too.
+            rows = dense.rows_of(g).contiguous()
+            if need[6]:
+                _, db2 = dense.slope_product(rows, None, 0, False, True)
+            if need[5]:
+                dw2 = dense.product(rows, h, trans_a=True, trans_b=True)
+            if any(need[:5]):
+                slope = h if ctx.kind == dense._FROM_SQUARE else keep
+                dz = dense.product(rows, w2, trans_b=True, slope=slope, slope_kind=ctx.kind,
+                                   out=dense.padded(*h.shape, h))
+                if need[4]:
+                    _, db1 = dense.slope_product(dz, None, 0, False, True)
+                if need[3]:
+                    dw1 = dense.product(dz, normed, trans_a=True, trans_b=True)
+                if any(need[:3]):
+                    dn = dense.product(dz, w1, trans_b=True)
+                    dx, dnw, dnb = dense.norm_backward(x, nw, stats, dn, ctx.layer, rows, ctx.dtype,
+                                                       need[1], need[2])
+        return dx, dnw, dnb, dw1, db1, dw2, db2, None, None, None
+
+
+def fused_mlp(x: Tensor, w1: Tensor, w2: Tensor, b1: Tensor | None = None,
+              b2: Tensor | None = None, *, norm: str = "rms", norm_weight: Tensor | None = None,
+              norm_bias: Tensor | None = None, eps: float | None = None,
+              activation: str = "relu2") -> Tensor:
+    """``x + activation(norm(x) @ w1.T + b1) @ w2.T + b2`` (see the module's note) of ``x`` [..., H],
+    ``w1`` [F, H], ``w2`` [H, F], ``b1`` [F] and ``b2`` [H], all float32 or all bfloat16. ``norm`` is
+    ``rms`` or ``layer`` (``eps`` 1e-6 or 1e-5 unless given; weight and bias as ``layer_norm``
+    takes them). Inside autocast the products run in its type, the norm and the sum in x's."""
+    what = "fused_mlp"
+    act = dense.need_activation(what, activation)
+    if norm not in ("rms", "layer"):
+        raise ValueError(f"{what}: norm must be rms or layer, not {norm!r}")
+    layer = norm == "layer"
+    if norm_bias is not None and not layer:
+        raise ValueError(f"{what}: the RMS norm has no bias")
+    eps = dense.need_eps(what, (1e-5 if layer else 1e-6) if eps is None else eps)
+    if torch.is_autocast_enabled("cuda"):
+        w1, w2, b1, b2 = _cast(w1, w2, b1, b2)
+        if x.dtype != w1.dtype:
+            normed = (layer_norm(x, norm_weight, norm_bias, eps=eps) if layer
+                      else rms_norm(x, norm_weight, eps=eps))
+            return fused_linear(fused_linear(normed, w1, b1, activation=activation), w2, b2,
+                                residual=x)
+    nw, nb = dense.need_norm(what, x, norm_weight, norm_bias)
+    h = int(x.shape[-1])
+    w1 = _weight(what, "w1", w1, x, h)
+    w2 = _weight(what, "w2", w2, x, int(w1.shape[0]))
+    if w2.shape[0] != h:
+        raise ValueError(f"{what}: w2 {tuple(w2.shape)} does not lead back to width {h}")
+    b1 = dense.need_vector(what, "b1", b1, int(w1.shape[0]), x.dtype)
+    b2 = dense.need_vector(what, "b2", b2, h, x.dtype)
+    dense.need_device(what, x, w1, w2, b1, b2, nw, nb)
+    rows = dense.rows_of(x)
+    leaves = (rows, nw, nb, w1, b1, w2, b2)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
+        out = _MLP.apply(*leaves, act, layer, eps)
+    else:
+        with dense.on(x):
+            normed, _ = dense.norm(rows, nw, nb, eps, layer, False)
+            mid = dense.product(normed, w1, bias=b1, act=act,
+                                out=dense.padded(rows.shape[0], w1.shape[0], rows))
+            out = dense.product(mid, w2, bias=b2, residual=rows)
+    return out if x.dim() == 2 else out.view(x.shape)

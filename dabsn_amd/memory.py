@@ -260,10 +260,13 @@ class DABSNMemory:
 
 def fingerprint_of(model: DABSNSequenceLM) -> dict[str, object]:
     """Architecture identity a memory must match: the reference's dictionary, key for key
-    (memory.py:149-161), so files cross-load in both directions; a scaled embedding, which the
-    reference has not, adds its scale."""
+    (memory.py:149-161), so files cross-load in both directions; a scaled embedding and an MLP of
+    another kind, which the reference has not, add theirs."""
     scale = getattr(model, "embed_scale", None)
     scaled = {} if scale is None else {"embed_scale": scale}
+    activation = getattr(model, "mlp_activation", None)
+    if activation is not None:
+        scaled["mlp"] = f"{model.mlp_norm} {activation}{' bias' if model.mlp_bias else ''}"
     return {
         **scaled,
         "vocab": int(model.vocab),

@@ -25,6 +25,8 @@ from .core import DABSNCore
 from .distill import chunked_linear_distillation
 from .embedding import scaled_embedding
 from .kernels import ops, pipeline
+from .kernels.dense import need_activation
+from .linear import fused_mlp
 from .read import DABSNRead
 from .scoring import TokenLogprobs, chunked_linear_token_logprobs
 
@@ -40,13 +42,31 @@ class MLPRMSNorm(nn.Module):
         return (inputs.float() * scale).to(inputs.dtype) * self.weight
 
 
+def check_mlp(ratio: float | None, activation: str | None, norm: str, bias: bool) -> None:
+    """Refuse an MLP that no path computes."""
+    if norm not in ("rms", "layer"):
+        raise ValueError(f"mlp_norm must be rms or layer, not {norm!r}")
+    if activation is None:
+        if norm != "rms" or bias:
+            raise ValueError("mlp_norm and mlp_bias go with mlp_activation")
+        return
+    if ratio is None:
+        raise ValueError("mlp_activation goes with mlp_ratio")
+    need_activation("mlp_activation", activation)
+
+
 class DABSNBlock(nn.Module):
     """One core plus admitted/permanent/induction/long read (seq, field or hybrid
-    geometry)."""
+    geometry).
+
+    ``mlp_activation`` (None: the reference's MLP, operation by operation) runs the MLP through
+    ``fused_mlp`` with that activation, ``relu2`` being the reference's; ``mlp_norm`` (``rms`` or
+    ``layer``) and ``mlp_bias`` then choose its norm and give its products biases."""
 
     def __init__(self, input_dim: int, hidden_dim: int, state_dim: int, read_geometry: str = "seq",
                  *, residual: bool = False, mlp_ratio: float | None = None,
-                 block_chunk_t: int | None = None) -> None:
+                 block_chunk_t: int | None = None, mlp_activation: str | None = None,
+                 mlp_norm: str = "rms", mlp_bias: bool = False) -> None:
         super().__init__()
         self.input_dim, self.hidden_dim, self.state_dim = input_dim, hidden_dim, state_dim
         self.read_geometry = read_geometry
@@ -65,14 +85,20 @@ class DABSNBlock(nn.Module):
             self.residual_skip = nn.Linear(input_dim, hidden_dim, bias=False)
             nn.init.normal_(self.residual_skip.weight, mean=0.0, std=(1.0 / input_dim) ** 0.5)
         self.mlp_ratio = None if mlp_ratio is None else float(mlp_ratio)
+        self.mlp_activation, self.mlp_bias = mlp_activation, bool(mlp_bias)
+        check_mlp(self.mlp_ratio, mlp_activation, mlp_norm, self.mlp_bias)
         self.mlp_norm = self.mlp_fc1 = self.mlp_fc2 = None
         if self.mlp_ratio is not None:
             inner = int(round(self.mlp_ratio * hidden_dim))
-            self.mlp_norm = MLPRMSNorm(hidden_dim)
-            self.mlp_fc1 = nn.Linear(hidden_dim, inner, bias=False)
-            self.mlp_fc2 = nn.Linear(inner, hidden_dim, bias=False)
+            self.mlp_norm = (nn.LayerNorm(hidden_dim) if mlp_norm == "layer"
+                             else MLPRMSNorm(hidden_dim))
+            self.mlp_fc1 = nn.Linear(hidden_dim, inner, bias=self.mlp_bias)
+            self.mlp_fc2 = nn.Linear(inner, hidden_dim, bias=self.mlp_bias)
             nn.init.normal_(self.mlp_fc1.weight, mean=0.0, std=0.02)
             nn.init.zeros_(self.mlp_fc2.weight)
+            if self.mlp_bias:
+                nn.init.zeros_(self.mlp_fc1.bias)
+                nn.init.zeros_(self.mlp_fc2.bias)
         self.block_chunk_t = block_chunk_t
         self.last_trace: dict[str, object] = {}
 
@@ -152,6 +178,12 @@ class DABSNBlock(nn.Module):
     def forward_mlp(self, hidden: Tensor) -> Tensor:
         if self.mlp_fc2 is None:
             return hidden
+        if self.mlp_activation is not None:
+            norm, fc1, fc2 = self.mlp_norm, self.mlp_fc1, self.mlp_fc2
+            return fused_mlp(hidden, fc1.weight, fc2.weight, fc1.bias, fc2.bias,
+                             norm="rms" if isinstance(norm, MLPRMSNorm) else "layer",
+                             norm_weight=norm.weight, norm_bias=getattr(norm, "bias", None),
+                             eps=norm.eps, activation=self.mlp_activation)
         if not torch.is_grad_enabled() and ops._same_dtype(hidden, self.mlp_norm.weight):
             # Inference on the device: the norm and the squared ReLU as one kernel each.
             normed = ops.rms_norm(hidden, self.mlp_norm.weight, self.mlp_norm.eps)
@@ -230,7 +262,8 @@ class DABSNBackbone(nn.Module):
     each block's world view followed by its inline MLP."""
 
     def __init__(self, input_dim: int, layers, *, residual: bool = False,
-                 mlp_ratio: float | None = None, block_chunk_t: int | None = None) -> None:
+                 mlp_ratio: float | None = None, block_chunk_t: int | None = None,
+                 **mlp) -> None:
         super().__init__()
         self.input_dim = int(input_dim)
         self.layer_specs = parse_layer_specs(layers)
@@ -241,7 +274,7 @@ class DABSNBackbone(nn.Module):
         for spec in self.layer_specs:
             blocks.append(DABSNBlock(width, spec.hidden_dim, spec.resolved_state_dim,
                                      spec.read_geometry, residual=residual, mlp_ratio=mlp_ratio,
-                                     block_chunk_t=block_chunk_t))
+                                     block_chunk_t=block_chunk_t, **mlp))
             width = spec.hidden_dim
         self.blocks = nn.ModuleList(blocks)
         self.output_dim = width
@@ -264,18 +297,21 @@ class DABSNSequenceLM(nn.Module):
     here; the field/hybrid geometries and the middle MLP stack are outside this backend.
 
     ``embed_scale`` (None: the plain embedding) multiplies the token embedding, as a model with
-    tied embeddings wants: the table then runs through ``scaled_embedding``.
+    tied embeddings wants: the table then runs through ``scaled_embedding``. ``mlp_activation``,
+    ``mlp_norm`` and ``mlp_bias`` are the blocks' (see ``DABSNBlock``).
     """
 
     is_dabsn_sequence_lm = True
     embed_scale: float | None = None
+    mlp_activation: str | None = None
 
     def __init__(self, vocab: int, hidden_dim: int, depth: int = 1, layer_geometries=None, *,
                  layers=None, state_dim: int | None = None, tie_embeddings: bool = False,
                  grad_checkpoint: bool = False, residual: bool = False,
                  mlp_ratio: float | None = None, mlp_middle_depth: int = 0,
                  mlp_depth_index: int = 0, block_chunk_t: int | None = None,
-                 embed_scale: float | None = None) -> None:
+                 embed_scale: float | None = None, mlp_activation: str | None = None,
+                 mlp_norm: str = "rms", mlp_bias: bool = False) -> None:
         super().__init__()
         del grad_checkpoint  # block time-chunking (block_chunk_t) is this backend's checkpoint
         if int(mlp_middle_depth) != 0:
@@ -288,6 +324,8 @@ class DABSNSequenceLM(nn.Module):
         self.mlp_ratio = None if mlp_ratio is None else float(mlp_ratio)
         self.mlp_middle_depth = int(mlp_middle_depth)
         self.mlp_depth_index = int(mlp_depth_index)
+        self.mlp_activation = mlp_activation
+        self.mlp_norm, self.mlp_bias = mlp_norm, bool(mlp_bias)
         specs = parse_layer_specs(layers)
         if not specs:
             geoms = layer_geometries or "seq"
@@ -301,7 +339,9 @@ class DABSNSequenceLM(nn.Module):
         self.embed_scale = None if embed_scale is None else float(embed_scale)
         self.embed = nn.Embedding(self.vocab, self.hidden_dim)
         self.backbone = DABSNBackbone(self.hidden_dim, specs, residual=self.residual,
-                                      mlp_ratio=self.mlp_ratio, block_chunk_t=block_chunk_t)
+                                      mlp_ratio=self.mlp_ratio, block_chunk_t=block_chunk_t,
+                                      mlp_activation=mlp_activation, mlp_norm=mlp_norm,
+                                      mlp_bias=mlp_bias)
         self.readout = nn.Linear(self.backbone.output_dim, self.vocab)
         if self.tie_embeddings and self.backbone.output_dim == self.hidden_dim:
             self.readout.weight = self.embed.weight

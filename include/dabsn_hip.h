@@ -17,7 +17,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#define DABSN_HIP_ABI_VERSION 22
+#define DABSN_HIP_ABI_VERSION 23
 
 /* Status codes returned by every entry point. */
 #define DABSN_OK 0
@@ -769,6 +769,51 @@ size_t dabsn_hip_embedding_workspace_bytes(int64_t n, int64_t V, int64_t H);
 int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const int64_t* ids,
                             int64_t padding_idx, const void* grad, float scale, void* dweight,
                             void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---- the block's MLP: norms, and products with their epilogue -----------------------
+ * New operators beside the MLP branch of the block (src/dabsn/model.py:35-45, 179-195):
+ *
+ * dabsn_hip_norm_fwd: out [rows, H] = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(mean of
+ * (x - mean)^2 + eps); layer = 0: the RMS norm, mean = 0. x has row stride ldx; weight and bias
+ * [H] (each NULL: none) have type wdtype: dtype's or fp32. H <= 16384. stats ([rows][2] or NULL)
+ * keeps (mean, rstd). _bwd: dx [rows, H] = the gradient of x for grad (row stride ldg), plus add
+ * [rows, H] (NULL: none); dweight and dbias [H] (each NULL: none) = sums over the rows, in fp32
+ * and a fixed order. Workspace (for dweight and dbias): dabsn_hip_norm_workspace_bytes.
+ *
+ * dabsn_hip_linear: C [M, N] = act(A B^T + bias) * slope + residual, fp32 until its one rounding.
+ * A [M, K], row stride lda; B [N, K], or with transB its transpose [K, N]; with transA
+ * (and transB) A is stored as [K, M] too; any alignment. act: 0 none, 1 squared ReLU, 2 GELU (by the error function), 3 SiLU. keep [M, N]
+ * (row stride ldk; NULL: none) receives the activation's derivative. slope_kind 1: slope [M, N] as it is, 2: slope
+ * holds the squared ReLU's output h and the factor is 2 sqrt(h). Sums over K are cut for few tiles
+ * and joined in order. Workspace: dabsn_hip_linear_workspace_bytes(dtype, M, N, K), 16-byte
+ * aligned (0: none).
+ * dabsn_hip_linear_slope: dz [rows, n] (row stride ldz; NULL: none) = grad * slope, and dbias [n]
+ * (NULL: none) its column sums before the rounding. */
+int dabsn_hip_norm_fwd(int dtype, int wdtype, int layer, int64_t rows, int64_t H, const void* x,
+                       int64_t ldx, const void* weight, const void* bias, float eps, void* out,
+                       float* stats, hipStream_t stream);
+size_t dabsn_hip_norm_workspace_bytes(int dtype, int64_t rows, int64_t H);
+int dabsn_hip_norm_bwd(int dtype, int wdtype, int layer, int64_t rows, int64_t H, const void* x,
+                       int64_t ldx, const void* weight, const float* stats, const void* grad,
+                       int64_t ldg, const void* add, void* dx, void* dweight, void* dbias,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+typedef struct dabsn_linear_call {
+  int dtype, transA, transB, act, slope_kind;
+  int64_t M, N, K;
+  const void *A, *B, *bias, *slope, *residual;
+  int64_t lda, ldb, lds, ldr, ldc, ldk;
+  void *C, *keep, *workspace;
+  size_t workspace_bytes;
+} dabsn_linear_call;
+
+size_t dabsn_hip_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int dabsn_hip_linear(const dabsn_linear_call* call, hipStream_t stream);
+size_t dabsn_hip_linear_slope_workspace_bytes(int dtype, int64_t rows, int64_t n);
+int dabsn_hip_linear_slope(int dtype, int64_t rows, int64_t n, const void* grad, int64_t ldg,
+                           const void* slope, int64_t lds, int slope_kind, void* dz, int64_t ldz,
+                           void* dbias, void* workspace, size_t workspace_bytes,
+                           hipStream_t stream);
 
 #ifdef __cplusplus
 }
