@@ -61,7 +61,8 @@ class CoreBwdCall(ctypes.Structure):
 class LinearCall(ctypes.Structure):
     """Mirror of ``dabsn_linear_call``."""
 
-    _fields_ = ([(n, i32) for n in ("dtype", "transA", "transB", "act", "slope_kind")]
+    _fields_ = ([(n, i32) for n in ("dtype", "transA", "transB", "padA", "padB", "padC", "act",
+                                     "slope_kind")]
                 + [(n, i64) for n in ("M", "N", "K")]
                 + [(n, vp) for n in ("A", "B", "bias", "slope", "residual")]
                 + [(n, i64) for n in ("lda", "ldb", "lds", "ldr", "ldc", "ldk")]
@@ -204,7 +205,7 @@ _SIGNATURES = {
     "dabsn_hip_norm_workspace_bytes": ([i32, i64, i64], sz),
     "dabsn_hip_norm_bwd": (
         [i32, i32, i32, i64, i64, vp, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp, sz, vp], i32),
-    "dabsn_hip_linear_workspace_bytes": ([i32, i64, i64, i64], sz),
+    "dabsn_hip_linear_workspace_bytes": ([ctypes.POINTER(LinearCall)], sz),
     "dabsn_hip_linear": ([ctypes.POINTER(LinearCall), vp], i32),
     "dabsn_hip_linear_slope_workspace_bytes": ([i32, i64, i64], sz),
     "dabsn_hip_linear_slope": (

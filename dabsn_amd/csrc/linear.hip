@@ -6,11 +6,6 @@
 // stored as its transpose, A[k * lda + m]: the forward needs neither transposed, the gradient of
 // the rows has B = W transposed, that of the weight both. The products are bound by the matrix
 // cores once there are a few hundred rows, by the weight's bytes below.
-//
-// A workgroup of WM x WN waves forms a BM x BN tile, BK deep steps through two buffers in LDS:
-// while the matrix instructions take step k from one, the loads of step k + 2 are on their way to
-// registers and step k + 1 goes to the other. Operands come at any alignment (unaligned 16-byte
-// loads), beyond their edge as zeros.
 #include "capi.hpp"
 #include "common.hpp"
 
@@ -31,8 +26,8 @@ enum Slope : int { kNoSlope = 0, kStored = 1, kFromSquare = 2 };
 template <typename E>
 struct Args {
   int M, N, K;
-  const E *A, *B;
-  int64_t lda, ldb;
+  const bf16 *A, *B;  // as they are, or as pack_kernel leaves them
+  int64_t lda, ldb, planeA, planeB;
   const E* bias;
   int act;
   const E* slope;
@@ -42,6 +37,7 @@ struct Args {
   int64_t ldr;
   E* C;
   int64_t ldc;
+  int padC;  // rows of C get zeros up to a multiple of 8
   E* keep;  // act'(z); NULL: not kept
   int64_t ldk;
   int mt, nt, splits, kper;
@@ -49,21 +45,48 @@ struct Args {
   int64_t ldp;
 };
 
-// act(z) and its derivative.
+// act(z) and its derivative. Where they are rounded to bf16, the hardware's exp and reciprocal do
+// (2^-22 and 2^-23 of their values), and erfc(x) = exp(-x^2) erfcx(x) with erfcx as a polynomial in
+// t = 1 / (1 + 0.46 x), a fit of our own for x >= 0 that is within 1.7e-5 of the value up to x = 60
+// (2^-8 is a rounding's): 20 instructions instead of erfcf's 70.
 template <typename E>
 __device__ __forceinline__ float activate(int act, float z, float& slope) {
+  constexpr bool low = sizeof(E) == 2;
+  constexpr float LOG2E = 1.44269504088896341f;
   if (act == kRelu2) {
     const float r = z > 0.0f || z != z ? z : 0.0f;
     slope = 2.0f * r;
     return r * r;
   }
   if (act == kGelu) {
-    const float below = 0.5f * erfcf(z * -0.70710678118654752f);
-    slope = fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), below);
+    float below, bell;  // the normal distribution function and exp(-z^2 / 2)
+    if constexpr (low) {
+      const float x = fabsf(z) * 0.70710678118654752f;
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.46f, x, 1.0f));
+      float q = fmaf(-0.12698957f, t, 0.2432926f);
+      q = fmaf(q, t, 0.12421153f);
+      q = fmaf(q, t, 0.24096189f);
+      q = fmaf(q, t, 0.25897348f);
+      q = fmaf(q, t, 0.25953397f);
+      bell = __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E));
+      const float tail = 0.5f * q * t * bell;
+      below = z > 0.0f ? 1.0f - tail : tail;
+    } else {
+      below = 0.5f * erfcf(z * -0.70710678118654752f);
+      bell = expf(-0.5f * z * z);
+    }
+    slope = fmaf(z * 0.39894228040143268f, bell, below);
     return z * below;
   }
   if (act == kSilu) {
-    const float s = 1.0f / (1.0f + expf(-z)), rest = 1.0f / (1.0f + expf(z));
+    float s, rest;
+    if constexpr (low) {
+      s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * z));
+      rest = 1.0f - s;
+    } else {
+      s = 1.0f / (1.0f + expf(-z));
+      rest = 1.0f / (1.0f + expf(z));
+    }
     slope = fmaf(z * s, rest, s);
     return z * s;
   }
@@ -75,111 +98,75 @@ __device__ __forceinline__ float factor(int kind, float s) {
   return kind == kFromSquare ? 2.0f * sqrtf(s) : s;
 }
 
+// Eight columns of a row, the first `left` of them within it, at any alignment.
 template <typename E>
-__device__ __forceinline__ void put_one(const Args<E>& a, int m, int n, float v) {
-  if (a.bias) v += ld(a.bias, n);
-  float slope;
-  v = activate<E>(a.act, v, slope);
-  if (a.keep) st(a.keep, static_cast<size_t>(m) * a.ldk + n, slope);
-  if (a.slope_kind) v *= factor(a.slope_kind, ld(a.slope, static_cast<size_t>(m) * a.lds + n));
-  if (a.residual) v += ld(a.residual, static_cast<size_t>(m) * a.ldr + n);
-  st(a.C, static_cast<size_t>(m) * a.ldc + n, v);
+__device__ __forceinline__ void take(const E* p, int left, float (&v)[8]) {
+  E raw[8];
+  if (left >= 8) {
+    __builtin_memcpy(raw, p, sizeof(raw));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) raw[e] = e < left ? p[e] : static_cast<E>(0);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = to_f(raw[e]);
+}
+template <typename E>
+__device__ __forceinline__ void put(E* p, int left, const float (&v)[8]) {
+  E raw[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) raw[e] = from_f<E>(v[e]);
+  if (left >= 8) {
+    __builtin_memcpy(p, raw, sizeof(raw));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) p[e] = raw[e];
+  }
 }
 
-template <typename E, bool T, int BT, int BK, int NTH>
-struct Stage {
-  static constexpr int VEC = 16 / static_cast<int>(sizeof(E));
-  static constexpr int COLS = T ? BT : BK, ROWS = T ? BK : BT;
-  static constexpr int CPR = COLS / VEC, NV = ROWS * CPR / NTH;
-  static_assert(ROWS * CPR % NTH == 0, "staging must divide evenly");
-
-  // Position of 16-byte chunk c in row r of the tile. K-contiguous rows are 128 bytes: the 16 lanes
-  // of one read (a chunk of 16 rows) then touch all 64 banks. Transposed rows are read in pieces of
-  // 32 bytes (bf16: four rows by 16 columns a 16 lanes) or 64 (fp32: 16 columns of a row), eight or
-  // four of them by different rows at once.
-  __device__ static int pos(int c, int r) {
-    if constexpr (!T) return c ^ ((r >> 1) & 7);
-    if constexpr (sizeof(E) == 2) return c ^ (((r & 3) | ((r >> 1) & 4)) << 1);
-    return c ^ (((r >> 2) & 3) << 2);
-  }
-
-  // Chunks of the tile at row r0, column c0 of a matrix of `rows` x `cols`, zeros beyond.
-  __device__ static void load(const E* p, int64_t ld, int r0, int c0, int rows, int cols, int tid,
-                              u32x4 (&v)[NV]) {
-    const bool inside = r0 + ROWS <= rows && c0 + COLS <= cols;
+// The epilogue of the sums v at row m, columns n to n + 7 (n < N a multiple of 8).
+template <typename E>
+__device__ __forceinline__ void finish(const Args<E>& a, int64_t m, int n, float (&v)[8],
+                                       const float (&bias)[8]) {
+  const int left = a.N - n;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int q = tid + i * NTH, r = r0 + q / CPR, c = c0 + q % CPR * VEC;
-      const E* at = p + static_cast<int64_t>(r) * ld + c;
-      if (inside || (r < rows && c + VEC <= cols)) {
-        __builtin_memcpy(&v[i], at, 16);
-      } else {
-        E raw[VEC];
+  for (int e = 0; e < 8; ++e) v[e] += bias[e];
+  if (a.act) {
+    float slope[8];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) raw[e] = r < rows && c + e < cols ? at[e] : static_cast<E>(0);
-        __builtin_memcpy(&v[i], raw, 16);
-      }
-    }
+    for (int e = 0; e < 8; ++e) v[e] = activate<E>(a.act, v[e], slope[e]);
+    if (a.keep) put(a.keep + m * a.ldk + n, left, slope);
   }
-  __device__ static void store(E* lds, int tid, const u32x4 (&v)[NV]) {
+  if (a.slope_kind) {
+    float s[8];
+    take(a.slope + m * a.lds + n, left, s);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int q = tid + i * NTH, r = q / CPR;
-      *reinterpret_cast<u32x4*>(lds + r * COLS + pos(q % CPR, r) * VEC) = v[i];
-    }
+    for (int e = 0; e < 8; ++e) v[e] *= factor(a.slope_kind, s[e]);
   }
-};
-
-// Fragments of a wave's 16-row tiles for the matrix instructions.
-template <typename E, bool T, int BT, int BK>
-struct Frag;
-template <bool T, int BT, int BK>
-struct Frag<bf16, T, BT, BK> {
-  static constexpr int KSTEP = 32;
-  using R = bf16x8;
-  // Rows row0 + (lane & 15), k = ks * 32 + (lane >> 4) * 8 + 0..7.
-  __device__ static R get(const bf16* lds, int row0, int ks, int lane) {
-    const int li = lane & 15, g = lane >> 4;
-    if constexpr (!T) {
-      const int r = row0 + li;
-      return __builtin_bit_cast(
-          R, *reinterpret_cast<const u32x4*>(lds + r * BK + ((ks * 4 + g) ^ ((r >> 1) & 7)) * 8));
-    } else {
-      // Two transposing reads: each takes four k of 16 columns per 16 lanes.
-      const int f = (li >> 2) | ((g & 1) << 2);
-      const bf16* at = lds + (ks * 32 + g * 8 + (li >> 2)) * BT + ((row0 >> 4) ^ f) * 16 + (li & 3) * 4;
-      using L = __attribute__((address_space(3))) s16x4;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)at);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(at + 4 * BT));
-      return __builtin_bit_cast(R, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-  }
-  __device__ static f32x4 mma(R a, R b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-};
-template <bool T, int BT, int BK>
-struct Frag<float, T, BT, BK> {
-  static constexpr int KSTEP = 16;
-  using R = f32x4;
-  // Rows row0 + (lane & 15), k = ks * 16 + (lane >> 4) * 4 + 0..3: four matrix instructions of
-  // four k each, one element of every group at a time.
-  __device__ static R get(const float* lds, int row0, int ks, int lane) {
-    const int li = lane & 15, g = lane >> 4;
-    if constexpr (!T) {
-      const int r = row0 + li;
-      return *reinterpret_cast<const f32x4*>(lds + r * BK + ((ks * 4 + g) ^ ((r >> 1) & 7)) * 4);
-    } else {
-      const float* at = lds + (ks * 16 + g * 4) * BT + ((row0 >> 4) ^ g) * 16 + li;
-      return (f32x4){at[0], at[BT], at[2 * BT], at[3 * BT]};
-    }
-  }
-  __device__ static f32x4 mma(R a, R b, f32x4 c) {
+  if (a.residual) {
+    float r[8];
+    take(a.residual + m * a.ldr + n, left, r);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
-    return c;
+    for (int e = 0; e < 8; ++e) v[e] += r[e];
   }
-};
+  if (a.padC) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < left ? v[e] : 0.0f;
+    put(a.C + m * a.ldc + n, 8, v);
+  } else {
+    put(a.C + m * a.ldc + n, left, v);
+  }
+}
+template <typename E>
+__device__ __forceinline__ void bias_of(const Args<E>& a, int n, float (&b)[8]) {
+  if (a.bias) {
+    take(a.bias + n, a.N - n, b);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+  }
+}
 
 // The tile and split of workgroup L: consecutive workgroups go round the 8 XCDs, so each XCD gets a
 // contiguous range of the order, patches of 8 x 8 tiles whose operands its L2 holds.
@@ -200,147 +187,408 @@ __device__ __forceinline__ bool tile_of(int L, int nblk, int splits, int mt_n, i
   return true;
 }
 
+// ---- the products -----------------------------------------------------------------------------
+constexpr int PK = 32, BUFS = 4;
+constexpr uint32_t NOWHERE = 0x80000000u;  // an offset beyond every buffer resource
+
+// A tile's way into LDS, BT rows (or columns, where transposed) by PK k a step: 16-byte chunks in
+// the order of their positions, K-contiguous rows of 64 bytes (16 lanes read a chunk of 16 rows) or
+// transposed rows of 2 BT bytes (32 lanes read 32 bytes of 8 rows), positions permuted so that
+// such a read touches every bank once.
+template <bool T, int BT, int NTH>
+struct Feed {
+  static constexpr int NV = BT * PK * 2 / 16 / NTH;
+  static_assert(BT * PK * 2 % (16 * NTH) == 0, "loads must divide evenly");
+  const bf16* base;  // the tile's first element
+  uint32_t bytes;    // from there to the matrix's end
+  u32x4 rsrc;
+  uint32_t off[NV], step;
+  int k[NV];
+
+  __device__ static int turn(int r) {
+    const int f = (r & 3) | ((r >> 1) & 4);
+    return BT >= 128 ? f : f >> 1;
+  }
+  __device__ void init(const bf16* p, int64_t ld, int r0, int rows, int k0, int len, int tid) {
+    base = T ? p + static_cast<int64_t>(k0) * ld + r0 : p + static_cast<int64_t>(r0) * ld + k0;
+    // K-contiguous rows hold zeros up to a whole chunk (and nothing needs the last row's).
+    const int64_t last = T ? static_cast<int64_t>(len - 1) * ld + (rows - r0)
+                           : static_cast<int64_t>(min(BT, rows - r0) - 1) * ld + (len + 7) / 8 * 8;
+    bytes = static_cast<uint32_t>((last * 2 + 3) & ~3ll);
+    step = static_cast<uint32_t>(T ? PK * ld * 2 : PK * 2);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int q = tid + i * NTH;
+      const int r = T ? q / (BT / 8) : q / 4;
+      const int c = T ? (q % (BT / 8)) ^ (turn(r) << 1) : (q % 4) ^ ((r >> 2) & 3);
+      off[i] = static_cast<uint32_t>((r * ld + c * 8) * 2);
+      k[i] = T ? r : c * 8;
+    }
+  }
+  __device__ void plane(int64_t at) {
+    const uint64_t p = reinterpret_cast<uint64_t>(base + at);
+    rsrc = (u32x4){static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xffffu, bytes, 0x00020000u};
+  }
+  // The chunks of step t to LDS from byte `lds` on, zeros where k is not below `len`. Written as
+  // assembly, since before a transposing read the compiler would wait for every load under way; the
+  // kernel counts them itself. (They write no register.)
+  __device__ void load(uint32_t lds, int t, int len) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t o = t * PK + k[i] < len ? off[i] + t * step : NOWHERE;
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                       lds + i * NTH * 16),
+                   "v"(o), "s"(rsrc)
+                   : "memory");
+    }
+  }
+};
+
+// A wave's fragments of a step: tile i of 16 rows from its first row on, eight k a lane. Addresses
+// are bytes of LDS; `at` covers two buffers by the instructions' 16-bit offsets, and is made anew
+// for each step (the compiler would keep one register for every tile and buffer).
+template <bool T, int BT>
+struct Reader {
+  uint32_t base;
+  __device__ void init(uint32_t lds, int row, int lane) {
+    const int li = lane & 15, g = lane >> 4, r = g * 8 + (li >> 2);
+    base = lds + (T ? r * BT * 2 + ((row / 16) ^ Feed<true, BT, 64>::turn(r)) * 32 + (li & 3) * 8
+                    : (row + li) * PK * 2 + (g ^ (li >> 2)) * 16);
+  }
+  __device__ uint32_t at(int bytes) const {
+    uint32_t p = base + bytes;
+    asm volatile("" : "+v"(p));
+    return p;
+  }
+  template <typename V>
+  using Lds = __attribute__((address_space(3))) V*;
+  __device__ static bf16x8 get(uint32_t at, int bytes, int i) {
+    if constexpr (!T) {
+      return __builtin_bit_cast(bf16x8, *(Lds<const u32x4>)(at + bytes + i * 16 * PK * 2));
+    } else {
+      // Two transposing reads, each of four k by 16 columns per 16 lanes. (A wave's rows start at a
+      // multiple of its tiles, so adding i to the tile's number is an exclusive or.)
+      const uint32_t p = (at ^ (i * 32)) + bytes;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds<s16x4>)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds<s16x4>)(p + 8 * BT));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// Steps of 32 k through four buffers in LDS, filled by loads that go there without registers.
+// During step t a wave issues its share of step t + 3's loads and multiplies step t's fragments,
+// which are in registers already; each fragment of A makes room for step t + 1's as soon as it has
+// been used, those of B have a second set. One barrier a step: before it a wave waits until its
+// loads of step t + 1 have landed (those of t + 2 may be under way) and all reads but step t - 1's
+// have; after it, all of step t + 1 is in LDS, and the buffer that step t + 3 overwrites, t - 1's,
+// was last read in step t - 2.
+//
+// fp32 operands come as three bf16 planes each (x = hi + mid + lo, 8 bits each, the remainders
+// exact): the steps then go through six products of planes, small ones first; the three left out
+// are below 2^-24 of the product. At 2.5 PFLOP/s for bf16 against 0.16 for fp32 this is 2.6 times
+// the fp32 instructions' rate.
 template <typename E, bool TA, bool TB, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nblk) {
-  constexpr int NTH = WM * WN * 64, BK = 128 / static_cast<int>(sizeof(E));
-  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  using SA = Stage<E, TA, BM, BK, NTH>;
-  using SB = Stage<E, TB, BN, BK, NTH>;
-  using FA = Frag<E, TA, BM, BK>;
-  using FB = Frag<E, TB, BN, BK>;
-  __shared__ __attribute__((aligned(16))) E ldsA[2][BM * BK], ldsB[2][BN * BK];
+  constexpr int NTH = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int PAIRS = sizeof(E) == 4 ? 6 : 1;
+  using FA = Feed<TA, BM, NTH>;
+  using FB = Feed<TB, BN, NTH>;
+  __shared__ __attribute__((aligned(16))) bf16 lds[BUFS][(BM + BN) * PK];
 
   int sp, mt, nt;
   if (!tile_of(blockIdx.x, nblk, a.splits, a.mt, a.nt, sp, mt, nt)) return;
   const int m0 = mt * BM, n0 = nt * BN;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-  const int k0 = sp * a.kper, kend = min(a.K, k0 + a.kper);
-  const int steps = (kend - k0 + BK - 1) / BK;
+  const int k0 = sp * a.kper, len = min(a.K - k0, a.kper);
+  const int each = (len + PK - 1) / PK, steps = PAIRS * each;
 
+  FA fa;
+  FB fb;
+  fa.init(a.A, a.lda, m0, a.M, k0, len, tid);
+  fb.init(a.B, a.ldb, n0, a.N, k0, len, tid);
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-  u32x4 va[SA::NV], vb[SB::NV];
-  auto load = [&](int it) {
-    const int k = k0 + it * BK;
-    if constexpr (TA) SA::load(a.A, a.lda, k, m0, kend, a.M, tid, va);
-    else SA::load(a.A, a.lda, m0, k, a.M, kend, tid, va);
-    if constexpr (TB) SB::load(a.B, a.ldb, k, n0, kend, a.N, tid, vb);
-    else SB::load(a.B, a.ldb, n0, k, a.N, kend, tid, vb);
+  constexpr int BUF = (BM + BN) * PK * 2;
+  const uint32_t lds0 = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) bf16*)lds[0]));
+  // The loads' place: step `at` of the pair. Those beyond the last step go too, as zeros and
+  // without traffic, so that every step has the same number of them.
+  int pair = 0, at = 0;
+  auto planes = [&]() {
+    // (lo hi) (hi lo) (mid mid) (mid hi) (hi mid) (hi hi), the planes hi, mid, lo in this order.
+    constexpr uint32_t PA = 0x001102, PB = 0x010120;
+    fa.plane(PAIRS > 1 ? static_cast<int64_t>((PA >> (4 * pair)) & 3) * a.planeA : 0);
+    fb.plane(PAIRS > 1 ? static_cast<int64_t>((PB >> (4 * pair)) & 3) * a.planeB : 0);
   };
-  auto store = [&](int buf) {
-    SA::store(ldsA[buf], tid, va);
-    SB::store(ldsB[buf], tid, vb);
-  };
-  if (steps > 0) {
-    load(0);
-    store(0);
-    if (steps > 1) load(1);
-  }
-  __syncthreads();
-  for (int it = 0; it < steps; ++it) {
-    const int buf = it & 1;
-    if (it + 1 < steps) {
-      store(buf ^ 1);  // released by the barrier that ended step it - 1
-      if (it + 2 < steps) load(it + 2);
+  planes();
+  auto feed = [&](int buf) {
+    fa.load(lds0 + buf * BUF + wave * 1024, at, len);
+    fb.load(lds0 + buf * BUF + BM * PK * 2 + wave * 1024, at, len);
+    ++at;
+    if (PAIRS > 1 && at == each && pair + 1 < PAIRS) {
+      at = 0;
+      ++pair;
+      planes();
     }
+  };
+  using RA = Reader<TA, BM>;
+  using RB = Reader<TB, BN>;
+  RA ra;
+  RB rb;
+  ra.init(lds0, wm, lane);
+  rb.init(lds0 + BM * PK * 2, wn, lane);
+  constexpr int READS = TM * (TA ? 2 : 1) + TN * (TB ? 2 : 1);
+  bf16x8 fra[TM], frb[2][TN];
+  auto meet = [&]() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" ::"n"(FA::NV + FB::NV),
+                 "n"(READS < 15 ? READS : 15)
+                 : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](int t, int set) {
+    const int next = (t + 1) % BUFS, bytes = next % 2 * BUF;
+    meet();
+    feed((t + 3) % BUFS);
+    const uint32_t pa = ra.at(next / 2 * 2 * BUF), pb = rb.at(next / 2 * 2 * BUF);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int ks = 0; ks < BK / FA::KSTEP; ++ks) {
-      typename FA::R af[TM];
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) af[i] = FA::get(ldsA[buf], wm + i * 16, ks, lane);
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frb[set][j], fra[i], acc[i][j], 0, 0, 0);
+      fra[i] = RA::get(pa, bytes, i);
+      if (i < TN) frb[set ^ 1][i] = RB::get(pb, bytes, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  static_assert(TN <= TM, "B's fragments are read beside A's");
+  feed(0);
+  feed(1);
+  meet();  // at most the second step's loads are under way
+  feed(2);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) frb[0][j] = RB::get(rb.base, 0, j);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) fra[i] = RA::get(ra.base, 0, i);
+  int t = 0;
+  for (; t + 4 <= steps; t += 4) {
+    step(0, 0);
+    step(1, 1);
+    step(2, 0);
+    step(3, 1);
+  }
+  if (t < steps) step(0, 0);
+  if (t + 1 < steps) step(1, 1);
+  if (t + 2 < steps) step(2, 0);
+  // No load may land after the workgroup has gone, nor in the epilogue's places.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  // B is the instruction's first operand: a lane holds four consecutive columns of a row. A wave
+  // turns HR rows at a time in its own part of LDS, positions of 16 bytes permuted by the row, and
+  // takes them back as eight columns a lane: whole lines for every access of the epilogue, and its
+  // code once.
+  constexpr int CW = TN * 16, HT = TM < 4 ? TM : 4, HR = HT * 16, LPR = CW / 8, RPP = 64 / LPR;
+  static_assert(sizeof(lds) >= static_cast<size_t>(WM * WN) * HR * CW * 4, "LDS holds the waves' parts");
+  float* mine = reinterpret_cast<float*>(lds) + wave * HR * CW;
+  const int n = n0 + wn + lane % LPR * 8, row = lane / LPR;
+  float bias[8];
+  if (n < a.N && !a.parts) bias_of(a, n, bias);
+#pragma unroll
+  for (int h = 0; h < TM / HT; ++h) {
+#pragma unroll
+    for (int i = 0; i < HT; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const typename FB::R bf = FB::get(ldsB[buf], wn + j * 16, ks, lane);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[i][j] = FA::mma(bf, af[i], acc[i][j]);
+        const int r = i * 16 + (lane & 15), c = j * 4 + (lane >> 4);
+        *reinterpret_cast<f32x4*>(mine + r * CW + (c ^ (r & (CW / 4 - 1))) * 4) = acc[h * HT + i][j];
       }
-    }
-    __syncthreads();
-  }
-
-  // B is the instruction's first operand: a lane holds four consecutive columns of a row.
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = m0 + wm + i * 16 + (lane & 15);
-    if (m >= a.M) continue;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+    for (int p = 0; p < HR; p += RPP) {
+      const int r = p + row, m = m0 + wm + h * HR + r;
+      if (m >= a.M || n >= a.N) continue;
+      const int c = lane % LPR * 2, x = r & (CW / 4 - 1);
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + r * CW + (c ^ x) * 4);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + r * CW + ((c + 1) ^ x) * 4);
       if (a.parts) {
-        float* p = a.parts + (static_cast<int64_t>(sp) * a.M + m) * a.ldp + n;
-        if (n < a.ldp) *reinterpret_cast<f32x4*>(p) = acc[i][j];  // ldp is a multiple of 4
+        f32x4* q = reinterpret_cast<f32x4*>(a.parts + (static_cast<int64_t>(sp) * a.M + m) * a.ldp + n);
+        q[0] = lo;
+        q[1] = hi;
       } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < a.N) put_one(a, m, n + r, acc[i][j][r]);
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        finish(a, m, n, v, bias);
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
-// The splits' sums in order, then the epilogue: a thread four columns.
+// An operand [rows][cols] of row stride ld as the products read it: rows of `to` values (a multiple
+// of 8) that end in zeros; fp32 as its planes hi, mid, lo, each [rows][to].
+template <typename E>
+__global__ void __launch_bounds__(256) pack_kernel(int64_t rows, int cols, const E* x, int64_t ld,
+                                                   int to, bf16* out, int64_t plane) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, per = to / 8;
+  if (i >= rows * per) return;
+  const int64_t r = i / per;
+  const int c = static_cast<int>(i % per) * 8;
+  const E* p = x + r * ld + c;
+  E v[8];
+  if (c + 8 <= cols) {
+    __builtin_memcpy(v, p, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[e] : static_cast<E>(0);
+  }
+  bf16* o = out + r * to + c;
+  if constexpr (sizeof(E) == 2) {
+    __builtin_memcpy(o, v, 16);
+  } else {
+    bf16 part[3][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float rest = v[e];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        bf16 h = f2bf(rest);
+        // A number that rounds to infinity is cut instead.
+        if ((h & 0x7fff) == 0x7f80 && fabsf(rest) < INFINITY)
+          h = static_cast<bf16>(__builtin_bit_cast(uint32_t, rest) >> 16);
+        part[k][e] = h;
+        rest = fabsf(rest) < INFINITY ? rest - bf2f(h) : 0.0f;  // infinity and NaN are in hi alone
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) __builtin_memcpy(o + k * plane, part[k], 16);
+  }
+}
+
+// The splits' sums in order, then the epilogue: a thread eight columns.
 template <typename E>
 __global__ void __launch_bounds__(256) join_kernel(Args<E> a) {
-  const int64_t quads = a.ldp / 4, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= quads * a.M) return;
-  const int m = static_cast<int>(i / quads), n = static_cast<int>(i % quads) * 4;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s)
-    v += *reinterpret_cast<const f32x4*>(a.parts + (static_cast<int64_t>(s) * a.M + m) * a.ldp + n);
+  const int64_t per = a.ldp / 8, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= per * a.M) return;
+  const int64_t m = i / per;
+  const int n = static_cast<int>(i % per) * 8;
+  float v[8] = {}, bias[8];
+  bias_of(a, n, bias);
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = a.parts + (s * static_cast<int64_t>(a.M) + m) * a.ldp + n;
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (n + r < a.N) put_one(a, m, n + r, v[r]);
+    for (int e = 0; e < 4; ++e) {
+      v[e] += lo[e];
+      v[4 + e] += hi[e];
+    }
+  }
+  finish(a, m, n, v, bias);
 }
 
-// Tiles of 128 x 128, and as many splits of K as bring the workgroups to the card's 256 units,
-// each of at least 8 steps.
+// How a product runs.
 struct Plan {
+  bool packA, packB;
+  int64_t lda, ldb, planeA, planeB;  // of the operands the kernel reads
+  bool big;                          // tiles of 256 x 256, else 128 x 128
   int mt, nt, splits, kper;
   int64_t ldp;
+  size_t atB, atParts, bytes;  // places in the workspace, which starts with A
 };
-static Plan plan_of(int64_t M, int64_t N, int64_t K, int size) {
-  const int64_t BK = 128 / size;
-  Plan p;
-  p.mt = static_cast<int>((M + 127) / 128);
-  p.nt = static_cast<int>((N + 127) / 128);
-  const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt, steps = (K + BK - 1) / BK;
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({256 / tiles, steps / 8, 64}));
+
+static size_t up16(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// bf16 operands are read where they lie if their chunks of 16 bytes are aligned and whole.
+static bool ready(const void* p, int64_t ld, bool trans, int64_t K, bool padded) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && (trans || padded || K % 8 == 0);
+}
+
+static Plan plan_of(const dabsn_linear_call& c) {
+  Plan p = {};
+  const bool f32 = c.dtype == kF32;
+  p.packA = f32 || !ready(c.A, c.lda, c.transA, c.K, c.padA);
+  p.packB = f32 || !ready(c.B, c.ldb, c.transB, c.K, c.padB);
+  const int64_t rowsA = c.transA ? c.K : c.M, rowsB = c.transB ? c.K : c.N;
+  p.lda = p.packA ? ((c.transA ? c.M : c.K) + 7) / 8 * 8 : c.lda;
+  p.ldb = p.packB ? ((c.transB ? c.N : c.K) + 7) / 8 * 8 : c.ldb;
+  p.planeA = p.packA ? rowsA * p.lda : 0;
+  p.planeB = p.packB ? rowsB * p.ldb : 0;
+  size_t at = p.packA ? up16(static_cast<size_t>(p.planeA) * (f32 ? 6 : 2)) : 0;
+  p.atB = at;
+  at += p.packB ? up16(static_cast<size_t>(p.planeB) * (f32 ? 6 : 2)) : 0;
+  p.atParts = at;
+  const int64_t big = ((c.M + 255) / 256) * ((c.N + 255) / 256);
+  p.big = big >= 192;
+  const int64_t edge = p.big ? 256 : 128;
+  p.mt = static_cast<int>((c.M + edge - 1) / edge);
+  p.nt = static_cast<int>((c.N + edge - 1) / edge);
+  const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt, steps = (c.K + PK - 1) / PK;
+  const int64_t room = p.big ? 256 : 512;
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({room / tiles, steps * (f32 ? 6 : 1) / 16, 64}));
+  // Offsets of a transposed operand's rows are 32 bits.
+  const int64_t ld = std::max<int64_t>(c.transA ? p.lda : 0, c.transB ? p.ldb : 0);
+  if (ld) splits = std::max<int64_t>(splits, (c.K * ld * 2 + (1ll << 30) - 1) >> 30);
   const int64_t each = std::max<int64_t>(1, (steps + splits - 1) / splits);
   p.splits = static_cast<int>(std::max<int64_t>(1, (steps + each - 1) / each));
-  p.kper = static_cast<int>(each * BK);
-  p.ldp = (N + 3) / 4 * 4;
+  p.kper = static_cast<int>(each * PK);
+  p.ldp = (c.N + 7) / 8 * 8;
+  if (p.splits > 1) at += static_cast<size_t>(p.splits) * c.M * p.ldp * sizeof(float);
+  p.bytes = at;
   return p;
 }
 
 template <typename E>
-static int run(const dabsn_linear_call& c, hipStream_t s) {
-  const Plan p = plan_of(c.M, c.N, c.K, sizeof(E));
+static int pack(int64_t rows, int64_t cols, const void* x, int64_t ld, int64_t to, bf16* out,
+                hipStream_t s) {
+  const int64_t blocks = (rows * (to / 8) + 255) / 256;
+  DABSN_REQUIRE(blocks < (1ll << 31), "linear: an operand of too many elements");
+  hipLaunchKernelGGL(pack_kernel<E>, dim3((unsigned)blocks), dim3(256), 0, s, rows, (int)cols,
+                     (const E*)x, ld, (int)to, out, rows * to);
+  DABSN_HIP_CHECK(hipGetLastError());
+  return DABSN_OK;
+}
+
+template <typename E>
+static int run(const dabsn_linear_call& c, const Plan& p, hipStream_t s) {
   Args<E> a = {};
   a.M = (int)c.M; a.N = (int)c.N; a.K = (int)c.K;
-  a.A = (const E*)c.A; a.B = (const E*)c.B; a.lda = c.lda; a.ldb = c.ldb;
+  char* ws = static_cast<char*>(c.workspace);
+  a.A = p.packA ? (const bf16*)ws : (const bf16*)c.A;
+  a.B = p.packB ? (const bf16*)(ws + p.atB) : (const bf16*)c.B;
+  a.lda = p.lda; a.ldb = p.ldb; a.planeA = p.planeA; a.planeB = p.planeB;
   a.bias = (const E*)c.bias; a.act = c.act;
   a.slope = (const E*)c.slope; a.lds = c.lds; a.slope_kind = c.slope ? c.slope_kind : kNoSlope;
   a.residual = (const E*)c.residual; a.ldr = c.ldr;
-  a.C = (E*)c.C; a.ldc = c.ldc; a.keep = (E*)c.keep; a.ldk = c.ldk;
-  a.mt = p.mt; a.nt = p.nt; a.splits = p.splits; a.kper = p.kper; a.ldp = p.ldp;
-  a.parts = p.splits > 1 ? (float*)c.workspace : nullptr;
-  const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt * p.splits;
-  DABSN_REQUIRE(tiles < (1ll << 31) - 8, "linear: too many tiles");
-  const int nblk = (int)((tiles + 7) / 8 * 8);
-#define L(TA, TB) \
-  hipLaunchKernelGGL((product_kernel<E, TA, TB, 128, 128, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk)
-  if (c.transA) L(true, true);
-  else if (c.transB) L(false, true);
-  else L(false, false);
+  a.C = (E*)c.C; a.ldc = c.ldc; a.keep = (E*)c.keep; a.ldk = c.ldk; a.padC = c.padC;
+  a.mt = p.mt; a.nt = p.nt; a.splits = c.K ? p.splits : 0; a.kper = p.kper; a.ldp = p.ldp;
+  a.parts = p.splits > 1 ? (float*)(ws + p.atParts) : nullptr;
+  if (c.K) {
+    int rc = DABSN_OK;
+    if (p.packA) rc = pack<E>(c.transA ? c.K : c.M, c.transA ? c.M : c.K, c.A, c.lda, p.lda, (bf16*)ws, s);
+    if (rc == DABSN_OK && p.packB)
+      rc = pack<E>(c.transB ? c.K : c.N, c.transB ? c.N : c.K, c.B, c.ldb, p.ldb, (bf16*)(ws + p.atB), s);
+    if (rc != DABSN_OK) return rc;
+    const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt * p.splits;
+    DABSN_REQUIRE(tiles < (1ll << 31) - 8, "linear: too many tiles");
+    const int nblk = (int)((tiles + 7) / 8 * 8);
+#define L(TA, TB)                                                                                     \
+  if (p.big)                                                                                          \
+    hipLaunchKernelGGL((product_kernel<E, TA, TB, 256, 256, 2, 4>), dim3(nblk), dim3(512), 0, s, a, nblk); \
+  else                                                                                                \
+    hipLaunchKernelGGL((product_kernel<E, TA, TB, 128, 128, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk)
+    if (c.transA) { L(true, true); }
+    else if (c.transB) { L(false, true); }
+    else { L(false, false); }
 #undef L
-  DABSN_HIP_CHECK(hipGetLastError());
-  if (a.parts) {
-    const int64_t blocks = (p.ldp / 4 * c.M + 255) / 256;
+    DABSN_HIP_CHECK(hipGetLastError());
+  }
+  if (a.parts || !c.K) {
+    const int64_t blocks = (p.ldp / 8 * c.M + 255) / 256;
     DABSN_REQUIRE(blocks < (1ll << 31), "linear: too many elements to join");
     hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)blocks), dim3(256), 0, s, a);
     DABSN_HIP_CHECK(hipGetLastError());
@@ -361,7 +609,9 @@ __global__ void __launch_bounds__(256) slope_kernel(int64_t rows, int n, const E
   const int64_t per = (rows + gridDim.y - 1) / gridDim.y;
   const int64_t r0 = blockIdx.y * per, r1 = std::min(rows, r0 + per);
   float sum[VEC] = {};
-  if (c < n) {
+  // dz's rows end in zeros up to a multiple of 8 where their stride has the room.
+  const int pad = (n + 7) / 8 * 8 <= ldz ? (n + 7) / 8 * 8 : n;
+  if (c < pad) {
     const bool whole = c + VEC <= n;
     for (int64_t r = r0 + wave; r < r1; r += 4) {
       E gv[VEC], sv[VEC], o[VEC];
@@ -388,7 +638,7 @@ __global__ void __launch_bounds__(256) slope_kernel(int64_t rows, int n, const E
         } else {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            if (c + e < n) dz[r * ldz + c + e] = o[e];
+            if (c + e < n || c + e < pad) dz[r * ldz + c + e] = o[e];  // o is 0 beyond n
         }
       }
     }
@@ -434,35 +684,45 @@ static int64_t slope_parts(int64_t rows, int64_t n, int size) {
 using namespace dabsn;
 using namespace dabsn::linear;
 
+static int check_linear(const dabsn_linear_call& c) {
+  DABSN_REQUIRE(c.dtype == kF32 || c.dtype == kBF16, "linear: bad dtype %d", c.dtype);
+  const int64_t top = (1ll << 31) - 65536, width = 1 << 22;
+  DABSN_REQUIRE(c.M >= 0 && c.M < top && c.N > 0 && c.N < top && c.K >= 0 && c.K < top,
+                "linear: bad shape M=%lld N=%lld K=%lld", (long long)c.M, (long long)c.N,
+                (long long)c.K);
+  DABSN_REQUIRE(!c.transA || c.transB, "linear: transA goes with transB");
+  DABSN_REQUIRE(c.lda >= (c.transA ? c.M : c.K) && c.ldb >= (c.transB ? c.N : c.K) && c.ldc >= c.N &&
+                    (!c.residual || c.ldr >= c.N) && (!c.slope || c.lds >= c.N) &&
+                    (!c.keep || c.ldk >= c.N),
+                "linear: a row stride is shorter than its row");
+  // 256 rows of an operand lie within 32-bit offsets.
+  DABSN_REQUIRE(c.lda < width && c.ldb < width, "linear: operands have rows of at most %lld elements",
+                (long long)width - 1);
+  DABSN_REQUIRE(c.act >= kNone && c.act <= kSilu && !(c.keep && c.act == kNone),
+                "linear: bad activation %d", c.act);
+  DABSN_REQUIRE(!c.slope || c.slope_kind == kStored || c.slope_kind == kFromSquare,
+                "linear: bad slope kind %d", c.slope_kind);
+  return DABSN_OK;
+}
+
 extern "C" {
 
-size_t dabsn_hip_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || (dtype != kF32 && dtype != kBF16)) return 0;
-  const Plan p = plan_of(M, N, K, dtype == kF32 ? 4 : 2);
-  return p.splits > 1 ? static_cast<size_t>(p.splits) * M * p.ldp * sizeof(float) : 0;
+size_t dabsn_hip_linear_workspace_bytes(const dabsn_linear_call* call) {
+  if (!call || call->M <= 0 || check_linear(*call) != DABSN_OK) return 0;
+  return plan_of(*call).bytes;
 }
 
 int dabsn_hip_linear(const dabsn_linear_call* call, hipStream_t stream) {
   DABSN_REQUIRE(call, "linear: null call");
   const dabsn_linear_call& c = *call;
-  DABSN_REQUIRE(c.dtype == kF32 || c.dtype == kBF16, "linear: bad dtype %d", c.dtype);
-  const int64_t top = (1ll << 31) - 65536;
-  DABSN_REQUIRE(c.M >= 0 && c.M < top && c.N > 0 && c.N < top && c.K >= 0 && c.K < top,
-                "linear: bad shape M=%lld N=%lld K=%lld", (long long)c.M, (long long)c.N,
-                (long long)c.K);
-  DABSN_REQUIRE(c.lda >= (c.transA ? c.M : c.K) && c.ldb >= (c.transB ? c.N : c.K) && c.ldc >= c.N &&
-                    (!c.residual || c.ldr >= c.N) && (!c.slope || c.lds >= c.N) && (!c.keep || c.ldk >= c.N),
-                "linear: a row stride is shorter than its row");
-  DABSN_REQUIRE(!c.transA || c.transB, "linear: transA goes with transB");
-  DABSN_REQUIRE(c.act >= kNone && c.act <= kSilu, "linear: bad activation %d", c.act);
-  DABSN_REQUIRE(!c.slope || c.slope_kind == kStored || c.slope_kind == kFromSquare,
-                "linear: bad slope kind %d", c.slope_kind);
-  if (c.M == 0) return DABSN_OK;
+  const int rc = check_linear(c);
+  if (rc != DABSN_OK || c.M == 0) return rc;
   DABSN_REQUIRE(c.C && (c.K == 0 || (c.A && c.B)), "linear: null pointer");
-  const size_t need = dabsn_hip_linear_workspace_bytes(c.dtype, c.M, c.N, c.K);
-  DABSN_REQUIRE(need == 0 || (c.workspace && c.workspace_bytes >= need),
-                "linear: workspace of %zu bytes, %zu needed", c.workspace_bytes, need);
-  return c.dtype == kF32 ? run<float>(c, stream) : run<bf16>(c, stream);
+  const Plan p = plan_of(c);
+  DABSN_REQUIRE(p.bytes == 0 || (c.workspace && c.workspace_bytes >= p.bytes &&
+                                 (reinterpret_cast<uintptr_t>(c.workspace) & 15u) == 0),
+                "linear: workspace of %zu bytes, %zu needed", c.workspace_bytes, p.bytes);
+  return c.dtype == kF32 ? run<float>(c, p, stream) : run<bf16>(c, p, stream);
 }
 
 size_t dabsn_hip_linear_slope_workspace_bytes(int dtype, int64_t rows, int64_t n) {
@@ -490,7 +750,7 @@ int dabsn_hip_linear_slope(int dtype, int64_t rows, int64_t n, const void* grad,
   const int64_t P = rows ? slope_parts(rows, n, size) : 0;
   const int kind = slope ? slope_kind : kNoSlope;
   if (rows) {
-    const dim3 grid((unsigned)((n + 1024 / size - 1) / (1024 / size)), (unsigned)P);
+    const dim3 grid((unsigned)(((n + 7) / 8 * 8 + 1024 / size - 1) / (1024 / size)), (unsigned)P);
     if (dtype == kF32)
       hipLaunchKernelGGL(slope_kernel<float>, grid, dim3(256), 0, stream, rows, (int)n,
                          (const float*)grad, ldg, (const float*)slope, lds, kind, (float*)dz, ldz, parts);

@@ -3,7 +3,6 @@ types inside autocast, and the launches."""
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -112,23 +111,26 @@ def padded(rows: int, n: int, like: Tensor) -> Tensor:
 def product(a: Tensor, b: Tensor, *, trans_a: bool = False, trans_b: bool = False,
             bias: Tensor | None = None, act: int = 0, keep: Tensor | None = None,
             slope: Tensor | None = None, slope_kind: int = 0, residual: Tensor | None = None,
-            out: Tensor | None = None) -> Tensor:
+            out: Tensor | None = None, pad_a: bool = False, pad_out: bool = False) -> Tensor:
     """act(a b^T + bias) * slope + residual (see ``dabsn_hip_linear``). a [M, K], or [K, M] with
-    ``trans_a``; b [N, K], or [K, N] with ``trans_b``."""
+    ``trans_a``; b [N, K], or [K, N] with ``trans_b``. ``pad_a``: a is a ``padded`` buffer that this
+    module filled; ``pad_out``: out is to be one."""
     lib = _lib.load()
     k, m = a.shape if trans_a else a.shape[::-1]
     n = b.shape[1] if trans_b else b.shape[0]
-    code = ops._code(a.dtype)
     if out is None:
-        out = a.new_empty((m, n))
-    nbytes = lib.dabsn_hip_linear_workspace_bytes(code, m, n, k)
-    ws = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        out = padded(m, n, a) if pad_out else a.new_empty((m, n))
     p, ld = ops._p, lambda t: 0 if t is None else row_stride(t)  # noqa: E731
+    call = _lib.LinearCall(
+        ops._code(a.dtype), trans_a, trans_b, pad_a, False, pad_out, act, slope_kind, m, n, k,
+        a.data_ptr(), b.data_ptr(), p(bias), p(slope), p(residual), row_stride(a), row_stride(b),
+        ld(slope), ld(residual), row_stride(out), ld(keep), out.data_ptr(), p(keep))
+    nbytes = lib.dabsn_hip_linear_workspace_bytes(call)
+    if nbytes:
+        ws = a.new_empty(nbytes, dtype=torch.uint8)
+        call.workspace, call.workspace_bytes = ws.data_ptr(), nbytes
     tk = ops.KernelTimer.begin("linear", a)
-    _lib.check(lib.dabsn_hip_linear(ctypes.byref(_lib.LinearCall(
-        code, trans_a, trans_b, act, slope_kind, m, n, k, a.data_ptr(), b.data_ptr(), p(bias),
-        p(slope), p(residual), row_stride(a), row_stride(b), ld(slope), ld(residual),
-        row_stride(out), ld(keep), out.data_ptr(), p(keep), p(ws), nbytes)), stream(a)), "linear")
+    _lib.check(lib.dabsn_hip_linear(call, stream(a)), "linear")
     ops.KernelTimer.end(tk)
     return out
 

@@ -67,7 +67,7 @@ class _Linear(torch.autograd.Function):
             rows = dense.rows_of(g)
             dz, db = dense.slope_product(rows, slope, ctx.kind, need[0] or need[1], need[2])
             if need[0]:
-                dx = dense.product(dz, weight, trans_b=True)
+                dx = dense.product(dz, weight, trans_b=True, pad_a=dz is not rows)
             if need[1]:
                 dw = dense.product(dz, x, trans_a=True, trans_b=True)
         return dx, dw, db, g if need[3] else None, None
@@ -115,9 +115,8 @@ class _MLP(torch.autograd.Function):
         with dense.on(x):
             normed, stats = dense.norm(x, nw, nb, eps, layer, True)
             keep, kind = _keeps(x, w1.shape[0], act, False)
-            h = dense.product(normed, w1, bias=b1, act=act, keep=keep,
-                              out=dense.padded(x.shape[0], w1.shape[0], x))
-            out = dense.product(h, w2, bias=b2, residual=x)
+            h = dense.product(normed, w1, bias=b1, act=act, keep=keep, pad_out=True)
+            out = dense.product(h, w2, bias=b2, residual=x, pad_a=True)
         ctx.save_for_backward(x, nw, stats, normed, w1, h, keep, w2)
         ctx.kind, ctx.layer = kind, layer
         ctx.dtype = (x if nw is None and nb is None else nb if nw is None else nw).dtype
@@ -139,13 +138,13 @@ class _MLP(torch.autograd.Function):
             if any(need[:5]):
                 slope = h if ctx.kind == dense._FROM_SQUARE else keep
                 dz = dense.product(rows, w2, trans_b=True, slope=slope, slope_kind=ctx.kind,
-                                   out=dense.padded(*h.shape, h))
+                                   pad_out=True)
                 if need[4]:
                     _, db1 = dense.slope_product(dz, None, 0, False, True)
                 if need[3]:
                     dw1 = dense.product(dz, normed, trans_a=True, trans_b=True)
                 if any(need[:3]):
-                    dn = dense.product(dz, w1, trans_b=True)
+                    dn = dense.product(dz, w1, trans_b=True, pad_a=True)
                     dx, dnw, dnb = dense.norm_backward(x, nw, stats, dn, ctx.layer, rows, ctx.dtype,
                                                        need[1], need[2])
         return dx, dnw, dnb, dw1, db1, dw2, db2, None, None, None
@@ -190,7 +189,6 @@ def fused_mlp(x: Tensor, w1: Tensor, w2: Tensor, b1: Tensor | None = None,
     else:
         with dense.on(x):
             normed, _ = dense.norm(rows, nw, nb, eps, layer, False)
-            mid = dense.product(normed, w1, bias=b1, act=act,
-                                out=dense.padded(rows.shape[0], w1.shape[0], rows))
-            out = dense.product(mid, w2, bias=b2, residual=rows)
+            mid = dense.product(normed, w1, bias=b1, act=act, pad_out=True)
+            out = dense.product(mid, w2, bias=b2, residual=rows, pad_a=True)
     return out if x.dim() == 2 else out.view(x.shape)

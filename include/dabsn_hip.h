@@ -784,10 +784,13 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
  * A [M, K], row stride lda; B [N, K], or with transB its transpose [K, N]; with transA
  * (and transB) A is stored as [K, M] too; any alignment. act: 0 none, 1 squared ReLU, 2 GELU (by the error function), 3 SiLU. keep [M, N]
  * (row stride ldk; NULL: none) receives the activation's derivative. slope_kind 1: slope [M, N] as it is, 2: slope
- * holds the squared ReLU's output h and the factor is 2 sqrt(h). Sums over K are cut for few tiles
- * and joined in order. Workspace: dabsn_hip_linear_workspace_bytes(dtype, M, N, K), 16-byte
- * aligned (0: none).
- * dabsn_hip_linear_slope: dz [rows, n] (row stride ldz; NULL: none) = grad * slope, and dbias [n]
+ * holds the squared ReLU's output h and the factor is 2 sqrt(h). fp32 operands
+ * are multiplied as three bf16 planes each, which hold all bits from 2^-110 up. padA, padB: the
+ * operand's rows end in zeros up to a multiple of 8 columns; padC: C's are to. Row strides of A and
+ * B are below 2^22. Workspace: dabsn_hip_linear_workspace_bytes of the same call (its workspace may
+ * be unset), 16-byte aligned (0: none).
+ * dabsn_hip_linear_slope: dz [rows, n] (row stride ldz; NULL: none) = grad * slope, its rows ending
+ * in zeros up to a multiple of 8 columns where ldz has the room, and dbias [n]
  * (NULL: none) its column sums before the rounding. */
 int dabsn_hip_norm_fwd(int dtype, int wdtype, int layer, int64_t rows, int64_t H, const void* x,
                        int64_t ldx, const void* weight, const void* bias, float eps, void* out,
@@ -799,7 +802,7 @@ int dabsn_hip_norm_bwd(int dtype, int wdtype, int layer, int64_t rows, int64_t H
                        void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 typedef struct dabsn_linear_call {
-  int dtype, transA, transB, act, slope_kind;
+  int dtype, transA, transB, padA, padB, padC, act, slope_kind;
   int64_t M, N, K;
   const void *A, *B, *bias, *slope, *residual;
   int64_t lda, ldb, lds, ldr, ldc, ldk;
@@ -807,7 +810,7 @@ typedef struct dabsn_linear_call {
   size_t workspace_bytes;
 } dabsn_linear_call;
 
-size_t dabsn_hip_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+size_t dabsn_hip_linear_workspace_bytes(const dabsn_linear_call* call);
 int dabsn_hip_linear(const dabsn_linear_call* call, hipStream_t stream);
 size_t dabsn_hip_linear_slope_workspace_bytes(int dtype, int64_t rows, int64_t n);
 int dabsn_hip_linear_slope(int dtype, int64_t rows, int64_t n, const void* grad, int64_t ldg,

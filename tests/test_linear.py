@@ -77,15 +77,18 @@ def test_library_refuses_bad_arguments_before_it_launches():
                 dict(ldb=15), dict(transB=1, ldb=7), dict(transA=1, transB=1, lda=3), dict(ldc=7),
                 dict(transA=1), dict(act=4), dict(act=-1), dict(slope=one, slope_kind=3),
                 dict(slope=one, slope_kind=0), dict(slope=one, slope_kind=1, lds=7),
-                dict(residual=one, ldr=7), dict(keep=one, ldk=7), dict(A=None), dict(B=None),
+                dict(residual=one, ldr=7), dict(keep=one, ldk=7, act=2), dict(keep=one),
+                dict(lda=1 << 22), dict(ldb=1 << 22), dict(A=None), dict(B=None),
                 dict(C=None)):
         assert call(**bad) == -2, bad
     assert lib.dabsn_hip_linear(None, None) == -2
-    need = lib.dabsn_hip_linear_workspace_bytes(1, 256, 2048, 8192)
-    assert need > 0 and lib.dabsn_hip_linear_workspace_bytes(1, 0, 2048, 8192) == 0
-    assert call(dtype=1, M=256, N=2048, K=8192, lda=8192, ldb=8192, ldc=2048, workspace=one,
-                workspace_bytes=need - 1) == -2
-    assert call(dtype=1, M=256, N=2048, K=8192, lda=8192, ldb=8192, ldc=2048) == -2
+    # fp32 operands are split in the workspace.
+    f = dict(dtype=0, M=256, N=2048, K=8192, A=one, B=one, C=one, lda=8192, ldb=8192, ldc=2048)
+    need = lib.dabsn_hip_linear_workspace_bytes(ctypes.byref(_lib.LinearCall(**f)))
+    assert need >= 6 * (256 + 2048) * 8192 and lib.dabsn_hip_linear_workspace_bytes(None) == 0
+    assert lib.dabsn_hip_linear_workspace_bytes(ctypes.byref(_lib.LinearCall(**{**f, "M": 0}))) == 0
+    for ws, n in ((one, need - 1), (None, need), (one + 8, need)):
+        assert call(**f, workspace=ws, workspace_bytes=n) == -2
     for dtype, rows, n, ldg, ws in ((2, 4, 8, 8, 1 << 30), (0, -1, 8, 8, 1 << 30), (0, 4, 0, 8, 1 << 30),
                                     (0, 4, 8, 7, 1 << 30), (0, 4, 8, 8, 0)):
         assert lib.dabsn_hip_linear_slope(dtype, rows, n, one, ldg, None, 0, 0, one, 8, one, one, ws,
