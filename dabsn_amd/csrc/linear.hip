@@ -188,13 +188,13 @@ __device__ __forceinline__ bool tile_of(int L, int nblk, int splits, int mt_n, i
 }
 
 // ---- the products -----------------------------------------------------------------------------
-constexpr int PK = 32, BUFS = 4;
+constexpr int PK = 64;
 constexpr uint32_t NOWHERE = 0x80000000u;  // an offset beyond every buffer resource
 
 // A tile's way into LDS, BT rows (or columns, where transposed) by PK k a step: 16-byte chunks in
-// the order of their positions, K-contiguous rows of 64 bytes (16 lanes read a chunk of 16 rows) or
-// transposed rows of 2 BT bytes (32 lanes read 32 bytes of 8 rows), positions permuted so that
-// such a read touches every bank once.
+// the order of their positions, K-contiguous rows of 128 bytes (eight lanes read a chunk of eight
+// rows at once) or transposed rows of 2 BT bytes (16 lanes read 32 bytes of four rows), positions
+// permuted so that such a read touches each of the 32 banks once.
 template <bool T, int BT, int NTH>
 struct Feed {
   static constexpr int NV = BT * PK * 2 / 16 / NTH;
@@ -202,73 +202,67 @@ struct Feed {
   const bf16* base;  // the tile's first element
   uint32_t bytes;    // from there to the matrix's end
   u32x4 rsrc;
-  uint32_t off[NV], step;
-  int k[NV];
+  uint32_t off0, step, stride;  // of the first chunk, from step to step, from chunk to chunk
+  int k0;                       // the first chunk's k
 
-  __device__ static int turn(int r) {
-    const int f = (r & 3) | ((r >> 1) & 4);
-    return BT >= 128 ? f : f >> 1;
-  }
-  __device__ void init(const bf16* p, int64_t ld, int r0, int rows, int k0, int len, int tid) {
-    base = T ? p + static_cast<int64_t>(k0) * ld + r0 : p + static_cast<int64_t>(r0) * ld + k0;
-    // K-contiguous rows hold zeros up to a whole chunk (and nothing needs the last row's).
+  __device__ static int turn(int r) { return r & 3; }
+  __device__ void init(const bf16* p, int64_t ld, int r0, int rows, int kbase, int len, int tid) {
+    base = T ? p + static_cast<int64_t>(kbase) * ld + r0 : p + static_cast<int64_t>(r0) * ld + kbase;
+    // K-contiguous rows hold zeros up to a whole chunk.
     const int64_t last = T ? static_cast<int64_t>(len - 1) * ld + (rows - r0)
                            : static_cast<int64_t>(min(BT, rows - r0) - 1) * ld + (len + 7) / 8 * 8;
     bytes = static_cast<uint32_t>((last * 2 + 3) & ~3ll);
+    // Chunk i of a thread lies ROWS rows below its chunk i - 1, at the same position.
+    constexpr int CPR = T ? BT / 8 : 8, ROWS = NTH / CPR;
+    static_assert(NTH % CPR == 0 && ROWS % 8 == 0, "a thread's chunks differ by rows alone");
+    const int r = tid / CPR, c = (tid % CPR) ^ (T ? turn(r) << 1 : r & 7);
+    off0 = static_cast<uint32_t>((r * ld + c * 8) * 2);
+    stride = static_cast<uint32_t>(ROWS * ld * 2);
     step = static_cast<uint32_t>(T ? PK * ld * 2 : PK * 2);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int q = tid + i * NTH;
-      const int r = T ? q / (BT / 8) : q / 4;
-      const int c = T ? (q % (BT / 8)) ^ (turn(r) << 1) : (q % 4) ^ ((r >> 2) & 3);
-      off[i] = static_cast<uint32_t>((r * ld + c * 8) * 2);
-      k[i] = T ? r : c * 8;
-    }
+    k0 = T ? r : c * 8;
   }
   __device__ void plane(int64_t at) {
     const uint64_t p = reinterpret_cast<uint64_t>(base + at);
     rsrc = (u32x4){static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xffffu, bytes, 0x00020000u};
   }
-  // The chunks of step t to LDS from byte `lds` on, zeros where k is not below `len`. Written as
+  // Chunk i of step t to LDS from byte `lds` on, zeros where k is not below `len`. Written as
   // assembly, since before a transposing read the compiler would wait for every load under way; the
-  // kernel counts them itself. (They write no register.)
-  __device__ void load(uint32_t lds, int t, int len) const {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t o = t * PK + k[i] < len ? off[i] + t * step : NOWHERE;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
-                       lds + i * NTH * 16),
-                   "v"(o), "s"(rsrc)
-                   : "memory");
-    }
+  // kernel waits for them itself. (They write no register.)
+  __device__ void load(uint32_t lds, int t, int len, int i) const {
+    constexpr int ROWS = NTH / (T ? BT / 8 : 8);
+    const uint32_t o = t * PK + k0 + (T ? i * ROWS : 0) < len ? off0 + t * step + i * stride : NOWHERE;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                     lds + i * NTH * 16),
+                 "v"(o), "s"(rsrc)
+                 : "memory");
   }
 };
 
-// A wave's fragments of a step: tile i of 16 rows from its first row on, eight k a lane. Addresses
-// are bytes of LDS; `at` covers two buffers by the instructions' 16-bit offsets, and is made anew
-// for each step (the compiler would keep one register for every tile and buffer).
+// A wave's fragments: tile i of 16 rows from its first row on, half a step of 32 k, eight k a lane.
+// Addresses are bytes of LDS; `at` is made anew for each half (the compiler would keep a register
+// for every tile and buffer).
 template <bool T, int BT>
 struct Reader {
   uint32_t base;
   __device__ void init(uint32_t lds, int row, int lane) {
     const int li = lane & 15, g = lane >> 4, r = g * 8 + (li >> 2);
-    base = lds + (T ? r * BT * 2 + ((row / 16) ^ Feed<true, BT, 64>::turn(r)) * 32 + (li & 3) * 8
-                    : (row + li) * PK * 2 + (g ^ (li >> 2)) * 16);
+    base = lds + (T ? r * BT * 2 + ((row / 16) ^ Feed<true, BT, 512>::turn(r)) * 32 + (li & 3) * 8
+                    : (row + li) * PK * 2 + (g ^ (li & 7)) * 16);
   }
-  __device__ uint32_t at(int bytes) const {
-    uint32_t p = base + bytes;
+  __device__ uint32_t at(int bytes, int half) const {
+    uint32_t p = (T ? base + half * 32 * BT * 2 : base ^ (half * 64)) + bytes;
     asm volatile("" : "+v"(p));
     return p;
   }
   template <typename V>
   using Lds = __attribute__((address_space(3))) V*;
-  __device__ static bf16x8 get(uint32_t at, int bytes, int i) {
+  __device__ static bf16x8 get(uint32_t at, int i) {
     if constexpr (!T) {
-      return __builtin_bit_cast(bf16x8, *(Lds<const u32x4>)(at + bytes + i * 16 * PK * 2));
+      return __builtin_bit_cast(bf16x8, *(Lds<const u32x4>)(at + i * 16 * PK * 2));
     } else {
       // Two transposing reads, each of four k by 16 columns per 16 lanes. (A wave's rows start at a
       // multiple of its tiles, so adding i to the tile's number is an exclusive or.)
-      const uint32_t p = (at ^ (i * 32)) + bytes;
+      const uint32_t p = at ^ (i * 32);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds<s16x4>)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds<s16x4>)(p + 8 * BT));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -276,13 +270,29 @@ struct Reader {
   }
 };
 
-// Steps of 32 k through four buffers in LDS, filled by loads that go there without registers.
-// During step t a wave issues its share of step t + 3's loads and multiplies step t's fragments,
-// which are in registers already; each fragment of A makes room for step t + 1's as soon as it has
-// been used, those of B have a second set. One barrier a step: before it a wave waits until its
-// loads of step t + 1 have landed (those of t + 2 may be under way) and all reads but step t - 1's
-// have; after it, all of step t + 1 is in LDS, and the buffer that step t + 3 overwrites, t - 1's,
-// was last read in step t - 2.
+// c += a b. Of a wave that has a SIMD's 512 registers to itself, `PIN` keeps the sums in its
+// accumulation registers (left to itself the compiler copies them to and fro). It does not see the
+// waits that these need: settle() stands between other writes or reads of the sums and the products.
+template <bool PIN>
+__device__ __forceinline__ void mma(f32x4& c, bf16x8 a, bf16x8 b) {
+  if constexpr (PIN) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+template <bool PIN>
+__device__ __forceinline__ void settle() {
+  if constexpr (PIN) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Steps of 64 k through two buffers in LDS, filled by loads that go there without registers, and two
+// sets of fragments of 32 k each. A step's first half multiplies its first set while the second is
+// read; its second half multiplies that one while the first set of the next step is read and the
+// loads of the step after it go out, over the buffer just read. One barrier a step, between the
+// halves: before it a wave waits until its own loads of the next step have landed (they had a step's
+// time) and its reads have; after it, all of the next step is in LDS and this one's buffer is free.
 //
 // fp32 operands come as three bf16 planes each (x = hi + mid + lo, 8 bits each, the remainders
 // exact): the steps then go through six products of planes, small ones first; the three left out
@@ -292,9 +302,10 @@ template <typename E, bool TA, bool TB, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nblk) {
   constexpr int NTH = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int PAIRS = sizeof(E) == 4 ? 6 : 1;
+  constexpr bool PIN = TM * TN == 64;
   using FA = Feed<TA, BM, NTH>;
   using FB = Feed<TB, BN, NTH>;
-  __shared__ __attribute__((aligned(16))) bf16 lds[BUFS][(BM + BN) * PK];
+  __shared__ __attribute__((aligned(16))) bf16 lds[2][(BM + BN) * PK];
 
   int sp, mt, nt;
   if (!tile_of(blockIdx.x, nblk, a.splits, a.mt, a.nt, sp, mt, nt)) return;
@@ -317,19 +328,20 @@ __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nb
   constexpr int BUF = (BM + BN) * PK * 2;
   const uint32_t lds0 = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) bf16*)lds[0]));
-  // The loads' place: step `at` of the pair. Those beyond the last step go too, as zeros and
-  // without traffic, so that every step has the same number of them.
+  // The loads' place: step `at` of the pair; steps beyond the last load zeros, without traffic.
   int pair = 0, at = 0;
-  auto planes = [&]() {
+  auto planes = [&]() __attribute__((always_inline)) {
     // (lo hi) (hi lo) (mid mid) (mid hi) (hi mid) (hi hi), the planes hi, mid, lo in this order.
     constexpr uint32_t PA = 0x001102, PB = 0x010120;
     fa.plane(PAIRS > 1 ? static_cast<int64_t>((PA >> (4 * pair)) & 3) * a.planeA : 0);
     fb.plane(PAIRS > 1 ? static_cast<int64_t>((PB >> (4 * pair)) & 3) * a.planeB : 0);
   };
   planes();
-  auto feed = [&](int buf) {
-    fa.load(lds0 + buf * BUF + wave * 1024, at, len);
-    fb.load(lds0 + buf * BUF + BM * PK * 2 + wave * 1024, at, len);
+  auto feed = [&](int buf, int i) __attribute__((always_inline)) {
+    if (i < FA::NV) fa.load(lds0 + buf * BUF + wave * 1024, at, len, i);
+    else fb.load(lds0 + buf * BUF + BM * PK * 2 + wave * 1024, at, len, i - FA::NV);
+  };
+  auto fed = [&]() __attribute__((always_inline)) {
     ++at;
     if (PAIRS > 1 && at == each && pair + 1 < PAIRS) {
       at = 0;
@@ -343,51 +355,63 @@ __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nb
   RB rb;
   ra.init(lds0, wm, lane);
   rb.init(lds0 + BM * PK * 2, wn, lane);
-  constexpr int READS = TM * (TA ? 2 : 1) + TN * (TB ? 2 : 1);
-  bf16x8 fra[TM], frb[2][TN];
-  auto meet = [&]() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" ::"n"(FA::NV + FB::NV),
-                 "n"(READS < 15 ? READS : 15)
-                 : "memory");
+  constexpr int LOADS = FA::NV + FB::NV;
+  bf16x8 fra[2][TM], frb[2][TN];
+  auto meet = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto step = [&](int t, int set) {
-    const int next = (t + 1) % BUFS, bytes = next % 2 * BUF;
-    meet();
-    feed((t + 3) % BUFS);
-    const uint32_t pa = ra.at(next / 2 * 2 * BUF), pb = rb.at(next / 2 * 2 * BUF);
-    __builtin_amdgcn_sched_barrier(0);
+  // Multiplies set `set` and reads the other from buffer `buf`; the loads too, if `go`, LOADS / 4 at
+  // each of the first groups of TN products.
+  auto half = [&](int set, int buf, bool go) __attribute__((always_inline)) {
+    const uint32_t pa = ra.at(buf * BUF, set ^ 1), pb = rb.at(buf * BUF, set ^ 1);
+    constexpr int PER = (TM + TN + TM - 2) / (TM - 1);  // reads a group: all but the last one's
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
       for (int j = 0; j < TN; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frb[set][j], fra[i], acc[i][j], 0, 0, 0);
-      fra[i] = RA::get(pa, bytes, i);
-      if (i < TN) frb[set ^ 1][i] = RB::get(pb, bytes, i);
+        mma<PIN>(acc[i][j], frb[set][j], fra[set][i]);
+#pragma unroll
+      for (int r = i * PER; r < (i + 1) * PER && r < TM + TN; ++r) {
+        if (r < TN) frb[set ^ 1][r] = RB::get(pb, r);
+        else fra[set ^ 1][r - TN] = RA::get(pa, r - TN);
+      }
+      if (go && i < 4)
+#pragma unroll
+        for (int l = i * LOADS / 4; l < (i + 1) * LOADS / 4; ++l) feed(buf ^ 1, l);
       __builtin_amdgcn_sched_barrier(0);
     }
+    if (go) fed();
   };
-  static_assert(TN <= TM, "B's fragments are read beside A's");
-  feed(0);
-  feed(1);
-  meet();  // at most the second step's loads are under way
-  feed(2);
 #pragma unroll
-  for (int j = 0; j < TN; ++j) frb[0][j] = RB::get(rb.base, 0, j);
+  for (int l = 0; l < LOADS; ++l) feed(0, l);
+  fed();
+  meet();
 #pragma unroll
-  for (int i = 0; i < TM; ++i) fra[i] = RA::get(ra.base, 0, i);
-  int t = 0;
-  for (; t + 4 <= steps; t += 4) {
-    step(0, 0);
-    step(1, 1);
-    step(2, 0);
-    step(3, 1);
+  for (int l = 0; l < LOADS; ++l) feed(1, l);
+  fed();
+  {
+    const uint32_t pa = ra.at(0, 0), pb = rb.at(0, 0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) frb[0][j] = RB::get(pb, j);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fra[0][i] = RA::get(pa, i);
   }
-  if (t < steps) step(0, 0);
-  if (t + 1 < steps) step(1, 1);
-  if (t + 2 < steps) step(2, 0);
+  auto step = [&](int buf) __attribute__((always_inline)) {
+    half(0, buf, false);
+    meet();
+    half(1, buf ^ 1, true);
+  };
+  settle<PIN>();
+  int t = 0;
+  for (; t + 2 <= steps; t += 2) {
+    step(0);
+    step(1);
+  }
+  if (t < steps) step(0);
   // No load may land after the workgroup has gone, nor in the epilogue's places.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  settle<PIN>();
   __syncthreads();
 
   // B is the instruction's first operand: a lane holds four consecutive columns of a row. A wave
@@ -578,7 +602,7 @@ static int run(const dabsn_linear_call& c, const Plan& p, hipStream_t s) {
     const int nblk = (int)((tiles + 7) / 8 * 8);
 #define L(TA, TB)                                                                                     \
   if (p.big)                                                                                          \
-    hipLaunchKernelGGL((product_kernel<E, TA, TB, 256, 256, 2, 4>), dim3(nblk), dim3(512), 0, s, a, nblk); \
+    hipLaunchKernelGGL((product_kernel<E, TA, TB, 256, 256, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk); \
   else                                                                                                \
     hipLaunchKernelGGL((product_kernel<E, TA, TB, 128, 128, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk)
     if (c.transA) { L(true, true); }
