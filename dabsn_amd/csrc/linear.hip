@@ -193,48 +193,63 @@ constexpr uint32_t NOWHERE = 0x80000000u;  // an offset beyond every buffer reso
 
 // A tile's way into LDS, BT rows (or columns, where transposed) by PK k a step: 16-byte chunks in
 // the order of their positions, K-contiguous rows of 128 bytes (eight lanes read a chunk of eight
-// rows at once) or transposed rows of 2 BT bytes (16 lanes read 32 bytes of four rows), positions
-// permuted so that such a read touches each of the 32 banks once.
+// rows at once) or transposed rows of 2 BT bytes (32 lanes read 32 bytes of eight rows), positions
+// permuted so that no bank is asked twice (by the counter of conflicts).
 template <bool T, int BT, int NTH>
 struct Feed {
   static constexpr int NV = BT * PK * 2 / 16 / NTH;
-  static_assert(BT * PK * 2 % (16 * NTH) == 0, "loads must divide evenly");
+  static constexpr int CPR = T ? BT / 8 : 8, ROWS = NTH / CPR;
+  static_assert(BT * PK * 2 % (16 * NTH) == 0 && NTH % CPR == 0 && ROWS % 8 == 0,
+                "a thread's chunks lie ROWS rows apart");
+  // Chunk i + 1 of a thread comes from the same columns as chunk i, or from 128 bytes on or back.
+  static constexpr bool SWAP = T && ROWS % 16 == 8 && BT >= 128;
   const bf16* base;  // the tile's first element
   uint32_t bytes;    // from there to the matrix's end
   u32x4 rsrc;
-  uint32_t off0, step, stride;  // of the first chunk, from step to step, from chunk to chunk
-  int k0;                       // the first chunk's k
+  uint32_t off, stride;  // of the first chunk in this step, from chunk to chunk
+  int32_t flip;  // 128 or -128
+  int64_t ld;
+  int k0, len;  // the first chunk's k, of `len`
 
-  __device__ static int turn(int r) { return r & 3; }
-  __device__ void init(const bf16* p, int64_t ld, int r0, int rows, int kbase, int len, int tid) {
+  __host__ __device__ static constexpr int turn(int r) {
+    const int f = (r & 3) | ((r >> 1) & 4);
+    return BT >= 128 ? f : f >> 1;
+  }
+  __device__ void init(const bf16* p, int64_t ld_, int r0, int rows, int kbase, int len_, int tid) {
+    ld = ld_;
+    len = len_;
     base = T ? p + static_cast<int64_t>(kbase) * ld + r0 : p + static_cast<int64_t>(r0) * ld + kbase;
     // K-contiguous rows hold zeros up to a whole chunk.
     const int64_t last = T ? static_cast<int64_t>(len - 1) * ld + (rows - r0)
                            : static_cast<int64_t>(min(BT, rows - r0) - 1) * ld + (len + 7) / 8 * 8;
     bytes = static_cast<uint32_t>((last * 2 + 3) & ~3ll);
-    // Chunk i of a thread lies ROWS rows below its chunk i - 1, at the same position.
-    constexpr int CPR = T ? BT / 8 : 8, ROWS = NTH / CPR;
-    static_assert(NTH % CPR == 0 && ROWS % 8 == 0, "a thread's chunks differ by rows alone");
     const int r = tid / CPR, c = (tid % CPR) ^ (T ? turn(r) << 1 : r & 7);
-    off0 = static_cast<uint32_t>((r * ld + c * 8) * 2);
-    stride = static_cast<uint32_t>(ROWS * ld * 2);
-    step = static_cast<uint32_t>(T ? PK * ld * 2 : PK * 2);
     k0 = T ? r : c * 8;
+    flip = c & 8 ? -128 : 128;
+    off = static_cast<uint32_t>((r * ld + c * 8) * 2);
+    stride = static_cast<uint32_t>(ROWS * ld * 2);
   }
   __device__ void plane(int64_t at) {
     const uint64_t p = reinterpret_cast<uint64_t>(base + at);
     rsrc = (u32x4){static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xffffu, bytes, 0x00020000u};
   }
-  // Chunk i of step t to LDS from byte `lds` on, zeros where k is not below `len`. Written as
-  // assembly, since before a transposing read the compiler would wait for every load under way; the
-  // kernel waits for them itself. (They write no register.)
-  __device__ void load(uint32_t lds, int t, int len, int i) const {
-    constexpr int ROWS = NTH / (T ? BT / 8 : 8);
-    const uint32_t o = t * PK + k0 + (T ? i * ROWS : 0) < len ? off0 + t * step + i * stride : NOWHERE;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
-                     lds + i * NTH * 16),
-                 "v"(o), "s"(rsrc)
-                 : "memory");
+  // Where step t's chunks are. Transposed rows beyond the last k lie beyond the resource; of the
+  // others' chunks those that start beyond it are sent there. Both load zeros.
+  __device__ uint32_t place(int t) const {
+    if constexpr (T) return off + static_cast<uint32_t>(t) * static_cast<uint32_t>(PK * ld * 2);
+    return t * PK + k0 < len ? off + t * PK * 2 : NOWHERE;
+  }
+  // Chunk I of the step at `at` to LDS, I * NTH * 16 bytes from `lds` on. Written as assembly, since
+  // before a transposing read the compiler would wait for every load under way; the kernel waits for
+  // them itself. (They write no register.)
+  template <int I>
+  __device__ void load(uint32_t lds, uint32_t at) const {
+    if constexpr (SWAP && I % 2 == 1) at += flip;
+    uint32_t o;
+    asm volatile("s_add_u32 m0, %1, %2\n\tv_add_u32 %0, %3, %4\n\tbuffer_load_dwordx4 %0, %5, 0 offen lds"
+                 : "=&v"(o)
+                 : "s"(lds), "n"(I * NTH * 16), "s"(I * stride), "v"(at), "s"(rsrc)
+                 : "memory", "scc");
   }
 };
 
@@ -269,6 +284,15 @@ struct Reader {
     }
   }
 };
+
+// f(0), f(1), ... f(N - 1), each with its number as a constant.
+template <int N, typename F>
+__device__ __forceinline__ void each_of(F&& f) {
+  if constexpr (N > 0) {
+    each_of<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
 
 // c += a b. Of a wave that has a SIMD's 512 registers to itself, `PIN` keeps the sums in its
 // accumulation registers (left to itself the compiler copies them to and fro). It does not see the
@@ -337,9 +361,13 @@ __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nb
     fb.plane(PAIRS > 1 ? static_cast<int64_t>((PB >> (4 * pair)) & 3) * a.planeB : 0);
   };
   planes();
-  auto feed = [&](int buf, int i) __attribute__((always_inline)) {
-    if (i < FA::NV) fa.load(lds0 + buf * BUF + wave * 1024, at, len, i);
-    else fb.load(lds0 + buf * BUF + BM * PK * 2 + wave * 1024, at, len, i - FA::NV);
+  uint32_t placeA = fa.place(0), placeB = fb.place(0);
+  constexpr int LOADS = FA::NV + FB::NV;
+  auto feed = [&](auto i, int buf) __attribute__((always_inline)) {
+    constexpr int I = decltype(i)::value;
+    const uint32_t to = lds0 + buf * BUF + wave * 1024;
+    if constexpr (I < FA::NV) fa.template load<I>(to, placeA);
+    else fb.template load<I - FA::NV>(to + BM * PK * 2, placeB);
   };
   auto fed = [&]() __attribute__((always_inline)) {
     ++at;
@@ -348,6 +376,8 @@ __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nb
       ++pair;
       planes();
     }
+    placeA = fa.place(at);
+    placeB = fb.place(at);
   };
   using RA = Reader<TA, BM>;
   using RB = Reader<TB, BN>;
@@ -355,40 +385,42 @@ __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nb
   RB rb;
   ra.init(lds0, wm, lane);
   rb.init(lds0 + BM * PK * 2, wn, lane);
-  constexpr int LOADS = FA::NV + FB::NV;
   bf16x8 fra[2][TM], frb[2][TN];
   auto meet = [&]() __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  // Multiplies set `set` and reads the other from buffer `buf`; the loads too, if `go`, LOADS / 4 at
-  // each of the first groups of TN products.
-  auto half = [&](int set, int buf, bool go) __attribute__((always_inline)) {
-    const uint32_t pa = ra.at(buf * BUF, set ^ 1), pb = rb.at(buf * BUF, set ^ 1);
-    constexpr int PER = (TM + TN + TM - 2) / (TM - 1);  // reads a group: all but the last one's
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-        mma<PIN>(acc[i][j], frb[set][j], fra[set][i]);
-#pragma unroll
-      for (int r = i * PER; r < (i + 1) * PER && r < TM + TN; ++r) {
-        if (r < TN) frb[set ^ 1][r] = RB::get(pb, r);
-        else fra[set ^ 1][r - TN] = RA::get(pa, r - TN);
+  // Multiplies set SET while the other is read from buffer BUFFER and, with GO, the next loads go to
+  // the other buffer. A product takes the matrix unit 16 cycles and the wave 4, so the reads and loads
+  // go between the products, one or two at a place, and the last quarter of the places stays free for
+  // them to land.
+  auto half = [&](auto set, auto buffer, auto go) __attribute__((always_inline)) {
+    constexpr int SET = decltype(set)::value, BUFFER = decltype(buffer)::value;
+    constexpr bool GO = decltype(go)::value;
+    constexpr int ALL = TM * TN, READS = TM + TN, RSTEP = ALL * 3 / 4 / READS, LSTEP = ALL * 3 / 4 / LOADS;
+    static_assert(RSTEP >= 1 && LSTEP >= 1, "places for all");
+    const uint32_t pa = ra.at(BUFFER * BUF, SET ^ 1), pb = rb.at(BUFFER * BUF, SET ^ 1);
+    each_of<ALL>([&](auto place) __attribute__((always_inline)) {
+      constexpr int P = decltype(place)::value, I = P / TN, J = P % TN;
+      mma<PIN>(acc[I][J], frb[SET][J], fra[SET][I]);
+      if constexpr (P % RSTEP == 0 && P / RSTEP < READS) {
+        constexpr int R = P / RSTEP;
+        if constexpr (R < TN) frb[SET ^ 1][R] = RB::get(pb, R);
+        else fra[SET ^ 1][R - TN] = RA::get(pa, R - TN);
       }
-      if (go && i < 4)
-#pragma unroll
-        for (int l = i * LOADS / 4; l < (i + 1) * LOADS / 4; ++l) feed(buf ^ 1, l);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (go) fed();
+      if constexpr (GO && P % LSTEP == LSTEP / 2 && P / LSTEP < LOADS)
+        feed(std::integral_constant<int, P / LSTEP>{}, BUFFER ^ 1);
+      if constexpr (PIN) __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (!PIN) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (GO) fed();
   };
-#pragma unroll
-  for (int l = 0; l < LOADS; ++l) feed(0, l);
+  using N0 = std::integral_constant<int, 0>;
+  using N1 = std::integral_constant<int, 1>;
+  each_of<LOADS>([&](auto i) __attribute__((always_inline)) { feed(i, 0); });
   fed();
   meet();
-#pragma unroll
-  for (int l = 0; l < LOADS; ++l) feed(1, l);
+  each_of<LOADS>([&](auto i) __attribute__((always_inline)) { feed(i, 1); });
   fed();
   {
     const uint32_t pa = ra.at(0, 0), pb = rb.at(0, 0);
@@ -397,18 +429,19 @@ __global__ void __launch_bounds__(WM * WN * 64) product_kernel(Args<E> a, int nb
 #pragma unroll
     for (int i = 0; i < TM; ++i) fra[0][i] = RA::get(pa, i);
   }
-  auto step = [&](int buf) __attribute__((always_inline)) {
-    half(0, buf, false);
+  auto step = [&](auto buffer) __attribute__((always_inline)) {
+    using Next = std::integral_constant<int, decltype(buffer)::value ^ 1>;
+    half(N0{}, buffer, std::false_type{});
     meet();
-    half(1, buf ^ 1, true);
+    half(N1{}, Next{}, std::true_type{});
   };
   settle<PIN>();
   int t = 0;
   for (; t + 2 <= steps; t += 2) {
-    step(0);
-    step(1);
+    step(N0{});
+    step(N1{});
   }
-  if (t < steps) step(0);
+  if (t < steps) step(N0{});
   // No load may land after the workgroup has gone, nor in the epilogue's places.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   settle<PIN>();
