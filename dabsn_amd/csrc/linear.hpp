@@ -1,0 +1,547 @@
+// Matrix products with the work around them in their epilogue, for the block's MLP.
+//
+//   C(m, n) = act(sum_k A(m, k) B(n, k) + bias(n)) * slope(m, n) + residual(m, n)
+//
+// in fp32, rounded once to the type of A and B. An operand is K-contiguous, A[m * lda + k], or
+// stored as its transpose, A[k * lda + m]: the forward needs neither transposed, the gradient of
+// the rows has B = W transposed, that of the weight both. The products are bound by the matrix
+// cores once there are a few hundred rows, by the weight's bytes below.
+#pragma once
+
+#include "common.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace dabsn {
+namespace linear {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// What the epilogue does with the sums: an activation (and then the residual is added), or a factor:
+// a stored slope, or the squared ReLU's output h, whose slope is 2 sqrt(h).
+enum Epi : int { kNone = 0, kRelu2 = 1, kGelu = 2, kSilu = 3, kStored = 4, kFromSquare = 5 };
+
+template <typename E>
+struct Args {
+  int M, N, K;
+  const bf16 *A, *B;  // as they are, or as pack_kernel leaves them
+  int64_t lda, ldb, planeA, planeB;
+  const E* bias;
+  const E* beside;  // the residual or the factor
+  int64_t ldr;
+  E* C;
+  int64_t ldc;
+  int padC;  // rows of C get zeros up to a multiple of 8
+  E* keep;  // act'(z); NULL: not kept
+  int64_t ldk;
+  int mt, nt, splits, kper;
+  float* parts;  // [splits][M][ldp]: the splits' sums, instead of C
+  int64_t ldp;
+};
+
+// act(z) and its derivative. Where they are rounded to bf16, the hardware's exp and reciprocal do
+// (2^-22 and 2^-23 of their values), and erfc(x) = exp(-x^2) erfcx(x) with erfcx as a polynomial in
+// t = 1 / (1 + 0.46 x), a fit of our own for x >= 0 that is within 1.7e-5 of the value up to x = 60
+// (2^-8 is a rounding's): 20 instructions instead of erfcf's 70.
+template <typename E, int EPI>
+__device__ __forceinline__ float activate(float z, float& slope) {
+  constexpr bool low = sizeof(E) == 2;
+  constexpr float LOG2E = 1.44269504088896341f;
+  if constexpr (EPI == kRelu2) {
+    const float r = z < 0.0f ? 0.0f : z;  // a NaN stays
+    slope = 2.0f * r;
+    return r * r;
+  }
+  if constexpr (EPI == kGelu) {
+    float below, bell;  // the normal distribution function and exp(-z^2 / 2)
+    if constexpr (low) {
+      const float x = fabsf(z) * 0.70710678118654752f;
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.46f, x, 1.0f));
+      float q = fmaf(-0.12698957f, t, 0.2432926f);
+      q = fmaf(q, t, 0.12421153f);
+      q = fmaf(q, t, 0.24096189f);
+      q = fmaf(q, t, 0.25897348f);
+      q = fmaf(q, t, 0.25953397f);
+      bell = __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E));
+      const float tail = 0.5f * q * t * bell;
+      below = z > 0.0f ? 1.0f - tail : tail;
+    } else {
+      below = 0.5f * erfcf(z * -0.70710678118654752f);
+      bell = expf(-0.5f * z * z);
+    }
+    slope = fmaf(z * 0.39894228040143268f, bell, below);
+    return z * below;
+  }
+  if constexpr (EPI == kSilu) {
+    float s, rest;
+    if constexpr (low) {
+      s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * z));
+      rest = 1.0f - s;
+    } else {
+      s = 1.0f / (1.0f + expf(-z));
+      rest = 1.0f / (1.0f + expf(z));
+    }
+    slope = fmaf(z * s, rest, s);
+    return z * s;
+  }
+  slope = 1.0f;
+  return z;
+}
+
+// (The hardware's root is off by 2^-23 of itself, which a factor of bf16 values does not see.)
+template <typename E, int EPI>
+__device__ __forceinline__ float factor(float s) {
+  if constexpr (EPI != kFromSquare) return s;
+  return 2.0f * (sizeof(E) == 2 ? __builtin_amdgcn_sqrtf(s) : sqrtf(s));
+}
+
+// Eight columns of a row as they are stored, at any alignment.
+template <typename E>
+struct Eight {
+  static constexpr int W = sizeof(E) * 2;
+  uint32_t w[W];
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w[e]);
+    else return __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(E) == 4) w[i] = __builtin_bit_cast(uint32_t, v[i]);
+      else w[i] = f2bf(v[2 * i]) | (static_cast<uint32_t>(f2bf(v[2 * i + 1])) << 16);
+    }
+  }
+  __device__ __forceinline__ void take(const E* p) { __builtin_memcpy(w, p, sizeof(w)); }
+  __device__ __forceinline__ void put(E* p) const { __builtin_memcpy(p, w, sizeof(w)); }
+};
+
+// The epilogue of the sums v at row m, columns n to n + 7 (a multiple of 8 on), all within the row.
+template <typename E, int EPI>
+__device__ __forceinline__ void finish(const Args<E>& a, int64_t m, int n, float (&v)[8],
+                                       const Eight<E>& bias, const Eight<E>& beside) {
+  if (a.bias) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += bias.get(e);
+  }
+  if constexpr (EPI == kRelu2 || EPI == kGelu || EPI == kSilu) {
+    float slope[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
+    if (a.keep) {
+      Eight<E> keep;
+      keep.set(slope);
+      keep.put(a.keep + m * a.ldk + n);
+    }
+  }
+  if constexpr (EPI == kStored || EPI == kFromSquare) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= factor<E, EPI>(beside.get(e));
+  } else if (a.beside) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += beside.get(e);
+  }
+  Eight<E> out;
+  out.set(v);
+  out.put(a.C + m * a.ldc + n);
+}
+
+// The same for one column, or for the zeros beyond the row's end.
+template <typename E, int EPI>
+__device__ __forceinline__ void finish_one(const Args<E>& a, int64_t m, int n, float v) {
+  E* out = a.C + m * a.ldc + n;
+  if (n >= a.N) {
+    if (a.padC) *out = static_cast<E>(0);
+    return;
+  }
+  float slope;
+  if (a.bias) v += ld(a.bias, n);
+  v = activate<E, EPI>(v, slope);
+  if (a.keep) st(a.keep, m * a.ldk + n, slope);
+  const float beside = a.beside ? ld(a.beside, m * a.ldr + n) : 0.0f;
+  st(out, 0, EPI == kStored || EPI == kFromSquare ? v * factor<E, EPI>(beside) : v + beside);
+}
+
+// The tile and split of workgroup L: consecutive workgroups go round the 8 XCDs, so each XCD gets a
+// contiguous range of the order, patches of 8 x 8 tiles whose operands its L2 holds.
+__device__ __forceinline__ bool tile_of(int L, int nblk, int splits, int mt_n, int nt_n, int& sp,
+                                        int& mt, int& nt) {
+  const int g = (L % 8) * (nblk / 8) + L / 8, per = mt_n * nt_n;
+  if (g >= splits * per) return false;
+  sp = g / per;
+  int r = g % per;
+  const int band = r / (8 * nt_n);
+  r %= 8 * nt_n;
+  const int rows = min(8, mt_n - band * 8);
+  const int pcol = r / (rows * 8);
+  r %= rows * 8;
+  const int cols = min(8, nt_n - pcol * 8);
+  mt = band * 8 + r / cols;
+  nt = pcol * 8 + r % cols;
+  return true;
+}
+
+// ---- the products -----------------------------------------------------------------------------
+constexpr int PK = 64;
+constexpr uint32_t NOWHERE = 0x80000000u;  // an offset beyond every buffer resource
+
+// A tile's way into LDS, BT rows (or columns, where transposed) by PK k a step: 16-byte chunks in
+// the order of their positions, K-contiguous rows of 128 bytes (eight lanes read a chunk of eight
+// rows at once) or transposed rows of 2 BT bytes (32 lanes read 32 bytes of eight rows), positions
+// permuted so that no bank is asked twice (by the counter of conflicts).
+template <bool T, int BT, int NTH>
+struct Feed {
+  static constexpr int NV = BT * PK * 2 / 16 / NTH;
+  static constexpr int CPR = T ? BT / 8 : 8, ROWS = NTH / CPR;
+  static_assert(BT * PK * 2 % (16 * NTH) == 0 && NTH % CPR == 0 && ROWS % 8 == 0,
+                "a thread's chunks lie ROWS rows apart");
+  // Chunk i + 1 of a thread comes from the same columns as chunk i, or from 128 bytes on or back.
+  static constexpr bool SWAP = T && ROWS % 16 == 8 && BT >= 128;
+  const bf16* base;  // the tile's first element
+  uint32_t bytes;    // from there to the matrix's end
+  u32x4 rsrc;
+  uint32_t off, stride;  // of the first chunk in this step, from chunk to chunk
+  int32_t flip;  // 128 or -128
+  int64_t ld;
+  int k0, len;  // the first chunk's k, of `len`
+
+  __host__ __device__ static constexpr int turn(int r) {
+    const int f = (r & 3) | ((r >> 1) & 4);
+    return BT >= 128 ? f : f >> 1;
+  }
+  __device__ void init(const bf16* p, int64_t ld_, int r0, int rows, int kbase, int len_, int tid) {
+    ld = ld_;
+    len = len_;
+    base = T ? p + static_cast<int64_t>(kbase) * ld + r0 : p + static_cast<int64_t>(r0) * ld + kbase;
+    // K-contiguous rows hold zeros up to a whole chunk.
+    const int64_t last = T ? static_cast<int64_t>(len - 1) * ld + (rows - r0)
+                           : static_cast<int64_t>(min(BT, rows - r0) - 1) * ld + (len + 7) / 8 * 8;
+    bytes = static_cast<uint32_t>((last * 2 + 3) & ~3ll);
+    const int r = tid / CPR, c = (tid % CPR) ^ (T ? turn(r) << 1 : r & 7);
+    k0 = T ? r : c * 8;
+    flip = c & 8 ? -128 : 128;
+    off = static_cast<uint32_t>((r * ld + c * 8) * 2);
+    stride = static_cast<uint32_t>(ROWS * ld * 2);
+  }
+  __device__ void plane(int64_t at) {
+    const uint64_t p = reinterpret_cast<uint64_t>(base + at);
+    rsrc = (u32x4){static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xffffu, bytes, 0x00020000u};
+  }
+  // Where step t's chunks are. Transposed rows beyond the last k lie beyond the resource; of the
+  // others' chunks those that start beyond it are sent there. Both load zeros.
+  __device__ uint32_t place(int t) const {
+    if constexpr (T) return off + static_cast<uint32_t>(t) * static_cast<uint32_t>(PK * ld * 2);
+    return t * PK + k0 < len ? off + t * PK * 2 : NOWHERE;
+  }
+  // Chunk I of the step at `at` to LDS, I * NTH * 16 bytes from `lds` on. Written as assembly, since
+  // before a transposing read the compiler would wait for every load under way; the kernel waits for
+  // them itself. (They write no register.)
+  template <int I>
+  __device__ void load(uint32_t lds, uint32_t at) const {
+    if constexpr (SWAP && I % 2 == 1) at += flip;
+    uint32_t o;
+    asm volatile("s_add_u32 m0, %1, %2\n\tv_add_u32 %0, %3, %4\n\tbuffer_load_dwordx4 %0, %5, 0 offen lds"
+                 : "=&v"(o)
+                 : "s"(lds), "n"(I * NTH * 16), "s"(I * stride), "v"(at), "s"(rsrc)
+                 : "memory", "scc");
+  }
+};
+
+// A wave's fragments: tile i of 16 rows from its first row on, half a step of 32 k, eight k a lane.
+// Addresses are bytes of LDS; `at` is made anew for each half (the compiler would keep a register
+// for every tile and buffer).
+template <bool T, int BT>
+struct Reader {
+  uint32_t base;
+  __device__ void init(uint32_t lds, int row, int lane) {
+    const int li = lane & 15, g = lane >> 4, r = g * 8 + (li >> 2);
+    base = lds + (T ? r * BT * 2 + ((row / 16) ^ Feed<true, BT, 512>::turn(r)) * 32 + (li & 3) * 8
+                    : (row + li) * PK * 2 + (g ^ (li & 7)) * 16);
+  }
+  __device__ uint32_t at(int bytes, int half) const {
+    uint32_t p = (T ? base + half * 32 * BT * 2 : base ^ (half * 64)) + bytes;
+    asm volatile("" : "+v"(p));
+    return p;
+  }
+  template <typename V>
+  using Lds = __attribute__((address_space(3))) V*;
+  __device__ static bf16x8 get(uint32_t at, int i) {
+    if constexpr (!T) {
+      return __builtin_bit_cast(bf16x8, *(Lds<const u32x4>)(at + i * 16 * PK * 2));
+    } else {
+      // Two transposing reads, each of four k by 16 columns per 16 lanes. (A wave's rows start at a
+      // multiple of its tiles, so adding i to the tile's number is an exclusive or.)
+      const uint32_t p = at ^ (i * 32);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds<s16x4>)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds<s16x4>)(p + 8 * BT));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// f(0), f(1), ... f(N - 1), each with its number as a constant.
+template <int N, typename F>
+__device__ __forceinline__ void each_of(F&& f) {
+  if constexpr (N > 0) {
+    each_of<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
+// c += a b. Of a wave that has a SIMD's 512 registers to itself, `PIN` keeps the sums in its
+// accumulation registers (left to itself the compiler copies them to and fro). It does not see the
+// waits that these need: settle() stands between other writes or reads of the sums and the products.
+template <bool PIN>
+__device__ __forceinline__ void mma(f32x4& c, bf16x8 a, bf16x8 b) {
+  if constexpr (PIN) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// Lane groups of 16: a's odd ones for b's even ones. (Assembly, as the compiler takes the builtin's
+// second result for its first here; the s_nop is the wait that the instruction needs after others.)
+__device__ __forceinline__ void trade(float (&a)[4], float (&b)[4]) {
+  asm("s_nop 3\n\t"
+      "v_permlane16_swap_b32 %0, %4\n\tv_permlane16_swap_b32 %1, %5\n\t"
+      "v_permlane16_swap_b32 %2, %6\n\tv_permlane16_swap_b32 %3, %7"
+      : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(b[0]), "+v"(b[1]), "+v"(b[2]), "+v"(b[3]));
+}
+template <bool PIN>
+__device__ __forceinline__ void settle() {
+  if constexpr (PIN) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Steps of 64 k through two buffers in LDS, filled by loads that go there without registers, and two
+// sets of fragments of 32 k each. A step's first half multiplies its first set while the second is
+// read; its second half multiplies that one while the first set of the next step is read and the
+// loads of the step after it go out, over the buffer just read. One barrier a step, between the
+// halves: before it a wave waits until its own loads of the next step have landed (they had a step's
+// time) and its reads have; after it, all of the next step is in LDS and this one's buffer is free.
+//
+// fp32 operands come as three bf16 planes each (x = hi + mid + lo, 8 bits each, the remainders
+// exact): the steps then go through six products of planes, small ones first; the three left out
+// are below 2^-24 of the product. At 2.5 PFLOP/s for bf16 against 0.16 for fp32 this is 2.6 times
+// the fp32 instructions' rate.
+template <typename E, int EPI, bool TA, bool TB, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kernel(Args<E> a, int nblk) {
+  constexpr int NTH = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int PAIRS = sizeof(E) == 4 ? 6 : 1;
+  constexpr bool PIN = TM * TN == 64;
+  using FA = Feed<TA, BM, NTH>;
+  using FB = Feed<TB, BN, NTH>;
+  __shared__ __attribute__((aligned(16))) bf16 lds[2][(BM + BN) * PK];
+
+  int sp, mt, nt;
+  if (!tile_of(blockIdx.x, nblk, a.splits, a.mt, a.nt, sp, mt, nt)) return;
+  const int m0 = mt * BM, n0 = nt * BN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const int k0 = sp * a.kper, len = min(a.K - k0, a.kper);
+  const int each = (len + PK - 1) / PK, steps = PAIRS * each;
+
+  FA fa;
+  FB fb;
+  fa.init(a.A, a.lda, m0, a.M, k0, len, tid);
+  fb.init(a.B, a.ldb, n0, a.N, k0, len, tid);
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+  constexpr int BUF = (BM + BN) * PK * 2;
+  const uint32_t lds0 = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) bf16*)lds[0]));
+  // The loads' place: step `at` of the pair; steps beyond the last load zeros, without traffic.
+  int pair = 0, at = 0;
+  auto planes = [&]() __attribute__((always_inline)) {
+    // (lo hi) (hi lo) (mid mid) (mid hi) (hi mid) (hi hi), the planes hi, mid, lo in this order.
+    constexpr uint32_t PA = 0x001102, PB = 0x010120;
+    fa.plane(PAIRS > 1 ? static_cast<int64_t>((PA >> (4 * pair)) & 3) * a.planeA : 0);
+    fb.plane(PAIRS > 1 ? static_cast<int64_t>((PB >> (4 * pair)) & 3) * a.planeB : 0);
+  };
+  planes();
+  uint32_t placeA = fa.place(0), placeB = fb.place(0);
+  constexpr int LOADS = FA::NV + FB::NV;
+  auto feed = [&](auto i, int buf) __attribute__((always_inline)) {
+    constexpr int I = decltype(i)::value;
+    const uint32_t to = lds0 + buf * BUF + wave * 1024;
+    if constexpr (I < FA::NV) fa.template load<I>(to, placeA);
+    else fb.template load<I - FA::NV>(to + BM * PK * 2, placeB);
+  };
+  auto fed = [&]() __attribute__((always_inline)) {
+    ++at;
+    if (PAIRS > 1 && at == each && pair + 1 < PAIRS) {
+      at = 0;
+      ++pair;
+      planes();
+    }
+    placeA = fa.place(at);
+    placeB = fb.place(at);
+  };
+  using RA = Reader<TA, BM>;
+  using RB = Reader<TB, BN>;
+  RA ra;
+  RB rb;
+  ra.init(lds0, wm, lane);
+  rb.init(lds0 + BM * PK * 2, wn, lane);
+  bf16x8 fra[2][TM], frb[2][TN];
+  auto meet = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Multiplies set SET while the other is read from buffer BUFFER and, with GO, the next loads go to
+  // the other buffer. A product takes the matrix unit 16 cycles and the wave 4, so the reads and loads
+  // go between the products, one or two at a place: the reads over three quarters of them, to be back
+  // at the end, the loads over all (8192^3, all three forms: 3% faster than over three quarters).
+  auto half = [&](auto set, auto buffer, auto go) __attribute__((always_inline)) {
+    constexpr int SET = decltype(set)::value, BUFFER = decltype(buffer)::value;
+    constexpr bool GO = decltype(go)::value;
+    constexpr int ALL = TM * TN, READS = TM + TN, RSTEP = ALL * 3 / 4 / READS, LSTEP = ALL / LOADS;
+    static_assert(RSTEP >= 1 && LSTEP >= 1, "places for all");
+    const uint32_t pa = ra.at(BUFFER * BUF, SET ^ 1), pb = rb.at(BUFFER * BUF, SET ^ 1);
+    each_of<ALL>([&](auto place) __attribute__((always_inline)) {
+      constexpr int P = decltype(place)::value, I = P / TN, J = P % TN;
+      mma<PIN>(acc[I][J], frb[SET][J], fra[SET][I]);
+      if constexpr (P % RSTEP == 0 && P / RSTEP < READS) {
+        constexpr int R = P / RSTEP;
+        if constexpr (R < TN) frb[SET ^ 1][R] = RB::get(pb, R);
+        else fra[SET ^ 1][R - TN] = RA::get(pa, R - TN);
+      }
+      if constexpr (GO && P % LSTEP == LSTEP / 2 && P / LSTEP < LOADS)
+        feed(std::integral_constant<int, P / LSTEP>{}, BUFFER ^ 1);
+      if constexpr (PIN) __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (!PIN) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (GO) fed();
+  };
+  using N0 = std::integral_constant<int, 0>;
+  using N1 = std::integral_constant<int, 1>;
+  each_of<LOADS>([&](auto i) __attribute__((always_inline)) { feed(i, 0); });
+  fed();
+  meet();
+  each_of<LOADS>([&](auto i) __attribute__((always_inline)) { feed(i, 1); });
+  fed();
+  {
+    const uint32_t pa = ra.at(0, 0), pb = rb.at(0, 0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) frb[0][j] = RB::get(pb, j);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fra[0][i] = RA::get(pa, i);
+  }
+  auto step = [&](auto buffer) __attribute__((always_inline)) {
+    using Next = std::integral_constant<int, decltype(buffer)::value ^ 1>;
+    half(N0{}, buffer, std::false_type{});
+    meet();
+    half(N1{}, Next{}, std::true_type{});
+  };
+  // The epilogue goes by places of two by two tiles. It loads what it needs ahead of its stores, since
+  // a load waits for the stores before it: the first of its operands (FIRST places) here, the next up to
+  // AHEAD places after the products, into the fragments' registers.
+  constexpr int PLACES = TM * TN / 4, WIDE = sizeof(E) == 2;
+  constexpr int AHEAD = PIN ? (WIDE ? 16 : 8) : PLACES, FIRST = PIN ? (WIDE ? 6 : 3) : WIDE ? 2 : 1;
+  const int li = lane & 15, group = lane >> 4;
+  auto column = [&](int p) __attribute__((always_inline)) {
+    return n0 + wn + (p % (TN / 2) * 2 + group % 2) * 16 + group / 2 * 8;
+  };
+  auto row = [&](int p, int b) __attribute__((always_inline)) {
+    return static_cast<int64_t>(m0 + wm + (p / (TN / 2) * 2 + b) * 16 + li);
+  };
+  Eight<E> bias[TN / 2], beside[AHEAD][2];
+  if (a.bias && !a.parts)
+#pragma unroll
+    for (int q = 0; q < TN / 2; ++q)
+      if (column(q) + 8 <= a.N) bias[q].take(a.bias + column(q));
+  auto fetch = [&](auto place) __attribute__((always_inline)) {
+    constexpr int P = decltype(place)::value;
+    if (!a.beside || a.parts) return;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      if (row(P, b) < a.M && column(P) + 8 <= a.N)
+        beside[P % AHEAD][b].take(a.beside + row(P, b) * a.ldr + column(P));
+  };
+  each_of<FIRST>(fetch);
+  settle<PIN>();
+  int t = 0;
+  for (; t + 2 <= steps; t += 2) {
+    step(N0{});
+    step(N1{});
+  }
+  if (t < steps) step(N0{});
+  // No load may land after the workgroup has gone.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  settle<PIN>();
+  each_of<AHEAD - FIRST>([&](auto i) __attribute__((always_inline)) {
+    fetch(std::integral_constant<int, decltype(i)::value + FIRST>{});
+  });
+  // A row's last columns, if they are fewer than eight, are left in LDS and done afterwards.
+  const int rest = a.N & ~7;
+  const bool ragged = rest < a.N && rest >= n0 && rest < n0 + BN && !a.parts;
+  float* left = reinterpret_cast<float*>(lds) + wave * (BM / WM) * 8;
+  if (ragged) __syncthreads();  // the waves' last reads
+
+  // B is the instruction's first operand: of tile (i, j) lane group g = lane / 16 holds columns 4 g
+  // to 4 g + 3 of row lane % 16. Two exchanges of lane groups among two by two tiles, group 2 h + 1
+  // of one register for group 2 h of the other, give each lane eight columns of a row: 64 bytes
+  // (bf16) of 16 rows an access. (Through LDS instead this took 5 us more a tile of 256 x 256.)
+  each_of<PLACES>([&](auto place) __attribute__((always_inline)) {
+    constexpr int P = decltype(place)::value, I = P / (TN / 2) * 2, J = P % (TN / 2) * 2;
+    float x[2][2][4];  // [tile row][tile column]
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[0][j][r] = acc[I][J + j][r];
+        x[1][j][r] = acc[I + 1][J + j][r];
+      }
+      trade(x[0][j], x[1][j]);
+    }
+    trade(x[0][0], x[0][1]);
+    trade(x[1][0], x[1][1]);
+    const int n = column(P);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int64_t m = row(P, b);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = x[e / 4][b][e % 4];
+      const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+      if (m >= a.M || n >= a.N) continue;
+      if (a.parts) {
+        f32x4* q = reinterpret_cast<f32x4*>(a.parts + (static_cast<int64_t>(sp) * a.M + m) * a.ldp + n);
+        q[0] = lo;
+        q[1] = hi;
+      } else if (ragged && n == rest) {
+        f32x4* q = reinterpret_cast<f32x4*>(left + (I * 16 + b * 16 + li) * 8);
+        q[0] = lo;
+        q[1] = hi;
+      } else {
+        finish<E, EPI>(a, m, n, v, bias[P % (TN / 2)], beside[P % AHEAD][b]);
+      }
+    }
+    if constexpr (P + AHEAD < PLACES) fetch(std::integral_constant<int, P + AHEAD>{});
+    __builtin_amdgcn_sched_barrier(0);
+  });
+  if (ragged && rest >= n0 + wn && rest < n0 + wn + BN / WN) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+    for (int r = lane; r < BM / WM; r += 64)
+      for (int e = 0; e < 8; ++e)
+        if (m0 + wm + r < a.M) finish_one<E, EPI>(a, m0 + wm + r, rest + e, left[r * 8 + e]);
+  }
+}
+
+// Tiles of 256 x 256 by four waves of 128 x 128 (`big`), or of 128 x 128.
+template <typename E, int EPI, bool TA, bool TB>
+void launch(const Args<E>& a, bool big, int nblk, hipStream_t s) {
+  if (big)
+    hipLaunchKernelGGL((product_kernel<E, EPI, TA, TB, 256, 256, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk);
+  else
+    hipLaunchKernelGGL((product_kernel<E, EPI, TA, TB, 128, 128, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk);
+}
+
+}  // namespace linear
+}  // namespace dabsn

@@ -780,7 +780,8 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
  * [rows, H] (NULL: none); dweight and dbias [H] (each NULL: none) = sums over the rows, in fp32
  * and a fixed order. Workspace (for dweight and dbias): dabsn_hip_norm_workspace_bytes.
  *
- * dabsn_hip_linear: C [M, N] = act(A B^T + bias) * slope + residual, fp32 until its one rounding.
+ * dabsn_hip_linear: C [M, N] = act(A B^T + bias) + residual, or with transB (A B^T) * slope, fp32
+ * until its one rounding.
  * A [M, K], row stride lda; B [N, K], or with transB its transpose [K, N]; with transA
  * (and transB) A is stored as [K, M] too; any alignment. act: 0 none, 1 squared ReLU, 2 GELU (by the error function), 3 SiLU. keep [M, N]
  * (row stride ldk; NULL: none) receives the activation's derivative. slope_kind 1: slope [M, N] as it is, 2: slope
