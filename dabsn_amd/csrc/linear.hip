@@ -15,7 +15,10 @@ namespace linear {
   DABSN_LINEAR(E, kRelu2, false, false); \
   DABSN_LINEAR(E, kGelu, false, false); \
   DABSN_LINEAR(E, kSilu, false, false); \
+  DABSN_LINEAR(E, kShare, false, false); \
   DABSN_LINEAR(E, kNone, false, true);  \
+  DABSN_LINEAR(E, kShare, false, true); \
+  DABSN_LINEAR(E, kShare, true, true);  \
   DABSN_LINEAR(E, kStored, false, true); \
   DABSN_LINEAR(E, kFromSquare, false, true); \
   DABSN_LINEAR(E, kNone, true, true)
@@ -70,10 +73,6 @@ __global__ void __launch_bounds__(256) join_kernel(Args<E> a) {
   const int64_t m = i / per;
   const int n = static_cast<int>(i % per) * 8;
   float v[8] = {};
-  Eight<E> bias, beside;
-  const bool whole = n + 8 <= a.N;
-  if (a.bias && whole) bias.take(a.bias + n);
-  if (a.beside && whole) beside.take(a.beside + m * a.ldr + n);
   for (int s = 0; s < a.splits; ++s) {
     const float* p = a.parts + (s * static_cast<int64_t>(a.M) + m) * a.ldp + n;
     const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
@@ -83,12 +82,34 @@ __global__ void __launch_bounds__(256) join_kernel(Args<E> a) {
       v[4 + e] += hi[e];
     }
   }
-  if (whole) {
-    finish<E, EPI>(a, m, n, v, bias, beside);
-  } else {
+  if (n + 8 > a.N) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) finish_one<E, EPI>(a, m, n + e, v[e]);
+    return;
   }
+  Eight<E> x;
+  if (a.bias) {
+    __builtin_memcpy(&x, a.bias + n, sizeof(x));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += x.get(e);
+  }
+  float slope[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
+  if (a.keep) {
+    x.set(slope);
+    __builtin_memcpy(a.keep + m * a.ldk + n, &x, sizeof(x));
+  }
+  if (a.beside) {
+    __builtin_memcpy(&x, a.beside + m * a.ldr + n, sizeof(x));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (EPI == kStored || EPI == kFromSquare) v[e] *= factor<E, EPI>(x.get(e));
+      else v[e] += x.get(e);
+    }
+  }
+  x.set(v);
+  __builtin_memcpy(a.C + m * a.ldc + n, &x, sizeof(x));
 }
 
 // How a product runs.
@@ -191,7 +212,11 @@ static int run(const dabsn_linear_call& c, const Plan& p, hipStream_t s) {
     DABSN_REQUIRE(tiles < (1ll << 31) - 8, "linear: too many tiles");
     const int nblk = (int)((tiles + 7) / 8 * 8);
     // The products the MLP has: activations go with the forward, factors with the rows' gradient.
-    if (c.transA) launch<E, kNone, true, true>(a, p.big, nblk, s);
+    if (a.parts) {
+      if (c.transA) launch<E, kShare, true, true>(a, p.big, nblk, s);
+      else if (c.transB) launch<E, kShare, false, true>(a, p.big, nblk, s);
+      else launch<E, kShare, false, false>(a, p.big, nblk, s);
+    } else if (c.transA) launch<E, kNone, true, true>(a, p.big, nblk, s);
     else if (c.transB) with_factor(c, [&](auto epi) { launch<E, decltype(epi)::value, false, true>(a, p.big, nblk, s); });
     else with_activation(c, [&](auto epi) { launch<E, decltype(epi)::value, false, false>(a, p.big, nblk, s); });
     DABSN_HIP_CHECK(hipGetLastError());
@@ -299,7 +324,7 @@ using namespace dabsn::linear;
 
 static int check_linear(const dabsn_linear_call& c) {
   DABSN_REQUIRE(c.dtype == kF32 || c.dtype == kBF16, "linear: bad dtype %d", c.dtype);
-  const int64_t top = (1ll << 31) - 65536, width = 1 << 22;
+  const int64_t top = (1ll << 31) - 65536, width = 1 << 21;
   DABSN_REQUIRE(c.M >= 0 && c.M < top && c.N > 0 && c.N < top && c.K >= 0 && c.K < top,
                 "linear: bad shape M=%lld N=%lld K=%lld", (long long)c.M, (long long)c.N,
                 (long long)c.K);
@@ -308,9 +333,10 @@ static int check_linear(const dabsn_linear_call& c) {
                     (!c.residual || c.ldr >= c.N) && (!c.slope || c.lds >= c.N) &&
                     (!c.keep || c.ldk >= c.N),
                 "linear: a row stride is shorter than its row");
-  // 256 rows of an operand lie within 32-bit offsets.
-  DABSN_REQUIRE(c.lda < width && c.ldb < width, "linear: operands have rows of at most %lld elements",
-                (long long)width - 1);
+  // 256 rows of any matrix lie within 31-bit offsets.
+  DABSN_REQUIRE(c.lda < width && c.ldb < width && c.ldc < width && (!c.residual || c.ldr < width) &&
+                    (!c.slope || c.lds < width) && (!c.keep || c.ldk < width),
+                "linear: rows of at most %lld elements", (long long)width - 1);
   DABSN_REQUIRE(c.act >= kNone && c.act <= kSilu && !(c.keep && c.act == kNone),
                 "linear: bad activation %d", c.act);
   DABSN_REQUIRE(!c.slope || c.slope_kind == 1 || c.slope_kind == 2, "linear: bad slope kind %d",

@@ -21,7 +21,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // What the epilogue does with the sums: an activation (and then the residual is added), or a factor:
 // a stored slope, or the squared ReLU's output h, whose slope is 2 sqrt(h).
-enum Epi : int { kNone = 0, kRelu2 = 1, kGelu = 2, kSilu = 3, kStored = 4, kFromSquare = 5 };
+// Or it leaves them as a split's share.
+enum Epi : int { kNone = 0, kRelu2 = 1, kGelu = 2, kSilu = 3, kStored = 4, kFromSquare = 5, kShare = 6 };
 
 template <typename E>
 struct Args {
@@ -97,55 +98,59 @@ __device__ __forceinline__ float factor(float s) {
   return 2.0f * (sizeof(E) == 2 ? __builtin_amdgcn_sqrtf(s) : sqrtf(s));
 }
 
-// Eight columns of a row as they are stored, at any alignment.
+// Eight columns of a row as they are stored.
 template <typename E>
 struct Eight {
-  static constexpr int W = sizeof(E) * 2;
-  uint32_t w[W];
+  static constexpr int Q = sizeof(E) / 2;
+  u32x4 q[Q];
   __device__ __forceinline__ float get(int e) const {
-    if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w[e]);
-    else return __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    const uint32_t w = q[sizeof(E) == 4 ? e / 4 : 0][sizeof(E) == 4 ? e % 4 : e / 2];
+    // (A bit cast of the vector's element itself would take its first.)
+    if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w);
+    else return __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
   }
   __device__ __forceinline__ void set(const float (&v)[8]) {
+    if constexpr (sizeof(E) == 4) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      if constexpr (sizeof(E) == 4) w[i] = __builtin_bit_cast(uint32_t, v[i]);
-      else w[i] = f2bf(v[2 * i]) | (static_cast<uint32_t>(f2bf(v[2 * i + 1])) << 16);
+      for (int e = 0; e < 8; ++e) q[e / 4][e % 4] = __builtin_bit_cast(uint32_t, v[e]);
+    } else {
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        q[0][i] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector(((f32x2){v[2 * i], v[2 * i + 1]}), bf16x2));
     }
   }
-  __device__ __forceinline__ void take(const E* p) { __builtin_memcpy(w, p, sizeof(w)); }
-  __device__ __forceinline__ void put(E* p) const { __builtin_memcpy(p, w, sizeof(w)); }
 };
 
-// The epilogue of the sums v at row m, columns n to n + 7 (a multiple of 8 on), all within the row.
-template <typename E, int EPI>
-__device__ __forceinline__ void finish(const Args<E>& a, int64_t m, int n, float (&v)[8],
-                                       const Eight<E>& bias, const Eight<E>& beside) {
-  if (a.bias) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += bias.get(e);
+// A tile's rows of a matrix, for accesses of eight columns at any alignment. The resource ends with the
+// matrix's last row, so rows beyond it are neither read (zeros) nor written; columns beyond their
+// row are sent to NOWHERE. No branch: between branches the compiler would wait for every store.
+constexpr uint32_t NOWHERE = 0x80000000u;  // an offset beyond every buffer resource
+template <typename E>
+struct Rows {
+  __amdgpu_buffer_rsrc_t rsrc;
+  uint32_t at, step;  // of the lane's row in the first 16, from 16 rows to the next
+  __device__ __forceinline__ void init(const E* p, int64_t ld, int m0, int n0, int rows, int cols, int row) {
+    const int64_t size = p ? ((rows - 1) * ld + cols) * static_cast<int64_t>(sizeof(E)) : 0;
+    rsrc = make_rsrc(p + m0 * ld + n0, static_cast<uint32_t>(size));
+    at = static_cast<uint32_t>(row * ld * sizeof(E));
+    step = static_cast<uint32_t>(16 * ld * sizeof(E));
   }
-  if constexpr (EPI == kRelu2 || EPI == kGelu || EPI == kSilu) {
-    float slope[8];
+  __device__ __forceinline__ Eight<E> take(int block, uint32_t column) const {
+    Eight<E> v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
-    if (a.keep) {
-      Eight<E> keep;
-      keep.set(slope);
-      keep.put(a.keep + m * a.ldk + n);
-    }
+    for (int i = 0; i < Eight<E>::Q; ++i)
+      v.q[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + block * step + column + 16 * i, 0, 0);
+    return v;
   }
-  if constexpr (EPI == kStored || EPI == kFromSquare) {
+  __device__ __forceinline__ void put(int block, uint32_t column, const Eight<E>& v) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= factor<E, EPI>(beside.get(e));
-  } else if (a.beside) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += beside.get(e);
+    for (int i = 0; i < Eight<E>::Q; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(v.q[i], rsrc, at + block * step + column + 16 * i, 0, 0);
   }
-  Eight<E> out;
-  out.set(v);
-  out.put(a.C + m * a.ldc + n);
-}
+};
 
 // The same for one column, or for the zeros beyond the row's end.
 template <typename E, int EPI>
@@ -184,7 +189,6 @@ __device__ __forceinline__ bool tile_of(int L, int nblk, int splits, int mt_n, i
 
 // ---- the products -----------------------------------------------------------------------------
 constexpr int PK = 64;
-constexpr uint32_t NOWHERE = 0x80000000u;  // an offset beyond every buffer resource
 
 // A tile's way into LDS, BT rows (or columns, where transposed) by PK k a step: 16-byte chunks in
 // the order of their positions, K-contiguous rows of 128 bytes (eight lanes read a chunk of eight
@@ -297,13 +301,23 @@ __device__ __forceinline__ void mma(f32x4& c, bf16x8 a, bf16x8 b) {
   if constexpr (PIN) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-// Lane groups of 16: a's odd ones for b's even ones. (Assembly, as the compiler takes the builtin's
-// second result for its first here; the s_nop is the wait that the instruction needs after others.)
+// Lane groups of 16: a's odd ones for b's even ones.
 __device__ __forceinline__ void trade(float (&a)[4], float (&b)[4]) {
-  asm("s_nop 3\n\t"
-      "v_permlane16_swap_b32 %0, %4\n\tv_permlane16_swap_b32 %1, %5\n\t"
-      "v_permlane16_swap_b32 %2, %6\n\tv_permlane16_swap_b32 %3, %7"
-      : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(b[0]), "+v"(b[1]), "+v"(b[2]), "+v"(b[3]));
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const auto both = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a[r]),
+                                                       __builtin_bit_cast(uint32_t, b[r]), false, false);
+    const uint32_t first = both[0], second = both[1];
+    a[r] = __builtin_bit_cast(float, first);
+    b[r] = __builtin_bit_cast(float, second);
+  }
+}
+template <bool PIN>
+__device__ __forceinline__ float value(float sum) {
+  if constexpr (!PIN) return sum;
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(sum));  // volatile: behind settle()
+  return v;
 }
 template <bool PIN>
 __device__ __forceinline__ void settle() {
@@ -333,6 +347,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kerne
   using FA = Feed<TA, BM, NTH>;
   using FB = Feed<TB, BN, NTH>;
   __shared__ __attribute__((aligned(16))) bf16 lds[2][(BM + BN) * PK];
+  __shared__ __attribute__((aligned(16))) float bias_lds[BN];
 
   int sp, mt, nt;
   if (!tile_of(blockIdx.x, nblk, a.splits, a.mt, a.nt, sp, mt, nt)) return;
@@ -442,28 +457,30 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kerne
   // a load waits for the stores before it: the first of its operands (FIRST places) here, the next up to
   // AHEAD places after the products, into the fragments' registers.
   constexpr int PLACES = TM * TN / 4, WIDE = sizeof(E) == 2;
-  constexpr int AHEAD = PIN ? (WIDE ? 16 : 8) : PLACES, FIRST = PIN ? (WIDE ? 6 : 3) : WIDE ? 2 : 1;
+  constexpr int AHEAD = PIN ? (WIDE ? 16 : 12) : PLACES, FIRST = PIN ? (WIDE ? 12 : 6) : WIDE ? 2 : 1;
+  constexpr bool FACTOR = EPI == kStored || EPI == kFromSquare, ACTS = EPI == kRelu2 || EPI == kGelu || EPI == kSilu;
   const int li = lane & 15, group = lane >> 4;
-  auto column = [&](int p) __attribute__((always_inline)) {
-    return n0 + wn + (p % (TN / 2) * 2 + group % 2) * 16 + group / 2 * 8;
-  };
-  auto row = [&](int p, int b) __attribute__((always_inline)) {
-    return static_cast<int64_t>(m0 + wm + (p / (TN / 2) * 2 + b) * 16 + li);
-  };
-  Eight<E> bias[TN / 2], beside[AHEAD][2];
-  if (a.bias && !a.parts)
+  const int rows = min(BM, a.M - m0), cols = min(BN, a.N - n0);
+  uint32_t column[TN / 2];  // in bytes from the tile's first
 #pragma unroll
-    for (int q = 0; q < TN / 2; ++q)
-      if (column(q) + 8 <= a.N) bias[q].take(a.bias + column(q));
+  for (int q = 0; q < TN / 2; ++q) {
+    const int c = wn + (q * 2 + group % 2) * 16 + group / 2 * 8;
+    column[q] = c + 8 <= cols ? c * static_cast<uint32_t>(sizeof(E)) : NOWHERE;
+  }
+  Rows<E> out, keep, besides;
+  Eight<E> beside[AHEAD][2];
+  if constexpr (EPI != kShare) {
+    besides.init(a.beside, a.ldr, m0, n0, rows, cols, wm + li);
+    for (int c = tid; c < BN; c += NTH)
+      bias_lds[c] = a.bias && c < cols ? ld(a.bias, n0 + c) : 0.0f;  // seen after the first barrier
+  }
   auto fetch = [&](auto place) __attribute__((always_inline)) {
-    constexpr int P = decltype(place)::value;
-    if (!a.beside || a.parts) return;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-      if (row(P, b) < a.M && column(P) + 8 <= a.N)
-        beside[P % AHEAD][b].take(a.beside + row(P, b) * a.ldr + column(P));
+    constexpr int P = decltype(place)::value, R = P / (TN / 2) * 2;
+    beside[P % AHEAD][0] = besides.take(R, column[P % (TN / 2)]);
+    beside[P % AHEAD][1] = besides.take(R + 1, column[P % (TN / 2)]);
   };
-  each_of<FIRST>(fetch);
+  if constexpr (EPI != kShare)
+    if (a.beside) each_of<FIRST>(fetch);
   settle<PIN>();
   int t = 0;
   for (; t + 2 <= steps; t += 2) {
@@ -474,63 +491,102 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kerne
   // No load may land after the workgroup has gone.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   settle<PIN>();
-  each_of<AHEAD - FIRST>([&](auto i) __attribute__((always_inline)) {
-    fetch(std::integral_constant<int, decltype(i)::value + FIRST>{});
-  });
+  if constexpr (EPI != kShare)
+    if (a.beside)
+      each_of<AHEAD - FIRST>([&](auto i) __attribute__((always_inline)) {
+        fetch(std::integral_constant<int, decltype(i)::value + FIRST>{});
+      });
   // A row's last columns, if they are fewer than eight, are left in LDS and done afterwards.
-  const int rest = a.N & ~7;
-  const bool ragged = rest < a.N && rest >= n0 && rest < n0 + BN && !a.parts;
+  const int rest = cols & ~7;
+  const bool ragged = EPI != kShare && rest < cols;
   float* left = reinterpret_cast<float*>(lds) + wave * (BM / WM) * 8;
-  if (ragged) __syncthreads();  // the waves' last reads
+  Rows<float> share;
+  if constexpr (EPI == kShare) {
+    share.init(a.parts + static_cast<int64_t>(sp) * a.M * a.ldp, a.ldp, m0, n0, rows,
+               static_cast<int>(min<int64_t>(BN, a.ldp - n0)), wm + li);
+  } else {
+    out.init(a.C, a.ldc, m0, n0, rows, cols, wm + li);
+    if constexpr (ACTS) keep.init(a.keep, a.ldk, m0, n0, rows, cols, wm + li);
+    if (ragged) __syncthreads();  // the waves' last reads
+  }
 
   // B is the instruction's first operand: of tile (i, j) lane group g = lane / 16 holds columns 4 g
   // to 4 g + 3 of row lane % 16. Two exchanges of lane groups among two by two tiles, group 2 h + 1
   // of one register for group 2 h of the other, give each lane eight columns of a row: 64 bytes
   // (bf16) of 16 rows an access. (Through LDS instead this took 5 us more a tile of 256 x 256.)
   each_of<PLACES>([&](auto place) __attribute__((always_inline)) {
-    constexpr int P = decltype(place)::value, I = P / (TN / 2) * 2, J = P % (TN / 2) * 2;
+    constexpr int P = decltype(place)::value, I = P / (TN / 2) * 2, Q = P % (TN / 2), J = Q * 2;
     float x[2][2][4];  // [tile row][tile column]
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[0][j][r] = acc[I][J + j][r];
-        x[1][j][r] = acc[I + 1][J + j][r];
+        x[0][j][r] = value<PIN>(acc[I][J + j][r]);
+        x[1][j][r] = value<PIN>(acc[I + 1][J + j][r]);
       }
       trade(x[0][j], x[1][j]);
     }
     trade(x[0][0], x[0][1]);
     trade(x[1][0], x[1][1]);
-    const int n = column(P);
+    const int c = wn + (J + group % 2) * 16 + group / 2 * 8;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int64_t m = row(P, b);
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = x[e / 4][b][e % 4];
-      const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
-      if (m >= a.M || n >= a.N) continue;
-      if (a.parts) {
-        f32x4* q = reinterpret_cast<f32x4*>(a.parts + (static_cast<int64_t>(sp) * a.M + m) * a.ldp + n);
-        q[0] = lo;
-        q[1] = hi;
-      } else if (ragged && n == rest) {
-        f32x4* q = reinterpret_cast<f32x4*>(left + (I * 16 + b * 16 + li) * 8);
-        q[0] = lo;
-        q[1] = hi;
-      } else {
-        finish<E, EPI>(a, m, n, v, bias[P % (TN / 2)], beside[P % AHEAD][b]);
+      if constexpr (EPI == kShare) {
+        Eight<float> all;
+        all.set(v);
+        share.put(I + b, c < static_cast<int>(a.ldp - n0) ? c * 4u : NOWHERE, all);
+        continue;
       }
+      if (ragged) {
+        if (c == rest) {
+          f32x4* q = reinterpret_cast<f32x4*>(left + (I * 16 + b * 16 + li) * 8);
+          q[0] = (f32x4){v[0], v[1], v[2], v[3]};
+          q[1] = (f32x4){v[4], v[5], v[6], v[7]};
+        }
+      }
+      if (a.bias) {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(bias_lds + c);
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(bias_lds + c + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] += lo[e];
+          v[4 + e] += hi[e];
+        }
+      }
+      Eight<E> done;
+      if constexpr (ACTS) {
+        float slope[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
+        if (a.keep) {
+          done.set(slope);
+          keep.put(I + b, column[Q], done);
+        }
+      }
+      if constexpr (FACTOR) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= factor<E, EPI>(beside[P % AHEAD][b].get(e));
+      } else if (a.beside) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += beside[P % AHEAD][b].get(e);
+      }
+      done.set(v);
+      out.put(I + b, column[Q], done);
     }
-    if constexpr (P + AHEAD < PLACES) fetch(std::integral_constant<int, P + AHEAD>{});
+    if constexpr (EPI != kShare && P + AHEAD < PLACES)
+      if (a.beside) fetch(std::integral_constant<int, P + AHEAD>{});
     __builtin_amdgcn_sched_barrier(0);
   });
-  if (ragged && rest >= n0 + wn && rest < n0 + wn + BN / WN) {
+  if (ragged && rest >= wn && rest < wn + BN / WN) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 1
     for (int r = lane; r < BM / WM; r += 64)
+#pragma unroll 1
       for (int e = 0; e < 8; ++e)
-        if (m0 + wm + r < a.M) finish_one<E, EPI>(a, m0 + wm + r, rest + e, left[r * 8 + e]);
+        if (wm + r < rows) finish_one<E, EPI>(a, m0 + wm + r, n0 + rest + e, left[r * 8 + e]);
   }
 }
 

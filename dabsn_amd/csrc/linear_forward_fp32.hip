@@ -7,6 +7,7 @@ namespace linear {
 template void launch<float, kNone, false, false>(const Args<float>&, bool, int, hipStream_t);
 template void launch<float, kRelu2, false, false>(const Args<float>&, bool, int, hipStream_t);
 template void launch<float, kGelu, false, false>(const Args<float>&, bool, int, hipStream_t);
+template void launch<float, kShare, false, false>(const Args<float>&, bool, int, hipStream_t);
 template void launch<float, kSilu, false, false>(const Args<float>&, bool, int, hipStream_t);
 
 }  // namespace linear

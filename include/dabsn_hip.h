@@ -787,8 +787,8 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
  * (row stride ldk; NULL: none) receives the activation's derivative. slope_kind 1: slope [M, N] as it is, 2: slope
  * holds the squared ReLU's output h and the factor is 2 sqrt(h). fp32 operands
  * are multiplied as three bf16 planes each, which hold all bits from 2^-110 up. padA, padB: the
- * operand's rows end in zeros up to a multiple of 8 columns; padC: C's are to. Row strides of A and
- * B are below 2^22. Workspace: dabsn_hip_linear_workspace_bytes of the same call (its workspace may
+ * operand's rows end in zeros up to a multiple of 8 columns; padC: C's are to. Row strides are below
+ * 2^21. Workspace: dabsn_hip_linear_workspace_bytes of the same call (its workspace may
  * be unset), 16-byte aligned (0: none).
  * dabsn_hip_linear_slope: dz [rows, n] (row stride ldz; NULL: none) = grad * slope, its rows ending
  * in zeros up to a multiple of 8 columns where ldz has the room, and dbias [n]

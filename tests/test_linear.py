@@ -78,7 +78,8 @@ def test_library_refuses_bad_arguments_before_it_launches():
                 dict(transA=1), dict(act=4), dict(act=-1), dict(slope=one, slope_kind=3),
                 dict(slope=one, slope_kind=0), dict(slope=one, slope_kind=1, lds=7),
                 dict(residual=one, ldr=7), dict(keep=one, ldk=7, act=2), dict(keep=one),
-                dict(lda=1 << 22), dict(ldb=1 << 22), dict(A=None), dict(B=None),
+                dict(lda=1 << 21), dict(ldb=1 << 21), dict(ldc=1 << 21), dict(transB=1, ldb=8, act=1),
+                dict(transB=1, ldb=8, bias=one), dict(transB=1, ldb=8, residual=one), dict(A=None), dict(B=None),
                 dict(C=None)):
         assert call(**bad) == -2, bad
     assert lib.dabsn_hip_linear(None, None) == -2
