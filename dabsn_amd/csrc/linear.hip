@@ -9,7 +9,7 @@ namespace linear {
 
 // Instantiated in linear_forward_*.hip and linear_gradients_*.hip.
 #define DABSN_LINEAR(E, EPI, TA, TB) \
-  extern template void launch<E, EPI, TA, TB>(const Args<E>&, bool, int, hipStream_t)
+  extern template void launch<E, EPI, TA, TB>(const Args<E>&, int, int, hipStream_t)
 #define DABSN_LINEAR_ALL(E)             \
   DABSN_LINEAR(E, kNone, false, false); \
   DABSN_LINEAR(E, kRelu2, false, false); \
@@ -28,21 +28,35 @@ DABSN_LINEAR_ALL(bf16);
 // An operand [rows][cols] of row stride ld as the products read it: rows of `to` values (a multiple
 // of 8) that end in zeros; fp32 as its planes hi, mid, lo, each [rows][to].
 template <typename E>
-__global__ void __launch_bounds__(256) pack_kernel(int64_t rows, int cols, const E* x, int64_t ld,
-                                                   int to, bf16* out, int64_t plane) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, per = to / 8;
-  if (i >= rows * per) return;
-  const int64_t r = i / per;
-  const int c = static_cast<int>(i % per) * 8;
-  const E* p = x + r * ld + c;
+struct Operand {
+  int64_t rows;
+  int cols, to;
+  const E* x;
+  int64_t ld;
+  bf16* out;
+  __host__ __device__ int64_t chunks() const { return rows * (to / 8); }
+};
+// One operand or both, a thread eight values.
+template <typename E>
+__global__ void __launch_bounds__(256) pack_kernel(Operand<E> p, Operand<E> other) {
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.chunks()) {
+    i -= p.chunks();
+    p = other;
+    if (i >= p.chunks()) return;
+  }
+  const int per = p.to / 8;
+  const int64_t r = i / per, plane = p.rows * p.to;
+  const int c = static_cast<int>(i - r * per) * 8;
+  const E* at = p.x + r * p.ld + c;
   E v[8];
-  if (c + 8 <= cols) {
-    __builtin_memcpy(v, p, sizeof(v));
+  if (c + 8 <= p.cols) {
+    __builtin_memcpy(v, at, sizeof(v));
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? p[e] : static_cast<E>(0);
+    for (int e = 0; e < 8; ++e) v[e] = c + e < p.cols ? at[e] : static_cast<E>(0);
   }
-  bf16* o = out + r * to + c;
+  bf16* o = p.out + r * p.to + c;
   if constexpr (sizeof(E) == 2) {
     __builtin_memcpy(o, v, 16);
   } else {
@@ -116,7 +130,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args<E> a) {
 struct Plan {
   bool packA, packB;
   int64_t lda, ldb, planeA, planeB;  // of the operands the kernel reads
-  bool big;                          // tiles of 256 x 256, else 128 x 128
+  int tile;
   int mt, nt, splits, kper;
   int64_t ldp;
   size_t atB, atParts, bytes;  // places in the workspace, which starts with A
@@ -143,35 +157,43 @@ static Plan plan_of(const dabsn_linear_call& c) {
   p.atB = at;
   at += p.packB ? up16(static_cast<size_t>(p.planeB) * (f32 ? 6 : 2)) : 0;
   p.atParts = at;
-  const int64_t big = ((c.M + 255) / 256) * ((c.N + 255) / 256);
-  p.big = big >= 192;
-  const int64_t edge = p.big ? 256 : 128;
-  p.mt = static_cast<int>((c.M + edge - 1) / edge);
-  p.nt = static_cast<int>((c.N + edge - 1) / edge);
-  const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt, steps = (c.K + PK - 1) / PK;
-  const int64_t room = p.big ? 256 : 512;
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({room / tiles, steps * (f32 ? 6 : 1) / 16, 64}));
+  // The tile and the splits of K by what they take, in us as measured (8192^3 in tiles of 256 x 256:
+  // 1.41 a step of all units; 128 x 128: 0.55 a step with a tile a unit, 0.9 with two; deep ones by
+  // their operands' way from L2, 100 KB/us a unit, or 0.2 a step; joining splits 6 and their bytes).
+  const int64_t steps = (c.K + PK - 1) / PK, times = f32 ? 6 : 1;
   // Offsets of a transposed operand's rows are 32 bits.
   const int64_t ld = std::max<int64_t>(c.transA ? p.lda : 0, c.transB ? p.ldb : 0);
-  if (ld) splits = std::max<int64_t>(splits, (c.K * ld * 2 + (1ll << 30) - 1) >> 30);
-  const int64_t each = std::max<int64_t>(1, (steps + splits - 1) / splits);
-  p.splits = static_cast<int>(std::max<int64_t>(1, (steps + each - 1) / each));
-  p.kper = static_cast<int>(each * PK);
+  const int64_t least = std::max<int64_t>(1, (c.K * ld * 2 + (1ll << 30) - 1) >> 30);
   p.ldp = (c.N + 7) / 8 * 8;
+  double best = 0;
+  for (int tile = kBig; tile <= (f32 || c.transB ? kMiddle : kDeepLow); ++tile) {
+    const TileOf size = tile_size(tile);
+    const int64_t mt = (c.M + size.m - 1) / size.m, nt = (c.N + size.n - 1) / size.n;
+    for (int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      const int64_t splits = std::max(want, least);
+      if (want > 1 && (want > steps || want < least)) continue;
+      const int64_t each = std::max<int64_t>(1, (steps + splits - 1) / splits);
+      const int64_t real = std::max<int64_t>(1, (steps + each - 1) / each), wgs = mt * nt * real;
+      const int64_t rounds = (wgs + 255) / 256;
+      double us = 0;
+      if (tile == kBig) us = rounds * (each * times * 1.41 + 7);
+      else if (tile == kMiddle)
+        us = (wgs <= 256 ? each * times * 0.55 : (rounds + 1) / 2 * (each * times * 0.9)) + 4;
+      else us = rounds * (each * std::max(0.2, (size.m + size.n) * PK * 2 / 100e3) + 4);
+      if (real > 1) us += 6 + (8.0 * real * c.M * p.ldp) / 7e6;
+      if (best == 0 || us < best) {
+        best = us;
+        p.tile = tile;
+        p.mt = static_cast<int>(mt);
+        p.nt = static_cast<int>(nt);
+        p.splits = static_cast<int>(real);
+        p.kper = static_cast<int>(each * PK);
+      }
+    }
+  }
   if (p.splits > 1) at += static_cast<size_t>(p.splits) * c.M * p.ldp * sizeof(float);
   p.bytes = at;
   return p;
-}
-
-template <typename E>
-static int pack(int64_t rows, int64_t cols, const void* x, int64_t ld, int64_t to, bf16* out,
-                hipStream_t s) {
-  const int64_t blocks = (rows * (to / 8) + 255) / 256;
-  DABSN_REQUIRE(blocks < (1ll << 31), "linear: an operand of too many elements");
-  hipLaunchKernelGGL(pack_kernel<E>, dim3((unsigned)blocks), dim3(256), 0, s, rows, (int)cols,
-                     (const E*)x, ld, (int)to, out, rows * to);
-  DABSN_HIP_CHECK(hipGetLastError());
-  return DABSN_OK;
 }
 
 template <typename F>
@@ -203,22 +225,28 @@ static int run(const dabsn_linear_call& c, const Plan& p, hipStream_t s) {
   a.mt = p.mt; a.nt = p.nt; a.splits = c.K ? p.splits : 0; a.kper = p.kper; a.ldp = p.ldp;
   a.parts = p.splits > 1 ? (float*)(ws + p.atParts) : nullptr;
   if (c.K) {
-    int rc = DABSN_OK;
-    if (p.packA) rc = pack<E>(c.transA ? c.K : c.M, c.transA ? c.M : c.K, c.A, c.lda, p.lda, (bf16*)ws, s);
-    if (rc == DABSN_OK && p.packB)
-      rc = pack<E>(c.transB ? c.K : c.N, c.transB ? c.N : c.K, c.B, c.ldb, p.ldb, (bf16*)(ws + p.atB), s);
-    if (rc != DABSN_OK) return rc;
+    Operand<E> pa = {}, pb = {};
+    if (p.packA)
+      pa = {c.transA ? c.K : c.M, (int)(c.transA ? c.M : c.K), (int)p.lda, (const E*)c.A, c.lda, (bf16*)ws};
+    if (p.packB)
+      pb = {c.transB ? c.K : c.N, (int)(c.transB ? c.N : c.K), (int)p.ldb, (const E*)c.B, c.ldb,
+            (bf16*)(ws + p.atB)};
+    const int64_t blocks = (pa.chunks() + pb.chunks() + 255) / 256;
+    DABSN_REQUIRE(blocks < (1ll << 31), "linear: operands of too many elements");
+    if (blocks)
+      hipLaunchKernelGGL(pack_kernel<E>, dim3((unsigned)blocks), dim3(256), 0, s, pa, pb);
+    DABSN_HIP_CHECK(hipGetLastError());
     const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt * p.splits;
     DABSN_REQUIRE(tiles < (1ll << 31) - 8, "linear: too many tiles");
     const int nblk = (int)((tiles + 7) / 8 * 8);
     // The products the MLP has: activations go with the forward, factors with the rows' gradient.
     if (a.parts) {
-      if (c.transA) launch<E, kShare, true, true>(a, p.big, nblk, s);
-      else if (c.transB) launch<E, kShare, false, true>(a, p.big, nblk, s);
-      else launch<E, kShare, false, false>(a, p.big, nblk, s);
-    } else if (c.transA) launch<E, kNone, true, true>(a, p.big, nblk, s);
-    else if (c.transB) with_factor(c, [&](auto epi) { launch<E, decltype(epi)::value, false, true>(a, p.big, nblk, s); });
-    else with_activation(c, [&](auto epi) { launch<E, decltype(epi)::value, false, false>(a, p.big, nblk, s); });
+      if (c.transA) launch<E, kShare, true, true>(a, p.tile, nblk, s);
+      else if (c.transB) launch<E, kShare, false, true>(a, p.tile, nblk, s);
+      else launch<E, kShare, false, false>(a, p.tile, nblk, s);
+    } else if (c.transA) launch<E, kNone, true, true>(a, p.tile, nblk, s);
+    else if (c.transB) with_factor(c, [&](auto epi) { launch<E, decltype(epi)::value, false, true>(a, p.tile, nblk, s); });
+    else with_activation(c, [&](auto epi) { launch<E, decltype(epi)::value, false, false>(a, p.tile, nblk, s); });
     DABSN_HIP_CHECK(hipGetLastError());
   }
   if (a.parts || !c.K) {

@@ -328,25 +328,171 @@ __device__ __forceinline__ void settle() {
   }
 }
 
-// Steps of 64 k through two buffers in LDS, filled by loads that go there without registers, and two
+// The epilogue of a wave's TM x TN tiles of 16 x 16 sums. It goes by places of two by two tiles, whose
+// operands it loads ahead of all its stores, since a load waits for the stores before it: those of
+// FIRST places before the products, those of the next up to AHEAD places after them, into registers that
+// held fragments.
+template <typename E, int EPI, int TM, int TN, int BM, int BN, int NTH, bool PIN>
+struct Epilogue {
+  static constexpr int PLACES = TM * TN / 4;
+  static constexpr bool WIDE = sizeof(E) == 2;
+  static constexpr int AHEAD = PIN ? (WIDE ? 16 : 12) : PLACES;
+  static constexpr int FIRST = std::min(PLACES, PIN ? (WIDE ? 12 : 6) : WIDE ? 2 : 1);
+  static constexpr bool FACTOR = EPI == kStored || EPI == kFromSquare;
+  static constexpr bool ACTS = EPI == kRelu2 || EPI == kGelu || EPI == kSilu;
+  const Args<E>& a;
+  const int sp, m0, n0, wm, wn, lane;  // the split, the tile's first element, the wave's in it
+  const int rows, cols;                // of the tile within the matrix
+  uint32_t column[TN / 2];             // in bytes from the tile's first
+  Rows<E> besides;
+  Eight<E> beside[AHEAD][2];
+
+  __device__ __forceinline__ Epilogue(const Args<E>& args, int sp_, int m0_, int n0_, int wm_, int wn_, int tid)
+      : a(args), sp(sp_), m0(m0_), n0(n0_), wm(wm_), wn(wn_), lane(tid & 63),
+        rows(min(BM, args.M - m0_)), cols(min(BN, args.N - n0_)) {}
+
+  template <int P>
+  __device__ __forceinline__ void fetch() {
+    constexpr int R = P / (TN / 2) * 2;
+    beside[P % AHEAD][0] = besides.take(R, column[P % (TN / 2)]);
+    beside[P % AHEAD][1] = besides.take(R + 1, column[P % (TN / 2)]);
+  }
+  // Before the products; `bias_lds` [BN] is seen after the next barrier.
+  __device__ __forceinline__ void begin(float* bias_lds, int tid) {
+    const int li = lane & 15, group = lane >> 4;
+#pragma unroll
+    for (int q = 0; q < TN / 2; ++q) {
+      const int c = wn + (q * 2 + group % 2) * 16 + group / 2 * 8;
+      column[q] = c + 8 <= cols ? c * static_cast<uint32_t>(sizeof(E)) : NOWHERE;
+    }
+    if constexpr (EPI != kShare) {
+      besides.init(a.beside, a.ldr, m0, n0, rows, cols, wm + li);
+      for (int c = tid; c < BN; c += NTH) bias_lds[c] = a.bias && c < cols ? ld(a.bias, n0 + c) : 0.0f;
+      if (a.beside)
+        each_of<FIRST>([&](auto i) __attribute__((always_inline)) { fetch<decltype(i)::value>(); });
+    }
+  }
+  // After them; no wave may still read the fragments' LDS, which `left` takes (8 floats a row).
+  __device__ __forceinline__ void end(f32x4 (&acc)[TM][TN], const float* bias_lds, float* left) {
+    const int li = lane & 15, group = lane >> 4;
+    if constexpr (EPI != kShare)
+      if (a.beside)
+        each_of<AHEAD - FIRST>(
+            [&](auto i) __attribute__((always_inline)) { fetch<decltype(i)::value + FIRST>(); });
+    // A row's last columns, if they are fewer than eight, are left in LDS and done afterwards.
+    const int rest = cols & ~7;
+    const bool ragged = EPI != kShare && rest < cols;
+    if (ragged) __syncthreads();
+    Rows<E> out, keep;
+    Rows<float> share;
+    if constexpr (EPI == kShare) {
+      share.init(a.parts + static_cast<int64_t>(sp) * a.M * a.ldp, a.ldp, m0, n0, rows,
+                 static_cast<int>(min<int64_t>(BN, a.ldp - n0)), wm + li);
+    } else {
+      out.init(a.C, a.ldc, m0, n0, rows, cols, wm + li);
+      if constexpr (ACTS) keep.init(a.keep, a.ldk, m0, n0, rows, cols, wm + li);
+    }
+
+    // B is the instruction's first operand: of tile (i, j) lane group g = lane / 16 holds columns 4 g
+    // to 4 g + 3 of row lane % 16. Two exchanges of lane groups among two by two tiles, group 2 h + 1
+    // of one register for group 2 h of the other, give each lane eight columns of a row: 64 bytes
+    // (bf16) of 16 rows an access. (Through LDS instead this took 5 us more a tile of 256 x 256.)
+    each_of<PLACES>([&](auto place) __attribute__((always_inline)) {
+      constexpr int P = decltype(place)::value, I = P / (TN / 2) * 2, Q = P % (TN / 2), J = Q * 2;
+      float x[2][2][4];  // [tile row][tile column]
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[0][j][r] = value<PIN>(acc[I][J + j][r]);
+          x[1][j][r] = value<PIN>(acc[I + 1][J + j][r]);
+        }
+        trade(x[0][j], x[1][j]);
+      }
+      trade(x[0][0], x[0][1]);
+      trade(x[1][0], x[1][1]);
+      const int c = wn + (J + group % 2) * 16 + group / 2 * 8;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = x[e / 4][b][e % 4];
+        if constexpr (EPI == kShare) {
+          Eight<float> all;
+          all.set(v);
+          share.put(I + b, c < static_cast<int>(a.ldp - n0) ? c * 4u : NOWHERE, all);
+          continue;
+        }
+        if (ragged) {
+          if (c == rest) {
+            f32x4* q = reinterpret_cast<f32x4*>(left + (I * 16 + b * 16 + li) * 8);
+            q[0] = (f32x4){v[0], v[1], v[2], v[3]};
+            q[1] = (f32x4){v[4], v[5], v[6], v[7]};
+          }
+        }
+        if (a.bias) {
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(bias_lds + c);
+          const f32x4 hi = *reinterpret_cast<const f32x4*>(bias_lds + c + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] += lo[e];
+            v[4 + e] += hi[e];
+          }
+        }
+        Eight<E> done;
+        if constexpr (ACTS) {
+          float slope[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
+          if (a.keep) {
+            done.set(slope);
+            keep.put(I + b, column[Q], done);
+          }
+        }
+        if constexpr (FACTOR) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= factor<E, EPI>(beside[P % AHEAD][b].get(e));
+        } else if (a.beside) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += beside[P % AHEAD][b].get(e);
+        }
+        done.set(v);
+        out.put(I + b, column[Q], done);
+      }
+      if constexpr (EPI != kShare && P + AHEAD < PLACES)
+        if (a.beside) fetch<P + AHEAD>();
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    if (ragged && rest >= wn && rest < wn + TN * 16) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+      for (int r = lane; r < TM * 16; r += 64)
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e)
+          if (wm + r < rows) finish_one<E, EPI>(a, m0 + wm + r, n0 + rest + e, left[r * 8 + e]);
+    }
+  }
+};
+
+// Steps of 64 k through BUFS buffers in LDS, filled by loads that go there without registers, and two
 // sets of fragments of 32 k each. A step's first half multiplies its first set while the second is
 // read; its second half multiplies that one while the first set of the next step is read and the
-// loads of the step after it go out, over the buffer just read. One barrier a step, between the
-// halves: before it a wave waits until its own loads of the next step have landed (they had a step's
+// loads of step t + BUFS go out, over the buffer just read. One barrier a step, between the halves:
+// before it a wave waits until its own loads of the next step have landed (they had BUFS - 1 steps'
 // time) and its reads have; after it, all of the next step is in LDS and this one's buffer is free.
 //
 // fp32 operands come as three bf16 planes each (x = hi + mid + lo, 8 bits each, the remainders
 // exact): the steps then go through six products of planes, small ones first; the three left out
 // are below 2^-24 of the product. At 2.5 PFLOP/s for bf16 against 0.16 for fp32 this is 2.6 times
 // the fp32 instructions' rate.
-template <typename E, int EPI, bool TA, bool TB, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kernel(Args<E> a, int nblk) {
+template <typename E, int EPI, bool TA, bool TB, int BM, int BN, int WM, int WN, int BUFS>
+__global__ void __launch_bounds__(WM * WN * 64, BM * BN == 128 * 128 ? 2 : 1) product_kernel(Args<E> a, int nblk) {
   constexpr int NTH = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int PAIRS = sizeof(E) == 4 ? 6 : 1;
   constexpr bool PIN = TM * TN == 64;
   using FA = Feed<TA, BM, NTH>;
   using FB = Feed<TB, BN, NTH>;
-  __shared__ __attribute__((aligned(16))) bf16 lds[2][(BM + BN) * PK];
+  __shared__ __attribute__((aligned(16))) bf16 lds[BUFS][(BM + BN) * PK];
   __shared__ __attribute__((aligned(16))) float bias_lds[BN];
 
   int sp, mt, nt;
@@ -404,19 +550,21 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kerne
   ra.init(lds0, wm, lane);
   rb.init(lds0 + BM * PK * 2, wn, lane);
   bf16x8 fra[2][TM], frb[2][TN];
-  auto meet = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // All but the loads of the last LATER steps have landed, and all reads.
+  auto meet = [&](auto later) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(later)::value * LOADS) : "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  // Multiplies set SET while the other is read from buffer BUFFER and, with GO, the next loads go to
-  // the other buffer. A product takes the matrix unit 16 cycles and the wave 4, so the reads and loads
+  static_assert((BUFS - 1) * LOADS < 64, "the counter of loads has six bits");
+  // Multiplies set SET while the other is read from buffer BUFFER and, with TO >= 0, the next loads go to
+  // buffer TO. A product takes the matrix unit 16 cycles and the wave 4, so the reads and loads
   // go between the products, one or two at a place: the reads over three quarters of them, to be back
   // at the end, the loads over all (8192^3, all three forms: 3% faster than over three quarters).
-  auto half = [&](auto set, auto buffer, auto go) __attribute__((always_inline)) {
-    constexpr int SET = decltype(set)::value, BUFFER = decltype(buffer)::value;
-    constexpr bool GO = decltype(go)::value;
-    constexpr int ALL = TM * TN, READS = TM + TN, RSTEP = ALL * 3 / 4 / READS, LSTEP = ALL / LOADS;
-    static_assert(RSTEP >= 1 && LSTEP >= 1, "places for all");
+  auto half = [&](auto set, auto buffer, auto target) __attribute__((always_inline)) {
+    constexpr int SET = decltype(set)::value, BUFFER = decltype(buffer)::value, TO = decltype(target)::value;
+    constexpr int ALL = TM * TN, READS = TM + TN;
+    constexpr int RSTEP = std::max(1, ALL * 3 / 4 / READS), LSTEP = std::max(1, ALL / LOADS);
+    static_assert(READS <= ALL && LOADS <= ALL, "places for all");
     const uint32_t pa = ra.at(BUFFER * BUF, SET ^ 1), pb = rb.at(BUFFER * BUF, SET ^ 1);
     each_of<ALL>([&](auto place) __attribute__((always_inline)) {
       constexpr int P = decltype(place)::value, I = P / TN, J = P % TN;
@@ -426,20 +574,22 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kerne
         if constexpr (R < TN) frb[SET ^ 1][R] = RB::get(pb, R);
         else fra[SET ^ 1][R - TN] = RA::get(pa, R - TN);
       }
-      if constexpr (GO && P % LSTEP == LSTEP / 2 && P / LSTEP < LOADS)
-        feed(std::integral_constant<int, P / LSTEP>{}, BUFFER ^ 1);
+      if constexpr (TO >= 0 && P % LSTEP == LSTEP / 2 && P / LSTEP < LOADS)
+        feed(std::integral_constant<int, P / LSTEP>{}, TO);
       if constexpr (PIN) __builtin_amdgcn_sched_barrier(0);
     });
     if constexpr (!PIN) __builtin_amdgcn_sched_barrier(0);
-    if constexpr (GO) fed();
+    if constexpr (TO >= 0) fed();
   };
   using N0 = std::integral_constant<int, 0>;
   using N1 = std::integral_constant<int, 1>;
-  each_of<LOADS>([&](auto i) __attribute__((always_inline)) { feed(i, 0); });
-  fed();
-  meet();
-  each_of<LOADS>([&](auto i) __attribute__((always_inline)) { feed(i, 1); });
-  fed();
+  Epilogue<E, EPI, TM, TN, BM, BN, NTH, PIN> epilogue(a, sp, m0, n0, wm, wn, tid);
+  epilogue.begin(bias_lds, tid);
+  each_of<BUFS>([&](auto buf) __attribute__((always_inline)) {
+    each_of<LOADS>([&](auto i) __attribute__((always_inline)) { feed(i, decltype(buf)::value); });
+    fed();
+  });
+  meet(std::integral_constant<int, BUFS - 1>{});
   {
     const uint32_t pa = ra.at(0, 0), pb = rb.at(0, 0);
 #pragma unroll
@@ -448,155 +598,45 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 ? 1 : 2) product_kerne
     for (int i = 0; i < TM; ++i) fra[0][i] = RA::get(pa, i);
   }
   auto step = [&](auto buffer) __attribute__((always_inline)) {
-    using Next = std::integral_constant<int, decltype(buffer)::value ^ 1>;
-    half(N0{}, buffer, std::false_type{});
-    meet();
-    half(N1{}, Next{}, std::true_type{});
+    using Next = std::integral_constant<int, (decltype(buffer)::value + 1) % BUFS>;
+    half(N0{}, buffer, std::integral_constant<int, -1>{});
+    meet(std::integral_constant<int, BUFS - 2>{});
+    half(N1{}, Next{}, buffer);
   };
-  // The epilogue goes by places of two by two tiles. It loads what it needs ahead of its stores, since
-  // a load waits for the stores before it: the first of its operands (FIRST places) here, the next up to
-  // AHEAD places after the products, into the fragments' registers.
-  constexpr int PLACES = TM * TN / 4, WIDE = sizeof(E) == 2;
-  constexpr int AHEAD = PIN ? (WIDE ? 16 : 12) : PLACES, FIRST = PIN ? (WIDE ? 12 : 6) : WIDE ? 2 : 1;
-  constexpr bool FACTOR = EPI == kStored || EPI == kFromSquare, ACTS = EPI == kRelu2 || EPI == kGelu || EPI == kSilu;
-  const int li = lane & 15, group = lane >> 4;
-  const int rows = min(BM, a.M - m0), cols = min(BN, a.N - n0);
-  uint32_t column[TN / 2];  // in bytes from the tile's first
-#pragma unroll
-  for (int q = 0; q < TN / 2; ++q) {
-    const int c = wn + (q * 2 + group % 2) * 16 + group / 2 * 8;
-    column[q] = c + 8 <= cols ? c * static_cast<uint32_t>(sizeof(E)) : NOWHERE;
-  }
-  Rows<E> out, keep, besides;
-  Eight<E> beside[AHEAD][2];
-  if constexpr (EPI != kShare) {
-    besides.init(a.beside, a.ldr, m0, n0, rows, cols, wm + li);
-    for (int c = tid; c < BN; c += NTH)
-      bias_lds[c] = a.bias && c < cols ? ld(a.bias, n0 + c) : 0.0f;  // seen after the first barrier
-  }
-  auto fetch = [&](auto place) __attribute__((always_inline)) {
-    constexpr int P = decltype(place)::value, R = P / (TN / 2) * 2;
-    beside[P % AHEAD][0] = besides.take(R, column[P % (TN / 2)]);
-    beside[P % AHEAD][1] = besides.take(R + 1, column[P % (TN / 2)]);
-  };
-  if constexpr (EPI != kShare)
-    if (a.beside) each_of<FIRST>(fetch);
   settle<PIN>();
   int t = 0;
-  for (; t + 2 <= steps; t += 2) {
-    step(N0{});
-    step(N1{});
-  }
-  if (t < steps) step(N0{});
+  for (; t + BUFS <= steps; t += BUFS) each_of<BUFS>(step);
+  each_of<BUFS - 1>([&](auto buffer) __attribute__((always_inline)) {
+    if (t + decltype(buffer)::value < steps) step(buffer);
+  });
   // No load may land after the workgroup has gone.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   settle<PIN>();
-  if constexpr (EPI != kShare)
-    if (a.beside)
-      each_of<AHEAD - FIRST>([&](auto i) __attribute__((always_inline)) {
-        fetch(std::integral_constant<int, decltype(i)::value + FIRST>{});
-      });
-  // A row's last columns, if they are fewer than eight, are left in LDS and done afterwards.
-  const int rest = cols & ~7;
-  const bool ragged = EPI != kShare && rest < cols;
-  float* left = reinterpret_cast<float*>(lds) + wave * (BM / WM) * 8;
-  Rows<float> share;
-  if constexpr (EPI == kShare) {
-    share.init(a.parts + static_cast<int64_t>(sp) * a.M * a.ldp, a.ldp, m0, n0, rows,
-               static_cast<int>(min<int64_t>(BN, a.ldp - n0)), wm + li);
-  } else {
-    out.init(a.C, a.ldc, m0, n0, rows, cols, wm + li);
-    if constexpr (ACTS) keep.init(a.keep, a.ldk, m0, n0, rows, cols, wm + li);
-    if (ragged) __syncthreads();  // the waves' last reads
-  }
-
-  // B is the instruction's first operand: of tile (i, j) lane group g = lane / 16 holds columns 4 g
-  // to 4 g + 3 of row lane % 16. Two exchanges of lane groups among two by two tiles, group 2 h + 1
-  // of one register for group 2 h of the other, give each lane eight columns of a row: 64 bytes
-  // (bf16) of 16 rows an access. (Through LDS instead this took 5 us more a tile of 256 x 256.)
-  each_of<PLACES>([&](auto place) __attribute__((always_inline)) {
-    constexpr int P = decltype(place)::value, I = P / (TN / 2) * 2, Q = P % (TN / 2), J = Q * 2;
-    float x[2][2][4];  // [tile row][tile column]
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[0][j][r] = value<PIN>(acc[I][J + j][r]);
-        x[1][j][r] = value<PIN>(acc[I + 1][J + j][r]);
-      }
-      trade(x[0][j], x[1][j]);
-    }
-    trade(x[0][0], x[0][1]);
-    trade(x[1][0], x[1][1]);
-    const int c = wn + (J + group % 2) * 16 + group / 2 * 8;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = x[e / 4][b][e % 4];
-      if constexpr (EPI == kShare) {
-        Eight<float> all;
-        all.set(v);
-        share.put(I + b, c < static_cast<int>(a.ldp - n0) ? c * 4u : NOWHERE, all);
-        continue;
-      }
-      if (ragged) {
-        if (c == rest) {
-          f32x4* q = reinterpret_cast<f32x4*>(left + (I * 16 + b * 16 + li) * 8);
-          q[0] = (f32x4){v[0], v[1], v[2], v[3]};
-          q[1] = (f32x4){v[4], v[5], v[6], v[7]};
-        }
-      }
-      if (a.bias) {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(bias_lds + c);
-        const f32x4 hi = *reinterpret_cast<const f32x4*>(bias_lds + c + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] += lo[e];
-          v[4 + e] += hi[e];
-        }
-      }
-      Eight<E> done;
-      if constexpr (ACTS) {
-        float slope[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
-        if (a.keep) {
-          done.set(slope);
-          keep.put(I + b, column[Q], done);
-        }
-      }
-      if constexpr (FACTOR) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= factor<E, EPI>(beside[P % AHEAD][b].get(e));
-      } else if (a.beside) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += beside[P % AHEAD][b].get(e);
-      }
-      done.set(v);
-      out.put(I + b, column[Q], done);
-    }
-    if constexpr (EPI != kShare && P + AHEAD < PLACES)
-      if (a.beside) fetch(std::integral_constant<int, P + AHEAD>{});
-    __builtin_amdgcn_sched_barrier(0);
-  });
-  if (ragged && rest >= wn && rest < wn + BN / WN) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 1
-    for (int r = lane; r < BM / WM; r += 64)
-#pragma unroll 1
-      for (int e = 0; e < 8; ++e)
-        if (wm + r < rows) finish_one<E, EPI>(a, m0 + wm + r, n0 + rest + e, left[r * 8 + e]);
-  }
+  epilogue.end(acc, bias_lds, reinterpret_cast<float*>(lds) + wave * (BM / WM) * 8);
 }
 
-// Tiles of 256 x 256 by four waves of 128 x 128 (`big`), or of 128 x 128.
+// Tiles of 256 x 256 by four waves of 128 x 128, of 128 x 128, or, where the loads are what takes
+// the time (few rows), of 128 x 64 and 64 x 64 with many steps' loads under way.
+enum Tile : int { kBig = 0, kMiddle = 1, kDeep = 2, kDeepLow = 3 };
+struct TileOf {
+  int m, n;
+};
+inline TileOf tile_size(int tile) {
+  return tile == kBig ? TileOf{256, 256} : tile == kMiddle ? TileOf{128, 128} : tile == kDeep ? TileOf{128, 64}
+                                                                                            : TileOf{64, 64};
+}
 template <typename E, int EPI, bool TA, bool TB>
-void launch(const Args<E>& a, bool big, int nblk, hipStream_t s) {
-  if (big)
-    hipLaunchKernelGGL((product_kernel<E, EPI, TA, TB, 256, 256, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk);
-  else
-    hipLaunchKernelGGL((product_kernel<E, EPI, TA, TB, 128, 128, 2, 2>), dim3(nblk), dim3(256), 0, s, a, nblk);
+void launch(const Args<E>& a, int tile, int nblk, hipStream_t s) {
+#define DABSN_LAUNCH(BM, BN, BUFS)                                                                         \
+  hipLaunchKernelGGL((product_kernel<E, EPI, TA, TB, BM, BN, 2, 2, BUFS>), dim3(nblk), dim3(256), 0, s, a, \
+                     nblk)
+  if (tile == kBig) DABSN_LAUNCH(256, 256, 2);
+  else if (tile == kMiddle) DABSN_LAUNCH(128, 128, 2);
+  if constexpr (!TB && sizeof(E) == 2) {
+    if (tile == kDeep) DABSN_LAUNCH(128, 64, 6);
+    else if (tile == kDeepLow) DABSN_LAUNCH(64, 64, 8);
+  }
+#undef DABSN_LAUNCH
 }
 
 }  // namespace linear

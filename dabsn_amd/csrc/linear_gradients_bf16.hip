@@ -4,12 +4,12 @@
 namespace dabsn {
 namespace linear {
 
-template void launch<bf16, kNone, false, true>(const Args<bf16>&, bool, int, hipStream_t);
-template void launch<bf16, kShare, false, true>(const Args<bf16>&, bool, int, hipStream_t);
-template void launch<bf16, kStored, false, true>(const Args<bf16>&, bool, int, hipStream_t);
-template void launch<bf16, kFromSquare, false, true>(const Args<bf16>&, bool, int, hipStream_t);
-template void launch<bf16, kShare, true, true>(const Args<bf16>&, bool, int, hipStream_t);
-template void launch<bf16, kNone, true, true>(const Args<bf16>&, bool, int, hipStream_t);
+template void launch<bf16, kNone, false, true>(const Args<bf16>&, int, int, hipStream_t);
+template void launch<bf16, kShare, false, true>(const Args<bf16>&, int, int, hipStream_t);
+template void launch<bf16, kStored, false, true>(const Args<bf16>&, int, int, hipStream_t);
+template void launch<bf16, kFromSquare, false, true>(const Args<bf16>&, int, int, hipStream_t);
+template void launch<bf16, kShare, true, true>(const Args<bf16>&, int, int, hipStream_t);
+template void launch<bf16, kNone, true, true>(const Args<bf16>&, int, int, hipStream_t);
 
 }  // namespace linear
 }  // namespace dabsn
