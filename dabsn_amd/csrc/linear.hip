@@ -143,43 +143,55 @@ static bool ready(const void* p, int64_t ld, bool trans, int64_t K, bool padded)
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && (trans || padded || K % 8 == 0);
 }
 
+// The tile and the splits of K are those that take least by these times in us, as measured:
+//   256 x 256   1.41 a step of 64 k for all units (8192^3), six times as many steps for fp32
+//   128 x 128   0.55 a step with one tile a unit, 0.9 with two
+//   deep        the operands' way from L2, 100 KB/us a unit, but at least 0.2 a step
+//   direct      2.3 a step of 32 k (128 x 128; 0.62 for 64 x 64, but 0.9) for each tile of a unit
+//   besides     4 to 7 a round of tiles; packing 4 and its bytes at 4.5 TB/s; joining splits 6 and
+//               their bytes at 7 TB/s
 static Plan plan_of(const dabsn_linear_call& c) {
   Plan p = {};
+  if (c.M <= 16 && !c.transB && c.K > 0) {
+    p.tile = kRows;
+    p.splits = 1;
+    p.lda = c.lda;
+    p.ldb = c.ldb;
+    return p;
+  }
   const bool f32 = c.dtype == kF32;
-  p.packA = f32 || !ready(c.A, c.lda, c.transA, c.K, c.padA);
-  p.packB = f32 || !ready(c.B, c.ldb, c.transB, c.K, c.padB);
+  const bool packA = f32 || !ready(c.A, c.lda, c.transA, c.K, c.padA);
+  const bool packB = f32 || !ready(c.B, c.ldb, c.transB, c.K, c.padB);
   const int64_t rowsA = c.transA ? c.K : c.M, rowsB = c.transB ? c.K : c.N;
-  p.lda = p.packA ? ((c.transA ? c.M : c.K) + 7) / 8 * 8 : c.lda;
-  p.ldb = p.packB ? ((c.transB ? c.N : c.K) + 7) / 8 * 8 : c.ldb;
-  p.planeA = p.packA ? rowsA * p.lda : 0;
-  p.planeB = p.packB ? rowsB * p.ldb : 0;
-  size_t at = p.packA ? up16(static_cast<size_t>(p.planeA) * (f32 ? 6 : 2)) : 0;
-  p.atB = at;
-  at += p.packB ? up16(static_cast<size_t>(p.planeB) * (f32 ? 6 : 2)) : 0;
-  p.atParts = at;
-  // The tile and the splits of K by what they take, in us as measured (8192^3 in tiles of 256 x 256:
-  // 1.41 a step of all units; 128 x 128: 0.55 a step with a tile a unit, 0.9 with two; deep ones by
-  // their operands' way from L2, 100 KB/us a unit, or 0.2 a step; joining splits 6 and their bytes).
-  const int64_t steps = (c.K + PK - 1) / PK, times = f32 ? 6 : 1;
-  // Offsets of a transposed operand's rows are 32 bits.
-  const int64_t ld = std::max<int64_t>(c.transA ? p.lda : 0, c.transB ? p.ldb : 0);
-  const int64_t least = std::max<int64_t>(1, (c.K * ld * 2 + (1ll << 30) - 1) >> 30);
+  const int64_t wideA = ((c.transA ? c.M : c.K) + 7) / 8 * 8, wideB = ((c.transB ? c.N : c.K) + 7) / 8 * 8;
+  const int64_t lda = packA ? wideA : c.lda, ldb = packB ? wideB : c.ldb;
   p.ldp = (c.N + 7) / 8 * 8;
+  const double values = (packA ? 1.0 * rowsA * wideA : 0) + (packB ? 1.0 * rowsB * wideB : 0);
+  const double pack = values ? 4 + values * (f32 ? 10 : 4) / 4.5e6 : 0;
+  // A transposed operand's rows of a split lie within 2^30 bytes.
+  const int64_t ld = std::max<int64_t>(c.transA ? lda : 0, c.transB ? ldb : 0);
+  const int64_t least = std::max<int64_t>(1, (c.K * ld * 2 + (1ll << 30) - 1) >> 30);
   double best = 0;
-  for (int tile = kBig; tile <= (f32 || c.transB ? kMiddle : kDeepLow); ++tile) {
+  for (int tile = kBig; tile <= kDirectLow; ++tile) {
+    const bool deep = tile == kDeep || tile == kDeepLow, direct = tile >= kDirect;
+    if ((deep && (f32 || c.transB)) || (direct && !f32)) continue;
     const TileOf size = tile_size(tile);
     const int64_t mt = (c.M + size.m - 1) / size.m, nt = (c.N + size.n - 1) / size.n;
-    for (int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-      const int64_t splits = std::max(want, least);
+    const int64_t deepness = direct ? 32 : PK, steps = (c.K + deepness - 1) / deepness;
+    const int64_t times = f32 && !direct ? 6 : 1;
+    for (int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
       if (want > 1 && (want > steps || want < least)) continue;
+      const int64_t splits = direct ? want : std::max(want, least);
       const int64_t each = std::max<int64_t>(1, (steps + splits - 1) / splits);
       const int64_t real = std::max<int64_t>(1, (steps + each - 1) / each), wgs = mt * nt * real;
       const int64_t rounds = (wgs + 255) / 256;
-      double us = 0;
-      if (tile == kBig) us = rounds * (each * times * 1.41 + 7);
+      double us = direct ? 0 : pack;
+      if (tile == kBig) us += rounds * (each * times * 1.41 + 7);
       else if (tile == kMiddle)
-        us = (wgs <= 256 ? each * times * 0.55 : (rounds + 1) / 2 * (each * times * 0.9)) + 4;
-      else us = rounds * (each * std::max(0.2, (size.m + size.n) * PK * 2 / 100e3) + 4);
+        us += (wgs <= 256 ? each * times * 0.55 : (rounds + 1) / 2 * (each * times * 0.9)) + 4;
+      else if (deep) us += rounds * (each * std::max(0.2, (size.m + size.n) * PK * 2 / 100e3) + 4);
+      else if (tile == kDirect) us += rounds * each * 2.3 + 4;
+      else us += each * std::max(0.9, rounds * 0.62) + 4;
       if (real > 1) us += 6 + (8.0 * real * c.M * p.ldp) / 7e6;
       if (best == 0 || us < best) {
         best = us;
@@ -187,12 +199,20 @@ static Plan plan_of(const dabsn_linear_call& c) {
         p.mt = static_cast<int>(mt);
         p.nt = static_cast<int>(nt);
         p.splits = static_cast<int>(real);
-        p.kper = static_cast<int>(each * PK);
+        p.kper = static_cast<int>(each * deepness);
       }
     }
   }
-  if (p.splits > 1) at += static_cast<size_t>(p.splits) * c.M * p.ldp * sizeof(float);
-  p.bytes = at;
+  const bool direct = p.tile >= kDirect;
+  p.packA = packA && !direct;
+  p.packB = packB && !direct;
+  p.lda = p.packA ? lda : c.lda;
+  p.ldb = p.packB ? ldb : c.ldb;
+  p.planeA = p.packA ? rowsA * p.lda : 0;
+  p.planeB = p.packB ? rowsB * p.ldb : 0;
+  p.atB = p.packA ? up16(static_cast<size_t>(p.planeA) * (f32 ? 6 : 2)) : 0;
+  p.atParts = p.atB + (p.packB ? up16(static_cast<size_t>(p.planeB) * (f32 ? 6 : 2)) : 0);
+  p.bytes = p.atParts + (p.splits > 1 ? static_cast<size_t>(p.splits) * c.M * p.ldp * sizeof(float) : 0);
   return p;
 }
 

@@ -615,15 +615,210 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN == 128 * 128 ? 2 : 1) pr
   epilogue.end(acc, bias_lds, reinterpret_cast<float*>(lds) + wave * (BM / WM) * 8);
 }
 
+// fp32 operands as they lie, at any alignment, by fp32 matrix instructions: where splitting them into
+// planes would take longer than it saves (few products a value, small calls). Four waves a tile; steps
+// of 32 k through two buffers: step t's products while step t + 1 goes from registers to LDS and step
+// t + 2 comes to registers. K-contiguous rows are 128 bytes, read as in product_kernel; transposed rows
+// are read 16 columns at a time by four rows.
+template <bool T, int BT>
+struct Stage {
+  static constexpr int COLS = T ? BT : 32, ROWS = T ? 32 : BT, CPR = COLS / 4, NV = ROWS * CPR / 256;
+  static_assert(ROWS * CPR % 256 == 0, "staging must divide evenly");
+  u32x4 v[NV];
+  __device__ static int pos(int c, int r) { return T ? c ^ (((r >> 2) & 3) << 2) : c ^ (r & 7); }
+  // The tile at row r0, column c0 of a matrix of `rows` x `cols`, zeros beyond.
+  __device__ __forceinline__ void load(const float* p, int64_t ld, int r0, int c0, int rows, int cols, int tid) {
+    const bool inside = r0 + ROWS <= rows && c0 + COLS <= cols;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int q = tid + i * 256, r = r0 + q / CPR, c = c0 + q % CPR * 4;
+      const float* at = p + static_cast<int64_t>(r) * ld + c;
+      if (inside || (r < rows && c + 4 <= cols)) {
+        __builtin_memcpy(&v[i], at, 16);
+      } else {
+        float raw[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[e] = r < rows && c + e < cols ? at[e] : 0.0f;
+        __builtin_memcpy(&v[i], raw, 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int q = tid + i * 256, r = q / CPR;
+      *reinterpret_cast<u32x4*>(lds + r * COLS + pos(q % CPR, r) * 4) = v[i];
+    }
+  }
+  // Rows row0 + (lane & 15), k = ks * 16 + (lane >> 4) * 4 + 0..3: four instructions of four k each,
+  // one element of every lane group at a time.
+  __device__ static f32x4 get(const float* lds, int row0, int ks, int lane) {
+    const int li = lane & 15, g = lane >> 4;
+    if constexpr (!T) {
+      return *reinterpret_cast<const f32x4*>(lds + (row0 + li) * 32 + ((ks * 4 + g) ^ (li & 7)) * 4);
+    } else {
+      const float* at = lds + (ks * 16 + g * 4) * BT + ((row0 >> 4) ^ g) * 16 + li;
+      return (f32x4){at[0], at[BT], at[2 * BT], at[3 * BT]};
+    }
+  }
+};
+
+template <int EPI, bool TA, bool TB, int BT>
+__global__ void __launch_bounds__(256, 2) direct_kernel(Args<float> a, int nblk) {
+  constexpr int TT = BT / 32;  // tiles of 16 a wave's edge
+  using SA = Stage<TA, BT>;
+  using SB = Stage<TB, BT>;
+  __shared__ __attribute__((aligned(16))) float ldsA[2][BT * 32], ldsB[2][BT * 32];
+  __shared__ __attribute__((aligned(16))) float bias_lds[BT];
+  int sp, mt, nt;
+  if (!tile_of(blockIdx.x, nblk, a.splits, a.mt, a.nt, sp, mt, nt)) return;
+  const int m0 = mt * BT, n0 = nt * BT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / 2 * (BT / 2), wn = wave % 2 * (BT / 2);
+  const int k0 = sp * a.kper, kend = min(a.K, k0 + a.kper), steps = (kend - k0 + 31) / 32;
+  const float* A = reinterpret_cast<const float*>(a.A);
+  const float* B = reinterpret_cast<const float*>(a.B);
+  f32x4 acc[TT][TT];
+#pragma unroll
+  for (int i = 0; i < TT; ++i)
+#pragma unroll
+    for (int j = 0; j < TT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  Epilogue<float, EPI, TT, TT, BT, BT, 256, false> epilogue(a, sp, m0, n0, wm, wn, tid);
+  epilogue.begin(bias_lds, tid);
+  SA va;
+  SB vb;
+  auto load = [&](int t) __attribute__((always_inline)) {
+    const int k = k0 + t * 32;
+    if constexpr (TA) va.load(A, a.lda, k, m0, kend, a.M, tid);
+    else va.load(A, a.lda, m0, k, a.M, kend, tid);
+    if constexpr (TB) vb.load(B, a.ldb, k, n0, kend, a.N, tid);
+    else vb.load(B, a.ldb, n0, k, a.N, kend, tid);
+  };
+  load(0);
+  va.store(ldsA[0], tid);
+  vb.store(ldsB[0], tid);
+  if (steps > 1) load(1);
+  __syncthreads();
+  for (int t = 0; t < steps; ++t) {
+    const int buf = t & 1;
+    if (t + 1 < steps) {
+      va.store(ldsA[buf ^ 1], tid);  // released by the barrier that ended step t - 1
+      vb.store(ldsB[buf ^ 1], tid);
+      if (t + 2 < steps) load(t + 2);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      f32x4 fa[TT];
+#pragma unroll
+      for (int i = 0; i < TT; ++i) fa[i] = SA::get(ldsA[buf], wm + i * 16, ks, lane);
+#pragma unroll
+      for (int j = 0; j < TT; ++j) {
+        const f32x4 fb = SB::get(ldsB[buf], wn + j * 16, ks, lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < TT; ++i)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[e], fa[i][e], acc[i][j], 0, 0, 0);
+      }
+    }
+    __syncthreads();
+  }
+  epilogue.end(acc, bias_lds, ldsA[0] + wave * (BT / 2) * 8);
+}
+
+// Up to 16 rows: bound by the way of B, which is read once, straight to registers at any alignment. A
+// workgroup has WAVES waves and TN tiles of 16 columns; the waves take every WAVES-th block of BK k
+// (128 bytes of each of B's rows), UNROLL blocks of loads at a time, and their sums meet in LDS in
+// order. Rows of A beyond M are not read (zeros).
+template <typename E, int EPI, int TN, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) rows_kernel(Args<E> a, const E* A, const E* B) {
+  constexpr int VEC = 16 / sizeof(E), BK = 128 / sizeof(E), UNROLL = 4 / TN;
+  __shared__ __attribute__((aligned(16))) float sums[WAVES][TN][256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16 * TN;
+  f32x4 acc[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const E* pa = A + static_cast<int64_t>(min(li, a.M - 1)) * a.lda + g * VEC;
+  const E* pb[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+    pb[j] = B + static_cast<int64_t>(min(n0 + j * 16 + li, a.N - 1)) * a.ldb + g * VEC;
+  // Chunk h of block k of a row: 16 bytes from k + h BK / 2 + g VEC on.
+  auto take = [&](const E* p, int k, bool any) __attribute__((always_inline)) {
+    u32x4 v = {0u, 0u, 0u, 0u};
+    const int left = a.K - k - g * VEC;
+    if (any && left >= VEC) {
+      __builtin_memcpy(&v, p + k, 16);
+    } else if (any && left > 0) {
+      E raw[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) raw[e] = e < left ? p[k + e] : static_cast<E>(0);
+      __builtin_memcpy(&v, raw, 16);
+    }
+    return v;
+  };
+  auto multiply = [&](f32x4& c, u32x4 b, u32x4 x) __attribute__((always_inline)) {
+    if constexpr (sizeof(E) == 2) {
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, x), c, 0, 0, 0);
+    } else {
+      const f32x4 fb = __builtin_bit_cast(f32x4, b), fx = __builtin_bit_cast(f32x4, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[e], fx[e], c, 0, 0, 0);
+    }
+  };
+  const int whole = a.K / BK * BK;  // blocks without an edge
+  int k = wave * BK;
+  for (; k + (UNROLL - 1) * WAVES * BK < whole; k += UNROLL * WAVES * BK) {
+    u32x4 x[UNROLL][2], b[UNROLL][TN][2];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = k + u * WAVES * BK + h * (BK / 2);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) __builtin_memcpy(&b[u][j][h], pb[j] + at, 16);
+        x[u][h] = (u32x4){0u, 0u, 0u, 0u};
+        if (li < a.M) __builtin_memcpy(&x[u][h], pa + at, 16);
+      }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) multiply(acc[j], b[u][j][h], x[u][h]);
+  }
+  for (; k < a.K; k += WAVES * BK)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 x = take(pa, k + h * (BK / 2), li < a.M);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) multiply(acc[j], take(pb[j], k + h * (BK / 2), true), x);
+    }
+  // Row li, columns 4 g to 4 g + 3 of tile j.
+#pragma unroll
+  for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(&sums[wave][j][li * 16 + g * 4]) = acc[j];
+  __syncthreads();
+  for (int i = tid; i < TN * 256; i += WAVES * 64) {
+    const int j = i / 256, m = i % 256 / 16, n = n0 + j * 16 + i % 16;
+    if (m >= a.M || n >= (a.padC ? (a.N + 7) & ~7 : a.N)) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += sums[w][j][i % 256];
+    finish_one<E, EPI>(a, m, n, s);
+  }
+}
+
 // Tiles of 256 x 256 by four waves of 128 x 128, of 128 x 128, or, where the loads are what takes
-// the time (few rows), of 128 x 64 and 64 x 64 with many steps' loads under way.
-enum Tile : int { kBig = 0, kMiddle = 1, kDeep = 2, kDeepLow = 3 };
+// the time (few rows), of 128 x 64 and 64 x 64 with many steps' loads under way; of 128 x 128 and 64 x
+// 64 by direct_kernel; rows_kernel's.
+enum Tile : int { kBig = 0, kMiddle = 1, kDeep = 2, kDeepLow = 3, kDirect = 4, kDirectLow = 5, kRows = 6 };
 struct TileOf {
   int m, n;
 };
 inline TileOf tile_size(int tile) {
-  return tile == kBig ? TileOf{256, 256} : tile == kMiddle ? TileOf{128, 128} : tile == kDeep ? TileOf{128, 64}
-                                                                                            : TileOf{64, 64};
+  constexpr TileOf all[] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {128, 128}, {64, 64}};
+  return all[tile];
 }
 template <typename E, int EPI, bool TA, bool TB>
 void launch(const Args<E>& a, int tile, int nblk, hipStream_t s) {
@@ -635,6 +830,25 @@ void launch(const Args<E>& a, int tile, int nblk, hipStream_t s) {
   if constexpr (!TB && sizeof(E) == 2) {
     if (tile == kDeep) DABSN_LAUNCH(128, 64, 6);
     else if (tile == kDeepLow) DABSN_LAUNCH(64, 64, 8);
+  }
+  if constexpr (sizeof(E) == 4) {
+    if (tile == kDirect)
+      hipLaunchKernelGGL((direct_kernel<EPI, TA, TB, 128>), dim3(nblk), dim3(256), 0, s, a, nblk);
+    else if (tile == kDirectLow)
+      hipLaunchKernelGGL((direct_kernel<EPI, TA, TB, 64>), dim3(nblk), dim3(256), 0, s, a, nblk);
+  }
+  if constexpr (!TB && EPI != kShare) {
+    if (tile == kRows) {
+      // Columns as they fill the units; more waves where they do not.
+      const E *A = reinterpret_cast<const E*>(a.A), *B = reinterpret_cast<const E*>(a.B);
+      const int tiles = (a.N + 15) / 16;
+      if (tiles > 1024)
+        hipLaunchKernelGGL((rows_kernel<E, EPI, 2, 4>), dim3((tiles + 1) / 2), dim3(256), 0, s, a, A, B);
+      else if (tiles > 256)
+        hipLaunchKernelGGL((rows_kernel<E, EPI, 1, 4>), dim3(tiles), dim3(256), 0, s, a, A, B);
+      else
+        hipLaunchKernelGGL((rows_kernel<E, EPI, 1, 16>), dim3(tiles), dim3(1024), 0, s, a, A, B);
+    }
   }
 #undef DABSN_LAUNCH
 }
