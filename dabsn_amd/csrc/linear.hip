@@ -299,32 +299,42 @@ __global__ void __launch_bounds__(256) slope_kernel(int64_t rows, int n, const E
   const int pad = (n + 7) / 8 * 8 <= ldz ? (n + 7) / 8 * 8 : n;
   if (c < pad) {
     const bool whole = c + VEC <= n;
-    for (int64_t r = r0 + wave; r < r1; r += 4) {
-      E gv[VEC], sv[VEC], o[VEC];
-      if (whole) {
-        __builtin_memcpy(gv, g + r * ldg + c, 16);
-        if (kind) __builtin_memcpy(sv, s + r * lds + c, 16);
-      } else {
+    constexpr int U = 4;  // rows on their way at once
+    for (int64_t r = r0 + wave; r < r1; r += 4 * U) {
+      E gv[U][VEC], sv[U][VEC], o[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          gv[e] = c + e < n ? g[r * ldg + c + e] : static_cast<E>(0);
-          if (kind) sv[e] = c + e < n ? s[r * lds + c + e] : static_cast<E>(0);
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = r + 4 * u;
+        if (row >= r1) break;
+        if (whole) {
+          __builtin_memcpy(gv[u], g + row * ldg + c, 16);
+          if (kind) __builtin_memcpy(sv[u], s + row * lds + c, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            gv[u][e] = c + e < n ? g[row * ldg + c + e] : static_cast<E>(0);
+            if (kind) sv[u][e] = c + e < n ? s[row * lds + c + e] : static_cast<E>(0);
+          }
         }
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float v = to_f(gv[e]);
-        if (kind) v *= kind == kFromSquare ? factor<E, kFromSquare>(to_f(sv[e])) : to_f(sv[e]);
-        sum[e] += v;
-        o[e] = from_f<E>(v);
-      }
-      if (dz) {
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = r + 4 * u;
+        if (row >= r1) break;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          float v = to_f(gv[u][e]);
+          if (kind) v *= kind == kFromSquare ? factor<E, kFromSquare>(to_f(sv[u][e])) : to_f(sv[u][e]);
+          sum[e] += v;
+          o[e] = from_f<E>(v);
+        }
+        if (!dz) continue;
         if (whole) {
-          __builtin_memcpy(dz + r * ldz + c, o, 16);
+          __builtin_memcpy(dz + row * ldz + c, o, 16);
         } else {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            if (c + e < n || c + e < pad) dz[r * ldz + c + e] = o[e];  // o is 0 beyond n
+            if (c + e < n || c + e < pad) dz[row * ldz + c + e] = o[e];  // o is 0 beyond n
         }
       }
     }

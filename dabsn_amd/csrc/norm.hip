@@ -26,7 +26,29 @@ constexpr int64_t MAX_WIDTH = 16384;
 template <typename E>
 constexpr int vec_of() { return 16 / static_cast<int>(sizeof(E)); }
 
-// VEC elements from p on, at any alignment; those beyond `left` are 0.
+// A thread's vector of a row as it is stored, at any alignment; elements beyond `left` are 0.
+template <typename E>
+struct Raw {
+  static constexpr int VEC = vec_of<E>();
+  u32x4 q;
+  __device__ __forceinline__ void load(const E* p, int left) {
+    if (left >= VEC) {
+      __builtin_memcpy(&q, p, 16);
+    } else {
+      E e[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = i < left ? p[i] : static_cast<E>(0);
+      __builtin_memcpy(&q, e, 16);
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    const uint32_t w = q[sizeof(E) == 4 ? e : e / 2];
+    if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w);
+    else return __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
+  }
+};
+
+// VEC elements of a weight or bias; those beyond `left` are 0.
 template <typename E, int VEC>
 __device__ __forceinline__ void load_row(const E* p, int left, float (&v)[VEC]) {
   if (left >= VEC) {
@@ -67,62 +89,82 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
   return total;
 }
 
+// Workgroup `blockIdx.x` of `gridDim.x` takes rows blockIdx.x * R + (its row slot), and so on by
+// gridDim.x * R, the next row on its way while one is worked on.
 template <typename E, typename W, int T, int NV>
 __global__ void __launch_bounds__(T < 256 ? 256 : T)
     fwd_kernel(int64_t rows, int H, const E* x, int64_t ldx, const W* weight, const W* bias,
                float eps, int center, E* out, float* stats) {
   constexpr int VEC = vec_of<E>(), R = T < 256 ? 256 / T : 1;
-  __shared__ float part[2][T / 64];
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / T;
-  if (row >= rows) return;  // whole waves only: a row of several waves is the workgroup's
+  __shared__ float part[2][2][T / 64];
   const int t = threadIdx.x % T;
-  const E* xr = x + row * ldx;
-  float v[NV][VEC];
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * T + t) * VEC;
-    load_row<E, VEC>(xr + c, H - c, v[i]);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) sum += v[i][e];
-  }
   const float inv = 1.0f / static_cast<float>(H);
-  const float mean = center ? row_sum<T>(sum, part[0]) * inv : 0.0f;
-  float sq = 0.0f;
+  Raw<E> next[NV];
+  auto fetch = [&](int64_t row) {
+    if (row >= rows) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * T + t) * VEC;
+      next[i].load(x + row * ldx + c, H - c);
+    }
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * R + threadIdx.x / T;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * R;
+  fetch(row);
+  float w[NV][VEC], b[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * T + t) * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      v[i][e] = c + e < H ? v[i][e] - mean : 0.0f;
-      sq = fmaf(v[i][e], v[i][e], sq);
+      w[i][e] = 1.0f;
+      b[i][e] = 0.0f;
     }
+    if (weight && c < H) load_row<W, VEC>(weight + c, H - c, w[i]);
+    if (bias && c < H) load_row<W, VEC>(bias + c, H - c, b[i]);
   }
-  const float rstd = 1.0f / sqrtf(fmaf(row_sum<T>(sq, part[1]), inv, eps));
-  if (stats && t == 0) {
-    stats[2 * row] = mean;
-    stats[2 * row + 1] = rstd;
-  }
-  E* o = out + row * H;
+  int turn = 0;
+  for (; row < rows; row += stride, turn ^= 1) {  // a row of several waves is the workgroup's
+    float v[NV][VEC];
+    float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * T + t) * VEC;
-    if (c >= H) break;
-    float w[VEC], b[VEC];
-    if (weight) load_row<W, VEC>(weight + c, H - c, w);
-    if (bias) load_row<W, VEC>(bias + c, H - c, b);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      v[i][e] *= rstd;
-      if (weight) v[i][e] *= w[e];
-      if (bias) v[i][e] += b[e];
+      for (int e = 0; e < VEC; ++e) {
+        v[i][e] = next[i].get(e);
+        sum += v[i][e];
+      }
+    fetch(row + stride);
+    // The slots alternate: a wave that is still adding the last row's finds them untouched.
+    const float mean = center ? row_sum<T>(sum, part[turn][0]) * inv : 0.0f;
+    float sq = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * T + t) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[i][e] = c + e < H ? v[i][e] - mean : 0.0f;
+        sq = fmaf(v[i][e], v[i][e], sq);
+      }
     }
-    store_row<E, VEC>(o + c, H - c, v[i]);
+    const float rstd = 1.0f / sqrtf(fmaf(row_sum<T>(sq, part[turn][1]), inv, eps));
+    if (stats && t == 0) {
+      stats[2 * row] = mean;
+      stats[2 * row + 1] = rstd;
+    }
+    E* o = out + row * H;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * T + t) * VEC;
+      if (c >= H) break;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i][e] = v[i][e] * rstd * w[i][e] + b[i][e];
+      store_row<E, VEC>(o + c, H - c, v[i]);
+    }
   }
 }
 
-// Workgroup `blockIdx.x` of `gridDim.x` takes rows blockIdx.x * R + (its row slot), and so on by
-// gridDim.x * R; parts [gridDim.x][2][H] (dw, db; NULL: not needed).
+// Rows as in fwd_kernel; parts [gridDim.x][2][H] (dw, db; NULL: not needed).
 template <typename E, typename W, int T, int NV>
 __global__ void __launch_bounds__(T < 256 ? 256 : T)
     bwd_kernel(int64_t rows, int H, const E* x, int64_t ldx, const W* weight, const float* stats,
@@ -143,25 +185,33 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T)
     }
     if (weight && c < H) load_row<W, VEC>(weight + c, H - c, w[i]);
   }
+  Raw<E> nextx[NV], nextg[NV];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](int64_t row) {
+    if (row >= rows) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * T + t) * VEC;
+      nextx[i].load(x + row * ldx + c, H - c);
+      nextg[i].load(grad + row * ldg + c, H - c);
+    }
+    next_mean = stats[2 * row];
+    next_rstd = stats[2 * row + 1];
+  };
   int turn = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * R + slot; row < rows;
-       row += static_cast<int64_t>(gridDim.x) * R, turn ^= 1) {
-    const E* xr = x + row * ldx;
-    const E* gr = grad + row * ldg;
-    const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+  int64_t row = static_cast<int64_t>(blockIdx.x) * R + slot;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * R;
+  fetch(row);
+  for (; row < rows; row += stride, turn ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
     float u[NV][VEC], g[NV][VEC];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * T + t) * VEC;
-      load_row<E, VEC>(xr + c, H - c, u[i]);
-      load_row<E, VEC>(gr + c, H - c, g[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        u[i][e] = (u[i][e] - mean) * rstd;  // beyond H: g = 0, and u meets nothing else
+        u[i][e] = (nextx[i].get(e) - mean) * rstd;  // beyond H: g = 0, and u meets nothing else
+        g[i][e] = nextg[i].get(e);
         dw[i][e] = fmaf(g[i][e], u[i][e], dw[i][e]);
         db[i][e] += g[i][e];
         g[i][e] *= w[i][e];
@@ -169,7 +219,7 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T)
         s2 = fmaf(g[i][e], u[i][e], s2);
       }
     }
-    // The slots alternate: a wave that is still adding the last row's finds them untouched.
+    fetch(row + stride);
     s1 = center ? row_sum<T>(s1, part[turn][0]) * inv : 0.0f;
     s2 = row_sum<T>(s2, part[turn][1]) * inv;
 #pragma unroll
@@ -257,11 +307,13 @@ static Plan plan_of(int64_t rows, int64_t H, int vec) {
   return p;
 }
 
-// Partial rows of the backward: workgroups that fill the card, each with 4 rows or more.
+// Partial rows of the backward: workgroups that fill the card once by their registers, each with 4
+// rows or more.
 static int64_t parts_of(int64_t rows, int64_t H, int vec) {
   const Plan p = plan_of(rows, H, vec);
   const int64_t slots = p.T < 256 ? 256 / p.T : 1;
-  const int64_t most = p.T == 1024 ? 256 : 1024;
+  const int values = p.NV * vec;
+  const int64_t most = 256 * (p.T == 1024 ? 1 : values <= 4 ? 8 : values <= 8 ? 4 : values <= 16 ? 3 : 2);
   return std::max<int64_t>(1, std::min<int64_t>(most, (rows + 4 * slots - 1) / (4 * slots)));
 }
 
@@ -282,7 +334,9 @@ static int run_fwd(int64_t rows, int H, const void* x, int64_t ldx, const void* 
   const Plan p = plan_of(rows, H, vec_of<E>());
   return with_plan(p, [&](auto T, auto NV) {
     constexpr int R = T < 256 ? 256 / T : 1;
-    hipLaunchKernelGGL((fwd_kernel<E, W, T, NV>), dim3((unsigned)((rows + R - 1) / R)),
+    // Eight workgroups a unit (two of 1024 threads), or one a row.
+    const int64_t most = T == 1024 ? 512 : 2048;
+    hipLaunchKernelGGL((fwd_kernel<E, W, T, NV>), dim3((unsigned)std::min((rows + R - 1) / R, most)),
                        dim3(T < 256 ? 256 : T), 0, s, rows, H, (const E*)x, ldx, (const W*)w,
                        (const W*)b, eps, center, (E*)out, stats);
     DABSN_HIP_CHECK(hipGetLastError());

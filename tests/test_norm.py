@@ -245,8 +245,8 @@ def test_long_inputs(cuda_device):
         part = x.detach()[s:s + 53_000].double()
         term = part * part / (part.square().mean(1, keepdim=True) + 1e-6).sqrt()
         ref += term.sum(0)
-    # At most 518 rows a partial sum, 64 partial sums a slot and 16 slots, each addition u of the sum.
-    within(dw, ref, (2 ** -8 + (D + 600) * U) * ref)  # the terms are positive
+    # At most 691 rows a partial sum, 64 partial sums a slot and 16 slots, each addition u of the sum.
+    within(dw, ref, (2 ** -8 + (D + 780) * U) * ref)  # the terms are positive
 
 
 @pytest.mark.gpu
