@@ -18,7 +18,8 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .kernels import dense
+from . import _lib
+from .kernels import dense, ops
 from .norm import layer_norm, rms_norm
 
 _RELU2 = dense.ACTIVATIONS["relu2"]
@@ -109,45 +110,65 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
     return out if x.dim() == 2 else out.view(shape)
 
 
+def _mlp_call(x, nw, nb, w1, b1, w2, b2, act, layer, eps, out=None, grad=None) -> _lib.MlpCall:
+    p = ops._p
+    vector = nw if nw is not None else nb if nb is not None else x
+    return _lib.MlpCall(
+        ops._code(x.dtype), ops._code(vector.dtype), layer, act, x.shape[0], x.shape[1], w1.shape[0],
+        x.data_ptr(), p(nw), p(nb), w1.data_ptr(), p(b1), w2.data_ptr(), p(b2), p(grad),
+        dense.row_stride(x), dense.row_stride(w1), dense.row_stride(w2), 0, 0, eps, None, None, None,
+        p(out))
+
+
+def _run_mlp(call: _lib.MlpCall, x: Tensor, backward: bool) -> None:
+    lib = _lib.load()
+    nbytes = lib.dabsn_hip_mlp_workspace_bytes(call, backward)
+    if nbytes:
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        call.workspace, call.workspace_bytes = ws.data_ptr(), nbytes
+    name = "mlp_bwd" if backward else "mlp"
+    tk = ops.KernelTimer.begin(name, x)
+    _lib.check((lib.dabsn_hip_mlp_bwd if backward else lib.dabsn_hip_mlp_fwd)(call, dense.stream(x)), name)
+    ops.KernelTimer.end(tk)
+
+
 class _MLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, nw, nb, w1, b1, w2, b2, act, layer, eps):
+        rows, f = x.shape[0], w1.shape[0]
         with dense.on(x):
-            normed, stats = dense.norm(x, nw, nb, eps, layer, True)
-            keep, kind = _keeps(x, w1.shape[0], act, False)
-            h = dense.product(normed, w1, bias=b1, act=act, keep=keep, pad_out=True)
-            out = dense.product(h, w2, bias=b2, residual=x, pad_a=True)
-        ctx.save_for_backward(x, nw, stats, normed, w1, h, keep, w2)
-        ctx.kind, ctx.layer = kind, layer
-        ctx.dtype = (x if nw is None and nb is None else nb if nw is None else nw).dtype
+            out, normed = x.new_empty(x.shape), x.new_empty(x.shape)
+            stats = x.new_empty((rows, 2), dtype=torch.float32)
+            h = dense.padded(rows, f, x)
+            keep, _ = _keeps(x, f, act, False)
+            call = _mlp_call(x, nw, nb, w1, b1, w2, b2, act, layer, eps, out)
+            call.normed, call.stats = normed.data_ptr(), stats.data_ptr()
+            call.h, call.ldh = h.data_ptr(), dense.row_stride(h)
+            if keep is not None:
+                call.keep, call.ldk = keep.data_ptr(), dense.row_stride(keep)
+            _run_mlp(call, x, False)
+        ctx.save_for_backward(x, nw, nb, w1, b1, w2, b2, normed, stats, h, keep)
+        ctx.args = act, layer, eps
         return out
 
     @staticmethod
     @dense.once
     def backward(ctx, g):
-        x, nw, stats, normed, w1, h, keep, w2 = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dnw = dnb = dw1 = db1 = dw2 = db2 = None
+        x, nw, nb, w1, b1, w2, b2, normed, stats, h, keep = ctx.saved_tensors
         with dense.on(x):
-            # Contiguous rows: they are the norm's `add` too.
             rows = dense.rows_of(g).contiguous()
-            if need[6]:
-                _, db2 = dense.slope_product(rows, None, 0, False, True)
-            if need[5]:
-                dw2 = dense.product(rows, h, trans_a=True, trans_b=True)
-            if any(need[:5]):
-                slope = h if ctx.kind == dense._FROM_SQUARE else keep
-                dz = dense.product(rows, w2, trans_b=True, slope=slope, slope_kind=ctx.kind,
-                                   pad_out=True)
-                if need[4]:
-                    _, db1 = dense.slope_product(dz, None, 0, False, True)
-                if need[3]:
-                    dw1 = dense.product(dz, normed, trans_a=True, trans_b=True)
-                if any(need[:3]):
-                    dn = dense.product(dz, w1, trans_b=True, pad_a=True)
-                    dx, dnw, dnb = dense.norm_backward(x, nw, stats, dn, ctx.layer, rows, ctx.dtype,
-                                                       need[1], need[2])
-        return dx, dnw, dnb, dw1, db1, dw2, db2, None, None, None
+            leaves = x, nw, nb, w1, b1, w2, b2
+            grads = [t.new_empty(t.shape) if need else None
+                     for t, need in zip(leaves, ctx.needs_input_grad)]
+            call = _mlp_call(*leaves, *ctx.args, grad=rows)
+            call.normed, call.stats = normed.data_ptr(), stats.data_ptr()
+            call.h, call.ldh = h.data_ptr(), h.stride(0)
+            if keep is not None:
+                call.keep, call.ldk = keep.data_ptr(), keep.stride(0)
+            (call.dx, call.dnorm_weight, call.dnorm_bias, call.dw1, call.db1, call.dw2,
+             call.db2) = map(ops._p, grads)
+            _run_mlp(call, x, True)
+        return (*grads, None, None, None)
 
 
 def fused_mlp(x: Tensor, w1: Tensor, w2: Tensor, b1: Tensor | None = None,
@@ -188,7 +209,6 @@ def fused_mlp(x: Tensor, w1: Tensor, w2: Tensor, b1: Tensor | None = None,
         out = _MLP.apply(*leaves, act, layer, eps)
     else:
         with dense.on(x):
-            normed, _ = dense.norm(rows, nw, nb, eps, layer, False)
-            mid = dense.product(normed, w1, bias=b1, act=act, pad_out=True)
-            out = dense.product(mid, w2, bias=b2, residual=rows, pad_a=True)
+            out = rows.new_empty(rows.shape)
+            _run_mlp(_mlp_call(*leaves, act, layer, eps, out), rows, False)
     return out if x.dim() == 2 else out.view(x.shape)

@@ -819,6 +819,28 @@ int dabsn_hip_linear_slope(int dtype, int64_t rows, int64_t n, const void* grad,
                            void* dbias, void* workspace, size_t workspace_bytes,
                            hipStream_t stream);
 
+/* dabsn_hip_mlp_fwd: out [M, H] = x + act(norm(x) w1^T + b1) w2^T + b2 by the calls above, x with row
+ * stride ldx, w1 [F, H], w2 [H, F] (row strides ldw1, ldw2). normed [M, H], stats [M][2] and h
+ * [M, ldh >= F rounded up to 8], the activated inner rows, are kept for the backward where given;
+ * keep [M, ldk], the activation's slope, is for GELU and SiLU. _bwd: the gradients that are asked
+ * for (not NULL) from grad [M, H] and these; dx holds the sum of both branches. Workspace:
+ * dabsn_hip_mlp_workspace_bytes of the same call (its workspace may be unset), 16-byte aligned. */
+typedef struct dabsn_mlp_call {
+  int dtype, wdtype, layer, act;
+  int64_t M, H, F;
+  const void *x, *norm_weight, *norm_bias, *w1, *b1, *w2, *b2, *grad;
+  int64_t ldx, ldw1, ldw2, ldh, ldk;
+  float eps;
+  void *normed, *h, *keep, *out;
+  float* stats;
+  void *dx, *dnorm_weight, *dnorm_bias, *dw1, *db1, *dw2, *db2, *workspace;
+  size_t workspace_bytes;
+} dabsn_mlp_call;
+
+size_t dabsn_hip_mlp_workspace_bytes(const dabsn_mlp_call* call, int backward);
+int dabsn_hip_mlp_fwd(const dabsn_mlp_call* call, hipStream_t stream);
+int dabsn_hip_mlp_bwd(const dabsn_mlp_call* call, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,10 +83,10 @@ def test_library_refuses_bad_arguments_before_it_launches():
                 dict(C=None)):
         assert call(**bad) == -2, bad
     assert lib.dabsn_hip_linear(None, None) == -2
-    # fp32 operands are split in the workspace.
+    # Parts of a split product, and fp32 operands' planes, lie in the workspace.
     f = dict(dtype=0, M=256, N=2048, K=8192, A=one, B=one, C=one, lda=8192, ldb=8192, ldc=2048)
     need = lib.dabsn_hip_linear_workspace_bytes(ctypes.byref(_lib.LinearCall(**f)))
-    assert need >= 6 * (256 + 2048) * 8192 and lib.dabsn_hip_linear_workspace_bytes(None) == 0
+    assert need > 0 and lib.dabsn_hip_linear_workspace_bytes(None) == 0
     assert lib.dabsn_hip_linear_workspace_bytes(ctypes.byref(_lib.LinearCall(**{**f, "M": 0}))) == 0
     for ws, n in ((one, need - 1), (None, need), (one + 8, need)):
         assert call(**f, workspace=ws, workspace_bytes=n) == -2
@@ -94,6 +94,37 @@ def test_library_refuses_bad_arguments_before_it_launches():
                                     (0, 4, 8, 7, 1 << 30), (0, 4, 8, 8, 0)):
         assert lib.dabsn_hip_linear_slope(dtype, rows, n, one, ldg, None, 0, 0, one, 8, one, one, ws,
                                           None) == -2
+
+
+def test_library_refuses_bad_arguments_of_the_mlp_before_it_launches():
+    import ctypes
+
+    from dabsn_amd import _lib
+
+    lib, one = _lib.load(), 1 << 20
+    good = dict(dtype=1, wdtype=0, act=2, M=5, H=16, F=24, x=one, w1=one, w2=one, grad=one, ldx=16,
+                ldw1=16, ldw2=24, ldh=24, ldk=24, normed=one, h=one, keep=one, out=one, stats=one, dx=one)
+
+    def status(backward, **change):
+        c = _lib.MlpCall(**{**good, **change})
+        if "workspace" not in change:
+            c.workspace = one
+            c.workspace_bytes = lib.dabsn_hip_mlp_workspace_bytes(ctypes.byref(c), backward)
+        return (lib.dabsn_hip_mlp_bwd if backward else lib.dabsn_hip_mlp_fwd)(ctypes.byref(c), None)
+
+    for backward in (0, 1):
+        for bad in (dict(dtype=2), dict(M=-1), dict(M=1 << 31), dict(H=0), dict(H=16385), dict(F=0),
+                    dict(F=1 << 21), dict(act=4), dict(act=-1), dict(act=0), dict(ldx=15), dict(ldw1=15),
+                    dict(ldw2=23), dict(ldh=23), dict(F=20, ldh=23), dict(ldk=23), dict(x=None), dict(w1=None),
+                    dict(w2=None), dict(wdtype=3), dict(ldx=1 << 21)):
+            assert status(backward, **bad) == -2, (backward, bad)
+    assert status(0, out=None) == -2 and status(0, normed=None, workspace=one, workspace_bytes=8) == -2
+    for bad in (dict(keep=None), dict(grad=None), dict(normed=None), dict(stats=None), dict(h=None),
+                dict(workspace=one, workspace_bytes=8), dict(workspace=None, workspace_bytes=1 << 30),
+                dict(workspace=one + 8, workspace_bytes=1 << 30)):
+        assert status(1, **bad) == -2, bad
+    assert lib.dabsn_hip_mlp_fwd(None, None) == -2 and lib.dabsn_hip_mlp_bwd(None, None) == -2
+    assert lib.dabsn_hip_mlp_workspace_bytes(None, 0) == 0
 
 
 class Val:
