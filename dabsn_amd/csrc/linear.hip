@@ -107,18 +107,18 @@ __global__ void __launch_bounds__(256) join_kernel(Args<E> a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += x.get(e);
   }
-  float slope[8];
+  float kept[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
+  for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], kept[e]);
   if (a.keep) {
-    x.set(slope);
+    x.template set<HALF<E, EPI>>(kept);
     __builtin_memcpy(a.keep + m * a.ldk + n, &x, sizeof(x));
   }
   if (a.beside) {
     __builtin_memcpy(&x, a.beside + m * a.ldr + n, sizeof(x));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if constexpr (EPI == kStored || EPI == kFromSquare) v[e] *= factor<E, EPI>(x.get(e));
+      if constexpr (EPI == kStored || EPI == kFromSquare) v[e] *= factor<E, EPI>(x.template get<HALF<E, EPI>>(e));
       else v[e] += x.get(e);
     }
   }
@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(256) slope_kernel(int64_t rows, int n, const E
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           float v = to_f(gv[u][e]);
-          if (kind) v *= kind == kFromSquare ? factor<E, kFromSquare>(to_f(sv[u][e])) : to_f(sv[u][e]);
+          if (kind)
+            v *= kind == kFromSquare ? factor<E, kFromSquare>(to_f(sv[u][e])) : beside_of<E, kStored>(sv[u], e);
           sum[e] += v;
           o[e] = from_f<E>(v);
         }

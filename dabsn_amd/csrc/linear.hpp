@@ -1,6 +1,6 @@
 // Matrix products with the work around them in their epilogue, for the block's MLP.
 //
-//   C(m, n) = act(sum_k A(m, k) B(n, k) + bias(n)) * slope(m, n) + residual(m, n)
+//   C(m, n) = act(sum_k A(m, k) B(n, k) + bias(n)) + residual(m, n)   or   sum * slope(m, n)
 //
 // in fp32, rounded once to the type of A and B. An operand is K-contiguous, A[m * lda + k], or
 // stored as its transpose, A[k * lda + m]: the forward needs neither transposed, the gradient of
@@ -16,7 +16,6 @@
 namespace dabsn {
 namespace linear {
 
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // What the epilogue does with the sums: an activation (and then the residual is added), or a factor:
@@ -35,25 +34,28 @@ struct Args {
   E* C;
   int64_t ldc;
   int padC;  // rows of C get zeros up to a multiple of 8
-  E* keep;  // act'(z); NULL: not kept
+  E* keep;  // what the backward needs of the activation; NULL: not kept
   int64_t ldk;
   int mt, nt, splits, kper;
   float* parts;  // [splits][M][ldp]: the splits' sums, instead of C
   int64_t ldp;
 };
 
-// act(z) and its derivative. Where they are rounded to bf16, the hardware's exp and reciprocal do
+// act(z), and what is kept for its derivative: of the squared ReLU the value itself (before a residual;
+// a rounding of it is half of one in the slope 2 sqrt(h)), else the derivative. With bf16 operands
+// that is stored in fp16: derivatives of GELU and SiLU lie in [-0.13, 1.13], where that is off by
+// 2^-11 of itself or 2^-25, an eighth of bf16's step, at the same bytes.
+// Where they are rounded to bf16, the hardware's exp and reciprocal do
 // (2^-22 and 2^-23 of their values), and erfc(x) = exp(-x^2) erfcx(x) with erfcx as a polynomial in
 // t = 1 / (1 + 0.46 x), a fit of our own for x >= 0 that is within 1.7e-5 of the value up to x = 60
 // (2^-8 is a rounding's): 20 instructions instead of erfcf's 70.
 template <typename E, int EPI>
-__device__ __forceinline__ float activate(float z, float& slope) {
+__device__ __forceinline__ float activate(float z, float& kept) {
   constexpr bool low = sizeof(E) == 2;
   constexpr float LOG2E = 1.44269504088896341f;
   if constexpr (EPI == kRelu2) {
     const float r = z < 0.0f ? 0.0f : z;  // a NaN stays
-    slope = 2.0f * r;
-    return r * r;
+    return kept = r * r;
   }
   if constexpr (EPI == kGelu) {
     float below, bell;  // the normal distribution function and exp(-z^2 / 2)
@@ -72,7 +74,7 @@ __device__ __forceinline__ float activate(float z, float& slope) {
       below = 0.5f * erfcf(z * -0.70710678118654752f);
       bell = expf(-0.5f * z * z);
     }
-    slope = fmaf(z * 0.39894228040143268f, bell, below);
+    kept = fmaf(z * 0.39894228040143268f, bell, below);
     return z * below;
   }
   if constexpr (EPI == kSilu) {
@@ -84,10 +86,10 @@ __device__ __forceinline__ float activate(float z, float& slope) {
       s = 1.0f / (1.0f + expf(-z));
       rest = 1.0f / (1.0f + expf(z));
     }
-    slope = fmaf(z * s, rest, s);
+    kept = fmaf(z * s, rest, s);
     return z * s;
   }
-  slope = 1.0f;
+  kept = 1.0f;
   return z;
 }
 
@@ -98,28 +100,36 @@ __device__ __forceinline__ float factor(float s) {
   return 2.0f * (sizeof(E) == 2 ? __builtin_amdgcn_sqrtf(s) : sqrtf(s));
 }
 
-// Eight columns of a row as they are stored.
+// Whether a derivative is kept for GELU and SiLU or read: fp16 in bf16's place.
+template <typename E, int EPI>
+constexpr bool HALF = sizeof(E) == 2 && (EPI == kGelu || EPI == kSilu || EPI == kStored);
+
+// Eight columns of a row as they are stored; with H as fp16 in bf16's place.
 template <typename E>
 struct Eight {
   static constexpr int Q = sizeof(E) / 2;
   u32x4 q[Q];
+  template <bool H = false>
   __device__ __forceinline__ float get(int e) const {
     const uint32_t w = q[sizeof(E) == 4 ? e / 4 : 0][sizeof(E) == 4 ? e % 4 : e / 2];
     // (A bit cast of the vector's element itself would take its first.)
     if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w);
+    else if constexpr (H)
+      return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(e % 2 ? w >> 16 : w)));
     else return __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
   }
+  template <bool H = false>
   __device__ __forceinline__ void set(const float (&v)[8]) {
     if constexpr (sizeof(E) == 4) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) q[e / 4][e % 4] = __builtin_bit_cast(uint32_t, v[e]);
     } else {
       typedef float f32x2 __attribute__((ext_vector_type(2)));
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      typedef std::conditional_t<H, _Float16, __bf16> low __attribute__((ext_vector_type(2)));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         q[0][i] = __builtin_bit_cast(
-            uint32_t, __builtin_convertvector(((f32x2){v[2 * i], v[2 * i + 1]}), bf16x2));
+            uint32_t, __builtin_convertvector(((f32x2){v[2 * i], v[2 * i + 1]}), low));
     }
   }
 };
@@ -152,6 +162,12 @@ struct Rows {
   }
 };
 
+template <typename E, int EPI>
+__device__ __forceinline__ float beside_of(const E* p, int64_t i) {
+  if constexpr (HALF<E, EPI>) return static_cast<float>(__builtin_bit_cast(_Float16, p[i]));
+  else return ld(p, i);
+}
+
 // The same for one column, or for the zeros beyond the row's end.
 template <typename E, int EPI>
 __device__ __forceinline__ void finish_one(const Args<E>& a, int64_t m, int n, float v) {
@@ -160,12 +176,18 @@ __device__ __forceinline__ void finish_one(const Args<E>& a, int64_t m, int n, f
     if (a.padC) *out = static_cast<E>(0);
     return;
   }
-  float slope;
+  float kept;
   if (a.bias) v += ld(a.bias, n);
-  v = activate<E, EPI>(v, slope);
-  if (a.keep) st(a.keep, m * a.ldk + n, slope);
-  const float beside = a.beside ? ld(a.beside, m * a.ldr + n) : 0.0f;
-  st(out, 0, EPI == kStored || EPI == kFromSquare ? v * factor<E, EPI>(beside) : v + beside);
+  v = activate<E, EPI>(v, kept);
+  if (a.keep) {
+    if constexpr (HALF<E, EPI>) a.keep[m * a.ldk + n] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(kept));
+    else st(a.keep, m * a.ldk + n, kept);
+  }
+  if constexpr (EPI == kStored || EPI == kFromSquare) {
+    st(out, 0, v * factor<E, EPI>(beside_of<E, EPI>(a.beside, m * a.ldr + n)));
+  } else {
+    st(out, 0, a.beside ? v + ld(a.beside, m * a.ldr + n) : v);
+  }
 }
 
 // The tile and split of workgroup L: consecutive workgroups go round the 8 XCDs, so each XCD gets a
@@ -248,7 +270,7 @@ struct Feed {
     asm volatile("s_add_u32 m0, %1, %2\n\tv_add_u32 %0, %3, %4\n\tbuffer_load_dwordx4 %0, %5, 0 offen lds"
                  : "=&v"(o)
                  : "s"(lds), "n"(I * NTH * 16), "s"(I * stride), "v"(at), "s"(rsrc)
-                 : "memory", "scc");
+                 : "memory", "scc", "m0");
   }
 };
 
@@ -441,17 +463,17 @@ struct Epilogue {
         }
         Eight<E> done;
         if constexpr (ACTS) {
-          float slope[8];
+          float kept[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], slope[e]);
+          for (int e = 0; e < 8; ++e) v[e] = activate<E, EPI>(v[e], kept[e]);
           if (a.keep) {
-            done.set(slope);
+            done.template set<HALF<E, EPI>>(kept);
             keep.put(I + b, column[Q], done);
           }
         }
         if constexpr (FACTOR) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= factor<E, EPI>(beside[P % AHEAD][b].get(e));
+          for (int e = 0; e < 8; ++e) v[e] *= factor<E, EPI>(beside[P % AHEAD][b].template get<HALF<E, EPI>>(e));
         } else if (a.beside) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] += beside[P % AHEAD][b].get(e);

@@ -58,7 +58,7 @@ static Forward forward(const dabsn_mlp_call& c, char* base) {
   f.first = product(c, c.M, c.F, c.H, f.normed, c.H, c.w1, c.ldw1, f.h, f.ldh);
   f.first.bias = c.b1;
   f.first.act = c.act;
-  f.first.keep = c.keep; f.first.ldk = c.ldk;
+  if (c.act > 1) f.first.keep = c.keep, f.first.ldk = c.ldk;
   f.first.padC = 1;
   f.second = product(c, c.M, c.H, c.F, f.h, f.ldh, c.w2, c.ldw2, c.out, c.H);
   f.second.bias = c.b2;
@@ -74,6 +74,7 @@ struct Backward {
   void *dz, *dn, *dx;
   int64_t ldz;
   dabsn_linear_call dz_call, dn_call, dw1_call, dw2_call;
+  bool rows, inner;  // whether dz, and what lies before it, is asked for
   size_t scratch_at, scratch, total;
 };
 static Backward backward(const dabsn_mlp_call& c, char* base) {
@@ -81,10 +82,11 @@ static Backward backward(const dabsn_mlp_call& c, char* base) {
   Space s{base};
   Backward b = {};
   b.ldz = padded(c.F);
-  const bool inner = c.dx || c.dnorm_weight || c.dnorm_bias;
-  b.dz = inner || c.dw1 || c.db1 ? s.take(static_cast<size_t>(c.M) * b.ldz * size) : nullptr;
-  b.dn = inner ? s.take(static_cast<size_t>(c.M) * c.H * size) : nullptr;
-  b.dx = c.dx || !inner ? c.dx : s.take(static_cast<size_t>(c.M) * c.H * size);
+  b.inner = c.dx || c.dnorm_weight || c.dnorm_bias;
+  b.rows = b.inner || c.dw1 || c.db1;
+  b.dz = b.rows ? s.take(static_cast<size_t>(c.M) * b.ldz * size) : nullptr;
+  b.dn = b.inner ? s.take(static_cast<size_t>(c.M) * c.H * size) : nullptr;
+  b.dx = c.dx || !b.inner ? c.dx : s.take(static_cast<size_t>(c.M) * c.H * size);
   const auto need = [&](const dabsn_linear_call& l) {
     b.scratch = std::max(b.scratch, dabsn_hip_linear_workspace_bytes(&l));
   };
@@ -93,13 +95,15 @@ static Backward backward(const dabsn_mlp_call& c, char* base) {
     b.dw2_call.transA = b.dw2_call.transB = 1;
     need(b.dw2_call);
   }
-  if (b.dz) {
+  if (b.rows) {
     b.dz_call = product(c, c.M, c.F, c.H, c.grad, c.H, c.w2, c.ldw2, b.dz, b.ldz);
     b.dz_call.transB = 1;
     b.dz_call.padC = 1;
-    b.dz_call.slope = c.keep ? c.keep : c.act ? c.h : nullptr;
-    b.dz_call.lds = c.keep ? c.ldk : c.ldh;
-    b.dz_call.slope_kind = c.keep ? 1 : 2;
+    if (c.act) {  // the squared ReLU's slope is its output's
+      b.dz_call.slope = c.act == 1 ? c.h : c.keep;
+      b.dz_call.lds = c.act == 1 ? c.ldh : c.ldk;
+      b.dz_call.slope_kind = c.act == 1 ? 2 : 1;
+    }
     need(b.dz_call);
   }
   if (c.dw1) {
@@ -107,7 +111,7 @@ static Backward backward(const dabsn_mlp_call& c, char* base) {
     b.dw1_call.transA = b.dw1_call.transB = 1;
     need(b.dw1_call);
   }
-  if (inner) {
+  if (b.inner) {
     b.dn_call = product(c, c.M, c.H, c.F, b.dz, b.ldz, c.w1, c.ldw1, b.dn, c.H);
     b.dn_call.transB = 1;
     b.dn_call.padA = 1;
@@ -179,8 +183,7 @@ int dabsn_hip_mlp_bwd(const dabsn_mlp_call* call, hipStream_t stream) {
   DABSN_STEP(check(c));
   DABSN_REQUIRE(c.w1 && c.w2 && (c.M == 0 || (c.x && c.grad && c.normed && c.stats && c.h)),
                 "mlp backward: null pointer");
-  // Activations but the squared ReLU, whose slope is its output's, have a slope kept.
-  DABSN_REQUIRE(c.act == 0 || c.act == 1 || c.keep || c.M == 0, "mlp backward: no slope");
+  DABSN_REQUIRE(c.act <= 1 || c.keep || c.M == 0, "mlp backward: no slope");
   char* ws = static_cast<char*>(c.workspace);
   const Backward b = backward(c, ws);
   DABSN_REQUIRE(b.total == 0 || (ws && c.workspace_bytes >= b.total && (reinterpret_cast<uintptr_t>(ws) & 15u) == 0),
@@ -190,12 +193,12 @@ int dabsn_hip_mlp_bwd(const dabsn_mlp_call* call, hipStream_t stream) {
     DABSN_STEP(dabsn_hip_linear_slope(c.dtype, c.M, c.H, c.grad, c.H, nullptr, 0, 0, nullptr, 0, c.db2, scratch,
                                       b.scratch, stream));
   if (c.dw2) DABSN_STEP(run(b.dw2_call, scratch, b.scratch, stream));
-  if (b.dz) DABSN_STEP(run(b.dz_call, scratch, b.scratch, stream));
+  if (b.rows) DABSN_STEP(run(b.dz_call, scratch, b.scratch, stream));
   if (c.db1)
     DABSN_STEP(dabsn_hip_linear_slope(c.dtype, c.M, c.F, b.dz, b.ldz, nullptr, 0, 0, nullptr, 0, c.db1, scratch,
                                       b.scratch, stream));
   if (c.dw1) DABSN_STEP(run(b.dw1_call, scratch, b.scratch, stream));
-  if (!b.dn) return DABSN_OK;
+  if (!b.inner) return DABSN_OK;
   DABSN_STEP(run(b.dn_call, scratch, b.scratch, stream));
   return dabsn_hip_norm_bwd(c.dtype, c.wdtype, c.layer, c.M, c.H, c.x, c.ldx, c.norm_weight, c.stats, b.dn, c.H,
                             c.grad, b.dx, c.dnorm_weight, c.dnorm_bias, scratch, b.scratch, stream);

@@ -8,9 +8,9 @@ Activations: ``none``, ``relu2`` (the squared ReLU of the reference's MLP), ``ge
 function) and ``silu``. (A plain ReLU is left out: its slope jumps at 0, so products of 16-bit
 operands would differ by whole terms.) Products are fp32 sums; everything up to the result is fp32
 and is rounded once. Both are differentiable in all their tensors. In the backward the products'
-operands have the inputs' type: dz = g activation'(z) is rounded once to it, from a slope that is
-rounded once too. The squared ReLU's slope is 2 sqrt of its output where that is at hand, so nothing
-more is kept.
+operands have the inputs' type: dz = g activation'(z) is rounded once to it. The slope is kept in
+fp32, or with bfloat16 in fp16 (2^-11 of itself or 2^-25 off); the squared ReLU's is 2 sqrt of its
+output, which is kept itself.
 """
 
 from __future__ import annotations
@@ -40,12 +40,11 @@ def _weight(what: str, name: str, w: Tensor, x: Tensor, width: int) -> Tensor:
 
 
 def _keeps(x: Tensor, n: int, act: int, residual: bool):
-    """(buffer for the slope or None, its kind) of an activated product's forward in training."""
-    if act == 0:
-        return None, 0
-    if act == _RELU2 and not residual:
-        return None, dense._FROM_SQUARE
-    return dense.padded(x.shape[0], n, x), dense._STORED
+    """(buffer for what the slope is made of or None, its kind) of an activated product's forward in
+    training. The squared ReLU's output is at hand where no residual is added to it."""
+    if act == 0 or (act == _RELU2 and not residual):
+        return None, dense._FROM_SQUARE if act else 0
+    return dense.padded(x.shape[0], n, x), dense._FROM_SQUARE if act == _RELU2 else dense._STORED
 
 
 class _Linear(torch.autograd.Function):
@@ -54,7 +53,7 @@ class _Linear(torch.autograd.Function):
         with dense.on(x):
             keep, kind = _keeps(x, weight.shape[0], act, residual is not None)
             out = dense.product(x, weight, bias=bias, act=act, keep=keep, residual=residual)
-        ctx.save_for_backward(x, weight, out if kind == dense._FROM_SQUARE else keep)
+        ctx.save_for_backward(x, weight, out if kind and keep is None else keep)
         ctx.kind = kind
         return out
 

@@ -782,14 +782,16 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
  *
  * dabsn_hip_linear: C [M, N] = act(A B^T + bias) + residual, or with transB (A B^T) * slope, fp32
  * until its one rounding.
- * A [M, K], row stride lda; B [N, K], or with transB its transpose [K, N]; with transA
- * (and transB) A is stored as [K, M] too; any alignment. act: 0 none, 1 squared ReLU, 2 GELU (by the error function), 3 SiLU. keep [M, N]
- * (row stride ldk; NULL: none) receives the activation's derivative. slope_kind 1: slope [M, N] as it is, 2: slope
- * holds the squared ReLU's output h and the factor is 2 sqrt(h). fp32 operands
- * are multiplied as three bf16 planes each, which hold all bits from 2^-110 up. padA, padB: the
- * operand's rows end in zeros up to a multiple of 8 columns; padC: C's are to. Row strides are below
- * 2^21. Workspace: dabsn_hip_linear_workspace_bytes of the same call (its workspace may
- * be unset), 16-byte aligned (0: none).
+ * A [M, K], row stride lda; B [N, K], or with transB its transpose [K, N]; with transA (and
+ * transB) A is stored as [K, M] too; any alignment. act: 0 none, 1 squared ReLU, 2 GELU (by the
+ * error function), 3 SiLU. keep [M, N] (row stride ldk; NULL: none) receives what the activation's
+ * slope is made of: the squared ReLU's value h = act(z), of which it is 2 sqrt(h) (slope_kind 2; without a
+ * residual C is h too), of the others the derivative (slope_kind 1), with bf16 operands in fp16.
+ * slope [M, N] is such a matrix. Large fp32 products multiply three bf16 planes of each operand,
+ * which hold all bits from 2^-110 up. padA, padB: the operand's rows end in zeros up to a multiple
+ * of 8 columns; padC: C's are to. Row strides are below 2^21. Workspace:
+ * dabsn_hip_linear_workspace_bytes of the same call (its workspace may be unset), 16-byte aligned
+ * (0: none).
  * dabsn_hip_linear_slope: dz [rows, n] (row stride ldz; NULL: none) = grad * slope, its rows ending
  * in zeros up to a multiple of 8 columns where ldz has the room, and dbias [n]
  * (NULL: none) its column sums before the rounding. */
@@ -822,7 +824,7 @@ int dabsn_hip_linear_slope(int dtype, int64_t rows, int64_t n, const void* grad,
 /* dabsn_hip_mlp_fwd: out [M, H] = x + act(norm(x) w1^T + b1) w2^T + b2 by the calls above, x with row
  * stride ldx, w1 [F, H], w2 [H, F] (row strides ldw1, ldw2). normed [M, H], stats [M][2] and h
  * [M, ldh >= F rounded up to 8], the activated inner rows, are kept for the backward where given;
- * keep [M, ldk], the activation's slope, is for GELU and SiLU. _bwd: the gradients that are asked
+ * keep [M, ldk], the activation's derivative, is for GELU and SiLU. _bwd: the gradients that are asked
  * for (not NULL) from grad [M, H] and these; dx holds the sum of both branches. Workspace:
  * dabsn_hip_mlp_workspace_bytes of the same call (its workspace may be unset), 16-byte aligned. */
 typedef struct dabsn_mlp_call {

@@ -181,14 +181,19 @@ def activated(z: Val, act: str):
             Val(s * (1 + v * (1 - s)), 0.5 * e + 16 * U * s * (1 + v.abs() * (1 - s))))
 
 
-def kept(slope: Val, h: Val, act: str, dtype, residual: bool):
+def kept(slope: Val, h: Val, act: str, dtype):
     """The slope as the backward has it."""
-    if act == "relu2" and not residual:
+    if act == "relu2":
         # From the rounded output: the root halves its relative error; small outputs by their own.
         h = h.rounded(dtype)
         low = 2 * (h.v - h.e).clamp(min=0).sqrt()
         high = 2 * (h.v + h.e).sqrt()
         return Val(slope.v, torch.maximum(high - slope.v, slope.v - low) + 4 * U * high)
+    if act != "none" and dtype == BF16:
+        # In fp16. GELU's distribution function is a fit there, whose tail, at most 1/2, is off by
+        # 1.7e-5 of itself: 8.5e-6, which the slope p(z) + z p'(z) has whole where it passes 0.
+        fit = 8.5e-6 if act == "gelu" else 0.0
+        return Val(slope.v, slope.e + fit + 2.0 ** -11 * (slope.v.abs() + slope.e + fit) + 2.0 ** -25)
     return slope if act == "none" else slope.rounded(dtype)
 
 
@@ -230,7 +235,7 @@ def check_linear(t, act, got):
     check("out", got["out"], h + (Val(t["residual"]) if res else None), dtype, k)
     if len(got) == 1:
         return
-    exact = g * kept(slope, h, act, dtype, res)
+    exact = g * kept(slope, h, act, dtype)
     dz = exact if act == "none" else exact.rounded(dtype)
     check("x", got["x"], dz @ w, dtype, k + n)
     check("weight", got["weight"], dz.t() @ x, dtype, k + m)
@@ -261,6 +266,60 @@ def test_linear(cuda_device, m, k, n, act, bias, residual, dtype):
     with torch.no_grad():
         plain = fused_linear(t["x"], t["weight"], t["bias"], activation=act, residual=t["residual"])
     assert torch.equal(plain, got["out"])
+
+
+# Sizes whose products take the large tiles, with splits and without, in each direction: 256 x 256
+# (the first two in all three, of either type; the second split in the forward), 128 x 64 (third and
+# fifth, bf16 forward), 128 x 128 (of fp32 planes, the third's weight gradient; of fp32 as it lies,
+# the fourth's forward and gradient of the rows and the sixth's weight gradient), and many splits.
+LARGE = [(4001, 4010, 3999), (2049, 9001, 2050), (300, 5000, 4100), (5000, 300, 700),
+         (515, 6000, 3000), (9000, 200, 2000), (5000, 700, 300), (300, 264, 33000), (20, 50000, 100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("act,bias,residual", [("relu2", False, False), ("gelu", True, True)])
+@pytest.mark.parametrize("m,k,n", LARGE)
+def test_linear_large(cuda_device, m, k, n, act, bias, residual, dtype):
+    t = tensors(m + k + n, m, k, n, dtype, bias, residual)
+    check_linear(t, act, run(t, act))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_linear_large_strides(cuda_device, dtype):
+    """256 x 256 tiles whose edges end inside wider arrays of NaN, at odd offsets; the results of
+    contiguous operands, bit for bit where the same tiles take them."""
+    m, k, n = 4001, 1000, 3999
+    t = tensors(1, m, k, n, dtype, True, True)
+    wide = {a: torch.full((v.shape[0], v.shape[1] + 5), math.nan, device=v.device, dtype=dtype)
+            for a, v in t.items() if v.dim() == 2}
+    for a, v in wide.items():
+        v[:, 3:-2] = t[a]
+    view = {**t, **{a: v[:, 3:-2] for a, v in wide.items()}}
+    leaves = {a: view[a].requires_grad_(True) for a in ("x", "weight", "residual")}
+    out = fused_linear(leaves["x"], leaves["weight"], t["bias"], activation="silu", residual=leaves["residual"])
+    gx, gw, gr = torch.autograd.grad(out, tuple(leaves.values()), view["grad"])
+    got = {"out": out.detach(), "x": gx, "weight": gw, "residual": gr}
+    check_linear({**t, "bias": t["bias"]}, "silu", {**got, "bias": run(t, "silu")["bias"]})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("m,k,n", [(1, 8, 300), (5, 1000, 1001), (16, 4104, 16), (9, 33, 5000), (4, 50000, 70)])
+def test_linear_few_rows_at_any_offset(cuda_device, m, k, n, dtype):
+    """Up to 16 rows, operands and results at every offset modulo eight values."""
+    t = tensors(m + n, m, k, n, dtype, True, True)
+    want = fused_linear(t["x"], t["weight"], t["bias"], activation="gelu", residual=t["residual"])
+    check_linear(t, "gelu", {"out": want})
+    for off in (1, 2, 3, 5, 8):
+        place = {}
+        for a in ("x", "weight", "residual"):
+            wide = torch.full((t[a].shape[0], t[a].shape[1] + off + 4), math.nan, device="cuda", dtype=dtype)
+            wide[:, off:off + t[a].shape[1]] = t[a]
+            place[a] = wide[:, off:off + t[a].shape[1]]
+        got = fused_linear(place["x"], place["weight"], t["bias"], activation="gelu", residual=place["residual"])
+        check_linear(t, "gelu", {"out": got})
 
 
 @pytest.mark.gpu
@@ -369,7 +428,7 @@ def test_activations_over_their_range(cuda_device, act, dtype):
     # is |z| 2^-126 of a product with z.
     low = (1 + z.abs()) * 2.0 ** -126
     within(out, h.v, (r + 400 * U) * h.v.abs() + low)
-    within(dx, slope.v, kept(slope, h, act, dtype, False).e + (r + 400 * U) * slope.v.abs() + low)
+    within(dx, slope.v, kept(slope, h, act, dtype).e + (r + 400 * U) * slope.v.abs() + low)
 
 
 @pytest.mark.gpu
@@ -447,7 +506,7 @@ def check_mlp(t, act, layer, got):
     f, width = t["w1"].shape
     check("out", got["out"], out, dtype, f + width)
     g = Val(t["grad"])
-    dz = ((g @ w2) * kept(slope, h, act, dtype, False)).rounded(dtype)
+    dz = ((g @ w2) * kept(slope, h, act, dtype)).rounded(dtype)
     dn = (dz @ w1).rounded(dtype)
     gw = dn * nw
     level = Val(gw.v.mean(1, keepdim=True), gw.e.mean(1, keepdim=True) + D * U * gw.v.abs().mean(1, keepdim=True))
@@ -489,6 +548,16 @@ def test_mlp(cuda_device, m, h, f, act, layer, bias, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("act,layer", [("relu2", False), ("gelu", True)])
+@pytest.mark.parametrize("m,h,f", [(4001, 1000, 3999), (300, 2048, 4100), (6000, 256, 1024)])
+def test_mlp_large(cuda_device, m, h, f, act, layer, dtype):
+    """The slopes in the epilogues of the large tiles."""
+    t = mlp_tensors(m, m, h, f, dtype, layer, True)
+    check_mlp(t, act, layer, run_mlp(t, act, layer))
+
+
+@pytest.mark.gpu
 def test_mlp_is_its_parts(cuda_device):
     """The MLP's forward is the norm and two products of the public operators, bit for bit."""
     t = mlp_tensors(3, 90, 72, 200, BF16, True, True)
@@ -522,6 +591,31 @@ def test_mlp_each_gradient_alone_and_shapes(cuda_device):
     assert float((got.double() - exact).abs().max()) < 1e-4
     none = fused_mlp(t["x"][:0], t["w1"], t["w2"])
     assert none.shape == (0, 40)
+    empty = run_mlp({**t, "x": t["x"][:0], "grad": t["grad"][:0]}, "gelu", True)
+    assert empty["x"].shape == (0, 40) and all(float(empty[a].abs().sum()) == 0 for a in NAMES)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("m", [3, 130])
+def test_mlp_strides(cuda_device, m, dtype):
+    """Rows and weights inside wider arrays of NaN, transposed weights, a gradient from expand."""
+    t = mlp_tensors(7, m, 40, 84, dtype, True, True)
+    want = run_mlp({**t, "grad": t["grad"][:1].expand(m, 40).contiguous()}, "silu", True)
+    views = {}
+    for a in ("x", "w1", "w2"):
+        wide = torch.full((t[a].shape[0], t[a].shape[1] + 7), math.nan, device="cuda", dtype=dtype)
+        wide[:, 3:-4] = t[a]
+        views[a] = wide[:, 3:-4]
+    for w1 in (views["w1"], t["w1"].t().contiguous().t()):
+        leaves = {**t, **views, "w1": w1}
+        leaves = {a: leaves[a].requires_grad_(True) if a in ("x", "w1", "w2") else t[a] for a in NAMES}
+        out = fused_mlp(leaves["x"], leaves["w1"], leaves["w2"], t["b1"], t["b2"], norm="layer",
+                        norm_weight=t["norm_weight"], norm_bias=t["norm_bias"], activation="silu")
+        assert torch.equal(out, want["out"])
+        grads = torch.autograd.grad(out, [leaves[a] for a in ("x", "w1", "w2")], t["grad"][:1].expand(m, 40))
+        for a, got in zip(("x", "w1", "w2"), grads):
+            assert got.shape == t[a].shape and torch.equal(got, want[a]), a
 
 
 @pytest.mark.gpu
