@@ -69,17 +69,25 @@ class LinearCall(ctypes.Structure):
                 + [(n, vp) for n in ("C", "keep", "workspace")] + [("workspace_bytes", sz)])
 
 
+class LinearGradsCall(ctypes.Structure):
+    """Mirror of ``dabsn_linear_grads_call``."""
+
+    _fields_ = ([(n, i32) for n in ("dtype", "slope_kind")] + [(n, i64) for n in ("M", "N", "K")]
+                + [(n, vp) for n in ("x", "w", "grad", "slope")]
+                + [(n, i64) for n in ("ldx", "ldw", "ldg", "lds")]
+                + [(n, vp) for n in ("dx", "dw", "db", "workspace")] + [("workspace_bytes", sz)])
+
+
 class MlpCall(ctypes.Structure):
     """Mirror of ``dabsn_mlp_call``."""
 
-    _fields_ = ([(n, i32) for n in ("dtype", "wdtype", "layer", "act")]
-                + [(n, i64) for n in ("M", "H", "F")]
+    _fields_ = ([(n, i32) for n in ("dtype", "wdtype", "layer", "act", "train")]
+                + [("eps", ctypes.c_float)] + [(n, i64) for n in ("M", "H", "F")]
                 + [(n, vp) for n in ("x", "norm_weight", "norm_bias", "w1", "b1", "w2", "b2", "grad")]
-                + [(n, i64) for n in ("ldx", "ldw1", "ldw2", "ldh", "ldk")]
-                + [("eps", ctypes.c_float)]
-                + [(n, vp) for n in ("normed", "h", "keep", "out", "stats", "dx", "dnorm_weight",
-                                     "dnorm_bias", "dw1", "db1", "dw2", "db2", "workspace")]
-                + [("workspace_bytes", sz)])
+                + [(n, i64) for n in ("ldx", "ldw1", "ldw2")]
+                + [(n, vp) for n in ("out", "dx", "dnorm_weight", "dnorm_bias", "dw1", "db1", "dw2",
+                                     "db2", "saved", "workspace")]
+                + [(n, sz) for n in ("saved_bytes", "workspace_bytes")])
 
 
 _SIGNATURES = {
@@ -220,7 +228,9 @@ _SIGNATURES = {
         [i32, i32, i32, i64, i64, vp, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp, sz, vp], i32),
     "dabsn_hip_linear_workspace_bytes": ([ctypes.POINTER(LinearCall)], sz),
     "dabsn_hip_linear": ([ctypes.POINTER(LinearCall), vp], i32),
-    "dabsn_hip_mlp_workspace_bytes": ([ctypes.POINTER(MlpCall), i32], sz),
+    "dabsn_hip_linear_grads_workspace_bytes": ([ctypes.POINTER(LinearGradsCall)], sz),
+    "dabsn_hip_linear_grads": ([ctypes.POINTER(LinearGradsCall), vp], i32),
+    "dabsn_hip_mlp_plan": ([ctypes.POINTER(MlpCall), i32], i32),
     "dabsn_hip_mlp_fwd": ([ctypes.POINTER(MlpCall), vp], i32),
     "dabsn_hip_mlp_bwd": ([ctypes.POINTER(MlpCall), vp], i32),
     "dabsn_hip_linear_slope_workspace_bytes": ([i32, i64, i64], sz),

@@ -14,7 +14,7 @@ from .vocab import need_device, need_float, on, row_stride, rows_of, stream  # n
 
 ACTIVATIONS = {"none": 0, "relu2": 1, "gelu": 2, "silu": 3}
 MAX_WIDTH = 16384
-_STORED, _FROM_SQUARE = 1, 2
+STORED, FROM_SQUARE = 1, 2
 
 
 def once(backward):
@@ -84,8 +84,8 @@ def norm(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float, laye
 
 
 def norm_backward(x: Tensor, weight: Tensor | None, stats: Tensor, g: Tensor, layer: bool,
-                  add: Tensor | None, dtype: torch.dtype, need_weight: bool, need_bias: bool):
-    """(dx [+ add], dweight, dbias); ``dtype`` is that of weight and bias."""
+                  dtype: torch.dtype, need_weight: bool, need_bias: bool):
+    """(dx, dweight, dbias); ``dtype`` is that of weight and bias."""
     lib, (rows, h) = _lib.load(), x.shape
     dx = x.new_empty((rows, h))
     dw = x.new_empty(h, dtype=dtype) if need_weight else None
@@ -96,7 +96,7 @@ def norm_backward(x: Tensor, weight: Tensor | None, stats: Tensor, g: Tensor, la
     tk = ops.KernelTimer.begin("norm_bwd", x)
     _lib.check(lib.dabsn_hip_norm_bwd(
         ops._code(x.dtype), ops._code(dtype), layer, rows, h, x.data_ptr(), row_stride(x),
-        ops._p(weight), stats.data_ptr(), g.data_ptr(), row_stride(g), ops._p(add), dx.data_ptr(),
+        ops._p(weight), stats.data_ptr(), g.data_ptr(), row_stride(g), None, dx.data_ptr(),
         ops._p(dw), ops._p(db), ops._p(ws), nbytes, stream(x)), "norm backward")
     ops.KernelTimer.end(tk)
     return dx, dw, db
@@ -108,23 +108,16 @@ def padded(rows: int, n: int, like: Tensor) -> Tensor:
     return like.new_empty((rows, ld))[:, :n]
 
 
-def product(a: Tensor, b: Tensor, *, trans_a: bool = False, trans_b: bool = False,
-            bias: Tensor | None = None, act: int = 0, keep: Tensor | None = None,
-            slope: Tensor | None = None, slope_kind: int = 0, residual: Tensor | None = None,
-            out: Tensor | None = None, pad_a: bool = False, pad_out: bool = False) -> Tensor:
-    """act(a b^T + bias) * slope + residual (see ``dabsn_hip_linear``). a [M, K], or [K, M] with
-    ``trans_a``; b [N, K], or [K, N] with ``trans_b``. ``pad_a``: a is a ``padded`` buffer that this
-    module filled; ``pad_out``: out is to be one."""
-    lib = _lib.load()
-    k, m = a.shape if trans_a else a.shape[::-1]
-    n = b.shape[1] if trans_b else b.shape[0]
-    if out is None:
-        out = padded(m, n, a) if pad_out else a.new_empty((m, n))
+def product(a: Tensor, b: Tensor, bias: Tensor | None = None, act: int = 0,
+            keep: Tensor | None = None, residual: Tensor | None = None) -> Tensor:
+    """act(a b^T + bias) + residual (see ``dabsn_hip_linear``) of a [M, K] and b [N, K]."""
+    lib, (m, k), n = _lib.load(), a.shape, b.shape[0]
+    out = a.new_empty((m, n))
     p, ld = ops._p, lambda t: 0 if t is None else row_stride(t)  # noqa: E731
     call = _lib.LinearCall(
-        ops._code(a.dtype), trans_a, trans_b, pad_a, False, pad_out, act, slope_kind, m, n, k,
-        a.data_ptr(), b.data_ptr(), p(bias), p(slope), p(residual), row_stride(a), row_stride(b),
-        ld(slope), ld(residual), row_stride(out), ld(keep), out.data_ptr(), p(keep))
+        ops._code(a.dtype), 0, 0, 0, 0, 0, act, 0, m, n, k, a.data_ptr(), b.data_ptr(), p(bias),
+        None, p(residual), row_stride(a), row_stride(b), 0, ld(residual), n, ld(keep),
+        out.data_ptr(), p(keep))
     nbytes = lib.dabsn_hip_linear_workspace_bytes(call)
     if nbytes:
         ws = a.new_empty(nbytes, dtype=torch.uint8)
@@ -135,22 +128,65 @@ def product(a: Tensor, b: Tensor, *, trans_a: bool = False, trans_b: bool = Fals
     return out
 
 
-def slope_product(g: Tensor, slope: Tensor | None, slope_kind: int, need_rows: bool,
-                  need_sums: bool) -> tuple[Tensor, Tensor | None]:
-    """(g * slope, its column sums or None); g itself without a slope."""
-    lib, (rows, n) = _lib.load(), g.shape
-    code = ops._code(g.dtype)
-    dz = padded(rows, n, g) if need_rows and slope is not None else None
-    sums = g.new_empty(n) if need_sums else None
-    if dz is None and sums is None:
-        return g, None
-    nbytes = lib.dabsn_hip_linear_slope_workspace_bytes(code, rows, n) if need_sums else 0
-    ws = g.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    tk = ops.KernelTimer.begin("linear_slope", g)
-    _lib.check(lib.dabsn_hip_linear_slope(
-        code, rows, n, g.data_ptr(), row_stride(g), ops._p(slope),
-        0 if slope is None else row_stride(slope), slope_kind, ops._p(dz),
-        0 if dz is None else row_stride(dz), ops._p(sums), ops._p(ws), nbytes, stream(g)),
-        "linear slope")
+def product_backward(x: Tensor, w: Tensor, g: Tensor, slope: Tensor | None, slope_kind: int, need):
+    """Gradients (None where not needed) of x, w and bias from g [M, N] of ``product`` without
+    residual; ``slope`` is what was kept."""
+    lib, (m, k), n, p = _lib.load(), x.shape, w.shape[0], ops._p
+    dx = x.new_empty((m, k)) if need[0] else None
+    dw = x.new_empty((n, k)) if need[1] else None
+    db = x.new_empty(n) if need[2] else None
+    call = _lib.LinearGradsCall(
+        ops._code(x.dtype), slope_kind, m, n, k, x.data_ptr(), w.data_ptr(), g.data_ptr(), p(slope),
+        row_stride(x), row_stride(w), row_stride(g), 0 if slope is None else row_stride(slope),
+        p(dx), p(dw), p(db))
+    nbytes = lib.dabsn_hip_linear_grads_workspace_bytes(call)
+    if nbytes:
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        call.workspace, call.workspace_bytes = ws.data_ptr(), nbytes
+    tk = ops.KernelTimer.begin("linear_bwd", x)
+    _lib.check(lib.dabsn_hip_linear_grads(call, stream(x)), "linear backward")
     ops.KernelTimer.end(tk)
-    return g if dz is None else dz, sums
+    return dx, dw, db
+
+
+def mlp(x: Tensor, leaves, act: int, layer: bool, eps: float, train: bool):
+    """(out, what the backward needs or None) of x [M, H] and leaves, norm weight and bias, w1, b1,
+    w2, b2 (see ``dabsn_hip_mlp_fwd``)."""
+    lib, out = _lib.load(), x.new_empty(x.shape)
+    call = _mlp_call(x, leaves, act, layer, eps, train)
+    call.out = out.data_ptr()
+    _lib.check(lib.dabsn_hip_mlp_plan(call, 0), "mlp")
+    saved = x.new_empty(call.saved_bytes, dtype=torch.uint8) if train else None
+    call.saved = ops._p(saved)
+    ws = x.new_empty(call.workspace_bytes, dtype=torch.uint8)
+    call.workspace = ws.data_ptr()
+    tk = ops.KernelTimer.begin("mlp", x)
+    _lib.check(lib.dabsn_hip_mlp_fwd(call, stream(x)), "mlp")
+    ops.KernelTimer.end(tk)
+    return out, saved
+
+
+def mlp_backward(x: Tensor, leaves, saved: Tensor, g: Tensor, act: int, layer: bool, eps: float, need):
+    """Gradients (None where not needed) of x and the leaves from g [M, H], contiguous."""
+    lib, p = _lib.load(), ops._p
+    grads = [t.new_empty(t.shape) if n else None for t, n in zip((x, *leaves), need)]
+    call = _mlp_call(x, leaves, act, layer, eps, True)
+    call.grad, call.saved = g.data_ptr(), saved.data_ptr()
+    (call.dx, call.dnorm_weight, call.dnorm_bias, call.dw1, call.db1, call.dw2,
+     call.db2) = map(p, grads)
+    _lib.check(lib.dabsn_hip_mlp_plan(call, 1), "mlp backward")
+    ws = x.new_empty(call.workspace_bytes, dtype=torch.uint8)
+    call.workspace = ws.data_ptr()
+    tk = ops.KernelTimer.begin("mlp_bwd", x)
+    _lib.check(lib.dabsn_hip_mlp_bwd(call, stream(x)), "mlp backward")
+    ops.KernelTimer.end(tk)
+    return grads
+
+
+def _mlp_call(x, leaves, act, layer, eps, train) -> _lib.MlpCall:
+    nw, nb, w1, b1, w2, b2 = leaves
+    p, vector = ops._p, nw if nw is not None else nb if nb is not None else x
+    return _lib.MlpCall(
+        ops._code(x.dtype), ops._code(vector.dtype), layer, act, train, eps, x.shape[0], x.shape[1],
+        w1.shape[0], x.data_ptr(), p(nw), p(nb), w1.data_ptr(), p(b1), w2.data_ptr(), p(b2), None,
+        row_stride(x), row_stride(w1), row_stride(w2))

@@ -18,8 +18,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import _lib
-from .kernels import dense, ops
+from .kernels import dense
 from .norm import layer_norm, rms_norm
 
 _RELU2 = dense.ACTIVATIONS["relu2"]
@@ -43,18 +42,17 @@ def _keeps(x: Tensor, n: int, act: int, residual: bool):
     """(buffer for what the slope is made of or None, its kind) of an activated product's forward in
     training. The squared ReLU's output is at hand where no residual is added to it."""
     if act == 0 or (act == _RELU2 and not residual):
-        return None, dense._FROM_SQUARE if act else 0
-    return dense.padded(x.shape[0], n, x), dense._FROM_SQUARE if act == _RELU2 else dense._STORED
+        return None, dense.FROM_SQUARE if act else 0
+    return dense.padded(x.shape[0], n, x), dense.FROM_SQUARE if act == _RELU2 else dense.STORED
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         with dense.on(x):
-            keep, kind = _keeps(x, weight.shape[0], act, residual is not None)
-            out = dense.product(x, weight, bias=bias, act=act, keep=keep, residual=residual)
-        ctx.save_for_backward(x, weight, out if kind and keep is None else keep)
-        ctx.kind = kind
+            keep, ctx.kind = _keeps(x, weight.shape[0], act, residual is not None)
+            out = dense.product(x, weight, bias, act, keep, residual)
+        ctx.save_for_backward(x, weight, out if ctx.kind and keep is None else keep)
         return out
 
     @staticmethod
@@ -62,15 +60,9 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, g):
         x, weight, slope = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx = dw = None
         with dense.on(x):
-            rows = dense.rows_of(g)
-            dz, db = dense.slope_product(rows, slope, ctx.kind, need[0] or need[1], need[2])
-            if need[0]:
-                dx = dense.product(dz, weight, trans_b=True, pad_a=dz is not rows)
-            if need[1]:
-                dw = dense.product(dz, x, trans_a=True, trans_b=True)
-        return dx, dw, db, g if need[3] else None, None
+            grads = dense.product_backward(x, weight, dense.rows_of(g), slope, ctx.kind, need)
+        return (*grads, g if need[3] else None, None)
 
 
 def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
@@ -105,68 +97,27 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
         out = _Linear.apply(rows, w, bias, res, act)
     else:
         with dense.on(x):
-            out = dense.product(rows, w, bias=bias, act=act, residual=res)
+            out = dense.product(rows, w, bias, act, None, res)
     return out if x.dim() == 2 else out.view(shape)
-
-
-def _mlp_call(x, nw, nb, w1, b1, w2, b2, act, layer, eps, out=None, grad=None) -> _lib.MlpCall:
-    p = ops._p
-    vector = nw if nw is not None else nb if nb is not None else x
-    return _lib.MlpCall(
-        ops._code(x.dtype), ops._code(vector.dtype), layer, act, x.shape[0], x.shape[1], w1.shape[0],
-        x.data_ptr(), p(nw), p(nb), w1.data_ptr(), p(b1), w2.data_ptr(), p(b2), p(grad),
-        dense.row_stride(x), dense.row_stride(w1), dense.row_stride(w2), 0, 0, eps, None, None, None,
-        p(out))
-
-
-def _run_mlp(call: _lib.MlpCall, x: Tensor, backward: bool) -> None:
-    lib = _lib.load()
-    nbytes = lib.dabsn_hip_mlp_workspace_bytes(call, backward)
-    if nbytes:
-        ws = x.new_empty(nbytes, dtype=torch.uint8)
-        call.workspace, call.workspace_bytes = ws.data_ptr(), nbytes
-    name = "mlp_bwd" if backward else "mlp"
-    tk = ops.KernelTimer.begin(name, x)
-    _lib.check((lib.dabsn_hip_mlp_bwd if backward else lib.dabsn_hip_mlp_fwd)(call, dense.stream(x)), name)
-    ops.KernelTimer.end(tk)
 
 
 class _MLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, nw, nb, w1, b1, w2, b2, act, layer, eps):
-        rows, f = x.shape[0], w1.shape[0]
+        leaves = nw, nb, w1, b1, w2, b2
         with dense.on(x):
-            out, normed = x.new_empty(x.shape), x.new_empty(x.shape)
-            stats = x.new_empty((rows, 2), dtype=torch.float32)
-            h = dense.padded(rows, f, x)
-            keep, _ = _keeps(x, f, act, False)
-            call = _mlp_call(x, nw, nb, w1, b1, w2, b2, act, layer, eps, out)
-            call.normed, call.stats = normed.data_ptr(), stats.data_ptr()
-            call.h, call.ldh = h.data_ptr(), dense.row_stride(h)
-            if keep is not None:
-                call.keep, call.ldk = keep.data_ptr(), dense.row_stride(keep)
-            _run_mlp(call, x, False)
-        ctx.save_for_backward(x, nw, nb, w1, b1, w2, b2, normed, stats, h, keep)
+            out, saved = dense.mlp(x, leaves, act, layer, eps, True)
+        ctx.save_for_backward(x, *leaves, saved)
         ctx.args = act, layer, eps
         return out
 
     @staticmethod
     @dense.once
     def backward(ctx, g):
-        x, nw, nb, w1, b1, w2, b2, normed, stats, h, keep = ctx.saved_tensors
+        x, *leaves, saved = ctx.saved_tensors
         with dense.on(x):
-            rows = dense.rows_of(g).contiguous()
-            leaves = x, nw, nb, w1, b1, w2, b2
-            grads = [t.new_empty(t.shape) if need else None
-                     for t, need in zip(leaves, ctx.needs_input_grad)]
-            call = _mlp_call(*leaves, *ctx.args, grad=rows)
-            call.normed, call.stats = normed.data_ptr(), stats.data_ptr()
-            call.h, call.ldh = h.data_ptr(), h.stride(0)
-            if keep is not None:
-                call.keep, call.ldk = keep.data_ptr(), keep.stride(0)
-            (call.dx, call.dnorm_weight, call.dnorm_bias, call.dw1, call.db1, call.dw2,
-             call.db2) = map(ops._p, grads)
-            _run_mlp(call, x, True)
+            grads = dense.mlp_backward(x, leaves, saved, dense.rows_of(g).contiguous(), *ctx.args,
+                                       ctx.needs_input_grad)
         return (*grads, None, None, None)
 
 
@@ -208,6 +159,5 @@ def fused_mlp(x: Tensor, w1: Tensor, w2: Tensor, b1: Tensor | None = None,
         out = _MLP.apply(*leaves, act, layer, eps)
     else:
         with dense.on(x):
-            out = rows.new_empty(rows.shape)
-            _run_mlp(_mlp_call(*leaves, act, layer, eps, out), rows, False)
+            out, _ = dense.mlp(rows, leaves[1:], act, layer, eps, False)
     return out if x.dim() == 2 else out.view(x.shape)

@@ -35,7 +35,7 @@ class _Norm(torch.autograd.Function):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         with dense.on(x):
-            dx, dw, db = dense.norm_backward(x, weight, stats, dense.rows_of(g), ctx.layer, None,
+            dx, dw, db = dense.norm_backward(x, weight, stats, dense.rows_of(g), ctx.layer,
                                              ctx.dtype if weight is None else weight.dtype, need[1],
                                              need[2])
         return dx, dw, db, None, None

@@ -821,25 +821,37 @@ int dabsn_hip_linear_slope(int dtype, int64_t rows, int64_t n, const void* grad,
                            void* dbias, void* workspace, size_t workspace_bytes,
                            hipStream_t stream);
 
+/* dabsn_hip_linear_grads: of C [M, N] = act(x w^T + bias), x [M, K] and w [N, K] with row strides ldx and
+ * ldw, the gradients that are asked for (not NULL; dx [M, K], dw [N, K], db [N]) from grad [M, N] (row
+ * stride ldg) and the slope (as above; NULL: no activation). N <= 2^21 - 8. Workspace as above. */
+typedef struct dabsn_linear_grads_call {
+  int dtype, slope_kind;
+  int64_t M, N, K;
+  const void *x, *w, *grad, *slope;
+  int64_t ldx, ldw, ldg, lds;
+  void *dx, *dw, *db, *workspace;
+  size_t workspace_bytes;
+} dabsn_linear_grads_call;
+
+size_t dabsn_hip_linear_grads_workspace_bytes(const dabsn_linear_grads_call* call);
+int dabsn_hip_linear_grads(const dabsn_linear_grads_call* call, hipStream_t stream);
+
 /* dabsn_hip_mlp_fwd: out [M, H] = x + act(norm(x) w1^T + b1) w2^T + b2 by the calls above, x with row
- * stride ldx, w1 [F, H], w2 [H, F] (row strides ldw1, ldw2). normed [M, H], stats [M][2] and h
- * [M, ldh >= F rounded up to 8], the activated inner rows, are kept for the backward where given;
- * keep [M, ldk], the activation's derivative, is for GELU and SiLU. _bwd: the gradients that are asked
- * for (not NULL) from grad [M, H] and these; dx holds the sum of both branches. Workspace:
- * dabsn_hip_mlp_workspace_bytes of the same call (its workspace may be unset), 16-byte aligned. */
+ * stride ldx, w1 [F, H], w2 [H, F] (row strides ldw1, ldw2); with train, what the backward needs is
+ * left in `saved`. _bwd: the gradients that are asked for (not NULL) from grad [M, H] and saved; dx
+ * holds the sum of both branches. _plan sets saved_bytes and workspace_bytes of a call that has all
+ * but these two buffers; both are 16-byte aligned. */
 typedef struct dabsn_mlp_call {
-  int dtype, wdtype, layer, act;
+  int dtype, wdtype, layer, act, train;
+  float eps;
   int64_t M, H, F;
   const void *x, *norm_weight, *norm_bias, *w1, *b1, *w2, *b2, *grad;
-  int64_t ldx, ldw1, ldw2, ldh, ldk;
-  float eps;
-  void *normed, *h, *keep, *out;
-  float* stats;
-  void *dx, *dnorm_weight, *dnorm_bias, *dw1, *db1, *dw2, *db2, *workspace;
-  size_t workspace_bytes;
+  int64_t ldx, ldw1, ldw2;
+  void *out, *dx, *dnorm_weight, *dnorm_bias, *dw1, *db1, *dw2, *db2, *saved, *workspace;
+  size_t saved_bytes, workspace_bytes;
 } dabsn_mlp_call;
 
-size_t dabsn_hip_mlp_workspace_bytes(const dabsn_mlp_call* call, int backward);
+int dabsn_hip_mlp_plan(dabsn_mlp_call* call, int backward);
 int dabsn_hip_mlp_fwd(const dabsn_mlp_call* call, hipStream_t stream);
 int dabsn_hip_mlp_bwd(const dabsn_mlp_call* call, hipStream_t stream);
 

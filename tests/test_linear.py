@@ -102,29 +102,50 @@ def test_library_refuses_bad_arguments_of_the_mlp_before_it_launches():
     from dabsn_amd import _lib
 
     lib, one = _lib.load(), 1 << 20
-    good = dict(dtype=1, wdtype=0, act=2, M=5, H=16, F=24, x=one, w1=one, w2=one, grad=one, ldx=16,
-                ldw1=16, ldw2=24, ldh=24, ldk=24, normed=one, h=one, keep=one, out=one, stats=one, dx=one)
+    good = dict(dtype=1, wdtype=0, act=2, train=1, M=5, H=16, F=24, x=one, w1=one, w2=one, grad=one,
+                ldx=16, ldw1=16, ldw2=24, out=one, dx=one, saved=one, workspace=one)
 
     def status(backward, **change):
         c = _lib.MlpCall(**{**good, **change})
-        if "workspace" not in change:
-            c.workspace = one
-            c.workspace_bytes = lib.dabsn_hip_mlp_workspace_bytes(ctypes.byref(c), backward)
+        lib.dabsn_hip_mlp_plan(ctypes.byref(c), backward)
+        for name in ("saved_bytes", "workspace_bytes"):
+            if name in change:
+                setattr(c, name, change[name])
         return (lib.dabsn_hip_mlp_bwd if backward else lib.dabsn_hip_mlp_fwd)(ctypes.byref(c), None)
 
     for backward in (0, 1):
         for bad in (dict(dtype=2), dict(M=-1), dict(M=1 << 31), dict(H=0), dict(H=16385), dict(F=0),
-                    dict(F=1 << 21), dict(act=4), dict(act=-1), dict(act=0), dict(ldx=15), dict(ldw1=15),
-                    dict(ldw2=23), dict(ldh=23), dict(F=20, ldh=23), dict(ldk=23), dict(x=None), dict(w1=None),
-                    dict(w2=None), dict(wdtype=3), dict(ldx=1 << 21)):
+                    dict(F=1 << 21), dict(act=4), dict(act=-1), dict(ldx=15), dict(ldw1=15),
+                    dict(ldw2=23), dict(x=None), dict(w1=None), dict(w2=None), dict(wdtype=3),
+                    dict(ldx=1 << 21), dict(ldw1=1 << 21), dict(ldw2=1 << 21), dict(saved=None),
+                    dict(saved=one + 8), dict(saved_bytes=8), dict(workspace=None, train=backward),
+                    dict(workspace=one + 8, train=backward), dict(workspace_bytes=8, train=backward)):
             assert status(backward, **bad) == -2, (backward, bad)
-    assert status(0, out=None) == -2 and status(0, normed=None, workspace=one, workspace_bytes=8) == -2
-    for bad in (dict(keep=None), dict(grad=None), dict(normed=None), dict(stats=None), dict(h=None),
-                dict(workspace=one, workspace_bytes=8), dict(workspace=None, workspace_bytes=1 << 30),
-                dict(workspace=one + 8, workspace_bytes=1 << 30)):
+    assert status(0, out=None) == -2
+    for bad in (dict(grad=None), dict(train=0)):
         assert status(1, **bad) == -2, bad
     assert lib.dabsn_hip_mlp_fwd(None, None) == -2 and lib.dabsn_hip_mlp_bwd(None, None) == -2
-    assert lib.dabsn_hip_mlp_workspace_bytes(None, 0) == 0
+    assert lib.dabsn_hip_mlp_plan(None, 0) == -2
+
+
+def test_library_refuses_bad_arguments_of_a_layers_gradients():
+    import ctypes
+
+    from dabsn_amd import _lib
+
+    lib, one = _lib.load(), 1 << 20
+    good = dict(dtype=1, slope_kind=1, M=40, N=24, K=16, x=one, w=one, grad=one, slope=one, ldx=16,
+                ldw=16, ldg=24, lds=24, dx=one, dw=one, db=one, workspace=one)
+    need = lib.dabsn_hip_linear_grads_workspace_bytes(ctypes.byref(_lib.LinearGradsCall(**good)))
+    assert need > 0 and lib.dabsn_hip_linear_grads_workspace_bytes(None) == 0
+    for bad in (dict(dtype=2), dict(M=-1), dict(M=1 << 31), dict(N=0), dict(N=1 << 21), dict(K=0),
+                dict(K=1 << 21), dict(ldx=15), dict(ldw=15), dict(ldg=23), dict(lds=23), dict(ldx=1 << 21),
+                dict(ldw=1 << 21), dict(ldg=1 << 21), dict(lds=1 << 21), dict(slope_kind=0),
+                dict(slope_kind=3), dict(x=None), dict(w=None), dict(grad=None), dict(workspace=None),
+                dict(workspace=one + 8), dict(workspace_bytes=need - 1)):
+        c = _lib.LinearGradsCall(**{**good, "workspace_bytes": need, **bad})
+        assert lib.dabsn_hip_linear_grads(ctypes.byref(c), None) == -2, bad
+    assert lib.dabsn_hip_linear_grads(None, None) == -2
 
 
 class Val:
