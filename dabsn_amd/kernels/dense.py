@@ -9,11 +9,12 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from . import ops
-from .vocab import need_device, need_float, on, row_stride, rows_of, stream  # noqa: F401
+from . import ops, vocab
+from .vocab import need_device, need_float, on, stream  # noqa: F401
 
 ACTIVATIONS = {"none": 0, "relu2": 1, "gelu": 2, "silu": 3}
-MAX_WIDTH = 16384
+MAX_WIDTH = 16384  # of a norm's rows
+MOST = 2 ** 21 - 8  # of a product's rows, and of the strides between them
 STORED, FROM_SQUARE = 1, 2
 
 
@@ -27,6 +28,17 @@ def once(backward):
         return backward(ctx, *grads)
 
     return run
+
+
+def rows_of(x: Tensor) -> Tensor:
+    """x [..., K] as [rows, K] with unit column stride and a row stride that the products take."""
+    x = vocab.rows_of(x)
+    return x.contiguous() if row_stride(x) > MOST >= x.shape[1] else x
+
+
+def row_stride(x: Tensor) -> int:
+    """The row stride of ``rows_of``'s result (a lone row's stride says nothing)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def need_activation(what: str, name: str) -> int:

@@ -33,6 +33,8 @@ def _cast(*tensors: Tensor | None):
 def _weight(what: str, name: str, w: Tensor, x: Tensor, width: int) -> Tensor:
     if w.dim() != 2 or w.shape[1] != width or 0 in w.shape:
         raise ValueError(f"{what}: {name} {tuple(w.shape)} does not match width {width}")
+    if w.shape[0] > dense.MOST or width > dense.MOST:
+        raise ValueError(f"{what}: {name} {tuple(w.shape)} has over {dense.MOST} rows or columns")
     if w.dtype != x.dtype:
         raise TypeError(f"{what}: {name} must be {x.dtype} as x is, not {w.dtype}")
     return dense.rows_of(w)

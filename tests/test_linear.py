@@ -61,6 +61,14 @@ def test_refusals(call, error, match):
         call()
 
 
+def test_products_refuse_more_columns_than_they_take():
+    w = torch.empty(1 << 21, 1)
+    for call in (lambda: fused_linear(torch.empty(2, 1), w), lambda: fused_linear(torch.empty(2, 1 << 21), w.t()),
+                 lambda: fused_mlp(torch.empty(2, 1), w, w.t())):
+        with pytest.raises(ValueError, match="rows or columns"):
+            call()
+
+
 def test_library_refuses_bad_arguments_before_it_launches():
     from dabsn_amd import _lib
 
@@ -576,6 +584,43 @@ def test_mlp_large(cuda_device, m, h, f, act, layer, dtype):
     """The slopes in the epilogues of the large tiles."""
     t = mlp_tensors(m, m, h, f, dtype, layer, True)
     check_mlp(t, act, layer, run_mlp(t, act, layer))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("m,h,f", [(5, 24, 61), (33, 130, 65), (130, 77, 331), (700, 1001, 777)])
+def test_buffers_start_as_they_like(cuda_device, m, h, f, dtype):
+    """Workspaces and results whose memory holds NaN before the call."""
+    def poison():
+        junk = [torch.full((1 << s,), math.nan, device="cuda") for s in range(8, 24)]
+        junk += [torch.full((1 << 23,), math.nan, device="cuda") for _ in range(6)]
+        torch.cuda.synchronize()
+
+    t = mlp_tensors(m, m, h, f, dtype, True, True)
+    lin = tensors(m, m, h, f, dtype, True, True)
+    for act in ("relu2", "gelu"):
+        poison()
+        check_mlp(t, act, True, run_mlp(t, act, True))
+        poison()
+        check_linear(lin, act, run(lin, act))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_row_strides_beyond_the_kernels(cuda_device, dtype):
+    """Rows further apart than the products take are copied: an operand, a weight and a gradient."""
+    t = tensors(3, 20, 40, 24, dtype, True, False)
+    want = run(t, "silu")
+    wide = {a: torch.empty(t[a].shape[0], (1 << 21) + 8, device="cuda", dtype=dtype) for a in ("x", "weight", "grad")}
+    for a, v in wide.items():
+        v[:, 8:8 + t[a].shape[1]] = t[a]
+        wide[a] = v[:, 8:8 + t[a].shape[1]]
+    x, w = wide["x"].requires_grad_(True), wide["weight"].requires_grad_(True)
+    out = fused_linear(x, w, t["bias"], activation="silu")
+    gx, gw = torch.autograd.grad(out, (x, w), wide["grad"])
+    assert torch.equal(out, want["out"]) and torch.equal(gx, want["x"]) and torch.equal(gw, want["weight"])
+    one = fused_linear(wide["x"].detach()[:1], t["weight"], t["bias"], activation="silu")
+    assert torch.equal(one, fused_linear(t["x"][:1], t["weight"], t["bias"], activation="silu"))
 
 
 @pytest.mark.gpu
