@@ -2,7 +2,7 @@
 // norm.hip and linear.hip one after the other, with what lies between them in the caller's workspace.
 // One call from the host instead of three to nine, and one buffer for all that the backward needs,
 // which is what small steps wait for (2048 x 256 x 1024 fp32, forward and backward: 235 us with a
-// call and a tensor each, 181 so, of which 139 are kernels).
+// call and a tensor each, 181 so, of which 136 are kernels).
 //
 // Rounded to bf16 on the way, where the operands are bf16, is what the matrix cores read: the normed
 // rows, h and dz, and dn, whose bytes the norm's backward is bound by. (Weights' gradients of the
