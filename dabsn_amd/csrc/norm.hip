@@ -7,7 +7,8 @@
 // HBM bound: the forward reads a row and writes one, the backward reads two and writes one. A
 // row is held in the registers of T threads (64: a wave, four rows a workgroup; 256 or 1024: a
 // workgroup), NV vectors of 16 bytes each, so that the mean, the squares around it and the
-// result come from one reading. Sums are fp32: a thread's, then a wave's, then the workgroup's.
+// result come from one reading: 65536 x 4096 bf16 in 211 us, backward 312 to 322 (5.1 and 5.0 TB/s; a
+// copy reaches 5.2; 332 and 534 before the next row was loaded ahead). Sums are fp32: a thread's, then a wave's, then the workgroup's.
 //
 // The backward's workgroups walk over the rows with a column's dw and db in the registers of the
 // thread that holds the column, and leave one partial row each; join_kernel adds these in order.
