@@ -245,6 +245,8 @@ static int run(const dabsn_linear_call& c, const Plan& p, hipStream_t s) {
   a.ldr = c.slope ? c.lds : c.ldr;
   a.C = (E*)c.C; a.ldc = c.ldc; a.keep = (E*)c.keep; a.ldk = c.ldk; a.padC = c.padC;
   a.mt = p.mt; a.nt = p.nt; a.splits = c.K ? p.splits : 0; a.kper = p.kper; a.ldp = p.ldp;
+  a.wholeA = (const E*)c.A; a.wholelda = c.lda;
+  a.wholeB = (const E*)c.B; a.wholeldb = c.ldb;
   a.parts = p.splits > 1 ? (float*)(ws + p.atParts) : nullptr;
   if (c.K) {
     Operand<E> pa = {}, pb = {};

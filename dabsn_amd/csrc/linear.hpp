@@ -39,6 +39,8 @@ struct Args {
   int mt, nt, splits, kper;
   float* parts;  // [splits][M][ldp]: the splits' sums, instead of C
   int64_t ldp;
+  const E *wholeA, *wholeB;  // as they are
+  int64_t wholelda, wholeldb;
 };
 
 // act(z), and what is kept for its derivative: of the squared ReLU the value itself (before a residual;
@@ -358,7 +360,7 @@ template <typename E, int EPI, int TM, int TN, int BM, int BN, int NTH, bool PIN
 struct Epilogue {
   static constexpr int PLACES = TM * TN / 4;
   static constexpr bool WIDE = sizeof(E) == 2;
-  static constexpr int AHEAD = PIN ? (WIDE ? 16 : 12) : PLACES;
+  static constexpr int AHEAD = PIN ? (WIDE ? 16 : 10) : PLACES;
   static constexpr int FIRST = std::min(PLACES, PIN ? (WIDE ? 12 : 6) : WIDE ? 2 : 1);
   static constexpr bool FACTOR = EPI == kStored || EPI == kFromSquare;
   static constexpr bool ACTS = EPI == kRelu2 || EPI == kGelu || EPI == kSilu;
@@ -368,6 +370,7 @@ struct Epilogue {
   uint32_t column[TN / 2];             // in bytes from the tile's first
   Rows<E> besides;
   Eight<E> beside[AHEAD][2];
+  float marked = 0.0f;  // NaN once a sum is not finite
 
   __device__ __forceinline__ Epilogue(const Args<E>& args, int sp_, int m0_, int n0_, int wm_, int wn_, int tid)
       : a(args), sp(sp_), m0(m0_), n0(n0_), wm(wm_), wn(wn_), lane(tid & 63),
@@ -439,6 +442,10 @@ struct Epilogue {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = x[e / 4][b][e % 4];
+        if constexpr (!WIDE) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) marked = fmaf(v[e], 0.0f, marked);
+        }
         if constexpr (EPI == kShare) {
           Eight<float> all;
           all.set(v);
@@ -492,6 +499,52 @@ struct Epilogue {
 #pragma unroll 1
         for (int e = 0; e < 8; ++e)
           if (wm + r < rows) finish_one<E, EPI>(a, m0 + wm + r, n0 + rest + e, left[r * 8 + e]);
+    }
+  }
+  // Of planes' products: an infinity meets the other operand's smaller planes too, which may be 0 or
+  // of the other sign, and so leaves NaN where the product itself is infinite. Where a sum was not
+  // finite, results that are NaN are formed anew from the operands as they lie, k0 to k0 + len.
+  template <bool TA, bool TB>
+  __device__ __forceinline__ void mend(int k0, int len) {
+    if (!__any(marked != marked)) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const float *A = reinterpret_cast<const float*>(a.wholeA) + (TA ? k0 * a.wholelda + m0 : m0 * a.wholelda + k0);
+    const float *B = reinterpret_cast<const float*>(a.wholeB) + (TB ? k0 * a.wholeldb + n0 : n0 * a.wholeldb + k0);
+    const int64_t rowA = TA ? 1 : a.wholelda, rowB = TB ? 1 : a.wholeldb;
+    const int64_t stepA = TA ? a.wholelda : 1, stepB = TB ? a.wholeldb : 1;
+    // Rows of either operand that hold a NaN have nothing but NaN for results, and are left.
+    uint32_t nanB = 0;
+#pragma unroll 1
+    for (int c = wn + lane; c < min(wn + TN * 16, cols); c += 64)
+#pragma unroll 1
+      for (int k = 0; k < len; ++k) {
+        const float v = B[c * rowB + k * stepB];
+        if (v != v) nanB |= 1u << ((c - wn) / 64);
+      }
+#pragma unroll 1
+    for (int r = wm; r < min(wm + TM * 16, rows); ++r) {
+      bool nanA = false;
+#pragma unroll 1
+      for (int k = lane; k < len; k += 64) {
+        const float v = A[r * rowA + k * stepA];
+        nanA |= v != v;
+      }
+      if (__any(nanA)) continue;
+      const int64_t m = m0 + r;
+#pragma unroll 1
+      for (int c = wn + lane; c < min(wn + TN * 16, cols); c += 64) {
+        if (nanB >> ((c - wn) / 64) & 1) continue;
+        const int n = n0 + c;
+        float* at = EPI == kShare ? a.parts + (static_cast<int64_t>(sp) * a.M + m) * a.ldp + n
+                                  : reinterpret_cast<float*>(a.C) + m * a.ldc + n;
+        const float old = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (old == old) continue;
+        float s = 0.0f;
+#pragma unroll 1
+        for (int k = 0; k < len && s == s; ++k) s = fmaf(A[r * rowA + k * stepA], B[c * rowB + k * stepB], s);
+        if constexpr (EPI == kShare) *at = s;
+        else finish_one<E, EPI>(a, m, n, s);
+      }
     }
   }
 };
@@ -640,6 +693,7 @@ __global__ void __launch_bounds__(WM * WN * 64, BM * BN == 128 * 128 ? 2 : 1) pr
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   settle<PIN>();
   epilogue.end(acc, bias_lds, reinterpret_cast<float*>(lds) + wave * (BM / WM) * 8);
+  if constexpr (PAIRS > 1) epilogue.template mend<TA, TB>(k0, len);
 }
 
 // fp32 operands as they lie, at any alignment, by fp32 matrix instructions: where splitting them into

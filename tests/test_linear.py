@@ -439,6 +439,27 @@ def test_nan_and_infinity_stay_in_their_rows(cuda_device, m, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("m,k,n", [(40, 64, 40), (1500, 500, 4000), (4001, 1000, 3999), (2049, 9001, 2050)])
+def test_infinity_times_round_numbers(cuda_device, m, k, n, dtype):
+    """An infinity times weights that bf16 holds whole, or times 0, in products of every kind (the
+    third large, the last split): what each sum of products is in 64 bits, infinite or NaN."""
+    g = torch.Generator(device=cuda_device).manual_seed(m)
+    t = {"x": torch.randn(m, k, device=cuda_device, generator=g), "grad": torch.randn(m, n, device=cuda_device, generator=g),
+         "weight": torch.randint(-2, 3, (n, k), device=cuda_device, generator=g).float()}
+    t["x"][3, k - 1], t["x"][m - 1, 0], t["x"][7, 1], t["x"][7, 2] = math.inf, -math.inf, math.inf, -math.inf
+    t["grad"][5, n - 1], t["grad"][m - 2, 0], t["x"][9, 5] = -math.inf, math.inf, math.nan
+    t = {a: v.to(dtype) for a, v in t.items()}
+    got = run({**t, "bias": None, "residual": None}, "none")
+    x, w, d = (t[a].double() for a in ("x", "weight", "grad"))
+    for name, want in (("out", x @ w.t()), ("x", d @ w), ("weight", d.t() @ x)):
+        have = got[name].double()
+        assert torch.equal(torch.isnan(have), torch.isnan(want)), name
+        odd = torch.isinf(want)
+        assert torch.equal(have[odd], want[odd]) and torch.equal(torch.isinf(have), odd), name
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["relu2", "gelu", "silu"])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_activations_over_their_range(cuda_device, act, dtype):
