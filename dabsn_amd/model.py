@@ -63,6 +63,10 @@ class DABSNBlock(nn.Module):
     ``fused_mlp`` with that activation, ``relu2`` being the reference's; ``mlp_norm`` (``rms`` or
     ``layer``) and ``mlp_bias`` then choose its norm and give its products biases."""
 
+    # Blocks that were pickled whole before these choices existed have the reference's MLP.
+    mlp_activation: str | None = None
+    mlp_bias = False
+
     def __init__(self, input_dim: int, hidden_dim: int, state_dim: int, read_geometry: str = "seq",
                  *, residual: bool = False, mlp_ratio: float | None = None,
                  block_chunk_t: int | None = None, mlp_activation: str | None = None,
