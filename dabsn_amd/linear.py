@@ -75,10 +75,9 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
     added afterwards, as ``F.linear(...) + residual`` would."""
     what = "fused_linear"
     act = dense.need_activation(what, activation)
-    if torch.is_autocast_enabled("cuda"):
+    autocast = torch.is_autocast_enabled("cuda")
+    if autocast:
         x, weight, bias = _cast(x, weight, bias)
-        if residual is not None and residual.dtype != x.dtype:
-            return fused_linear(x, weight, bias, activation=activation) + residual
     dense.need_float(what, "x", x)
     if x.dim() < 1:
         raise ValueError(f"{what}: expected x [..., K]")
@@ -90,8 +89,12 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *,
         if residual.shape != shape:
             raise ValueError(f"{what}: residual {tuple(residual.shape)} does not match {shape}")
         if residual.dtype != x.dtype:
-            raise TypeError(f"{what}: residual must be {x.dtype} as x is, not {residual.dtype}")
+            if not autocast:
+                raise TypeError(f"{what}: residual must be {x.dtype} as x is, not {residual.dtype}")
+            dense.need_float(what, "residual", residual)
     dense.need_device(what, x, w, bias, residual)
+    if residual is not None and residual.dtype != x.dtype:
+        return fused_linear(x, w, bias, activation=activation) + residual
     rows = dense.rows_of(x)
     res = None if residual is None else dense.rows_of(residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
@@ -142,6 +145,8 @@ def fused_mlp(x: Tensor, w1: Tensor, w2: Tensor, b1: Tensor | None = None,
     if torch.is_autocast_enabled("cuda"):
         w1, w2, b1, b2 = _cast(w1, w2, b1, b2)
         if x.dtype != w1.dtype:
+            if w2.dim() == 2 and w2.shape[:1] != x.shape[-1:]:
+                raise ValueError(f"{what}: w2 {tuple(w2.shape)} does not lead back to x {tuple(x.shape)}")
             normed = (layer_norm(x, norm_weight, norm_bias, eps=eps) if layer
                       else rms_norm(x, norm_weight, eps=eps))
             return fused_linear(fused_linear(normed, w1, b1, activation=activation), w2, b2,
