@@ -14,6 +14,7 @@ import os
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from .. import _lib
 from . import ops
@@ -65,7 +66,11 @@ def once(backward):
 
 
 def need_device(what: str, *tensors: Tensor | None) -> None:
-    """All tensors on one ROCm device."""
+    """All tensors on one ROCm device, and none of them with a tangent: the calls that autograd does
+    not see would drop it without a word."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: DABSN HIP operators have no forward-mode derivatives")
     first = None
     for t in tensors:
         if t is None:
