@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
+from torch.nn.modules.module import _has_any_global_hook
 from torch.utils.checkpoint import checkpoint
 
 from .core import DABSNCore
@@ -55,13 +56,29 @@ def check_mlp(ratio: float | None, activation: str | None, norm: str, bias: bool
     need_activation("mlp_activation", activation)
 
 
+_ACTIVATIONS = {"none": lambda z: z, "relu2": lambda z: F.relu(z).square(), "gelu": F.gelu,
+                "silu": F.silu}
+
+
+def _as_made(module: nn.Module, *types: type) -> bool:
+    """Whether calling the module is its class's formula of its parameters: no hooks (which pruning and
+    sharding use too), no other ``forward``. (A parametrized module is: its class inherits it.)"""
+    hooks = (module._forward_hooks, module._forward_pre_hooks, module._backward_hooks,
+             module._backward_pre_hooks)
+    return (not any(hooks) and "forward" not in module.__dict__
+            and any(isinstance(module, t) and type(module).forward is t.forward for t in types)
+            and not _has_any_global_hook())
+
+
 class DABSNBlock(nn.Module):
     """One core plus admitted/permanent/induction/long read (seq, field or hybrid
     geometry).
 
     ``mlp_activation`` (None: the reference's MLP, operation by operation) runs the MLP through
     ``fused_mlp`` with that activation, ``relu2`` being the reference's; ``mlp_norm`` (``rms`` or
-    ``layer``) and ``mlp_bias`` then choose its norm and give its products biases."""
+    ``layer``) and ``mlp_bias`` then choose its norm and give its products biases. Where one of
+    ``mlp_norm``, ``mlp_fc1`` and ``mlp_fc2`` has hooks or has been replaced by a module with another
+    ``forward``, the three are called one by one instead."""
 
     # Blocks that were pickled whole before these choices existed have the reference's MLP.
     mlp_activation: str | None = None
@@ -184,6 +201,9 @@ class DABSNBlock(nn.Module):
             return hidden
         if self.mlp_activation is not None:
             norm, fc1, fc2 = self.mlp_norm, self.mlp_fc1, self.mlp_fc2
+            if not (_as_made(norm, MLPRMSNorm, nn.LayerNorm) and _as_made(fc1, nn.Linear)
+                    and _as_made(fc2, nn.Linear)):
+                return hidden + fc2(_ACTIVATIONS[self.mlp_activation](fc1(norm(hidden))))
             return fused_mlp(hidden, fc1.weight, fc2.weight, fc1.bias, fc2.bias,
                              norm="rms" if isinstance(norm, MLPRMSNorm) else "layer",
                              norm_weight=norm.weight, norm_bias=getattr(norm, "bias", None),

@@ -4,9 +4,27 @@ from __future__ import annotations
 
 import io
 
+import pytest
 import torch
+import torch.nn.functional as F
+from torch.nn.utils import parametrize, prune
 
 import dabsn_amd
+
+ACTS = {"none": lambda z: z, "relu2": lambda z: F.relu(z) ** 2, "gelu": F.gelu, "silu": F.silu}
+
+
+def _block(act, norm="layer", bias=True):
+    torch.manual_seed(0)
+    block = dabsn_amd.DABSNBlock(8, 8, 8, mlp_ratio=2.0, mlp_activation=act, mlp_norm=norm, mlp_bias=bias)
+    for p in (block.mlp_fc1, block.mlp_fc2, block.mlp_norm):
+        for q in p.parameters():
+            torch.nn.init.normal_(q)
+    return block
+
+
+def _parts(block, h, act):
+    return h + block.mlp_fc2(ACTS[act](block.mlp_fc1(block.mlp_norm(h))))
 
 
 def test_a_block_pickled_before_the_choices_existed_runs():
@@ -24,3 +42,85 @@ def test_a_block_pickled_before_the_choices_existed_runs():
     old = torch.load(file, weights_only=False)  # written above
     assert "mlp_activation" not in old.__dict__
     assert torch.equal(old.forward_mlp(h), want)
+
+
+@pytest.mark.parametrize("act,norm,bias", [("relu2", "rms", False), ("gelu", "layer", True), ("silu", "rms", True),
+                                           ("none", "layer", False)])
+@pytest.mark.parametrize("layer", ["mlp_norm", "mlp_fc1", "mlp_fc2"])
+def test_hooks_of_its_layers_run(layer, act, norm, bias):
+    block, h = _block(act, norm, bias), torch.randn(2, 3, 8)
+    handle = getattr(block, layer).register_forward_hook(lambda m, a, out: out + 1)
+    want = _parts(block, h, act)
+    assert torch.equal(block.forward_mlp(h), want)
+    with torch.no_grad():
+        assert torch.equal(block.forward_mlp(h), want)
+    handle.remove()
+    with pytest.raises(RuntimeError, match="device"):  # the fused call again
+        block.forward_mlp(h)
+    seen = []
+    for register in ("register_forward_pre_hook", "register_full_backward_hook",
+                     "register_full_backward_pre_hook"):
+        handle = getattr(getattr(block, layer), register)(lambda *a: seen.append(register))
+        block.forward_mlp(h.clone().requires_grad_(True)).sum().backward()
+        assert seen == [register]
+        seen.clear()
+        handle.remove()
+
+
+class Doubled(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+def test_replaced_and_pruned_layers_run():
+    block, h = _block("gelu"), torch.randn(2, 3, 8)
+    base = _parts(block, h, "gelu")
+    fc2 = block.mlp_fc2
+    block.mlp_fc2 = Doubled(16, 8)
+    block.mlp_fc2.load_state_dict(fc2.state_dict())
+    assert torch.allclose(block.forward_mlp(h), h + 2 * (base - h), atol=1e-5)
+    block.mlp_fc2 = torch.nn.Sequential(fc2)
+    assert torch.equal(block.forward_mlp(h), base)
+    block.mlp_fc2 = fc2
+    fc2.forward = lambda x: torch.zeros(2, 3, 8)
+    assert torch.equal(block.forward_mlp(h), h)
+    del fc2.forward
+    prune.random_unstructured(block.mlp_fc1, "weight", amount=0.5)
+    for _ in range(2):  # pruning forms the weight anew in each call
+        block.forward_mlp(h).sum().backward()
+    assert bool((block.mlp_fc1.weight_orig.grad[block.mlp_fc1.weight_mask == 0] == 0).all())
+
+
+def test_a_hook_for_all_modules_runs():
+    block, h, seen = _block("silu"), torch.randn(2, 3, 8), []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, a, out: seen.append(m))
+    try:
+        block.forward_mlp(h)
+    finally:
+        handle.remove()
+    assert seen == [block.mlp_norm, block.mlp_fc1, block.mlp_fc2]
+
+
+def test_a_parametrized_layer_is_fused():
+    class Half(torch.nn.Module):
+        def forward(self, w):
+            return w / 2
+
+    block = _block("silu")
+    parametrize.register_parametrization(block.mlp_fc1, "weight", Half())
+    with pytest.raises(RuntimeError, match="device"):
+        block.forward_mlp(torch.randn(2, 3, 8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,norm,bias", [("relu2", "rms", False), ("gelu", "layer", True), ("silu", "rms", True),
+                                           ("none", "layer", False)])
+def test_one_by_one_is_the_same_function(cuda_device, act, norm, bias):
+    """fp32 sums of at most 16 terms of order one on both sides: some 2^-20 of the values' 1 to 100."""
+    block, h = _block(act, norm, bias).cuda(), torch.randn(2, 3, 8, device=cuda_device)
+    fused = block.forward_mlp(h)
+    handle = block.mlp_fc1.register_forward_hook(lambda m, a, out: None)
+    parts = block.forward_mlp(h)
+    handle.remove()
+    assert not torch.equal(fused, h)
+    assert float((fused - parts).abs().max()) <= 1e-5 * float(parts.abs().max())
