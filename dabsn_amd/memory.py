@@ -266,7 +266,8 @@ def fingerprint_of(model: DABSNSequenceLM) -> dict[str, object]:
     scaled = {} if scale is None else {"embed_scale": scale}
     activation = getattr(model, "mlp_activation", None)
     if activation is not None:
-        scaled["mlp"] = f"{model.mlp_norm} {activation}{' bias' if model.mlp_bias else ''}"
+        norm, bias = getattr(model, "mlp_norm", "rms"), getattr(model, "mlp_bias", False)
+        scaled["mlp"] = f"{norm} {activation}{' bias' if bias else ''}"
     return {
         **scaled,
         "vocab": int(model.vocab),

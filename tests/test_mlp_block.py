@@ -10,6 +10,7 @@ import torch.nn.functional as F
 from torch.nn.utils import parametrize, prune
 
 import dabsn_amd
+from dabsn_amd import memory as mem
 
 ACTS = {"none": lambda z: z, "relu2": lambda z: F.relu(z) ** 2, "gelu": F.gelu, "silu": F.silu}
 
@@ -124,3 +125,22 @@ def test_one_by_one_is_the_same_function(cuda_device, act, norm, bias):
     handle.remove()
     assert not torch.equal(fused, h)
     assert float((fused - parts).abs().max()) <= 1e-5 * float(parts.abs().max())
+
+
+def _lm(**mlp):
+    torch.manual_seed(3)
+    return dabsn_amd.DABSNSequenceLM(40, 24, 2, residual=True, mlp_ratio=2.0, **mlp)
+
+
+def test_a_callers_model_that_names_its_activation_has_a_fingerprint():
+    model = _lm()
+
+    class Own:
+        mlp_activation = "gelu"
+
+        def __getattr__(self, name):
+            if name in ("mlp_norm", "mlp_bias"):
+                raise AttributeError(name)
+            return getattr(model, name)
+
+    assert mem.fingerprint_of(Own()) == {**mem.fingerprint_of(model), "mlp": "rms gelu"}
