@@ -261,7 +261,7 @@ class DABSNMemory:
 def fingerprint_of(model: DABSNSequenceLM) -> dict[str, object]:
     """Architecture identity a memory must match: the reference's dictionary, key for key
     (memory.py:149-161), so files cross-load in both directions; a scaled embedding and an MLP of
-    another kind, which the reference has not, add theirs."""
+    chosen kind, which the reference has not, add theirs."""
     scale = getattr(model, "embed_scale", None)
     scaled = {} if scale is None else {"embed_scale": scale}
     activation = getattr(model, "mlp_activation", None)
@@ -282,10 +282,15 @@ def fingerprint_of(model: DABSNSequenceLM) -> dict[str, object]:
     }
 
 
+#: The chosen kind that is the reference's MLP. Files do not name it, so that they cross-load with the
+#: reference's and with models that run the MLP operation by operation.
+_REFERENCE_MLP = "rms relu2"
+
+
 def _check_fingerprint(memory: DABSNMemory, model: DABSNSequenceLM) -> None:
     """The reference's rule (memory.py:164-181): an empty fingerprint passes; keys that
     predate residual/MLP support default to the disabled architecture; anything else must
-    equal the model's fingerprint."""
+    equal the model's fingerprint. A memory that names no kind of MLP is one of the reference's."""
     if not memory.fingerprint:
         return
     expected = fingerprint_of(model)
@@ -294,6 +299,8 @@ def _check_fingerprint(memory: DABSNMemory, model: DABSNSequenceLM) -> None:
     observed.setdefault("mlp_ratio", None)
     observed.setdefault("mlp_middle_depth", 0)
     observed.setdefault("mlp_depth_index", 0)
+    if expected.get("mlp") == _REFERENCE_MLP:
+        observed.setdefault("mlp", _REFERENCE_MLP)
     if observed != expected:
         bad = [f"{k}: memory={observed.get(k)!r} model={expected.get(k)!r}"
                for k in {**expected, **observed} if observed.get(k) != expected.get(k)]
@@ -436,9 +443,9 @@ def _to_payload(memory: DABSNMemory) -> dict[str, object]:
         bank["stats"] = stats.detach().cpu()
         layers.append({"bank": bank, "core": [t.detach().cpu() for t in layer.core],
                        "long": [t.detach().cpu() for t in layer.long]})
+    fingerprint = {k: v for k, v in memory.fingerprint.items() if (k, v) != ("mlp", _REFERENCE_MLP)}
     return {"format": FORMAT, "position": int(memory.position),
-            "batch_size": int(memory.batch_size), "fingerprint": dict(memory.fingerprint),
-            "layers": layers}
+            "batch_size": int(memory.batch_size), "fingerprint": fingerprint, "layers": layers}
 
 
 def _from_payload(payload) -> DABSNMemory:

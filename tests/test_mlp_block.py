@@ -132,6 +132,45 @@ def _lm(**mlp):
     return dabsn_amd.DABSNSequenceLM(40, 24, 2, residual=True, mlp_ratio=2.0, **mlp)
 
 
+def _carried(model):
+    """A memory of the model's architecture, as if two tokens had been read."""
+    layers = []
+    for block in model.blocks:
+        bank = mem.BankStore(1, int(block.state_dim), device="cpu", dtype=torch.float32)
+        bank.append(torch.ones(1, 2, int(block.state_dim)), torch.ones(1, 2, 6))
+        state = lambda: tuple(torch.zeros(1, int(block.state_dim)) for _ in range(3))  # noqa: E731
+        layers.append(mem.LayerMemory(bank=bank, core=state(), long=state()))
+    return mem.DABSNMemory(layers=layers, position=2, batch_size=1, fingerprint=mem.fingerprint_of(model))
+
+
+def test_memory_files_of_the_reference_mlp_cross_load(tmp_path):
+    """``mlp_activation="relu2"`` with the RMS norm and no bias has the reference's parameters and
+    function: its files carry the reference's fingerprint and load into either model, as do the plain
+    model's. Other kinds are still refused, in both directions."""
+    plain, fused, other = _lm(), _lm(mlp_activation="relu2"), _lm(mlp_activation="gelu")
+    biased = _lm(mlp_activation="relu2", mlp_bias=True)
+    for source in (plain, fused):
+        path = mem.save(_carried(source), tmp_path / "a.dmem")
+        payload = torch.load(path, weights_only=True)
+        assert payload["fingerprint"] == mem.fingerprint_of(plain)
+        for target in (plain, fused):
+            loaded = mem.load(path, model=target)
+            assert loaded.fingerprint == mem.fingerprint_of(target) and loaded.entries == 2
+        torch.save({"model": {}}, tmp_path / "c.pt")
+        mem.embed_in_checkpoint(mem.load(path), tmp_path / "c.pt")
+        for target in (plain, fused):
+            assert mem.extract_from_checkpoint(tmp_path / "c.pt", model=target).entries == 2
+        for target in (other, biased):
+            with pytest.raises(ValueError, match="mlp"):
+                mem.load(path, model=target)
+    for source in (other, biased):
+        path = mem.save(_carried(source), tmp_path / "b.dmem")
+        assert mem.load(path, model=source).entries == 2
+        for target in (plain, fused, *({other, biased} - {source})):
+            with pytest.raises(ValueError, match="mlp"):
+                mem.load(path, model=target)
+
+
 def test_a_callers_model_that_names_its_activation_has_a_fingerprint():
     model = _lm()
 
