@@ -314,8 +314,7 @@ struct Piece {
   __device__ __forceinline__ float get(int e) const {
     const uint32_t w = q[sizeof(E) == 4 ? e : e / 2];
     if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w);
-    else if constexpr (H)
-      return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(e % 2 ? w >> 16 : w)));
+    else if constexpr (H) return from_half(static_cast<uint16_t>(e % 2 ? w >> 16 : w));
     else return __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
   }
 };

@@ -45,8 +45,10 @@ struct Args {
 
 // act(z), and what is kept for its derivative: of the squared ReLU the value itself (before a residual;
 // a rounding of it is half of one in the slope 2 sqrt(h)), else the derivative. With bf16 operands
-// that is stored in fp16: derivatives of GELU and SiLU lie in [-0.13, 1.13], where that is off by
-// 2^-11 of itself or 2^-25, an eighth of bf16's step, at the same bytes.
+// that is stored as its 2^14-fold in fp16: derivatives of GELU and SiLU lie in [-0.13, 1.13], so that
+// none overflows and each is off by 2^-11 of itself or 2^-39, an eighth of bf16's step at the same
+// bytes. (By itself, without the factor, all below 2^-25 would be 0, and the gradients of rows that
+// lie there whole.)
 // Where they are rounded to bf16, the hardware's exp and reciprocal do
 // (2^-22 and 2^-23 of their values), and erfc(x) = exp(-x^2) erfcx(x) with erfcx as a polynomial in
 // t = 1 / (1 + 0.46 x), a fit of our own for x >= 0 that is within 1.7e-5 of the value up to x = 60
@@ -105,6 +107,10 @@ __device__ __forceinline__ float factor(float s) {
 // Whether a derivative is kept for GELU and SiLU or read: fp16 in bf16's place.
 template <typename E, int EPI>
 constexpr bool HALF = sizeof(E) == 2 && (EPI == kGelu || EPI == kSilu || EPI == kStored);
+constexpr float HALF_UNIT = 0x1p14f;  // 1 as it is stored so
+__device__ __forceinline__ float from_half(uint16_t h) {
+  return static_cast<float>(__builtin_bit_cast(_Float16, h)) * (1.0f / HALF_UNIT);
+}
 
 // Eight columns of a row as they are stored; with H as fp16 in bf16's place.
 template <typename E>
@@ -116,8 +122,7 @@ struct Eight {
     const uint32_t w = q[sizeof(E) == 4 ? e / 4 : 0][sizeof(E) == 4 ? e % 4 : e / 2];
     // (A bit cast of the vector's element itself would take its first.)
     if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w);
-    else if constexpr (H)
-      return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(e % 2 ? w >> 16 : w)));
+    else if constexpr (H) return from_half(static_cast<uint16_t>(e % 2 ? w >> 16 : w));
     else return __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
   }
   template <bool H = false>
@@ -128,10 +133,11 @@ struct Eight {
     } else {
       typedef float f32x2 __attribute__((ext_vector_type(2)));
       typedef std::conditional_t<H, _Float16, __bf16> low __attribute__((ext_vector_type(2)));
+      constexpr float unit = H ? HALF_UNIT : 1.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         q[0][i] = __builtin_bit_cast(
-            uint32_t, __builtin_convertvector(((f32x2){v[2 * i], v[2 * i + 1]}), low));
+            uint32_t, __builtin_convertvector(((f32x2){v[2 * i] * unit, v[2 * i + 1] * unit}), low));
     }
   }
 };
@@ -166,7 +172,7 @@ struct Rows {
 
 template <typename E, int EPI>
 __device__ __forceinline__ float beside_of(const E* p, int64_t i) {
-  if constexpr (HALF<E, EPI>) return static_cast<float>(__builtin_bit_cast(_Float16, p[i]));
+  if constexpr (HALF<E, EPI>) return from_half(p[i]);
   else return ld(p, i);
 }
 
@@ -182,7 +188,7 @@ __device__ __forceinline__ void finish_one(const Args<E>& a, int64_t m, int n, f
   if (a.bias) v += ld(a.bias, n);
   v = activate<E, EPI>(v, kept);
   if (a.keep) {
-    if constexpr (HALF<E, EPI>) a.keep[m * a.ldk + n] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(kept));
+    if constexpr (HALF<E, EPI>) a.keep[m * a.ldk + n] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(kept * HALF_UNIT));
     else st(a.keep, m * a.ldk + n, kept);
   }
   if constexpr (EPI == kStored || EPI == kFromSquare) {

@@ -9,7 +9,7 @@ function) and ``silu``. (A plain ReLU is left out: its slope jumps at 0, so prod
 operands would differ by whole terms.) Products are fp32 sums; everything up to the result is fp32
 and is rounded once. Both are differentiable in all their tensors. In the backward the products'
 operands have the inputs' type: dz = g activation'(z) is rounded once to it. The slope is kept in
-fp32, or with bfloat16 in fp16 (2^-11 of itself or 2^-25 off); the squared ReLU's is 2 sqrt of its
+fp32, or with bfloat16 in 16 bits (2^-11 of itself or 2^-39 off); the squared ReLU's is 2 sqrt of its
 output, which is kept itself.
 """
 

@@ -17,7 +17,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#define DABSN_HIP_ABI_VERSION 23
+#define DABSN_HIP_ABI_VERSION 24
 
 /* Status codes returned by every entry point. */
 #define DABSN_OK 0
@@ -786,7 +786,8 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
  * transB) A is stored as [K, M] too; any alignment. act: 0 none, 1 squared ReLU, 2 GELU (by the
  * error function), 3 SiLU. keep [M, N] (row stride ldk; NULL: none) receives what the activation's
  * slope is made of: the squared ReLU's value h = act(z), of which it is 2 sqrt(h) (slope_kind 2; without a
- * residual C is h too), of the others the derivative (slope_kind 1), with bf16 operands in fp16.
+ * residual C is h too), of the others the derivative (slope_kind 1), with bf16 operands as its
+ * 2^14-fold in fp16.
  * slope [M, N] is such a matrix. Large fp32 products multiply three bf16 planes of each operand,
  * which hold all bits from 2^-110 up. padA, padB: the operand's rows end in zeros up to a multiple
  * of 8 columns; padC: C's are to. Row strides are below 2^21. Workspace:
