@@ -509,48 +509,91 @@ struct Epilogue {
   }
   // Of planes' products: an infinity meets the other operand's smaller planes too, which may be 0 or
   // of the other sign, and so leaves NaN where the product itself is infinite. Where a sum was not
-  // finite, results that are NaN are formed anew from the operands as they lie, k0 to k0 + len.
+  // finite, results that are NaN are formed anew from the operands as they lie, k0 to k0 + len, by
+  // blocks of 64 x 64 with fp32 matrix instructions: 4096 x 2048 x 4096 with an infinite column of A,
+  // which leaves no finite result, 1.33 ms, without it 0.32 (57 ms when a lane formed one result at a time).
   template <bool TA, bool TB>
   __device__ __forceinline__ void mend(int k0, int len) {
+    static_assert(TM % 4 == 0 && TN % 4 == 0, "a wave has blocks of 64 x 64");
     if (!__any(marked != marked)) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const float *A = reinterpret_cast<const float*>(a.wholeA) + (TA ? k0 * a.wholelda + m0 : m0 * a.wholelda + k0);
     const float *B = reinterpret_cast<const float*>(a.wholeB) + (TB ? k0 * a.wholeldb + n0 : n0 * a.wholeldb + k0);
-    const int64_t rowA = TA ? 1 : a.wholelda, rowB = TB ? 1 : a.wholeldb;
-    const int64_t stepA = TA ? a.wholelda : 1, stepB = TB ? a.wholeldb : 1;
-    // Rows of either operand that hold a NaN have nothing but NaN for results, and are left.
-    uint32_t nanB = 0;
+    const int li = lane & 15, group = lane >> 4;
+    const auto place = [&](int r, int c) __attribute__((always_inline)) {
+      return EPI == kShare ? a.parts + (static_cast<int64_t>(sp) * a.M + m0 + r) * a.ldp + n0 + c
+                           : reinterpret_cast<float*>(a.C) + static_cast<int64_t>(m0 + r) * a.ldc + n0 + c;
+    };
+    const auto is_nan = [](const float* at) __attribute__((always_inline)) {
+      const float old = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return old != old;
+    };
 #pragma unroll 1
-    for (int c = wn + lane; c < min(wn + TN * 16, cols); c += 64)
+    for (int block = 0; block < TM * TN / 16; ++block) {
+      const int r0 = wm + block / (TN / 4) * 64, c0 = wn + block % (TN / 4) * 64;
+      bool bad = false;
+      if (c0 + lane < cols)
 #pragma unroll 1
-      for (int k = 0; k < len; ++k) {
-        const float v = B[c * rowB + k * stepB];
-        if (v != v) nanB |= 1u << ((c - wn) / 64);
+        for (int r = r0; r < min(r0 + 64, rows); ++r) bad |= is_nan(place(r, c0 + lane));
+      if (!__any(bad)) continue;
+      f32x4 c[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      // Four k of a row (or, where transposed, of a column), zeros beyond an edge.
+      const auto take = [&](auto trans, const float* p, int64_t ld, int row, int end, int k) __attribute__((always_inline)) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (row < end) {
+          if constexpr (decltype(trans)::value) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k + e < len) v[e] = p[(k + e) * ld + row];
+          } else if (k + 4 <= len) {
+            __builtin_memcpy(&v, p + row * ld + k, 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k + e < len) v[e] = p[row * ld + k + e];
+          }
+        }
+        return v;
+      };
+#pragma unroll 1
+      for (int k = 0; k < len; k += 16) {
+        f32x4 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = take(std::bool_constant<TA>{}, A, a.wholelda, r0 + i * 16 + li, rows, k + group * 4);
+          y[i] = take(std::bool_constant<TB>{}, B, a.wholeldb, c0 + i * 16 + li, cols, k + group * 4);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              c[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[j][e], x[i][e], c[i][j], 0, 0, 0);
       }
+      // The sums go where the NaN are, and from there, by the lane that left them, through the epilogue.
+      uint64_t left = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = r0 + i * 16 + li, col = c0 + j * 16 + group * 4 + e;
+            if (r >= rows || col >= cols || !is_nan(place(r, col))) continue;
+            *place(r, col) = c[i][j][e];
+            left |= 1ull << (i * 16 + j * 4 + e);
+          }
+      if constexpr (EPI != kShare)
 #pragma unroll 1
-    for (int r = wm; r < min(wm + TM * 16, rows); ++r) {
-      bool nanA = false;
-#pragma unroll 1
-      for (int k = lane; k < len; k += 64) {
-        const float v = A[r * rowA + k * stepA];
-        nanA |= v != v;
-      }
-      if (__any(nanA)) continue;
-      const int64_t m = m0 + r;
-#pragma unroll 1
-      for (int c = wn + lane; c < min(wn + TN * 16, cols); c += 64) {
-        if (nanB >> ((c - wn) / 64) & 1) continue;
-        const int n = n0 + c;
-        float* at = EPI == kShare ? a.parts + (static_cast<int64_t>(sp) * a.M + m) * a.ldp + n
-                                  : reinterpret_cast<float*>(a.C) + m * a.ldc + n;
-        const float old = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (old == old) continue;
-        float s = 0.0f;
-#pragma unroll 1
-        for (int k = 0; k < len && s == s; ++k) s = fmaf(A[r * rowA + k * stepA], B[c * rowB + k * stepB], s);
-        if constexpr (EPI == kShare) *at = s;
-        else finish_one<E, EPI>(a, m, n, s);
-      }
+        for (; left; left &= left - 1) {
+          const int at = __builtin_ctzll(left), r = r0 + at / 16 * 16 + li, col = c0 + at / 4 % 4 * 16 + group * 4 + at % 4;
+          finish_one<E, EPI>(a, m0 + r, n0 + col, *place(r, col));
+        }
     }
   }
 };

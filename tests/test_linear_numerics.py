@@ -55,3 +55,98 @@ def test_gradients_of_tails_of_the_mlp(cuda_device, act, m):
     (db,) = torch.autograd.grad(fused_mlp(x, w1, w2, b1, activation=act), b1, up)
     # All rows have the same dz, rounded to bf16; their number is a power of two.
     within(db / m, slope, tol + 2.0 ** -8 * (slope.abs() + tol))
+
+
+# ---- infinities and NaN -----------------------------------------------------------------------
+def _same_kind(name, got, want):
+    """NaN where NaN, infinite where infinite, and finite elsewhere."""
+    got, want = got.double(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), name
+    odd = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), odd) and torch.equal(got[odd], want[odd]), name
+
+
+def _mixed(g, *shape):
+    """Values that one bf16 holds whole, zeros among them, and values that take three."""
+    v = torch.randn(*shape, device="cuda", generator=g)
+    v[::2] = torch.randint(-2, 3, v[::2].shape, device="cuda", generator=g).float()
+    return v
+
+
+# Products of planes in tiles of 256 x 256 (the last in splits) and of fp32 as it lies.
+KINDS = [(40, 64, 40), (4001, 1000, 3999), (2049, 9001, 2050)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,residual", [("relu2", False), ("relu2", True), ("gelu", True), ("silu", False)])
+@pytest.mark.parametrize("m,k,n", KINDS)
+def test_infinities_through_activations(cuda_device, m, k, n, act, residual):
+    g = torch.Generator(device=cuda_device).manual_seed(m)
+    x, w, grad = torch.randn(m, k, device=cuda_device, generator=g), _mixed(g, n, k) / 8, _mixed(g, m, n)
+    x[3, k - 1], x[m - 1, 0], x[7, 1], x[7, 2], x[9, 5] = math.inf, -math.inf, math.inf, -math.inf, math.nan
+    b, res = 0.1 * torch.randn(n, device=cuda_device, generator=g), None
+    if residual:
+        res = torch.randn(m, n, device=cuda_device, generator=g)
+        res[3, ::3], res[5, 5] = -math.inf, math.inf
+    leaves = [t.requires_grad_(True) for t in (x, w, b, *((res,) if residual else ()))]
+    out = fused_linear(x, w, b, activation=act, residual=res)
+    dx, dw, db = torch.autograd.grad(out, leaves, grad)[:3]
+    z = Val(x).v @ Val(w).v.t() + b.detach().double()
+    h, slope = activated(Val(z), act)
+    _same_kind("out", out.detach(), h.v if res is None else h.v + res.detach().double())
+    dz = grad.double() * slope.v
+    _same_kind("x", dx, dz @ w.detach().double())
+    _same_kind("weight", dw, dz.t() @ x.detach().double())
+    _same_kind("bias", db, dz.sum(0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["relu2", "gelu"])
+@pytest.mark.parametrize("m,h,f", [(40, 24, 61), (4001, 1000, 3999), (300, 2048, 4100), (6000, 256, 1024)])
+def test_infinite_gradients_through_the_mlps_slopes(cuda_device, m, h, f, act):
+    """An infinite gradient times the second layer times the slope, seen in the first layer's bias; an
+    infinite inner value through the second product and the residual."""
+    g = torch.Generator(device=cuda_device).manual_seed(m)
+    x, w1 = torch.randn(m, h, device=cuda_device, generator=g), torch.randn(f, h, device=cuda_device, generator=g)
+    w1, w2, up = w1 / math.sqrt(h), _mixed(g, h, f) / 8, torch.randn(m, h, device=cuda_device, generator=g)
+    up[2, 4], up[m - 1, h - 1], up[5, 3], up[5, 6] = math.inf, -math.inf, math.inf, math.inf
+    b1 = (0.1 * torch.randn(f, device=cuda_device, generator=g)).requires_grad_(True)
+    (db,) = torch.autograd.grad(fused_mlp(x, w1, w2, b1, activation=act), b1, up)
+    X, W1, W2 = x.double(), w1.double(), w2.double()
+    z = (X / (X.square().mean(1, keepdim=True) + 1e-6).sqrt()) @ W1.t()
+    _, slope = activated(Val(z + b1.detach().double()), act)
+    _same_kind("b1", db, ((up.double() @ W2) * slope.v).sum(0))
+    with torch.no_grad():
+        b1[f // 2], x[4, 1] = 1e30, math.inf  # one column of infinities where squared, and a row of NaN
+        out = fused_mlp(x, w1, w2, b1, activation=act)
+        X = x.double()
+        z = (X / (X.square().mean(1, keepdim=True) + 1e-6).sqrt()) @ W1.t() + b1.double()
+        hidden = activated(Val(z), act)[0].v.float().double()  # 1e60 is infinite in fp32
+        _same_kind("out", out, X + hidden @ W2.t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("m,k,n", [(2048, 1024, 2048), (4096, 2048, 4096)])
+def test_results_without_a_finite_one_take_no_age(cuda_device, m, k, n, value):
+    """All results infinite or NaN (a training step that has run off): forming them anew by fp32 matrix
+    instructions takes 1.5 times the planes' time again by their rates, and what the loads' latency adds
+    (measured 2.4 and 4.2 times in all); elements one by one, as it was, took 67 and 180 times."""
+    x = torch.randn(m, k, device=cuda_device)
+    w = torch.randn(n, k, device=cuda_device)
+
+    def fastest():
+        times = []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            fused_linear(x, w)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    finite = fastest()
+    x[:, k // 3] = value
+    assert fastest() < 15 * finite
+    _same_kind("out", fused_linear(x, w), x.double() @ w.double().t())
