@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from dabsn_amd import fused_linear, fused_mlp
-from test_linear import Val, activated
+from test_linear import Val, activated, check_linear, run, tensors
 from test_norm import U, within
 
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -150,3 +150,79 @@ def test_results_without_a_finite_one_take_no_age(cuda_device, m, k, n, value):
     x[:, k // 3] = value
     assert fastest() < 15 * finite
     _same_kind("out", fused_linear(x, w), x.double() @ w.double().t())
+
+
+# ---- fp32 as planes ---------------------------------------------------------------------------
+# Six products of bf16 planes (hi, mid, lo) make an fp32 one. Bounds by the terms' magnitudes grow with
+# their number n beyond what a missing product would change (2.4e-6 of the result in the norm for lo hi
+# and hi lo, 2.8e-6 for mid mid, at any n). In the norm, sums of n products in at most n / 8
+# additions, whose partial sums grow as the root of their number and whose roundings of at most u = 2^-24
+# have independent signs, are off by u sqrt(n / 8 / 6) or less, and their last rounding by u / sqrt(3);
+# what the planes leave out is 6e-9.
+def _norm_bound(n):
+    return U * (1 + 2 * math.sqrt(n / 48))
+
+
+def _off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("n", [300, 4001])
+def test_the_bound_sees_a_missing_product_of_planes(n):
+    g = torch.Generator().manual_seed(n)
+    a, b = torch.randn(150, n, generator=g), torch.randn(130, n, generator=g)
+
+    def planes(rest):
+        for _ in range(3):
+            part = rest.to(BF16).float()
+            yield part.double()
+            rest = rest - part
+
+    pa, pb = list(planes(a)), list(planes(b))
+    want = a.double() @ b.double().t()
+    pairs = [(2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)]
+    products = {p: pa[p[0]] @ pb[p[1]].t() for p in pairs}
+    whole = sum(products.values())
+    assert _off(whole, want) < 1e-8
+    for p in pairs:
+        assert _off(whole - products[p], want) > _norm_bound(n), p
+
+
+# Between them these take 256 x 256 and 128 x 128 tiles of planes, split and whole, in all three
+# directions.
+PLANES = [(515, 1500, 4001), (4001, 777, 1001), (1001, 2050, 2050), (300, 2050, 4001), (2050, 300, 4001),
+          (2050, 4001, 300)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", PLANES)
+def test_fp32_products_hold_24_bits(cuda_device, m, k, n):
+    t = tensors(m + k + n, m, k, n, FP32, False, False)
+    got = run(t, "none")
+    x, w, g = (t[a].double() for a in ("x", "weight", "grad"))
+    for name, want, terms in (("out", x @ w.t(), k), ("x", g @ w, n), ("weight", g.t() @ x, m)):
+        assert _off(got[name], want) <= _norm_bound(terms), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_all_gradients_of_strided_operands(cuda_device, dtype):
+    """256 x 256 tiles on rows inside wider arrays of NaN at odd offsets. fp32 operands are packed into
+    planes wherever they lie: the contiguous ones' results, bit for bit."""
+    m, k, n = 4001, 1000, 3999
+    t = tensors(1, m, k, n, dtype, True, True)
+    view = {}
+    for a in ("x", "weight", "residual", "grad"):
+        wide = torch.full((t[a].shape[0], t[a].shape[1] + 5), math.nan, device=cuda_device, dtype=dtype)
+        wide[:, 3:-2] = t[a]
+        view[a] = wide[:, 3:-2]
+    leaves = {a: v.requires_grad_(True) for a, v in view.items() if a != "grad"}
+    leaves["bias"] = t["bias"].clone().requires_grad_(True)
+    out = fused_linear(leaves["x"], leaves["weight"], leaves["bias"], activation="silu",
+                       residual=leaves["residual"])
+    grads = torch.autograd.grad(out, tuple(leaves.values()), view["grad"])
+    got = {"out": out.detach(), **dict(zip(leaves, grads))}
+    check_linear(t, "silu", got)
+    want = run(t, "silu")
+    same = want if dtype == FP32 else ("bias", "residual")
+    assert all(torch.equal(got[a], want[a]) for a in same)
