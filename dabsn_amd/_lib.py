@@ -13,7 +13,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_build" / "libdabsn_hip.so"
-ABI_VERSION = 24
+ABI_VERSION = 25
 
 _lock = threading.Lock()
 _lib = None
@@ -61,7 +61,7 @@ class CoreBwdCall(ctypes.Structure):
 class LinearCall(ctypes.Structure):
     """Mirror of ``dabsn_linear_call``."""
 
-    _fields_ = ([(n, i32) for n in ("dtype", "transA", "transB", "padA", "padB", "padC", "act",
+    _fields_ = ([(n, i32) for n in ("dtype", "transA", "transB", "padA", "padC", "wideC", "act",
                                      "slope_kind")]
                 + [(n, i64) for n in ("M", "N", "K")]
                 + [(n, vp) for n in ("A", "B", "bias", "slope", "residual")]

@@ -163,7 +163,7 @@ static Plan plan_of(const dabsn_linear_call& c) {
   }
   const bool f32 = c.dtype == kF32;
   const bool packA = f32 || !ready(c.A, c.lda, c.transA, c.K, c.padA);
-  const bool packB = f32 || !ready(c.B, c.ldb, c.transB, c.K, c.padB);
+  const bool packB = f32 || !ready(c.B, c.ldb, c.transB, c.K, false);
   const int64_t rowsA = c.transA ? c.K : c.M, rowsB = c.transB ? c.K : c.N;
   const int64_t wideA = ((c.transA ? c.M : c.K) + 7) / 8 * 8, wideB = ((c.transB ? c.N : c.K) + 7) / 8 * 8;
   const int64_t lda = packA ? wideA : c.lda, ldb = packB ? wideB : c.ldb;
@@ -248,6 +248,11 @@ static int run(const dabsn_linear_call& c, const Plan& p, hipStream_t s) {
   a.wholeA = (const E*)c.A; a.wholelda = c.lda;
   a.wholeB = (const E*)c.B; a.wholeldb = c.ldb;
   a.parts = p.splits > 1 ? (float*)(ws + p.atParts) : nullptr;
+  const bool wide = c.wideC && c.K && p.splits == 1;  // the only share is the result
+  if (wide) {
+    a.parts = (float*)c.C;
+    a.ldp = c.ldc;
+  }
   if (c.K) {
     Operand<E> pa = {}, pb = {};
     if (p.packA)
@@ -273,13 +278,18 @@ static int run(const dabsn_linear_call& c, const Plan& p, hipStream_t s) {
     else with_activation(c, [&](auto epi) { launch<E, decltype(epi)::value, false, false>(a, p.tile, nblk, s); });
     DABSN_HIP_CHECK(hipGetLastError());
   }
-  if (a.parts || !c.K) {
+  if ((a.parts && !wide) || !c.K) {
     const int64_t blocks = (p.ldp / 8 * c.M + 255) / 256;
     DABSN_REQUIRE(blocks < (1ll << 31), "linear: too many elements to join");
     auto join = [&](auto epi) {
       hipLaunchKernelGGL((join_kernel<E, decltype(epi)::value>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     };
-    if (c.slope) with_factor(c, join);
+    if (c.wideC) {
+      Args<float> f = {};
+      f.M = a.M; f.N = a.N; f.splits = a.splits; f.parts = a.parts; f.ldp = a.ldp;
+      f.C = (float*)c.C; f.ldc = c.ldc; f.padC = 1;
+      hipLaunchKernelGGL((join_kernel<float, kNone>), dim3((unsigned)blocks), dim3(256), 0, s, f);
+    } else if (c.slope) with_factor(c, join);
     else with_activation(c, join);
     DABSN_HIP_CHECK(hipGetLastError());
   }
@@ -446,6 +456,8 @@ static int check_linear(const dabsn_linear_call& c) {
   DABSN_REQUIRE(!c.transB || (c.act == kNone && !c.bias && !c.residual),
                 "linear: no activation, bias or residual with transB");
   DABSN_REQUIRE(!c.slope || (c.transB && !c.transA), "linear: a slope goes with transB alone");
+  DABSN_REQUIRE(!c.wideC || (c.dtype == kBF16 && c.transB && !c.transA && !c.slope && c.ldc % 8 == 0),
+                "linear: a wide C goes with bf16, transB alone, no slope and rows of a multiple of 8");
   return DABSN_OK;
 }
 

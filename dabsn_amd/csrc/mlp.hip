@@ -5,10 +5,14 @@
 // call and a tensor each, 181 so, of which 136 are kernels).
 //
 // Rounded to bf16 on the way, where the operands are bf16, is what the matrix cores read: the normed
-// rows, h and dz, and dn, whose bytes the norm's backward is bound by. (Weights' gradients of the
-// branch are 0.3% off in the norm by these, a single rounding of the result 0.17%.) Sums stay fp32.
-#include "capi.hpp"
+// rows, h and dz. (Weights' gradients of the branch are 0.3% off in the norm by these, a single rounding
+// of the result 0.17%.) Sums stay fp32, and so does dn, which only the norm's backward reads: rounded
+// too it made dx 0.28% off and the norm's weight 0.33%, now 0.25% and
+// 0.29%, for 1.1% of the time (65536 x 2048 x 8192).
+// b1's gradient sums dz as the products have it: the roundings of its terms have independent signs and
+// leave it off by no more than its own rounding does (0.17% of the root of the sum of the terms' squares).
 #include "common.hpp"
+#include "norm.hpp"
 
 #include <algorithm>
 #include <initializer_list>
@@ -113,7 +117,9 @@ static Forward forward(const dabsn_mlp_call& c, char* base) {
 
 struct Backward {
   Saved v;
-  void *dz, *dn, *dx;
+  void *dz, *dx;
+  void* dn;  // [M][ldn] in fp32
+  int64_t ldn;
   dabsn_linear_call dz_call, dn_call, dw1_call, dw2_call;
   bool rows, inner;  // whether dz, and what lies before it, is asked for
   size_t scratch_at, scratch, total;
@@ -127,7 +133,8 @@ static Backward backward(const dabsn_mlp_call& c, char* base) {
   b.inner = c.dx || c.dnorm_weight || c.dnorm_bias;
   b.rows = b.inner || c.dw1 || c.db1;
   b.dz = b.rows ? s.take(M * ldh * size) : nullptr;
-  b.dn = b.inner ? s.take(M * c.H * size) : nullptr;
+  b.ldn = c.dtype == kF32 ? c.H : padded(c.H);
+  b.dn = b.inner ? s.take(M * b.ldn * sizeof(float)) : nullptr;
   b.dx = c.dx || !b.inner ? c.dx : s.take(M * c.H * size);
   const auto need = [&](const dabsn_linear_call& l) {
     b.scratch = std::max(b.scratch, dabsn_hip_linear_workspace_bytes(&l));
@@ -145,8 +152,9 @@ static Backward backward(const dabsn_mlp_call& c, char* base) {
   }
   if (c.dw1) need(b.dw1_call = weight_grad(c.dtype, c.M, c.F, c.H, b.dz, ldh, b.v.normed, c.H, c.dw1));
   if (b.inner) {
-    b.dn_call = rows_grad(c.dtype, c.M, c.F, c.H, b.dz, ldh, c.w1, c.ldw1, b.dn, c.H);
+    b.dn_call = rows_grad(c.dtype, c.M, c.F, c.H, b.dz, ldh, c.w1, c.ldw1, b.dn, b.ldn);
     b.dn_call.padA = 1;
+    b.dn_call.wideC = c.dtype == kBF16;
     need(b.dn_call);
     b.scratch = std::max(b.scratch, dabsn_hip_norm_workspace_bytes(c.dtype, c.M, c.H));
   }
@@ -290,8 +298,8 @@ int dabsn_hip_mlp_bwd(const dabsn_mlp_call* call, hipStream_t stream) {
   if (c.dw1) DABSN_STEP(run(b.dw1_call, scratch, b.scratch, stream));
   if (!b.inner) return DABSN_OK;
   DABSN_STEP(run(b.dn_call, scratch, b.scratch, stream));
-  return dabsn_hip_norm_bwd(c.dtype, c.wdtype, c.layer, c.M, c.H, c.x, c.ldx, c.norm_weight, b.v.stats, b.dn,
-                            c.H, c.grad, b.dx, c.dnorm_weight, c.dnorm_bias, scratch, b.scratch, stream);
+  return norm::backward(c.dtype, c.wdtype, kF32, c.layer, c.M, c.H, c.x, c.ldx, c.norm_weight, b.v.stats, b.dn,
+                        b.ldn, c.grad, b.dx, c.dnorm_weight, c.dnorm_bias, scratch, b.scratch, stream);
 }
 
 size_t dabsn_hip_linear_grads_workspace_bytes(const dabsn_linear_grads_call* call) {

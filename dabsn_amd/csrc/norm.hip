@@ -13,7 +13,8 @@
 // The backward's workgroups walk over the rows with a column's dw and db in the registers of the
 // thread that holds the column, and leave one partial row each; join_kernel adds these in order.
 // The same inputs give the same bits.
-#include "capi.hpp"
+#include "norm.hpp"
+
 #include "common.hpp"
 
 #include <algorithm>
@@ -28,22 +29,22 @@ template <typename E>
 constexpr int vec_of() { return 16 / static_cast<int>(sizeof(E)); }
 
 // A thread's vector of a row as it is stored, at any alignment; elements beyond `left` are 0.
-template <typename E>
+template <typename E, int VEC = vec_of<E>()>
 struct Raw {
-  static constexpr int VEC = vec_of<E>();
-  u32x4 q;
+  static constexpr int PER = vec_of<E>();
+  u32x4 q[VEC / PER];
   __device__ __forceinline__ void load(const E* p, int left) {
     if (left >= VEC) {
-      __builtin_memcpy(&q, p, 16);
+      __builtin_memcpy(q, p, sizeof(q));
     } else {
       E e[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) e[i] = i < left ? p[i] : static_cast<E>(0);
-      __builtin_memcpy(&q, e, 16);
+      __builtin_memcpy(q, e, sizeof(q));
     }
   }
   __device__ __forceinline__ float get(int e) const {
-    const uint32_t w = q[sizeof(E) == 4 ? e : e / 2];
+    const uint32_t w = q[e / PER][sizeof(E) == 4 ? e % PER : e % PER / 2];
     if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, w);
     else return __builtin_bit_cast(float, e % 2 ? w & 0xffff0000u : w << 16);
   }
@@ -165,13 +166,14 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T)
   }
 }
 
-// Rows as in fwd_kernel; parts [gridDim.x][2][H] (dw, db; NULL: not needed). With ADD the rows to add
-// are on their way with the next row too (loaded where they are used they waited for it: 65536 x 2048
+// Rows as in fwd_kernel; parts [gridDim.x][2][H] (dw, db; NULL: not needed). G: type of the gradient's
+// rows, which the block's MLP leaves in fp32 beside bf16 (65536 x 2048 with ADD: 252 us, 5.3 TB/s). With
+// ADD the rows to add are on their way with the next row too (loaded where they are used they waited for it: 65536 x 2048
 // bf16 299 us, 200 so; without ADD their registers cost 77 -> 95 us at 30011 x 1001 fp32).
-template <typename E, typename W, int T, int NV, bool ADD>
+template <typename E, typename W, typename G, int T, int NV, bool ADD>
 __global__ void __launch_bounds__(T < 256 ? 256 : T)
     bwd_kernel(int64_t rows, int H, const E* x, int64_t ldx, const W* weight, const float* stats,
-               int center, const E* grad, int64_t ldg, const E* add, E* dx, float* parts) {
+               int center, const G* grad, int64_t ldg, const E* add, E* dx, float* parts) {
   constexpr int VEC = vec_of<E>(), R = T < 256 ? 256 / T : 1;
   __shared__ float part[2][2][T / 64];
   __shared__ float lds[R > 1 ? R : 1][R > 1 ? 2 * T * VEC : 1];
@@ -188,7 +190,8 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T)
     }
     if (weight && c < H) load_row<W, VEC>(weight + c, H - c, w[i]);
   }
-  Raw<E> nextx[NV], nextg[NV], nexta[NV];
+  Raw<E> nextx[NV], nexta[NV];
+  Raw<G, VEC> nextg[NV];
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch = [&](int64_t row) {
     if (row >= rows) return;
@@ -348,7 +351,7 @@ static int run_fwd(int64_t rows, int H, const void* x, int64_t ldx, const void* 
   });
 }
 
-template <typename E, typename W>
+template <typename E, typename W, typename G>
 static int run_bwd(int64_t rows, int H, const void* x, int64_t ldx, const void* w,
                    const float* stats, int center, const void* g, int64_t ldg, const void* add,
                    void* dx, void* dw, void* db, float* parts, hipStream_t s) {
@@ -357,9 +360,10 @@ static int run_bwd(int64_t rows, int H, const void* x, int64_t ldx, const void* 
   const int rc = with_plan(p, [&](auto T, auto NV) {
     const auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)P), dim3(T < 256 ? 256 : T), 0, s, rows, H, (const E*)x,
-                         ldx, (const W*)w, stats, center, (const E*)g, ldg, (const E*)add, (E*)dx, parts);
+                         ldx, (const W*)w, stats, center, (const G*)g, ldg, (const E*)add, (E*)dx, parts);
     };
-    add ? launch(bwd_kernel<E, W, T, NV, true>) : launch(bwd_kernel<E, W, T, NV, false>);
+    if (add) launch(bwd_kernel<E, W, G, T, NV, true>);
+    else if constexpr (std::is_same_v<E, G>) launch(bwd_kernel<E, W, G, T, NV, false>);
     DABSN_HIP_CHECK(hipGetLastError());
     return DABSN_OK;
   });
@@ -383,6 +387,44 @@ static int check_norm(const char* what, int dtype, int wdtype, int64_t rows, int
                 "%s: bad shape rows=%lld H=%lld ld=%lld", what, (long long)rows, (long long)H,
                 (long long)ldx);
   return DABSN_OK;
+}
+
+int norm::backward(int dtype, int wdtype, int gdtype, int layer, int64_t rows, int64_t H, const void* x,
+                   int64_t ldx, const void* weight, const float* stats, const void* grad, int64_t ldg,
+                   const void* add, void* dx, void* dweight, void* dbias, void* workspace,
+                   size_t workspace_bytes, hipStream_t stream) {
+  const int rc = check_norm("norm backward", dtype, wdtype, rows, H, std::min(ldx, ldg));
+  if (rc != DABSN_OK) return rc;
+  DABSN_REQUIRE(gdtype == dtype || (gdtype == kF32 && (add || rows == 0)), "norm backward: bad gradient dtype %d", gdtype);
+  float* parts = nullptr;
+  if (dweight || dbias) {
+    parts = static_cast<float*>(workspace);
+    const size_t need = dabsn_hip_norm_workspace_bytes(dtype, rows, H);
+    DABSN_REQUIRE(rows == 0 || (parts && workspace_bytes >= need),
+                  "norm backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  }
+  if (rows == 0) {  // no rows: zero sums
+    for (void* p : {dweight, dbias})
+      if (p) {
+        const unsigned blocks = (unsigned)((H + 63) / 64);
+        if (wdtype == kF32)
+          hipLaunchKernelGGL(join_kernel<float>, dim3(blocks), dim3(1024), 0, stream, 0, (int)H,
+                             (int)H, nullptr, (float*)p, (float*)nullptr);
+        else
+          hipLaunchKernelGGL(join_kernel<bf16>, dim3(blocks), dim3(1024), 0, stream, 0, (int)H,
+                             (int)H, nullptr, (bf16*)p, (bf16*)nullptr);
+        DABSN_HIP_CHECK(hipGetLastError());
+      }
+    return DABSN_OK;
+  }
+  DABSN_REQUIRE(x && stats && grad && dx, "norm backward: null pointer");
+  const auto run = [&](auto kernels) {
+    return kernels(rows, (int)H, x, ldx, weight, stats, layer != 0, grad, ldg, add, dx, dweight, dbias, parts,
+                   stream);
+  };
+  if (dtype == kF32) return run(run_bwd<float, float, float>);
+  if (gdtype == dtype) return wdtype == kF32 ? run(run_bwd<bf16, float, bf16>) : run(run_bwd<bf16, bf16, bf16>);
+  return wdtype == kF32 ? run(run_bwd<bf16, float, float>) : run(run_bwd<bf16, bf16, float>);
 }
 
 extern "C" {
@@ -411,38 +453,8 @@ int dabsn_hip_norm_bwd(int dtype, int wdtype, int layer, int64_t rows, int64_t H
                        int64_t ldx, const void* weight, const float* stats, const void* grad,
                        int64_t ldg, const void* add, void* dx, void* dweight, void* dbias,
                        void* workspace, size_t workspace_bytes, hipStream_t stream) {
-  const int rc = check_norm("norm backward", dtype, wdtype, rows, H, std::min(ldx, ldg));
-  if (rc != DABSN_OK) return rc;
-  float* parts = nullptr;
-  if (dweight || dbias) {
-    parts = static_cast<float*>(workspace);
-    const size_t need = dabsn_hip_norm_workspace_bytes(dtype, rows, H);
-    DABSN_REQUIRE(rows == 0 || (parts && workspace_bytes >= need),
-                  "norm backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  }
-  if (rows == 0) {  // no rows: zero sums
-    for (void* p : {dweight, dbias})
-      if (p) {
-        const unsigned blocks = (unsigned)((H + 63) / 64);
-        if (wdtype == kF32)
-          hipLaunchKernelGGL(join_kernel<float>, dim3(blocks), dim3(1024), 0, stream, 0, (int)H,
-                             (int)H, nullptr, (float*)p, (float*)nullptr);
-        else
-          hipLaunchKernelGGL(join_kernel<bf16>, dim3(blocks), dim3(1024), 0, stream, 0, (int)H,
-                             (int)H, nullptr, (bf16*)p, (bf16*)nullptr);
-        DABSN_HIP_CHECK(hipGetLastError());
-      }
-    return DABSN_OK;
-  }
-  DABSN_REQUIRE(x && stats && grad && dx, "norm backward: null pointer");
-  if (dtype == kF32)
-    return run_bwd<float, float>(rows, (int)H, x, ldx, weight, stats, layer != 0, grad, ldg, add, dx,
-                                 dweight, dbias, parts, stream);
-  if (wdtype == kF32)
-    return run_bwd<bf16, float>(rows, (int)H, x, ldx, weight, stats, layer != 0, grad, ldg, add, dx,
-                                dweight, dbias, parts, stream);
-  return run_bwd<bf16, bf16>(rows, (int)H, x, ldx, weight, stats, layer != 0, grad, ldg, add, dx,
-                             dweight, dbias, parts, stream);
+  return norm::backward(dtype, wdtype, dtype, layer, rows, H, x, ldx, weight, stats, grad, ldg, add, dx,
+                        dweight, dbias, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -17,7 +17,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#define DABSN_HIP_ABI_VERSION 24
+#define DABSN_HIP_ABI_VERSION 25
 
 /* Status codes returned by every entry point. */
 #define DABSN_OK 0
@@ -789,8 +789,9 @@ int dabsn_hip_embedding_bwd(int dtype, int64_t n, int64_t V, int64_t H, const in
  * residual C is h too), of the others the derivative (slope_kind 1), with bf16 operands as its
  * 2^14-fold in fp16.
  * slope [M, N] is such a matrix. Large fp32 products multiply three bf16 planes of each operand,
- * which hold all bits from 2^-110 up. padA, padB: the operand's rows end in zeros up to a multiple
- * of 8 columns; padC: C's are to. Row strides are below 2^21. Workspace:
+ * which hold all bits from 2^-110 up. padA: A's rows end in zeros up to a multiple of 8 columns; padC:
+ * C's are to. wideC: C is fp32 beside bf16 operands, with transB alone and no slope; ldc is a multiple of
+ * 8, and what lies between N and ldc is overwritten. Row strides are below 2^21. Workspace:
  * dabsn_hip_linear_workspace_bytes of the same call (its workspace may be unset), 16-byte aligned
  * (0: none).
  * dabsn_hip_linear_slope: dz [rows, n] (row stride ldz; NULL: none) = grad * slope, its rows ending
@@ -806,7 +807,7 @@ int dabsn_hip_norm_bwd(int dtype, int wdtype, int layer, int64_t rows, int64_t H
                        void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 typedef struct dabsn_linear_call {
-  int dtype, transA, transB, padA, padB, padC, act, slope_kind;
+  int dtype, transA, transB, padA, padC, wideC, act, slope_kind;
   int64_t M, N, K;
   const void *A, *B, *bias, *slope, *residual;
   int64_t lda, ldb, lds, ldr, ldc, ldk;

@@ -226,3 +226,28 @@ def test_all_gradients_of_strided_operands(cuda_device, dtype):
     want = run(t, "silu")
     same = want if dtype == FP32 else ("bias", "residual")
     assert all(torch.equal(got[a], want[a]) for a in same)
+
+
+# ---- what the branch's backward hands on ------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,h,f", [(1, 8, 300), (40, 24, 61), (300, 77, 5000), (300, 512, 8192), (4001, 1000, 3999)])
+def test_the_normed_rows_gradient_is_not_rounded(cuda_device, m, h, f):
+    """Whole numbers throughout: dz = g W2 (|dz| < 256) is exact in bf16, its product with W1 in fp32, and
+    so are that one's sums over the rows, the norm's bias in fp32. A rounding of the product to 8 bits
+    would show."""
+    g = torch.Generator(device=cuda_device).manual_seed(m + f)
+
+    def whole(most, *shape):
+        return torch.randint(-most, most + 1, shape, device=cuda_device, generator=g).to(BF16)
+
+    x, up, w1, w2 = torch.randn(m, h, device=cuda_device).to(BF16), whole(1, m, h), whole(2, f, h), whole(1, h, f)
+    nb = torch.zeros(h, device=cuda_device, requires_grad=True)
+    nw = torch.ones(h, device=cuda_device)
+    out = fused_mlp(x, w1, w2, norm="layer", norm_weight=nw, norm_bias=nb, activation="none")
+    (db,) = torch.autograd.grad(out, nb, up)
+    dz = up.double() @ w2.double()
+    assert float(dz.abs().max()) <= 256
+    dn = dz @ w1.double()
+    assert float(dn.abs().sum(0).max()) < 2 ** 24
+    assert f < 1000 or bool((dn.to(BF16).double() != dn).any())  # sums of a few hundred terms have 8 bits
+    assert torch.equal(db.double(), dn.sum(0))
