@@ -607,8 +607,8 @@ struct Epilogue {
 //
 // fp32 operands come as three bf16 planes each (x = hi + mid + lo, 8 bits each, the remainders
 // exact): the steps then go through six products of planes, small ones first; the three left out
-// are below 2^-24 of the product. At 2.5 PFLOP/s for bf16 against 0.16 for fp32 this is 2.6 times
-// the fp32 instructions' rate.
+// are below 2^-24 of the product. By the peaks, 2.5 PFLOP/s for bf16 against 0.16 for fp32, this is 2.6
+// times the fp32 instructions' rate; at the clocks that the power allows it is 1.4 to 1.5 times.
 //
 // Bound by the matrix cores at the clock that the power allows. bf16: 8192^3 722 us, 1520 TFLOP/s;
 // 65536 x 2048 x 8192 1660 us, its rows' gradient 1550 to 1570, its weight's 1460 to 1520. fp32:

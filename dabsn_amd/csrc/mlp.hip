@@ -2,15 +2,16 @@
 // norm.hip and linear.hip one after the other, with what lies between them in the caller's workspace.
 // One call from the host instead of three to nine, and one buffer for all that the backward needs,
 // which is what small steps wait for (2048 x 256 x 1024 fp32, forward and backward: 235 us with a
-// call and a tensor each, 181 so, of which 136 are kernels).
+// call and a tensor each, 180 to 188 so, of which 131 are kernels).
 //
 // Rounded to bf16 on the way, where the operands are bf16, is what the matrix cores read: the normed
 // rows, h and dz. (Weights' gradients of the branch are 0.3% off in the norm by these, a single rounding
 // of the result 0.17%.) Sums stay fp32, and so does dn, which only the norm's backward reads: rounded
-// too it made dx 0.28% off and the norm's weight 0.33%, now 0.25% and
-// 0.29%, for 1.1% of the time (65536 x 2048 x 8192).
-// b1's gradient sums dz as the products have it: the roundings of its terms have independent signs and
-// leave it off by no more than its own rounding does (0.17% of the root of the sum of the terms' squares).
+// too it left dx 0.28% off and the norm's weight 0.33%, now 0.25% and 0.29%, for 1.1% of the time
+// (65536 x 2048 x 8192). b1's gradient sums dz as the products have it, in a pass of its own (190 us
+// there): dz before its rounding is in no memory. The roundings of the terms have independent signs and
+// add up to 0.17% of the root of the terms' squares, which is the size of a sum of gradients of
+// either sign, and as much as the result's own rounding.
 #include "common.hpp"
 #include "norm.hpp"
 

@@ -324,13 +324,14 @@ static int64_t parts_of(int64_t rows, int64_t H, int vec) {
   return std::max<int64_t>(1, std::min<int64_t>(most, (rows + 4 * slots - 1) / (4 * slots)));
 }
 
-template <typename F>
+template <typename E, typename F>
 static int with_plan(const Plan& p, F&& f) {
 #define C(T_, NV_) \
   if (p.T == T_ && p.NV == NV_) return f(std::integral_constant<int, T_>{}, std::integral_constant<int, NV_>{})
   C(64, 1); C(64, 2); C(64, 4);
   C(256, 1); C(256, 2); C(256, 4);
-  C(1024, 1); C(1024, 2); C(1024, 4);
+  C(1024, 1); C(1024, 2);
+  if constexpr (1024 * 2 * vec_of<E>() < MAX_WIDTH) C(1024, 4);
 #undef C
   return DABSN_ERR_ARG;
 }
@@ -339,7 +340,7 @@ template <typename E, typename W>
 static int run_fwd(int64_t rows, int H, const void* x, int64_t ldx, const void* w, const void* b,
                    float eps, int center, void* out, float* stats, hipStream_t s) {
   const Plan p = plan_of(rows, H, vec_of<E>());
-  return with_plan(p, [&](auto T, auto NV) {
+  return with_plan<E>(p, [&](auto T, auto NV) {
     constexpr int R = T < 256 ? 256 / T : 1;
     // Eight workgroups a unit (two of 1024 threads), or one a row.
     const int64_t most = T == 1024 ? 512 : 2048;
@@ -357,7 +358,7 @@ static int run_bwd(int64_t rows, int H, const void* x, int64_t ldx, const void* 
                    void* dx, void* dw, void* db, float* parts, hipStream_t s) {
   const Plan p = plan_of(rows, H, vec_of<E>());
   const int64_t P = parts_of(rows, H, vec_of<E>());
-  const int rc = with_plan(p, [&](auto T, auto NV) {
+  const int rc = with_plan<E>(p, [&](auto T, auto NV) {
     const auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)P), dim3(T < 256 ? 256 : T), 0, s, rows, H, (const E*)x,
                          ldx, (const W*)w, stats, center, (const G*)g, ldg, (const E*)add, (E*)dx, parts);
