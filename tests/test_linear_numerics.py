@@ -57,6 +57,35 @@ def test_gradients_of_tails_of_the_mlp(cuda_device, act, m):
     within(db / m, slope, tol + 2.0 ** -8 * (slope.abs() + tol))
 
 
+# ---- GELU beside bf16 where its value or its slope cancels ------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_a_residual_that_cancels_gelu(cuda_device, m):
+    """The value is not rounded before the residual is added: what is left of it is right to fp32's
+    bounds (an argument of one term, 8 u of the value and 2 u of the argument) and one rounding."""
+    z = torch.linspace(-6, 6, 4096).to(BF16).cuda()
+    h = activated(Val(z), "gelu")[0]
+    res = (-h.v).to(BF16)
+    x = torch.ones(m, 1, device=cuda_device, dtype=BF16)
+    out = fused_linear(x, z[:, None], activation="gelu", residual=res.expand(m, -1))
+    want = h.v + res.double()
+    tol = h.e + U * want.abs() + 48 * U * h.v.abs()  # exp's argument, up to 18, u of itself off
+    for row in out:
+        within(row, want, tol + 2.0 ** -8 * (want.abs() + tol))
+
+
+@pytest.mark.gpu
+def test_gelus_slope_where_it_passes_zero(cuda_device):
+    """-0.75 and a small bias: the slope's bound is of fp32, and 2^-11 and 2^-8 of its own small value."""
+    b = torch.linspace(-0.01, 0.01, 2001).to(BF16).cuda().requires_grad_(True)
+    x = torch.full((1, 1), -0.75, device=cuda_device, dtype=BF16)
+    one = torch.ones(2001, 1, device=cuda_device, dtype=BF16)
+    (db,) = torch.autograd.grad(fused_linear(x, one, b, activation="gelu"), b, torch.ones_like(b)[None])
+    slope = activated(Val(b.detach().double() - 0.75), "gelu")[1]
+    tol = slope.e + 2.0 ** -11 * slope.v.abs() + 2.0 ** -39
+    within(db, slope.v, tol + 2.0 ** -8 * (slope.v.abs() + tol))
+
+
 # ---- infinities and NaN -----------------------------------------------------------------------
 def _same_kind(name, got, want):
     """NaN where NaN, infinite where infinite, and finite elsewhere."""
