@@ -39,3 +39,17 @@ def test_autocast_refuses_an_mlp_that_does_not_lead_back(autocast):
 def test_autocast_asks_for_the_residuals_device(autocast):
     with pytest.raises(RuntimeError, match="device"):
         fused_linear(torch.zeros(3, 4), torch.zeros(5, 4), residual=torch.zeros(3, 5))
+
+
+def test_library_refuses_wide_results_that_no_kernel_forms():
+    """fp32 results beside bf16 operands: the rows' gradient alone, without a slope, in whole eights."""
+    import ctypes
+
+    from dabsn_amd import _lib
+
+    lib, one = _lib.load(), 1 << 20
+    good = dict(dtype=1, transB=1, wideC=1, M=4, N=8, K=16, A=one, B=one, C=one, lda=16, ldb=8, ldc=8)
+    for bad in (dict(dtype=0), dict(transB=0, ldb=16), dict(transA=1, lda=8), dict(ldc=9), dict(ldc=12),
+                dict(slope=one, slope_kind=1, lds=8)):
+        assert lib.dabsn_hip_linear(ctypes.byref(_lib.LinearCall(**{**good, **bad})), None) == -2, bad
+        assert lib.dabsn_hip_linear_workspace_bytes(ctypes.byref(_lib.LinearCall(**{**good, **bad}))) == 0
