@@ -5,9 +5,9 @@ With mean and variance over the last axis,
   layer_norm   (x - mean) / sqrt(var + eps) * weight + bias
   rms_norm     x / sqrt(mean(x^2) + eps) * weight
 
-in fp32 from one reading of the row, so of rows whose squares are numbers there (sizes from 1e-18 to
-1e18 are; larger ones overflow, smaller ones count as eps alone), rounded once to x's type (``ops.rms_norm``, the block's
-inference kernel, rounds before the weight as the reference's module does). Both are
+in fp32 from one reading of the row, rounded once to x's type (``ops.rms_norm``, the block's
+inference kernel, rounds before the weight as the reference's module does). The squares are summed as
+they are: values up to 1e17 fit at any width, and those below 1e-18 count as 0 beside eps. Both are
 differentiable in x, weight and bias: the gradients of weight and bias are sums over the rows in
 fp32 and in a fixed order, so the same inputs give the same bits.
 """
